@@ -284,6 +284,66 @@ int kfa_cp_grad_finalize(const KfaAcc32* acc, const KfaTensor4* grad, int dtype,
 int kfa_copy_rows(void* dst, int64_t dst_pitch, const void* src, int64_t src_pitch, int64_t row_bytes,
                   int64_t rows, int to_device, void* stream);
 
+/* ---------------------------------------------------------------------------------------------
+ * A cache of keys and values, and what generation does with it. No counterpart in the reference.
+ *
+ * The cache is made of pages: k and v are [N, Hkv, page, D] views (conventions above; D a multiple of 8 up to 128).
+ * Position p of sequence b lies in page table[b * table_stride + p / page] at slot p % page; table NULL: N is the
+ * batch and page b is sequence b's. With a table `page` is a multiple of 8. Positions 0 .. lengths[b] - 1 hold keys and values, what lies behind
+ * them is never used. A table entry that is needed and outside 0 .. N - 1, or a length outside 0 .. capacity
+ * (table_cols * page), is reported in the status word (KFA_DEV_BAD_CACHE); nothing outside the pages is touched.
+ * A call never changes lengths or table.
+ * --------------------------------------------------------------------------------------------- */
+#define KFA_DEV_BAD_CACHE 90
+typedef struct KfaCache {
+  KfaTensor4 k, v;
+  const int32_t* table; /* [batch, table_cols], rows table_stride entries apart; or NULL */
+  int64_t table_stride, table_cols;
+  const int32_t* lengths; /* [batch] */
+  int64_t batch;
+} KfaCache;
+
+/* Which of the T rows of q (or of new k, v) a call takes: row i of sequence b is index[b * index_stride + i] (NULL: i), for
+ * i < counts[b] (NULL: steps). Entries of index outside 0 .. T - 1 are reported like a bad table; counts are clamped to 0 .. steps. */
+typedef struct KfaRows {
+  const int32_t* index;
+  int64_t index_stride;
+  const int32_t* counts;
+  int64_t steps;
+} KfaRows;
+
+/* out[b, h, t] for t < counts[b] (NULL: T): attention of q [B, H, T, D] to the cached positions and to the new tokens j <
+ * counts[b] whose k, v [B, Hkv, T, D] are given (both NULL: none), where tree[b, t, j] is nonzero (bytes, strides in bytes; NULL: j <= t).
+ * stats (may be NULL): fp32 [B, H, 2, T] contiguous, the plane of raw row maxima and that of log2 l, as kfa_fwd leaves them. A row that sees
+ * nothing, or that counts leaves out: output 0, statistics (+inf, 0). A hidden key never reaches a row, whatever it holds.
+ * scratch: kfa_cache_attend_bytes bytes, 16-byte aligned, used by this call alone while it runs. scale >= 0. */
+int64_t kfa_cache_attend_bytes(const KfaTensor4* q, const KfaCache* cache, const KfaTensor4* k);
+int kfa_cache_attend(const KfaTensor4* q, const KfaCache* cache, const KfaTensor4* k, const KfaTensor4* v, const uint8_t* tree,
+                     const int64_t* tree_stride, const int32_t* counts, const KfaTensor4* out, float* stats, void* scratch,
+                     float scale, int dtype, int* dev_status, void* stream);
+
+/* Position lengths[b] + i of the cache <- k, v row of the i-th of the given rows. Positions at or behind the capacity are not
+ * written and reported. The written pages belong to one sequence each. */
+int kfa_cache_append(const KfaCache* cache, const KfaTensor4* k, const KfaTensor4* v, const KfaRows* rows, int* dev_status,
+                     void* stream);
+
+/* weights[b, g, p] = (add: +=) the attention that the given rows of q gave to cached position p, summed over rows and over the query heads
+ * of K / V head g. Row i stands at position lengths[b] + i (appended before this call) and sees positions up to its own; its
+ * weights are exp2((q k - m) * scale * log2 e - log2 l) with m, log2 l from stats, fp32 [B, H, 2, T] contiguous (a row with m =
+ * +inf gives none). weights: fp32, last dim contiguous, strides in floats, `room` positions; add = 0 writes all `room` of them
+ * (0 behind the last row), add = 1 touches the positions that rows see only. */
+int kfa_cache_weigh(const KfaTensor4* q, const float* stats, const KfaCache* cache, const KfaRows* rows, float* weights,
+                    const int64_t* weights_stride, int64_t room, int add, float scale, int dtype, int* dev_status, void* stream);
+
+/* Each (sequence, K / V head) of `cache` keeps min(lengths[b], keep) positions: the `recent` newest and of the others those of the largest
+ * weights (fp32 [B, Hkv, >= capacity], strides in floats; of equal ones the lower position; NaN counts as largest). They are
+ * written to positions 0, 1, ... of `out` in ascending order (out->lengths is not read; its capacity is at least keep, and the pages that are written are none of those that are read).
+ * kept: int32 [B, Hkv, keep], the positions, -1 behind the last; weights_out: fp32 [B, Hkv, keep], their weights, 0 behind the last;
+ * lengths_out: int32 [B]. clear: rows of `out` behind the last kept position up to keep are zeroed, else left. */
+int kfa_cache_evict(const KfaCache* cache, const float* weights, const int64_t* weights_stride, int64_t keep, int64_t recent,
+                    const KfaCache* out, float* weights_out, int32_t* kept, int32_t* lengths_out, int clear, int* dev_status,
+                    void* stream);
+
 /* Diagnostic: the raw scores Q K^T (unscaled, unmasked) as fp32 [B, H, Sq, Skv] (contiguous), produced by
  * the same tensor-core instruction sequence the attention kernels use (one fp32-accumulating MMA per 16
  * elements of the head dim, in ascending order). What comes out is NOT the correctly rounded dot

@@ -17,6 +17,7 @@ import torch
 LIB_PATH = Path(os.environ.get("KFA_LIBRARY") or Path(__file__).resolve().parent / "libkfa.so")
 
 KFA_F16, KFA_BF16 = 0, 1
+DEV_BAD_CACHE = 90  # KFA_DEV_BAD_CACHE
 ABI_VERSION = 1
 
 # Every entry point include/kfa.h declares (checked against the built library by the tests).
@@ -55,6 +56,11 @@ SYMBOLS = (
     "kfa_bwd_parts",
     "kfa_bwd_parts_n",
     "kfa_varlen_zero_rows",
+    "kfa_cache_attend_bytes",
+    "kfa_cache_attend",
+    "kfa_cache_append",
+    "kfa_cache_weigh",
+    "kfa_cache_evict",
 )
 
 
@@ -77,6 +83,27 @@ class KfaMaskWords(ctypes.Structure):
 
 class KfaMaskTiles(ctypes.Structure):
     _fields_ = [("any", ctypes.c_void_p), ("stride_batch", ctypes.c_int64), ("stride_head", ctypes.c_int64)]
+
+
+class KfaCache(ctypes.Structure):
+    _fields_ = [
+        ("k", KfaTensor4),
+        ("v", KfaTensor4),
+        ("table", ctypes.c_void_p),
+        ("table_stride", ctypes.c_int64),
+        ("table_cols", ctypes.c_int64),
+        ("lengths", ctypes.c_void_p),
+        ("batch", ctypes.c_int64),
+    ]
+
+
+class KfaRows(ctypes.Structure):
+    _fields_ = [
+        ("index", ctypes.c_void_p),
+        ("index_stride", ctypes.c_int64),
+        ("counts", ctypes.c_void_p),
+        ("steps", ctypes.c_int64),
+    ]
 
 
 class KfaAcc32(ctypes.Structure):
@@ -158,8 +185,16 @@ def load() -> ctypes.CDLL:
         lib.kfa_copy_rows.argtypes = [vp, i64, vp, i64, i64, i64, i32, vp]
         lib.kfa_scores.argtypes = [T, T, fp, i32, ip, vp]
         lib.kfa_selftest.argtypes = [ctypes.c_char_p, ctypes.c_int]
+        C, R, I64P = ctypes.POINTER(KfaCache), ctypes.POINTER(KfaRows), ctypes.POINTER(ctypes.c_int64)
+        lib.kfa_cache_attend_bytes.restype = ctypes.c_int64
+        lib.kfa_cache_attend_bytes.argtypes = [T, C, T]
+        lib.kfa_cache_attend.argtypes = [T, C, T, T, vp, I64P, ip, T, fp, vp, f32, i32, ip, vp]
+        lib.kfa_cache_append.argtypes = [C, T, T, R, ip, vp]
+        lib.kfa_cache_weigh.argtypes = [T, fp, C, R, fp, I64P, i64, i32, f32, i32, ip, vp]
+        lib.kfa_cache_evict.argtypes = [C, fp, I64P, i64, i64, C, fp, ip, ip, i32, ip, vp]
         for name in SYMBOLS:
-            if name not in ("kfa_abi_version", "kfa_last_error", "kfa_bwd_stats_bytes", "kfa_bwd_dq_acc_bytes", "kfa_bwd_parts_bytes"):
+            if name not in ("kfa_abi_version", "kfa_last_error", "kfa_bwd_stats_bytes", "kfa_bwd_dq_acc_bytes", "kfa_bwd_parts_bytes",
+                            "kfa_cache_attend_bytes"):  # fmt: skip
                 getattr(lib, name).restype = ctypes.c_int
         if lib.kfa_abi_version() != ABI_VERSION:
             raise KfaError(f"libkfa ABI {lib.kfa_abi_version()} != expected {ABI_VERSION}: rebuild")
@@ -172,6 +207,7 @@ HOST_SYMBOLS = (
     "kfa_last_error", "kfa_fwd", "kfa_bwd", "kfa_bwd_fused", "kfa_fwd_masked", "kfa_bwd_masked", "kfa_fwd_varlen",
     "kfa_bwd_varlen", "kfa_pack_mask", "kfa_fwd_narrow", "kfa_bwd_narrow",
     "kfa_bwd_parts_bytes", "kfa_bwd_parts_count", "kfa_bwd_parts", "kfa_varlen_zero_rows",
+    "kfa_cache_attend_bytes", "kfa_cache_attend", "kfa_cache_append", "kfa_cache_weigh", "kfa_cache_evict",
 )  # fmt: skip
 HOST_PATH = Path(__file__).resolve().parent / "_kfa_host.so"
 _host = None
@@ -261,15 +297,21 @@ def reset_device_status(device=None) -> None:
 
 def check_status(device=None) -> None:
     """Raises ``KfaError`` if a kernel on ``device`` (default: the current one) gave up on an internal
-    wait since the last ``reset_status``.
+    wait, or a call on a ``KVCache`` on what its table, lengths or index say, since the last ``reset_status``.
 
     The kernels never hang: a wait that exceeds its (seconds-long) limit makes the CTA fill the output
     rows it owns with NaN, record ``100 + wait id`` in a per-device status word and leave; every later
-    launch on that device may still do part or all of its work, but leaves its outputs as NaN as well. Nothing on the
+    launch on that device may still do part or all of its work, but leaves its outputs as NaN as well (what only copies, ``cache_append``
+    and ``cache_evict``, runs on). Nothing on the
     launch path reads the word back (that would synchronise), so call this where the program
     synchronises anyway, e.g. after ``loss.item()`` or the optimizer step: NaN gradients plus a nonzero
     status mean "a kernel timed out", not "the model diverged". Reads one int from the device."""
     code = device_status(device)
+    if code == DEV_BAD_CACHE:
+        raise KfaError(
+            f"a call on a KVCache met a page outside the pool, a length or position outside the capacity, or an index outside its rows "
+            f"(status {code}); outputs since then are NaN. Call reset_status() to re-enable the kernels"
+        )
     if code != 0:
         raise KfaError(
             f"a libkfa kernel timed out waiting on its pipeline (status {code} = 100 + wait id); outputs since then "

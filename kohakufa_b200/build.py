@@ -13,6 +13,7 @@ import shutil
 import subprocess
 import sys
 import sysconfig
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -25,25 +26,20 @@ LIB_SHORT_WAIT = PKG / "libkfa_shortwait.so"
 SHORT_WAIT_FLAGS = ["-DKFA_WAIT_CYCLES=300ll"]
 HOST = PKG / "_kfa_host.so"
 HOST_SOURCES = [CSRC / "kfa_host.cpp", PKG.parent / "include" / "kfa.h"]
-SOURCES = [CSRC / "kfa_api.cu"]
-HEADERS = [
-    CSRC / "kfa_ptx.cuh",
-    CSRC / "kfa_fwd.cuh",
-    CSRC / "kfa_bwd.cuh",
-    CSRC / "kfa_bwd_fused.cuh",
-    CSRC / "kfa_selftest.cuh",
-    CSRC / "kfa_cp.cuh",
-    CSRC / "kfa_mask.cuh",
-    CSRC / "kfa_scores.cuh",
-    PKG.parent / "include" / "kfa.h",
-]
+SHARED = [CSRC / "kfa_ptx.cuh", CSRC / "kfa_call.cuh", PKG.parent / "include" / "kfa.h"]
+# Each source and what it includes; compiled side by side, a source whose object is newer than all of these is not compiled again.
+SOURCES = {
+    CSRC / "kfa_api.cu": SHARED
+    + [CSRC / f"kfa_{part}.cuh" for part in ("fwd", "bwd", "bwd_fused", "selftest", "cp", "mask", "scores")],
+    CSRC / "kfa_cache.cu": SHARED + [CSRC / "kfa_cache.cuh"],
+}
+OBJECTS = CSRC / "build"
 NVCC_FLAGS = [
     "-gencode",
     "arch=compute_100a,code=sm_100a",
     "-lineinfo",
     "-O3",
     "-std=c++17",
-    "-shared",
     "-Xcompiler",
     "-fPIC",
     "-Xptxas",
@@ -74,7 +70,7 @@ def stale(lib: Path = LIB) -> bool:
     if not lib.exists() or (lib == HOST and not host_fits(lib)):
         return True
     built = lib.stat().st_mtime
-    return any(p.stat().st_mtime > built for p in (HOST_SOURCES if lib == HOST else SOURCES + HEADERS))
+    return any(p.stat().st_mtime > built for p in (HOST_SOURCES if lib == HOST else [f for s in SOURCES for f in (s, *SOURCES[s])]))
 
 
 def _run(cmd, log: str, verbose: bool) -> None:
@@ -86,8 +82,20 @@ def _run(cmd, log: str, verbose: bool) -> None:
         print(proc.stderr)
 
 
-def _compile(lib: Path, extra, log: str, verbose: bool) -> None:
-    _run([nvcc_path(), *NVCC_FLAGS, *extra, "-o", str(lib), *map(str, SOURCES)], log, verbose)
+def _object(lib: Path, source: Path) -> Path:
+    return OBJECTS / f"{lib.stem}_{source.stem}.o"
+
+
+def _compile(lib: Path, source: Path, extra, force: bool, verbose: bool) -> None:
+    obj = _object(lib, source)
+    if not force and obj.exists() and all(p.stat().st_mtime <= obj.stat().st_mtime for p in (source, *SOURCES[source])):
+        return
+    _run([nvcc_path(), *NVCC_FLAGS, *extra, "-c", "-o", str(obj), str(source)], f"csrc/build/{obj.stem}.log", verbose)
+
+
+def _link(lib: Path) -> None:
+    cmd = [nvcc_path(), *NVCC_FLAGS[:2], "-shared", "-o", str(lib), *(str(_object(lib, s)) for s in SOURCES)]
+    _run(cmd, f"csrc/build/{lib.stem}_link.log", False)
 
 
 def _compile_host() -> None:
@@ -101,18 +109,23 @@ def _compile_host() -> None:
     cmd.append(f'-DKFA_HOST_STAMP="{host_stamp().decode()}"')
     cmd += [f"-I{d}" for d in include] + ["-o", str(HOST), str(HOST_SOURCES[0]), f"-L{root / 'lib'}"]
     cmd += ["-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch", "-ltorch_python"]
-    _run(cmd, "build_host.log", False)
+    _run(cmd, "csrc/build/host.log", False)
 
 
 def build(force: bool = False, verbose: bool = False, short_wait: bool = True) -> Path:
     """Compile the library, the host extension (and, with ``short_wait``, the library's short-wait test twin) if
     missing or older than the sources; returns the library's path."""
-    jobs = [(LIB, [], "build.log")] + ([(LIB_SHORT_WAIT, SHORT_WAIT_FLAGS, "build_shortwait.log")] if short_wait else [])
-    if force or stale(HOST):
-        _compile_host()
-    for lib, extra, log in jobs:
-        if force or stale(lib):
-            _compile(lib, extra, log, verbose and lib is LIB)
+    libs = [(LIB, [])] + ([(LIB_SHORT_WAIT, SHORT_WAIT_FLAGS)] if short_wait else [])
+    libs = [(lib, extra) for lib, extra in libs if force or stale(lib)]
+    OBJECTS.mkdir(exist_ok=True)
+    with ThreadPoolExecutor() as pool:
+        jobs = [pool.submit(_compile, lib, src, extra, force, verbose and lib is LIB) for lib, extra in libs for src in SOURCES]
+        if force or stale(HOST):
+            jobs.append(pool.submit(_compile_host))
+        for job in jobs:
+            job.result()
+    for lib, _ in libs:
+        _link(lib)
     return LIB
 
 

@@ -16,56 +16,10 @@
 #include "../../include/kfa.h"
 #include "kfa_bwd.cuh"
 #include "kfa_bwd_fused.cuh"
+#include "kfa_call.cuh"
 #include "kfa_fwd.cuh"
 
 namespace {
-
-thread_local char g_err[512] = "";
-
-int fail(int code, const char* fmt, ...) {
-  va_list ap;
-  va_start(ap, fmt);
-  vsnprintf(g_err, sizeof(g_err), fmt, ap);
-  va_end(ap);
-  return code;
-}
-
-#define KFA_CUDA(expr)                                                                    \
-  do {                                                                                    \
-    cudaError_t e_ = (expr);                                                              \
-    if (e_ != cudaSuccess) return fail(KFA_ERR_CUDA, "%s: %s", #expr, cudaGetErrorString(e_)); \
-  } while (0)
-
-using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                              const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                              CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-EncodeFn encode_fn() {
-  static std::atomic<EncodeFn> cached{nullptr};
-  EncodeFn f = cached.load();
-  if (f) return f;
-  void* sym = nullptr;
-  cudaDriverEntryPointQueryResult q;
-  if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &sym, cudaEnableDefault, &q) != cudaSuccess ||
-      q != cudaDriverEntryPointSuccess || !sym)
-    return nullptr;
-  f = reinterpret_cast<EncodeFn>(sym);
-  cached.store(f);
-  return f;
-}
-
-int check_tensor(const KfaTensor4* t, const char* name) {
-  if (!t || !t->ptr) return fail(KFA_ERR_ARG, "%s: null tensor", name);
-  if (reinterpret_cast<uintptr_t>(t->ptr) % 16) return fail(KFA_ERR_ARG, "%s: base not 16-byte aligned", name);
-  if (t->stride[3] != 1) return fail(KFA_ERR_ARG, "%s: last dimension must be contiguous", name);
-  for (int i = 0; i < 3; ++i)
-    if (t->shape[i] > 1 && (t->stride[i] % 8 != 0 || t->stride[i] <= 0))
-      return fail(KFA_ERR_ARG, "%s: stride[%d]=%lld must be a positive multiple of 8 elements", name, i,
-                  static_cast<long long>(t->stride[i]));
-  for (int i = 0; i < 4; ++i)
-    if (t->shape[i] < 1 || t->shape[i] > 0x7fffffff) return fail(KFA_ERR_ARG, "%s: bad shape[%d]", name, i);
-  return KFA_OK;
-}
 
 // The head dim whose kernels compute tensors of D columns.
 int kernel_dim(int64_t D) { return static_cast<int>((D + 15) / 16 * 16); }
@@ -657,7 +611,7 @@ extern "C" {
 
 int kfa_abi_version(void) { return KFA_ABI_VERSION; }
 
-const char* kfa_last_error(void) { return g_err; }
+const char* kfa_last_error(void) { return kfa::g_err; }
 
 int64_t kfa_bwd_stats_bytes(int64_t B, int64_t H, int64_t Sq) {
   return B * H * ((Sq + 127) / 128) * 3 * 128 * 4;

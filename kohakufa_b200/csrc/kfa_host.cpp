@@ -21,6 +21,7 @@
 #include <c10/cuda/CUDAStream.h>
 
 #include <array>
+#include <cmath>
 #include <initializer_list>
 #include <string>
 #include <tuple>
@@ -45,6 +46,11 @@ struct Api {
   decltype(&kfa_bwd_parts_count) bwd_parts_count = nullptr;
   decltype(&kfa_bwd_parts) bwd_parts = nullptr;
   decltype(&kfa_varlen_zero_rows) varlen_zero_rows = nullptr;
+  decltype(&kfa_cache_attend_bytes) cache_attend_bytes = nullptr;
+  decltype(&kfa_cache_attend) cache_attend = nullptr;
+  decltype(&kfa_cache_append) cache_append = nullptr;
+  decltype(&kfa_cache_weigh) cache_weigh = nullptr;
+  decltype(&kfa_cache_evict) cache_evict = nullptr;
 } api;
 
 PyObject* g_error = nullptr;  // kohakufa_b200._lib.KfaError
@@ -638,6 +644,244 @@ PyObject* py_pack_mask(Args a, Py_ssize_t n) {
   }));
 }
 
+// ---------------------------------------------------------------------------------------------------------------------
+// A cache of keys and values (cache.py). Optional arguments are None in Python, undefined tensors here.
+// ---------------------------------------------------------------------------------------------------------------------
+at::Tensor maybe(PyObject* o) { return o == Py_None ? at::Tensor() : tensor(o); }
+
+struct Cache {
+  at::Tensor k, v, lengths, table;
+};
+Cache cache_of(Args a) { return {tensor(a[0]), tensor(a[1]), tensor(a[2]), maybe(a[3])}; }
+
+int64_t capacity(const Cache& c) { return c.table.defined() ? c.table.size(1) * c.k.size(2) : c.k.size(2); }
+
+// (Numbers go into messages through std::to_string: c10 formats them with a stream whose locale another libstdc++ may own.)
+// Everything that the kernels take for granted about a cache, and that a program may have changed since it was made.
+void check_cache(const char* who, const Cache& c) {
+  TORCH_CHECK_TYPE((c.k.scalar_type() == at::kHalf || c.k.scalar_type() == at::kBFloat16) && c.v.scalar_type() == c.k.scalar_type(), who,
+                   ": the cache's pages must be fp16 or bf16 (both the same)");
+  TORCH_CHECK_VALUE(c.k.dim() == 4 && c.k.sizes() == c.v.sizes() && c.k.numel() > 0, who, ": the cache's pages must be [N, Hkv, page, D]");
+  TORCH_CHECK_VALUE(c.k.size(3) % 8 == 0 && c.k.size(3) <= 128, who, ": head_dim ", std::to_string(c.k.size(3)), ": a multiple of 8 up to 128");
+  TORCH_CHECK_VALUE(strides_ok(c.k) && strides_ok(c.v), who, ": the cache's pages need a contiguous last dim and 16-byte strides");
+  TORCH_CHECK_TYPE(c.lengths.scalar_type() == at::kInt, who, ": lengths must be int32");
+  TORCH_CHECK_VALUE(c.lengths.dim() == 1 && c.lengths.is_contiguous() && c.lengths.numel() > 0, who, ": lengths must be a contiguous vector");
+  if (c.table.defined()) {
+    TORCH_CHECK_TYPE(c.table.scalar_type() == at::kInt, who, ": table must be int32");
+    TORCH_CHECK_VALUE(c.table.dim() == 2 && c.table.size(0) == c.lengths.numel() && c.table.size(1) > 0 && c.table.stride(1) == 1 &&
+                          c.table.stride(0) >= 0,
+                      who, ": table must be [B, M] with contiguous rows");
+    TORCH_CHECK_VALUE(c.k.size(2) % 8 == 0, who, ": pages of ", std::to_string(c.k.size(2)), " positions: a multiple of 8");
+  } else {
+    TORCH_CHECK_VALUE(c.k.size(0) == c.lengths.numel(), who, ": without a table one page per sequence");
+  }
+}
+
+// [B, heads, T, D] rows of new tokens beside the cache (heads: 0 for any multiple of its own)
+void check_new(const char* who, const char* name, const Cache& c, const at::Tensor& t, int64_t heads) {
+  TORCH_CHECK_TYPE(t.scalar_type() == c.k.scalar_type(), who, ": ", name, " must have the cache's type");
+  TORCH_CHECK_VALUE(t.dim() == 4 && t.numel() > 0 && t.size(0) == c.lengths.numel() && t.size(3) == c.k.size(3) &&
+                        (heads ? t.size(1) == heads : t.size(1) % c.k.size(1) == 0),
+                    who, ": ", name, " must be [B, heads, T, D] of the cache's batch, heads and head dim");
+  TORCH_CHECK_VALUE(strides_ok(t), who, ": ", name, " needs a contiguous last dim and 16-byte strides");
+}
+
+void check_counts(const char* who, const Cache& c, const at::Tensor& counts) {
+  if (!counts.defined()) return;
+  TORCH_CHECK_TYPE(counts.scalar_type() == at::kInt, who, ": counts must be int32");
+  TORCH_CHECK_VALUE(counts.dim() == 1 && counts.is_contiguous() && counts.numel() == c.lengths.numel(), who,
+                    ": counts must be a contiguous vector, one entry per sequence");
+}
+
+KfaRows rows_of(const char* who, const Cache& c, const at::Tensor& index, const at::Tensor& counts, int64_t tokens) {
+  check_counts(who, c, counts);
+  KfaRows r{nullptr, 0, counts.defined() ? counts.data_ptr<int32_t>() : nullptr, tokens};
+  if (index.defined()) {
+    TORCH_CHECK_TYPE(index.scalar_type() == at::kInt, who, ": index must be int32");
+    TORCH_CHECK_VALUE(index.dim() == 2 && index.size(0) == c.lengths.numel() && index.size(1) > 0 && index.stride(1) == 1 &&
+                          index.stride(0) >= 0,
+                      who, ": index must be [B, A] with contiguous rows");
+    r.index = index.data_ptr<int32_t>();
+    r.index_stride = index.stride(0);
+    r.steps = index.size(1);
+  }
+  return r;
+}
+
+void check_where(const char* who, const Cache& c, std::initializer_list<const at::Tensor*> others) {
+  TORCH_CHECK_VALUE(c.k.is_cuda(), who, ": CUDA tensors only (there is no CPU path)");
+  for (const at::Tensor* t : {&c.v, &c.lengths, &c.table}) TORCH_CHECK_VALUE(!t->defined() || t->device() == c.k.device(), who, ": tensors on different devices");
+  for (const at::Tensor* t : others) TORCH_CHECK_VALUE(!t->defined() || t->device() == c.k.device(), who, ": tensors on different devices");
+}
+
+void check_no_grad(const char* who, std::initializer_list<const at::Tensor*> tensors) {
+  if (!at::GradMode::is_enabled()) return;
+  for (const at::Tensor* t : tensors)
+    TORCH_CHECK(!t->defined() || !t->requires_grad(), who, ": has no gradient; call it under torch.no_grad() or on detached tensors");
+}
+
+void check_scale(const char* who, double scale) { TORCH_CHECK_VALUE(std::isfinite(scale) && scale >= 0, who, ": scale must be finite and not negative"); }
+
+KfaCache cache_desc(const Cache& c) {
+  KfaCache d{desc(c.k), desc(c.v), nullptr, 0, 0, c.lengths.data_ptr<int32_t>(), c.lengths.numel()};
+  if (c.table.defined()) {
+    d.table = c.table.data_ptr<int32_t>();
+    d.table_stride = c.table.size(0) > 1 ? c.table.stride(0) : 0;
+    d.table_cols = c.table.size(1);
+  }
+  return d;
+}
+
+// cached_attention(q, k_pages, v_pages, lengths, table, k, v, tree, counts, scale, return_stats, status) -> out, or out and stats
+PyObject* py_cached_attention(Args a, Py_ssize_t n) {
+  need(n, 12);
+  const char* who = "attention_cached";
+  const at::Tensor q = tensor(a[0]), k = maybe(a[5]), v = maybe(a[6]), tree = maybe(a[7]), counts = maybe(a[8]), status = maybe(a[11]);
+  const Cache c = cache_of(a + 1);
+  const double scale = number(a[9]);
+  const bool with_stats = PyObject_IsTrue(a[10]);
+  check_no_grad(who, {&q, &c.k, &c.v, &k, &v});
+  check_cache(who, c);
+  check_new(who, "q", c, q, 0);
+  TORCH_CHECK_VALUE(k.defined() == v.defined(), who, ": give k and v, or neither");
+  TORCH_CHECK_VALUE(!tree.defined() || k.defined(), who, ": tree shows new tokens to one another: it needs k and v");
+  int64_t tree_stride[3] = {0, 0, 0};
+  if (k.defined()) {
+    check_new(who, "k", c, k, c.k.size(1));
+    check_new(who, "v", c, v, c.k.size(1));
+    TORCH_CHECK_VALUE(k.size(2) == q.size(2) && v.size(2) == q.size(2), who, ": k and v must have as many tokens as q");
+  }
+  if (tree.defined()) {
+    const int64_t t = q.size(2), d = tree.dim();
+    TORCH_CHECK_TYPE(tree.scalar_type() == at::kBool, who, ": tree must be bool");
+    TORCH_CHECK_VALUE((d == 2 || (d == 3 && (tree.size(0) == q.size(0) || tree.size(0) == 1))) && tree.size(d - 1) == t && tree.size(d - 2) == t,
+                      who, ": tree must be [T, T] or [B, T, T]");
+    tree_stride[0] = d == 3 && tree.size(0) > 1 ? tree.stride(0) : 0;
+    tree_stride[1] = tree.stride(d - 2);
+    tree_stride[2] = tree.stride(d - 1);
+  }
+  check_counts(who, c, counts);
+  check_scale(who, scale);
+  check_where(who, c, {&q, &k, &v, &tree, &counts, &status});
+  auto [out, stats] = released([&] {
+    const c10::cuda::CUDAGuard guard(q.device());
+    at::Tensor o = bshd_like(q), st;
+    if (with_stats) st = floats(q, {q.size(0), q.size(1), 2, q.size(2)});
+    const KfaTensor4 dq = desc(q), dout = desc(o), dk = k.defined() ? desc(k) : KfaTensor4{}, dv = k.defined() ? desc(v) : KfaTensor4{};
+    const KfaCache dc = cache_desc(c);
+    const int64_t bytes = api.cache_attend_bytes(&dq, &dc, k.defined() ? &dk : nullptr);
+    const at::Tensor scratch = bytes ? floats(q, {(bytes + 3) / 4}) : at::Tensor();
+    check(api.cache_attend(&dq, &dc, k.defined() ? &dk : nullptr, k.defined() ? &dv : nullptr,
+                           tree.defined() ? static_cast<const uint8_t*>(tree.data_ptr()) : nullptr, tree_stride,
+                           counts.defined() ? counts.data_ptr<int32_t>() : nullptr, &dout, st.defined() ? st.data_ptr<float>() : nullptr,
+                           bytes ? scratch.data_ptr() : nullptr, static_cast<float>(scale), dtype_code(q), status.data_ptr<int32_t>(),
+                           stream_of(q)));
+    return Two{std::move(o), std::move(st)};
+  });
+  if (!with_stats) return THPVariable_Wrap(std::move(out));
+  return pack(Two{std::move(out), std::move(stats)});
+}
+
+// cache_append(k_pages, v_pages, lengths, table, k, v, index, counts, status)
+PyObject* py_cache_append(Args a, Py_ssize_t n) {
+  need(n, 9);
+  const char* who = "cache_append";
+  const Cache c = cache_of(a);
+  const at::Tensor k = tensor(a[4]), v = tensor(a[5]), index = maybe(a[6]), counts = maybe(a[7]), status = maybe(a[8]);
+  check_no_grad(who, {&c.k, &c.v, &k, &v});
+  check_cache(who, c);
+  check_new(who, "k", c, k, c.k.size(1));
+  check_new(who, "v", c, v, c.k.size(1));
+  TORCH_CHECK_VALUE(k.size(2) == v.size(2), who, ": k and v must have as many tokens");
+  const KfaRows rows = rows_of(who, c, index, counts, k.size(2));
+  check_where(who, c, {&k, &v, &index, &counts, &status});
+  released([&] {
+    const c10::cuda::CUDAGuard guard(k.device());
+    const KfaCache dc = cache_desc(c);
+    const KfaTensor4 dk = desc(k), dv = desc(v);
+    check(api.cache_append(&dc, &dk, &dv, &rows, status.data_ptr<int32_t>(), stream_of(k)));
+    return 0;
+  });
+  c.k.unsafeGetTensorImpl()->bump_version();
+  c.v.unsafeGetTensorImpl()->bump_version();
+  Py_RETURN_NONE;
+}
+
+void check_weights(const char* who, const Cache& c, const at::Tensor& w) {
+  TORCH_CHECK_TYPE(w.scalar_type() == at::kFloat, who, ": weights must be fp32");
+  TORCH_CHECK_VALUE(w.dim() == 3 && w.size(0) == c.lengths.numel() && w.size(1) == c.k.size(1) && w.size(2) >= capacity(c) && w.stride(2) == 1 &&
+                        w.stride(0) >= 0 && w.stride(1) >= 0,
+                    who, ": weights must be [B, Hkv, W] with W at least the cache's capacity and contiguous rows");
+}
+
+// cache_weights(k_pages, v_pages, lengths, table, q, stats, index, counts, weights, add, scale, status)
+PyObject* py_cache_weights(Args a, Py_ssize_t n) {
+  need(n, 12);
+  const char* who = "cache_weights";
+  const Cache c = cache_of(a);
+  const at::Tensor q = tensor(a[4]), stats = tensor(a[5]), index = maybe(a[6]), counts = maybe(a[7]), w = tensor(a[8]), status = maybe(a[11]);
+  const bool add = PyObject_IsTrue(a[9]);
+  const double scale = number(a[10]);
+  check_no_grad(who, {&c.k, &q, &stats, &w});
+  check_cache(who, c);
+  check_new(who, "q", c, q, 0);
+  TORCH_CHECK_TYPE(stats.scalar_type() == at::kFloat, who, ": stats must be fp32");
+  TORCH_CHECK_VALUE(stats.dim() == 4 && stats.size(0) == q.size(0) && stats.size(1) == q.size(1) && stats.size(2) == 2 &&
+                        stats.size(3) == q.size(2) && stats.is_contiguous(),
+                    who, ": stats must be the contiguous [B, H, 2, T] of these queries");
+  const KfaRows rows = rows_of(who, c, index, counts, q.size(2));
+  check_weights(who, c, w);
+  for (int i = 0; i < 2; ++i)  // (it is written: no two entries may be one)
+    TORCH_CHECK_VALUE(w.size(i) == 1 || w.stride(i) >= w.size(2), who, ": weights must not overlap itself");
+  check_scale(who, scale);
+  check_where(who, c, {&q, &stats, &index, &counts, &w, &status});
+  released([&] {
+    const c10::cuda::CUDAGuard guard(q.device());
+    const KfaCache dc = cache_desc(c);
+    const KfaTensor4 dq = desc(q);
+    const int64_t stride[2] = {w.stride(0), w.stride(1)};
+    check(api.cache_weigh(&dq, stats.data_ptr<float>(), &dc, &rows, w.data_ptr<float>(), stride, w.size(2), add,
+                          static_cast<float>(scale), dtype_code(q), status.data_ptr<int32_t>(), stream_of(q)));
+    return 0;
+  });
+  w.unsafeGetTensorImpl()->bump_version();
+  Py_RETURN_NONE;
+}
+
+// cache_evict(k_pages, v_pages, lengths, table, weights, keep, recent, k_out, v_out, table_out, lengths_out, weights_out, kept, clear, status)
+PyObject* py_cache_evict(Args a, Py_ssize_t n) {
+  need(n, 15);
+  const char* who = "cache_evict";
+  const Cache c = cache_of(a), o{tensor(a[7]), tensor(a[8]), tensor(a[10]), maybe(a[9])};
+  const at::Tensor w = tensor(a[4]), w_out = tensor(a[11]), kept = tensor(a[12]), status = maybe(a[14]);
+  const int64_t keep = integer(a[5]), recent = integer(a[6]);
+  const bool clear = PyObject_IsTrue(a[13]);
+  check_no_grad(who, {&c.k, &c.v, &w, &o.k, &o.v});
+  check_cache(who, c);
+  check_cache(who, o);
+  check_weights(who, c, w);
+  const int64_t b = c.lengths.numel(), heads = c.k.size(1);
+  TORCH_CHECK_TYPE(o.k.scalar_type() == c.k.scalar_type(), who, ": out must have the cache's type");
+  TORCH_CHECK_VALUE(o.lengths.numel() == b && o.k.size(1) == heads && o.k.size(3) == c.k.size(3), who,
+                    ": out must have the cache's batch, heads and head dim");
+  TORCH_CHECK_VALUE(capacity(o) >= keep, who, ": out has room for ", std::to_string(capacity(o)), " positions, keep is ", std::to_string(keep));
+  TORCH_CHECK(w_out.scalar_type() == at::kFloat && kept.scalar_type() == at::kInt && w_out.is_contiguous() && kept.is_contiguous() &&
+                  w_out.numel() == b * heads * keep && kept.numel() == b * heads * keep,
+              who, ": results of another size");
+  check_where(who, c, {&w, &o.k, &o.v, &o.lengths, &o.table, &w_out, &kept, &status});
+  released([&] {
+    const c10::cuda::CUDAGuard guard(w.device());
+    const KfaCache dc = cache_desc(c), dn = cache_desc(o);
+    const int64_t stride[2] = {w.stride(0), w.stride(1)};
+    check(api.cache_evict(&dc, w.data_ptr<float>(), stride, keep, recent, &dn, w_out.data_ptr<float>(), kept.data_ptr<int32_t>(),
+                          o.lengths.data_ptr<int32_t>(), clear, status.data_ptr<int32_t>(), stream_of(w)));
+    return 0;
+  });
+  o.k.unsafeGetTensorImpl()->bump_version();
+  o.v.unsafeGetTensorImpl()->bump_version();
+  Py_RETURN_NONE;
+}
+
 // bind(KfaError, {entry point: address}, route)
 PyObject* py_bind(Args a, Py_ssize_t n) {
   need(n, 3);
@@ -664,6 +908,11 @@ PyObject* py_bind(Args a, Py_ssize_t n) {
   take("kfa_bwd_parts_count", api.bwd_parts_count);
   take("kfa_bwd_parts", api.bwd_parts);
   take("kfa_varlen_zero_rows", api.varlen_zero_rows);
+  take("kfa_cache_attend_bytes", api.cache_attend_bytes);
+  take("kfa_cache_attend", api.cache_attend);
+  take("kfa_cache_append", api.cache_append);
+  take("kfa_cache_weigh", api.cache_weigh);
+  take("kfa_cache_evict", api.cache_evict);
   Py_INCREF(a[0]);
   Py_XDECREF(g_error);
   g_error = a[0];
@@ -705,6 +954,10 @@ PyMethodDef methods[] = {
     KFA_METHOD(attention_masked),
     KFA_METHOD(attention_varlen),
     KFA_METHOD(pack_mask),
+    KFA_METHOD(cached_attention),
+    KFA_METHOD(cache_append),
+    KFA_METHOD(cache_weights),
+    KFA_METHOD(cache_evict),
     {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_kfa_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
