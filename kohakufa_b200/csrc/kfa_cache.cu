@@ -3,6 +3,7 @@
 #include <cmath>
 #include <cstring>
 
+#include "kfa_attend.cuh"
 #include "kfa_cache.cuh"
 #include "kfa_call.cuh"
 
@@ -79,19 +80,102 @@ int check_dtype(int dtype) {
   return dtype == KFA_F16 || dtype == KFA_BF16 ? KFA_OK : fail(KFA_ERR_ARG, "dtype %d: KFA_F16 or KFA_BF16", dtype);
 }
 
+// 4-D tiled map over rows of D 16-bit columns: dims (D, n1, n2, n3) with element strides s1, s2, s3, boxes of 64 columns (128 bytes,
+// swizzled) x b1 x b2; what is out of range reads as zeros.
+int make_box_map(void* ptr, int64_t D, int64_t n1, int64_t s1, int64_t n2, int64_t s2, int64_t n3, int64_t s3, int b1, int b2, int dtype,
+                 CUtensorMap* map, const char* name) {
+  EncodeFn enc = encode_fn();
+  if (!enc) return fail(KFA_ERR_CUDA, "cuTensorMapEncodeTiled not available from the driver");
+  auto st = [&](int64_t n, int64_t s) { return static_cast<cuuint64_t>(n > 1 ? s : D) * 2; };  // (an extent of 1 never advances)
+  const cuuint64_t dims[4] = {static_cast<cuuint64_t>(D), static_cast<cuuint64_t>(n1), static_cast<cuuint64_t>(n2), static_cast<cuuint64_t>(n3)};
+  const cuuint64_t strides[3] = {st(n1, s1), st(n2, s2), st(n3, s3)};
+  const cuuint32_t box[4] = {64, static_cast<cuuint32_t>(b1), static_cast<cuuint32_t>(b2), 1}, one[4] = {1, 1, 1, 1};
+  const CUresult r = enc(map, dtype == KFA_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, ptr, dims, strides, box,
+                         one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(KFA_ERR_CUDA, "cuTensorMapEncodeTiled(%s) failed with CUresult %d", name, static_cast<int>(r));
+  return KFA_OK;
+}
+
+constexpr int SMS = 148;  // (what this library is built for)
+
+// How an attention call is cut up: a function of the shapes alone, so that the scratch it needs is known beforehand.
+struct AttendPlan {
+  int nr, gt, tt, head_tiles, row_tiles, grid;
+  bool whole;
+  int64_t meta_bytes, ml_bytes, bytes;
+};
+
+AttendPlan plan_attend(int64_t batch, int64_t heads, int64_t kv_heads, int64_t T, int64_t capacity, bool fresh) {
+  AttendPlan a;
+  const int64_t group = heads / kv_heads;
+  // Rows that share a K / V head, up to 128 of them in a tile: whole groups of heads, the tokens in equal parts.
+  const int64_t gt = std::min<int64_t>(group, 128), most = 128 / gt;
+  const int64_t token_tiles = (T + most - 1) / most;
+  const int64_t tt = (T + token_tiles - 1) / token_tiles;
+  a.gt = static_cast<int>(gt);
+  a.tt = static_cast<int>(tt);
+  a.head_tiles = static_cast<int>((group + gt - 1) / gt);
+  a.row_tiles = static_cast<int>(a.head_tiles * ((T + tt - 1) / tt));
+  a.nr = gt * tt <= 16 ? 16 : (gt * tt <= 32 ? 32 : (gt * tt <= 64 ? 64 : 128));
+  const int64_t items = batch * kv_heads * a.row_tiles;
+  const int64_t units = std::max<int64_t>((capacity + 31) / 32 + (fresh ? (T + 31) / 32 : 0), 1);
+  a.whole = units <= 8;
+  a.grid = static_cast<int>(std::min<int64_t>(SMS, a.whole ? items : (items * units + 3) / 4));
+  a.meta_bytes = a.ml_bytes = a.bytes = 0;
+  if (!a.whole) {
+    a.meta_bytes = (16 * a.grid + 255) / 256 * 256;
+    a.ml_bytes = 2ll * a.grid * 3 * a.nr * 4;
+    a.bytes = a.meta_bytes + a.ml_bytes + 2ll * a.grid * a.nr * 128 * 4;
+  }
+  return a;
+}
+
+template <int NC, int NR, bool BF16>
+int launch_attend(const CUtensorMap (&m)[5], const kfa::AttendParams& p, const AttendPlan& plan, cudaStream_t s) {
+  auto kern = kfa::kfa_cache_attend_kernel<NC, NR, BF16>;
+  using Cfg = kfa::AttCfg<NC, NR>;
+  KFA_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM));
+  kern<<<plan.grid, kfa::ATT_THREADS, Cfg::SMEM, s>>>(m[0], m[1], m[2], m[3], m[4], p);
+  KFA_CUDA(cudaGetLastError());
+  if (plan.whole) return KFA_OK;
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3(plan.grid, NR / 8);
+  config.blockDim = dim3(256);
+  config.stream = s;
+  cudaLaunchAttribute early[1];
+  early[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early[0].val.programmaticStreamSerializationAllowed = 1;
+  config.attrs = early;
+  config.numAttrs = 1;
+  KFA_CUDA(cudaLaunchKernelEx(&config, kfa::kfa_cache_join_kernel<NR, BF16>, p));
+  return KFA_OK;
+}
+
+template <int NC, bool BF16>
+int launch_attend_rows(const CUtensorMap (&m)[5], const kfa::AttendParams& p, const AttendPlan& plan, cudaStream_t s) {
+  switch (plan.nr) {
+    case 16: return launch_attend<NC, 16, BF16>(m, p, plan, s);
+    case 32: return launch_attend<NC, 32, BF16>(m, p, plan, s);
+    case 64: return launch_attend<NC, 64, BF16>(m, p, plan, s);
+    default: return launch_attend<NC, 128, BF16>(m, p, plan, s);
+  }
+}
+
 }  // namespace
 
 extern "C" {
 
 int64_t kfa_cache_attend_bytes(const KfaTensor4* q, const KfaCache* cache, const KfaTensor4* k) {
-  (void)q, (void)cache, (void)k;
-  return 0;
+  if (!q || !cache) return 0;
+  const int64_t page = cache->k.shape[2], kv_heads = cache->k.shape[1];
+  if (q->shape[0] < 1 || q->shape[1] < 1 || q->shape[2] < 1 || kv_heads < 1 || q->shape[1] < kv_heads || page < 1) return 0;  // (refused by the call)
+  return plan_attend(q->shape[0], q->shape[1], kv_heads, q->shape[2], cache->table ? cache->table_cols * page : page, k != nullptr).bytes;
 }
 
 int kfa_cache_attend(const KfaTensor4* q, const KfaCache* cache, const KfaTensor4* k, const KfaTensor4* v, const uint8_t* tree,
                      const int64_t* tree_stride, const int32_t* counts, const KfaTensor4* out, float* stats, void* scratch,
                      float scale, int dtype, int* dev_status, void* stream) {
-  (void)scratch;
   kfa::AttendParams p;
   std::memset(&p, 0, sizeof(p));
   int rc;
@@ -108,11 +192,8 @@ int kfa_cache_attend(const KfaTensor4* q, const KfaCache* cache, const KfaTensor
     if (k->shape[2] != q->shape[2] || v->shape[2] != q->shape[2]) return fail(KFA_ERR_ARG, "k, v: as many new tokens as q");
     p.k = static_cast<const uint8_t*>(k->ptr);
     p.v = static_cast<const uint8_t*>(v->ptr);
-    p.k_sb = 2 * k->stride[0], p.k_sh = 2 * k->stride[1], p.k_ss = 2 * k->stride[2];
     p.v_sb = 2 * v->stride[0], p.v_sh = 2 * v->stride[1], p.v_ss = 2 * v->stride[2];
   }
-  p.q = static_cast<const uint8_t*>(q->ptr);
-  p.q_sb = 2 * q->stride[0], p.q_sh = 2 * q->stride[1], p.q_ss = 2 * q->stride[2];
   p.o = static_cast<uint8_t*>(out->ptr);
   p.o_sb = 2 * out->stride[0], p.o_sh = 2 * out->stride[1], p.o_ss = 2 * out->stride[2];
   p.tree = tree;
@@ -122,15 +203,48 @@ int kfa_cache_attend(const KfaTensor4* q, const KfaCache* cache, const KfaTensor
   p.H = static_cast<int>(q->shape[1]);
   p.T = static_cast<int>(q->shape[2]);
   p.group = p.H / p.c.heads;
-  p.scale_log2 = scale * LOG2E;
+  // (a scale of 0 makes all scores equal: so does this one, and hidden scores of -inf stay what they are)
+  p.c_log2 = std::max(scale * LOG2E, 1e-30f);
+  p.slack = 8.f / p.c_log2;
   p.status = dev_status;
-  if (p.H > 65535) return fail(KFA_ERR_ARG, "too many heads");
-  const dim3 grid(p.T, p.H, p.c.batch);
+  const AttendPlan plan = plan_attend(p.c.batch, p.H, p.c.heads, p.T, p.c.capacity, k != nullptr);
+  if (static_cast<int64_t>(p.c.batch) * p.c.heads * plan.row_tiles > 0x7fffffff) return fail(KFA_ERR_ARG, "too many rows in one call");
+  if (plan.bytes && (!scratch || reinterpret_cast<uintptr_t>(scratch) % 16)) return fail(KFA_ERR_ARG, "scratch: null or not 16-byte aligned");
+  p.gt = plan.gt;
+  p.tt = plan.tt;
+  p.head_tiles = plan.head_tiles;
+  p.row_tiles = plan.row_tiles;
+  p.items = p.c.heads * plan.row_tiles;
+  p.by_gt = kfa::FastDiv::by(p.gt);
+  p.by_items = kfa::FastDiv::by(p.items);
+  p.by_row_tiles = kfa::FastDiv::by(p.row_tiles);
+  p.by_head_tiles = kfa::FastDiv::by(p.head_tiles);
+  p.whole = plan.whole;
+  p.box = p.c.table ? (p.c.page % 32 == 0 ? 32 : (p.c.page % 16 == 0 ? 16 : 8)) : 32;
+  if (!plan.whole) {
+    uint8_t* at = static_cast<uint8_t*>(scratch);
+    p.part_meta = reinterpret_cast<int4*>(at);
+    p.part_ml = reinterpret_cast<float*>(at + plan.meta_bytes);
+    p.part_o = reinterpret_cast<float*>(at + plan.meta_bytes + plan.ml_bytes);
+  }
+  CUtensorMap m[5];
+  const KfaTensor4 *ck = &cache->k, *cv = &cache->v;
+  const int64_t D = p.c.cols;
+  auto pages = [&](const KfaTensor4* t, CUtensorMap* map, const char* name) {
+    return make_box_map(t->ptr, D, t->shape[2], t->stride[2], t->shape[1], t->stride[1], t->shape[0], t->stride[0], p.box, 1, dtype, map, name);
+  };
+  if ((rc = make_box_map(q->ptr, D, p.H, q->stride[1], p.T, q->stride[2], p.c.batch, q->stride[0], p.gt, p.tt, dtype, &m[0], "q")) ||
+      (rc = pages(ck, &m[1], "cache keys")) || (rc = pages(cv, &m[2], "cache values")))
+    return rc;
+  m[3] = m[1];
+  m[4] = m[2];
+  auto fresh = [&](const KfaTensor4* t, CUtensorMap* map, const char* name) {
+    return make_box_map(t->ptr, D, p.T, t->stride[2], p.c.heads, t->stride[1], p.c.batch, t->stride[0], kfa::ATT_UNIT, 1, dtype, map, name);
+  };
+  if (k && ((rc = fresh(k, &m[3], "k")) || (rc = fresh(v, &m[4], "v")))) return rc;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (dtype == KFA_BF16) kfa::kfa_cache_attend_simple_kernel<true><<<grid, 128, 0, s>>>(p);
-  else kfa::kfa_cache_attend_simple_kernel<false><<<grid, 128, 0, s>>>(p);
-  KFA_CUDA(cudaGetLastError());
-  return KFA_OK;
+  if (dtype == KFA_BF16) return D > 64 ? launch_attend_rows<2, true>(m, p, plan, s) : launch_attend_rows<1, true>(m, p, plan, s);
+  return D > 64 ? launch_attend_rows<2, false>(m, p, plan, s) : launch_attend_rows<1, false>(m, p, plan, s);
 }
 
 int kfa_cache_append(const KfaCache* cache, const KfaTensor4* k, const KfaTensor4* v, const KfaRows* rows, int* dev_status,

@@ -46,94 +46,6 @@ __device__ __forceinline__ bool cache_place(const CacheView& c, int b, int pos, 
   return page >= 0 && page < c.n_pages;
 }
 
-// ---- attention of new tokens ---------------------------------------------------------------------------------------------
-struct AttendParams {
-  CacheView c;
-  const uint8_t *q, *k, *v;  // k, v null: no new keys
-  long long q_sb, q_sh, q_ss, k_sb, k_sh, k_ss, v_sb, v_sh, v_ss;  // bytes
-  const uint8_t* tree;
-  long long tree_sb, tree_st, tree_sj;
-  const int* counts;
-  uint8_t* o;
-  long long o_sb, o_sh, o_ss;
-  float* stats;
-  int H, T, group;
-  float scale_log2;
-  int* status;
-};
-
-// One CTA per query row: its four warps take every fourth key, a lane four columns; their parts are joined at the end.
-template <bool BF16>
-__global__ void __launch_bounds__(128) kfa_cache_attend_simple_kernel(const AttendParams p) {
-  const int t = blockIdx.x, h = blockIdx.y, b = blockIdx.z, g = h / p.group;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, cols = p.c.cols;
-  __shared__ float s_m[4], s_l[4], s_o[4][128];
-  const int count = p.counts ? min(max(p.counts[b], 0), p.T) : p.T;
-  const int len = cache_length(p.c, b);
-  bool bad = !length_ok(p.c, b);
-  float q[4], o[4] = {0.f, 0.f, 0.f, 0.f}, m = -INFINITY, l = 0.f;
-  const uint8_t* q_row = p.q + b * p.q_sb + h * p.q_sh + t * p.q_ss;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) q[i] = 4 * lane + i < cols ? load16<BF16>(q_row + 2 * (4 * lane + i)) : 0.f;
-  const int keys = t < count ? len + (p.k ? count : 0) : 0;
-  for (int j = warp; j < keys; j += 4) {
-    const uint8_t *k, *v;
-    if (j < len) {
-      int page, slot;
-      if (!cache_place(p.c, b, j, page, slot)) {
-        bad = true;
-        continue;
-      }
-      k = p.c.k + page * p.c.k_sn + g * p.c.k_sh + slot * p.c.k_ss;
-      v = p.c.v + page * p.c.v_sn + g * p.c.v_sh + slot * p.c.v_ss;
-    } else {
-      const int n = j - len;
-      if (p.tree ? p.tree[b * p.tree_sb + t * p.tree_st + n * p.tree_sj] == 0 : n > t) continue;
-      k = p.k + b * p.k_sb + g * p.k_sh + n * p.k_ss;
-      v = p.v + b * p.v_sb + g * p.v_sh + n * p.v_ss;
-    }
-    float s = 0.f;
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (4 * lane + i < cols) s += q[i] * load16<BF16>(k + 2 * (4 * lane + i));
-#pragma unroll
-    for (int w = 16; w; w >>= 1) s += __shfl_xor_sync(0xffffffffu, s, w);
-    const float m_new = fmaxf(m, s), alpha = ex2((m - m_new) * p.scale_log2), e = ex2((s - m_new) * p.scale_log2);
-    l = (m == -INFINITY ? 0.f : l * alpha) + e;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float x = 4 * lane + i < cols ? load16<BF16>(v + 2 * (4 * lane + i)) : 0.f;
-      o[i] = (m == -INFINITY ? 0.f : o[i] * alpha) + e * x;
-    }
-    m = m_new;
-  }
-  if (lane == 0) s_m[warp] = m, s_l[warp] = l;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) s_o[warp][4 * lane + i] = o[i];
-  bad = __syncthreads_or(bad) || *reinterpret_cast<volatile int*>(p.status) != 0;
-  if (!length_ok(p.c, b) && threadIdx.x == 0) report(p.status, DEV_BAD_CACHE);
-  if (bad && threadIdx.x == 0) report(p.status, DEV_BAD_CACHE);
-  const float m_all = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
-  float l_all = 0.f, x = 0.f;
-  for (int w = 0; w < 4; ++w) {
-    if (s_m[w] == -INFINITY) continue;
-    const float a = ex2((s_m[w] - m_all) * p.scale_log2);
-    l_all += s_l[w] * a;
-    x += s_o[w][threadIdx.x] * a;
-  }
-  const bool some = l_all != 0.f;
-  x = bad ? __int_as_float(0x7fc00000) : (some ? x / l_all : 0.f);
-  if (threadIdx.x < cols) {
-    const uint32_t w = pack16<BF16>(x, x);
-    *reinterpret_cast<uint16_t*>(p.o + b * p.o_sb + h * p.o_sh + t * p.o_ss + 2 * threadIdx.x) = static_cast<uint16_t>(w);
-  }
-  if (p.stats && threadIdx.x == 0) {
-    float* at = p.stats + (static_cast<long long>(b) * p.H + h) * 2 * p.T + t;
-    at[0] = bad ? __int_as_float(0x7fc00000) : (some ? m_all : INFINITY);
-    at[p.T] = bad ? __int_as_float(0x7fc00000) : (some ? log2f(l_all) : 0.f);
-  }
-}
-
 // ---- append --------------------------------------------------------------------------------------------------------------
 struct AppendParams {
   CacheView c;
