@@ -3,22 +3,26 @@
 //   S = q K^T,  m = max S,  P = exp2((S - m) c),  l = sum P,  out = P V / l,  c = scale * log2(e)
 //
 // What bounds it: the keys and values, read once each (2 x 2 D bytes a position and K / V head). All query rows that share them, the
-// query heads of a K / V head times the new tokens, are one tile; with few rows that is far below what makes the tensor core
-// the limit, so the tile is turned around: the KEYS are the 128 rows of the matrix instructions, the query rows their N columns
-// (16, 32 or 64), and nothing is computed for rows that are not there:
+// query heads of a K / V head times the new tokens, are one tile of rows. There are two kernels.
+//
+// Up to 64 rows (kfa_cache_attend_kernel): far below what makes the tensor core the limit, so the tile is turned around: the KEYS are the
+// 128 rows of the matrix instructions, the query rows their N columns (16, 32 or 64), and little is computed for rows that are not there:
 //   S^T [128 keys x N] = K Q^T                 A = K from shared memory as copied, B = Q
 //   O^T [D x N]       += V^T P^T               A = V as copied (the transposed, MN-major, operand), B = P^T from shared memory
 // A thread holds one key's scores. The maximum over keys is a warp reduction per column and an exchange between four warps; the sum
-// over keys stays in the thread until the end. O^T is rescaled only when a row's maximum grew by more than a factor of 2^8
-// (the numerators may be up to 2^8 then, which 16-bit P takes at the same relative precision).
+// over keys stays in the thread until the end.
+// More rows (kfa_cache_attend_rows_kernel): rows on the matrix rows, a thread a row, P from tensor memory, as in the forward of whole
+// sequences. (A thread of the first kernel spends 3400 clk on 128 rows x 128 keys, one of this kernel 3600 on 256 x 128.)
+// In both O is rescaled only when a row's maximum grew by more than a factor of 2^8 (the numerators may be up to 2^8 then, which 16-bit P
+// takes at the same relative precision).
 //
 // Work is cut by keys, not by sequences: the keys of all (sequence, K / V head, row tile) items are counted in units of 32 and every CTA
-// takes an equal stretch, whatever the lengths (which only the device knows). An item that one CTA has whole is written by it;
-// of the others the CTA leaves its part (unnormalised O in fp32, m, l) in scratch and a second kernel joins them in the order of the keys, so
-// that results repeat bit for bit.
+// takes an equal stretch, whatever the lengths (which only the device knows). An item counts some units more than it has, for what its
+// beginning and its end take. An item that one CTA has whole is written by it; of the others the CTA leaves its part (unnormalised O in
+// fp32, m, l) in scratch and a second kernel joins them in the order of the keys, so that results repeat bit for bit.
 //
-//   warps 0-3, 4-7  two streams. N <= 64: tiles of 128 keys go to the two in turn, each with its own maxima, sums and O, joined at the
-//                   item's end; 128 rows: both see every tile, each with 64 of the rows.
+//   warps 0-3, 4-7  two streams: tiles of 128 keys go to the two in turn, each with its own maxima, sums and O, joined at the item's end
+//                   (with more than 128 rows both see every tile, each with half of the rows)
 //   warps 8, 9      MMA issue for the two streams
 //   warps 10, 11    TMA producers: keys (and queries), values; a lane per box of up to 32 rows inside a page
 #pragma once
@@ -47,45 +51,58 @@ struct AttendParams {
   int H, T, group;
   int gt, tt, head_tiles, row_tiles;  // a row tile: gt heads x tt tokens, head_tiles x token tiles = row_tiles of them per K / V head
   FastDiv by_gt, by_items, by_row_tiles, by_head_tiles;
+  FastDiv by_grid;
   int items;       // per sequence: K / V heads x row tiles
   int whole;       // every item is one CTA's (short caches: nothing is cut)
+  int least;       // the shortest stretch of a CTA, in units
+  int extra;       // units that an item counts more than it has
   int box;         // rows of a page's TMA box
+  int rows;        // of scratch per part
   float c_log2, slack;  // scale * log2 e; how far a maximum may grow before O is rescaled
-  float* part_o;   // [slot][NR][128]
-  float* part_ml;  // [slot][3][NR]: m, l, largest score
+  float* part_o;   // [slot][rows][128]
+  float* part_ml;  // [slot][3][rows]: m, l, largest score
   int4* part_meta; // [CTA]: parts of the item that begins in it and ends in another (0: none), sequence, item
   int* status;
 };
 
-// The stretch of work of a CTA, walked item by item; every role walks for itself.
+// The stretch of work of a CTA, from (b, item, unit) to (end_b, end_item, end_unit), walked item by item; every role walks for itself.
 struct Walk {
-  int b, item, unit, units, uc, ud, len, count;  // unit: first of the current segment; uc, ud: units of cached and of new keys
-  int n;                                         // units of the current segment
-  long long left;                                // units (whole: items) left, the current segment's included
+  int b, item, unit, end_b, end_item, end_unit;
+  int units, uc, ud, len, count;  // of the item; uc, ud: units of cached and of new keys
+  int n;                          // units of the current segment, the part of the item that is this CTA's
   __device__ __forceinline__ static void size(const AttendParams& p, int b, int& len, int& count, int& uc, int& ud) {
     len = cache_length(p.c, b);
     count = p.counts ? min(max(p.counts[b], 0), p.T) : p.T;
     uc = count ? (len + ATT_UNIT - 1) / ATT_UNIT : 0;
     ud = count && p.k ? (count + ATT_UNIT - 1) / ATT_UNIT : 0;
   }
+  __device__ __forceinline__ static int units_of(const AttendParams& p, int b) {
+    int len, count, uc, ud;
+    size(p, b, len, count, uc, ud);
+    return max(uc + ud, 1);
+  }
+  __device__ __forceinline__ bool last() const { return b == end_b && item == end_item; }
   __device__ __forceinline__ void load(const AttendParams& p) {
     size(p, b, len, count, uc, ud);
     units = max(uc + ud, 1);
   }
-  __device__ __forceinline__ void cut(const AttendParams& p) {
-    n = units - unit;
-    if (!p.whole && n > left) n = static_cast<int>(left);
+  __device__ __forceinline__ void cut() { n = (last() ? min(units, end_unit) : units) - unit; }
+  __device__ __forceinline__ bool start(const AttendParams& p) {  // false: nothing to do
+    if (b == end_b && (item > end_item || (item == end_item && unit >= end_unit))) return false;
+    load(p);
+    cut();
+    return true;
   }
-  __device__ __forceinline__ bool next(const AttendParams& p) {  // false: that was the last segment
-    left -= p.whole ? 1 : n;
-    if (left <= 0) return false;
+  __device__ __forceinline__ bool next(const AttendParams& p) {  // false: that was the last segment, and it stays the current one
+    if (last()) return false;
+    const bool other = item + 1 == p.items;
+    const int b2 = b + (other ? 1 : 0), item2 = other ? 0 : item + 1;
+    if (b2 == end_b && item2 == end_item && end_unit == 0) return false;
+    b = b2;
+    item = item2;
     unit = 0;
-    if (++item == p.items) {
-      item = 0;
-      ++b;
-      load(p);
-    }
-    cut(p);
+    if (other) load(p);
+    cut();
     return true;
   }
   __device__ __forceinline__ int tiles() const { return (n + 3) >> 2; }
@@ -93,35 +110,113 @@ struct Walk {
   __device__ __forceinline__ bool ends() const { return unit + n == units; }
 };
 
-template <int NC, int NR>
-struct AttCfg {
-  static constexpr bool BY_ROWS = NR == 128;        // the streams share the rows, not the tiles
-  static constexpr int N = BY_ROWS ? 64 : NR;       // columns of a stream
-  static constexpr int NQ = BY_ROWS ? 1 : 2;        // buffers for queries
-  static constexpr int NP = N <= 32 ? 2 : 1;        // buffers for P per stream
-  static constexpr int CHUNK = 128 * 64 * 2;        // 128 keys x 64 columns
+// Which work is this CTA's (all its threads; s_i: 32 ints of shared memory). Synchronises the CTA. chunk, end: units per CTA and where this
+// one's stretch ends, both as they are counted.
+__device__ __forceinline__ bool my_work(const AttendParams& p, int* s_i, Walk& w, int& chunk, int& end) {
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  chunk = end = 0;
+  if (p.whole) {
+    const unsigned all = static_cast<unsigned>(p.c.batch) * p.items;
+    const unsigned i0 = p.by_grid.div(static_cast<unsigned>(all)) * blockIdx.x + min(blockIdx.x, all - p.by_grid.div(all) * gridDim.x);
+    const unsigned i1 = i0 + p.by_grid.div(all) + (blockIdx.x < all - p.by_grid.div(all) * gridDim.x ? 1 : 0);
+    w.b = static_cast<int>(p.by_items.div(i0));
+    w.item = static_cast<int>(i0 - w.b * p.items);
+    w.end_b = static_cast<int>(p.by_items.div(i1));
+    w.end_item = static_cast<int>(i1 - w.end_b * p.items);
+    w.unit = w.end_unit = 0;
+    __syncthreads();
+    return w.start(p);
+  }
+  // the whole batch, 384 sequences at a time; then the sequences in which this CTA's stretch begins and ends
+  auto counted = [&](int b) { return b < p.c.batch ? (Walk::units_of(p, b) + p.extra) * p.items : 0; };
+  auto warp_scan = [&](int x) {
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+      const int up = __shfl_up_sync(0xffffffffu, x, off);
+      if (lane >= off) x += up;
+    }
+    return x;
+  };
+  int total = 0;
+  const int own0 = counted(tid), scan0 = warp_scan(own0);
+  for (int b0 = 0; b0 < p.c.batch; b0 += ATT_THREADS) {
+    const int s = b0 == 0 ? scan0 : warp_scan(counted(b0 + tid));
+    if (b0 > 0) __syncthreads();
+    if (lane == 31) s_i[8 + warp] = s;
+    __syncthreads();
+    for (int i = 0; i < ATT_THREADS / 32; ++i) total += s_i[8 + i];
+  }
+  chunk = max(static_cast<int>(p.by_grid.div(total + gridDim.x - 1)), p.least);
+  const long long at[2] = {static_cast<long long>(chunk) * blockIdx.x, static_cast<long long>(chunk) * (blockIdx.x + 1)};
+  int before = 0;
+  for (int b0 = 0; b0 < p.c.batch; b0 += ATT_THREADS) {
+    const int own = b0 == 0 ? own0 : counted(b0 + tid);
+    int upto = b0 == 0 ? scan0 : warp_scan(own);
+    if (p.c.batch > ATT_THREADS) {
+      __syncthreads();
+      if (lane == 31) s_i[8 + warp] = upto;
+      __syncthreads();
+    }
+    int all = 0;
+    for (int i = 0; i < ATT_THREADS / 32; ++i) {
+      const int x = s_i[8 + i];
+      if (i < warp) upto += x;
+      all += x;
+    }
+    upto += before;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      if (at[i] >= upto - own && at[i] < upto) {
+        s_i[2 * i] = b0 + tid;
+        s_i[2 * i + 1] = static_cast<int>(at[i]) - (upto - own);
+      }
+    }
+    before += all;
+  }
+  __syncthreads();
+  auto place = [&](int i, int& b, int& item, int& unit) {
+    b = p.c.batch;
+    item = unit = 0;
+    if (at[i] >= total) return;
+    b = s_i[2 * i];
+    const int off = s_i[2 * i + 1], each = Walk::units_of(p, b) + p.extra;
+    item = off / each;
+    unit = max(off - item * each - p.extra, 0);
+  };
+  place(0, w.b, w.item, w.unit);
+  place(1, w.end_b, w.end_item, w.end_unit);
+  end = static_cast<int>(at[1]);
+  return w.b < p.c.batch && w.start(p);
+}
+
+// Shared memory and rings that both kernels lay out alike. NC: chunks of 64 columns of the head dim; Q_ROWS: rows of the query buffer;
+// BOTH: both streams see every tile (else they take turns); OTHER: bytes beside keys, values and queries.
+template <int NC_, int Q_ROWS_, int NQ_, bool BOTH_, int OTHER_>
+struct AttRings {
+  static constexpr int NC = NC_, Q_ROWS = Q_ROWS_, NQ = NQ_;
+  static constexpr bool BOTH = BOTH_;
+  static constexpr int CHUNK = 128 * 64 * 2;  // 128 keys x 64 columns
   static constexpr int STAGE = NC * CHUNK;
-  static constexpr int Q_BYTES = NC * NR * 128;
-  static constexpr int P_BYTES = 128 * N * 2;
-  static constexpr int SMALL = 1024 + 2 * 2 * 4 * N * 4 + 8 * N * 4 + 2 * 2 * 6 * N * 4;  // barriers; maxima; shifts; final sums
-  static constexpr int FIXED = 1024 + NQ * Q_BYTES + 2 * NP * P_BYTES + SMALL;
+  static constexpr int Q_CHUNK = Q_ROWS * 128, Q_BYTES = NC * Q_CHUNK;
+  static constexpr int FIXED = 1024 + NQ * Q_BYTES + OTHER_;
   static constexpr int FIT = (232448 - FIXED) / STAGE;
-  // Rings of key tiles and of value tiles, in turn for each stream (BY_ROWS: one of each for both). A stage has one producer and the
-  // same consumers every time: who waits for a phase of its barrier has waited for the one before, and a parity means one phase.
-  static constexpr int RINGS = BY_ROWS ? 1 : 2;
-  static constexpr int DEEP = FIT / RINGS, MOST = BY_ROWS ? 4 : 2;
+  // Rings of key tiles and of value tiles, in turn for each stream (BOTH: one of each for both). A stage has one producer and the
+  // same consumers every time: who waits for a phase of its barrier has waited for the one before, so that a parity means one phase.
+  static constexpr int RINGS = BOTH ? 1 : 2;
+  static constexpr int DEEP = FIT / RINGS, MOST = BOTH ? 4 : 2;
   static constexpr int DV = DEEP / 2 < MOST ? DEEP / 2 : MOST;
   static constexpr int DK = DEEP - DV < MOST ? DEEP - DV : MOST;
   static_assert(DV >= 1 && DK >= 1, "no room for a tile of keys and one of values");
   static constexpr int NS = RINGS * (DK + DV);
-  static_assert(NS <= FIT, "ring too long");
   static constexpr int SMEM = FIXED + NS * STAGE;
-  __device__ static __forceinline__ int k_stage(int T) { return BY_ROWS ? T % DK : (T & 1) * DK + (T >> 1) % DK; }
-  __device__ static __forceinline__ int v_stage(int T) { return RINGS * DK + (BY_ROWS ? T % DV : (T & 1) * DV + (T >> 1) % DV); }
-  __device__ static __forceinline__ int k_turn(int T) { return (BY_ROWS ? T : T >> 1) / DK; }
-  __device__ static __forceinline__ int v_turn(int T) { return (BY_ROWS ? T : T >> 1) / DV; }
-  static constexpr uint32_t TMEM = N == 64 ? 512 : (N == 32 ? 256 : 128);  // 6 N columns: S 2 x 2, O 2
-  // (P and "P V has retired" have a barrier per buffer: a stream may be a buffer ahead of what waits for it.)
+  __device__ static __forceinline__ int k_stage(int T) { return BOTH ? T % DK : (T & 1) * DK + (T >> 1) % DK; }
+  __device__ static __forceinline__ int v_stage(int T) { return RINGS * DK + (BOTH ? T % DV : (T & 1) * DV + (T >> 1) % DV); }
+  __device__ static __forceinline__ int k_turn(int T) { return (BOTH ? T : T >> 1) / DK; }
+  __device__ static __forceinline__ int v_turn(int T) { return (BOTH ? T : T >> 1) / DV; }
+  // barriers: tiles there and free, queries there, scores there, P there, P V done, O read, all done
+  static constexpr int B_KV = 0, B_KVFREE = NS, B_Q = 2 * NS, B_S = B_Q + NQ, B_P = B_S + 4, B_PV = B_P + 4, B_OFREE = B_PV + 4,
+                       B_DRAIN = B_OFREE + 2, N_BARS = B_DRAIN + 2;
+  static_assert(N_BARS * 8 + 256 <= 1024, "barrier block");
 };
 
 __device__ __forceinline__ float warp_max(float x) {  // NaN counts as nothing
@@ -200,11 +295,12 @@ __device__ __forceinline__ float part_factor(float m, float l, float m_all, floa
   return ex2((m - m_all) * c_log2);
 }
 
-// The heads and tokens of a row tile's rows, and where a row's output lies (bytes), < 0: there is no such row.
+// The heads and tokens of a row tile's rows.
 struct RowMap {
-  int h0, heads, t0;  // first head, heads that exist, first token
+  int g, h0, heads, t0;  // K / V head; first head, heads that exist, first token
   __device__ __forceinline__ RowMap(const AttendParams& p, int item) {
-    const int g = static_cast<int>(p.by_row_tiles.div(item)), rt = item - g * p.row_tiles;
+    g = static_cast<int>(p.by_row_tiles.div(item));
+    const int rt = item - g * p.row_tiles;
     const int tile_t = static_cast<int>(p.by_head_tiles.div(rt)), tile_h = rt - tile_t * p.head_tiles;
     h0 = g * p.group + tile_h * p.gt;
     heads = min(p.gt, p.group - tile_h * p.gt);
@@ -218,285 +314,388 @@ struct RowMap {
   }
 };
 
-template <int NC, int NR, bool BF16>
-__global__ void __launch_bounds__(ATT_THREADS, 1)
-kfa_cache_attend_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
-                        const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmKn,
-                        const __grid_constant__ CUtensorMap tmVn, const AttendParams p) {
-  using Cfg = AttCfg<NC, NR>;
-  constexpr int N = Cfg::N, NS = Cfg::NS, NQ = Cfg::NQ, NP = Cfg::NP;
-  constexpr bool BY_ROWS = Cfg::BY_ROWS;
+// Control block of a CTA behind its barriers.
+struct AttCtl {
+  uint32_t* tmem;
+  volatile int *abort, *bad;  // bad: the cache says something that is not so, or an earlier kernel failed
+  volatile int* odd;          // [stream] 1 + the last segment in which it met new values that are not finite
+  int* ints;                  // 32, for my_work
+  __device__ __forceinline__ explicit AttCtl(uint64_t* behind) {
+    tmem = reinterpret_cast<uint32_t*>(behind);
+    abort = reinterpret_cast<volatile int*>(tmem + 1);
+    bad = abort + 1;
+    odd = abort + 2;
+    ints = reinterpret_cast<int*>(tmem + 8);
+  }
+};
 
-  extern __shared__ uint8_t smem_raw[];
-  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
-  uint8_t* smem = smem_raw + (base - smem_u32(smem_raw));
-  const uint32_t sKV = base, sQ = sKV + NS * Cfg::STAGE, sP = sQ + NQ * Cfg::Q_BYTES;
-  uint8_t* small = smem + NS * Cfg::STAGE + NQ * Cfg::Q_BYTES + 2 * NP * Cfg::P_BYTES;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(small);
-  float* s_max = reinterpret_cast<float*>(small + 1024);  // [stream][tile & 1][warp][N]
-  float* s_shift = s_max + 2 * 2 * 4 * N;                 // [warp][N]
-  float* s_fin = s_shift + 8 * N;                         // [segment & 1][stream]: l of four warps, m, largest score, each [N]
-  constexpr int B_KV = 0, B_KVFREE = NS, B_Q = 2 * NS, B_S = B_Q + NQ, B_P = B_S + 4, B_PV = B_P + 4, B_OFREE = B_PV + 4,
-                B_DRAIN = B_OFREE + 2, N_BARS = B_DRAIN + 2;
-  static_assert(N_BARS * 8 + 256 <= 1024, "barrier block");
-  uint32_t* s_tmem = reinterpret_cast<uint32_t*>(bars + N_BARS);
-  volatile int* s_abort = reinterpret_cast<volatile int*>(s_tmem + 1);
-  volatile int* s_bad = s_abort + 1;  // the cache says something that is not so, or an earlier kernel failed
-  volatile int* s_odd = s_abort + 2;  // [stream] 1 + the last segment in which it met new values that are not finite
-  int* s_b = reinterpret_cast<int*>(s_tmem + 5);                        // first sequence
-  long long* s_work = reinterpret_cast<long long*>(bars + N_BARS + 4);  // first unit in it; from [2]: warps' sums
-  const uint32_t bar0 = smem_u32(bars);
-  auto bar = [&](int i) { return bar0 + 8u * i; };
-
-  const int tid = threadIdx.x, warp = warp_index(), lane = tid & 31;
-
-  // ---- setup; which work is this CTA's ----
+// Both kernels' beginning: barriers, tensor memory, the CTA's work. p_arrivals: threads that announce a P buffer.
+template <class R>
+__device__ __forceinline__ bool att_setup(const AttendParams& p, uint32_t bar0, const AttCtl& ctl, int tmem_cols, Walk& first, int& chunk,
+                                          int& end) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (warp == 10) {
-    for (int i = lane; i < N_BARS; i += 32) {
+    for (int i = lane; i < R::N_BARS; i += 32) {
       int count = 1;
-      if (i >= B_KVFREE && i < B_Q) count = BY_ROWS ? 2 : 1;
-      if (i >= B_P && i < B_PV) count = 128;
-      if (i >= B_OFREE && i < B_DRAIN) count = BY_ROWS ? 128 : 256;
-      mbar_init(bar(i), count);
+      if (i >= R::B_KVFREE && i < R::B_Q) count = R::BOTH ? 2 : 1;
+      if (i >= R::B_P && i < R::B_PV) count = 128;
+      if (i >= R::B_OFREE && i < R::B_DRAIN) count = R::BOTH ? 128 : 256;
+      mbar_init(bar0 + 8u * i, count);
     }
     if (lane == 0) {
-      *s_abort = 0;
-      *s_bad = load_status(p.status) != 0;
-      s_odd[0] = s_odd[1] = 0;
+      *ctl.abort = 0;
+      *ctl.bad = load_status(p.status) != 0;
+      ctl.odd[0] = ctl.odd[1] = 0;
     }
     fence_mbar_init();
     fence_async_smem();
   }
   if (warp == 8) {
-    tmem_alloc(smem_u32(s_tmem), Cfg::TMEM);
+    tmem_alloc(smem_u32(ctl.tmem), tmem_cols);
     tmem_relinquish();
   }
-  Walk first;
-  long long chunk = 0, u1 = 0;  // units per CTA, the end of this one's
-  if (p.whole) {
-    const long long all = static_cast<long long>(p.c.batch) * p.items;
-    const long long i0 = all * blockIdx.x / gridDim.x, i1 = all * (blockIdx.x + 1) / gridDim.x;
-    first.b = static_cast<int>(p.by_items.div(static_cast<uint32_t>(i0)));
-    first.item = static_cast<int>(i0 - static_cast<long long>(first.b) * p.items);
-    first.left = i1 - i0;
-    first.unit = 0;
-    tc_fence_before();
-    __syncthreads();
-    tc_fence_after();
-  } else {
-    // units of the whole batch, 384 sequences at a time; then the sequence in which this CTA's stretch begins
-    auto units_of = [&](int b) {
-      if (b >= p.c.batch) return 0ll;
-      int len, count, uc, ud;
-      Walk::size(p, b, len, count, uc, ud);
-      return static_cast<long long>(max(uc + ud, 1)) * p.items;
-    };
-    auto warp_scan = [&](long long x) {
+  tc_fence_before();
+  const bool work = my_work(p, ctl.ints, first, chunk, end);
+  tc_fence_after();
+  if (!p.whole) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // (the joining kernel waits for this one's end all the same)
+  return work;
+}
+
+// The producers' role: warp 10 queries and keys, warp 11 values. Leaves how many tiles and segments' queries it has started.
+template <class R>
+__device__ __forceinline__ void att_produce(const AttendParams& p, const Walk& first, bool values, uint32_t sKV, uint32_t sQ, uint32_t bar0,
+                                            const AttCtl& ac, const CUtensorMap* q_map, const CUtensorMap* map, const CUtensorMap* map_new,
+                                            int& kv_issued, int& q_issued) {
+  const int lane = threadIdx.x & 31;
+  const Ctl ctl{ac.abort};
+  auto bar = [&](int i) { return bar0 + 8u * i; };
+  Walk w = first;
+  const int per_unit = ATT_UNIT / p.box, boxes = 4 * per_unit;
+  bool ok = true, more = true;
+  int T = 0, s = 0;  // tiles and segments so far
+  while (more && ok) {
+    const RowMap rows(p, w.item);
+    if (lane == 0 && !length_ok(p.c, w.b)) *ac.bad = 1;
+    if (!values) {
+      if (s >= R::NQ) {  // both streams are done with the segment that used this buffer
+        ok = mbar_wait_warp(bar(R::B_OFREE), (s - R::NQ) & 1, ctl, 70) && mbar_wait_warp(bar(R::B_OFREE + 1), (s - R::NQ) & 1, ctl, 71);
+        if (!ok) break;
+      }
+      if (lane == 0) {
+        mbar_expect_tx(bar(R::B_Q + s % R::NQ), R::NC * p.gt * p.tt * 128);
+        for (int ch = 0; ch < R::NC; ++ch)
+          tma_load_4d(sQ + (s % R::NQ) * R::Q_BYTES + ch * R::Q_CHUNK, q_map, bar(R::B_Q + s % R::NQ), ch * 64, rows.h0, rows.t0, w.b);
+      }
+      q_issued = s + 1;
+    }
+    const int tiles = w.tiles();
+    for (int t = 0; t < tiles && ok; ++t, ++T) {
+      // this lane's box
+      const int in_unit = (lane % per_unit) * p.box, unit = w.unit + 4 * t + lane / per_unit;
+      const bool mine = lane < boxes && unit < w.unit + w.n;
+      const int row = (lane / per_unit) * ATT_UNIT + in_unit;
+      int c1 = 0, c3 = w.b, kind = 0;  // 1: cached rows, 2: new ones
+      if (mine && unit < w.uc) {
+        const int pos = unit * ATT_UNIT + in_unit;
+        if (pos < w.len) {
+          if (cache_place(p.c, w.b, pos, c3, c1)) kind = 1;
+          else *ac.bad = 1;
+        }
+      } else if (mine && in_unit == 0) {
+        c1 = (unit - w.uc) * ATT_UNIT;
+        if (c1 < w.count && w.ud > 0) kind = 2;
+      }
+      const unsigned cached = __ballot_sync(0xffffffffu, kind == 1), fresh = __ballot_sync(0xffffffffu, kind == 2);
+      const int stage = values ? R::v_stage(T) : R::k_stage(T), turn = values ? R::v_turn(T) : R::k_turn(T);
+      if (turn > 0) {
+        ok = mbar_wait_warp(bar(R::B_KVFREE + stage), (turn - 1) & 1, ctl, 72);
+        if (!ok) break;
+      }
+      if (lane == 0) mbar_expect_tx(bar(R::B_KV + stage), R::NC * 128 * (__popc(cached) * p.box + __popc(fresh) * ATT_UNIT));
+      __syncwarp();
+      if (kind != 0) {
+        const uint32_t dst = sKV + stage * R::STAGE + row * 128;
+        for (int ch = 0; ch < R::NC; ++ch) tma_load_4d(dst + ch * R::CHUNK, kind == 1 ? map : map_new, bar(R::B_KV + stage), ch * 64, c1, rows.g, c3);
+      }
+      kv_issued = T + 1;
+    }
+    if (ok) {
+      ++s;
+      more = w.next(p);
+    }
+  }
+}
+
+// A stream's tiles one after the other, over all segments.
+struct AttTile {
+  int T, s;
+  bool opens;  // the stream's first tile of segment s
+};
+template <bool BOTH>
+struct AttTiles {
+  Walk w;
+  int st, at = 0, T = 0, s = 0;
+  bool more = true, opens = true;
+  __device__ __forceinline__ bool take(const AttendParams& p, AttTile& t) {
+    while (more) {
+      while (at < w.tiles()) {
+        ++at;
+        const int now = T++;
+        if (BOTH || (now & 1) == st) {
+          t = {now, s, opens};
+          opens = false;
+          return true;
+        }
+      }
+      at = 0;
+      ++s;
+      opens = true;
+      more = w.next(p);
+    }
+    return false;
+  }
+};
+
+// The issuing warps' loop: scores of piece i as soon as their keys (and queries) are there and the columns free, which they are once the
+// values of piece i - 2 have been issued, values of piece j as soon as P and V are there, whichever comes first: neither holds the other up
+// (keys that are late would delay values whose results others wait for). PIECES of a tile: 1, or 2 halves of 64 keys.
+// issue_S(tile, c, piece), issue_PV(tile, c, piece) issue and commit; c counts the stream's tiles.
+template <class R, int PIECES, int NP, typename FS, typename FP>
+__device__ __forceinline__ void att_issue(const AttendParams& p, const Walk& first, int st, uint32_t bar0, const AttCtl& ac, FS issue_S, FP issue_PV) {
+  auto ready = [&](int i, uint32_t parity) { return __all_sync(0xffffffffu, mbar_test(bar0 + 8u * i, parity)); };
+  AttTiles<R::BOTH> tiles{first, st};
+  AttTile ahead = {0, 0, false}, even = ahead, odd = ahead;  // the next to get scores; those that have, by c (at most two wait for values)
+  bool have = tiles.take(p, ahead);
+  int i_s = 0, i_p = 0;  // pieces of scores and of values issued
+  long long t0 = clock64();
+  while (have || i_p < i_s) {
+    bool went = false;
+    if (have && i_s <= i_p + 1) {
+      const int c = i_s / PIECES, piece = i_s % PIECES;
+      if (piece > 0 || (ready(R::B_KV + R::k_stage(ahead.T), R::k_turn(ahead.T) & 1) &&
+                        (!ahead.opens || ready(R::B_Q + ahead.s % R::NQ, (ahead.s / R::NQ) & 1)))) {
+        tc_fence_after();
+        issue_S(ahead, c, piece);
+        ++i_s;
+        went = true;
+        if (piece == PIECES - 1) {
+          if (c & 1) odd = ahead;
+          else even = ahead;
+          have = tiles.take(p, ahead);
+        }
+      }
+    }
+    if (i_p < i_s) {
+      const int c = i_p / PIECES, piece = i_p % PIECES;
+      const AttTile now = (c * PIECES + PIECES > i_s) ? ahead : ((c & 1) ? odd : even);  // (its second half may have no scores yet)
+      if (ready(R::B_P + 2 * st + (PIECES == 2 ? piece : c % NP), (PIECES == 2 ? c : c / NP) & 1) &&
+          (piece > 0 || (ready(R::B_KV + R::v_stage(now.T), R::v_turn(now.T) & 1) &&
+                         (!now.opens || now.s == 0 || ready(R::B_OFREE + st, (now.s - 1) & 1))))) {
+        tc_fence_after();
+        issue_PV(now, c, piece);
+        ++i_p;
+        went = true;
+      }
+    }
+    if (went) {
+      t0 = clock64();
+    } else if (*ac.abort != 0) {
+      break;
+    } else if (clock64() - t0 > KFA_WAIT_CYCLES) {
+      *ac.abort = KFA_DEV_TIMEOUT_BASE + 73;
+      break;
+    }
+  }
+  // what was issued has retired before tensor memory is freed
+  const bool lead = elect_one();
+  umma_commit_lead(lead, bar0 + 8u * (R::B_DRAIN + st));
+  mbar_drain(bar0 + 8u * (R::B_DRAIN + st), 0);
+}
+
+// Which keys of a unit the row of token t sees, a bit each (the first pass of a masked tile).
+__device__ __forceinline__ uint32_t seen_word(const AttendParams& p, const Walk& w, int unit, int t) {
+  if (unit >= w.unit + w.n) return 0u;
+  if (unit < w.uc) {
+    const int left = w.len - unit * ATT_UNIT;
+    return left >= ATT_UNIT ? 0xffffffffu : (1u << left) - 1u;
+  }
+  if (w.ud == 0 || t >= w.count) return 0u;
+  const int j0 = (unit - w.uc) * ATT_UNIT, left = w.count - j0;
+  if (left <= 0) return 0u;
+  uint32_t there = left >= ATT_UNIT ? 0xffffffffu : (1u << left) - 1u;
+  if (p.tree == nullptr) {
+    const int upto = t - j0;  // tokens 0 .. t
+    return upto < 0 ? 0u : (upto >= ATT_UNIT - 1 ? there : there & ((2u << upto) - 1u));
+  }
+  const uint8_t* tree = p.tree + w.b * p.tree_sb + t * p.tree_st + j0 * p.tree_sj;
+  uint32_t seen = 0;
+#pragma unroll 8
+  for (int j = 0; j < ATT_UNIT; ++j)
+    if (j < left && tree[j * p.tree_sj] != 0) seen |= 1u << j;
+  return seen & there;
+}
+
+// Values behind the end may be anything, and 0 * NaN is no 0: in a tile that is not full of cached keys, the thread of key `key` zeroes
+// its row of the tile. So it does with the values of a new token that are not finite, which would otherwise reach rows that do not see it; the
+// epilogue hands them to those that do. Returns whether there were such. fresh: the new token that the key is, < 0: a cached one.
+template <int NC, bool BF16>
+__device__ __forceinline__ bool clean_values(const AttendParams& p, const Walk& w, int g, uint32_t stage, int key, bool valid, int fresh) {
+  const uint32_t row = stage + key * 128;
+  bool found = false;
+  if (!valid) {
 #pragma unroll
-      for (int off = 1; off < 32; off <<= 1) {
-        const long long up = __shfl_up_sync(0xffffffffu, x, off);
-        if (lane >= off) x += up;
+    for (int i = 0; i < NC * 8; ++i)
+      asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(row + (i >> 3) * (128 * 128) + (i & 7) * 16), "r"(0) : "memory");
+  } else if (fresh >= 0) {
+    const uint8_t* g_row = p.v + w.b * p.v_sb + g * p.v_sh + fresh * p.v_ss;
+#pragma unroll 4
+    for (int i = 0; i < p.c.cols / 8; ++i) {
+      const uint4 q4 = *reinterpret_cast<const uint4*>(g_row + 16 * i);
+      uint32_t q[4] = {q4.x, q4.y, q4.z, q4.w};
+      bool odd = false;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        constexpr uint32_t E = BF16 ? 0x7f80u : 0x7c00u;  // all exponent bits: infinity or NaN
+        if ((q[j] & E) == E) q[j] &= 0xffff0000u, odd = true;
+        if (((q[j] >> 16) & E) == E) q[j] &= 0xffffu, odd = true;
       }
-      return x;
-    };
-    long long total = 0;
-    const long long mine0 = units_of(tid), scan0 = warp_scan(mine0);
-    for (int b0 = 0; b0 < p.c.batch; b0 += ATT_THREADS) {
-      const long long s = b0 == 0 ? scan0 : warp_scan(units_of(b0 + tid));
-      if (b0 > 0) __syncthreads();
-      if (lane == 31) s_work[2 + warp] = s;
-      __syncthreads();
-      for (int w = 0; w < ATT_THREADS / 32; ++w) total += s_work[2 + w];
-    }
-    chunk = max((total + gridDim.x - 1) / gridDim.x, 4ll);
-    const long long u0 = chunk * blockIdx.x;
-    u1 = min(u0 + chunk, total);
-    long long before = 0;
-    for (int b0 = 0; b0 < p.c.batch; b0 += ATT_THREADS) {
-      const long long own = b0 == 0 ? mine0 : units_of(b0 + tid);
-      long long end = b0 == 0 ? scan0 : warp_scan(own);
-      if (p.c.batch > ATT_THREADS) {
-        __syncthreads();
-        if (lane == 31) s_work[2 + warp] = end;
-        __syncthreads();
+      if (odd) {
+        found = true;
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(row + (i >> 3) * (128 * 128) + (((i & 7) ^ (key & 7)) << 4)),
+                     "r"(q[0]), "r"(q[1]), "r"(q[2]), "r"(q[3])
+                     : "memory");
       }
-      for (int w = 0; w < ATT_THREADS / 32; ++w) {
-        if (w < warp) end += s_work[2 + w];
-      }
-      if (u0 >= before + end - own && u0 < before + end) {
-        *s_b = b0 + tid;
-        s_work[0] = u0 - (before + end - own);
-      }
-      for (int w = 0; w < ATT_THREADS / 32; ++w) before += s_work[2 + w];
-    }
-    tc_fence_before();
-    __syncthreads();
-    tc_fence_after();
-    first.left = max(u1 - u0, 0ll);
-    first.b = first.item = first.unit = 0;
-    if (first.left > 0) {
-      first.b = *s_b;
-      int len, count, uc, ud;
-      Walk::size(p, first.b, len, count, uc, ud);
-      const int units = max(uc + ud, 1);
-      first.item = static_cast<int>(s_work[0] / units);
-      first.unit = static_cast<int>(s_work[0] - static_cast<long long>(first.item) * units);
     }
   }
-  const bool work = first.left > 0;
-  if (work) {
-    first.load(p);
-    first.cut(p);
+  return found;
+}
+// What key `key` of the tile at unit ub is: whether it exists; the new token that it is, < 0: a cached one.
+__device__ __forceinline__ bool which_key(const Walk& w, int ub, int key, int& fresh) {
+  const int unit = ub + (key >> 5);
+  fresh = -1;
+  if (unit >= w.unit + w.n) return false;
+  if (unit < w.uc) return unit * ATT_UNIT + (key & 31) < w.len;
+  const int j = (unit - w.uc) * ATT_UNIT + (key & 31);
+  if (w.ud == 0 || j >= w.count) return false;
+  fresh = j;
+  return true;
+}
+// Whether the row of token t sees new token j.
+__device__ __forceinline__ bool sees_new(const AttendParams& p, const Walk& w, int t, int j) {
+  return t < w.count && (p.tree ? p.tree[w.b * p.tree_sb + t * p.tree_st + j * p.tree_sj] != 0 : j <= t);
+}
+
+// After a wait that ran out: the copies that the producers have started land, and the rows of what the CTA had whole read as NaN (what
+// was cut, the joining kernel sees to). All threads, behind a barrier.
+template <class R>
+__device__ __forceinline__ void att_give_up(const AttendParams& p, const Walk& first, bool work, uint32_t bar0, const AttCtl& ac, int kv_issued,
+                                            int q_issued) {
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (tid == 0) report_abort(ac.abort, p.status);
+  if (warp >= 10 && lane == 0) {
+    for (int s = max(q_issued - R::NQ, 0); s < q_issued; ++s) mbar_drain(bar0 + 8u * (R::B_Q + s % R::NQ), (s / R::NQ) & 1);
+    for (int T = max(kv_issued - R::RINGS * (warp == 10 ? R::DK : R::DV), 0); T < kv_issued; ++T)
+      mbar_drain(bar0 + 8u * (R::B_KV + (warp == 10 ? R::k_stage(T) : R::v_stage(T))), (warp == 10 ? R::k_turn(T) : R::v_turn(T)) & 1);
   }
-  const uint32_t tmem = *s_tmem;
-  const Ctl ctl{s_abort};
+  Walk w = first;
+  bool more = work;
+  while (more) {
+    if (w.begins() && w.ends()) {
+      const RowMap rows(p, w.item);
+      const int pieces = p.c.cols / 8;
+      for (int i = tid; i < p.gt * p.tt * pieces; i += ATT_THREADS) {
+        int h, t;
+        if (!rows.row(p, i / pieces, h, t)) continue;
+        *reinterpret_cast<uint4*>(p.o + w.b * p.o_sb + h * p.o_sh + t * p.o_ss + 16 * (i % pieces)) =
+            make_uint4(0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu);
+        if (p.stats && i % pieces == 0) {
+          float* at = p.stats + (static_cast<long long>(w.b) * p.H + h) * 2 * p.T + t;
+          at[0] = at[p.T] = __int_as_float(0x7fc00000);
+        }
+      }
+    }
+    more = w.next(p);
+  }
+}
+
+// What begins in this CTA and ends in another, for the joining kernel: only its last item can. w: the walk at its end.
+__device__ __forceinline__ void note_parts(const AttendParams& p, const Walk& w, bool work, int chunk, int end) {
+  int4 meta = make_int4(0, 0, 0, 0);
+  if (work && w.begins() && !w.ends()) meta = make_int4((end - w.n + w.units - 1) / chunk - static_cast<int>(blockIdx.x) + 1, w.b, w.item, 0);
+  p.part_meta[blockIdx.x] = meta;
+}
+
+// ---- up to 64 rows --------------------------------------------------------------------------------------------------------
+template <int NC, int N>
+struct AttCfg : AttRings<NC, N, 2, false, 2 * (N <= 32 ? 2 : 1) * 128 * N * 2 + 1024 + 16 * N * 4 + 8 * N * 4 + 24 * N * 4> {
+  static constexpr int NP = N <= 32 ? 2 : 1;  // buffers for P per stream (each with barriers of its own: a stream may be a buffer ahead)
+  static constexpr int P_BYTES = 128 * N * 2;
+  static constexpr int TMEM = N == 64 ? 512 : (N == 32 ? 256 : 128);  // 6 N columns: S 2 x 2, O 2
+};
+
+template <int NC, int N, bool BF16>
+__global__ void __launch_bounds__(ATT_THREADS, 1)
+kfa_cache_attend_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
+                        const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmKn,
+                        const __grid_constant__ CUtensorMap tmVn, const AttendParams p) {
+  using R = AttCfg<NC, N>;
+  constexpr int NP = R::NP;
+
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  uint8_t* smem = smem_raw + (base - smem_u32(smem_raw));
+  const uint32_t sKV = base, sQ = sKV + R::NS * R::STAGE, sP = sQ + R::NQ * R::Q_BYTES;
+  uint8_t* small = smem + R::NS * R::STAGE + R::NQ * R::Q_BYTES + 2 * NP * R::P_BYTES;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(small);
+  float* s_max = reinterpret_cast<float*>(small + 1024);  // [stream][tile & 1][warp][N]
+  float* s_shift = s_max + 16 * N;                        // [warp][N]
+  float* s_fin = s_shift + 8 * N;                         // [segment & 1][stream]: l of four warps, m, largest score, each [N]
+  const AttCtl ac(bars + R::N_BARS);
+  const uint32_t bar0 = smem_u32(bars);
+  auto bar = [&](int i) { return bar0 + 8u * i; };
+  const int tid = threadIdx.x, warp = warp_index(), lane = tid & 31;
+  Walk first;
+  int chunk, end;
+  const bool work = att_setup<R>(p, bar0, ac, R::TMEM, first, chunk, end);
+  const uint32_t tmem = *ac.tmem;
+  const Ctl ctl{ac.abort};
   const uint32_t tmS = tmem, tmO = tmem + 4 * N;
-  int kv_issued = 0, q_issued = 0;  // producers: ring slots filled, segments' queries
+  int kv_issued = 0, q_issued = 0;
 
   if (!work) {
-    if (tid == 0 && !p.whole) p.part_meta[blockIdx.x] = make_int4(0, 0, 0, 0);
+    if (tid == 0 && !p.whole) note_parts(p, first, false, 1, 0);
   } else if (warp >= 10) {
-    // =========================== TMA producers ===========================
     if constexpr (N == 64) reg_budget<ATT_REGS_ISSUE, ATT_REGS>();
     const bool values = warp == 11;
-    const CUtensorMap *map = values ? &tmV : &tmK, *map_new = values ? &tmVn : &tmKn;
-    Walk w = first;
-    const int per_unit = ATT_UNIT / p.box, boxes = 4 * per_unit;
-    bool ok = true, more = true;
-    int T = 0, s = 0;  // tiles and segments so far
-    while (more && ok) {
-      const RowMap rows(p, w.item);
-      const int g = static_cast<int>(p.by_row_tiles.div(w.item));
-      if (lane == 0 && w.unit == 0 && !length_ok(p.c, w.b)) *s_bad = 1;
-      if (!values) {
-        if (s >= NQ) {
-          ok = mbar_wait_warp(bar(B_OFREE), ((s - NQ) & 1), ctl, 70) && mbar_wait_warp(bar(B_OFREE + 1), ((s - NQ) & 1), ctl, 71);
-          if (!ok) break;
-        }
-        if (lane == 0) {
-          mbar_expect_tx(bar(B_Q + s % NQ), NC * p.gt * p.tt * 128);
-          for (int ch = 0; ch < NC; ++ch)
-            tma_load_4d(sQ + (s % NQ) * Cfg::Q_BYTES + ch * NR * 128, &tmQ, bar(B_Q + s % NQ), ch * 64, rows.h0, rows.t0, w.b);
-        }
-        q_issued = s + 1;
-      }
-      const int tiles = w.tiles();
-      for (int t = 0; t < tiles && ok; ++t, ++T) {
-        // this lane's box
-        const int in_unit = (lane % per_unit) * p.box, unit = w.unit + 4 * t + lane / per_unit;
-        const bool mine = lane < boxes && unit < w.unit + w.n;
-        const int row = (lane / per_unit) * ATT_UNIT + in_unit;
-        int c1 = 0, c3 = w.b, kind = 0;  // 1: cached rows, 2: new ones
-        if (mine && unit < w.uc) {
-          const int pos = unit * ATT_UNIT + in_unit;
-          if (pos < w.len) {
-            if (cache_place(p.c, w.b, pos, c3, c1)) kind = 1;
-            else *s_bad = 1;
-          }
-        } else if (mine && in_unit == 0) {
-          c1 = (unit - w.uc) * ATT_UNIT;
-          if (c1 < w.count && w.ud > 0) kind = 2;
-        }
-        const unsigned cached = __ballot_sync(0xffffffffu, kind == 1), fresh = __ballot_sync(0xffffffffu, kind == 2);
-        const int stage = values ? Cfg::v_stage(T) : Cfg::k_stage(T), turn = values ? Cfg::v_turn(T) : Cfg::k_turn(T);
-        if (turn > 0) {
-          ok = mbar_wait_warp(bar(B_KVFREE + stage), (turn - 1) & 1, ctl, 72);
-          if (!ok) break;
-        }
-        if (lane == 0) mbar_expect_tx(bar(B_KV + stage), NC * 128 * (__popc(cached) * p.box + __popc(fresh) * ATT_UNIT));
-        __syncwarp();
-        if (kind != 0) {
-          const uint32_t dst = sKV + stage * Cfg::STAGE + row * 128;
-          for (int ch = 0; ch < NC; ++ch)
-            tma_load_4d(dst + ch * Cfg::CHUNK, kind == 1 ? map : map_new, bar(B_KV + stage), ch * 64, c1, g, c3);
-        }
-        kv_issued = T + 1;
-      }
-      if (ok) {
-        ++s;
-        more = w.next(p);
-      }
-    }
+    att_produce<R>(p, first, values, sKV, sQ, bar0, ac, &tmQ, values ? &tmV : &tmK, values ? &tmVn : &tmKn, kv_issued, q_issued);
   } else if (warp >= 8) {
-    // =========================== MMA issue ===========================
     if constexpr (N == 64) reg_budget<ATT_REGS_ISSUE, ATT_REGS>();
     const int st = warp - 8;
     const bool lead = elect_one();
     constexpr uint32_t IDESC_S = make_idesc(BF16, false, 128, N), IDESC_O = make_idesc(BF16, true, 128, N) | (1u << 15);
     constexpr uint32_t HI_P = sdesc_hi_for(N);
     const int k_steps = (p.c.cols + 15) / 16;
-    bool ok = true;
-    struct Tile {
-      int T, s;
-      bool opens;  // the stream's first tile of the segment
-    };
-    Walk w = first;
-    int at = 0, T_next = 0, s_next = 0;  // inside the segment; over all
-    bool more = true, opens = true;
-    auto take = [&](Tile& t) {  // the stream's next tile
-      while (more) {
-        while (at < w.tiles()) {
-          ++at;
-          const int T = T_next++;
-          if (BY_ROWS || (T & 1) == st) {
-            t = {T, s_next, opens};
-            opens = false;
-            return true;
-          }
-        }
-        at = 0;
-        ++s_next;
-        opens = true;
-        more = w.next(p);
-      }
-      return false;
-    };
-    auto issue_S = [&](const Tile& t, int c) {
-      const int stage = Cfg::k_stage(t.T);
-      ok = mbar_wait_warp(bar(B_KV + stage), Cfg::k_turn(t.T) & 1, ctl, 73);
-      if (ok && t.opens) ok = mbar_wait_warp(bar(B_Q + t.s % NQ), (t.s / NQ) & 1, ctl, 74);
-      if (!ok) return;
-      tc_fence_after();
-      const uint32_t k_lo = sdesc_lo(sKV + stage * Cfg::STAGE, 16);
-      const uint32_t q_lo = sdesc_lo(sQ + (t.s % NQ) * Cfg::Q_BYTES + (BY_ROWS ? st * 64 * 128 : 0), 16);
-      for (int kk = 0; kk < k_steps; ++kk)
-        umma_ss_lead2(lead, tmS + (2 * st + (c & 1)) * N, k_lo + (((kk >> 2) * Cfg::CHUNK + (kk & 3) * 32) >> 4), SDESC_HI,
-                      q_lo + (((kk >> 2) * (NR * 128) + (kk & 3) * 32) >> 4), SDESC_HI, IDESC_S, kk > 0 ? 1u : 0u);
-      umma_commit_lead(lead, bar(B_S + 2 * st + (c & 1)));
-      umma_commit_lead(lead, bar(B_KVFREE + stage));
-    };
-    auto issue_PV = [&](const Tile& t, int c) {
-      const int stage = Cfg::v_stage(t.T);
-      ok = mbar_wait_warp(bar(B_KV + stage), Cfg::v_turn(t.T) & 1, ctl, 75) && mbar_wait_warp(bar(B_P + 2 * st + c % NP), (c / NP) & 1, ctl, 76);
-      if (ok && t.opens && t.s > 0) ok = mbar_wait_warp(bar(B_OFREE + st), (t.s - 1) & 1, ctl, 77);
-      if (!ok) return;
-      tc_fence_after();
-      const uint32_t v_lo = sdesc_lo(sKV + stage * Cfg::STAGE, NC == 2 ? Cfg::CHUNK : 0);
-      const uint32_t p_lo = sdesc_lo(sP + (st * NP + c % NP) * Cfg::P_BYTES, 16);
+    att_issue<R, 1, NP>(
+        p, first, st, bar0, ac,
+        [&](const AttTile& t, int c, int) {
+          const uint32_t k_lo = sdesc_lo(sKV + R::k_stage(t.T) * R::STAGE, 16), q_lo = sdesc_lo(sQ + (t.s % R::NQ) * R::Q_BYTES, 16);
+          for (int kk = 0; kk < k_steps; ++kk)
+            umma_ss_lead2(lead, tmS + (2 * st + (c & 1)) * N, k_lo + (((kk >> 2) * R::CHUNK + (kk & 3) * 32) >> 4), SDESC_HI,
+                          q_lo + (((kk >> 2) * R::Q_CHUNK + (kk & 3) * 32) >> 4), SDESC_HI, IDESC_S, kk > 0 ? 1u : 0u);
+          umma_commit_lead(lead, bar(R::B_S + 2 * st + (c & 1)));
+          umma_commit_lead(lead, bar(R::B_KVFREE + R::k_stage(t.T)));
+        },
+        [&](const AttTile& t, int c, int) {
+          // (64 columns or fewer: the matrix' rows 64 .. 127 repeat the first ones, and nobody reads them)
+          const uint32_t v_lo = sdesc_lo(sKV + R::v_stage(t.T) * R::STAGE, NC == 2 ? R::CHUNK : 0);
+          const uint32_t p_lo = sdesc_lo(sP + (st * NP + c % NP) * R::P_BYTES, 16);
 #pragma unroll
-      for (int kk = 0; kk < 8; ++kk)
-        umma_ss_lead2(lead, tmO + st * N, v_lo + ((kk * 16 * 128) >> 4), SDESC_HI, p_lo + ((kk * 16 * 2 * N) >> 4), HI_P, IDESC_O,
-                      (!t.opens || kk > 0) ? 1u : 0u);
-      umma_commit_lead(lead, bar(B_PV + 2 * st + c % NP));
-      umma_commit_lead(lead, bar(B_KVFREE + stage));
-    };
-    Tile now, then;
-    int c = 0;
-    bool have = take(now);
-    if (have) issue_S(now, 0);
-    while (have && ok) {
-      const bool again = take(then);
-      // (A segment's queries are only loaded once the segment NQ before it is finished, for which this tile's values may be needed.)
-      const bool ahead = again && then.s - now.s < NQ;
-      if (ahead) issue_S(then, c + 1);
-      if (ok) issue_PV(now, c);
-      if (ok && again && !ahead) issue_S(then, c + 1);
-      now = then;
-      have = again;
-      ++c;
-    }
-    umma_commit_lead(lead, bar(B_DRAIN + st));  // what was issued has retired before tensor memory is freed
-    mbar_drain(bar(B_DRAIN + st), 0);
+          for (int kk = 0; kk < 8; ++kk)
+            umma_ss_lead2(lead, tmO + st * N, v_lo + ((kk * 16 * 128) >> 4), SDESC_HI, p_lo + ((kk * 16 * 2 * N) >> 4), HI_P, IDESC_O,
+                          (!t.opens || kk > 0) ? 1u : 0u);
+          umma_commit_lead(lead, bar(R::B_PV + 2 * st + c % NP));
+          umma_commit_lead(lead, bar(R::B_KVFREE + R::v_stage(t.T)));
+        });
   } else {
     // =========================== softmax, output ===========================
     // (After a wait that ran out the role goes on without waiting: the warps of a stream meet at barriers.)
@@ -520,39 +719,48 @@ kfa_cache_attend_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
       const int tiles = w.tiles();
       for (int t = 0; t < tiles; ++t) {
         const int T = T0 + t;
-        if (!BY_ROWS && (T & 1) != st) continue;
+        if ((T & 1) != st) continue;
         const int ub = w.unit + 4 * t;
         const bool full = 4 * t + 4 <= w.n && (ub + 4) * ATT_UNIT <= w.len && ub + 4 <= w.uc;
-        if (ok) ok = mbar_wait_warp(bar(B_S + 2 * st + (c & 1)), (c >> 1) & 1, ctl, 78);
+        int fresh = -1;
+        const bool valid = full || which_key(w, ub, key, fresh);
+        if (ok) ok = mbar_wait_warp(bar(R::B_S + 2 * st + (c & 1)), (c >> 1) & 1, ctl, 78);
         tc_fence_after();
         float x[N];
         tmem_ld_cols<N>(tmS + lane_base + (2 * st + (c & 1)) * N, x);
         tmem_wait_ld();
-        int fresh = -1;  // the new token that this key is
-        bool valid = true;
         if (!full) {
-          const int unit = ub + (key >> 5);
-          if (unit >= w.unit + w.n) valid = false;
-          else if (unit < w.uc) valid = unit * ATT_UNIT + (key & 31) < w.len;
-          else {
-            fresh = (unit - w.uc) * ATT_UNIT + (key & 31);
-            valid = w.ud > 0 && fresh < w.count;
-            if (!valid) fresh = -1;
-          }
-          const uint8_t* tree = p.tree ? p.tree + w.b * p.tree_sb + static_cast<long long>(max(fresh, 0)) * p.tree_sj : nullptr;
-          const int r0 = BY_ROWS ? st * 64 : 0;
-          bool sees = true;
-          int t_last = -1;
+          if (!valid) {
 #pragma unroll
-          for (int i = 0; i < N; ++i) {
-            if (fresh >= 0) {
-              const int row_t = rows.t0 + static_cast<int>(p.by_gt.div(r0 + i));
-              if (row_t != t_last) {
-                t_last = row_t;
-                sees = row_t < w.count && (tree ? tree[row_t * p.tree_st] != 0 : fresh <= row_t);
+            for (int i = 0; i < N; ++i) x[i] = -INFINITY;
+          } else if (fresh >= 0 && (p.T > 1 || p.tree != nullptr || w.count == 0)) {
+            // a bit per token of the row tile: which of them see this new token (N rows hold at most N tokens)
+            uint32_t see[PER];
+#pragma unroll
+            for (int i = 0; i < PER; ++i) see[i] = 0u;
+            const int most = min(p.tt, p.T - rows.t0);
+            if (p.tree == nullptr) {
+              for (int i = 0; i < most; ++i)
+                if (rows.t0 + i >= fresh && rows.t0 + i < w.count) see[i / 32] |= 1u << (i & 31);
+            } else {
+              const uint8_t* tree = p.tree + w.b * p.tree_sb + rows.t0 * p.tree_st + fresh * p.tree_sj;
+#pragma unroll
+              for (int k = 0; k < PER; ++k)
+#pragma unroll 8
+                for (int i = 0; i < 32; ++i)
+                  if (32 * k + i < most && tree[(32 * k + i) * p.tree_st] != 0) see[k] |= 1u << i;
+#pragma unroll
+              for (int k = 0; k < PER; ++k) {  // tokens that the sequence does not have see nothing
+                const int left = w.count - rows.t0 - 32 * k;
+                see[k] = left <= 0 ? 0u : (left >= 32 ? see[k] : see[k] & ((1u << left) - 1u));
               }
             }
-            if (!valid || !sees) x[i] = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+              const int dt = static_cast<int>(p.by_gt.div(i));
+              const uint32_t word = PER == 1 || dt < 32 ? see[0] : see[PER - 1];
+              if (!((word >> (dt & 31)) & 1u)) x[i] = -INFINITY;
+            }
           }
         }
         // ---- column maxima ----
@@ -588,7 +796,7 @@ kfa_cache_attend_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
         __syncwarp();
         if (grew && !opens) {
           // sums and O of the earlier tiles, to the new maxima
-          if (ok) ok = mbar_wait_warp(bar(B_PV + 2 * st + (c - 1) % NP), ((c - 1) / NP) & 1, ctl, 79);
+          if (ok) ok = mbar_wait_warp(bar(R::B_PV + 2 * st + (c - 1) % NP), ((c - 1) / NP) & 1, ctl, 79);
           tc_fence_after();
 #pragma unroll
           for (int i = 0; i < N; i += 16) {
@@ -606,8 +814,8 @@ kfa_cache_attend_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
           tmem_wait_st();
         }
         // ---- P ----
-        if (c >= NP && ok) ok = mbar_wait_warp(bar(B_PV + 2 * st + c % NP), (c / NP - 1) & 1, ctl, 80);  // its buffer has been read
-        const uint32_t sp = sP + (st * NP + c % NP) * Cfg::P_BYTES;
+        if (c >= NP && ok) ok = mbar_wait_warp(bar(R::B_PV + 2 * st + c % NP), (c / NP - 1) & 1, ctl, 80);  // its buffer has been read
+        const uint32_t sp = sP + (st * NP + c % NP) * R::P_BYTES;
 #pragma unroll
         for (int i = 0; i < N; i += 8) {
           const float4 a = *reinterpret_cast<const float4*>(shift + i), b = *reinterpret_cast<const float4*>(shift + i + 4);
@@ -623,47 +831,19 @@ kfa_cache_attend_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
                        : "memory");
         }
         if (!full) {
-          // Values behind the end may be anything, and 0 * NaN is no 0: their rows become zeros. So do a new token's values that
-          // are not finite, which would otherwise reach rows that do not see it; the epilogue hands them to those that do.
           // (The tile before has to be done with: until then the barrier of this one's stage may be a turn behind.)
-          const int stage = Cfg::v_stage(T);
-          if (c > 0 && ok) ok = mbar_wait_warp(bar(B_PV + 2 * st + (c - 1) % NP), ((c - 1) / NP) & 1, ctl, 81);
-          if (ok) ok = mbar_wait_warp(bar(B_KV + stage), Cfg::v_turn(T) & 1, ctl, 83);
-          const uint32_t row = sKV + stage * Cfg::STAGE + key * 128;
-          if (!valid) {
-#pragma unroll
-            for (int i = 0; i < NC * 8; ++i)
-              asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(row + (i >> 3) * Cfg::CHUNK + (i & 7) * 16), "r"(0) : "memory");
-          } else if (fresh >= 0) {
-            const uint8_t* g_row = p.v + w.b * p.v_sb + static_cast<long long>(p.by_row_tiles.div(w.item)) * p.v_sh + fresh * p.v_ss;
-            for (int i = 0; i < p.c.cols / 8; ++i) {
-              const uint4 q4 = *reinterpret_cast<const uint4*>(g_row + 16 * i);
-              uint32_t q[4] = {q4.x, q4.y, q4.z, q4.w};
-              bool odd = false;
-#pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                constexpr uint32_t E = BF16 ? 0x7f80u : 0x7c00u;  // all exponent bits: infinity or NaN
-                if ((q[j] & E) == E) q[j] &= 0xffff0000u, odd = true;
-                if ((q[j] >> 16 & E) == E) q[j] &= 0xffffu, odd = true;
-              }
-              if (odd) {
-                s_odd[st] = s + 1;
-                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(row + (i >> 3) * Cfg::CHUNK + (((i & 7) ^ (key & 7)) << 4)),
-                             "r"(q[0]), "r"(q[1]), "r"(q[2]), "r"(q[3])
-                             : "memory");
-              }
-            }
-          }
+          if (c > 0 && ok) ok = mbar_wait_warp(bar(R::B_PV + 2 * st + (c - 1) % NP), ((c - 1) / NP) & 1, ctl, 81);
+          if (ok) ok = mbar_wait_warp(bar(R::B_KV + R::v_stage(T)), R::v_turn(T) & 1, ctl, 82);
+          if (clean_values<NC, BF16>(p, w, rows.g, sKV + R::v_stage(T) * R::STAGE, key, valid, fresh)) ac.odd[st] = s + 1;
         }
         fence_async_smem();
         tc_fence_before();
-        mbar_arrive(bar(B_P + 2 * st + c % NP));
+        mbar_arrive(bar(R::B_P + 2 * st + c % NP));
         opens = false;
         ++c;
       }
       T0 += tiles;
       // ---- the segment's end ----
-      if (!opens && ok) ok = mbar_wait_warp(bar(B_PV + 2 * st + (c - 1) % NP), ((c - 1) / NP) & 1, ctl, 82);
       columns_over_lanes<N>(l, lane);
       float* fin = s_fin + ((s & 1) * 2 + st) * 6 * N;
       if constexpr (N == 64) {
@@ -682,150 +862,378 @@ kfa_cache_attend_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
             fin[5 * N + lane + 32 * i] = m_top[i];
           }
       }
+      if (!opens && ok) ok = mbar_wait_warp(bar(R::B_PV + 2 * st + (c - 1) % NP), ((c - 1) / NP) & 1, ctl, 83);
       tc_fence_before();
-      if constexpr (BY_ROWS) {
-        if (st == 0) named_sync<1, 128>();
-        else named_sync<2, 128>();
-      } else {
-        named_sync<3, 256>();
-      }
+      named_sync<3, 256>();
       tc_fence_after();
-      const bool bad = *s_bad != 0;
+      const bool bad = *ac.bad != 0;
       const bool whole = w.begins() && w.ends();
       const long long slot = 2ll * blockIdx.x + (w.begins() ? 1 : 0);
       // new tokens of the segment, where some of their values were left out (a stream may be one segment ahead: >=)
-      const bool odd = s_odd[st] >= s + 1 || (!BY_ROWS && s_odd[1 - st] >= s + 1);
+      const bool odd = ac.odd[0] >= s + 1 || ac.odd[1] >= s + 1;
       const int j0 = max(w.unit - w.uc, 0) * ATT_UNIT, j1 = odd ? min((w.unit + w.n - w.uc) * ATT_UNIT, w.count) : 0;
       const int d = wl * 32 + lane;
-      constexpr int W = BY_ROWS ? 32 : N / 2;  // columns a thread writes at a time
-      for (int part = 0; part < (BY_ROWS ? 2 : 1); ++part) {
-        const int c0 = BY_ROWS ? 32 * part : st * W;  // in the stream's columns
-        const int r0 = BY_ROWS ? 64 * st + c0 : c0;   // in the tile's rows
-        // lane i (i < W): column i's factors and statistics
-        const int col = c0 + (lane & (W - 1));
-        const float* f0 = s_fin + ((s & 1) * 2 + (BY_ROWS ? st : 0)) * 6 * N + col;
-        float l0 = f0[0] + f0[N] + f0[2 * N] + f0[3 * N], m0 = f0[4 * N], top0 = f0[5 * N];
-        float a0 = 1.f, a1 = 0.f;
-        if constexpr (!BY_ROWS) {
-          const float* f1 = f0 + 6 * N;
-          const float l1 = f1[0] + f1[N] + f1[2 * N] + f1[3 * N], m1 = f1[4 * N];
-          const float mm = fmaxf(m0, m1);
-          a0 = part_factor(m0, l0, mm, c_log2);
-          a1 = part_factor(m1, l1, mm, c_log2);
-          l0 = l0 * a0 + l1 * a1;
-          m0 = mm;
-          top0 = fmaxf(top0, f1[5 * N]);
-        } else if (m0 == -INFINITY) {
-          a0 = part_factor(m0, l0, m0, c_log2);
+      constexpr int W = N / 2;  // columns of a thread
+      const int c0 = st * W;
+      // lane i (i < W): column i's factors and statistics
+      const float* f0 = s_fin + (s & 1) * 12 * N + c0 + (lane & (W - 1));
+      const float* f1 = f0 + 6 * N;
+      const float m0 = f0[4 * N], m1 = f1[4 * N], m = fmaxf(m0, m1), top = fmaxf(f0[5 * N], f1[5 * N]);
+      const float l0 = (f0[0] + f0[N]) + (f0[2 * N] + f0[3 * N]), l1 = (f1[0] + f1[N]) + (f1[2 * N] + f1[3 * N]);
+      float a0 = part_factor(m0, l0, m, c_log2), a1 = part_factor(m1, l1, m, c_log2);
+      const float l_all = l0 * a0 + l1 * a1;
+      int h, tk;
+      const bool exists = rows.row(p, c0 + (lane & (W - 1)), h, tk);
+      const long long off = exists ? w.b * p.o_sb + h * p.o_sh + tk * p.o_ss : -1;
+      const bool some = exists && tk < w.count && l_all != 0.f;
+      const float nan = __int_as_float(0x7fc00000);
+      if (whole) {
+        const float inv = some ? 1.f / l_all : 0.f;
+        if (p.stats && wl == 0 && exists && lane < W) {
+          float* at = p.stats + (static_cast<long long>(w.b) * p.H + h) * 2 * p.T + tk;
+          at[0] = bad ? nan : (some ? top : INFINITY);
+          at[p.T] = bad ? nan : (some ? log2f(l_all) + (m - top) * c_log2 : 0.f);
         }
-        int h, tk;
-        const bool exists = rows.row(p, r0 + (lane & (W - 1)), h, tk);
-        const bool counts = exists && tk < w.count;
-        long long off = exists ? w.b * p.o_sb + h * p.o_sh + tk * p.o_ss : -1;
-        const bool some = counts && l0 != 0.f;
-        const float nan = __int_as_float(0x7fc00000);
-        if (whole) {
-          const float inv = some ? 1.f / l0 : 0.f;
-          if (p.stats && wl == 0 && exists && lane < W) {
-            float* at = p.stats + (static_cast<long long>(w.b) * p.H + h) * 2 * p.T + tk;
-            at[0] = bad ? nan : (some ? top0 : INFINITY);
-            at[p.T] = bad ? nan : (some ? log2f(l0) + (m0 - top0) * c_log2 : 0.f);
-          }
-          a0 = some ? a0 * inv : 0.f;
-          a1 = some ? a1 * inv : 0.f;
-        } else if (wl == 0 && lane < W) {
-          float* at = p.part_ml + slot * 3 * NR + r0 + lane;
-          at[0] = m0;
-          at[NR] = l0;
-          at[2 * NR] = top0;
-        }
-        float o0[W], o1[W];
-        tmem_ld_cols<W>(tmO + lane_base + (BY_ROWS ? st * N : 0) + c0, o0);
-        if constexpr (!BY_ROWS) tmem_ld_cols<W>(tmO + lane_base + N + c0, o1);
-        tmem_wait_ld();
+        a0 = some ? a0 * inv : 0.f;
+        a1 = some ? a1 * inv : 0.f;
+      } else if (wl == 0 && lane < W) {
+        float* at = p.part_ml + slot * 3 * p.rows + c0 + lane;
+        at[0] = m;
+        at[p.rows] = l_all;
+        at[2 * p.rows] = top;
+      }
+      float o0[W], o1[W];
+      tmem_ld_cols<W>(tmO + lane_base + c0, o0);
+      tmem_ld_cols<W>(tmO + lane_base + N + c0, o1);
+      tmem_wait_ld();
 #pragma unroll
-        for (int i = 0; i < W; ++i) {
-          const float x0 = __shfl_sync(0xffffffffu, a0, i), x1 = __shfl_sync(0xffffffffu, a1, i);
-          float y = x0 == 0.f ? 0.f : o0[i] * x0;  // (a stream without tiles has left nothing there)
-          if constexpr (!BY_ROWS) y += x1 == 0.f ? 0.f : o1[i] * x1;
-          o0[i] = y;
-        }
-        if (d < p.c.cols) {
-          for (int j = j0; j < j1; ++j) {
-            const float y = load16<BF16>(p.v + w.b * p.v_sb + static_cast<long long>(p.by_row_tiles.div(w.item)) * p.v_sh + j * p.v_ss + 2 * d);
-            if (fabsf(y) < INFINITY) continue;
+      for (int i = 0; i < W; ++i) {
+        const float x0 = __shfl_sync(0xffffffffu, a0, i), x1 = __shfl_sync(0xffffffffu, a1, i);
+        o0[i] = (x0 == 0.f ? 0.f : o0[i] * x0) + (x1 == 0.f ? 0.f : o1[i] * x1);  // (a stream without tiles has left nothing there)
+      }
+      if (d < p.c.cols) {
+        for (int j = j0; j < j1; ++j) {
+          const float y = load16<BF16>(p.v + w.b * p.v_sb + rows.g * p.v_sh + j * p.v_ss + 2 * d);
+          if (fabsf(y) < INFINITY) continue;
 #pragma unroll
-            for (int i = 0; i < W; ++i) {
-              const int row_t = rows.t0 + static_cast<int>(p.by_gt.div(r0 + i));
-              if (row_t < w.count && (p.tree ? p.tree[w.b * p.tree_sb + row_t * p.tree_st + j * p.tree_sj] != 0 : j <= row_t)) o0[i] += y;
-            }
-          }
+          for (int i = 0; i < W; ++i)
+            if (sees_new(p, w, rows.t0 + static_cast<int>(p.by_gt.div(c0 + i)), j)) o0[i] += y;
         }
+      }
+      if (whole) {
 #pragma unroll
         for (int i = 0; i < W; ++i) {
           const long long at = __shfl_sync(0xffffffffu, off, i);
-          if (whole) {
-            if (at >= 0 && d < p.c.cols) {
-              const uint32_t y = pack16<BF16>(bad ? nan : o0[i], 0.f);
-              *reinterpret_cast<uint16_t*>(p.o + at + 2 * d) = static_cast<uint16_t>(y);
-            }
-          } else {
-            p.part_o[(slot * NR + r0 + i) * 128 + d] = o0[i];
+          if (at >= 0 && d < p.c.cols) {
+            const uint32_t y = pack16<BF16>(bad ? nan : o0[i], 0.f);
+            *reinterpret_cast<uint16_t*>(p.o + at + 2 * d) = static_cast<uint16_t>(y);
           }
         }
+      } else {
+#pragma unroll
+        for (int i = 0; i < W; ++i)
+          if (c0 + i < p.gt * p.tt) p.part_o[(slot * p.rows + c0 + i) * 128 + d] = o0[i];
       }
       tc_fence_before();
-      mbar_arrive(bar(B_OFREE + st));
-      if constexpr (!BY_ROWS) mbar_arrive(bar(B_OFREE + 1 - st));
+      mbar_arrive(bar(R::B_OFREE + st));
+      mbar_arrive(bar(R::B_OFREE + 1 - st));
       ++s;
       more = w.next(p);
     }
-    if (tid == 0 && !p.whole) {  // only the last item can begin here and end in another CTA
-      int4 meta = make_int4(0, 0, 0, 0);
-      if (w.begins() && !w.ends()) meta = make_int4(static_cast<int>((u1 - w.n + w.units - 1) / chunk - blockIdx.x) + 1, w.b, w.item, 0);
-      p.part_meta[blockIdx.x] = meta;
-    }
+    if (tid == 0 && !p.whole) note_parts(p, w, true, chunk, end);
   }
 
   // ---- teardown (every thread gets here, also after an abort) ----
   tc_fence_before();
   __syncthreads();
-  if (tid == 0 && *s_bad) report(p.status, DEV_BAD_CACHE);
-  if (*s_abort) {
-    if (tid == 0) report_abort(s_abort, p.status);
-    if (warp >= 10 && lane == 0) {  // the copies it has started land before the CTA leaves its shared memory
-      for (int s = max(q_issued - NQ, 0); s < q_issued; ++s) mbar_drain(bar(B_Q + s % NQ), (s / NQ) & 1);
-      for (int T = max(kv_issued - Cfg::RINGS * (warp == 10 ? Cfg::DK : Cfg::DV), 0); T < kv_issued; ++T)
-        mbar_drain(bar(B_KV + (warp == 10 ? Cfg::k_stage(T) : Cfg::v_stage(T))), (warp == 10 ? Cfg::k_turn(T) : Cfg::v_turn(T)) & 1);
-    }
-    Walk w = first;
-    bool more = work;
-    while (more) {  // the rows of what it had whole read as NaN; what was cut, the joining kernel sees to
-      if (w.begins() && w.ends()) {
-        const RowMap rows(p, w.item);
-        for (int i = tid; i < NR * (p.c.cols / 8); i += ATT_THREADS) {
-          int h, t;
-          if (!rows.row(p, i / (p.c.cols / 8), h, t)) continue;
-          const uint4 nan8 = make_uint4(0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu);
-          *reinterpret_cast<uint4*>(p.o + w.b * p.o_sb + h * p.o_sh + t * p.o_ss + 16 * (i % (p.c.cols / 8))) = nan8;
-          if (p.stats && i % (p.c.cols / 8) == 0) {
-            float* at = p.stats + (static_cast<long long>(w.b) * p.H + h) * 2 * p.T + t;
-            at[0] = at[p.T] = __int_as_float(0x7fc00000);
-          }
-        }
-      }
-      more = w.next(p);
-    }
-  }
+  if (tid == 0 && *ac.bad) report(p.status, DEV_BAD_CACHE);
+  if (*ac.abort) att_give_up<R>(p, first, work, bar0, ac, kv_issued, q_issued);
   if (warp == 8) {
     tc_fence_after();
-    tmem_dealloc(tmem, Cfg::TMEM);
+    tmem_dealloc(tmem, R::TMEM);
+  }
+}
+
+// ---- more rows ------------------------------------------------------------------------------------------------------------
+// HALVES: 1: up to 128 rows, tiles to the streams in turn; 2: up to 256 rows, a half of them to each stream.
+template <int NC, int HALVES>
+struct AttRowsCfg : AttRings<NC, 128 * HALVES, HALVES == 1 ? 2 : 1, HALVES == 2, 1024 + 2 * 2 * 128 * 3 * 4> {
+  static constexpr int TMEM = 512;  // S 2 x 128; O 2 x 128
+};
+
+// A tile's 128 score columns are made and used as two halves of 64 keys, each with its own barriers: P (16-bit) lies over the first 32
+// of its half's columns, and while one half's values are multiplied and its next scores made, the thread works on the other.
+template <int NC, int HALVES, bool BF16>
+__global__ void __launch_bounds__(ATT_THREADS, 1)
+kfa_cache_attend_rows_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
+                             const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmKn,
+                             const __grid_constant__ CUtensorMap tmVn, const AttendParams p) {
+  using R = AttRowsCfg<NC, HALVES>;
+  constexpr bool BOTH = R::BOTH;
+  constexpr int D = 64 * NC;  // columns of O (those that the head dim does not have are zeros)
+
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  uint8_t* smem = smem_raw + (base - smem_u32(smem_raw));
+  const uint32_t sKV = base, sQ = sKV + R::NS * R::STAGE;
+  uint8_t* small = smem + R::NS * R::STAGE + R::NQ * R::Q_BYTES;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(small);
+  float* s_fin = reinterpret_cast<float*>(small + 1024);  // [segment & 1][stream][m, l, largest score][128 rows]
+  const AttCtl ac(bars + R::N_BARS);
+  const uint32_t bar0 = smem_u32(bars);
+  auto bar = [&](int i) { return bar0 + 8u * i; };
+  const int tid = threadIdx.x, warp = warp_index();
+  Walk first;
+  int chunk, end;
+  const bool work = att_setup<R>(p, bar0, ac, R::TMEM, first, chunk, end);
+  const uint32_t tmem = *ac.tmem;
+  const Ctl ctl{ac.abort};
+  int kv_issued = 0, q_issued = 0;
+
+  if (!work) {
+    if (tid == 0 && !p.whole) note_parts(p, first, false, 1, 0);
+  } else if (warp >= 10) {
+    reg_budget<ATT_REGS_ISSUE, ATT_REGS>();
+    const bool values = warp == 11;
+    att_produce<R>(p, first, values, sKV, sQ, bar0, ac, &tmQ, values ? &tmV : &tmK, values ? &tmVn : &tmKn, kv_issued, q_issued);
+  } else if (warp >= 8) {
+    reg_budget<ATT_REGS_ISSUE, ATT_REGS>();
+    const int st = warp - 8;
+    const bool lead = elect_one();
+    constexpr uint32_t IDESC_S = make_idesc(BF16, false, 128, 64), IDESC_O = make_idesc(BF16, true, 128, D);
+    const uint32_t tS = tmem + 128 * st, tO = tmem + 256 + 128 * st;
+    const int k_steps = (p.c.cols + 15) / 16;
+    att_issue<R, 2, 1>(
+        p, first, st, bar0, ac,
+        [&](const AttTile& t, int, int half) {
+          const uint32_t q_lo = sdesc_lo(sQ + (t.s % R::NQ) * R::Q_BYTES + (BOTH ? st * 128 * 128 : 0), 16);
+          const uint32_t k_lo = sdesc_lo(sKV + R::k_stage(t.T) * R::STAGE + half * 64 * 128, 16);
+          for (int kk = 0; kk < k_steps; ++kk)
+            umma_ss_lead(lead, tS + 64 * half, q_lo + (((kk >> 2) * R::Q_CHUNK + (kk & 3) * 32) >> 4),
+                         k_lo + (((kk >> 2) * R::CHUNK + (kk & 3) * 32) >> 4), IDESC_S, kk > 0 ? 1u : 0u);
+          umma_commit_lead(lead, bar(R::B_S + 2 * st + half));
+          if (half == 1) umma_commit_lead(lead, bar(R::B_KVFREE + R::k_stage(t.T)));
+        },
+        [&](const AttTile& t, int, int half) {
+          const uint32_t v_lo = sdesc_lo(sKV + R::v_stage(t.T) * R::STAGE + half * 64 * 128, R::CHUNK);
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk)
+            umma_ts_lead(lead, tO, tS + 64 * half + kk * 8, v_lo + ((kk * 16 * 128) >> 4), IDESC_O, (!t.opens || half > 0 || kk > 0) ? 1u : 0u);
+          umma_commit_lead(lead, bar(R::B_PV + 2 * st + half));
+          if (half == 1) umma_commit_lead(lead, bar(R::B_KVFREE + R::v_stage(t.T)));
+        });
+  } else {
+    // =========================== softmax, output ===========================
+    // (After a wait that ran out the role goes on without waiting: the streams meet at barriers.)
+    reg_budget<ATT_REGS_STREAM, ATT_REGS>();
+    const int st = warp >> 2, wl = warp & 3, r_in = tid & 127;
+    const uint32_t lane_base = static_cast<uint32_t>(wl * 32) << 16;
+    const uint32_t tS = tmem + 128 * st + lane_base, tO = tmem + 256 + 128 * st + lane_base;
+    const float c_log2 = p.c_log2;
+    const float2 c2 = make_float2(c_log2, c_log2);
+    const int r = (BOTH ? 128 * st : 0) + r_in;  // the thread's row of the tile
+    Walk w = first;
+    bool more = true, ok = true;
+    int c = 0, T0 = 0, s = 0;  // the stream's tiles; tiles and segments before
+    while (more) {
+      const RowMap rows(p, w.item);
+      int h, tk;
+      const bool exists = rows.row(p, r, h, tk);
+      float l = 0.f, m_ref = -INFINITY, m_top = -INFINITY;
+      bool opens = true;
+      const int tiles = w.tiles();
+      for (int t = 0; t < tiles; ++t) {
+        const int T = T0 + t;
+        if (!BOTH && (T & 1) != st) continue;
+        const int ub = w.unit + 4 * t;
+        const bool full = 4 * t + 4 <= w.n && (ub + 4) * ATT_UNIT <= w.len && ub + 4 <= w.uc;
+#pragma unroll 1
+        for (int half = 0; half < 2; ++half) {
+          uint32_t seen[2] = {0xffffffffu, 0xffffffffu};
+          if (!full) {
+            seen[0] = exists ? seen_word(p, w, ub + 2 * half, tk) : 0u;
+            seen[1] = exists ? seen_word(p, w, ub + 2 * half + 1, tk) : 0u;
+          }
+          if (ok) ok = mbar_wait_warp(bar(R::B_S + 2 * st + half), c & 1, ctl, 78);
+          tc_fence_after();
+          float2 x[32];
+          tmem_ld_cols<64>(tS + 64 * half, reinterpret_cast<float*>(x));
+          tmem_wait_ld();
+          if (!full) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+              if (!((seen[i / 16] >> (2 * i & 31)) & 1u)) x[i].x = -INFINITY;
+              if (!((seen[i / 16] >> ((2 * i + 1) & 31)) & 1u)) x[i].y = -INFINITY;
+            }
+          }
+          float y[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int i = 0; i < 32; ++i) y[i & 3] = fmaxf(y[i & 3], fmaxf(x[i].x, x[i].y));
+          const float top = fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3]));
+          m_top = fmaxf(m_top, top);
+          const bool move = m_ref == -INFINITY ? top > -INFINITY : top > m_ref + p.slack;
+          if (__any_sync(0xffffffffu, move)) {
+            const float alpha = !move ? 1.f : (m_ref == -INFINITY ? 0.f : ex2((m_ref - top) * c_log2));
+            if (!opens || half > 0) {  // every product issued so far has to have retired; it is the last but one of this half's
+              const int before = 2 * c + half - 1;
+              if (ok) ok = mbar_wait_warp(bar(R::B_PV + 2 * st + (before & 1)), (before >> 1) & 1, ctl, 79);
+              tc_fence_after();
+#pragma unroll
+              for (int i = 0; i < D; i += 32) {
+                float o[32];
+                tmem_ld32(tO + i, reinterpret_cast<uint32_t*>(o));
+                tmem_wait_ld();
+#pragma unroll
+                for (int j = 0; j < 32; ++j) o[j] *= alpha;
+                tmem_st32(tO + i, reinterpret_cast<const uint32_t*>(o));
+              }
+              tmem_wait_st();
+              l *= alpha;
+            }
+            if (move) m_ref = top;
+          }
+          const float sh = m_ref == -INFINITY ? 0.f : -m_ref;
+          const float2 s2 = make_float2(sh, sh);
+          float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+          uint32_t pk[32];
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            float2 e = __fmul2_rn(__fadd2_rn(x[i], s2), c2);
+            e.x = ex2(e.x);
+            e.y = ex2(e.y);
+            sum[i & 1] = __fadd2_rn(sum[i & 1], e);
+            pk[i] = pack16<BF16>(e.x, e.y);
+          }
+          l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+          tmem_st32(tS + 64 * half, pk);
+          tmem_wait_st();
+          if (!full && half == 0) {
+            // (The tile before has to be done with: until then the barrier of this one's stage may be a turn behind.)
+            if (c > 0 && ok) ok = mbar_wait_warp(bar(R::B_PV + 2 * st + 1), (c - 1) & 1, ctl, 81);
+            if (ok) ok = mbar_wait_warp(bar(R::B_KV + R::v_stage(T)), R::v_turn(T) & 1, ctl, 82);
+            int fresh;
+            const bool valid = which_key(w, ub, r_in, fresh);
+            if (clean_values<NC, BF16>(p, w, rows.g, sKV + R::v_stage(T) * R::STAGE, r_in, valid, fresh)) ac.odd[st] = s + 1;
+            fence_async_smem();
+          }
+          tc_fence_before();
+          mbar_arrive(bar(R::B_P + 2 * st + half));
+        }
+        opens = false;
+        ++c;
+      }
+      T0 += tiles;
+      // ---- the segment's end ----
+      if (!opens && ok) ok = mbar_wait_warp(bar(R::B_PV + 2 * st + 1), (c - 1) & 1, ctl, 83);
+      float a0 = 1.f, a1 = 0.f, m = m_ref, top = m_top, l_all = l;  // factors of the streams' O, the row's statistics
+      tc_fence_before();
+      if constexpr (BOTH) {
+        if (st == 0) named_sync<1, 128>();  // (what the stream's threads have met of values that are not finite)
+        else named_sync<2, 128>();
+        a0 = part_factor(m, l, m, c_log2);
+      } else {
+        float* fin = s_fin + (s & 1) * 768 + st * 384 + r_in;
+        fin[0] = m_ref;
+        fin[128] = l;
+        fin[256] = m_top;
+        named_sync<3, 256>();
+        const float* f = s_fin + (s & 1) * 768 + r_in;
+        const float m0 = f[0], m1 = f[384], l0 = f[128], l1 = f[512];
+        m = fmaxf(m0, m1);
+        top = fmaxf(f[256], f[640]);
+        a0 = part_factor(m0, l0, m, c_log2);
+        a1 = part_factor(m1, l1, m, c_log2);
+        l_all = l0 * a0 + l1 * a1;
+      }
+      tc_fence_after();
+      const bool bad = *ac.bad != 0;
+      const bool whole = w.begins() && w.ends();
+      const long long slot = 2ll * blockIdx.x + (w.begins() ? 1 : 0);
+      const bool odd = ac.odd[st] >= s + 1 || (!BOTH && ac.odd[1 - st] >= s + 1);
+      const int j0 = max(w.unit - w.uc, 0) * ATT_UNIT, j1 = odd ? min((w.unit + w.n - w.uc) * ATT_UNIT, w.count) : 0;
+      const bool some = exists && tk < w.count && l_all != 0.f;
+      const float nan = __int_as_float(0x7fc00000);
+      const bool writes = BOTH || st == 0;  // of the row's statistics
+      if (whole) {
+        const float inv = some ? 1.f / l_all : 0.f;
+        if (p.stats && exists && writes) {
+          float* at = p.stats + (static_cast<long long>(w.b) * p.H + h) * 2 * p.T + tk;
+          at[0] = bad ? nan : (some ? top : INFINITY);
+          at[p.T] = bad ? nan : (some ? log2f(l_all) + (m - top) * c_log2 : 0.f);
+        }
+        a0 = some ? a0 * inv : 0.f;
+        a1 = some ? a1 * inv : 0.f;
+      } else if (writes && r < p.gt * p.tt) {
+        float* at = p.part_ml + slot * 3 * p.rows + r;
+        at[0] = m;
+        at[p.rows] = l_all;
+        at[2 * p.rows] = top;
+      }
+      // columns: all of the stream's own rows (BOTH), or every second 32 of the shared ones
+      uint8_t* out = p.o + w.b * p.o_sb + static_cast<long long>(h) * p.o_sh + tk * p.o_ss;
+      float* part = p.part_o + (slot * p.rows + r) * 128;
+#pragma unroll 1
+      for (int i = BOTH ? 0 : 32 * st; i < D; i += BOTH ? 32 : 64) {
+        float o0[32];
+        tmem_ld32((BOTH ? tO : tmem + 256 + lane_base) + i, reinterpret_cast<uint32_t*>(o0));
+        tmem_wait_ld();
+#pragma unroll
+        for (int j = 0; j < 32; ++j) o0[j] = a0 == 0.f ? 0.f : o0[j] * a0;
+        if constexpr (!BOTH) {
+          float o1[32];
+          tmem_ld32(tmem + 384 + lane_base + i, reinterpret_cast<uint32_t*>(o1));
+          tmem_wait_ld();
+#pragma unroll
+          for (int j = 0; j < 32; ++j) o0[j] += a1 == 0.f ? 0.f : o1[j] * a1;
+        }
+        for (int j = j0; j < j1; ++j) {
+          if (!exists || !sees_new(p, w, tk, j)) continue;
+          const uint8_t* v = p.v + w.b * p.v_sb + rows.g * p.v_sh + j * p.v_ss + 2 * i;
+#pragma unroll
+          for (int k = 0; k < 32; ++k) {
+            if (i + k >= p.c.cols) break;
+            const float y = load16<BF16>(v + 2 * k);
+            if (!(fabsf(y) < INFINITY)) o0[k] += y;
+          }
+        }
+        if (whole) {
+          if (exists) {
+#pragma unroll
+            for (int j = 0; j < 32; j += 8)
+              if (i + j < p.c.cols)
+                *reinterpret_cast<uint4*>(out + 2 * (i + j)) =
+                    bad ? make_uint4(0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu)
+                        : make_uint4(pack16<BF16>(o0[j], o0[j + 1]), pack16<BF16>(o0[j + 2], o0[j + 3]), pack16<BF16>(o0[j + 4], o0[j + 5]),
+                                     pack16<BF16>(o0[j + 6], o0[j + 7]));
+          }
+        } else if (r < p.gt * p.tt) {
+#pragma unroll
+          for (int j = 0; j < 32; j += 4) *reinterpret_cast<float4*>(part + i + j) = make_float4(o0[j], o0[j + 1], o0[j + 2], o0[j + 3]);
+        }
+      }
+      tc_fence_before();
+      mbar_arrive(bar(R::B_OFREE + st));
+      if constexpr (!BOTH) mbar_arrive(bar(R::B_OFREE + 1 - st));
+      ++s;
+      more = w.next(p);
+    }
+    if (tid == 0 && !p.whole) note_parts(p, w, true, chunk, end);
+  }
+
+  // ---- teardown (every thread gets here, also after an abort) ----
+  tc_fence_before();
+  __syncthreads();
+  if (tid == 0 && *ac.bad) report(p.status, DEV_BAD_CACHE);
+  if (*ac.abort) att_give_up<R>(p, first, work, bar0, ac, kv_issued, q_issued);
+  if (warp == 8) {
+    tc_fence_after();
+    tmem_dealloc(tmem, R::TMEM);
   }
 }
 
 // Joins the parts of the items that were cut: CTA x has the item that begins in CTA x of the kernel above, a warp a row, a lane four
 // columns. Starts while that kernel ends and waits for it.
-template <int NR, bool BF16>
+template <bool BF16>
 __global__ void __launch_bounds__(256) kfa_cache_join_kernel(const AttendParams p) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int4 meta = p.part_meta[blockIdx.x];
@@ -840,9 +1248,9 @@ __global__ void __launch_bounds__(256) kfa_cache_join_kernel(const AttendParams 
   auto slot = [&](int i) { return 2ll * (blockIdx.x + i) + (i == 0 ? 1 : 0); };
   float m = -INFINITY, top = -INFINITY;
   for (int i = lane; i < meta.x; i += 32) {
-    const float* ml = p.part_ml + slot(i) * 3 * NR + r;
+    const float* ml = p.part_ml + slot(i) * 3 * p.rows + r;
     m = fmaxf(m, ml[0]);
-    top = fmaxf(top, ml[2 * NR]);
+    top = fmaxf(top, ml[2 * p.rows]);
   }
   m = warp_max(m);
   top = warp_max(top);
@@ -851,16 +1259,16 @@ __global__ void __launch_bounds__(256) kfa_cache_join_kernel(const AttendParams 
   for (int i0 = 0; i0 < meta.x; i0 += 32) {
     float a = 0.f, li = 0.f;
     if (i0 + lane < meta.x) {
-      const float* ml = p.part_ml + slot(i0 + lane) * 3 * NR + r;
-      a = part_factor(ml[0], ml[NR], m, p.c_log2);
-      li = a * ml[NR];
+      const float* ml = p.part_ml + slot(i0 + lane) * 3 * p.rows + r;
+      a = part_factor(ml[0], ml[p.rows], m, p.c_log2);
+      li = a * ml[p.rows];
     }
     const int n = min(32, meta.x - i0);
 #pragma unroll 4
     for (int i = 0; i < n; ++i) {
       const float ai = __shfl_sync(0xffffffffu, a, i);
       l += __shfl_sync(0xffffffffu, li, i);
-      const float4 x = *reinterpret_cast<const float4*>(p.part_o + (slot(i0 + i) * NR + r) * 128 + 4 * lane);
+      const float4 x = *reinterpret_cast<const float4*>(p.part_o + (slot(i0 + i) * p.rows + r) * 128 + 4 * lane);
       if (ai != 0.f) {
         o.x += ai * x.x;
         o.y += ai * x.y;

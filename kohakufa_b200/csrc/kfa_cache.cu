@@ -101,46 +101,47 @@ constexpr int SMS = 148;  // (what this library is built for)
 
 // How an attention call is cut up: a function of the shapes alone, so that the scratch it needs is known beforehand.
 struct AttendPlan {
-  int nr, gt, tt, head_tiles, row_tiles, grid;
+  int rows, gt, tt, head_tiles, row_tiles, grid, extra, least;
   bool whole;
-  int64_t meta_bytes, ml_bytes, bytes;
+  int64_t most_units, meta_bytes, ml_bytes, bytes;
 };
 
-AttendPlan plan_attend(int64_t batch, int64_t heads, int64_t kv_heads, int64_t T, int64_t capacity, bool fresh) {
+AttendPlan plan_attend(int64_t batch, int64_t heads, int64_t kv_heads, int64_t T, int64_t capacity, int64_t D, bool fresh) {
   AttendPlan a;
   const int64_t group = heads / kv_heads;
-  // Rows that share a K / V head, up to 128 of them in a tile: whole groups of heads, the tokens in equal parts.
-  const int64_t gt = std::min<int64_t>(group, 128), most = 128 / gt;
+  // Rows that share a K / V head, up to 256 of them in a tile: whole groups of heads, the tokens in equal parts.
+  const int64_t gt = std::min<int64_t>(group, 256), most = 256 / gt;
   const int64_t token_tiles = (T + most - 1) / most;
   const int64_t tt = (T + token_tiles - 1) / token_tiles;
   a.gt = static_cast<int>(gt);
   a.tt = static_cast<int>(tt);
   a.head_tiles = static_cast<int>((group + gt - 1) / gt);
   a.row_tiles = static_cast<int>(a.head_tiles * ((T + tt - 1) / tt));
-  a.nr = gt * tt <= 16 ? 16 : (gt * tt <= 32 ? 32 : (gt * tt <= 64 ? 64 : 128));
+  a.rows = gt * tt <= 16 ? 16 : (gt * tt <= 32 ? 32 : (gt * tt <= 64 ? 64 : (gt * tt <= 128 ? 128 : 256)));
   const int64_t items = batch * kv_heads * a.row_tiles;
   const int64_t units = std::max<int64_t>((capacity + 31) / 32 + (fresh ? (T + 31) / 32 : 0), 1);
   a.whole = units <= 8;
+  a.extra = D > 64 ? 6 : 10;
+  a.least = 4;
+  a.most_units = items * (units + a.extra);
   a.grid = static_cast<int>(std::min<int64_t>(SMS, a.whole ? items : (items * units + 3) / 4));
   a.meta_bytes = a.ml_bytes = a.bytes = 0;
   if (!a.whole) {
     a.meta_bytes = (16 * a.grid + 255) / 256 * 256;
-    a.ml_bytes = 2ll * a.grid * 3 * a.nr * 4;
-    a.bytes = a.meta_bytes + a.ml_bytes + 2ll * a.grid * a.nr * 128 * 4;
+    a.ml_bytes = 2ll * a.grid * 3 * a.rows * 4;
+    a.bytes = a.meta_bytes + a.ml_bytes + 2ll * a.grid * a.rows * 128 * 4;
   }
   return a;
 }
 
-template <int NC, int NR, bool BF16>
-int launch_attend(const CUtensorMap (&m)[5], const kfa::AttendParams& p, const AttendPlan& plan, cudaStream_t s) {
-  auto kern = kfa::kfa_cache_attend_kernel<NC, NR, BF16>;
-  using Cfg = kfa::AttCfg<NC, NR>;
-  KFA_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM));
-  kern<<<plan.grid, kfa::ATT_THREADS, Cfg::SMEM, s>>>(m[0], m[1], m[2], m[3], m[4], p);
+template <bool BF16, class R, typename K>
+int launch_attend(K kern, const CUtensorMap (&m)[5], const kfa::AttendParams& p, const AttendPlan& plan, cudaStream_t s) {
+  KFA_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, R::SMEM));
+  kern<<<plan.grid, kfa::ATT_THREADS, R::SMEM, s>>>(m[0], m[1], m[2], m[3], m[4], p);
   KFA_CUDA(cudaGetLastError());
   if (plan.whole) return KFA_OK;
   cudaLaunchConfig_t config = {};
-  config.gridDim = dim3(plan.grid, NR / 8);
+  config.gridDim = dim3(plan.grid, (plan.gt * plan.tt + 7) / 8);
   config.blockDim = dim3(256);
   config.stream = s;
   cudaLaunchAttribute early[1];
@@ -148,17 +149,18 @@ int launch_attend(const CUtensorMap (&m)[5], const kfa::AttendParams& p, const A
   early[0].val.programmaticStreamSerializationAllowed = 1;
   config.attrs = early;
   config.numAttrs = 1;
-  KFA_CUDA(cudaLaunchKernelEx(&config, kfa::kfa_cache_join_kernel<NR, BF16>, p));
+  KFA_CUDA(cudaLaunchKernelEx(&config, kfa::kfa_cache_join_kernel<BF16>, p));
   return KFA_OK;
 }
 
 template <int NC, bool BF16>
 int launch_attend_rows(const CUtensorMap (&m)[5], const kfa::AttendParams& p, const AttendPlan& plan, cudaStream_t s) {
-  switch (plan.nr) {
-    case 16: return launch_attend<NC, 16, BF16>(m, p, plan, s);
-    case 32: return launch_attend<NC, 32, BF16>(m, p, plan, s);
-    case 64: return launch_attend<NC, 64, BF16>(m, p, plan, s);
-    default: return launch_attend<NC, 128, BF16>(m, p, plan, s);
+  switch (plan.rows) {
+    case 16: return launch_attend<BF16, kfa::AttCfg<NC, 16>>(kfa::kfa_cache_attend_kernel<NC, 16, BF16>, m, p, plan, s);
+    case 32: return launch_attend<BF16, kfa::AttCfg<NC, 32>>(kfa::kfa_cache_attend_kernel<NC, 32, BF16>, m, p, plan, s);
+    case 64: return launch_attend<BF16, kfa::AttCfg<NC, 64>>(kfa::kfa_cache_attend_kernel<NC, 64, BF16>, m, p, plan, s);
+    case 128: return launch_attend<BF16, kfa::AttRowsCfg<NC, 1>>(kfa::kfa_cache_attend_rows_kernel<NC, 1, BF16>, m, p, plan, s);
+    default: return launch_attend<BF16, kfa::AttRowsCfg<NC, 2>>(kfa::kfa_cache_attend_rows_kernel<NC, 2, BF16>, m, p, plan, s);
   }
 }
 
@@ -170,7 +172,9 @@ int64_t kfa_cache_attend_bytes(const KfaTensor4* q, const KfaCache* cache, const
   if (!q || !cache) return 0;
   const int64_t page = cache->k.shape[2], kv_heads = cache->k.shape[1];
   if (q->shape[0] < 1 || q->shape[1] < 1 || q->shape[2] < 1 || kv_heads < 1 || q->shape[1] < kv_heads || page < 1) return 0;  // (refused by the call)
-  return plan_attend(q->shape[0], q->shape[1], kv_heads, q->shape[2], cache->table ? cache->table_cols * page : page, k != nullptr).bytes;
+  return plan_attend(q->shape[0], q->shape[1], kv_heads, q->shape[2], cache->table ? cache->table_cols * page : page,
+                     cache->k.shape[3], k != nullptr)
+      .bytes;
 }
 
 int kfa_cache_attend(const KfaTensor4* q, const KfaCache* cache, const KfaTensor4* k, const KfaTensor4* v, const uint8_t* tree,
@@ -207,8 +211,8 @@ int kfa_cache_attend(const KfaTensor4* q, const KfaCache* cache, const KfaTensor
   p.c_log2 = std::max(scale * LOG2E, 1e-30f);
   p.slack = 8.f / p.c_log2;
   p.status = dev_status;
-  const AttendPlan plan = plan_attend(p.c.batch, p.H, p.c.heads, p.T, p.c.capacity, k != nullptr);
-  if (static_cast<int64_t>(p.c.batch) * p.c.heads * plan.row_tiles > 0x7fffffff) return fail(KFA_ERR_ARG, "too many rows in one call");
+  const AttendPlan plan = plan_attend(p.c.batch, p.H, p.c.heads, p.T, p.c.capacity, p.c.cols, k != nullptr);
+  if (plan.most_units > 0x3fffffff) return fail(KFA_ERR_ARG, "too many rows in one call");
   if (plan.bytes && (!scratch || reinterpret_cast<uintptr_t>(scratch) % 16)) return fail(KFA_ERR_ARG, "scratch: null or not 16-byte aligned");
   p.gt = plan.gt;
   p.tt = plan.tt;
@@ -219,7 +223,11 @@ int kfa_cache_attend(const KfaTensor4* q, const KfaCache* cache, const KfaTensor
   p.by_items = kfa::FastDiv::by(p.items);
   p.by_row_tiles = kfa::FastDiv::by(p.row_tiles);
   p.by_head_tiles = kfa::FastDiv::by(p.head_tiles);
+  p.by_grid = kfa::FastDiv::by(plan.grid);
   p.whole = plan.whole;
+  p.least = plan.least;
+  p.extra = plan.extra;
+  p.rows = plan.rows;
   p.box = p.c.table ? (p.c.page % 32 == 0 ? 32 : (p.c.page % 16 == 0 ? 16 : 8)) : 32;
   if (!plan.whole) {
     uint8_t* at = static_cast<uint8_t*>(scratch);
