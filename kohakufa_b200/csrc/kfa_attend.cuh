@@ -166,25 +166,23 @@ __device__ __forceinline__ bool my_work(const AttendParams& p, int* s_i, Walk& w
     upto += before;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      if (at[i] >= upto - own && at[i] < upto) {
-        s_i[2 * i] = b0 + tid;
-        s_i[2 * i + 1] = static_cast<int>(at[i]) - (upto - own);
+      if (at[i] >= upto - own && at[i] < upto) {  // (one thread's sequence)
+        const int off = static_cast<int>(at[i]) - (upto - own), each = own / p.items, item = off / each;
+        s_i[3 * i] = b0 + tid;
+        s_i[3 * i + 1] = item;
+        s_i[3 * i + 2] = max(off - item * each - p.extra, 0);
       }
     }
     before += all;
   }
   __syncthreads();
-  auto place = [&](int i, int& b, int& item, int& unit) {
-    b = p.c.batch;
-    item = unit = 0;
-    if (at[i] >= total) return;
-    b = s_i[2 * i];
-    const int off = s_i[2 * i + 1], each = Walk::units_of(p, b) + p.extra;
-    item = off / each;
-    unit = max(off - item * each - p.extra, 0);
-  };
-  place(0, w.b, w.item, w.unit);
-  place(1, w.end_b, w.end_item, w.end_unit);
+  const bool inside[2] = {at[0] < total, at[1] < total};
+  w.b = inside[0] ? s_i[0] : p.c.batch;
+  w.item = inside[0] ? s_i[1] : 0;
+  w.unit = inside[0] ? s_i[2] : 0;
+  w.end_b = inside[1] ? s_i[3] : p.c.batch;
+  w.end_item = inside[1] ? s_i[4] : 0;
+  w.end_unit = inside[1] ? s_i[5] : 0;
   end = static_cast<int>(at[1]);
   return w.b < p.c.batch && w.start(p);
 }
@@ -213,9 +211,10 @@ struct AttRings {
   __device__ static __forceinline__ int v_stage(int T) { return RINGS * DK + (BOTH ? T % DV : (T & 1) * DV + (T >> 1) % DV); }
   __device__ static __forceinline__ int k_turn(int T) { return (BOTH ? T : T >> 1) / DK; }
   __device__ static __forceinline__ int v_turn(int T) { return (BOTH ? T : T >> 1) / DV; }
-  // barriers: tiles there and free, queries there, scores there, P there, P V done, O read, all done
-  static constexpr int B_KV = 0, B_KVFREE = NS, B_Q = 2 * NS, B_S = B_Q + NQ, B_P = B_S + 4, B_PV = B_P + 4, B_OFREE = B_PV + 4,
-                       B_DRAIN = B_OFREE + 2, N_BARS = B_DRAIN + 2;
+  // barriers: tiles there and free, queries there, scores there, P there, P V done, a segment is finished, a stream's O has been read (in the
+  // segments in which the stream had tiles), all done
+  static constexpr int B_KV = 0, B_KVFREE = NS, B_Q = 2 * NS, B_S = B_Q + NQ, B_P = B_S + 4, B_PV = B_P + 4, B_QFREE = B_PV + 4,
+                       B_OFREE = B_QFREE + 1, B_DRAIN = B_OFREE + 2, N_BARS = B_DRAIN + 2;
   static_assert(N_BARS * 8 + 256 <= 1024, "barrier block");
 };
 
@@ -339,6 +338,7 @@ __device__ __forceinline__ bool att_setup(const AttendParams& p, uint32_t bar0, 
       int count = 1;
       if (i >= R::B_KVFREE && i < R::B_Q) count = R::BOTH ? 2 : 1;
       if (i >= R::B_P && i < R::B_PV) count = 128;
+      if (i == R::B_QFREE) count = 256;
       if (i >= R::B_OFREE && i < R::B_DRAIN) count = R::BOTH ? 128 : 256;
       mbar_init(bar0 + 8u * i, count);
     }
@@ -378,7 +378,7 @@ __device__ __forceinline__ void att_produce(const AttendParams& p, const Walk& f
     if (lane == 0 && !length_ok(p.c, w.b)) *ac.bad = 1;
     if (!values) {
       if (s >= R::NQ) {  // both streams are done with the segment that used this buffer
-        ok = mbar_wait_warp(bar(R::B_OFREE), (s - R::NQ) & 1, ctl, 70) && mbar_wait_warp(bar(R::B_OFREE + 1), (s - R::NQ) & 1, ctl, 71);
+        ok = mbar_wait_warp(bar(R::B_QFREE), (s - R::NQ) & 1, ctl, 70);
         if (!ok) break;
       }
       if (lane == 0) {
@@ -429,12 +429,13 @@ __device__ __forceinline__ void att_produce(const AttendParams& p, const Walk& f
 // A stream's tiles one after the other, over all segments.
 struct AttTile {
   int T, s;
+  int uses;    // segments before in which the stream had tiles
   bool opens;  // the stream's first tile of segment s
 };
 template <bool BOTH>
 struct AttTiles {
   Walk w;
-  int st, at = 0, T = 0, s = 0;
+  int st, at = 0, T = 0, s = 0, uses = 0;
   bool more = true, opens = true;
   __device__ __forceinline__ bool take(const AttendParams& p, AttTile& t) {
     while (more) {
@@ -442,13 +443,14 @@ struct AttTiles {
         ++at;
         const int now = T++;
         if (BOTH || (now & 1) == st) {
-          t = {now, s, opens};
+          t = {now, s, uses, opens};
           opens = false;
           return true;
         }
       }
       at = 0;
       ++s;
+      uses += opens ? 0 : 1;
       opens = true;
       more = w.next(p);
     }
@@ -464,7 +466,7 @@ template <class R, int PIECES, int NP, typename FS, typename FP>
 __device__ __forceinline__ void att_issue(const AttendParams& p, const Walk& first, int st, uint32_t bar0, const AttCtl& ac, FS issue_S, FP issue_PV) {
   auto ready = [&](int i, uint32_t parity) { return __all_sync(0xffffffffu, mbar_test(bar0 + 8u * i, parity)); };
   AttTiles<R::BOTH> tiles{first, st};
-  AttTile ahead = {0, 0, false}, even = ahead, odd = ahead;  // the next to get scores; those that have, by c (at most two wait for values)
+  AttTile ahead = {0, 0, 0, false}, even = ahead, odd = ahead;  // the next to get scores; those that have, by c (at most two wait for values)
   bool have = tiles.take(p, ahead);
   int i_s = 0, i_p = 0;  // pieces of scores and of values issued
   long long t0 = clock64();
@@ -487,10 +489,14 @@ __device__ __forceinline__ void att_issue(const AttendParams& p, const Walk& fir
     }
     if (i_p < i_s) {
       const int c = i_p / PIECES, piece = i_p % PIECES;
+      // (nothing else can go before these values: no need to look at both)
+      if ((!have || i_s > i_p + 1) &&
+          !mbar_wait_warp(bar0 + 8u * (R::B_P + 2 * st + (PIECES == 2 ? piece : c % NP)), (PIECES == 2 ? c : c / NP) & 1, Ctl{ac.abort}, 74))
+        break;
       const AttTile now = (c * PIECES + PIECES > i_s) ? ahead : ((c & 1) ? odd : even);  // (its second half may have no scores yet)
       if (ready(R::B_P + 2 * st + (PIECES == 2 ? piece : c % NP), (PIECES == 2 ? c : c / NP) & 1) &&
           (piece > 0 || (ready(R::B_KV + R::v_stage(now.T), R::v_turn(now.T) & 1) &&
-                         (!now.opens || now.s == 0 || ready(R::B_OFREE + st, (now.s - 1) & 1))))) {
+                         (!now.opens || now.uses == 0 || ready(R::B_OFREE + st, (now.uses - 1) & 1))))) {
         tc_fence_after();
         issue_PV(now, c, piece);
         ++i_p;
@@ -512,6 +518,21 @@ __device__ __forceinline__ void att_issue(const AttendParams& p, const Walk& fir
   mbar_drain(bar0 + 8u * (R::B_DRAIN + st), 0);
 }
 
+// A bit for each of the first n (at most 32) bytes `stride` apart that are not 0. (The loads do not wait for one another.)
+__device__ __forceinline__ uint32_t tree_bits(const uint8_t* at, long long stride, int n) {
+  uint32_t bits = 0;
+#pragma unroll 1
+  for (int i0 = 0; i0 < min(n, 32); i0 += 8) {
+    uint8_t x[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = at[min(i0 + i, n - 1) * stride];
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (i0 + i < n && x[i] != 0) bits |= 1u << (i0 + i);
+  }
+  return bits;
+}
+
 // Which keys of a unit the row of token t sees, a bit each (the first pass of a masked tile).
 __device__ __forceinline__ uint32_t seen_word(const AttendParams& p, const Walk& w, int unit, int t) {
   if (unit >= w.unit + w.n) return 0u;
@@ -527,47 +548,53 @@ __device__ __forceinline__ uint32_t seen_word(const AttendParams& p, const Walk&
     const int upto = t - j0;  // tokens 0 .. t
     return upto < 0 ? 0u : (upto >= ATT_UNIT - 1 ? there : there & ((2u << upto) - 1u));
   }
-  const uint8_t* tree = p.tree + w.b * p.tree_sb + t * p.tree_st + j0 * p.tree_sj;
-  uint32_t seen = 0;
-#pragma unroll 8
-  for (int j = 0; j < ATT_UNIT; ++j)
-    if (j < left && tree[j * p.tree_sj] != 0) seen |= 1u << j;
-  return seen & there;
+  return there & tree_bits(p.tree + w.b * p.tree_sb + t * p.tree_st + j0 * p.tree_sj, p.tree_sj, left);
 }
 
 // Values behind the end may be anything, and 0 * NaN is no 0: in a tile that is not full of cached keys, the thread of key `key` zeroes
 // its row of the tile. So it does with the values of a new token that are not finite, which would otherwise reach rows that do not see it; the
-// epilogue hands them to those that do. Returns whether there were such. fresh: the new token that the key is, < 0: a cached one.
-template <int NC, bool BF16>
-__device__ __forceinline__ bool clean_values(const AttendParams& p, const Walk& w, int g, uint32_t stage, int key, bool valid, int fresh) {
-  const uint32_t row = stage + key * 128;
-  bool found = false;
-  if (!valid) {
-#pragma unroll
-    for (int i = 0; i < NC * 8; ++i)
-      asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(row + (i >> 3) * (128 * 128) + (i & 7) * 16), "r"(0) : "memory");
-  } else if (fresh >= 0) {
-    const uint8_t* g_row = p.v + w.b * p.v_sb + g * p.v_sh + fresh * p.v_ss;
-#pragma unroll 4
-    for (int i = 0; i < p.c.cols / 8; ++i) {
-      const uint4 q4 = *reinterpret_cast<const uint4*>(g_row + 16 * i);
-      uint32_t q[4] = {q4.x, q4.y, q4.z, q4.w};
-      bool odd = false;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        constexpr uint32_t E = BF16 ? 0x7f80u : 0x7c00u;  // all exponent bits: infinity or NaN
-        if ((q[j] & E) == E) q[j] &= 0xffff0000u, odd = true;
-        if (((q[j] >> 16) & E) == E) q[j] &= 0xffffu, odd = true;
-      }
-      if (odd) {
-        found = true;
-        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(row + (i >> 3) * (128 * 128) + (((i & 7) ^ (key & 7)) << 4)),
-                     "r"(q[0]), "r"(q[1]), "r"(q[2]), "r"(q[3])
-                     : "memory");
-      }
-    }
+// epilogue hands them to those that do. odd_values looks for them in memory, ahead of the scores: which 16-byte pieces hold any.
+template <bool BF16>
+__device__ __forceinline__ bool odd_half(uint32_t x) {  // all exponent bits: infinity or NaN
+  constexpr uint32_t E = BF16 ? 0x7f80u : 0x7c00u;
+  return (x & E) == E;
+}
+template <bool BF16>
+__device__ __forceinline__ uint32_t odd_values(const AttendParams& p, const Walk& w, int g, int fresh) {
+  if (fresh < 0) return 0u;
+  const uint8_t* row = p.v + w.b * p.v_sb + g * p.v_sh + fresh * p.v_ss;
+  uint32_t found = 0;
+#pragma unroll 8
+  for (int i = 0; i < p.c.cols / 8; ++i) {
+    const uint4 q = *reinterpret_cast<const uint4*>(row + 16 * i);
+    const bool odd = odd_half<BF16>(q.x) || odd_half<BF16>(q.x >> 16) || odd_half<BF16>(q.y) || odd_half<BF16>(q.y >> 16) ||
+                     odd_half<BF16>(q.z) || odd_half<BF16>(q.z >> 16) || odd_half<BF16>(q.w) || odd_half<BF16>(q.w >> 16);
+    found |= (odd ? 1u : 0u) << i;
   }
   return found;
+}
+template <int NC, bool BF16>
+__device__ __forceinline__ void clean_values(const AttendParams& p, const Walk& w, int g, uint32_t stage, int key, bool valid, int fresh, uint32_t odd) {
+  const uint32_t row = stage + key * 128;
+  if (!valid) {
+#pragma unroll
+    for (int i = 0; i < NC * 8; ++i)  // (rows begin at the same bank: each thread in an order of its own)
+      asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(row + (i >> 3) * (128 * 128) + (((i ^ key) & 7) << 4)), "r"(0) : "memory");
+  }
+  while (odd != 0) {
+    const int i = __ffs(odd) - 1;
+    odd &= odd - 1;
+    const uint4 q4 = *reinterpret_cast<const uint4*>(p.v + w.b * p.v_sb + g * p.v_sh + fresh * p.v_ss + 16 * i);
+    uint32_t q[4] = {q4.x, q4.y, q4.z, q4.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (odd_half<BF16>(q[j])) q[j] &= 0xffff0000u;
+      if (odd_half<BF16>(q[j] >> 16)) q[j] &= 0xffffu;
+    }
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(row + (i >> 3) * (128 * 128) + (((i ^ key) & 7) << 4)), "r"(q[0]), "r"(q[1]),
+                 "r"(q[2]), "r"(q[3])
+                 : "memory");
+  }
 }
 // What key `key` of the tile at unit ub is: whether it exists; the new token that it is, < 0: a cached one.
 __device__ __forceinline__ bool which_key(const Walk& w, int ub, int key, int& fresh) {
@@ -654,6 +681,9 @@ kfa_cache_attend_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
   const uint32_t bar0 = smem_u32(bars);
   auto bar = [&](int i) { return bar0 + 8u * i; };
   const int tid = threadIdx.x, warp = warp_index(), lane = tid & 31;
+  if (tid == 32 * 11) {
+    for (const CUtensorMap* map : {&tmQ, &tmK, &tmV, &tmKn, &tmVn}) asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
+  }
   Walk first;
   int chunk, end;
   const bool work = att_setup<R>(p, bar0, ac, R::TMEM, first, chunk, end);
@@ -724,43 +754,32 @@ kfa_cache_attend_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
         const bool full = 4 * t + 4 <= w.n && (ub + 4) * ATT_UNIT <= w.len && ub + 4 <= w.uc;
         int fresh = -1;
         const bool valid = full || which_key(w, ub, key, fresh);
+        // ahead of the scores: a bit per token of the row tile that sees this new token (N rows hold at most N tokens)
+        uint32_t see[PER], odd = 0u;
+        if (!full) {
+#pragma unroll
+          for (int k = 0; k < PER; ++k) {
+            see[k] = valid ? 0xffffffffu : 0u;
+            if (fresh >= 0) {
+              const int t0 = rows.t0 + 32 * k, n = min(min(p.tt - 32 * k, p.T - t0), w.count - t0);  // tokens that there are
+              see[k] = n <= 0 ? 0u : (n >= 32 ? 0xffffffffu : (1u << n) - 1u);
+              if (n > 0 && p.tree != nullptr) see[k] = tree_bits(p.tree + w.b * p.tree_sb + t0 * p.tree_st + fresh * p.tree_sj, p.tree_st, n);
+              if (p.tree == nullptr && fresh > t0) see[k] &= fresh - t0 >= 32 ? 0u : 0xffffffffu << (fresh - t0);
+            }
+          }
+          odd = odd_values<BF16>(p, w, rows.g, fresh);
+        }
         if (ok) ok = mbar_wait_warp(bar(R::B_S + 2 * st + (c & 1)), (c >> 1) & 1, ctl, 78);
         tc_fence_after();
         float x[N];
         tmem_ld_cols<N>(tmS + lane_base + (2 * st + (c & 1)) * N, x);
         tmem_wait_ld();
         if (!full) {
-          if (!valid) {
 #pragma unroll
-            for (int i = 0; i < N; ++i) x[i] = -INFINITY;
-          } else if (fresh >= 0 && (p.T > 1 || p.tree != nullptr || w.count == 0)) {
-            // a bit per token of the row tile: which of them see this new token (N rows hold at most N tokens)
-            uint32_t see[PER];
-#pragma unroll
-            for (int i = 0; i < PER; ++i) see[i] = 0u;
-            const int most = min(p.tt, p.T - rows.t0);
-            if (p.tree == nullptr) {
-              for (int i = 0; i < most; ++i)
-                if (rows.t0 + i >= fresh && rows.t0 + i < w.count) see[i / 32] |= 1u << (i & 31);
-            } else {
-              const uint8_t* tree = p.tree + w.b * p.tree_sb + rows.t0 * p.tree_st + fresh * p.tree_sj;
-#pragma unroll
-              for (int k = 0; k < PER; ++k)
-#pragma unroll 8
-                for (int i = 0; i < 32; ++i)
-                  if (32 * k + i < most && tree[(32 * k + i) * p.tree_st] != 0) see[k] |= 1u << i;
-#pragma unroll
-              for (int k = 0; k < PER; ++k) {  // tokens that the sequence does not have see nothing
-                const int left = w.count - rows.t0 - 32 * k;
-                see[k] = left <= 0 ? 0u : (left >= 32 ? see[k] : see[k] & ((1u << left) - 1u));
-              }
-            }
-#pragma unroll
-            for (int i = 0; i < N; ++i) {
-              const int dt = static_cast<int>(p.by_gt.div(i));
-              const uint32_t word = PER == 1 || dt < 32 ? see[0] : see[PER - 1];
-              if (!((word >> (dt & 31)) & 1u)) x[i] = -INFINITY;
-            }
+          for (int i = 0; i < N; ++i) {
+            const int dt = fresh >= 0 ? static_cast<int>(p.by_gt.div(i)) : 0;
+            const uint32_t word = PER == 1 || dt < 32 ? see[0] : see[PER - 1];
+            if (!((word >> (dt & 31)) & 1u)) x[i] = -INFINITY;
           }
         }
         // ---- column maxima ----
@@ -834,7 +853,8 @@ kfa_cache_attend_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
           // (The tile before has to be done with: until then the barrier of this one's stage may be a turn behind.)
           if (c > 0 && ok) ok = mbar_wait_warp(bar(R::B_PV + 2 * st + (c - 1) % NP), ((c - 1) / NP) & 1, ctl, 81);
           if (ok) ok = mbar_wait_warp(bar(R::B_KV + R::v_stage(T)), R::v_turn(T) & 1, ctl, 82);
-          if (clean_values<NC, BF16>(p, w, rows.g, sKV + R::v_stage(T) * R::STAGE, key, valid, fresh)) ac.odd[st] = s + 1;
+          clean_values<NC, BF16>(p, w, rows.g, sKV + R::v_stage(T) * R::STAGE, key, valid, fresh, odd);
+          if (odd != 0) ac.odd[st] = s + 1;
         }
         fence_async_smem();
         tc_fence_before();
@@ -935,8 +955,9 @@ kfa_cache_attend_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
           if (c0 + i < p.gt * p.tt) p.part_o[(slot * p.rows + c0 + i) * 128 + d] = o0[i];
       }
       tc_fence_before();
-      mbar_arrive(bar(R::B_OFREE + st));
-      mbar_arrive(bar(R::B_OFREE + 1 - st));
+      if (tiles > 1 || ((T0 - 1) & 1) == 0) mbar_arrive(bar(R::B_OFREE));
+      if (tiles > 1 || ((T0 - 1) & 1) == 1) mbar_arrive(bar(R::B_OFREE + 1));
+      mbar_arrive(bar(R::B_QFREE));
       ++s;
       more = w.next(p);
     }
@@ -957,7 +978,7 @@ kfa_cache_attend_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
 // ---- more rows ------------------------------------------------------------------------------------------------------------
 // HALVES: 1: up to 128 rows, tiles to the streams in turn; 2: up to 256 rows, a half of them to each stream.
 template <int NC, int HALVES>
-struct AttRowsCfg : AttRings<NC, 128 * HALVES, HALVES == 1 ? 2 : 1, HALVES == 2, 1024 + 2 * 2 * 128 * 3 * 4> {
+struct AttRowsCfg : AttRings<NC, 128 * HALVES, HALVES == 1 ? 2 : 1, HALVES == 2, 1024 + 2 * 2 * 128 * 3 * 4 + (HALVES * NC == 1 ? 32768 : 0)> {
   static constexpr int TMEM = 512;  // S 2 x 128; O 2 x 128
 };
 
@@ -982,7 +1003,10 @@ kfa_cache_attend_rows_kernel(const __grid_constant__ CUtensorMap tmQ, const __gr
   const AttCtl ac(bars + R::N_BARS);
   const uint32_t bar0 = smem_u32(bars);
   auto bar = [&](int i) { return bar0 + 8u * i; };
-  const int tid = threadIdx.x, warp = warp_index();
+  const int tid = threadIdx.x, warp = warp_index(), lane = tid & 31;
+  if (tid == 32 * 11) {
+    for (const CUtensorMap* map : {&tmQ, &tmK, &tmV, &tmKn, &tmVn}) asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
+  }
   Walk first;
   int chunk, end;
   const bool work = att_setup<R>(p, bar0, ac, R::TMEM, first, chunk, end);
@@ -1047,6 +1071,13 @@ kfa_cache_attend_rows_kernel(const __grid_constant__ CUtensorMap tmQ, const __gr
         if (!BOTH && (T & 1) != st) continue;
         const int ub = w.unit + 4 * t;
         const bool full = 4 * t + 4 <= w.n && (ub + 4) * ATT_UNIT <= w.len && ub + 4 <= w.uc;
+        int fresh = -1;
+        bool valid = true;
+        uint32_t odd = 0u;
+        if (!full) {
+          valid = which_key(w, ub, r_in, fresh);
+          odd = odd_values<BF16>(p, w, rows.g, fresh);
+        }
 #pragma unroll 1
         for (int half = 0; half < 2; ++half) {
           uint32_t seen[2] = {0xffffffffu, 0xffffffffu};
@@ -1111,9 +1142,8 @@ kfa_cache_attend_rows_kernel(const __grid_constant__ CUtensorMap tmQ, const __gr
             // (The tile before has to be done with: until then the barrier of this one's stage may be a turn behind.)
             if (c > 0 && ok) ok = mbar_wait_warp(bar(R::B_PV + 2 * st + 1), (c - 1) & 1, ctl, 81);
             if (ok) ok = mbar_wait_warp(bar(R::B_KV + R::v_stage(T)), R::v_turn(T) & 1, ctl, 82);
-            int fresh;
-            const bool valid = which_key(w, ub, r_in, fresh);
-            if (clean_values<NC, BF16>(p, w, rows.g, sKV + R::v_stage(T) * R::STAGE, r_in, valid, fresh)) ac.odd[st] = s + 1;
+            clean_values<NC, BF16>(p, w, rows.g, sKV + R::v_stage(T) * R::STAGE, r_in, valid, fresh, odd);
+            if (odd != 0) ac.odd[st] = s + 1;
             fence_async_smem();
           }
           tc_fence_before();
@@ -1169,9 +1199,14 @@ kfa_cache_attend_rows_kernel(const __grid_constant__ CUtensorMap tmQ, const __gr
         at[p.rows] = l_all;
         at[2 * p.rows] = top;
       }
-      // columns: all of the stream's own rows (BOTH), or every second 32 of the shared ones
-      uint8_t* out = p.o + w.b * p.o_sb + static_cast<long long>(h) * p.o_sh + tk * p.o_ss;
-      float* part = p.part_o + (slot * p.rows + r) * 128;
+      // Columns: all of the stream's own rows (BOTH), or every second 32 of the shared ones. A thread holds a row, and a store of 16 bytes by
+      // each of 32 rows touches 32 lines: through 4 KB a warp of the queries' buffer, which the segment has done with (of two
+      // streams' 128 rows x 64 columns: memory of its own), whole pieces of rows are written one after the other. 10000 -> 5000 clk.
+      const uint32_t turn = lane & 7;
+      const uint32_t out_stage = HALVES * NC == 1 ? smem_u32(s_fin) + 6144 + (st * 4 + wl) * 4096
+                                                  : sQ + (s % R::NQ) * R::Q_BYTES + (BOTH ? st * 128 * 128 : st * R::Q_CHUNK) + wl * 4096;
+      const long long off = exists ? w.b * p.o_sb + static_cast<long long>(h) * p.o_sh + tk * p.o_ss : -1;
+      const int r_warp = r - lane;
 #pragma unroll 1
       for (int i = BOTH ? 0 : 32 * st; i < D; i += BOTH ? 32 : 64) {
         float o0[32];
@@ -1196,24 +1231,55 @@ kfa_cache_attend_rows_kernel(const __grid_constant__ CUtensorMap tmQ, const __gr
             if (!(fabsf(y) < INFINITY)) o0[k] += y;
           }
         }
+        __syncwarp();
         if (whole) {
-          if (exists) {
 #pragma unroll
-            for (int j = 0; j < 32; j += 8)
-              if (i + j < p.c.cols)
-                *reinterpret_cast<uint4*>(out + 2 * (i + j)) =
-                    bad ? make_uint4(0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu)
-                        : make_uint4(pack16<BF16>(o0[j], o0[j + 1]), pack16<BF16>(o0[j + 2], o0[j + 3]), pack16<BF16>(o0[j + 4], o0[j + 5]),
-                                     pack16<BF16>(o0[j + 6], o0[j + 7]));
+          for (int j = 0; j < 4; ++j)  // rows of 64 bytes: 4 pieces
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(out_stage + lane * 64 + ((j ^ ((turn >> 1) & 3)) << 4)),
+                         "r"(pack16<BF16>(o0[8 * j], o0[8 * j + 1])), "r"(pack16<BF16>(o0[8 * j + 2], o0[8 * j + 3])),
+                         "r"(pack16<BF16>(o0[8 * j + 4], o0[8 * j + 5])), "r"(pack16<BF16>(o0[8 * j + 6], o0[8 * j + 7]))
+                         : "memory");
+          __syncwarp();
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const int row = 8 * k + (lane >> 2), piece = lane & 3;
+            const long long at = __shfl_sync(0xffffffffu, off, row);
+            uint4 y;
+            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                         : "=r"(y.x), "=r"(y.y), "=r"(y.z), "=r"(y.w)
+                         : "r"(out_stage + row * 64 + ((piece ^ ((row >> 1) & 3)) << 4))
+                         : "memory");
+            if (bad) y = make_uint4(0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu);
+            if (at >= 0 && i + 8 * piece < p.c.cols) *reinterpret_cast<uint4*>(p.o + at + 2 * i + 16 * piece) = y;
           }
-        } else if (r < p.gt * p.tt) {
+        } else {
 #pragma unroll
-          for (int j = 0; j < 32; j += 4) *reinterpret_cast<float4*>(part + i + j) = make_float4(o0[j], o0[j + 1], o0[j + 2], o0[j + 3]);
+          for (int j = 0; j < 8; ++j)  // rows of 128 bytes: 8 pieces
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(out_stage + lane * 128 + ((j ^ turn) << 4)), "r"(__float_as_uint(o0[4 * j])),
+                         "r"(__float_as_uint(o0[4 * j + 1])), "r"(__float_as_uint(o0[4 * j + 2])), "r"(__float_as_uint(o0[4 * j + 3]))
+                         : "memory");
+          __syncwarp();
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const int row = 4 * k + (lane >> 3), piece = lane & 7;
+            uint4 y;
+            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                         : "=r"(y.x), "=r"(y.y), "=r"(y.z), "=r"(y.w)
+                         : "r"(out_stage + row * 128 + ((piece ^ (row & 7)) << 4))
+                         : "memory");
+            if (r_warp + row < p.gt * p.tt) *reinterpret_cast<uint4*>(p.part_o + (slot * p.rows + r_warp + row) * 128 + i + 4 * piece) = y;
+          }
         }
       }
+      fence_async_smem();  // (the next queries are copied over what was written)
       tc_fence_before();
-      mbar_arrive(bar(R::B_OFREE + st));
-      if constexpr (!BOTH) mbar_arrive(bar(R::B_OFREE + 1 - st));
+      if (BOTH) {
+        mbar_arrive(bar(R::B_OFREE + st));
+      } else {
+        if (tiles > 1 || ((T0 - 1) & 1) == 0) mbar_arrive(bar(R::B_OFREE));
+        if (tiles > 1 || ((T0 - 1) & 1) == 1) mbar_arrive(bar(R::B_OFREE + 1));
+      }
+      mbar_arrive(bar(R::B_QFREE));
       ++s;
       more = w.next(p);
     }
