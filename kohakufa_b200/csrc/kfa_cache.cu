@@ -106,7 +106,7 @@ struct AttendPlan {
   int64_t most_units, meta_bytes, ml_bytes, bytes;
 };
 
-AttendPlan plan_attend(int64_t batch, int64_t heads, int64_t kv_heads, int64_t T, int64_t capacity, int64_t D, bool fresh) {
+AttendPlan plan_attend(int64_t batch, int64_t heads, int64_t kv_heads, int64_t T, int64_t capacity, bool fresh) {
   AttendPlan a;
   const int64_t group = heads / kv_heads;
   // Rows that share a K / V head, up to 256 of them in a tile: whole groups of heads, the tokens in equal parts.
@@ -121,7 +121,10 @@ AttendPlan plan_attend(int64_t batch, int64_t heads, int64_t kv_heads, int64_t T
   const int64_t items = batch * kv_heads * a.row_tiles;
   const int64_t units = std::max<int64_t>((capacity + 31) / 32 + (fresh ? (T + 31) / 32 : 0), 1);
   a.whole = units <= 8;
-  a.extra = D > 64 ? 6 : 10;
+  // What an item's beginning and end take, in units of 32 keys. Graph time per call in us with 4, 8, 12, 16, 24: 64 sequences of 1 to 4096
+  // positions, one token each (D = 128) 116, 105, 101, 103, 103; 32 x 12 heads over 0 to 1500 (D = 80) 44, 34, 30, 28, 28; 8 sequences of 300 to
+  // 2048, 7 tokens (D = 64) 17.5, 16.5, 15.4, 15.7, 15.6; 16 of 2048 to 4096, 256 rows 116, 112, 111, 105, 106.
+  a.extra = a.rows > 64 ? 16 : 12;
   a.least = 4;
   a.most_units = items * (units + a.extra);
   a.grid = static_cast<int>(std::min<int64_t>(SMS, a.whole ? items : (items * units + 3) / 4));
@@ -172,9 +175,7 @@ int64_t kfa_cache_attend_bytes(const KfaTensor4* q, const KfaCache* cache, const
   if (!q || !cache) return 0;
   const int64_t page = cache->k.shape[2], kv_heads = cache->k.shape[1];
   if (q->shape[0] < 1 || q->shape[1] < 1 || q->shape[2] < 1 || kv_heads < 1 || q->shape[1] < kv_heads || page < 1) return 0;  // (refused by the call)
-  return plan_attend(q->shape[0], q->shape[1], kv_heads, q->shape[2], cache->table ? cache->table_cols * page : page,
-                     cache->k.shape[3], k != nullptr)
-      .bytes;
+  return plan_attend(q->shape[0], q->shape[1], kv_heads, q->shape[2], cache->table ? cache->table_cols * page : page, k != nullptr).bytes;
 }
 
 int kfa_cache_attend(const KfaTensor4* q, const KfaCache* cache, const KfaTensor4* k, const KfaTensor4* v, const uint8_t* tree,
@@ -211,7 +212,7 @@ int kfa_cache_attend(const KfaTensor4* q, const KfaCache* cache, const KfaTensor
   p.c_log2 = std::max(scale * LOG2E, 1e-30f);
   p.slack = 8.f / p.c_log2;
   p.status = dev_status;
-  const AttendPlan plan = plan_attend(p.c.batch, p.H, p.c.heads, p.T, p.c.capacity, p.c.cols, k != nullptr);
+  const AttendPlan plan = plan_attend(p.c.batch, p.H, p.c.heads, p.T, p.c.capacity, k != nullptr);
   if (plan.most_units > 0x3fffffff) return fail(KFA_ERR_ARG, "too many rows in one call");
   if (plan.bytes && (!scratch || reinterpret_cast<uintptr_t>(scratch) % 16)) return fail(KFA_ERR_ARG, "scratch: null or not 16-byte aligned");
   p.gt = plan.gt;
