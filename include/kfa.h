@@ -331,9 +331,10 @@ int kfa_cache_append(const KfaCache* cache, const KfaTensor4* k, const KfaTensor
  * of K / V head g. Row i stands at position lengths[b] + i (appended before this call) and sees positions up to its own; its
  * weights are exp2((q k - m) * scale * log2 e - log2 l) with m, log2 l from stats, fp32 [B, H, 2, T] contiguous (a row with m =
  * +inf gives none). weights: fp32, last dim contiguous, strides in floats, `room` positions; add = 0 writes all `room` of them
- * (0 behind the last row), add = 1 touches the positions that rows see only. */
+ * (0 behind the last row), add = 1 touches the positions that rows see only. scratch: kfa_cache_weigh_bytes bytes, as above. */
+int64_t kfa_cache_weigh_bytes(const KfaTensor4* q, const KfaCache* cache, const KfaRows* rows);
 int kfa_cache_weigh(const KfaTensor4* q, const float* stats, const KfaCache* cache, const KfaRows* rows, float* weights,
-                    const int64_t* weights_stride, int64_t room, int add, float scale, int dtype, int* dev_status, void* stream);
+                    const int64_t* weights_stride, int64_t room, int add, void* scratch, float scale, int dtype, int* dev_status, void* stream);
 
 /* Each (sequence, K / V head) of `cache` keeps min(lengths[b], keep) positions: the `recent` newest and of the others those of the largest
  * weights (fp32 [B, Hkv, >= capacity], strides in floats; of equal ones the lower position; NaN counts as largest). They are

@@ -59,6 +59,7 @@ SYMBOLS = (
     "kfa_cache_attend_bytes",
     "kfa_cache_attend",
     "kfa_cache_append",
+    "kfa_cache_weigh_bytes",
     "kfa_cache_weigh",
     "kfa_cache_evict",
 )
@@ -190,11 +191,13 @@ def load() -> ctypes.CDLL:
         lib.kfa_cache_attend_bytes.argtypes = [T, C, T]
         lib.kfa_cache_attend.argtypes = [T, C, T, T, vp, I64P, ip, T, fp, vp, f32, i32, ip, vp]
         lib.kfa_cache_append.argtypes = [C, T, T, R, ip, vp]
-        lib.kfa_cache_weigh.argtypes = [T, fp, C, R, fp, I64P, i64, i32, f32, i32, ip, vp]
+        lib.kfa_cache_weigh_bytes.restype = ctypes.c_int64
+        lib.kfa_cache_weigh_bytes.argtypes = [T, C, R]
+        lib.kfa_cache_weigh.argtypes = [T, fp, C, R, fp, I64P, i64, i32, vp, f32, i32, ip, vp]
         lib.kfa_cache_evict.argtypes = [C, fp, I64P, i64, i64, C, fp, ip, ip, i32, ip, vp]
         for name in SYMBOLS:
             if name not in ("kfa_abi_version", "kfa_last_error", "kfa_bwd_stats_bytes", "kfa_bwd_dq_acc_bytes", "kfa_bwd_parts_bytes",
-                            "kfa_cache_attend_bytes"):  # fmt: skip
+                            "kfa_cache_attend_bytes", "kfa_cache_weigh_bytes"):  # fmt: skip
                 getattr(lib, name).restype = ctypes.c_int
         if lib.kfa_abi_version() != ABI_VERSION:
             raise KfaError(f"libkfa ABI {lib.kfa_abi_version()} != expected {ABI_VERSION}: rebuild")
@@ -207,7 +210,8 @@ HOST_SYMBOLS = (
     "kfa_last_error", "kfa_fwd", "kfa_bwd", "kfa_bwd_fused", "kfa_fwd_masked", "kfa_bwd_masked", "kfa_fwd_varlen",
     "kfa_bwd_varlen", "kfa_pack_mask", "kfa_fwd_narrow", "kfa_bwd_narrow",
     "kfa_bwd_parts_bytes", "kfa_bwd_parts_count", "kfa_bwd_parts", "kfa_varlen_zero_rows",
-    "kfa_cache_attend_bytes", "kfa_cache_attend", "kfa_cache_append", "kfa_cache_weigh", "kfa_cache_evict",
+    "kfa_cache_attend_bytes", "kfa_cache_attend", "kfa_cache_append", "kfa_cache_weigh_bytes", "kfa_cache_weigh",
+    "kfa_cache_evict",
 )  # fmt: skip
 HOST_PATH = Path(__file__).resolve().parent / "_kfa_host.so"
 _host = None

@@ -31,7 +31,7 @@ SHARED = [CSRC / "kfa_ptx.cuh", CSRC / "kfa_call.cuh", PKG.parent / "include" / 
 SOURCES = {
     CSRC / "kfa_api.cu": SHARED
     + [CSRC / f"kfa_{part}.cuh" for part in ("fwd", "bwd", "bwd_fused", "selftest", "cp", "mask", "scores")],
-    CSRC / "kfa_cache.cu": SHARED + [CSRC / "kfa_cache.cuh", CSRC / "kfa_attend.cuh"],
+    CSRC / "kfa_cache.cu": SHARED + [CSRC / "kfa_cache.cuh", CSRC / "kfa_attend.cuh", CSRC / "kfa_weigh.cuh"],
 }
 OBJECTS = CSRC / "build"
 NVCC_FLAGS = [

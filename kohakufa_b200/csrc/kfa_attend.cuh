@@ -58,6 +58,7 @@ struct AttendParams {
   int extra;       // units that an item counts more than it has
   int box;         // rows of a page's TMA box
   int rows;        // of scratch per part
+  int appended;    // the new tokens are in the cache already (cache_weights): positions lengths .. lengths + counts - 1
   float c_log2, slack;  // scale * log2 e; how far a maximum may grow before O is rescaled
   float* part_o;   // [slot][rows][128]
   float* part_ml;  // [slot][3][rows]: m, l, largest score
@@ -73,6 +74,7 @@ struct Walk {
   __device__ __forceinline__ static void size(const AttendParams& p, int b, int& len, int& count, int& uc, int& ud) {
     len = cache_length(p.c, b);
     count = p.counts ? min(max(p.counts[b], 0), p.T) : p.T;
+    if (p.appended) len = count ? min(len + count, p.c.capacity) : 0;
     uc = count ? (len + ATT_UNIT - 1) / ATT_UNIT : 0;
     ud = count && p.k ? (count + ATT_UNIT - 1) / ATT_UNIT : 0;
   }
@@ -110,25 +112,13 @@ struct Walk {
   __device__ __forceinline__ bool ends() const { return unit + n == units; }
 };
 
-// Which work is this CTA's (all its threads; s_i: 32 ints of shared memory). Synchronises the CTA. chunk, end: units per CTA and where this
-// one's stretch ends, both as they are counted.
-__device__ __forceinline__ bool my_work(const AttendParams& p, int* s_i, Walk& w, int& chunk, int& end) {
+// Shares out the whole batch's work, counted(b) of it sequence b's (0 or more), equally: at[0] .. at[1] is this CTA's stretch, found(i, b, off,
+// counted(b)) is called by one thread for each of the two ends that lies inside sequence b, off into it. All threads of the CTA; s_i: 32 ints of
+// shared memory, of which the first 8 are found's. Returns the length of a stretch.
+template <typename F, typename G>
+__device__ __forceinline__ int att_share(const AttendParams& p, int* s_i, F counted, int (&at)[2], int& total, G found) {
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  chunk = end = 0;
-  if (p.whole) {
-    const unsigned all = static_cast<unsigned>(p.c.batch) * p.items;
-    const unsigned i0 = p.by_grid.div(static_cast<unsigned>(all)) * blockIdx.x + min(blockIdx.x, all - p.by_grid.div(all) * gridDim.x);
-    const unsigned i1 = i0 + p.by_grid.div(all) + (blockIdx.x < all - p.by_grid.div(all) * gridDim.x ? 1 : 0);
-    w.b = static_cast<int>(p.by_items.div(i0));
-    w.item = static_cast<int>(i0 - w.b * p.items);
-    w.end_b = static_cast<int>(p.by_items.div(i1));
-    w.end_item = static_cast<int>(i1 - w.end_b * p.items);
-    w.unit = w.end_unit = 0;
-    __syncthreads();
-    return w.start(p);
-  }
-  // the whole batch, 384 sequences at a time; then the sequences in which this CTA's stretch begins and ends
-  auto counted = [&](int b) { return b < p.c.batch ? (Walk::units_of(p, b) + p.extra) * p.items : 0; };
+  auto of = [&](int b) { return b < p.c.batch ? counted(b) : 0; };
   auto warp_scan = [&](int x) {
 #pragma unroll
     for (int off = 1; off < 32; off <<= 1) {
@@ -137,20 +127,22 @@ __device__ __forceinline__ bool my_work(const AttendParams& p, int* s_i, Walk& w
     }
     return x;
   };
-  int total = 0;
-  const int own0 = counted(tid), scan0 = warp_scan(own0);
+  // 384 sequences at a time; then the sequences in which this CTA's stretch begins and ends
+  total = 0;
+  const int own0 = of(tid), scan0 = warp_scan(own0);
   for (int b0 = 0; b0 < p.c.batch; b0 += ATT_THREADS) {
-    const int s = b0 == 0 ? scan0 : warp_scan(counted(b0 + tid));
+    const int s = b0 == 0 ? scan0 : warp_scan(of(b0 + tid));
     if (b0 > 0) __syncthreads();
     if (lane == 31) s_i[8 + warp] = s;
     __syncthreads();
     for (int i = 0; i < ATT_THREADS / 32; ++i) total += s_i[8 + i];
   }
-  chunk = max(static_cast<int>(p.by_grid.div(total + gridDim.x - 1)), p.least);
-  const long long at[2] = {static_cast<long long>(chunk) * blockIdx.x, static_cast<long long>(chunk) * (blockIdx.x + 1)};
+  const int chunk = max(static_cast<int>(p.by_grid.div(total + gridDim.x - 1)), p.least);
+  at[0] = chunk * static_cast<int>(blockIdx.x);
+  at[1] = at[0] + chunk;
   int before = 0;
   for (int b0 = 0; b0 < p.c.batch; b0 += ATT_THREADS) {
-    const int own = b0 == 0 ? own0 : counted(b0 + tid);
+    const int own = b0 == 0 ? own0 : of(b0 + tid);
     int upto = b0 == 0 ? scan0 : warp_scan(own);
     if (p.c.batch > ATT_THREADS) {
       __syncthreads();
@@ -165,17 +157,37 @@ __device__ __forceinline__ bool my_work(const AttendParams& p, int* s_i, Walk& w
     }
     upto += before;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      if (at[i] >= upto - own && at[i] < upto) {  // (one thread's sequence)
-        const int off = static_cast<int>(at[i]) - (upto - own), each = own / p.items, item = off / each;
-        s_i[3 * i] = b0 + tid;
-        s_i[3 * i + 1] = item;
-        s_i[3 * i + 2] = max(off - item * each - p.extra, 0);
-      }
-    }
+    for (int i = 0; i < 2; ++i)
+      if (at[i] >= upto - own && at[i] < upto) found(i, b0 + tid, at[i] - (upto - own), own);
     before += all;
   }
   __syncthreads();
+  return chunk;
+}
+
+// Which work is this CTA's (all its threads; s_i: 32 ints of shared memory). Synchronises the CTA. chunk, end: units per CTA and where this
+// one's stretch ends, both as they are counted.
+__device__ __forceinline__ bool my_work(const AttendParams& p, int* s_i, Walk& w, int& chunk, int& end) {
+  chunk = end = 0;
+  if (p.whole) {
+    const unsigned all = static_cast<unsigned>(p.c.batch) * p.items;
+    const unsigned i0 = p.by_grid.div(static_cast<unsigned>(all)) * blockIdx.x + min(blockIdx.x, all - p.by_grid.div(all) * gridDim.x);
+    const unsigned i1 = i0 + p.by_grid.div(all) + (blockIdx.x < all - p.by_grid.div(all) * gridDim.x ? 1 : 0);
+    w.b = static_cast<int>(p.by_items.div(i0));
+    w.item = static_cast<int>(i0 - w.b * p.items);
+    w.end_b = static_cast<int>(p.by_items.div(i1));
+    w.end_item = static_cast<int>(i1 - w.end_b * p.items);
+    w.unit = w.end_unit = 0;
+    __syncthreads();
+    return w.start(p);
+  }
+  int at[2], total;
+  chunk = att_share(p, s_i, [&](int b) { return (Walk::units_of(p, b) + p.extra) * p.items; }, at, total, [&](int i, int b, int off, int own) {
+    const int each = own / p.items, item = off / each;
+    s_i[3 * i] = b;
+    s_i[3 * i + 1] = item;
+    s_i[3 * i + 2] = max(off - item * each - p.extra, 0);
+  });
   const bool inside[2] = {at[0] < total, at[1] < total};
   w.b = inside[0] ? s_i[0] : p.c.batch;
   w.item = inside[0] ? s_i[1] : 0;
@@ -183,7 +195,7 @@ __device__ __forceinline__ bool my_work(const AttendParams& p, int* s_i, Walk& w
   w.end_b = inside[1] ? s_i[3] : p.c.batch;
   w.end_item = inside[1] ? s_i[4] : 0;
   w.end_unit = inside[1] ? s_i[5] : 0;
-  end = static_cast<int>(at[1]);
+  end = at[1];
   return w.b < p.c.batch && w.start(p);
 }
 

@@ -6,6 +6,7 @@
 #include "kfa_attend.cuh"
 #include "kfa_cache.cuh"
 #include "kfa_call.cuh"
+#include "kfa_weigh.cuh"
 
 namespace {
 
@@ -137,14 +138,11 @@ AttendPlan plan_attend(int64_t batch, int64_t heads, int64_t kv_heads, int64_t T
   return a;
 }
 
-template <bool BF16, class R, typename K>
-int launch_attend(K kern, const CUtensorMap (&m)[5], const kfa::AttendParams& p, const AttendPlan& plan, cudaStream_t s) {
-  KFA_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, R::SMEM));
-  kern<<<plan.grid, kfa::ATT_THREADS, R::SMEM, s>>>(m[0], m[1], m[2], m[3], m[4], p);
-  KFA_CUDA(cudaGetLastError());
-  if (plan.whole) return KFA_OK;
+// A kernel (256 threads) that waits itself for the end of the one before it in the stream, and may be launched while that one still runs.
+template <typename... P>
+int launch_early(void (*kern)(P...), dim3 grid, cudaStream_t s, const P&... params) {
   cudaLaunchConfig_t config = {};
-  config.gridDim = dim3(plan.grid, (plan.gt * plan.tt + 7) / 8);
+  config.gridDim = grid;
   config.blockDim = dim3(256);
   config.stream = s;
   cudaLaunchAttribute early[1];
@@ -152,9 +150,21 @@ int launch_attend(K kern, const CUtensorMap (&m)[5], const kfa::AttendParams& p,
   early[0].val.programmaticStreamSerializationAllowed = 1;
   config.attrs = early;
   config.numAttrs = 1;
-  KFA_CUDA(cudaLaunchKernelEx(&config, kfa::kfa_cache_join_kernel<BF16>, p));
+  KFA_CUDA(cudaLaunchKernelEx(&config, kern, params...));
   return KFA_OK;
 }
+
+template <bool BF16, class R, typename K>
+int launch_attend(K kern, const CUtensorMap (&m)[5], const kfa::AttendParams& p, const AttendPlan& plan, cudaStream_t s) {
+  KFA_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, R::SMEM));
+  kern<<<plan.grid, kfa::ATT_THREADS, R::SMEM, s>>>(m[0], m[1], m[2], m[3], m[4], p);
+  KFA_CUDA(cudaGetLastError());
+  if (plan.whole) return KFA_OK;
+  return launch_early(kfa::kfa_cache_join_kernel<BF16>, dim3(plan.grid, (plan.gt * plan.tt + 7) / 8), s, p);
+}
+
+// Rows of a TMA box that a page holds whole numbers of (without a table: the last box may end behind the page, and reads zeros there).
+int page_box(const kfa::CacheView& c) { return c.table ? (c.page % 32 == 0 ? 32 : (c.page % 16 == 0 ? 16 : 8)) : 32; }
 
 template <int NC, bool BF16>
 int launch_attend_rows(const CUtensorMap (&m)[5], const kfa::AttendParams& p, const AttendPlan& plan, cudaStream_t s) {
@@ -165,6 +175,65 @@ int launch_attend_rows(const CUtensorMap (&m)[5], const kfa::AttendParams& p, co
     case 128: return launch_attend<BF16, kfa::AttRowsCfg<NC, 1>>(kfa::kfa_cache_attend_rows_kernel<NC, 1, BF16>, m, p, plan, s);
     default: return launch_attend<BF16, kfa::AttRowsCfg<NC, 2>>(kfa::kfa_cache_attend_rows_kernel<NC, 2, BF16>, m, p, plan, s);
   }
+}
+
+struct WeighPlan {
+  int64_t rows, work, bytes, part_floats, stats_floats;
+  int grid, least, extra, block, blocks, tile_h, tile_t;
+};
+
+WeighPlan plan_weigh(int64_t batch, int64_t heads, int64_t kv_heads, int64_t steps, int64_t capacity, int64_t D, bool index) {
+  WeighPlan w;
+  std::memset(&w, 0, sizeof(w));
+  const int64_t group = heads / kv_heads;
+  w.rows = std::min<int64_t>(group * steps, 1 << 30);
+  if (w.rows <= 64) {
+    const int64_t units = (capacity + 31) / 32;
+    w.extra = 8;
+    w.least = 4;
+    w.work = batch * kv_heads * (units + w.extra);
+    w.grid = static_cast<int>(std::min<int64_t>(SMS, (batch * kv_heads * units + 3) / 4));
+    return w;
+  }
+  w.tile_h = static_cast<int>(std::min<int64_t>(group, 64));
+  w.tile_t = 64 / w.tile_h;
+  // Blocks of 512 tokens, at most 8 of them: what an SM does is a number of equal items (and what each block adds goes through memory).
+  const int64_t block = std::max<int64_t>(512, (steps + 7) / 8);
+  w.block = static_cast<int>(block);
+  w.blocks = static_cast<int>((steps + block - 1) / block);
+  w.least = 1;
+  w.work = batch * kv_heads * w.blocks * ((capacity + 127) / 128);
+  w.grid = static_cast<int>(std::min<int64_t>(SMS, w.work));
+  w.part_floats = (w.blocks * batch * kv_heads * capacity + 63) / 64 * 64;
+  if (index) w.stats_floats = (2 * batch * heads * steps + 63) / 64 * 64;
+  w.bytes = 4 * (w.part_floats + w.stats_floats) + (index ? 2 * batch * heads * steps * D : 0);
+  return w;
+}
+
+template <class R, typename K>
+int launch_weigh_few(K kern, const CUtensorMap& mk, const kfa::AttendParams& a, const kfa::WeighParams& p, const WeighPlan& plan, cudaStream_t s) {
+  KFA_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, R::SMEM));
+  kern<<<plan.grid, kfa::ATT_THREADS, R::SMEM, s>>>(mk, a, p);
+  KFA_CUDA(cudaGetLastError());
+  return KFA_OK;
+}
+template <int NC, bool BF16>
+int launch_weigh_few(const CUtensorMap& mk, const kfa::AttendParams& a, const kfa::WeighParams& p, const WeighPlan& plan, cudaStream_t s) {
+  if (plan.rows <= 16) return launch_weigh_few<kfa::WeighCfg<NC, 16>>(kfa::kfa_cache_weigh_kernel<NC, 16, BF16>, mk, a, p, plan, s);
+  if (plan.rows <= 32) return launch_weigh_few<kfa::WeighCfg<NC, 32>>(kfa::kfa_cache_weigh_kernel<NC, 32, BF16>, mk, a, p, plan, s);
+  return launch_weigh_few<kfa::WeighCfg<NC, 64>>(kfa::kfa_cache_weigh_kernel<NC, 64, BF16>, mk, a, p, plan, s);
+}
+
+template <int NC, bool BF16>
+int launch_weigh_many(const CUtensorMap& mq, const CUtensorMap& mk, const kfa::AttendParams& a, const kfa::WeighParams& p, const WeighPlan& plan,
+                      cudaStream_t s) {
+  using R = kfa::WeighRowsCfg<NC>;
+  auto kern = kfa::kfa_cache_weigh_rows_kernel<NC, BF16>;
+  KFA_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, R::SMEM));
+  kern<<<plan.grid, kfa::ATT_THREADS, R::SMEM, s>>>(mq, mk, a, p);
+  KFA_CUDA(cudaGetLastError());
+  const dim3 grid(static_cast<unsigned>(std::min<int64_t>((p.room + 255) / 256, 256)), a.c.heads, a.c.batch);
+  return launch_early(kfa::kfa_cache_sum_blocks_kernel, grid, s, a, p);
 }
 
 }  // namespace
@@ -229,7 +298,7 @@ int kfa_cache_attend(const KfaTensor4* q, const KfaCache* cache, const KfaTensor
   p.least = plan.least;
   p.extra = plan.extra;
   p.rows = plan.rows;
-  p.box = p.c.table ? (p.c.page % 32 == 0 ? 32 : (p.c.page % 16 == 0 ? 16 : 8)) : 32;
+  p.box = page_box(p.c);
   if (!plan.whole) {
     uint8_t* at = static_cast<uint8_t*>(scratch);
     p.part_meta = reinterpret_cast<int4*>(at);
@@ -281,34 +350,98 @@ int kfa_cache_append(const KfaCache* cache, const KfaTensor4* k, const KfaTensor
   return KFA_OK;
 }
 
+int64_t kfa_cache_weigh_bytes(const KfaTensor4* q, const KfaCache* cache, const KfaRows* rows) {
+  if (!q || !cache || !rows) return 0;
+  const int64_t page = cache->k.shape[2], kv_heads = cache->k.shape[1];
+  if (q->shape[1] < kv_heads || kv_heads < 1 || rows->steps < 1) return 0;  // (refused by the call)
+  return plan_weigh(cache->batch, q->shape[1], kv_heads, rows->steps, cache->table ? cache->table_cols * page : page, cache->k.shape[3],
+                    rows->index != nullptr)
+      .bytes;
+}
+
 int kfa_cache_weigh(const KfaTensor4* q, const float* stats, const KfaCache* cache, const KfaRows* rows, float* weights,
-                    const int64_t* weights_stride, int64_t room, int add, float scale, int dtype, int* dev_status, void* stream) {
+                    const int64_t* weights_stride, int64_t room, int add, void* scratch, float scale, int dtype, int* dev_status,
+                    void* stream) {
+  kfa::AttendParams a;
   kfa::WeighParams p;
+  std::memset(&a, 0, sizeof(a));
   std::memset(&p, 0, sizeof(p));
   int rc;
-  if ((rc = check_cache(cache, &p.c)) || (rc = check_new(q, p.c, 0, "q")) || (rc = check_rows(rows, q->shape[2], &p.r)) ||
+  if ((rc = check_cache(cache, &a.c)) || (rc = check_new(q, a.c, 0, "q")) || (rc = check_rows(rows, q->shape[2], &p.r)) ||
       (rc = check_scale(scale)) || (rc = check_dtype(dtype)))
     return rc;
   if (!stats || !weights || !weights_stride || !dev_status) return fail(KFA_ERR_ARG, "kfa_cache_weigh: null pointer");
-  if (room < p.c.capacity || room > 0x7fff0000) return fail(KFA_ERR_ARG, "weights: at least the cache's %d positions", p.c.capacity);
+  if (room < a.c.capacity || room > 0x7fff0000) return fail(KFA_ERR_ARG, "weights: at least the cache's %d positions", a.c.capacity);
+  const int64_t D = a.c.cols;
+  a.H = static_cast<int>(q->shape[1]);
+  a.group = a.H / a.c.heads;
+  a.T = p.r.steps;
+  a.counts = p.r.counts;
+  a.appended = 1;
+  a.c_log2 = std::max(scale * LOG2E, 1e-30f);  // (see kfa_cache_attend)
+  a.status = dev_status;
+  a.row_tiles = a.head_tiles = 1;
+  a.items = a.c.heads;
+  a.gt = a.group;
+  a.by_gt = kfa::FastDiv::by(a.gt);
+  a.by_items = kfa::FastDiv::by(a.items);
+  a.by_row_tiles = a.by_head_tiles = kfa::FastDiv::by(1);
+  a.box = page_box(a.c);
   p.q = static_cast<const uint8_t*>(q->ptr);
   p.q_sb = 2 * q->stride[0], p.q_sh = 2 * q->stride[1], p.q_ss = 2 * q->stride[2];
   p.stats = stats;
   p.w = weights;
   p.w_sb = weights_stride[0];
   p.w_sh = weights_stride[1];
-  p.H = static_cast<int>(q->shape[1]);
-  p.group = p.H / p.c.heads;
   p.room = static_cast<int>(room);
   p.add = add != 0;
-  p.scale_log2 = scale * LOG2E;
-  p.status = dev_status;
-  const dim3 grid(static_cast<unsigned>((room + 127) / 128), p.c.heads, p.c.batch);
+  p.by_piece = kfa::FastDiv::by(static_cast<uint32_t>(D / 8));
+  const WeighPlan plan = plan_weigh(a.c.batch, a.H, a.c.heads, p.r.steps, a.c.capacity, D, p.r.index != nullptr);
+  if (plan.work > 0x3fffffff) return fail(KFA_ERR_ARG, "too many rows in one call");
+  if (plan.bytes && (!scratch || reinterpret_cast<uintptr_t>(scratch) % 16)) return fail(KFA_ERR_ARG, "scratch: null or not 16-byte aligned");
+  a.by_grid = kfa::FastDiv::by(plan.grid);
+  a.least = plan.least;
+  a.extra = plan.extra;
+  CUtensorMap mk, mq;
+  const KfaTensor4* ck = &cache->k;
+  if ((rc = make_box_map(ck->ptr, D, ck->shape[2], ck->stride[2], ck->shape[1], ck->stride[1], ck->shape[0], ck->stride[0], a.box, 1, dtype, &mk,
+                         "cache keys")))
+    return rc;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (dtype == KFA_BF16) kfa::kfa_cache_weigh_simple_kernel<true><<<grid, 128, 0, s>>>(p);
-  else kfa::kfa_cache_weigh_simple_kernel<false><<<grid, 128, 0, s>>>(p);
-  KFA_CUDA(cudaGetLastError());
-  return KFA_OK;
+  if (plan.rows <= 64) {
+    if (dtype == KFA_BF16) return D > 64 ? launch_weigh_few<2, true>(mk, a, p, plan, s) : launch_weigh_few<1, true>(mk, a, p, plan, s);
+    return D > 64 ? launch_weigh_few<2, false>(mk, a, p, plan, s) : launch_weigh_few<1, false>(mk, a, p, plan, s);
+  }
+  p.block = plan.block;
+  p.blocks = plan.blocks;
+  p.tile_h = plan.tile_h;
+  p.tile_t = plan.tile_t;
+  p.head_tiles = (a.group + p.tile_h - 1) / p.tile_h;
+  p.by_tile_h = kfa::FastDiv::by(p.tile_h);
+  p.part = static_cast<float*>(scratch);
+  KfaTensor4 rows_q = *q;
+  if (p.r.index) {
+    p.stats_to = p.part + plan.part_floats;
+    p.q_to = reinterpret_cast<uint8_t*>(p.stats_to + plan.stats_floats);
+    const int64_t total = static_cast<int64_t>(a.c.batch) * p.r.steps * a.H * (D / 8);
+    if (total > 0xffffff00ll) return fail(KFA_ERR_ARG, "too many rows in one call");
+    kfa::kfa_cache_take_rows_kernel<<<static_cast<unsigned>((total + 255) / 256), 256, 0, s>>>(
+        a, p, p.by_piece, kfa::FastDiv::by(a.H), kfa::FastDiv::by(p.r.steps), static_cast<unsigned>(total));
+    KFA_CUDA(cudaGetLastError());
+    rows_q.ptr = p.q_to;
+    rows_q.shape[2] = p.r.steps;
+    rows_q.stride[2] = a.H * D;
+    rows_q.stride[1] = D;
+    rows_q.stride[0] = static_cast<int64_t>(p.r.steps) * a.H * D;
+    p.stats = p.stats_to;
+    p.r.index = nullptr;
+    p.r.T = p.r.steps;
+  }
+  if ((rc = make_box_map(rows_q.ptr, D, a.H, rows_q.stride[1], rows_q.shape[2], rows_q.stride[2], a.c.batch, rows_q.stride[0], p.tile_h, p.tile_t,
+                         dtype, &mq, "q")))
+    return rc;
+  if (dtype == KFA_BF16) return D > 64 ? launch_weigh_many<2, true>(mq, mk, a, p, plan, s) : launch_weigh_many<1, true>(mq, mk, a, p, plan, s);
+  return D > 64 ? launch_weigh_many<2, false>(mq, mk, a, p, plan, s) : launch_weigh_many<1, false>(mq, mk, a, p, plan, s);
 }
 
 int kfa_cache_evict(const KfaCache* cache, const float* weights, const int64_t* weights_stride, int64_t keep, int64_t recent,

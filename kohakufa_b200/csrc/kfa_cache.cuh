@@ -1,5 +1,4 @@
-// A cache of keys and values in pages, and the operators of generation on it: attention of new tokens, append, accumulated
-// attention weights, eviction.
+// A cache of keys and values in pages, and what copies on it: append, eviction. (Attention: kfa_attend.cuh; accumulated weights: kfa_weigh.cuh.)
 #pragma once
 
 #include "kfa_ptx.cuh"
@@ -76,60 +75,6 @@ __global__ void __launch_bounds__(256) kfa_cache_append_kernel(const AppendParam
   const uint4 v = *reinterpret_cast<const uint4*>(p.v + b * p.v_sb + g * p.v_sh + t * p.v_ss + 16 * piece);
   *reinterpret_cast<uint4*>(p.c.k + page * p.c.k_sn + g * p.c.k_sh + slot * p.c.k_ss + 16 * piece) = k;
   *reinterpret_cast<uint4*>(p.c.v + page * p.c.v_sn + g * p.c.v_sh + slot * p.c.v_ss + 16 * piece) = v;
-}
-
-// ---- accumulated weights -------------------------------------------------------------------------------------------------
-struct WeighParams {
-  CacheView c;
-  RowsView r;
-  const uint8_t* q;
-  long long q_sb, q_sh, q_ss;  // bytes
-  const float* stats;
-  float* w;
-  long long w_sb, w_sh;
-  int H, group, room, add;
-  float scale_log2;
-  int* status;
-};
-
-// A thread per position; the rows one after the other, each from shared memory.
-template <bool BF16>
-__global__ void __launch_bounds__(128) kfa_cache_weigh_simple_kernel(const WeighParams p) {
-  const int b = blockIdx.z, g = blockIdx.y, pos = blockIdx.x * 128 + threadIdx.x, cols = p.c.cols;
-  const int count = p.r.count(b), len = p.c.lengths[b];
-  __shared__ float s_q[128], s_m, s_l;
-  int page = 0, slot = 0;
-  bool bad = count > 0 && (len < 0 || static_cast<long long>(len) + count > p.c.capacity);
-  const int seen = bad ? 0 : (count > 0 ? len + count : 0);
-  if (pos < seen && !cache_place(p.c, b, pos, page, slot)) bad = true;
-  const uint8_t* k = p.c.k + page * p.c.k_sn + g * p.c.k_sh + slot * p.c.k_ss;
-  float w = 0.f;
-  for (int i = 0; i < count; ++i) {
-    const int t = p.r.row(b, i);
-    if (t < 0 || t >= p.r.T) {
-      bad = true;
-      continue;
-    }
-    for (int h = g * p.group; h < (g + 1) * p.group; ++h) {
-      __syncthreads();
-      if (threadIdx.x < cols) s_q[threadIdx.x] = load16<BF16>(p.q + b * p.q_sb + h * p.q_sh + t * p.q_ss + 2 * threadIdx.x);
-      if (threadIdx.x == 0) {
-        const float* at = p.stats + (static_cast<long long>(b) * p.H + h) * 2 * p.r.T + t;
-        s_m = at[0];
-        s_l = at[p.r.T];
-      }
-      __syncthreads();
-      if (pos >= seen || pos > len + i || bad || s_m == INFINITY) continue;
-      float s = 0.f;
-      for (int d = 0; d < cols; ++d) s += s_q[d] * load16<BF16>(k + 2 * d);
-      w += ex2((s - s_m) * p.scale_log2 - s_l);
-    }
-  }
-  bad = __syncthreads_or(bad);
-  if (bad && threadIdx.x == 0) report(p.status, DEV_BAD_CACHE);
-  if (pos >= p.room || (p.add && pos >= seen && !bad)) return;
-  float* at = p.w + b * p.w_sb + g * p.w_sh + pos;
-  *at = bad ? __int_as_float(0x7fc00000) : (p.add ? *at + w : w);
 }
 
 // ---- eviction ------------------------------------------------------------------------------------------------------------

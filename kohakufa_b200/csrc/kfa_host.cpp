@@ -49,6 +49,7 @@ struct Api {
   decltype(&kfa_cache_attend_bytes) cache_attend_bytes = nullptr;
   decltype(&kfa_cache_attend) cache_attend = nullptr;
   decltype(&kfa_cache_append) cache_append = nullptr;
+  decltype(&kfa_cache_weigh_bytes) cache_weigh_bytes = nullptr;
   decltype(&kfa_cache_weigh) cache_weigh = nullptr;
   decltype(&kfa_cache_evict) cache_evict = nullptr;
 } api;
@@ -840,8 +841,11 @@ PyObject* py_cache_weights(Args a, Py_ssize_t n) {
     const KfaCache dc = cache_desc(c);
     const KfaTensor4 dq = desc(q);
     const int64_t stride[2] = {w.stride(0), w.stride(1)};
+    const int64_t bytes = api.cache_weigh_bytes(&dq, &dc, &rows);
+    const at::Tensor scratch = bytes ? floats(q, {(bytes + 3) / 4}) : at::Tensor();
     check(api.cache_weigh(&dq, stats.data_ptr<float>(), &dc, &rows, w.data_ptr<float>(), stride, w.size(2), add,
-                          static_cast<float>(scale), dtype_code(q), status.data_ptr<int32_t>(), stream_of(q)));
+                          bytes ? scratch.data_ptr() : nullptr, static_cast<float>(scale), dtype_code(q), status.data_ptr<int32_t>(),
+                          stream_of(q)));
     return 0;
   });
   w.unsafeGetTensorImpl()->bump_version();
@@ -911,6 +915,7 @@ PyObject* py_bind(Args a, Py_ssize_t n) {
   take("kfa_cache_attend_bytes", api.cache_attend_bytes);
   take("kfa_cache_attend", api.cache_attend);
   take("kfa_cache_append", api.cache_append);
+  take("kfa_cache_weigh_bytes", api.cache_weigh_bytes);
   take("kfa_cache_weigh", api.cache_weigh);
   take("kfa_cache_evict", api.cache_evict);
   Py_INCREF(a[0]);
