@@ -477,9 +477,8 @@ int kfa_cache_evict(const KfaCache* cache, const float* weights, const int64_t* 
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   kfa::kfa_cache_select_kernel<<<dim3(p.c.heads, p.c.batch), kfa::SELECT_THREADS, 0, s>>>(p);
   KFA_CUDA(cudaGetLastError());
-  kfa::kfa_cache_gather_kernel<<<static_cast<unsigned>((total + 255) / 256), 256, 0, s>>>(p);
-  KFA_CUDA(cudaGetLastError());
-  return KFA_OK;
+  const long long per = 256ll * kfa::GATHER_ROWS;
+  return launch_early(kfa::kfa_cache_gather_kernel, dim3(static_cast<unsigned>((total + per - 1) / per)), s, p);
 }
 
 }  // extern "C"

@@ -100,12 +100,14 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
   return (u & 0x80000000u) ? ~u : u | 0x80000000u;
 }
 
-// Which positions stay, per (sequence, K / V head). The key of the last one that stays is found digit by digit (8 bits, from the
-// top): a histogram of the digit among the positions that agree in the digits before it. Then one pass in ascending order: all
-// above that key stay, of those equal to it the first ones, until there are enough.
+// Which positions stay, per (sequence, K / V head). The key of the last one that stays is found digit by digit (11, 11 and 10 bits, from the
+// top): a histogram of the digit among the positions that agree in the digits before it. It ends early when all that agree stay. Then every
+// warp takes a stretch of the positions, counts those above that key and those equal to it, and lists them in ascending order: all above it
+// stay, of the equal ones the first, until there are enough. Bound by latency: 16 positions a thread at 8192, read from L1 after the first time.
 __global__ void __launch_bounds__(SELECT_THREADS) kfa_cache_select_kernel(const EvictParams p) {
+  constexpr int WARPS = SELECT_THREADS / 32, BINS = 2048, PER = BINS / SELECT_THREADS;
   const int g = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  __shared__ int hist[256], warp_gt[SELECT_THREADS / 32], warp_eq[SELECT_THREADS / 32], s_digit, s_need;
+  __shared__ int hist[BINS], warp_gt[WARPS], warp_eq[WARPS], s_digit, s_need, s_all;
   const int len = cache_length(p.c, b);
   if (tid == 0 && !length_ok(p.c, b)) report(p.status, DEV_BAD_CACHE);
   const float* w = p.w + b * p.w_sb + g * p.w_sh;
@@ -133,74 +135,128 @@ __global__ void __launch_bounds__(SELECT_THREADS) kfa_cache_select_kernel(const 
   if (want == 0) return;
   uint32_t prefix = 0, mask = 0;
   int need = want;
-  for (int shift = 24; shift >= 0; shift -= 8) {
-    for (int i = tid; i < 256; i += SELECT_THREADS) hist[i] = 0;
+  for (int shift = 21;; shift = shift == 21 ? 10 : 0) {
+    const uint32_t digits = shift == 0 ? 1023u : 2047u;
+    for (int i = tid; i < BINS; i += SELECT_THREADS) hist[i] = 0;
     __syncthreads();
-    for (int i = tid; i < old; i += SELECT_THREADS) {
-      const uint32_t key = weight_key(w[i]);
-      if ((key & mask) == prefix) atomicAdd(&hist[(key >> shift) & 255u], 1);
+#pragma unroll 4
+    for (int i0 = 0; i0 < old; i0 += SELECT_THREADS) {
+      const int i = i0 + tid;
+      const uint32_t key = i < old ? weight_key(w[i]) : 0u;
+      const bool in = i < old && (key & mask) == prefix;
+      const uint32_t digit = (key >> shift) & digits;
+      // (many equal weights: one addition a warp)
+      const unsigned act = __ballot_sync(0xffffffffu, in);
+      const uint32_t lead = __shfl_sync(0xffffffffu, digit, act ? __ffs(act) - 1 : 0);
+      if (__all_sync(0xffffffffu, !in || digit == lead)) {
+        if (act != 0 && lane == 0) atomicAdd(&hist[lead], __popc(act));
+      } else if (in) {
+        atomicAdd(&hist[digit], 1);
+      }
     }
     __syncthreads();
-    if (tid == 0) {
-      int d = 255, above = 0;
-      while (above + hist[d] < need) above += hist[d--];
-      s_digit = d;
-      s_need = need - above;
+    // bins from the top, PER a thread: in whose are the last ones that are needed?
+    int mine = 0, upto;
+#pragma unroll
+    for (int k = 0; k < PER; ++k) mine += hist[BINS - 1 - (PER * tid + k)];
+    upto = mine;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+      const int up = __shfl_up_sync(0xffffffffu, upto, off);
+      if (lane >= off) upto += up;
+    }
+    if (lane == 31) warp_gt[warp] = upto;
+    __syncthreads();
+    for (int o = 0; o < warp; ++o) upto += warp_gt[o];
+    int above = upto - mine;
+    if (above < need && upto >= need) {
+#pragma unroll
+      for (int k = 0; k < PER; ++k) {
+        const int n = hist[BINS - 1 - (PER * tid + k)];
+        if (above < need && above + n >= need) {
+          s_digit = BINS - 1 - (PER * tid + k);
+          s_need = need - above;
+          s_all = n == need - above;
+        }
+        above += n;
+      }
     }
     __syncthreads();
     need = s_need;
     prefix |= static_cast<uint32_t>(s_digit) << shift;
-    mask |= 255u << shift;
-    __syncthreads();
+    mask |= digits << shift;
+    if (s_all || shift == 0) break;
   }
-  int done_gt = 0, done_eq = 0;  // before this stretch of positions
-  for (int i0 = 0; i0 < old; i0 += SELECT_THREADS) {
-    const int i = i0 + tid;
-    const float x = i < old ? w[i] : 0.f;
-    const uint32_t key = weight_key(x);
-    const bool gt = i < old && key > prefix, eq = i < old && key == prefix;
+  // (above the prefix and equal to it in the digits looked at; where all that are equal stay, the other digits do not matter)
+  const int stretch = (old + 32 * WARPS - 1) / (32 * WARPS) * 32, i_first = warp * stretch, i_last = min(i_first + stretch, old);
+  int gts = 0, eqs = 0;
+#pragma unroll 4
+  for (int i0 = i_first; i0 < i_last; i0 += 32) {
+    const uint32_t key = i0 + lane < i_last ? weight_key(w[i0 + lane]) & mask : 0u;
+    gts += __popc(__ballot_sync(0xffffffffu, i0 + lane < i_last && key > prefix));
+    eqs += __popc(__ballot_sync(0xffffffffu, i0 + lane < i_last && key == prefix));
+  }
+  __syncthreads();
+  if (lane == 0) warp_gt[warp] = gts, warp_eq[warp] = eqs;
+  __syncthreads();
+  gts = eqs = 0;
+  for (int o = 0; o < warp; ++o) gts += warp_gt[o], eqs += warp_eq[o];
+  const unsigned below = (1u << lane) - 1u;
+#pragma unroll 2
+  for (int i0 = i_first; i0 < i_last; i0 += 32) {
+    const int i = i0 + lane;
+    const float x = i < i_last ? w[i] : 0.f;
+    const uint32_t key = weight_key(x) & mask;
+    const bool gt = i < i_last && key > prefix, eq = i < i_last && key == prefix;
     const unsigned bg = __ballot_sync(0xffffffffu, gt), be = __ballot_sync(0xffffffffu, eq);
-    if (lane == 0) warp_gt[warp] = __popc(bg), warp_eq[warp] = __popc(be);
-    __syncthreads();
-    int gts = done_gt, eqs = done_eq;
-    for (int o = 0; o < SELECT_THREADS / 32; ++o) {
-      if (o < warp) gts += warp_gt[o], eqs += warp_eq[o];
-      done_gt += warp_gt[o];
-      done_eq += warp_eq[o];
-    }
-    const unsigned below = (1u << lane) - 1u;
-    gts += __popc(bg & below);
-    eqs += __popc(be & below);
-    if (gt || (eq && eqs < need)) {
-      const int at = gts + min(eqs, need);
+    const int my_eq = eqs + __popc(be & below);
+    if (gt || (eq && my_eq < need)) {
+      const int at = gts + __popc(bg & below) + min(my_eq, need);
       kept[at] = i;
       w_out[at] = x;
     }
-    __syncthreads();
+    gts += __popc(bg);
+    eqs += __popc(be);
   }
 }
 
-// Moves the rows that stay: a thread 16 bytes of a key and of its value.
+// Moves the rows that stay: a thread 16 bytes of a key and of its value, of GATHER_ROWS rows far apart, whose loads are in flight together.
+constexpr int GATHER_ROWS = 4;
 __global__ void __launch_bounds__(256) kfa_cache_gather_kernel(const EvictParams p) {
-  const unsigned at = blockIdx.x * 256u + threadIdx.x;
-  if (at >= p.total) return;
-  const unsigned row = p.by_piece.div(at), piece = at - row * p.by_piece.d;
-  const unsigned rest = p.by_head.div(row), g = row - rest * p.by_head.d;
-  const unsigned b = p.by_slot.div(rest), i = rest - b * p.by_slot.d;
-  const int pos = p.kept[(static_cast<long long>(b) * p.c.heads + g) * p.keep + i];
-  if (pos < 0 && !p.clear) return;
-  int page = 0, slot = 0, page_o, slot_o;
-  if ((pos >= 0 && !cache_place(p.c, b, pos, page, slot)) || !cache_place(p.out, b, i, page_o, slot_o)) {
-    report(p.status, DEV_BAD_CACHE);
-    return;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const unsigned step = gridDim.x * 256u;
+  uint4 k[GATHER_ROWS], v[GATHER_ROWS];
+  uint8_t *ko[GATHER_ROWS], *vo[GATHER_ROWS];
+#pragma unroll
+  for (int n = 0; n < GATHER_ROWS; ++n) {
+    const unsigned long long at64 = static_cast<unsigned long long>(n) * step + blockIdx.x * 256u + threadIdx.x;
+    ko[n] = nullptr;
+    if (at64 >= p.total) continue;
+    const unsigned at = static_cast<unsigned>(at64);
+    const unsigned row = p.by_piece.div(at), piece = at - row * p.by_piece.d;
+    const unsigned rest = p.by_head.div(row), g = row - rest * p.by_head.d;
+    const unsigned b = p.by_slot.div(rest), i = rest - b * p.by_slot.d;
+    const int pos = p.kept[(static_cast<long long>(b) * p.c.heads + g) * p.keep + i];
+    if (pos < 0 && !p.clear) continue;
+    int page = 0, slot = 0, page_o, slot_o;
+    if ((pos >= 0 && !cache_place(p.c, b, pos, page, slot)) || !cache_place(p.out, b, i, page_o, slot_o)) {
+      report(p.status, DEV_BAD_CACHE);
+      continue;
+    }
+    k[n] = v[n] = make_uint4(0, 0, 0, 0);
+    if (pos >= 0) {
+      k[n] = *reinterpret_cast<const uint4*>(p.c.k + page * p.c.k_sn + g * p.c.k_sh + slot * p.c.k_ss + 16 * piece);
+      v[n] = *reinterpret_cast<const uint4*>(p.c.v + page * p.c.v_sn + g * p.c.v_sh + slot * p.c.v_ss + 16 * piece);
+    }
+    ko[n] = p.out.k + page_o * p.out.k_sn + g * p.out.k_sh + slot_o * p.out.k_ss + 16 * piece;
+    vo[n] = p.out.v + page_o * p.out.v_sn + g * p.out.v_sh + slot_o * p.out.v_ss + 16 * piece;
   }
-  uint4 k = make_uint4(0, 0, 0, 0), v = k;
-  if (pos >= 0) {
-    k = *reinterpret_cast<const uint4*>(p.c.k + page * p.c.k_sn + g * p.c.k_sh + slot * p.c.k_ss + 16 * piece);
-    v = *reinterpret_cast<const uint4*>(p.c.v + page * p.c.v_sn + g * p.c.v_sh + slot * p.c.v_ss + 16 * piece);
+#pragma unroll
+  for (int n = 0; n < GATHER_ROWS; ++n) {
+    if (ko[n] == nullptr) continue;
+    *reinterpret_cast<uint4*>(ko[n]) = k[n];
+    *reinterpret_cast<uint4*>(vo[n]) = v[n];
   }
-  *reinterpret_cast<uint4*>(p.out.k + page_o * p.out.k_sn + g * p.out.k_sh + slot_o * p.out.k_ss + 16 * piece) = k;
-  *reinterpret_cast<uint4*>(p.out.v + page_o * p.out.v_sn + g * p.out.v_sh + slot_o * p.out.v_ss + 16 * piece) = v;
 }
 
 }  // namespace kfa
