@@ -203,7 +203,7 @@ WeighPlan plan_weigh(int64_t batch, int64_t heads, int64_t kv_heads, int64_t ste
   w.blocks = static_cast<int>((steps + block - 1) / block);
   w.least = 1;
   w.work = batch * kv_heads * w.blocks * ((capacity + 127) / 128);
-  w.grid = static_cast<int>(std::min<int64_t>(SMS, w.work));
+  w.grid = static_cast<int>(std::min<int64_t>(2 * SMS, w.work));
   w.part_floats = (w.blocks * batch * kv_heads * capacity + 63) / 64 * 64;
   if (index) w.stats_floats = (2 * batch * heads * steps + 63) / 64 * 64;
   w.bytes = 4 * (w.part_floats + w.stats_floats) + (index ? 2 * batch * heads * steps * D : 0);
@@ -467,18 +467,16 @@ int kfa_cache_evict(const KfaCache* cache, const float* weights, const int64_t* 
   p.w_out = weights_out;
   p.kept = kept;
   p.lengths_out = lengths_out;
-  const long long total = static_cast<long long>(p.c.batch) * keep * p.c.heads * (p.c.cols / 8);
-  if (total > 0xffffff00ll) return fail(KFA_ERR_ARG, "kfa_cache_evict: more than 64 GB in one call");
-  p.by_piece = kfa::FastDiv::by(p.c.cols / 8);
+  const long long groups = (keep + 31) / 32, total = static_cast<long long>(p.c.batch) * p.c.heads * groups;
+  if (total > 0x7fffffffll) return fail(KFA_ERR_ARG, "kfa_cache_evict: too many rows in one call");
+  p.by_slot = kfa::FastDiv::by(static_cast<uint32_t>(groups));
   p.by_head = kfa::FastDiv::by(p.c.heads);
-  p.by_slot = kfa::FastDiv::by(static_cast<uint32_t>(keep));
   p.total = static_cast<unsigned>(total);
   p.status = dev_status;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   kfa::kfa_cache_select_kernel<<<dim3(p.c.heads, p.c.batch), kfa::SELECT_THREADS, 0, s>>>(p);
   KFA_CUDA(cudaGetLastError());
-  const long long per = 256ll * kfa::GATHER_ROWS;
-  return launch_early(kfa::kfa_cache_gather_kernel, dim3(static_cast<unsigned>((total + per - 1) / per)), s, p);
+  return launch_early(kfa::kfa_cache_gather_kernel, dim3(static_cast<unsigned>((total + 7) / 8)), s, p);
 }
 
 }  // extern "C"

@@ -86,12 +86,12 @@ struct EvictParams {
   float* w_out;
   int* kept;
   int* lengths_out;
-  FastDiv by_slot, by_head, by_piece;
-  unsigned total;
+  FastDiv by_slot, by_head;  // 32 slots of a (sequence, head) at a time; heads
+  unsigned total;            // such groups
   int* status;
 };
 
-constexpr int SELECT_THREADS = 512;
+constexpr int SELECT_THREADS = 1024, SELECT_HELD = 8;  // positions of a thread that stay in registers
 
 // Numbers whose order as unsigned integers is the weights' order: -0 and 0 are equal, NaN is the largest.
 __device__ __forceinline__ uint32_t weight_key(float w) {
@@ -103,7 +103,7 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
 // Which positions stay, per (sequence, K / V head). The key of the last one that stays is found digit by digit (11, 11 and 10 bits, from the
 // top): a histogram of the digit among the positions that agree in the digits before it. It ends early when all that agree stay. Then every
 // warp takes a stretch of the positions, counts those above that key and those equal to it, and lists them in ascending order: all above it
-// stay, of the equal ones the first, until there are enough. Bound by latency: 16 positions a thread at 8192, read from L1 after the first time.
+// stay, of the equal ones the first, until there are enough. Bound by latency; the first 8192 positions are read once and held.
 __global__ void __launch_bounds__(SELECT_THREADS) kfa_cache_select_kernel(const EvictParams p) {
   constexpr int WARPS = SELECT_THREADS / 32, BINS = 2048, PER = BINS / SELECT_THREADS;
   const int g = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -135,25 +135,34 @@ __global__ void __launch_bounds__(SELECT_THREADS) kfa_cache_select_kernel(const 
   if (want == 0) return;
   uint32_t prefix = 0, mask = 0;
   int need = want;
+  float held[SELECT_HELD];
+#pragma unroll
+  for (int k = 0; k < SELECT_HELD; ++k) {
+    const int i = k * SELECT_THREADS + tid;
+    held[k] = i < old ? w[i] : 0.f;
+  }
   for (int shift = 21;; shift = shift == 21 ? 10 : 0) {
     const uint32_t digits = shift == 0 ? 1023u : 2047u;
     for (int i = tid; i < BINS; i += SELECT_THREADS) hist[i] = 0;
     __syncthreads();
-#pragma unroll 4
-    for (int i0 = 0; i0 < old; i0 += SELECT_THREADS) {
-      const int i = i0 + tid;
-      const uint32_t key = i < old ? weight_key(w[i]) : 0u;
+    auto tally = [&](int i, float x) {
+      const uint32_t key = weight_key(x), digit = (key >> shift) & digits;
       const bool in = i < old && (key & mask) == prefix;
-      const uint32_t digit = (key >> shift) & digits;
       // (many equal weights: one addition a warp)
       const unsigned act = __ballot_sync(0xffffffffu, in);
-      const uint32_t lead = __shfl_sync(0xffffffffu, digit, act ? __ffs(act) - 1 : 0);
+      if (act == 0) return;
+      const uint32_t lead = __shfl_sync(0xffffffffu, digit, __ffs(act) - 1);
       if (__all_sync(0xffffffffu, !in || digit == lead)) {
-        if (act != 0 && lane == 0) atomicAdd(&hist[lead], __popc(act));
+        if (lane == 0) atomicAdd(&hist[lead], __popc(act));
       } else if (in) {
         atomicAdd(&hist[digit], 1);
       }
-    }
+    };
+#pragma unroll
+    for (int k = 0; k < SELECT_HELD; ++k)
+      if (k * SELECT_THREADS < old) tally(k * SELECT_THREADS + tid, held[k]);
+#pragma unroll 4
+    for (int i0 = SELECT_HELD * SELECT_THREADS; i0 < old; i0 += SELECT_THREADS) tally(i0 + tid, i0 + tid < old ? w[i0 + tid] : 0.f);
     __syncthreads();
     // bins from the top, PER a thread: in whose are the last ones that are needed?
     int mine = 0, upto;
@@ -220,42 +229,52 @@ __global__ void __launch_bounds__(SELECT_THREADS) kfa_cache_select_kernel(const 
   }
 }
 
-// Moves the rows that stay: a thread 16 bytes of a key and of its value, of GATHER_ROWS rows far apart, whose loads are in flight together.
-constexpr int GATHER_ROWS = 4;
+// Moves the rows that stay. A warp takes 32 slots of a (sequence, K / V head): each lane finds where one of them comes from and goes to, then
+// lanes 0 - 15 move the key's 16-byte pieces and lanes 16 - 31 the value's, row after row (short rows several at once), GATHER_ROWS
+// loads in flight. Bound by memory: 2 x 2 D bytes read and written a row.
+constexpr int GATHER_ROWS = 8;
 __global__ void __launch_bounds__(256) kfa_cache_gather_kernel(const EvictParams p) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const unsigned step = gridDim.x * 256u;
-  uint4 k[GATHER_ROWS], v[GATHER_ROWS];
-  uint8_t *ko[GATHER_ROWS], *vo[GATHER_ROWS];
-#pragma unroll
-  for (int n = 0; n < GATHER_ROWS; ++n) {
-    const unsigned long long at64 = static_cast<unsigned long long>(n) * step + blockIdx.x * 256u + threadIdx.x;
-    ko[n] = nullptr;
-    if (at64 >= p.total) continue;
-    const unsigned at = static_cast<unsigned>(at64);
-    const unsigned row = p.by_piece.div(at), piece = at - row * p.by_piece.d;
-    const unsigned rest = p.by_head.div(row), g = row - rest * p.by_head.d;
-    const unsigned b = p.by_slot.div(rest), i = rest - b * p.by_slot.d;
-    const int pos = p.kept[(static_cast<long long>(b) * p.c.heads + g) * p.keep + i];
-    if (pos < 0 && !p.clear) continue;
-    int page = 0, slot = 0, page_o, slot_o;
-    if ((pos >= 0 && !cache_place(p.c, b, pos, page, slot)) || !cache_place(p.out, b, i, page_o, slot_o)) {
+  const unsigned group = blockIdx.x * 8u + (threadIdx.x >> 5);
+  if (group >= p.total) return;
+  const int lane = threadIdx.x & 31;
+  const unsigned row = p.by_slot.div(group), first = (group - row * p.by_slot.d) * 32u;  // (sequence, head); first slot
+  const unsigned b = p.by_head.div(row), g = row - b * p.by_head.d;
+  const int i = static_cast<int>(first) + lane;
+  int pos = -1, page = 0, slot = 0, page_o = -1, slot_o = 0;
+  if (i < p.keep) {
+    pos = p.kept[static_cast<long long>(row) * p.keep + i];
+    if ((pos >= 0 && !cache_place(p.c, b, pos, page, slot)) || ((pos >= 0 || p.clear) && !cache_place(p.out, b, i, page_o, slot_o))) {
       report(p.status, DEV_BAD_CACHE);
-      continue;
+      page_o = -1;
     }
-    k[n] = v[n] = make_uint4(0, 0, 0, 0);
-    if (pos >= 0) {
-      k[n] = *reinterpret_cast<const uint4*>(p.c.k + page * p.c.k_sn + g * p.c.k_sh + slot * p.c.k_ss + 16 * piece);
-      v[n] = *reinterpret_cast<const uint4*>(p.c.v + page * p.c.v_sn + g * p.c.v_sh + slot * p.c.v_ss + 16 * piece);
-    }
-    ko[n] = p.out.k + page_o * p.out.k_sn + g * p.out.k_sh + slot_o * p.out.k_ss + 16 * piece;
-    vo[n] = p.out.v + page_o * p.out.v_sn + g * p.out.v_sh + slot_o * p.out.v_ss + 16 * piece;
   }
+  const unsigned live = __ballot_sync(0xffffffffu, page_o >= 0);
+  if (live == 0) return;
+  const bool values = lane >= 16;
+  const int pieces = p.c.cols / 8, span = pieces > 8 ? 16 : (pieces > 4 ? 8 : 4), at_once = 16 / span;  // rows at once
+  const int mine = (lane & 15) / span, piece = (lane & 15) % span;
+  const uint8_t* from = (values ? p.c.v + g * p.c.v_sh : p.c.k + g * p.c.k_sh) + 16 * piece;
+  uint8_t* to = (values ? p.out.v + g * p.out.v_sh : p.out.k + g * p.out.k_sh) + 16 * piece;
+  const long long f_n = values ? p.c.v_sn : p.c.k_sn, f_s = values ? p.c.v_ss : p.c.k_ss;
+  const long long t_n = values ? p.out.v_sn : p.out.k_sn, t_s = values ? p.out.v_ss : p.out.k_ss;
+  for (int r0 = 0; r0 < 32; r0 += GATHER_ROWS * at_once) {
+    uint4 x[GATHER_ROWS];
+    uint8_t* dst[GATHER_ROWS];
 #pragma unroll
-  for (int n = 0; n < GATHER_ROWS; ++n) {
-    if (ko[n] == nullptr) continue;
-    *reinterpret_cast<uint4*>(ko[n]) = k[n];
-    *reinterpret_cast<uint4*>(vo[n]) = v[n];
+    for (int k = 0; k < GATHER_ROWS; ++k) {
+      const int r = (r0 + k * at_once + mine) & 31;
+      const int at = __shfl_sync(0xffffffffu, pos, r), pg = __shfl_sync(0xffffffffu, page, r), sl = __shfl_sync(0xffffffffu, slot, r);
+      const int pg_o = __shfl_sync(0xffffffffu, page_o, r), sl_o = __shfl_sync(0xffffffffu, slot_o, r);
+      dst[k] = nullptr;
+      x[k] = make_uint4(0, 0, 0, 0);
+      if (pg_o < 0 || piece >= pieces || r0 + k * at_once + mine >= 32) continue;
+      if (at >= 0) x[k] = *reinterpret_cast<const uint4*>(from + pg * f_n + sl * f_s);
+      dst[k] = to + pg_o * t_n + sl_o * t_s;
+    }
+#pragma unroll
+    for (int k = 0; k < GATHER_ROWS; ++k)
+      if (dst[k] != nullptr) *reinterpret_cast<uint4*>(dst[k]) = x[k];
   }
 }
 

@@ -318,13 +318,13 @@ template <int NC>
 struct WeighRowsCfg {
   static constexpr int CHUNK = 128 * 64 * 2, STAGE = NC * CHUNK;
   static constexpr int Q_CHUNK = 64 * 128, Q_BYTES = NC * Q_CHUNK;
-  static constexpr int DK = 2, DQ = 3;  // key tiles; row tiles per stream
+  static constexpr int DK = 1, DQ = 2;  // key tiles; row tiles per stream (two CTAs an SM: what one waits for, the other fills)
   static constexpr int SMALL = 1024 + 2 * DQ * 64 * 8 + 2 * 128 * 4 * 2;
   static constexpr int SMEM = 1024 + DK * STAGE + 2 * DQ * Q_BYTES + SMALL;
   static constexpr int TMEM = 256;  // S 2 x 2 x 64
   static constexpr int B_K = 0, B_KFREE = DK, B_Q = 2 * DK, B_QFREE = B_Q + 2 * DQ, B_S = B_QFREE + 2 * DQ, B_SFREE = B_S + 4,
                        B_DRAIN = B_SFREE + 4, N_BARS = B_DRAIN + 2;
-  static_assert(SMEM <= 232448 && N_BARS * 8 + 256 <= 1024, "shared memory");
+  static_assert(2 * (SMEM + 1024) <= 233472 && N_BARS * 8 + 256 <= 1024, "shared memory");
 };
 
 // Items of a sequence: K / V head slowest, then block of tokens, then tile of 128 keys: those that some token of the block sees.
@@ -378,7 +378,7 @@ struct ItemWalk {
 };
 
 template <int NC, bool BF16>
-__global__ void __launch_bounds__(ATT_THREADS, 1)
+__global__ void __launch_bounds__(ATT_THREADS, 2)
 kfa_cache_weigh_rows_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const AttendParams a,
                             const WeighParams p) {
   using R = WeighRowsCfg<NC>;
@@ -566,15 +566,22 @@ kfa_cache_weigh_rows_kernel(const __grid_constant__ CUtensorMap tmQ, const __gri
           if (ok) ok = mbar_wait_warp(bar(R::B_Q + stage), q_turn(T) & 1, ctl, 89);
           if (ok) ok = mbar_wait_warp(bar(R::B_S + 2 * st + (c & 1)), (c >> 1) & 1, ctl, 90);
           tc_fence_after();
-          float x[64];
-          tmem_ld_cols<64>(tmem + lane_base + (2 * st + (c & 1)) * 64, x);
-          tmem_wait_ld();
-          tc_fence_before();
-          mbar_arrive(bar(R::B_SFREE + 2 * st + (c & 1)));
           const float2* rows = s_rows + stage * 64;
-          const bool odd = __any_sync(0xffffffffu, rows[lane].x == INFINITY || rows[lane + 32].x == INFINITY);
-          if (slow || odd) sum += weigh_scores<64>(x, rows, a.c_log2, true, [&](int r) { return pos <= w.len + token + static_cast<int>(p.by_tile_h.div(r)); });
-          else sum += weigh_scores<64>(x, rows, a.c_log2, false, [](int) { return true; });
+          const bool odd = slow || __any_sync(0xffffffffu, rows[lane].x == INFINITY || rows[lane + 32].x == INFINITY);
+#pragma unroll
+          for (int i = 0; i < 64; i += 32) {
+            float x[32];
+            tmem_ld32(tmem + lane_base + (2 * st + (c & 1)) * 64 + i, reinterpret_cast<uint32_t*>(x));
+            tmem_wait_ld();
+            if (i == 32) {
+              tc_fence_before();
+              mbar_arrive(bar(R::B_SFREE + 2 * st + (c & 1)));
+            }
+            if (odd)
+              sum += weigh_scores<32>(x, rows + i, a.c_log2, true, [&](int r) { return pos <= w.len + token + static_cast<int>(p.by_tile_h.div(i + r)); });
+            else
+              sum += weigh_scores<32>(x, rows + i, a.c_log2, false, [](int) { return true; });
+          }
           mbar_arrive(bar(R::B_QFREE + stage));
           ++c;
         }
