@@ -747,6 +747,7 @@ kfa_cache_attend_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
     constexpr int PER = N / 32 > 0 ? N / 32 : 1;  // columns whose maximum a lane keeps: lane, lane + 32
     float* shift = s_shift + warp * N;
     const float c_log2 = p.c_log2;
+    const float2 c2 = make_float2(c_log2, c_log2);
     Walk w = first;
     bool more = true, ok = true;
     int c = 0, T0 = 0, s = 0;  // the stream's tiles; tiles and segments before
@@ -821,7 +822,7 @@ kfa_cache_attend_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
             m_ref[i] = y;
           }
           grew |= move;
-          if (lane + 32 * i < N) shift[col] = m_ref[i] == -INFINITY ? 0.f : m_ref[i];
+          if (lane + 32 * i < N) shift[col] = m_ref[i] == -INFINITY ? 0.f : -m_ref[i];
         }
         grew = __any_sync(0xffffffffu, grew);  // the same in all warps of the stream
         __syncwarp();
@@ -850,12 +851,16 @@ kfa_cache_attend_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
 #pragma unroll
         for (int i = 0; i < N; i += 8) {
           const float4 a = *reinterpret_cast<const float4*>(shift + i), b = *reinterpret_cast<const float4*>(shift + i + 4);
-          const float mm[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+          const float2 mm[4] = {make_float2(a.x, a.y), make_float2(a.z, a.w), make_float2(b.x, b.y), make_float2(b.z, b.w)};
           float e[8];
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            e[j] = ex2((x[i + j] - mm[j]) * c_log2);
-            l[i + j] += e[j];
+          for (int j = 0; j < 8; j += 2) {
+            const float2 y = __fmul2_rn(__fadd2_rn(make_float2(x[i + j], x[i + j + 1]), mm[j / 2]), c2);
+            e[j] = ex2(y.x);
+            e[j + 1] = ex2(y.y);
+            const float2 sum = __fadd2_rn(make_float2(l[i + j], l[i + j + 1]), make_float2(e[j], e[j + 1]));
+            l[i + j] = sum.x;
+            l[i + j + 1] = sum.y;
           }
           asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(sp + p_piece<N>(key, i / 8)), "r"(pack16<BF16>(e[0], e[1])),
                        "r"(pack16<BF16>(e[2], e[3])), "r"(pack16<BF16>(e[4], e[5])), "r"(pack16<BF16>(e[6], e[7]))

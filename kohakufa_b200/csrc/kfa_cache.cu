@@ -474,7 +474,9 @@ int kfa_cache_evict(const KfaCache* cache, const float* weights, const int64_t* 
   p.total = static_cast<unsigned>(total);
   p.status = dev_status;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  kfa::kfa_cache_select_kernel<<<dim3(p.c.heads, p.c.batch), kfa::SELECT_THREADS, 0, s>>>(p);
+  const dim3 heads(p.c.heads, p.c.batch);
+  if (p.c.capacity <= 2048) kfa::kfa_cache_select_kernel<256><<<heads, 256, 0, s>>>(p);
+  else kfa::kfa_cache_select_kernel<1024><<<heads, 1024, 0, s>>>(p);
   KFA_CUDA(cudaGetLastError());
   return launch_early(kfa::kfa_cache_gather_kernel, dim3(static_cast<unsigned>((total + 7) / 8)), s, p);
 }

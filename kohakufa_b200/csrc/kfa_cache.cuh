@@ -91,7 +91,7 @@ struct EvictParams {
   int* status;
 };
 
-constexpr int SELECT_THREADS = 1024, SELECT_HELD = 8;  // positions of a thread that stay in registers
+constexpr int SELECT_HELD = 8;  // positions of a thread that stay in registers
 
 // Numbers whose order as unsigned integers is the weights' order: -0 and 0 are equal, NaN is the largest.
 __device__ __forceinline__ uint32_t weight_key(float w) {
@@ -104,6 +104,9 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
 // top): a histogram of the digit among the positions that agree in the digits before it. It ends early when all that agree stay. Then every
 // warp takes a stretch of the positions, counts those above that key and those equal to it, and lists them in ascending order: all above it
 // stay, of the equal ones the first, until there are enough. Bound by latency; the first 8192 positions are read once and held.
+// SELECT_THREADS: 256 for caches of up to 2048 positions, else 1024 (a cache of 320 positions 9.2 us with 512, 11.3 with 1024; 8192
+// positions 23 us with 512, 13.5 with 1024).
+template <int SELECT_THREADS>
 __global__ void __launch_bounds__(SELECT_THREADS) kfa_cache_select_kernel(const EvictParams p) {
   constexpr int WARPS = SELECT_THREADS / 32, BINS = 2048, PER = BINS / SELECT_THREADS;
   const int g = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -232,7 +235,7 @@ __global__ void __launch_bounds__(SELECT_THREADS) kfa_cache_select_kernel(const 
 // Moves the rows that stay. A warp takes 32 slots of a (sequence, K / V head): each lane finds where one of them comes from and goes to, then
 // lanes 0 - 15 move the key's 16-byte pieces and lanes 16 - 31 the value's, row after row (short rows several at once), GATHER_ROWS
 // loads in flight. Bound by memory: 2 x 2 D bytes read and written a row.
-constexpr int GATHER_ROWS = 8;
+constexpr int GATHER_ROWS = 4;
 __global__ void __launch_bounds__(256) kfa_cache_gather_kernel(const EvictParams p) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const unsigned group = blockIdx.x * 8u + (threadIdx.x >> 5);

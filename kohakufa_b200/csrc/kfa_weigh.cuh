@@ -34,23 +34,29 @@ __device__ __forceinline__ float2 row_stats(const AttendParams& a, const WeighPa
   return make_float2(at[0], at[p.r.T]);
 }
 
-// The weights of a key: N scores against N rows. odd: some rows are not there (m = +inf), and their scores may be anything.
-// first: the rows that see the key are those of tokens `first` and later, `tokens(r)` being row r's.
-template <int N, typename F>
-__device__ __forceinline__ float weigh_scores(const float* x, const float2* rows, float c_log2, bool slow, F sees) {
-  float sum[4] = {0.f, 0.f, 0.f, 0.f};
+// The weights of a key, summed: N scores against N rows, whose -m and -log2 l stand one after the other (two at a time in the packed
+// instructions). slow: some rows are not there (-m = -inf, and their scores may be anything), or do not see the key: those below r_min.
+template <int N>
+__device__ __forceinline__ float weigh_scores(const float* x, const float* neg_m, const float* neg_l, float c_log2, bool slow, int r_min) {
+  const float2 c2 = make_float2(c_log2, c_log2);
+  float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
-  for (int i = 0; i < N; i += 2) {
-    const float4 s = *reinterpret_cast<const float4*>(rows + i);
-    float e0 = ex2(fmaf(x[i] - s.x, c_log2, -s.y)), e1 = ex2(fmaf(x[i + 1] - s.z, c_log2, -s.w));
+  for (int i = 0; i < N; i += 4) {
+    const float4 m = *reinterpret_cast<const float4*>(neg_m + i), l = *reinterpret_cast<const float4*>(neg_l + i);
+    float2 e0 = __ffma2_rn(__fadd2_rn(make_float2(x[i], x[i + 1]), make_float2(m.x, m.y)), c2, make_float2(l.x, l.y));
+    float2 e1 = __ffma2_rn(__fadd2_rn(make_float2(x[i + 2], x[i + 3]), make_float2(m.z, m.w)), c2, make_float2(l.z, l.w));
+    e0 = make_float2(ex2(e0.x), ex2(e0.y));
+    e1 = make_float2(ex2(e1.x), ex2(e1.y));
     if (slow) {
-      if (s.x == INFINITY || !sees(i)) e0 = 0.f;
-      if (s.z == INFINITY || !sees(i + 1)) e1 = 0.f;
+      if (m.x == -INFINITY || i < r_min) e0.x = 0.f;
+      if (m.y == -INFINITY || i + 1 < r_min) e0.y = 0.f;
+      if (m.z == -INFINITY || i + 2 < r_min) e1.x = 0.f;
+      if (m.w == -INFINITY || i + 3 < r_min) e1.y = 0.f;
     }
-    sum[i & 2] += e0;
-    sum[(i & 2) + 1] += e1;
+    sum[0] = __fadd2_rn(sum[0], e0);
+    sum[1] = __fadd2_rn(sum[1], e1);
   }
-  return (sum[0] + sum[1]) + (sum[2] + sum[3]);
+  return (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
 }
 
 // ---- up to 64 rows -------------------------------------------------------------------------------------------------------------
@@ -77,7 +83,7 @@ kfa_cache_weigh_kernel(const __grid_constant__ CUtensorMap tmK, const AttendPara
   const uint32_t sK = base, sQ = sK + R::NS * R::STAGE;
   uint8_t* small = smem + R::NS * R::STAGE + 2 * R::Q_BYTES;
   uint64_t* bars = reinterpret_cast<uint64_t*>(small);
-  float2* s_rows = reinterpret_cast<float2*>(small + 1024);  // [segment & 1][N]
+  float* s_rows = reinterpret_cast<float*>(small + 1024);  // [segment & 1][-m, -log2 l][N]
   const AttCtl ac(bars + R::N_BARS);
   const uint32_t bar0 = smem_u32(bars);
   auto bar = [&](int i) { return bar0 + 8u * i; };
@@ -169,7 +175,8 @@ kfa_cache_weigh_kernel(const __grid_constant__ CUtensorMap tmK, const AttendPara
           if (t >= 0 && t < p.r.T) st = row_stats(a, p, w.b, h, t);
           else *ac.bad = 1;
         }
-        s_rows[(s & 1) * N + r] = st;
+        s_rows[(s & 1) * 2 * N + r] = -st.x;
+        s_rows[(s & 1) * 2 * N + N + r] = -st.y;
       }
       const uint32_t dst = sQ + (s & 1) * R::Q_BYTES;
       const int total = w.count * a.gt * pieces;
@@ -254,8 +261,8 @@ kfa_cache_weigh_kernel(const __grid_constant__ CUtensorMap tmK, const AttendPara
         tc_fence_before();
         mbar_arrive(bar(R::B_SFREE + 2 * st + (c & 1)));
         // (tokens that are not there have m = +inf; their scores come from what the buffer held before)
-        const float sum = weigh_scores<N>(x, s_rows + (s & 1) * N, a.c_log2, true,
-                                          [&](int r) { return pos <= old + static_cast<int>(a.by_gt.div(r)); });
+        const float* rows = s_rows + (s & 1) * 2 * N;
+        const float sum = weigh_scores<N>(x, rows, rows + N, a.c_log2, true, (pos - old) * a.gt);  // (token i sees positions up to old + i)
         if (mine) out[pos] = *ac.bad != 0 ? __int_as_float(0x7fc00000) : before + sum;
         ++c;
       }
@@ -388,7 +395,7 @@ kfa_cache_weigh_rows_kernel(const __grid_constant__ CUtensorMap tmQ, const __gri
   const uint32_t sK = base, sQ = sK + R::DK * R::STAGE;
   uint8_t* small = smem + R::DK * R::STAGE + 2 * R::DQ * R::Q_BYTES;
   uint64_t* bars = reinterpret_cast<uint64_t*>(small);
-  float2* s_rows = reinterpret_cast<float2*>(small + 1024);                              // [stage][64]
+  float* s_rows = reinterpret_cast<float*>(small + 1024);                                // [stage][-m, -log2 l][64]
   float* s_sum = reinterpret_cast<float*>(small + 1024 + 2 * R::DQ * 64 * 8);            // [item & 1][128]: the second stream's
   const AttCtl ac(bars + R::N_BARS);
   const uint32_t bar0 = smem_u32(bars);
@@ -497,8 +504,11 @@ kfa_cache_weigh_rows_kernel(const __grid_constant__ CUtensorMap tmQ, const __gri
         const int stage = q_stage(T);
         if (q_turn(T) > 0) ok = mbar_wait_warp(bar(R::B_QFREE + stage), (q_turn(T) - 1) & 1, ctl, 85);
         if (!ok) break;
-        s_rows[stage * 64 + lane] = st[0];
-        s_rows[stage * 64 + 32 + lane] = st[1];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          s_rows[stage * 128 + 32 * k + lane] = -st[k].x;
+          s_rows[stage * 128 + 64 + 32 * k + lane] = -st[k].y;
+        }
         if (lane == 0) {
           mbar_expect_tx(bar(R::B_Q + stage), NC * p.tile_t * p.tile_h * 128);
           for (int ch = 0; ch < NC; ++ch)
@@ -566,8 +576,9 @@ kfa_cache_weigh_rows_kernel(const __grid_constant__ CUtensorMap tmQ, const __gri
           if (ok) ok = mbar_wait_warp(bar(R::B_Q + stage), q_turn(T) & 1, ctl, 89);
           if (ok) ok = mbar_wait_warp(bar(R::B_S + 2 * st + (c & 1)), (c >> 1) & 1, ctl, 90);
           tc_fence_after();
-          const float2* rows = s_rows + stage * 64;
-          const bool odd = slow || __any_sync(0xffffffffu, rows[lane].x == INFINITY || rows[lane + 32].x == INFINITY);
+          const float* rows = s_rows + stage * 128;
+          const bool odd = slow || __any_sync(0xffffffffu, rows[lane] == -INFINITY || rows[lane + 32] == -INFINITY);
+          const int r_min = (pos - w.len - token) * p.tile_h;  // (token t sees positions up to len + t)
 #pragma unroll
           for (int i = 0; i < 64; i += 32) {
             float x[32];
@@ -577,10 +588,8 @@ kfa_cache_weigh_rows_kernel(const __grid_constant__ CUtensorMap tmQ, const __gri
               tc_fence_before();
               mbar_arrive(bar(R::B_SFREE + 2 * st + (c & 1)));
             }
-            if (odd)
-              sum += weigh_scores<32>(x, rows + i, a.c_log2, true, [&](int r) { return pos <= w.len + token + static_cast<int>(p.by_tile_h.div(i + r)); });
-            else
-              sum += weigh_scores<32>(x, rows + i, a.c_log2, false, [](int) { return true; });
+            if (odd) sum += weigh_scores<32>(x, rows + i, rows + 64 + i, a.c_log2, true, r_min - i);
+            else sum += weigh_scores<32>(x, rows + i, rows + 64 + i, a.c_log2, false, 0);
           }
           mbar_arrive(bar(R::B_QFREE + stage));
           ++c;
