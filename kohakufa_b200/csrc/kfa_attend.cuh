@@ -199,6 +199,40 @@ __device__ __forceinline__ bool my_work(const AttendParams& p, int* s_i, Walk& w
   return w.b < p.c.batch && w.start(p);
 }
 
+// mbar_wait_warp for kernels in which many warps wait at the same time: the hardware may suspend a thread for up to 10 us (the hint)
+// instead of the default, and suspended warps take no issue slots from those that compute.
+__device__ __forceinline__ bool mbar_suspend(uint32_t bar, uint32_t parity) {
+  if constexpr (KFA_SHORT_WAITS) {
+    return mbar_try_wait(bar, parity);
+  } else {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.b32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity), "r"(10000u)
+        : "memory");
+    return ok != 0;
+  }
+}
+__device__ __forceinline__ bool wait_warp(uint32_t bar, uint32_t parity, const Ctl& ctl, int site) {
+  bool ok = mbar_suspend(bar, parity);
+  if (__builtin_expect(__all_sync(0xffffffffu, ok), 1)) return true;
+  if (!ok) {
+    const long long t0 = clock64();
+#pragma unroll 1
+    while (!(ok = mbar_suspend(bar, parity))) {
+      if (*ctl.s_abort != 0) break;
+      if (clock64() - t0 > KFA_WAIT_CYCLES) {
+        *ctl.s_abort = KFA_DEV_TIMEOUT_BASE + site;
+        break;
+      }
+    }
+  }
+  return __all_sync(0xffffffffu, ok);
+}
+
 // Shared memory and rings that both kernels lay out alike. NC: chunks of 64 columns of the head dim; Q_ROWS: rows of the query buffer;
 // BOTH: both streams see every tile (else they take turns); OTHER: bytes beside keys, values and queries.
 template <int NC_, int Q_ROWS_, int NQ_, bool BOTH_, int OTHER_>
@@ -390,7 +424,7 @@ __device__ __forceinline__ void att_produce(const AttendParams& p, const Walk& f
     if (lane == 0 && !length_ok(p.c, w.b)) *ac.bad = 1;
     if (!values) {
       if (s >= R::NQ) {  // both streams are done with the segment that used this buffer
-        ok = mbar_wait_warp(bar(R::B_QFREE), (s - R::NQ) & 1, ctl, 70);
+        ok = wait_warp(bar(R::B_QFREE), (s - R::NQ) & 1, ctl, 70);
         if (!ok) break;
       }
       if (lane == 0) {
@@ -420,7 +454,7 @@ __device__ __forceinline__ void att_produce(const AttendParams& p, const Walk& f
       const unsigned cached = __ballot_sync(0xffffffffu, kind == 1), fresh = __ballot_sync(0xffffffffu, kind == 2);
       const int stage = values ? R::v_stage(T) : R::k_stage(T), turn = values ? R::v_turn(T) : R::k_turn(T);
       if (turn > 0) {
-        ok = mbar_wait_warp(bar(R::B_KVFREE + stage), (turn - 1) & 1, ctl, 72);
+        ok = wait_warp(bar(R::B_KVFREE + stage), (turn - 1) & 1, ctl, 72);
         if (!ok) break;
       }
       if (lane == 0) mbar_expect_tx(bar(R::B_KV + stage), R::NC * 128 * (__popc(cached) * p.box + __popc(fresh) * ATT_UNIT));
@@ -503,7 +537,7 @@ __device__ __forceinline__ void att_issue(const AttendParams& p, const Walk& fir
       const int c = i_p / PIECES, piece = i_p % PIECES;
       // (nothing else can go before these values: no need to look at both)
       if ((!have || i_s > i_p + 1) &&
-          !mbar_wait_warp(bar0 + 8u * (R::B_P + 2 * st + (PIECES == 2 ? piece : c % NP)), (PIECES == 2 ? c : c / NP) & 1, Ctl{ac.abort}, 74))
+          !wait_warp(bar0 + 8u * (R::B_P + 2 * st + (PIECES == 2 ? piece : c % NP)), (PIECES == 2 ? c : c / NP) & 1, Ctl{ac.abort}, 74))
         break;
       const AttTile now = (c * PIECES + PIECES > i_s) ? ahead : ((c & 1) ? odd : even);  // (its second half may have no scores yet)
       if (ready(R::B_P + 2 * st + (PIECES == 2 ? piece : c % NP), (PIECES == 2 ? c : c / NP) & 1) &&
@@ -782,7 +816,7 @@ kfa_cache_attend_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
           }
           odd = odd_values<BF16>(p, w, rows.g, fresh);
         }
-        if (ok) ok = mbar_wait_warp(bar(R::B_S + 2 * st + (c & 1)), (c >> 1) & 1, ctl, 78);
+        if (ok) ok = wait_warp(bar(R::B_S + 2 * st + (c & 1)), (c >> 1) & 1, ctl, 78);
         tc_fence_after();
         float x[N];
         tmem_ld_cols<N>(tmS + lane_base + (2 * st + (c & 1)) * N, x);
@@ -828,7 +862,7 @@ kfa_cache_attend_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
         __syncwarp();
         if (grew && !opens) {
           // sums and O of the earlier tiles, to the new maxima
-          if (ok) ok = mbar_wait_warp(bar(R::B_PV + 2 * st + (c - 1) % NP), ((c - 1) / NP) & 1, ctl, 79);
+          if (ok) ok = wait_warp(bar(R::B_PV + 2 * st + (c - 1) % NP), ((c - 1) / NP) & 1, ctl, 79);
           tc_fence_after();
 #pragma unroll
           for (int i = 0; i < N; i += 16) {
@@ -846,7 +880,7 @@ kfa_cache_attend_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
           tmem_wait_st();
         }
         // ---- P ----
-        if (c >= NP && ok) ok = mbar_wait_warp(bar(R::B_PV + 2 * st + c % NP), (c / NP - 1) & 1, ctl, 80);  // its buffer has been read
+        if (c >= NP && ok) ok = wait_warp(bar(R::B_PV + 2 * st + c % NP), (c / NP - 1) & 1, ctl, 80);  // its buffer has been read
         const uint32_t sp = sP + (st * NP + c % NP) * R::P_BYTES;
 #pragma unroll
         for (int i = 0; i < N; i += 8) {
@@ -868,8 +902,8 @@ kfa_cache_attend_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
         }
         if (!full) {
           // (The tile before has to be done with: until then the barrier of this one's stage may be a turn behind.)
-          if (c > 0 && ok) ok = mbar_wait_warp(bar(R::B_PV + 2 * st + (c - 1) % NP), ((c - 1) / NP) & 1, ctl, 81);
-          if (ok) ok = mbar_wait_warp(bar(R::B_KV + R::v_stage(T)), R::v_turn(T) & 1, ctl, 82);
+          if (c > 0 && ok) ok = wait_warp(bar(R::B_PV + 2 * st + (c - 1) % NP), ((c - 1) / NP) & 1, ctl, 81);
+          if (ok) ok = wait_warp(bar(R::B_KV + R::v_stage(T)), R::v_turn(T) & 1, ctl, 82);
           clean_values<NC, BF16>(p, w, rows.g, sKV + R::v_stage(T) * R::STAGE, key, valid, fresh, odd);
           if (odd != 0) ac.odd[st] = s + 1;
         }
@@ -899,7 +933,7 @@ kfa_cache_attend_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
             fin[5 * N + lane + 32 * i] = m_top[i];
           }
       }
-      if (!opens && ok) ok = mbar_wait_warp(bar(R::B_PV + 2 * st + (c - 1) % NP), ((c - 1) / NP) & 1, ctl, 83);
+      if (!opens && ok) ok = wait_warp(bar(R::B_PV + 2 * st + (c - 1) % NP), ((c - 1) / NP) & 1, ctl, 83);
       tc_fence_before();
       named_sync<3, 256>();
       tc_fence_after();
@@ -1102,7 +1136,7 @@ kfa_cache_attend_rows_kernel(const __grid_constant__ CUtensorMap tmQ, const __gr
             seen[0] = exists ? seen_word(p, w, ub + 2 * half, tk) : 0u;
             seen[1] = exists ? seen_word(p, w, ub + 2 * half + 1, tk) : 0u;
           }
-          if (ok) ok = mbar_wait_warp(bar(R::B_S + 2 * st + half), c & 1, ctl, 78);
+          if (ok) ok = wait_warp(bar(R::B_S + 2 * st + half), c & 1, ctl, 78);
           tc_fence_after();
           float2 x[32];
           tmem_ld_cols<64>(tS + 64 * half, reinterpret_cast<float*>(x));
@@ -1124,7 +1158,7 @@ kfa_cache_attend_rows_kernel(const __grid_constant__ CUtensorMap tmQ, const __gr
             const float alpha = !move ? 1.f : (m_ref == -INFINITY ? 0.f : ex2((m_ref - top) * c_log2));
             if (!opens || half > 0) {  // every product issued so far has to have retired; it is the last but one of this half's
               const int before = 2 * c + half - 1;
-              if (ok) ok = mbar_wait_warp(bar(R::B_PV + 2 * st + (before & 1)), (before >> 1) & 1, ctl, 79);
+              if (ok) ok = wait_warp(bar(R::B_PV + 2 * st + (before & 1)), (before >> 1) & 1, ctl, 79);
               tc_fence_after();
 #pragma unroll
               for (int i = 0; i < D; i += 32) {
@@ -1157,8 +1191,8 @@ kfa_cache_attend_rows_kernel(const __grid_constant__ CUtensorMap tmQ, const __gr
           tmem_wait_st();
           if (!full && half == 0) {
             // (The tile before has to be done with: until then the barrier of this one's stage may be a turn behind.)
-            if (c > 0 && ok) ok = mbar_wait_warp(bar(R::B_PV + 2 * st + 1), (c - 1) & 1, ctl, 81);
-            if (ok) ok = mbar_wait_warp(bar(R::B_KV + R::v_stage(T)), R::v_turn(T) & 1, ctl, 82);
+            if (c > 0 && ok) ok = wait_warp(bar(R::B_PV + 2 * st + 1), (c - 1) & 1, ctl, 81);
+            if (ok) ok = wait_warp(bar(R::B_KV + R::v_stage(T)), R::v_turn(T) & 1, ctl, 82);
             clean_values<NC, BF16>(p, w, rows.g, sKV + R::v_stage(T) * R::STAGE, r_in, valid, fresh, odd);
             if (odd != 0) ac.odd[st] = s + 1;
             fence_async_smem();
@@ -1171,7 +1205,7 @@ kfa_cache_attend_rows_kernel(const __grid_constant__ CUtensorMap tmQ, const __gr
       }
       T0 += tiles;
       // ---- the segment's end ----
-      if (!opens && ok) ok = mbar_wait_warp(bar(R::B_PV + 2 * st + 1), (c - 1) & 1, ctl, 83);
+      if (!opens && ok) ok = wait_warp(bar(R::B_PV + 2 * st + 1), (c - 1) & 1, ctl, 83);
       float a0 = 1.f, a1 = 0.f, m = m_ref, top = m_top, l_all = l;  // factors of the streams' O, the row's statistics
       tc_fence_before();
       if constexpr (BOTH) {

@@ -178,8 +178,8 @@ int launch_attend_rows(const CUtensorMap (&m)[5], const kfa::AttendParams& p, co
 }
 
 struct WeighPlan {
-  int64_t rows, work, bytes, part_floats, stats_floats;
-  int grid, least, extra, block, blocks, tile_h, tile_t;
+  int64_t rows, work, bytes, meta_floats, part_floats, stats_floats;
+  int grid, least, extra, tile_h, tile_t;
 };
 
 WeighPlan plan_weigh(int64_t batch, int64_t heads, int64_t kv_heads, int64_t steps, int64_t capacity, int64_t D, bool index) {
@@ -195,18 +195,16 @@ WeighPlan plan_weigh(int64_t batch, int64_t heads, int64_t kv_heads, int64_t ste
     w.grid = static_cast<int>(std::min<int64_t>(SMS, (batch * kv_heads * units + 3) / 4));
     return w;
   }
-  w.tile_h = static_cast<int>(std::min<int64_t>(group, 64));
-  w.tile_t = 64 / w.tile_h;
-  // Blocks of 512 tokens, at most 8 of them: what an SM does is a number of equal items (and what each block adds goes through memory).
-  const int64_t block = std::max<int64_t>(512, (steps + 7) / 8);
-  w.block = static_cast<int>(block);
-  w.blocks = static_cast<int>((steps + block - 1) / block);
+  w.tile_h = static_cast<int>(std::min<int64_t>(group, 128));
+  w.tile_t = 128 / w.tile_h;
   w.least = 1;
-  w.work = batch * kv_heads * w.blocks * ((capacity + 127) / 128);
+  const int64_t blocks = (steps + kfa::WEIGH_BLOCK - 1) / kfa::WEIGH_BLOCK;
+  w.work = batch * kv_heads * blocks * ((capacity + 127) / 128);
   w.grid = static_cast<int>(std::min<int64_t>(2 * SMS, w.work));
-  w.part_floats = (w.blocks * batch * kv_heads * capacity + 63) / 64 * 64;
+  w.meta_floats = (4 * w.grid + 63) / 64 * 64;
+  w.part_floats = 2ll * w.grid * 128;
   if (index) w.stats_floats = (2 * batch * heads * steps + 63) / 64 * 64;
-  w.bytes = 4 * (w.part_floats + w.stats_floats) + (index ? 2 * batch * heads * steps * D : 0);
+  w.bytes = 4 * (w.meta_floats + w.part_floats + w.stats_floats) + (index ? 2 * batch * heads * steps * D : 0);
   return w;
 }
 
@@ -232,8 +230,7 @@ int launch_weigh_many(const CUtensorMap& mq, const CUtensorMap& mk, const kfa::A
   KFA_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, R::SMEM));
   kern<<<plan.grid, kfa::ATT_THREADS, R::SMEM, s>>>(mq, mk, a, p);
   KFA_CUDA(cudaGetLastError());
-  const dim3 grid(static_cast<unsigned>(std::min<int64_t>((p.room + 255) / 256, 256)), a.c.heads, a.c.batch);
-  return launch_early(kfa::kfa_cache_sum_blocks_kernel, grid, s, a, p);
+  return launch_early(kfa::kfa_cache_join_weights_kernel, dim3(plan.grid + a.c.batch), s, a, p, plan.grid);
 }
 
 }  // namespace
@@ -412,13 +409,13 @@ int kfa_cache_weigh(const KfaTensor4* q, const float* stats, const KfaCache* cac
     if (dtype == KFA_BF16) return D > 64 ? launch_weigh_few<2, true>(mk, a, p, plan, s) : launch_weigh_few<1, true>(mk, a, p, plan, s);
     return D > 64 ? launch_weigh_few<2, false>(mk, a, p, plan, s) : launch_weigh_few<1, false>(mk, a, p, plan, s);
   }
-  p.block = plan.block;
-  p.blocks = plan.blocks;
   p.tile_h = plan.tile_h;
   p.tile_t = plan.tile_t;
   p.head_tiles = (a.group + p.tile_h - 1) / p.tile_h;
   p.by_tile_h = kfa::FastDiv::by(p.tile_h);
-  p.part = static_cast<float*>(scratch);
+  p.by_tile_t = kfa::FastDiv::by(p.tile_t);
+  p.part_meta = static_cast<int4*>(scratch);
+  p.part = static_cast<float*>(scratch) + plan.meta_floats;
   KfaTensor4 rows_q = *q;
   if (p.r.index) {
     p.stats_to = p.part + plan.part_floats;
