@@ -86,10 +86,6 @@ def _new_cache(k: Tensor, v: Tensor, lengths: Tensor, table: Tensor | None) -> K
     return cache
 
 
-def _plain(*tensors) -> bool:
-    return _lib.plain_eager(*(t for t in tensors if t is not None))
-
-
 def _refuse_autograd(name: str, *tensors) -> None:
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
         raise RuntimeError(f"{name}: has no gradient; call it under torch.no_grad() or on detached tensors")
@@ -150,7 +146,7 @@ def attention_cached(
     (+inf, 0). Results repeat bit for bit."""
     pages = cache._tensors()
     softmax_scale = float(q.shape[-1] ** -0.5 if scale is None else scale)
-    if _plain(q, *pages, k, v, tree, counts):
+    if _lib.plain_eager(q, *pages, k, v, tree, counts):
         return _lib.host().cached_attention(
             q, *pages, k, v, tree, counts, softmax_scale, return_stats, _lib.status_word(q.device) if q.is_cuda else None
         )
@@ -173,7 +169,7 @@ def cache_append(cache: KVCache, k: Tensor, v: Tensor, *, index: Tensor | None =
     counts[b]`` (int32 ``[B]``; without it all). ``lengths`` is left as it is: add the counts to it once all layers have appended. The pages that
     are written must belong to one sequence each. Positions beyond the capacity are dropped and reported by ``check_status``."""
     pages = cache._tensors()
-    if _plain(*pages, k, v, index, counts):
+    if _lib.plain_eager(*pages, k, v, index, counts):
         _lib.host().cache_append(*pages, k, v, index, counts, _lib.status_word(k.device) if k.is_cuda else None)
         return
     _refuse_autograd("cache_append", cache.k, cache.v, k, v)
@@ -211,7 +207,7 @@ def cache_weights(
     add = weights is not None
     if weights is None:
         weights = torch.empty(q.shape[0], cache.k.shape[1], cache.capacity, dtype=torch.float32, device=q.device)
-    if _plain(*pages, q, stats, index, counts, weights):
+    if _lib.plain_eager(*pages, q, stats, index, counts, weights):
         word = _lib.status_word(q.device) if q.is_cuda else None
         _lib.host().cache_weights(*pages, q, stats, index, counts, weights, add, softmax_scale, word)
         return weights
@@ -248,21 +244,18 @@ def cache_evict(
         raise ValueError(f"cache_evict: keep {keep}, recent {recent}: 0 <= recent <= keep, keep at least 1")
     if out is cache:
         raise ValueError("cache_evict: out must have pages of its own")
-    k, device = cache.k, cache.k.device
+    k, target = cache.k, (None, None, None, None) if out is None else out._tensors()
+    if _lib.plain_eager(*pages, weights, *target):
+        word = _lib.status_word(k.device) if k.is_cuda else None
+        k_out, v_out, lengths_out, weights_out, kept = _lib.host().evict(*pages, weights, keep, recent, *target, word)
+        return _new_cache(k_out, v_out, lengths_out, target[3]), weights_out, kept
+    _refuse_autograd("cache_evict", cache.k, cache.v, weights, *target[:2])
     batch, heads, dim = cache.lengths.numel(), k.shape[1], k.shape[3]
-    clear = out is None
+    k_out, v_out, _, table_out = target
     if out is None:
-        k_out, v_out = (torch.empty(batch, keep, heads, dim, dtype=k.dtype, device=device).transpose(1, 2) for _ in range(2))
-        table_out = None
-    else:
-        k_out, v_out, table_out = out.k, out.v, out.table
-    lengths_out = torch.empty(batch, dtype=torch.int32, device=device)
-    weights_out = torch.empty(batch, heads, keep, dtype=torch.float32, device=device)
-    kept = torch.empty(batch, heads, keep, dtype=torch.int32, device=device)
-    args = (*pages, weights, keep, recent, k_out, v_out, table_out, lengths_out, weights_out, kept, clear)
-    if _plain(*pages, weights, k_out, v_out, table_out):
-        _lib.host().cache_evict(*args, _lib.status_word(device) if k.is_cuda else None)
-    else:
-        _refuse_autograd("cache_evict", cache.k, cache.v, weights, k_out, v_out)
-        cache_evict_op(*args)
+        k_out, v_out = (k.new_empty(batch, keep, heads, dim).transpose(1, 2) for _ in range(2))
+    lengths_out = cache.lengths.new_empty(batch)
+    weights_out = k.new_empty(batch, heads, keep, dtype=torch.float32)
+    kept = cache.lengths.new_empty(batch, heads, keep)
+    cache_evict_op(*pages, weights, keep, recent, k_out, v_out, table_out, lengths_out, weights_out, kept, out is None)
     return _new_cache(k_out, v_out, lengths_out, table_out), weights_out, kept

@@ -1,5 +1,6 @@
 // C ABI of the operators on a cache of keys and values (declared in include/kfa.h): argument checks and launches.
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <cstring>
 
@@ -100,6 +101,18 @@ int make_box_map(void* ptr, int64_t D, int64_t n1, int64_t s1, int64_t n2, int64
 
 constexpr int SMS = 148;  // (what this library is built for)
 
+// A kernel's dynamic shared memory is allowed once per device (the runtime call costs a small problem's launch about as much as its checks).
+// done: the kernel's own, a bit per device.
+int allow_smem(std::atomic<uint64_t>& done, const void* kern, int bytes) {
+  int dev = 0;
+  KFA_CUDA(cudaGetDevice(&dev));
+  const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+  if (done.load(std::memory_order_relaxed) & bit) return KFA_OK;
+  KFA_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+  done.fetch_or(bit, std::memory_order_relaxed);
+  return KFA_OK;
+}
+
 // How an attention call is cut up: a function of the shapes alone, so that the scratch it needs is known beforehand.
 struct AttendPlan {
   int rows, gt, tt, head_tiles, row_tiles, grid, extra, least;
@@ -156,7 +169,9 @@ int launch_early(void (*kern)(P...), dim3 grid, cudaStream_t s, const P&... para
 
 template <bool BF16, class R, typename K>
 int launch_attend(K kern, const CUtensorMap (&m)[5], const kfa::AttendParams& p, const AttendPlan& plan, cudaStream_t s) {
-  KFA_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, R::SMEM));
+  static std::atomic<uint64_t> allowed{0};
+  const int rc = allow_smem(allowed, reinterpret_cast<const void*>(kern), R::SMEM);
+  if (rc) return rc;
   kern<<<plan.grid, kfa::ATT_THREADS, R::SMEM, s>>>(m[0], m[1], m[2], m[3], m[4], p);
   KFA_CUDA(cudaGetLastError());
   if (plan.whole) return KFA_OK;
@@ -208,18 +223,20 @@ WeighPlan plan_weigh(int64_t batch, int64_t heads, int64_t kv_heads, int64_t ste
   return w;
 }
 
-template <class R, typename K>
+template <bool BF16, class R, typename K>
 int launch_weigh_few(K kern, const CUtensorMap& mk, const kfa::AttendParams& a, const kfa::WeighParams& p, const WeighPlan& plan, cudaStream_t s) {
-  KFA_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, R::SMEM));
+  static std::atomic<uint64_t> allowed{0};
+  const int rc = allow_smem(allowed, reinterpret_cast<const void*>(kern), R::SMEM);
+  if (rc) return rc;
   kern<<<plan.grid, kfa::ATT_THREADS, R::SMEM, s>>>(mk, a, p);
   KFA_CUDA(cudaGetLastError());
   return KFA_OK;
 }
 template <int NC, bool BF16>
 int launch_weigh_few(const CUtensorMap& mk, const kfa::AttendParams& a, const kfa::WeighParams& p, const WeighPlan& plan, cudaStream_t s) {
-  if (plan.rows <= 16) return launch_weigh_few<kfa::WeighCfg<NC, 16>>(kfa::kfa_cache_weigh_kernel<NC, 16, BF16>, mk, a, p, plan, s);
-  if (plan.rows <= 32) return launch_weigh_few<kfa::WeighCfg<NC, 32>>(kfa::kfa_cache_weigh_kernel<NC, 32, BF16>, mk, a, p, plan, s);
-  return launch_weigh_few<kfa::WeighCfg<NC, 64>>(kfa::kfa_cache_weigh_kernel<NC, 64, BF16>, mk, a, p, plan, s);
+  if (plan.rows <= 16) return launch_weigh_few<BF16, kfa::WeighCfg<NC, 16>>(kfa::kfa_cache_weigh_kernel<NC, 16, BF16>, mk, a, p, plan, s);
+  if (plan.rows <= 32) return launch_weigh_few<BF16, kfa::WeighCfg<NC, 32>>(kfa::kfa_cache_weigh_kernel<NC, 32, BF16>, mk, a, p, plan, s);
+  return launch_weigh_few<BF16, kfa::WeighCfg<NC, 64>>(kfa::kfa_cache_weigh_kernel<NC, 64, BF16>, mk, a, p, plan, s);
 }
 
 template <int NC, bool BF16>
@@ -227,7 +244,9 @@ int launch_weigh_many(const CUtensorMap& mq, const CUtensorMap& mk, const kfa::A
                       cudaStream_t s) {
   using R = kfa::WeighRowsCfg<NC>;
   auto kern = kfa::kfa_cache_weigh_rows_kernel<NC, BF16>;
-  KFA_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, R::SMEM));
+  static std::atomic<uint64_t> allowed{0};
+  const int rc = allow_smem(allowed, reinterpret_cast<const void*>(kern), R::SMEM);
+  if (rc) return rc;
   kern<<<plan.grid, kfa::ATT_THREADS, R::SMEM, s>>>(mq, mk, a, p);
   KFA_CUDA(cudaGetLastError());
   return launch_early(kfa::kfa_cache_join_weights_kernel, dim3(plan.grid + a.c.batch), s, a, p, plan.grid);

@@ -214,7 +214,7 @@ void need(Py_ssize_t got, Py_ssize_t want) {
 
 using Args = PyObject* const*;
 
-// plain(*tensors) -> bool: whether an operator on these tensors would go straight to its kernel. That is, no dispatch or
+// plain(*tensors, None among them) -> bool: whether an operator on these tensors would go straight to its kernel. That is, no dispatch or
 // function mode, no torch.func transform and no tracer is active, and each is a torch.Tensor (no subclass) whose address
 // points to its value: batched tensors (gradients of `is_grads_batched`), pending negations and zero tensors are
 // torch.Tensor too, but only the dispatcher resolves them.
@@ -237,7 +237,7 @@ bool plain_tensor(PyObject* o) {
 PyObject* py_plain(Args a, Py_ssize_t n) {
   if (!nothing_interposed()) Py_RETURN_FALSE;
   for (Py_ssize_t i = 0; i < n; ++i)
-    if (!plain_tensor(a[i])) Py_RETURN_FALSE;
+    if (a[i] != Py_None && !plain_tensor(a[i])) Py_RETURN_FALSE;
   Py_RETURN_TRUE;
 }
 
@@ -852,37 +852,91 @@ PyObject* py_cache_weights(Args a, Py_ssize_t n) {
   Py_RETURN_NONE;
 }
 
-// cache_evict(k_pages, v_pages, lengths, table, weights, keep, recent, k_out, v_out, table_out, lengths_out, weights_out, kept, clear, status)
+// What cache_evict fills: the pages of `out`, or of a new cache of one stretch per sequence, lengths, weights, positions.
+struct Evicted {
+  Cache out;
+  at::Tensor weights, kept;
+};
+
+void run_evict(const Cache& c, const at::Tensor& w, int64_t keep, int64_t recent, const Evicted& e, bool clear, const at::Tensor& status) {
+  const KfaCache dc = cache_desc(c), dn = cache_desc(e.out);
+  const int64_t stride[2] = {w.stride(0), w.stride(1)};
+  check(api.cache_evict(&dc, w.data_ptr<float>(), stride, keep, recent, &dn, e.weights.data_ptr<float>(), e.kept.data_ptr<int32_t>(),
+                        e.out.lengths.data_ptr<int32_t>(), clear, status.data_ptr<int32_t>(), stream_of(w)));
+}
+
+void check_evict(const Cache& c, const at::Tensor& w, int64_t keep, int64_t recent) {
+  const char* who = "cache_evict";
+  check_cache(who, c);
+  check_weights(who, c, w);
+  TORCH_CHECK_VALUE(recent >= 0 && recent <= keep && keep >= 1 && keep <= 0x7fffffff, who, ": 0 <= recent <= keep, keep at least 1");
+}
+void check_evict_out(const Cache& c, const Cache& o, int64_t keep) {
+  const char* who = "cache_evict";
+  check_cache(who, o);
+  TORCH_CHECK_TYPE(o.k.scalar_type() == c.k.scalar_type(), who, ": out must have the cache's type");
+  TORCH_CHECK_VALUE(o.lengths.numel() == c.lengths.numel() && o.k.size(1) == c.k.size(1) && o.k.size(3) == c.k.size(3), who,
+                    ": out must have the cache's batch, heads and head dim");
+  TORCH_CHECK_VALUE(capacity(o) >= keep, who, ": out has room for ", std::to_string(capacity(o)), " positions, keep is ", std::to_string(keep));
+}
+
+// evict(k_pages, v_pages, lengths, table, weights, keep, recent, k_out or None, v_out, lengths of out, table_out, status) -> k_out, v_out, lengths,
+// weights, kept
+PyObject* py_evict(Args a, Py_ssize_t n) {
+  need(n, 12);
+  const char* who = "cache_evict";
+  const Cache c = cache_of(a);
+  const at::Tensor w = tensor(a[4]), status = maybe(a[11]);
+  const int64_t keep = integer(a[5]), recent = integer(a[6]);
+  const bool clear = a[7] == Py_None;
+  Evicted e;
+  if (!clear) e.out = cache_of(a + 7);
+  check_no_grad(who, {&c.k, &c.v, &w, &e.out.k, &e.out.v});
+  check_evict(c, w, keep, recent);
+  if (!clear) check_evict_out(c, e.out, keep);
+  check_where(who, c, {&w, &e.out.k, &e.out.v, &e.out.table, &status});
+  const int64_t b = c.lengths.numel(), heads = c.k.size(1);
+  released([&] {
+    const c10::cuda::CUDAGuard guard(w.device());
+    if (clear) {
+      e.out.k = at::empty({b, keep, heads, c.k.size(3)}, c.k.options()).transpose(1, 2);
+      e.out.v = at::empty({b, keep, heads, c.k.size(3)}, c.k.options()).transpose(1, 2);
+    }
+    e.out.lengths = at::empty({b}, c.lengths.options());
+    e.weights = floats(w, {b, heads, keep});
+    e.kept = at::empty({b, heads, keep}, c.lengths.options());
+    run_evict(c, w, keep, recent, e, clear, status);
+    return 0;
+  });
+  if (!clear) {
+    e.out.k.unsafeGetTensorImpl()->bump_version();
+    e.out.v.unsafeGetTensorImpl()->bump_version();
+  }
+  return pack(std::make_tuple(std::move(e.out.k), std::move(e.out.v), std::move(e.out.lengths), std::move(e.weights), std::move(e.kept)));
+}
+
+// cache_evict(k_pages, v_pages, lengths, table, weights, keep, recent, k_out, v_out, table_out, lengths_out, weights_out, kept, clear, status):
+// into tensors that are there (the registered op)
 PyObject* py_cache_evict(Args a, Py_ssize_t n) {
   need(n, 15);
   const char* who = "cache_evict";
-  const Cache c = cache_of(a), o{tensor(a[7]), tensor(a[8]), tensor(a[10]), maybe(a[9])};
-  const at::Tensor w = tensor(a[4]), w_out = tensor(a[11]), kept = tensor(a[12]), status = maybe(a[14]);
-  const int64_t keep = integer(a[5]), recent = integer(a[6]);
+  const Cache c = cache_of(a);
+  const Evicted e{{tensor(a[7]), tensor(a[8]), tensor(a[10]), maybe(a[9])}, tensor(a[11]), tensor(a[12])};
+  const at::Tensor w = tensor(a[4]), status = maybe(a[14]);
+  const int64_t keep = integer(a[5]), recent = integer(a[6]), size = c.lengths.numel() * c.k.size(1) * keep;
   const bool clear = PyObject_IsTrue(a[13]);
-  check_no_grad(who, {&c.k, &c.v, &w, &o.k, &o.v});
-  check_cache(who, c);
-  check_cache(who, o);
-  check_weights(who, c, w);
-  const int64_t b = c.lengths.numel(), heads = c.k.size(1);
-  TORCH_CHECK_TYPE(o.k.scalar_type() == c.k.scalar_type(), who, ": out must have the cache's type");
-  TORCH_CHECK_VALUE(o.lengths.numel() == b && o.k.size(1) == heads && o.k.size(3) == c.k.size(3), who,
-                    ": out must have the cache's batch, heads and head dim");
-  TORCH_CHECK_VALUE(capacity(o) >= keep, who, ": out has room for ", std::to_string(capacity(o)), " positions, keep is ", std::to_string(keep));
-  TORCH_CHECK(w_out.scalar_type() == at::kFloat && kept.scalar_type() == at::kInt && w_out.is_contiguous() && kept.is_contiguous() &&
-                  w_out.numel() == b * heads * keep && kept.numel() == b * heads * keep,
+  check_no_grad(who, {&c.k, &c.v, &w, &e.out.k, &e.out.v});
+  check_evict(c, w, keep, recent);
+  check_evict_out(c, e.out, keep);
+  TORCH_CHECK(e.weights.scalar_type() == at::kFloat && e.kept.scalar_type() == at::kInt && e.weights.is_contiguous() && e.kept.is_contiguous() &&
+                  e.weights.numel() == size && e.kept.numel() == size,
               who, ": results of another size");
-  check_where(who, c, {&w, &o.k, &o.v, &o.lengths, &o.table, &w_out, &kept, &status});
+  check_where(who, c, {&w, &e.out.k, &e.out.v, &e.out.lengths, &e.out.table, &e.weights, &e.kept, &status});
   released([&] {
     const c10::cuda::CUDAGuard guard(w.device());
-    const KfaCache dc = cache_desc(c), dn = cache_desc(o);
-    const int64_t stride[2] = {w.stride(0), w.stride(1)};
-    check(api.cache_evict(&dc, w.data_ptr<float>(), stride, keep, recent, &dn, w_out.data_ptr<float>(), kept.data_ptr<int32_t>(),
-                          o.lengths.data_ptr<int32_t>(), clear, status.data_ptr<int32_t>(), stream_of(w)));
+    run_evict(c, w, keep, recent, e, clear, status);
     return 0;
   });
-  o.k.unsafeGetTensorImpl()->bump_version();
-  o.v.unsafeGetTensorImpl()->bump_version();
   Py_RETURN_NONE;
 }
 
@@ -962,6 +1016,7 @@ PyMethodDef methods[] = {
     KFA_METHOD(cached_attention),
     KFA_METHOD(cache_append),
     KFA_METHOD(cache_weights),
+    KFA_METHOD(evict),
     KFA_METHOD(cache_evict),
     {nullptr, nullptr, 0, nullptr},
 };

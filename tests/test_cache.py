@@ -221,12 +221,56 @@ def test_attention_layouts():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dim", range(8, 129, 24))
+@pytest.mark.parametrize("tokens", [1, 30])
+def test_attention_head_dims(dim, tokens):
+    """Head dims that are multiples of 8, in both kernels (4 and 120 rows a K / V head)."""
+    check_attention(make_cache([333, 40, 0], 2, dim, torch.bfloat16, 16), 8, tokens, torch.bfloat16, "tree", seed=dim)
+
+
+@pytest.mark.gpu
+def test_attention_many_sequences():
+    """More sequences than the threads of a CTA, most of them short, some empty."""
+    gen = torch.Generator().manual_seed(0)
+    lengths = torch.randint(0, 40, (900,), generator=gen).tolist()
+    lengths[5], lengths[850], lengths[-1] = 1500, 700, 0
+    check_attention(make_cache(lengths, 1, 64, torch.float16, 8), 4, 1, torch.float16, "causal")
+
+
+@pytest.mark.gpu
+def test_attention_many_heads_and_tokens():
+    check_attention(make_cache([70], 1, 64, torch.bfloat16, 16), 300, 1, torch.bfloat16, "causal")  # two tiles of heads
+    check_attention(make_cache([100, 3], 1, 32, torch.bfloat16, 16), 4, 200, torch.bfloat16, "causal")  # four of tokens
+    check_attention(make_cache([2600], 1, 64, torch.float16, 16), 4, 20, torch.float16, "tree")  # 80 rows, cut
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tokens", [1, 40])
+def test_a_nan_that_is_seen_is_passed_on(tokens):
+    dtype = torch.bfloat16
+    cache = make_cache([200, 600], 2, 64, dtype, 16)
+    q, k, v = (rows(2, h, tokens, 64, dtype, s) for h, s in ((4, 1), (2, 2), (2, 3)))
+    clean, stats = attention_cached(q, cache, k, v, return_stats=True)
+    cache.k[int(cache.table[1, 7]), 1, 3, 9] = float("nan")
+    got, got_stats = attention_cached(q, cache, k, v, return_stats=True)
+    assert bool(torch.isnan(got[1, 2:]).all()) and bool(torch.isnan(got_stats[1, 2:, 1]).all())
+    assert torch.equal(got[0], clean[0]) and torch.equal(got[1, :2], clean[1, :2]) and torch.equal(got_stats[0], stats[0])
+    q[0, 1] = float("nan")
+    got = attention_cached(q, cache, k, v)
+    assert bool(torch.isnan(got[0, 1]).all()) and torch.equal(got[0, [0, 2, 3]], clean[0, [0, 2, 3]])
+    cache = make_cache([0, 0], 2, 64, dtype, 16)  # nothing but NaN to see
+    assert bool(torch.isnan(attention_cached(q, cache, k, v)[0, 1]).all())
+
+
+@pytest.mark.gpu
 def test_large_scores_and_scales():
     dtype = torch.float16
     cache = make_cache([300, 40], 2, 64, dtype, 16)
     q = rows(2, 4, 3, 64, dtype, 9) * 8
     check_attention(cache, 4, 3, dtype, "causal", q=q, scale=0.25)
     check_attention(cache, 4, 3, dtype, "causal", scale=0.0)
+    check_attention(cache, 4, 50, dtype, "tree", q=rows(2, 4, 50, 64, dtype, 9) * 8, scale=0.25)
+    check_attention(cache, 4, 50, dtype, "tree", scale=0.0)
     check_attention(cache, 4, 3, dtype, "none", q=-q.abs(), scale=1.0)
 
 
@@ -277,6 +321,48 @@ def test_weights(shape, accepted):
     for b, n in enumerate(lengths):
         last = 0 if counts is not None and int(counts[b]) == 0 else n + (tokens if counts is None else int(counts[b]))
         assert torch.equal(sums[b, :, last:], before[b, :, last:])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tokens", [3, 90])
+def test_weights_of_large_scores(tokens):
+    """Scores of some hundreds, where a row's maximum and log2 sum do not fit into one fp32 number: the exponent's error stays 2^-24 of the
+    score's terms (64 products of up to 8 * 4, summed: 2^-24 * 64 * 32 * 8 * 0.25 * log2 e = 2^-10.5)."""
+    dtype = torch.float16
+    cache = make_cache([300, 40], 2, 64, dtype, 16, extra=tokens)
+    q, k, v = rows(2, 4, tokens, 64, dtype, 1) * 8, rows(2, 2, tokens, 64, dtype, 2), rows(2, 2, tokens, 64, dtype, 3)
+    _, stats = attention_cached(q, cache, k, v, scale=0.25, return_stats=True)
+    cache_append(cache, k, v)
+    got = cache_weights(cache, q, stats, scale=0.25)
+    want = exact_weights(cache, q, stats, None, None, 0.25)
+    assert torch.allclose(got.double().cpu(), want, rtol=2.0**-10, atol=2.0**-24)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("heads,tokens", [(4, 6), (8, 40)])
+def test_weights_skip_what_is_not_there(heads, tokens):
+    """Rows that counts leaves out, and rows that saw nothing (m = +inf), hold NaN; weights of a tensor with wider rows; a sequence without
+    tokens; more sequences than the threads of a CTA."""
+    dtype, batch = torch.bfloat16, 500
+    gen = torch.Generator().manual_seed(1)
+    lengths = torch.randint(0, 30, (batch,), generator=gen).tolist()
+    cache = make_cache(lengths, 2, 64, dtype, 16, extra=tokens, fill=float("nan"))
+    q, k, v = (rows(batch, h, tokens, 64, dtype, s) for h, s in ((heads, 1), (2, 2), (2, 3)))
+    counts = torch.randint(0, tokens + 1, (batch,), generator=gen).to(torch.int32).cuda()
+    _, stats = attention_cached(q, cache, k, v, counts=counts, return_stats=True)
+    cache_append(cache, k, v, counts=counts)
+    behind = torch.arange(tokens, device="cuda") >= counts[:, None]
+    q.masked_fill_(behind[:, None, :, None], float("nan"))
+    stats[:, :, 0, 1] = math.inf  # the second token saw nothing
+    q[:, :, 1] = float("nan")
+    wide = torch.full((batch, 2, cache.capacity + 40), 7.0, device="cuda")
+    got = cache_weights(cache, q, stats, counts=counts, weights=wide)
+    want = exact_weights(cache, torch.nan_to_num(q), stats, None, counts, 64**-0.5)
+    assert torch.allclose(got[..., : cache.capacity].double().cpu(), want + 7, rtol=2.0**-13, atol=2.0**-13)
+    assert bool((got[..., cache.capacity :] == 7).all())
+    fresh = cache_weights(cache, q, stats, counts=counts)
+    assert torch.allclose(fresh.double().cpu(), want, rtol=2.0**-13, atol=2.0**-24)
+    assert _lib.device_status() == 0
 
 
 @pytest.mark.gpu
