@@ -384,7 +384,7 @@ __device__ __forceinline__ bool att_setup(const AttendParams& p, uint32_t bar0, 
       int count = 1;
       if (i >= R::B_KVFREE && i < R::B_Q) count = R::BOTH ? 2 : 1;
       if (i >= R::B_P && i < R::B_PV) count = 128;
-      if (i == R::B_QFREE) count = 256;
+      if (i == R::B_QFREE) count = R::BOTH ? 2 : 256;
       if (i >= R::B_OFREE && i < R::B_DRAIN) count = R::BOTH ? 128 : 256;
       mbar_init(bar0 + 8u * i, count);
     }
@@ -477,6 +477,7 @@ struct AttTile {
   int T, s;
   int uses;    // segments before in which the stream had tiles
   bool opens;  // the stream's first tile of segment s
+  bool closes; // the segment's last tile
 };
 template <bool BOTH>
 struct AttTiles {
@@ -489,7 +490,7 @@ struct AttTiles {
         ++at;
         const int now = T++;
         if (BOTH || (now & 1) == st) {
-          t = {now, s, uses, opens};
+          t = {now, s, uses, opens, at == w.tiles()};
           opens = false;
           return true;
         }
@@ -512,7 +513,7 @@ template <class R, int PIECES, int NP, typename FS, typename FP>
 __device__ __forceinline__ void att_issue(const AttendParams& p, const Walk& first, int st, uint32_t bar0, const AttCtl& ac, FS issue_S, FP issue_PV) {
   auto ready = [&](int i, uint32_t parity) { return __all_sync(0xffffffffu, mbar_test(bar0 + 8u * i, parity)); };
   AttTiles<R::BOTH> tiles{first, st};
-  AttTile ahead = {0, 0, 0, false}, even = ahead, odd = ahead;  // the next to get scores; those that have, by c (at most two wait for values)
+  AttTile ahead = {0, 0, 0, false, false}, even = ahead, odd = ahead;  // the next to get scores; those that have, by c (at most two wait for values)
   bool have = tiles.take(p, ahead);
   int i_s = 0, i_p = 0;  // pieces of scores and of values issued
   long long t0 = clock64();
@@ -1029,7 +1030,7 @@ kfa_cache_attend_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
 // ---- more rows ------------------------------------------------------------------------------------------------------------
 // HALVES: 1: up to 128 rows, tiles to the streams in turn; 2: up to 256 rows, a half of them to each stream.
 template <int NC, int HALVES>
-struct AttRowsCfg : AttRings<NC, 128 * HALVES, HALVES == 1 ? 2 : 1, HALVES == 2, 1024 + 2 * 2 * 128 * 3 * 4 + (HALVES * NC == 1 ? 32768 : 0)> {
+struct AttRowsCfg : AttRings<NC, 128 * HALVES, HALVES == 1 ? 2 : 1, HALVES == 2, 1024 + 2 * 2 * 128 * 3 * 4 + 8 * 2048> {
   static constexpr int TMEM = 512;  // S 2 x 128; O 2 x 128
 };
 
@@ -1088,6 +1089,7 @@ kfa_cache_attend_rows_kernel(const __grid_constant__ CUtensorMap tmQ, const __gr
                          k_lo + (((kk >> 2) * R::CHUNK + (kk & 3) * 32) >> 4), IDESC_S, kk > 0 ? 1u : 0u);
           umma_commit_lead(lead, bar(R::B_S + 2 * st + half));
           if (half == 1) umma_commit_lead(lead, bar(R::B_KVFREE + R::k_stage(t.T)));
+          if (BOTH && half == 1 && t.closes) umma_commit_lead(lead, bar(R::B_QFREE));  // (one buffer: the next queries come as soon as may be)
         },
         [&](const AttTile& t, int, int half) {
           const uint32_t v_lo = sdesc_lo(sKV + R::v_stage(t.T) * R::STAGE + half * 64 * 128, R::CHUNK);
@@ -1115,94 +1117,117 @@ kfa_cache_attend_rows_kernel(const __grid_constant__ CUtensorMap tmQ, const __gr
       int h, tk;
       const bool exists = rows.row(p, r, h, tk);
       float l = 0.f, m_ref = -INFINITY, m_top = -INFINITY;
-      bool opens = true;
       const int tiles = w.tiles();
-      for (int t = 0; t < tiles; ++t) {
-        const int T = T0 + t;
-        if (!BOTH && (T & 1) != st) continue;
-        const int ub = w.unit + 4 * t;
-        const bool full = 4 * t + 4 <= w.n && (ub + 4) * ATT_UNIT <= w.len && ub + 4 <= w.uc;
-        int fresh = -1;
-        bool valid = true;
-        uint32_t odd = 0u;
-        if (!full) {
-          valid = which_key(w, ub, r_in, fresh);
-          odd = odd_values<BF16>(p, w, rows.g, fresh);
-        }
+      // the stream's tiles of the segment, every STEP-th from t_first on, as pieces of 64 keys; those below t_full hold cached keys only
+      constexpr int STEP = BOTH ? 1 : 2;
+      const int t_first = BOTH || (T0 & 1) == st ? 0 : 1, pieces = 2 * ((tiles - t_first + STEP - 1) / STEP);
+      const int t_full = max(min(w.n, min(w.len / ATT_UNIT, w.uc) - w.unit), 0) / 4;
+      const int c0 = c;
+      float2 x[32];
+      bool loaded = false;
+      int fresh = -1;
+      bool valid = true;
+      uint32_t odd_bits = 0u;
 #pragma unroll 1
-        for (int half = 0; half < 2; ++half) {
-          uint32_t seen[2] = {0xffffffffu, 0xffffffffu};
-          if (!full) {
-            seen[0] = exists ? seen_word(p, w, ub + 2 * half, tk) : 0u;
-            seen[1] = exists ? seen_word(p, w, ub + 2 * half + 1, tk) : 0u;
+      for (int i = 0; i < pieces; ++i) {
+        const int half = i & 1, t = t_first + (i >> 1) * STEP;
+        c = c0 + (i >> 1);
+        const bool full = t < t_full;
+        uint32_t seen[2] = {0xffffffffu, 0xffffffffu};
+        if (!full) {
+          const int ub = w.unit + 4 * t;
+          if (half == 0) {
+            valid = which_key(w, ub, r_in, fresh);
+            odd_bits = odd_values<BF16>(p, w, rows.g, fresh);
           }
+          seen[0] = exists ? seen_word(p, w, ub + 2 * half, tk) : 0u;
+          seen[1] = exists ? seen_word(p, w, ub + 2 * half + 1, tk) : 0u;
+        }
+        if (!loaded) {
           if (ok) ok = wait_warp(bar(R::B_S + 2 * st + half), c & 1, ctl, 78);
           tc_fence_after();
-          float2 x[32];
           tmem_ld_cols<64>(tS + 64 * half, reinterpret_cast<float*>(x));
           tmem_wait_ld();
-          if (!full) {
+        }
+        if (!full) {
 #pragma unroll
-            for (int i = 0; i < 32; ++i) {
-              if (!((seen[i / 16] >> (2 * i & 31)) & 1u)) x[i].x = -INFINITY;
-              if (!((seen[i / 16] >> ((2 * i + 1) & 31)) & 1u)) x[i].y = -INFINITY;
-            }
+          for (int j = 0; j < 32; ++j) {
+            if (!((seen[j / 16] >> (2 * j & 31)) & 1u)) x[j].x = -INFINITY;
+            if (!((seen[j / 16] >> ((2 * j + 1) & 31)) & 1u)) x[j].y = -INFINITY;
           }
-          float y[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        }
+        float y[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-          for (int i = 0; i < 32; ++i) y[i & 3] = fmaxf(y[i & 3], fmaxf(x[i].x, x[i].y));
-          const float top = fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3]));
-          m_top = fmaxf(m_top, top);
-          const bool move = m_ref == -INFINITY ? top > -INFINITY : top > m_ref + p.slack;
-          if (__any_sync(0xffffffffu, move)) {
-            const float alpha = !move ? 1.f : (m_ref == -INFINITY ? 0.f : ex2((m_ref - top) * c_log2));
-            if (!opens || half > 0) {  // every product issued so far has to have retired; it is the last but one of this half's
-              const int before = 2 * c + half - 1;
-              if (ok) ok = wait_warp(bar(R::B_PV + 2 * st + (before & 1)), (before >> 1) & 1, ctl, 79);
-              tc_fence_after();
+        for (int j = 0; j < 32; ++j) y[j & 3] = fmaxf(y[j & 3], fmaxf(x[j].x, x[j].y));
+        const float top = fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3]));
+        m_top = fmaxf(m_top, top);
+        const bool move = m_ref == -INFINITY ? top > -INFINITY : top > m_ref + p.slack;
+        if (__any_sync(0xffffffffu, move)) {
+          const float alpha = !move ? 1.f : (m_ref == -INFINITY ? 0.f : ex2((m_ref - top) * c_log2));
+          if (i > 0) {  // every product issued so far has to have retired
+            const int before = 2 * c + half - 1;
+            if (ok) ok = wait_warp(bar(R::B_PV + 2 * st + (before & 1)), (before >> 1) & 1, ctl, 79);
+            tc_fence_after();
 #pragma unroll
-              for (int i = 0; i < D; i += 32) {
-                float o[32];
-                tmem_ld32(tO + i, reinterpret_cast<uint32_t*>(o));
-                tmem_wait_ld();
+            for (int k = 0; k < D; k += 32) {
+              float o[32];
+              tmem_ld32(tO + k, reinterpret_cast<uint32_t*>(o));
+              tmem_wait_ld();
 #pragma unroll
-                for (int j = 0; j < 32; ++j) o[j] *= alpha;
-                tmem_st32(tO + i, reinterpret_cast<const uint32_t*>(o));
-              }
-              tmem_wait_st();
-              l *= alpha;
+              for (int j = 0; j < 32; ++j) o[j] *= alpha;
+              tmem_st32(tO + k, reinterpret_cast<const uint32_t*>(o));
             }
-            if (move) m_ref = top;
+            tmem_wait_st();
+            l *= alpha;
           }
-          const float sh = m_ref == -INFINITY ? 0.f : -m_ref;
-          const float2 s2 = make_float2(sh, sh);
-          float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-          uint32_t pk[32];
+          if (move) m_ref = top;
+        }
+        const float sh = m_ref == -INFINITY ? 0.f : -m_ref;
+        const float2 s2 = make_float2(sh, sh);
+        float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            float2 e = __fmul2_rn(__fadd2_rn(x[i], s2), c2);
+        for (int k = 0; k < 32; k += 16) {  // (stored by the half: fewer registers at once)
+          uint32_t pk[16];
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            float2 e = __fmul2_rn(__fadd2_rn(x[k + j], s2), c2);
             e.x = ex2(e.x);
             e.y = ex2(e.y);
-            sum[i & 1] = __fadd2_rn(sum[i & 1], e);
-            pk[i] = pack16<BF16>(e.x, e.y);
+            sum[j & 1] = __fadd2_rn(sum[j & 1], e);
+            pk[j] = pack16<BF16>(e.x, e.y);
           }
-          l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
-          tmem_st32(tS + 64 * half, pk);
+          tmem_st16(tS + 64 * half + k, pk);
+        }
+        const bool early = mbar_test(bar(R::B_S + 2 * st + (half ^ 1)), (c + half) & 1);  // the next piece's scores are there already
+        l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+        if (!full && half == 0) {
+          // (The tile before has to be done with: until then the barrier of this one's stage may be a turn behind.)
+          const int stage = R::v_stage(T0 + t), turn = R::v_turn(T0 + t);
+          if (c > 0 && ok) ok = wait_warp(bar(R::B_PV + 2 * st + 1), (c - 1) & 1, ctl, 81);
+          if (ok) ok = wait_warp(bar(R::B_KV + stage), turn & 1, ctl, 82);
+          clean_values<NC, BF16>(p, w, rows.g, sKV + stage * R::STAGE, r_in, valid, fresh, odd_bits);
+          if (odd_bits != 0) ac.odd[st] = s + 1;
+          fence_async_smem();
+        }
+        // The next piece's scores are fetched while P is on its way into tensor memory. (A wait costs 300 clk even for what is there, the way
+        // in 200.)
+        loaded = i + 1 < pieces && __all_sync(0xffffffffu, early);
+        auto announce = [&] {
           tmem_wait_st();
-          if (!full && half == 0) {
-            // (The tile before has to be done with: until then the barrier of this one's stage may be a turn behind.)
-            if (c > 0 && ok) ok = wait_warp(bar(R::B_PV + 2 * st + 1), (c - 1) & 1, ctl, 81);
-            if (ok) ok = wait_warp(bar(R::B_KV + R::v_stage(T)), R::v_turn(T) & 1, ctl, 82);
-            clean_values<NC, BF16>(p, w, rows.g, sKV + R::v_stage(T) * R::STAGE, r_in, valid, fresh, odd);
-            if (odd != 0) ac.odd[st] = s + 1;
-            fence_async_smem();
-          }
           tc_fence_before();
           mbar_arrive(bar(R::B_P + 2 * st + half));
+        };
+        if (loaded) {  // (load and wait in one piece of straight code: nothing moves the registers in between)
+          tc_fence_after();
+          tmem_ld_cols<64>(tS + 64 * (half ^ 1), reinterpret_cast<float*>(x));
+          announce();
+          tmem_wait_ld();
+        } else {
+          announce();
         }
-        opens = false;
-        ++c;
       }
+      const bool opens = pieces == 0;  // the stream had no tile
+      c = c0 + pieces / 2;
       T0 += tiles;
       // ---- the segment's end ----
       if (!opens && ok) ok = wait_warp(bar(R::B_PV + 2 * st + 1), (c - 1) & 1, ctl, 83);
@@ -1251,11 +1276,10 @@ kfa_cache_attend_rows_kernel(const __grid_constant__ CUtensorMap tmQ, const __gr
         at[2 * p.rows] = top;
       }
       // Columns: all of the stream's own rows (BOTH), or every second 32 of the shared ones. A thread holds a row, and a store of 16 bytes by
-      // each of 32 rows touches 32 lines: through 4 KB a warp of the queries' buffer, which the segment has done with (of two
-      // streams' 128 rows x 64 columns: memory of its own), whole pieces of rows are written one after the other. 10000 -> 5000 clk.
-      const uint32_t turn = lane & 7;
-      const uint32_t out_stage = HALVES * NC == 1 ? smem_u32(s_fin) + 6144 + (st * 4 + wl) * 4096
-                                                  : sQ + (s % R::NQ) * R::Q_BYTES + (BOTH ? st * 128 * 128 : st * R::Q_CHUNK) + wl * 4096;
+      // each of 32 rows touches 32 lines: through 2 KB a warp of shared memory whole pieces of rows are written one after the other
+      // (10000 -> 5000 clk for 256 rows x 128 columns).
+      const uint32_t turn = (lane >> 1) & 3;
+      const uint32_t out_stage = smem_u32(s_fin) + 6144 + warp * 2048;  // 32 rows of 64 bytes
       const long long off = exists ? w.b * p.o_sb + static_cast<long long>(h) * p.o_sh + tk * p.o_ss : -1;
       const int r_warp = r - lane;
 #pragma unroll 1
@@ -1286,7 +1310,7 @@ kfa_cache_attend_rows_kernel(const __grid_constant__ CUtensorMap tmQ, const __gr
         if (whole) {
 #pragma unroll
           for (int j = 0; j < 4; ++j)  // rows of 64 bytes: 4 pieces
-            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(out_stage + lane * 64 + ((j ^ ((turn >> 1) & 3)) << 4)),
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(out_stage + lane * 64 + ((j ^ turn) << 4)),
                          "r"(pack16<BF16>(o0[8 * j], o0[8 * j + 1])), "r"(pack16<BF16>(o0[8 * j + 2], o0[8 * j + 3])),
                          "r"(pack16<BF16>(o0[8 * j + 4], o0[8 * j + 5])), "r"(pack16<BF16>(o0[8 * j + 6], o0[8 * j + 7]))
                          : "memory");
@@ -1305,32 +1329,36 @@ kfa_cache_attend_rows_kernel(const __grid_constant__ CUtensorMap tmQ, const __gr
           }
         } else {
 #pragma unroll
-          for (int j = 0; j < 8; ++j)  // rows of 128 bytes: 8 pieces
-            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(out_stage + lane * 128 + ((j ^ turn) << 4)), "r"(__float_as_uint(o0[4 * j])),
-                         "r"(__float_as_uint(o0[4 * j + 1])), "r"(__float_as_uint(o0[4 * j + 2])), "r"(__float_as_uint(o0[4 * j + 3]))
-                         : "memory");
-          __syncwarp();
+          for (int q = 0; q < 32; q += 16) {
+            if (q > 0) __syncwarp();
 #pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            const int row = 4 * k + (lane >> 3), piece = lane & 7;
-            uint4 y;
-            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-                         : "=r"(y.x), "=r"(y.y), "=r"(y.z), "=r"(y.w)
-                         : "r"(out_stage + row * 128 + ((piece ^ (row & 7)) << 4))
-                         : "memory");
-            if (r_warp + row < p.gt * p.tt) *reinterpret_cast<uint4*>(p.part_o + (slot * p.rows + r_warp + row) * 128 + i + 4 * piece) = y;
+            for (int j = 0; j < 4; ++j)
+              asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(out_stage + lane * 64 + ((j ^ turn) << 4)),
+                           "r"(__float_as_uint(o0[q + 4 * j])), "r"(__float_as_uint(o0[q + 4 * j + 1])), "r"(__float_as_uint(o0[q + 4 * j + 2])),
+                           "r"(__float_as_uint(o0[q + 4 * j + 3]))
+                           : "memory");
+            __syncwarp();
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const int row = 8 * k + (lane >> 2), piece = lane & 3;
+              uint4 y;
+              asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                           : "=r"(y.x), "=r"(y.y), "=r"(y.z), "=r"(y.w)
+                           : "r"(out_stage + row * 64 + ((piece ^ ((row >> 1) & 3)) << 4))
+                           : "memory");
+              if (r_warp + row < p.gt * p.tt) *reinterpret_cast<uint4*>(p.part_o + (slot * p.rows + r_warp + row) * 128 + i + q + 4 * piece) = y;
+            }
           }
         }
       }
-      fence_async_smem();  // (the next queries are copied over what was written)
       tc_fence_before();
       if (BOTH) {
-        mbar_arrive(bar(R::B_OFREE + st));
+        mbar_arrive(bar(R::B_OFREE + st));  // (its queries were freed by the last scores)
       } else {
+        mbar_arrive(bar(R::B_QFREE));
         if (tiles > 1 || ((T0 - 1) & 1) == 0) mbar_arrive(bar(R::B_OFREE));
         if (tiles > 1 || ((T0 - 1) & 1) == 1) mbar_arrive(bar(R::B_OFREE + 1));
       }
-      mbar_arrive(bar(R::B_QFREE));
       ++s;
       more = w.next(p);
     }
