@@ -388,11 +388,7 @@ __device__ __forceinline__ bool att_setup(const AttendParams& p, uint32_t bar0, 
       if (i >= R::B_OFREE && i < R::B_DRAIN) count = R::BOTH ? 128 : 256;
       mbar_init(bar0 + 8u * i, count);
     }
-    if (lane == 0) {
-      *ctl.abort = 0;
-      *ctl.bad = load_status(p.status) != 0;
-      ctl.odd[0] = ctl.odd[1] = 0;
-    }
+    if (lane == 0) *ctl.abort = ctl.odd[0] = ctl.odd[1] = 0;
     fence_mbar_init();
     fence_async_smem();
   }
@@ -400,10 +396,11 @@ __device__ __forceinline__ bool att_setup(const AttendParams& p, uint32_t bar0, 
     tmem_alloc(smem_u32(ctl.tmem), tmem_cols);
     tmem_relinquish();
   }
+  wait_for_previous();
+  if (warp == 10 && lane == 0) *ctl.bad = load_status(p.status) != 0;
   tc_fence_before();
   const bool work = my_work(p, ctl.ints, first, chunk, end);
   tc_fence_after();
-  if (!p.whole) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // (the joining kernel waits for this one's end all the same)
   return work;
 }
 
@@ -1380,7 +1377,7 @@ kfa_cache_attend_rows_kernel(const __grid_constant__ CUtensorMap tmQ, const __gr
 // columns. Starts while that kernel ends and waits for it.
 template <bool BF16>
 __global__ void __launch_bounds__(256) kfa_cache_join_kernel(const AttendParams p) {
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  wait_for_previous();
   const int4 meta = p.part_meta[blockIdx.x];
   if (meta.x == 0) return;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = blockIdx.y * 8 + warp;

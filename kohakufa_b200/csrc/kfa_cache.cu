@@ -151,12 +151,14 @@ AttendPlan plan_attend(int64_t batch, int64_t heads, int64_t kv_heads, int64_t T
   return a;
 }
 
-// A kernel (256 threads) that waits itself for the end of the one before it in the stream, and may be launched while that one still runs.
+// A launch that need not wait for the kernel before it in the stream to end: the kernels here wait for that themselves, behind what they
+// set up first. (Decoding of a short sequence 7.5 -> XX us, drafts of 7 tokens 15.4 -> XX, one call after the other.)
 template <typename... P>
-int launch_early(void (*kern)(P...), dim3 grid, cudaStream_t s, const P&... params) {
+int launch(void (*kern)(P...), dim3 grid, int threads, int smem, cudaStream_t s, const P&... params) {
   cudaLaunchConfig_t config = {};
   config.gridDim = grid;
-  config.blockDim = dim3(256);
+  config.blockDim = dim3(threads);
+  config.dynamicSmemBytes = smem;
   config.stream = s;
   cudaLaunchAttribute early[1];
   early[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -170,12 +172,10 @@ int launch_early(void (*kern)(P...), dim3 grid, cudaStream_t s, const P&... para
 template <bool BF16, class R, typename K>
 int launch_attend(K kern, const CUtensorMap (&m)[5], const kfa::AttendParams& p, const AttendPlan& plan, cudaStream_t s) {
   static std::atomic<uint64_t> allowed{0};
-  const int rc = allow_smem(allowed, reinterpret_cast<const void*>(kern), R::SMEM);
+  int rc = allow_smem(allowed, reinterpret_cast<const void*>(kern), R::SMEM);
   if (rc) return rc;
-  kern<<<plan.grid, kfa::ATT_THREADS, R::SMEM, s>>>(m[0], m[1], m[2], m[3], m[4], p);
-  KFA_CUDA(cudaGetLastError());
-  if (plan.whole) return KFA_OK;
-  return launch_early(kfa::kfa_cache_join_kernel<BF16>, dim3(plan.grid, (plan.gt * plan.tt + 7) / 8), s, p);
+  if ((rc = launch(kern, dim3(plan.grid), kfa::ATT_THREADS, R::SMEM, s, m[0], m[1], m[2], m[3], m[4], p)) || plan.whole) return rc;
+  return launch(kfa::kfa_cache_join_kernel<BF16>, dim3(plan.grid, (plan.gt * plan.tt + 7) / 8), 256, 0, s, p);
 }
 
 // Rows of a TMA box that a page holds whole numbers of (without a table: the last box may end behind the page, and reads zeros there).
@@ -226,11 +226,9 @@ WeighPlan plan_weigh(int64_t batch, int64_t heads, int64_t kv_heads, int64_t ste
 template <bool BF16, class R, typename K>
 int launch_weigh_few(K kern, const CUtensorMap& mk, const kfa::AttendParams& a, const kfa::WeighParams& p, const WeighPlan& plan, cudaStream_t s) {
   static std::atomic<uint64_t> allowed{0};
-  const int rc = allow_smem(allowed, reinterpret_cast<const void*>(kern), R::SMEM);
+  int rc = allow_smem(allowed, reinterpret_cast<const void*>(kern), R::SMEM);
   if (rc) return rc;
-  kern<<<plan.grid, kfa::ATT_THREADS, R::SMEM, s>>>(mk, a, p);
-  KFA_CUDA(cudaGetLastError());
-  return KFA_OK;
+  return launch(kern, dim3(plan.grid), kfa::ATT_THREADS, R::SMEM, s, mk, a, p);
 }
 template <int NC, bool BF16>
 int launch_weigh_few(const CUtensorMap& mk, const kfa::AttendParams& a, const kfa::WeighParams& p, const WeighPlan& plan, cudaStream_t s) {
@@ -245,11 +243,10 @@ int launch_weigh_many(const CUtensorMap& mq, const CUtensorMap& mk, const kfa::A
   using R = kfa::WeighRowsCfg<NC>;
   auto kern = kfa::kfa_cache_weigh_rows_kernel<NC, BF16>;
   static std::atomic<uint64_t> allowed{0};
-  const int rc = allow_smem(allowed, reinterpret_cast<const void*>(kern), R::SMEM);
+  int rc = allow_smem(allowed, reinterpret_cast<const void*>(kern), R::SMEM);
   if (rc) return rc;
-  kern<<<plan.grid, kfa::ATT_THREADS, R::SMEM, s>>>(mq, mk, a, p);
-  KFA_CUDA(cudaGetLastError());
-  return launch_early(kfa::kfa_cache_join_weights_kernel, dim3(plan.grid + a.c.batch), s, a, p, plan.grid);
+  if ((rc = launch(kern, dim3(plan.grid), kfa::ATT_THREADS, R::SMEM, s, mq, mk, a, p))) return rc;
+  return launch(kfa::kfa_cache_join_weights_kernel, dim3(plan.grid + a.c.batch), 256, 0, s, a, p, plan.grid);
 }
 
 }  // namespace
@@ -361,9 +358,7 @@ int kfa_cache_append(const KfaCache* cache, const KfaTensor4* k, const KfaTensor
   p.by_step = kfa::FastDiv::by(p.r.steps);
   p.total = static_cast<unsigned>(total);
   p.status = dev_status;
-  kfa::kfa_cache_append_kernel<<<static_cast<unsigned>((total + 255) / 256), 256, 0, static_cast<cudaStream_t>(stream)>>>(p);
-  KFA_CUDA(cudaGetLastError());
-  return KFA_OK;
+  return launch(kfa::kfa_cache_append_kernel, dim3(static_cast<unsigned>((total + 255) / 256)), 256, 0, static_cast<cudaStream_t>(stream), p);
 }
 
 int64_t kfa_cache_weigh_bytes(const KfaTensor4* q, const KfaCache* cache, const KfaRows* rows) {
@@ -441,9 +436,9 @@ int kfa_cache_weigh(const KfaTensor4* q, const float* stats, const KfaCache* cac
     p.q_to = reinterpret_cast<uint8_t*>(p.stats_to + plan.stats_floats);
     const int64_t total = static_cast<int64_t>(a.c.batch) * p.r.steps * a.H * (D / 8);
     if (total > 0xffffff00ll) return fail(KFA_ERR_ARG, "too many rows in one call");
-    kfa::kfa_cache_take_rows_kernel<<<static_cast<unsigned>((total + 255) / 256), 256, 0, s>>>(
-        a, p, p.by_piece, kfa::FastDiv::by(a.H), kfa::FastDiv::by(p.r.steps), static_cast<unsigned>(total));
-    KFA_CUDA(cudaGetLastError());
+    if ((rc = launch(kfa::kfa_cache_take_rows_kernel, dim3(static_cast<unsigned>((total + 255) / 256)), 256, 0, s, a, p, p.by_piece,
+                     kfa::FastDiv::by(a.H), kfa::FastDiv::by(p.r.steps), static_cast<unsigned>(total))))
+      return rc;
     rows_q.ptr = p.q_to;
     rows_q.shape[2] = p.r.steps;
     rows_q.stride[2] = a.H * D;
@@ -491,10 +486,9 @@ int kfa_cache_evict(const KfaCache* cache, const float* weights, const int64_t* 
   p.status = dev_status;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const dim3 heads(p.c.heads, p.c.batch);
-  if (p.c.capacity <= 2048) kfa::kfa_cache_select_kernel<256><<<heads, 256, 0, s>>>(p);
-  else kfa::kfa_cache_select_kernel<1024><<<heads, 1024, 0, s>>>(p);
-  KFA_CUDA(cudaGetLastError());
-  return launch_early(kfa::kfa_cache_gather_kernel, dim3(static_cast<unsigned>((total + 7) / 8)), s, p);
+  rc = p.c.capacity <= 2048 ? launch(kfa::kfa_cache_select_kernel<256>, heads, 256, 0, s, p) : launch(kfa::kfa_cache_select_kernel<1024>, heads, 1024, 0, s, p);
+  if (rc) return rc;
+  return launch(kfa::kfa_cache_gather_kernel, dim3(static_cast<unsigned>((total + 7) / 8)), 256, 0, s, p);
 }
 
 }  // extern "C"

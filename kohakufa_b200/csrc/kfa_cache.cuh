@@ -27,6 +27,13 @@ struct RowsView {
   __device__ __forceinline__ int row(int b, int i) const { return index ? index[b * index_stride + i] : i; }
 };
 
+// Kernels here are launched while the one before them in the stream may still run: each sets up what touches no global memory, then
+// waits for that one's end (its writes are visible then), and lets the next be launched as soon as all its own CTAs have started.
+__device__ __forceinline__ void wait_for_previous() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+
 __device__ __forceinline__ void report(int* status, int code) { atomicCAS(status, 0, code); }
 
 // The length of sequence b; one that the cache has no room for is cut off (and reported by the caller's check).
@@ -59,6 +66,7 @@ struct AppendParams {
 // A thread moves 16 bytes of a key and 16 of the value: pieces of a row fastest, then heads, then rows.
 __global__ void __launch_bounds__(256) kfa_cache_append_kernel(const AppendParams p) {
   const unsigned at = blockIdx.x * 256u + threadIdx.x;
+  wait_for_previous();
   if (at >= p.total) return;
   const unsigned row = p.by_piece.div(at), piece = at - row * p.by_piece.d;
   const unsigned rest = p.by_head.div(row), g = row - rest * p.by_head.d;
@@ -111,6 +119,7 @@ __global__ void __launch_bounds__(SELECT_THREADS) kfa_cache_select_kernel(const 
   constexpr int WARPS = SELECT_THREADS / 32, BINS = 2048, PER = BINS / SELECT_THREADS;
   const int g = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   __shared__ int hist[BINS], warp_gt[WARPS], warp_eq[WARPS], s_digit, s_need, s_all;
+  wait_for_previous();
   const int len = cache_length(p.c, b);
   if (tid == 0 && !length_ok(p.c, b)) report(p.status, DEV_BAD_CACHE);
   const float* w = p.w + b * p.w_sb + g * p.w_sh;
@@ -237,7 +246,7 @@ __global__ void __launch_bounds__(SELECT_THREADS) kfa_cache_select_kernel(const 
 // loads in flight. Bound by memory: 2 x 2 D bytes read and written a row.
 constexpr int GATHER_ROWS = 4;
 __global__ void __launch_bounds__(256) kfa_cache_gather_kernel(const EvictParams p) {
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  wait_for_previous();
   const unsigned group = blockIdx.x * 8u + (threadIdx.x >> 5);
   if (group >= p.total) return;
   const int lane = threadIdx.x & 31;

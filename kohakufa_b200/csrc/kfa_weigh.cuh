@@ -118,10 +118,7 @@ kfa_cache_weigh_kernel(const __grid_constant__ CUtensorMap tmK, const AttendPara
       if (i >= R::B_SFREE && i < R::B_DRAIN) count = 128;
       mbar_init(bar(i), count);
     }
-    if (lane == 0) {
-      *ac.abort = 0;
-      *ac.bad = load_status(a.status) != 0;
-    }
+    if (lane == 0) *ac.abort = 0;
     fence_mbar_init();
     fence_async_smem();
   }
@@ -129,6 +126,8 @@ kfa_cache_weigh_kernel(const __grid_constant__ CUtensorMap tmK, const AttendPara
     tmem_alloc(smem_u32(ac.tmem), R::TMEM);
     tmem_relinquish();
   }
+  wait_for_previous();
+  if (warp == 10 && lane == 0) *ac.bad = load_status(a.status) != 0;
   tc_fence_before();
   Walk first;
   int chunk, end;
@@ -323,6 +322,7 @@ kfa_cache_weigh_kernel(const __grid_constant__ CUtensorMap tmK, const AttendPara
 __global__ void __launch_bounds__(256) kfa_cache_take_rows_kernel(const AttendParams a, const WeighParams p, FastDiv by_piece, FastDiv by_head,
                                                                   FastDiv by_step, unsigned total) {
   const unsigned at = blockIdx.x * 256u + threadIdx.x;
+  wait_for_previous();
   if (at >= total) return;
   const unsigned row = by_piece.div(at), piece = at - row * by_piece.d;
   const unsigned rest = by_head.div(row), h = row - rest * by_head.d;
@@ -458,10 +458,7 @@ kfa_cache_weigh_rows_kernel(const __grid_constant__ CUtensorMap tmQ, const __gri
       if (i >= R::B_SFREE && i < R::B_DRAIN) count = 256;
       mbar_init(bar(i), count);
     }
-    if (lane == 0) {
-      *ac.abort = 0;
-      *ac.bad = load_status(a.status) != 0;
-    }
+    if (lane == 0) *ac.abort = 0;
     fence_mbar_init();
     fence_async_smem();
   }
@@ -469,6 +466,8 @@ kfa_cache_weigh_rows_kernel(const __grid_constant__ CUtensorMap tmQ, const __gri
     tmem_alloc(smem_u32(ac.tmem), R::TMEM);
     tmem_relinquish();
   }
+  wait_for_previous();
+  if (warp == 10 && lane == 0) *ac.bad = load_status(a.status) != 0;
   tc_fence_before();
   // which items: an equal number for each CTA
   ItemWalk first;
@@ -708,7 +707,7 @@ kfa_cache_weigh_rows_kernel(const __grid_constant__ CUtensorMap tmQ, const __gri
 // Key tiles that were cut, CTA x the one that begins in CTA x of the kernel above: w (+)= the parts, in order. The CTAs behind those: a
 // sequence each that has no items, whose weights are 0 (add: left), or NaN if its length or count says something that is not so.
 __global__ void __launch_bounds__(256) kfa_cache_join_weights_kernel(const AttendParams a, const WeighParams p, int cut) {
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  wait_for_previous();
   const float nan = __int_as_float(0x7fc00000);
   int len, count;
   if (static_cast<int>(blockIdx.x) >= cut) {
