@@ -12,7 +12,7 @@
 // A thread holds one key's scores. The maximum over keys is a warp reduction per column and an exchange between four warps; the sum
 // over keys stays in the thread until the end.
 // More rows (kfa_cache_attend_rows_kernel): rows on the matrix rows, a thread a row, P from tensor memory, as in the forward of whole
-// sequences. (A thread of the first kernel spends 3400 clk on 128 rows x 128 keys, one of this kernel 3600 on 256 x 128.)
+// sequences. (A thread of the first kernel would spend 6800 clk on 256 rows x 128 keys, one of this kernel spends 4400.)
 // In both O is rescaled only when a row's maximum grew by more than a factor of 2^8 (the numerators may be up to 2^8 then, which 16-bit P
 // takes at the same relative precision).
 //
@@ -374,7 +374,7 @@ struct AttCtl {
   }
 };
 
-// Both kernels' beginning: barriers, tensor memory, the CTA's work. p_arrivals: threads that announce a P buffer.
+// Both kernels' beginning: barriers, tensor memory, the CTA's work.
 template <class R>
 __device__ __forceinline__ bool att_setup(const AttendParams& p, uint32_t bar0, const AttCtl& ctl, int tmem_cols, Walk& first, int& chunk,
                                           int& end) {
@@ -400,6 +400,7 @@ __device__ __forceinline__ bool att_setup(const AttendParams& p, uint32_t bar0, 
   if (warp == 10 && lane == 0) *ctl.bad = load_status(p.status) != 0;
   tc_fence_before();
   const bool work = my_work(p, ctl.ints, first, chunk, end);
+  let_next_begin();
   tc_fence_after();
   return work;
 }
@@ -1373,59 +1374,102 @@ kfa_cache_attend_rows_kernel(const __grid_constant__ CUtensorMap tmQ, const __gr
   }
 }
 
-// Joins the parts of the items that were cut: CTA x has the item that begins in CTA x of the kernel above, a warp a row, a lane four
-// columns. Starts while that kernel ends and waits for it.
-template <bool BF16>
+// Joins the parts of the items that were cut: CTA x has the item that begins in CTA x of the kernel above, LANES lanes a row. Starts while
+// that kernel ends and waits for it. A chunk of LANES parts at a time: each lane has the factor of one, and all add up their columns; the
+// first AHEAD parts' columns are on their way while the factors are found. With many rows in few parts its cost is the instructions for a
+// row, which four rows of a warp share (16 trees of 64 tokens, 256 rows in two parts: 101.0 us with a warp a row, 96.4 with 8 lanes); with
+// few rows in many parts it is the loop over the parts (16 rows in 18: 88.4 us with a warp a row, 90.1 with 8 lanes).
+template <bool BF16, int LANES>
 __global__ void __launch_bounds__(256) kfa_cache_join_kernel(const AttendParams p) {
+  constexpr int VECS = 32 / LANES, AHEAD = LANES == 32 ? 4 : 2;
   wait_for_previous();
+  let_next_begin();
   const int4 meta = p.part_meta[blockIdx.x];
   if (meta.x == 0) return;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = blockIdx.y * 8 + warp;
+  const int lane = threadIdx.x % LANES;
+  int r = blockIdx.y * (256 / LANES) + threadIdx.x / LANES;
   const RowMap rows(p, meta.z);
   int h, t;
-  if (!rows.row(p, r, h, t)) return;
+  const bool exists = rows.row(p, r, h, t);
+  if (!exists) r = 0;  // (row 0 always exists; its lanes only keep the others company)
   const bool bad = *reinterpret_cast<const volatile int*>(p.status) != 0;
   const int count = p.counts ? min(max(p.counts[meta.y], 0), p.T) : p.T;
   // part i: the first in slot 1 of its CTA, the others in slot 0 of theirs
   auto slot = [&](int i) { return 2ll * (blockIdx.x + i) + (i == 0 ? 1 : 0); };
-  float m = -INFINITY, top = -INFINITY;
-  for (int i = lane; i < meta.x; i += 32) {
-    const float* ml = p.part_ml + slot(i) * 3 * p.rows + r;
-    m = fmaxf(m, ml[0]);
-    top = fmaxf(top, ml[2 * p.rows]);
-  }
-  m = warp_max(m);
-  top = warp_max(top);
-  float l = 0.f;
-  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int i0 = 0; i0 < meta.x; i0 += 32) {
-    float a = 0.f, li = 0.f;
-    if (i0 + lane < meta.x) {
+  const float* o_row = p.part_o + r * 128 + 4 * lane;
+  float m = -INFINITY, top = -INFINITY, l = 0.f;
+  float4 o[VECS];
+#pragma unroll
+  for (int v = 0; v < VECS; ++v) o[v] = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int i0 = 0; i0 < meta.x; i0 += LANES) {
+    const int n = min(LANES, meta.x - i0);
+    float4 x[AHEAD][VECS];
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+      const float* from = o_row + slot(i0 + min(i, n - 1)) * p.rows * 128;
+#pragma unroll
+      for (int v = 0; v < VECS; ++v) x[i][v] = *reinterpret_cast<const float4*>(from + 4 * LANES * v);
+    }
+    float mi = -INFINITY, li = 0.f, ti = -INFINITY;
+    if (lane < n) {
       const float* ml = p.part_ml + slot(i0 + lane) * 3 * p.rows + r;
-      a = part_factor(ml[0], ml[p.rows], m, p.c_log2);
-      li = a * ml[p.rows];
+      mi = ml[0];
+      li = ml[p.rows];
+      ti = ml[2 * p.rows];
     }
-    const int n = min(32, meta.x - i0);
-#pragma unroll 4
-    for (int i = 0; i < n; ++i) {
-      const float ai = __shfl_sync(0xffffffffu, a, i);
-      l += __shfl_sync(0xffffffffu, li, i);
-      const float4 x = *reinterpret_cast<const float4*>(p.part_o + (slot(i0 + i) * p.rows + r) * 128 + 4 * lane);
+    float m_new = fmaxf(m, mi);
+#pragma unroll
+    for (int k = 1; k < LANES; k *= 2) {
+      m_new = fmaxf(m_new, __shfl_xor_sync(0xffffffffu, m_new, k));
+      ti = fmaxf(ti, __shfl_xor_sync(0xffffffffu, ti, k));
+    }
+    top = fmaxf(top, ti);
+    if (i0) {
+      const float a = part_factor(m, l, m_new, p.c_log2);
+      l *= a;
+#pragma unroll
+      for (int v = 0; v < VECS; ++v) o[v] = make_float4(o[v].x * a, o[v].y * a, o[v].z * a, o[v].w * a);
+    }
+    m = m_new;
+    const float a = lane < n ? part_factor(mi, li, m, p.c_log2) : 0.f;
+    li *= a;
+    auto add = [&](int i, const float4 (&y)[VECS]) {
+      const float ai = __shfl_sync(0xffffffffu, a, i, LANES);
+      l += __shfl_sync(0xffffffffu, li, i, LANES);
       if (ai != 0.f) {
-        o.x += ai * x.x;
-        o.y += ai * x.y;
-        o.z += ai * x.z;
-        o.w += ai * x.w;
+#pragma unroll
+        for (int v = 0; v < VECS; ++v) {
+          o[v].x += ai * y[v].x;
+          o[v].y += ai * y[v].y;
+          o[v].z += ai * y[v].z;
+          o[v].w += ai * y[v].w;
+        }
       }
+    };
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i)
+      if (i < n) add(i, x[i]);
+#pragma unroll 2
+    for (int i = AHEAD; i < n; ++i) {
+      const float* from = o_row + slot(i0 + i) * p.rows * 128;
+      float4 y[VECS];
+#pragma unroll
+      for (int v = 0; v < VECS; ++v) y[v] = *reinterpret_cast<const float4*>(from + 4 * LANES * v);
+      add(i, y);
     }
   }
+  if (!exists) return;
   const bool some = t < count && l != 0.f;
   const float nan = __int_as_float(0x7fc00000), inv = some ? 1.f / l : 0.f;
-  if (bad) o = make_float4(nan, nan, nan, nan);
-  else if (!some) o = make_float4(0.f, 0.f, 0.f, 0.f);
-  else o = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
-  if (4 * lane < p.c.cols)
-    *reinterpret_cast<uint2*>(p.o + meta.y * p.o_sb + h * p.o_sh + t * p.o_ss + 8 * lane) = make_uint2(pack16<BF16>(o.x, o.y), pack16<BF16>(o.z, o.w));
+  unsigned char* out = p.o + meta.y * p.o_sb + h * p.o_sh + t * p.o_ss + 8 * lane;
+#pragma unroll
+  for (int v = 0; v < VECS; ++v) {
+    float4 y = make_float4(o[v].x * inv, o[v].y * inv, o[v].z * inv, o[v].w * inv);
+    if (!some) y = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (bad) y = make_float4(nan, nan, nan, nan);
+    if (4 * (lane + LANES * v) < p.c.cols)
+      *reinterpret_cast<uint2*>(out + 8 * LANES * v) = make_uint2(pack16<BF16>(y.x, y.y), pack16<BF16>(y.z, y.w));
+  }
   if (p.stats && lane == 0) {
     float* at = p.stats + (static_cast<long long>(meta.y) * p.H + h) * 2 * p.T + t;
     at[0] = bad ? nan : (some ? top : INFINITY);

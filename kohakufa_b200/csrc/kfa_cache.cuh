@@ -28,11 +28,10 @@ struct RowsView {
 };
 
 // Kernels here are launched while the one before them in the stream may still run: each sets up what touches no global memory, then
-// waits for that one's end (its writes are visible then), and lets the next be launched as soon as all its own CTAs have started.
-__device__ __forceinline__ void wait_for_previous() {
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-}
+// waits for that one's end (its writes are visible then), and lets the next be launched as soon as all its own CTAs have come that far.
+// One that uses tensor memory lets it only when it has its own: the next one's CTAs keep theirs while they wait.
+__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void let_next_begin() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
 __device__ __forceinline__ void report(int* status, int code) { atomicCAS(status, 0, code); }
 
@@ -67,6 +66,7 @@ struct AppendParams {
 __global__ void __launch_bounds__(256) kfa_cache_append_kernel(const AppendParams p) {
   const unsigned at = blockIdx.x * 256u + threadIdx.x;
   wait_for_previous();
+  let_next_begin();
   if (at >= p.total) return;
   const unsigned row = p.by_piece.div(at), piece = at - row * p.by_piece.d;
   const unsigned rest = p.by_head.div(row), g = row - rest * p.by_head.d;
@@ -120,6 +120,7 @@ __global__ void __launch_bounds__(SELECT_THREADS) kfa_cache_select_kernel(const 
   const int g = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   __shared__ int hist[BINS], warp_gt[WARPS], warp_eq[WARPS], s_digit, s_need, s_all;
   wait_for_previous();
+  let_next_begin();
   const int len = cache_length(p.c, b);
   if (tid == 0 && !length_ok(p.c, b)) report(p.status, DEV_BAD_CACHE);
   const float* w = p.w + b * p.w_sb + g * p.w_sh;
@@ -247,6 +248,7 @@ __global__ void __launch_bounds__(SELECT_THREADS) kfa_cache_select_kernel(const 
 constexpr int GATHER_ROWS = 4;
 __global__ void __launch_bounds__(256) kfa_cache_gather_kernel(const EvictParams p) {
   wait_for_previous();
+  let_next_begin();
   const unsigned group = blockIdx.x * 8u + (threadIdx.x >> 5);
   if (group >= p.total) return;
   const int lane = threadIdx.x & 31;

@@ -132,6 +132,7 @@ kfa_cache_weigh_kernel(const __grid_constant__ CUtensorMap tmK, const AttendPara
   Walk first;
   int chunk, end;
   const bool work = my_work(a, ac.ints, first, chunk, end);
+  let_next_begin();
   tc_fence_after();
   const uint32_t tmem = *ac.tmem;
   const Ctl ctl{ac.abort};
@@ -323,6 +324,7 @@ __global__ void __launch_bounds__(256) kfa_cache_take_rows_kernel(const AttendPa
                                                                   FastDiv by_step, unsigned total) {
   const unsigned at = blockIdx.x * 256u + threadIdx.x;
   wait_for_previous();
+  let_next_begin();
   if (at >= total) return;
   const unsigned row = by_piece.div(at), piece = at - row * by_piece.d;
   const unsigned rest = by_head.div(row), h = row - rest * by_head.d;
@@ -482,6 +484,7 @@ kfa_cache_weigh_rows_kernel(const __grid_constant__ CUtensorMap tmQ, const __gri
               ac.ints[3 * i] = b;
               ac.ints[3 * i + 1] = off;
             });
+  let_next_begin();
   tc_fence_after();
   first.left = min(share[1], total) - share[0];
   const bool work = first.left > 0;
@@ -708,6 +711,7 @@ kfa_cache_weigh_rows_kernel(const __grid_constant__ CUtensorMap tmQ, const __gri
 // sequence each that has no items, whose weights are 0 (add: left), or NaN if its length or count says something that is not so.
 __global__ void __launch_bounds__(256) kfa_cache_join_weights_kernel(const AttendParams a, const WeighParams p, int cut) {
   wait_for_previous();
+  let_next_begin();
   const float nan = __int_as_float(0x7fc00000);
   int len, count;
   if (static_cast<int>(blockIdx.x) >= cut) {
