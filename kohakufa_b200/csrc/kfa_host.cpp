@@ -723,6 +723,16 @@ void check_no_grad(const char* who, std::initializer_list<const at::Tensor*> ten
 
 void check_scale(const char* who, double scale) { TORCH_CHECK_VALUE(std::isfinite(scale) && scale >= 0, who, ": scale must be finite and not negative"); }
 
+// Pages that a call writes: a place that is both a key's and a value's would get whichever came last.
+void check_written(const char* who, const Cache& c) {
+  TORCH_CHECK_VALUE(c.k.data_ptr() != c.v.data_ptr(), who, ": keys and values that are written must have memory of their own");
+}
+
+// (Before the launch: it refuses inference tensors outside of inference mode.)
+void will_write(std::initializer_list<const at::Tensor*> tensors) {
+  for (const at::Tensor* t : tensors) t->unsafeGetTensorImpl()->bump_version();
+}
+
 KfaCache cache_desc(const Cache& c) {
   KfaCache d{desc(c.k), desc(c.v), nullptr, 0, 0, c.lengths.data_ptr<int32_t>(), c.lengths.numel()};
   if (c.table.defined()) {
@@ -795,7 +805,9 @@ PyObject* py_cache_append(Args a, Py_ssize_t n) {
   check_new(who, "v", c, v, c.k.size(1));
   TORCH_CHECK_VALUE(k.size(2) == v.size(2), who, ": k and v must have as many tokens");
   const KfaRows rows = rows_of(who, c, index, counts, k.size(2));
+  check_written(who, c);
   check_where(who, c, {&k, &v, &index, &counts, &status});
+  will_write({&c.k, &c.v});
   released([&] {
     const c10::cuda::CUDAGuard guard(k.device());
     const KfaCache dc = cache_desc(c);
@@ -803,8 +815,6 @@ PyObject* py_cache_append(Args a, Py_ssize_t n) {
     check(api.cache_append(&dc, &dk, &dv, &rows, status.data_ptr<int32_t>(), stream_of(k)));
     return 0;
   });
-  c.k.unsafeGetTensorImpl()->bump_version();
-  c.v.unsafeGetTensorImpl()->bump_version();
   Py_RETURN_NONE;
 }
 
@@ -836,6 +846,7 @@ PyObject* py_cache_weights(Args a, Py_ssize_t n) {
     TORCH_CHECK_VALUE(w.size(i) == 1 || w.stride(i) >= w.size(2), who, ": weights must not overlap itself");
   check_scale(who, scale);
   check_where(who, c, {&q, &stats, &index, &counts, &w, &status});
+  will_write({&w});
   released([&] {
     const c10::cuda::CUDAGuard guard(q.device());
     const KfaCache dc = cache_desc(c);
@@ -848,7 +859,6 @@ PyObject* py_cache_weights(Args a, Py_ssize_t n) {
                           stream_of(q)));
     return 0;
   });
-  w.unsafeGetTensorImpl()->bump_version();
   Py_RETURN_NONE;
 }
 
@@ -878,6 +888,10 @@ void check_evict_out(const Cache& c, const Cache& o, int64_t keep) {
   TORCH_CHECK_VALUE(o.lengths.numel() == c.lengths.numel() && o.k.size(1) == c.k.size(1) && o.k.size(3) == c.k.size(3), who,
                     ": out must have the cache's batch, heads and head dim");
   TORCH_CHECK_VALUE(capacity(o) >= keep, who, ": out has room for ", std::to_string(capacity(o)), " positions, keep is ", std::to_string(keep));
+  check_written(who, o);
+  // (two tables over one pool may name different pages)
+  const bool tables = c.table.defined() && o.table.defined() && c.table.data_ptr() != o.table.data_ptr();
+  TORCH_CHECK_VALUE(tables || (c.k.data_ptr() != o.k.data_ptr() && c.v.data_ptr() != o.v.data_ptr()), who, ": out must have pages of its own");
 }
 
 // evict(k_pages, v_pages, lengths, table, weights, keep, recent, k_out or None, v_out, lengths of out, table_out, status) -> k_out, v_out, lengths,
@@ -896,6 +910,7 @@ PyObject* py_evict(Args a, Py_ssize_t n) {
   if (!clear) check_evict_out(c, e.out, keep);
   check_where(who, c, {&w, &e.out.k, &e.out.v, &e.out.table, &status});
   const int64_t b = c.lengths.numel(), heads = c.k.size(1);
+  if (!clear) will_write({&e.out.k, &e.out.v});
   released([&] {
     const c10::cuda::CUDAGuard guard(w.device());
     if (clear) {
@@ -908,10 +923,6 @@ PyObject* py_evict(Args a, Py_ssize_t n) {
     run_evict(c, w, keep, recent, e, clear, status);
     return 0;
   });
-  if (!clear) {
-    e.out.k.unsafeGetTensorImpl()->bump_version();
-    e.out.v.unsafeGetTensorImpl()->bump_version();
-  }
   return pack(std::make_tuple(std::move(e.out.k), std::move(e.out.v), std::move(e.out.lengths), std::move(e.weights), std::move(e.kept)));
 }
 

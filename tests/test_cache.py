@@ -575,6 +575,100 @@ def test_other_stream():
 
 
 @pytest.mark.gpu
+def test_a_pool_of_more_than_32_bits():
+    """Pages whose offsets pass 2^32 bytes, read and written; the pool's other pages hold whatever was there."""
+    page, dim, count = 16, 128, 1_100_000  # 4.5 GB each
+    k, v = (torch.empty(count, page, 1, dim, dtype=torch.bfloat16, device="cuda").transpose(1, 2) for _ in range(2))
+    gen = torch.Generator().manual_seed(0)
+    table = torch.randint(1_060_000, count, (2, 24), generator=gen).unique()[:40].flip(0).view(2, 20).to(torch.int32).cuda()
+    cache = KVCache(k, v, torch.tensor([200, 37], dtype=torch.int32).cuda(), table)
+    for pages in (k, v):
+        pages[table.long()] = torch.randn(2, 20, 1, page, dim, generator=gen).to(torch.bfloat16).cuda()
+    small = KVCache(k[table.flatten().long()], v[table.flatten().long()], cache.lengths, torch.arange(40, dtype=torch.int32).view(2, 20).cuda())
+    q, kn, vn = (rows(2, h, 5, dim, torch.bfloat16, s) for h, s in ((4, 1), (1, 2), (1, 3)))
+    results = []
+    for c in (cache, small):
+        out, stats = attention_cached(q, c, kn, vn, return_stats=True)
+        cache_append(c, kn, vn)
+        weights = cache_weights(c, q, stats)
+        left, w_left, kept = cache_evict(c, weights, 40, recent=3)
+        results.append((out, stats, weights, left.k, left.v, w_left, kept, c.k[c.table.long()], c.v[c.table.long()]))
+    for a, b in zip(*results):
+        assert torch.equal(a, b)
+    assert _lib.device_status() == 0
+
+
+@pytest.mark.gpu
+def test_eviction_inside_one_pool_captured():
+    """Out of some pages of a pool into others, in a graph: positions, lengths and weights are read when it runs."""
+    pool = make_cache([128] * 8, 2, 64, torch.float16, 16)
+    lengths, tables = torch.tensor([100, 9, 40], dtype=torch.int32).cuda(), [pool.table[i : i + 3].clone() for i in (0, 3)]
+    source, target = (KVCache(pool.k, pool.v, lengths, t) for t in tables)
+    weights = torch.rand(3, 2, 128, device="cuda")
+    cache_evict(source, weights, 24, recent=4, out=target)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got, w_out, kept = cache_evict(source, weights, 24, recent=4, out=target)
+    for n in ([100, 9, 40], [128, 0, 24], [25, 128, 1]):
+        lengths.copy_(torch.tensor(n, dtype=torch.int32))
+        weights.copy_(torch.rand(3, 2, 128))
+        k, rest = logical(source, "k"), logical(pool, "k")[6:]
+        graph.replay()
+        want = expect_evicted(weights, n, 24, 4)
+        assert torch.equal(kept.cpu(), want) and got.lengths.tolist() == [min(x, 24) for x in n]
+        moved = k.gather(2, want.clamp(min=0).long()[..., None].expand(-1, -1, -1, 64))
+        assert torch.equal(logical(got, "k")[:, :, :24][want >= 0], moved[want >= 0])
+        assert torch.equal(logical(source, "k"), k) and torch.equal(logical(pool, "k")[6:], rest)
+    assert _lib.device_status() == 0
+
+
+@pytest.mark.gpu
+def test_inference_mode():
+    with torch.inference_mode():
+        cache = KVCache.empty(2, 2, 64, 64)
+        q, k, v = (rows(2, h, 3, 64, torch.bfloat16, s) for h, s in ((8, 1), (2, 2), (2, 3)))
+        out, stats = attention_cached(q, cache, k, v, return_stats=True)
+        cache_append(cache, k, v)
+        weights = cache_weights(cache, q, stats)
+        cache.lengths += 3
+        less, _, _ = cache_evict(cache, weights, 2, out=KVCache.empty(2, 2, 8, 64))
+        assert torch.equal(cache.k[:, :, :3], k) and less.lengths.tolist() == [2, 2]
+    before = cache.k.clone()
+    with pytest.raises(RuntimeError, match="nference"):  # as torch has it for every write
+        cache_append(cache, k, v)
+    assert torch.equal(cache.k, before)
+
+
+@pytest.mark.gpu
+def test_calls_one_behind_the_other_among_others():
+    """A long run of calls on two streams between kernels of every other kind, without a wait on the host: each result as if alone."""
+    cache = make_cache([900, 30, 2000], 2, 128, torch.bfloat16, 16, extra=70)
+    cases = [(t, [rows(3, h, t, 128, torch.bfloat16, 7 * t + i) for i, h in enumerate((8, 2, 2))]) for t in (1, 5, 16, 64)]
+    want = []
+    for _, (q, k, v) in cases:
+        out, stats = attention_cached(q, cache, k, v, return_stats=True)
+        cache_append(cache, k, v)
+        want.append((out, cache_weights(cache, q, stats)))
+    streams, got = [torch.cuda.Stream(), torch.cuda.Stream()], []
+    caches = [KVCache(cache.k.clone(), cache.v.clone(), cache.lengths, cache.table) for _ in streams]
+    torch.cuda.synchronize()
+    for n in range(24):
+        for stream, c in zip(streams, caches):
+            with torch.cuda.stream(stream):
+                i = n % len(cases)
+                q, k, v = cases[i][1]
+                q = q * 1.0  # (a kernel of another library right before and behind)
+                out, stats = attention_cached(q, c, k, v, return_stats=True)
+                cache_append(c, k, v)
+                got.append((i, out * 1.0, cache_weights(c, q, stats)))
+    torch.cuda.synchronize()
+    for i, out, weights in got:
+        assert torch.equal(out, want[i][0]) and torch.equal(weights, want[i][1])
+    assert _lib.device_status() == 0
+
+
+@pytest.mark.gpu
 def test_compiled_calls_take_the_custom_ops():
     cache = make_cache([60, 12], 2, 64, torch.bfloat16, 16, extra=3)
     q, k, v = (rows(2, h, 3, 64, torch.bfloat16, s) for h, s in ((8, 1), (2, 2), (2, 3)))
@@ -718,6 +812,7 @@ def test_refused_calls():
         (ValueError, (c, k, k), dict(index=ints(3, 2))),
         (ValueError, (c, k, k), dict(index=ints(2, 0))),
         (ValueError, (c, k, k), dict(counts=ints(1))),
+        (ValueError, (KVCache(c.k, c.k, c.lengths, c.table), k, k), {}),
         (RuntimeError, (c, k.clone().requires_grad_(), k), {}),
     ):
         with pytest.raises(error, match="cache_append"):
@@ -736,7 +831,7 @@ def test_refused_calls():
     ):
         with pytest.raises(error, match="cache_weights"):
             cache_weights(*args, **more)
-    other = cpu_cache(k=bf(4, 1, 16, 64), v=bf(4, 1, 16, 64))
+    other, other_pages = cpu_cache(k=bf(4, 1, 16, 64), v=bf(4, 1, 16, 64)), cpu_cache()
     for error, args, more in (
         (ValueError, (c, w, 16), {}),
         (ValueError, (c, w, 0), {}),
@@ -747,6 +842,10 @@ def test_refused_calls():
         (ValueError, (c, w, 4), dict(out=c)),
         (ValueError, (c, w, 4), dict(out=other)),
         (ValueError, (c, w, 33), dict(out=cpu_cache())),
+        (ValueError, (c, w, 4), dict(out=KVCache(c.k, c.v, ints(2), c.table))),
+        (ValueError, (c, w, 4), dict(out=KVCache(c.k, bf(4, 2, 16, 64), ints(2), c.table))),
+        (ValueError, (c, w, 4), dict(out=KVCache(c.k[:2], c.v[:2], ints(2)))),
+        (ValueError, (c, w, 4), dict(out=KVCache(other_pages.k, other_pages.k, ints(2), c.table))),
     ):
         with pytest.raises(error, match="cache_evict"):
             cache_evict(*args, **more)
