@@ -60,7 +60,7 @@ struct AttendParams {
   int rows;        // of scratch per part
   int appended;    // the new tokens are in the cache already (cache_weights): positions lengths .. lengths + counts - 1
   float c_log2, slack;  // scale * log2 e; how far a maximum may grow before O is rescaled
-  float* part_o;   // [slot][rows][128]
+  float* part_o;   // [slot][rows][128]; of the kernel for more rows [slot][rows / 32][128 / 4][32][4]
   float* part_ml;  // [slot][3][rows]: m, l, largest score
   int4* part_meta; // [CTA]: parts of the item that begins in it and ends in another (0: none), sequence, item
   int* status;
@@ -1274,8 +1274,8 @@ kfa_cache_attend_rows_kernel(const __grid_constant__ CUtensorMap tmQ, const __gr
         at[2 * p.rows] = top;
       }
       // Columns: all of the stream's own rows (BOTH), or every second 32 of the shared ones. A thread holds a row, and a store of 16 bytes by
-      // each of 32 rows touches 32 lines: through 2 KB a warp of shared memory whole pieces of rows are written one after the other
-      // (10000 -> 5000 clk for 256 rows x 128 columns).
+      // each of 32 rows touches 32 lines: through 2 KB a warp of shared memory whole pieces of rows are written one after the other. A part
+      // lies as the threads have it, 4 columns of 32 rows after 4 columns of 32 rows: each store is 512 bytes in one piece.
       const uint32_t turn = (lane >> 1) & 3;
       const uint32_t out_stage = smem_u32(s_fin) + 6144 + warp * 2048;  // 32 rows of 64 bytes
       const long long off = exists ? w.b * p.o_sb + static_cast<long long>(h) * p.o_sh + tk * p.o_ss : -1;
@@ -1325,28 +1325,10 @@ kfa_cache_attend_rows_kernel(const __grid_constant__ CUtensorMap tmQ, const __gr
             if (bad) y = make_uint4(0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu);
             if (at >= 0 && i + 8 * piece < p.c.cols) *reinterpret_cast<uint4*>(p.o + at + 2 * i + 16 * piece) = y;
           }
-        } else {
+        } else if (r_warp < p.gt * p.tt) {
+          float4* at = reinterpret_cast<float4*>(p.part_o + (slot * p.rows + r_warp) * 128) + 8 * i + lane;
 #pragma unroll
-          for (int q = 0; q < 32; q += 16) {
-            if (q > 0) __syncwarp();
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-              asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(out_stage + lane * 64 + ((j ^ turn) << 4)),
-                           "r"(__float_as_uint(o0[q + 4 * j])), "r"(__float_as_uint(o0[q + 4 * j + 1])), "r"(__float_as_uint(o0[q + 4 * j + 2])),
-                           "r"(__float_as_uint(o0[q + 4 * j + 3]))
-                           : "memory");
-            __syncwarp();
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const int row = 8 * k + (lane >> 2), piece = lane & 3;
-              uint4 y;
-              asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-                           : "=r"(y.x), "=r"(y.y), "=r"(y.z), "=r"(y.w)
-                           : "r"(out_stage + row * 64 + ((piece ^ ((row >> 1) & 3)) << 4))
-                           : "memory");
-              if (r_warp + row < p.gt * p.tt) *reinterpret_cast<uint4*>(p.part_o + (slot * p.rows + r_warp + row) * 128 + i + q + 4 * piece) = y;
-            }
-          }
+          for (int j = 0; j < 8; ++j) at[32 * j] = make_float4(o0[4 * j], o0[4 * j + 1], o0[4 * j + 2], o0[4 * j + 3]);
         }
       }
       tc_fence_before();
@@ -1374,42 +1356,33 @@ kfa_cache_attend_rows_kernel(const __grid_constant__ CUtensorMap tmQ, const __gr
   }
 }
 
-// Joins the parts of the items that were cut: CTA x has the item that begins in CTA x of the kernel above, LANES lanes a row. Starts while
-// that kernel ends and waits for it. A chunk of LANES parts at a time: each lane has the factor of one, and all add up their columns; the
-// first AHEAD parts' columns are on their way while the factors are found. With many rows in few parts its cost is the instructions for a
-// row, which four rows of a warp share (16 trees of 64 tokens, 256 rows in two parts: 101.0 us with a warp a row, 96.4 with 8 lanes); with
-// few rows in many parts it is the loop over the parts (16 rows in 18: 88.4 us with a warp a row, 90.1 with 8 lanes).
-template <bool BF16, int LANES>
+// Joins the parts of the items that were cut: CTA x has the item that begins in CTA x of the kernel above, a warp a row, a lane four
+// columns. Starts while that kernel ends and waits for it. 32 parts at a time: a lane has the factor of one, and all add up their columns; the
+// first AHEAD parts' columns are on their way while the factors are found (drafts of 7 tokens 15.2 -> 14.2 us).
+template <bool BF16>
 __global__ void __launch_bounds__(256) kfa_cache_join_kernel(const AttendParams p) {
-  constexpr int VECS = 32 / LANES, AHEAD = LANES == 32 ? 4 : 2;
+  constexpr int AHEAD = 4;
   wait_for_previous();
   let_next_begin();
   const int4 meta = p.part_meta[blockIdx.x];
   if (meta.x == 0) return;
-  const int lane = threadIdx.x % LANES;
-  int r = blockIdx.y * (256 / LANES) + threadIdx.x / LANES;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = blockIdx.y * 8 + warp;
   const RowMap rows(p, meta.z);
   int h, t;
-  const bool exists = rows.row(p, r, h, t);
-  if (!exists) r = 0;  // (row 0 always exists; its lanes only keep the others company)
+  if (!rows.row(p, r, h, t)) return;
   const bool bad = *reinterpret_cast<const volatile int*>(p.status) != 0;
   const int count = p.counts ? min(max(p.counts[meta.y], 0), p.T) : p.T;
   // part i: the first in slot 1 of its CTA, the others in slot 0 of theirs
   auto slot = [&](int i) { return 2ll * (blockIdx.x + i) + (i == 0 ? 1 : 0); };
   const float* o_row = p.part_o + r * 128 + 4 * lane;
   float m = -INFINITY, top = -INFINITY, l = 0.f;
-  float4 o[VECS];
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int i0 = 0; i0 < meta.x; i0 += 32) {
+    const int n = min(32, meta.x - i0);
+    auto part = [&](int i) { return *reinterpret_cast<const float4*>(o_row + slot(i0 + i) * p.rows * 128); };
+    float4 x[AHEAD];
 #pragma unroll
-  for (int v = 0; v < VECS; ++v) o[v] = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int i0 = 0; i0 < meta.x; i0 += LANES) {
-    const int n = min(LANES, meta.x - i0);
-    float4 x[AHEAD][VECS];
-#pragma unroll
-    for (int i = 0; i < AHEAD; ++i) {
-      const float* from = o_row + slot(i0 + min(i, n - 1)) * p.rows * 128;
-#pragma unroll
-      for (int v = 0; v < VECS; ++v) x[i][v] = *reinterpret_cast<const float4*>(from + 4 * LANES * v);
-    }
+    for (int i = 0; i < AHEAD; ++i) x[i] = part(min(i, n - 1));
     float mi = -INFINITY, li = 0.f, ti = -INFINITY;
     if (lane < n) {
       const float* ml = p.part_ml + slot(i0 + lane) * 3 * p.rows + r;
@@ -1417,60 +1390,97 @@ __global__ void __launch_bounds__(256) kfa_cache_join_kernel(const AttendParams 
       li = ml[p.rows];
       ti = ml[2 * p.rows];
     }
-    float m_new = fmaxf(m, mi);
-#pragma unroll
-    for (int k = 1; k < LANES; k *= 2) {
-      m_new = fmaxf(m_new, __shfl_xor_sync(0xffffffffu, m_new, k));
-      ti = fmaxf(ti, __shfl_xor_sync(0xffffffffu, ti, k));
-    }
-    top = fmaxf(top, ti);
+    const float m_new = fmaxf(m, warp_max(mi));
+    top = fmaxf(top, warp_max(ti));
     if (i0) {
       const float a = part_factor(m, l, m_new, p.c_log2);
       l *= a;
-#pragma unroll
-      for (int v = 0; v < VECS; ++v) o[v] = make_float4(o[v].x * a, o[v].y * a, o[v].z * a, o[v].w * a);
+      o = make_float4(o.x * a, o.y * a, o.z * a, o.w * a);
     }
     m = m_new;
     const float a = lane < n ? part_factor(mi, li, m, p.c_log2) : 0.f;
     li *= a;
-    auto add = [&](int i, const float4 (&y)[VECS]) {
-      const float ai = __shfl_sync(0xffffffffu, a, i, LANES);
-      l += __shfl_sync(0xffffffffu, li, i, LANES);
+    auto add = [&](int i, const float4& y) {
+      const float ai = __shfl_sync(0xffffffffu, a, i);
+      l += __shfl_sync(0xffffffffu, li, i);
       if (ai != 0.f) {
-#pragma unroll
-        for (int v = 0; v < VECS; ++v) {
-          o[v].x += ai * y[v].x;
-          o[v].y += ai * y[v].y;
-          o[v].z += ai * y[v].z;
-          o[v].w += ai * y[v].w;
-        }
+        o.x += ai * y.x;
+        o.y += ai * y.y;
+        o.z += ai * y.z;
+        o.w += ai * y.w;
       }
     };
 #pragma unroll
     for (int i = 0; i < AHEAD; ++i)
       if (i < n) add(i, x[i]);
-#pragma unroll 2
-    for (int i = AHEAD; i < n; ++i) {
-      const float* from = o_row + slot(i0 + i) * p.rows * 128;
-      float4 y[VECS];
-#pragma unroll
-      for (int v = 0; v < VECS; ++v) y[v] = *reinterpret_cast<const float4*>(from + 4 * LANES * v);
-      add(i, y);
-    }
+#pragma unroll 4
+    for (int i = AHEAD; i < n; ++i) add(i, part(i));
   }
-  if (!exists) return;
   const bool some = t < count && l != 0.f;
   const float nan = __int_as_float(0x7fc00000), inv = some ? 1.f / l : 0.f;
-  unsigned char* out = p.o + meta.y * p.o_sb + h * p.o_sh + t * p.o_ss + 8 * lane;
-#pragma unroll
-  for (int v = 0; v < VECS; ++v) {
-    float4 y = make_float4(o[v].x * inv, o[v].y * inv, o[v].z * inv, o[v].w * inv);
-    if (!some) y = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (bad) y = make_float4(nan, nan, nan, nan);
-    if (4 * (lane + LANES * v) < p.c.cols)
-      *reinterpret_cast<uint2*>(out + 8 * LANES * v) = make_uint2(pack16<BF16>(y.x, y.y), pack16<BF16>(y.z, y.w));
-  }
+  if (bad) o = make_float4(nan, nan, nan, nan);
+  else if (!some) o = make_float4(0.f, 0.f, 0.f, 0.f);
+  else o = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+  if (4 * lane < p.c.cols)
+    *reinterpret_cast<uint2*>(p.o + meta.y * p.o_sb + h * p.o_sh + t * p.o_ss + 8 * lane) = make_uint2(pack16<BF16>(o.x, o.y), pack16<BF16>(o.z, o.w));
   if (p.stats && lane == 0) {
+    float* at = p.stats + (static_cast<long long>(meta.y) * p.H + h) * 2 * p.T + t;
+    at[0] = bad ? nan : (some ? top : INFINITY);
+    at[p.T] = bad ? nan : (some ? log2f(l) + (m - top) * p.c_log2 : 0.f);
+  }
+}
+
+// The same for the kernel for more rows, whose parts lie by columns: a lane a row, a warp 16 columns of 32 rows, nothing exchanged. One pass:
+// what is there is scaled down when a part has a larger maximum. (16 trees of 64 tokens, 256 rows mostly in two parts: 102.9 us with parts by
+// rows and a warp a row, 96.4 with 8 lanes a row, 93.7 so.)
+template <bool BF16>
+__global__ void __launch_bounds__(256) kfa_cache_join_rows_kernel(const AttendParams p) {
+  wait_for_previous();
+  let_next_begin();
+  const int4 meta = p.part_meta[blockIdx.x];
+  if (meta.x == 0) return;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = blockIdx.y * 32 + lane;
+  const RowMap rows(p, meta.z);
+  int h, t;
+  if (16 * warp >= p.c.cols || !rows.row(p, r, h, t)) return;
+  const bool bad = *reinterpret_cast<const volatile int*>(p.status) != 0;
+  const int count = p.counts ? min(max(p.counts[meta.y], 0), p.T) : p.T;
+  const float* ml = p.part_ml + (2ll * blockIdx.x + 1) * 3 * p.rows + r;  // the first part in slot 1 of its CTA, the others in slot 0 of theirs
+  const float4* from = reinterpret_cast<const float4*>(p.part_o + ((2ll * blockIdx.x + 1) * p.rows + 32 * blockIdx.y) * 128) + 128 * warp + lane;
+  float m = -INFINITY, top = -INFINITY, l = 0.f, o[16];
+#pragma unroll
+  for (int k = 0; k < 16; ++k) o[k] = 0.f;
+#pragma unroll 2
+  for (int i = 0; i < meta.x; ++i) {
+    const float mi = ml[0], li = ml[p.rows], ti = ml[2 * p.rows];
+    float4 x[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) x[k] = from[32 * k];
+    const int next = i == 0 ? 1 : 2;  // slots
+    ml += next * 3 * p.rows;
+    from += next * p.rows * 32;
+    const float m_new = fmaxf(m, mi), f = part_factor(m, l, m_new, p.c_log2), fi = part_factor(mi, li, m_new, p.c_log2);
+    top = fmaxf(top, ti);
+    m = m_new;
+    l = l * f + li * fi;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float y[4] = {x[k].x, x[k].y, x[k].z, x[k].w};
+#pragma unroll
+      for (int q = 0; q < 4; ++q) o[4 * k + q] = o[4 * k + q] * f + (fi == 0.f ? 0.f : y[q] * fi);
+    }
+  }
+  const bool some = t < count && l != 0.f;
+  const float nan = __int_as_float(0x7fc00000), inv = some ? 1.f / l : 0.f;
+#pragma unroll
+  for (int k = 0; k < 16; ++k) o[k] = bad ? nan : (some ? o[k] * inv : 0.f);
+  unsigned char* out = p.o + meta.y * p.o_sb + h * p.o_sh + t * p.o_ss + 32 * warp;
+#pragma unroll
+  for (int k = 0; k < 16; k += 8)
+    if (16 * warp + k < p.c.cols)
+      *reinterpret_cast<uint4*>(out + 2 * k) = make_uint4(pack16<BF16>(o[k], o[k + 1]), pack16<BF16>(o[k + 2], o[k + 3]),
+                                                          pack16<BF16>(o[k + 4], o[k + 5]), pack16<BF16>(o[k + 6], o[k + 7]));
+  if (p.stats && warp == 0) {
     float* at = p.stats + (static_cast<long long>(meta.y) * p.H + h) * 2 * p.T + t;
     at[0] = bad ? nan : (some ? top : INFINITY);
     at[p.T] = bad ? nan : (some ? log2f(l) + (m - top) * p.c_log2 : 0.f);

@@ -176,9 +176,8 @@ int launch_attend(K kern, const CUtensorMap (&m)[5], const kfa::AttendParams& p,
   int rc = allow_smem(allowed, reinterpret_cast<const void*>(kern), R::SMEM);
   if (rc) return rc;
   if ((rc = launch(kern, dim3(plan.grid), kfa::ATT_THREADS, R::SMEM, s, m[0], m[1], m[2], m[3], m[4], p)) || plan.whole) return rc;
-  const int rows = plan.gt * plan.tt;
-  if (rows <= 16) return launch(kfa::kfa_cache_join_kernel<BF16, 32>, dim3(plan.grid, (rows + 7) / 8), 256, 0, s, p);
-  return launch(kfa::kfa_cache_join_kernel<BF16, 8>, dim3(plan.grid, (rows + 31) / 32), 256, 0, s, p);
+  if (plan.rows > 64) return launch(kfa::kfa_cache_join_rows_kernel<BF16>, dim3(plan.grid, (plan.gt * plan.tt + 31) / 32), 256, 0, s, p);
+  return launch(kfa::kfa_cache_join_kernel<BF16>, dim3(plan.grid, (plan.gt * plan.tt + 7) / 8), 256, 0, s, p);
 }
 
 // Rows of a TMA box that a page holds whole numbers of (without a table: the last box may end behind the page, and reads zeros there).
