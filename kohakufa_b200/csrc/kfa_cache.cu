@@ -488,7 +488,7 @@ int kfa_cache_evict(const KfaCache* cache, const float* weights, const int64_t* 
   p.status = dev_status;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const dim3 heads(p.c.heads, p.c.batch);
-  rc = p.c.capacity <= 2048 ? launch(kfa::kfa_cache_select_kernel<256>, heads, 256, 0, s, p) : launch(kfa::kfa_cache_select_kernel<1024>, heads, 1024, 0, s, p);
+  rc = p.c.capacity <= 2048 ? launch(kfa::kfa_cache_select_kernel<512>, heads, 512, 0, s, p) : launch(kfa::kfa_cache_select_kernel<1024>, heads, 1024, 0, s, p);
   if (rc) return rc;
   return launch(kfa::kfa_cache_gather_kernel, dim3(static_cast<unsigned>((total + 7) / 8)), 256, 0, s, p);
 }

@@ -111,9 +111,9 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
 // Which positions stay, per (sequence, K / V head). The key of the last one that stays is found digit by digit (11, 11 and 10 bits, from the
 // top): a histogram of the digit among the positions that agree in the digits before it. It ends early when all that agree stay. Then every
 // warp takes a stretch of the positions, counts those above that key and those equal to it, and lists them in ascending order: all above it
-// stay, of the equal ones the first, until there are enough. Bound by latency; the first 8192 positions are read once and held.
-// SELECT_THREADS: 256 for caches of up to 2048 positions, else 1024 (a cache of 320 positions 9.2 us with 512, 11.3 with 1024; 8192
-// positions 23 us with 512, 13.5 with 1024).
+// stay, of the equal ones the first, until there are enough. Bound by latency; a thread's first 8 positions are read once and held.
+// SELECT_THREADS: 512 for caches of up to 2048 positions, else 1024. (The whole call in us with 256, 512, 1024: 2 x 4 heads over 320
+// positions 10.7, 10.0, 11.1; 16 x 8 over 1500 to 8192 93.7, 76.8, 57.4.)
 template <int SELECT_THREADS>
 __global__ void __launch_bounds__(SELECT_THREADS) kfa_cache_select_kernel(const EvictParams p) {
   constexpr int WARPS = SELECT_THREADS / 32, BINS = 2048, PER = BINS / SELECT_THREADS;
