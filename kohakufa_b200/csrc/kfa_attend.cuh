@@ -260,7 +260,7 @@ struct AttRings {
   // barriers: tiles there and free, queries there, scores there, P there, P V done, a segment is finished, a stream's O has been read (in the
   // segments in which the stream had tiles), all done
   static constexpr int B_KV = 0, B_KVFREE = NS, B_Q = 2 * NS, B_S = B_Q + NQ, B_P = B_S + 4, B_PV = B_P + 4, B_QFREE = B_PV + 4,
-                       B_OFREE = B_QFREE + 1, B_DRAIN = B_OFREE + 2, N_BARS = B_DRAIN + 2;
+                       B_OFREE = B_QFREE + NQ, B_DRAIN = B_OFREE + 2, N_BARS = B_DRAIN + 2;
   static_assert(N_BARS * 8 + 256 <= 1024, "barrier block");
 };
 
@@ -384,7 +384,7 @@ __device__ __forceinline__ bool att_setup(const AttendParams& p, uint32_t bar0, 
       int count = 1;
       if (i >= R::B_KVFREE && i < R::B_Q) count = R::BOTH ? 2 : 1;
       if (i >= R::B_P && i < R::B_PV) count = 128;
-      if (i == R::B_QFREE) count = R::BOTH ? 2 : 256;
+      if (i >= R::B_QFREE && i < R::B_OFREE) count = R::BOTH ? 2 : 256;
       if (i >= R::B_OFREE && i < R::B_DRAIN) count = R::BOTH ? 128 : 256;
       mbar_init(bar0 + 8u * i, count);
     }
@@ -422,7 +422,7 @@ __device__ __forceinline__ void att_produce(const AttendParams& p, const Walk& f
     if (lane == 0 && !length_ok(p.c, w.b)) *ac.bad = 1;
     if (!values) {
       if (s >= R::NQ) {  // both streams are done with the segment that used this buffer
-        ok = wait_warp(bar(R::B_QFREE), (s - R::NQ) & 1, ctl, 70);
+        ok = wait_warp(bar(R::B_QFREE + s % R::NQ), (s / R::NQ - 1) & 1, ctl, 70);
         if (!ok) break;
       }
       if (lane == 0) {
@@ -1007,7 +1007,7 @@ kfa_cache_attend_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
       tc_fence_before();
       if (tiles > 1 || ((T0 - 1) & 1) == 0) mbar_arrive(bar(R::B_OFREE));
       if (tiles > 1 || ((T0 - 1) & 1) == 1) mbar_arrive(bar(R::B_OFREE + 1));
-      mbar_arrive(bar(R::B_QFREE));
+      mbar_arrive(bar(R::B_QFREE + s % R::NQ));
       ++s;
       more = w.next(p);
     }
@@ -1087,7 +1087,7 @@ kfa_cache_attend_rows_kernel(const __grid_constant__ CUtensorMap tmQ, const __gr
                          k_lo + (((kk >> 2) * R::CHUNK + (kk & 3) * 32) >> 4), IDESC_S, kk > 0 ? 1u : 0u);
           umma_commit_lead(lead, bar(R::B_S + 2 * st + half));
           if (half == 1) umma_commit_lead(lead, bar(R::B_KVFREE + R::k_stage(t.T)));
-          if (BOTH && half == 1 && t.closes) umma_commit_lead(lead, bar(R::B_QFREE));  // (one buffer: the next queries come as soon as may be)
+          if (BOTH && half == 1 && t.closes) umma_commit_lead(lead, bar(R::B_QFREE + t.s % R::NQ));  // (one buffer: the next queries come as soon as may be)
         },
         [&](const AttTile& t, int, int half) {
           const uint32_t v_lo = sdesc_lo(sKV + R::v_stage(t.T) * R::STAGE + half * 64 * 128, R::CHUNK);
@@ -1335,7 +1335,7 @@ kfa_cache_attend_rows_kernel(const __grid_constant__ CUtensorMap tmQ, const __gr
       if (BOTH) {
         mbar_arrive(bar(R::B_OFREE + st));  // (its queries were freed by the last scores)
       } else {
-        mbar_arrive(bar(R::B_QFREE));
+        mbar_arrive(bar(R::B_QFREE + s % R::NQ));
         if (tiles > 1 || ((T0 - 1) & 1) == 0) mbar_arrive(bar(R::B_OFREE));
         if (tiles > 1 || ((T0 - 1) & 1) == 1) mbar_arrive(bar(R::B_OFREE + 1));
       }

@@ -89,7 +89,7 @@ struct WeighCfg {
   static constexpr int SMALL = 1024 + 2 * N * 8;
   static constexpr int SMEM = 1024 + NS * STAGE + 2 * Q_BYTES + SMALL;
   static constexpr int TMEM = N == 64 ? 256 : (N == 32 ? 128 : 64);  // S 2 x 2
-  static constexpr int B_K = 0, B_KFREE = NS, B_Q = 2 * NS, B_QFREE = B_Q + 2, B_S = B_QFREE + 1, B_SFREE = B_S + 4, B_DRAIN = B_SFREE + 4,
+  static constexpr int B_K = 0, B_KFREE = NS, B_Q = 2 * NS, B_QFREE = B_Q + 2, B_S = B_QFREE + 2, B_SFREE = B_S + 4, B_DRAIN = B_SFREE + 4,
                        N_BARS = B_DRAIN + 2;
   static_assert(SMEM <= 232448 && N_BARS * 8 + 256 <= 1024, "shared memory");
 };
@@ -114,7 +114,7 @@ kfa_cache_weigh_kernel(const __grid_constant__ CUtensorMap tmK, const AttendPara
     for (int i = lane; i < R::N_BARS; i += 32) {
       int count = 1;
       if (i >= R::B_Q && i < R::B_QFREE) count = 32;
-      if (i == R::B_QFREE) count = 256;
+      if (i >= R::B_QFREE && i < R::B_S) count = 256;
       if (i >= R::B_SFREE && i < R::B_DRAIN) count = 128;
       mbar_init(bar(i), count);
     }
@@ -182,7 +182,7 @@ kfa_cache_weigh_kernel(const __grid_constant__ CUtensorMap tmK, const AttendPara
     const int pieces = a.c.cols / 8;
     while (more && ok) {
       const int g = static_cast<int>(a.by_row_tiles.div(w.item));
-      if (s >= 2) ok = wait_warp(bar(R::B_QFREE), (s - 2) & 1, ctl, 85);
+      if (s >= 2) ok = wait_warp(bar(R::B_QFREE + (s & 1)), ((s >> 1) - 1) & 1, ctl, 85);
       if (!ok) break;
       if (lane == 0) {
         const int len = a.c.lengths[w.b];
@@ -267,13 +267,13 @@ kfa_cache_weigh_kernel(const __grid_constant__ CUtensorMap tmK, const AttendPara
       const int g = static_cast<int>(a.by_row_tiles.div(w.item)), tiles = w.tiles();
       const int old = w.len - w.count;  // positions before the first of these tokens
       float* out = p.w + w.b * p.w_sb + g * p.w_sh;
-      // (its statistics are there: the keys' scores are waited for below, but a stream without tiles in the segment looks at nothing)
+      // Both streams wait for every segment's queries, with a tile in it or not: neither says twice that a buffer is free before the other has.
+      if (ok) ok = wait_warp(bar(R::B_Q + (s & 1)), (s >> 1) & 1, ctl, 89);
       for (int t = 0; t < tiles; ++t) {
         if (((T0 + t) & 1) != st) continue;
         const int pos0 = (w.unit + 4 * t) * ATT_UNIT, pos = pos0 + key;
         const bool mine = pos < w.len && (key >> 5) < w.n - 4 * t;
         const float before = p.add && mine ? out[pos] : 0.f;
-        if (ok) ok = wait_warp(bar(R::B_Q + (s & 1)), (s >> 1) & 1, ctl, 89);
         if (ok) ok = wait_warp(bar(R::B_S + 2 * st + (c & 1)), (c >> 1) & 1, ctl, 90);
         tc_fence_after();
         float x[N];
@@ -290,7 +290,7 @@ kfa_cache_weigh_kernel(const __grid_constant__ CUtensorMap tmK, const AttendPara
       T0 += tiles;
       if (w.ends() && !p.add)  // behind the last position
         for (int i = w.len + tid; i < p.room; i += 256) out[i] = 0.f;
-      mbar_arrive(bar(R::B_QFREE));
+      mbar_arrive(bar(R::B_QFREE + (s & 1)));
       ++s;
       more = w.next(a);
     }

@@ -366,6 +366,37 @@ def test_weights_skip_what_is_not_there(heads, tokens):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dim", [80, 64])
+def test_weights_of_many_short_pieces(dim):
+    """Sequences without tokens next to others: a CTA's two streams take a piece each, and while one waits for its keys the other is done
+    with pieces that have none. Long sequences between them keep the memory busy."""
+    batch, kv_heads = 200, 8
+    gen = torch.Generator().manual_seed(4)
+    counts = torch.randint(0, 2, (batch,), generator=gen).to(torch.int32).cuda()
+    lengths = [(900, 639, 100, 30, 1)[int(i)] for i in torch.randint(0, 5, (batch,), generator=gen)]
+    cache = make_cache(lengths, kv_heads, dim, torch.float16, extra=4)
+    q, k, v = (rows(batch, kv_heads, 4, dim, torch.float16, s) for s in (1, 2, 3))
+    _, stats = attention_cached(q, cache, k, v, return_stats=True)
+    cache_append(cache, k, v, counts=counts)
+    want = exact_weights(cache, q, stats, None, counts, dim**-0.5)
+    other = torch.empty(1 << 28, dtype=torch.uint8, device="cuda")
+    first = None
+    for n in range(60):
+        if n % 2 == 0:
+            other.fill_(n)  # (the keys come from memory, not from the cache of the device)
+        got = cache_weights(cache, q, stats, counts=counts)
+        first = got if first is None else first
+        assert torch.equal(got, first), n
+    assert torch.allclose(first.double().cpu(), want, rtol=2.0**-13, atol=2.0**-24)
+    out = attention_cached(q, cache, k, v, counts=counts)
+    for n in range(60):
+        if n % 2 == 0:
+            other.fill_(n)
+        assert torch.equal(attention_cached(q, cache, k, v, counts=counts), out), n
+    assert _lib.device_status() == 0
+
+
+@pytest.mark.gpu
 def test_weights_of_a_prompt_sum_to_its_rows():
     """Every row's weights add up to 1: with an empty cache all positions together got one per row and head."""
     dtype, tokens = torch.bfloat16, 700
