@@ -135,9 +135,9 @@ AttendPlan plan_attend(int64_t batch, int64_t heads, int64_t kv_heads, int64_t T
   const int64_t items = batch * kv_heads * a.row_tiles;
   const int64_t units = std::max<int64_t>((capacity + 31) / 32 + (fresh ? (T + 31) / 32 : 0), 1);
   a.whole = units <= 8;
-  // What an item's beginning and end take, in units of 32 keys. Graph time per call in us with 4, 8, 12, 16, 24: 64 sequences of 1 to 4096
-  // positions, one token each (D = 128) 116, 105, 101, 103, 103; 32 x 12 heads over 0 to 1500 (D = 80) 44, 34, 30, 28, 28; 8 sequences of 300 to
-  // 2048, 7 tokens (D = 64) 17.5, 16.5, 15.4, 15.7, 15.6; 16 of 2048 to 4096, 256 rows 116, 112, 111, 105, 106.
+  // What an item's beginning and end take, in units of 32 keys. Graph time per call in us with 8, 10, 12, 14: 64 sequences of 1 to 4096 positions,
+  // one token each (D = 128) 104.6, 100.0, 98.6, 99.5; 32 x 12 heads over 0 to 1500 (D = 80) 34.8, 32.4, 30.2, 29.6; 8 sequences of 300 to 2048,
+  // 7 tokens (D = 64) 15.4, 14.3, 14.1, 14.2. With 10, 13, 16, 20: 16 sequences of 2048 to 4096, 256 rows 94.1, 94.3, 93.7, 93.7.
   a.extra = a.rows > 64 ? 16 : 12;
   a.least = 4;
   a.most_units = items * (units + a.extra);
