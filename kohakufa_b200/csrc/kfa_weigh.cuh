@@ -38,6 +38,10 @@ __device__ __forceinline__ float2 row_stats(const AttendParams& a, const WeighPa
   return make_float2(at[0], at[p.r.T]);
 }
 
+// How many of a tile's rows, `heads` a token, stand before a key that lies `ahead` positions behind the tile's first token: those do not see it.
+// (Most keys lie far before the token: the product of that distance would pass 32 bits in a long cache. Behind the token are less than 256, what is left of its tile and of the rows' tile.)
+__device__ __forceinline__ int rows_before(int ahead, int heads) { return max(ahead, 0) * heads; }
+
 // The weights of a key, summed: N scores against N rows, whose -m and -log2 l stand one after the other (two at a time in the packed
 // instructions). slow: some rows are not there (-m = -inf, and their scores may be anything), or do not see the key: those below r_min.
 template <int N>
@@ -283,7 +287,7 @@ kfa_cache_weigh_kernel(const __grid_constant__ CUtensorMap tmK, const AttendPara
         mbar_arrive(bar(R::B_SFREE + 2 * st + (c & 1)));
         // (tokens that are not there have m = +inf; their scores come from what the buffer held before)
         const float* rows = s_rows + (s & 1) * 2 * N;
-        const float sum = weigh_scores<N>(x, rows, rows + N, a.c_log2, true, (pos - old) * a.gt);  // (token i sees positions up to old + i)
+        const float sum = weigh_scores<N>(x, rows, rows + N, a.c_log2, true, rows_before(pos - old, a.gt));  // (token i sees positions up to old + i)
         if (mine) out[pos] = *ac.bad != 0 ? __int_as_float(0x7fc00000) : before + sum;
         ++c;
       }
@@ -650,7 +654,7 @@ kfa_cache_weigh_rows_kernel(const __grid_constant__ CUtensorMap tmQ, const __gri
             if (one) {
               part += weigh_scores_one<32>(x, rows + i, a.c_log2);
             } else {  // (token t sees positions up to len + t)
-              part += weigh_scores<32>(x, rows + 128 + i, rows + 256 + i, a.c_log2, true, (pos - w.len - token) * p.tile_h - 64 * half - i);
+              part += weigh_scores<32>(x, rows + 128 + i, rows + 256 + i, a.c_log2, true, rows_before(pos - w.len - token, p.tile_h) - 64 * half - i);
             }
           }
           mbar_arrive(bar(R::B_STFREE + slot));
