@@ -333,10 +333,11 @@ __device__ __forceinline__ void columns_over_lanes(float* x, int lane) {
   }
 }
 
-// What a part with maximum m and sum l counts beside the maximum of all parts: nothing if it saw no key (its O is not defined
-// then); a sum that is NaN without any maximum (all its scores were NaN) counts, as NaN.
+// What a part with maximum m and sum l counts beside the maximum of all parts: < 0 if it saw no key (its O is not defined then, its l is 0);
+// a sum that is NaN without any maximum (all its scores were NaN) counts, as NaN. A part that counts 0 because its scores are far below the others' is
+// multiplied like the rest: 0 * NaN of a value that is seen is NaN, whatever part the value lies in.
 __device__ __forceinline__ float part_factor(float m, float l, float m_all, float c_log2) {
-  if (m == -INFINITY) return l == 0.f ? 0.f : 1.f;
+  if (m == -INFINITY) return l == 0.f ? -1.f : 1.f;
   return ex2((m - m_all) * c_log2);
 }
 
@@ -964,8 +965,8 @@ kfa_cache_attend_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
           at[0] = bad ? nan : (some ? top : INFINITY);
           at[p.T] = bad ? nan : (some ? log2f(l_all) + (m - top) * c_log2 : 0.f);
         }
-        a0 = some ? a0 * inv : 0.f;
-        a1 = some ? a1 * inv : 0.f;
+        a0 = some ? a0 * inv : -1.f;
+        a1 = some ? a1 * inv : -1.f;
       } else if (wl == 0 && lane < W) {
         float* at = p.part_ml + slot * 3 * p.rows + c0 + lane;
         at[0] = m;
@@ -979,7 +980,7 @@ kfa_cache_attend_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
 #pragma unroll
       for (int i = 0; i < W; ++i) {
         const float x0 = __shfl_sync(0xffffffffu, a0, i), x1 = __shfl_sync(0xffffffffu, a1, i);
-        o0[i] = (x0 == 0.f ? 0.f : o0[i] * x0) + (x1 == 0.f ? 0.f : o1[i] * x1);  // (a stream without tiles has left nothing there)
+        o0[i] = (x0 < 0.f ? 0.f : o0[i] * x0) + (x1 < 0.f ? 0.f : o1[i] * x1);  // (a stream without tiles has left nothing there)
       }
       if (d < p.c.cols) {
         for (int j = j0; j < j1; ++j) {
@@ -1265,8 +1266,8 @@ kfa_cache_attend_rows_kernel(const __grid_constant__ CUtensorMap tmQ, const __gr
           at[0] = bad ? nan : (some ? top : INFINITY);
           at[p.T] = bad ? nan : (some ? log2f(l_all) + (m - top) * c_log2 : 0.f);
         }
-        a0 = some ? a0 * inv : 0.f;
-        a1 = some ? a1 * inv : 0.f;
+        a0 = some ? a0 * inv : -1.f;
+        a1 = some ? a1 * inv : -1.f;
       } else if (writes && r < p.gt * p.tt) {
         float* at = p.part_ml + slot * 3 * p.rows + r;
         at[0] = m;
@@ -1286,13 +1287,13 @@ kfa_cache_attend_rows_kernel(const __grid_constant__ CUtensorMap tmQ, const __gr
         tmem_ld32((BOTH ? tO : tmem + 256 + lane_base) + i, reinterpret_cast<uint32_t*>(o0));
         tmem_wait_ld();
 #pragma unroll
-        for (int j = 0; j < 32; ++j) o0[j] = a0 == 0.f ? 0.f : o0[j] * a0;
+        for (int j = 0; j < 32; ++j) o0[j] = a0 < 0.f ? 0.f : o0[j] * a0;
         if constexpr (!BOTH) {
           float o1[32];
           tmem_ld32(tmem + 384 + lane_base + i, reinterpret_cast<uint32_t*>(o1));
           tmem_wait_ld();
 #pragma unroll
-          for (int j = 0; j < 32; ++j) o0[j] += a1 == 0.f ? 0.f : o1[j] * a1;
+          for (int j = 0; j < 32; ++j) o0[j] += a1 < 0.f ? 0.f : o1[j] * a1;
         }
         for (int j = j0; j < j1; ++j) {
           if (!exists || !sees_new(p, w, tk, j)) continue;
@@ -1393,17 +1394,17 @@ __global__ void __launch_bounds__(256) kfa_cache_join_kernel(const AttendParams 
     const float m_new = fmaxf(m, warp_max(mi));
     top = fmaxf(top, warp_max(ti));
     if (i0) {
-      const float a = part_factor(m, l, m_new, p.c_log2);
+      const float before = part_factor(m, l, m_new, p.c_log2), a = before < 0.f ? 0.f : before;
       l *= a;
       o = make_float4(o.x * a, o.y * a, o.z * a, o.w * a);
     }
     m = m_new;
-    const float a = lane < n ? part_factor(mi, li, m, p.c_log2) : 0.f;
+    const float a = lane < n ? part_factor(mi, li, m, p.c_log2) : -1.f;
     li *= a;
     auto add = [&](int i, const float4& y) {
       const float ai = __shfl_sync(0xffffffffu, a, i);
       l += __shfl_sync(0xffffffffu, li, i);
-      if (ai != 0.f) {
+      if (!(ai < 0.f)) {
         o.x += ai * y.x;
         o.y += ai * y.y;
         o.z += ai * y.z;
@@ -1467,7 +1468,7 @@ __global__ void __launch_bounds__(256) kfa_cache_join_rows_kernel(const AttendPa
     for (int k = 0; k < 4; ++k) {
       const float y[4] = {x[k].x, x[k].y, x[k].z, x[k].w};
 #pragma unroll
-      for (int q = 0; q < 4; ++q) o[4 * k + q] = o[4 * k + q] * f + (fi == 0.f ? 0.f : y[q] * fi);
+      for (int q = 0; q < 4; ++q) o[4 * k + q] = o[4 * k + q] * f + (fi < 0.f ? 0.f : y[q] * fi);
     }
   }
   const bool some = t < count && l != 0.f;

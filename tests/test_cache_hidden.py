@@ -6,7 +6,7 @@ import math
 import pytest
 import torch
 
-from kohakufa_b200 import _lib, attention_cached
+from kohakufa_b200 import KVCache, _lib, attention_cached
 from tests.test_cache import check_attention, make_cache, random_tree, rows
 
 TOKENS = [2, 5, 20, 40]  # 8, 20, 80 and 160 rows
@@ -76,3 +76,30 @@ def test_rows_that_see_nothing(tokens, columns):
     assert bool((got[0, :, :-1] == 0).all()) and bool((got[1] != 0).any(-1).all())
     got = check_attention(make_cache([0, 10], 2, 128, dtype, 16, columns=columns), 8, tokens, dtype, "none")
     assert bool((got[0] == 0).all()) and bool((got[1] != 0).any(-1).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tokens", TOKENS)
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("length,places", [(240, [50, 130, 239]), (6000, [0, 200, 3000, 5990])], ids=["short", "long"])
+def test_a_value_that_is_seen_is_passed_on_whatever_its_weight(tokens, dtype, length, places):
+    """0 * NaN is NaN: a visible value that is not finite shows in its column also where its weight is 0 in fp32, whichever tile, stream or part
+    it lies in. The first 128 positions' scores are 1024, the others' -1024."""
+    dim = 64
+    cache = make_cache([length], 2, dim, dtype, 16, spare=0)
+    at = torch.arange(length, device="cuda")
+    page, slot = cache.table[0].long()[at // 16], at % 16
+    cache.k.transpose(1, 2)[page, slot] = torch.where(at < 128, 4.0, -4.0).to(dtype)[:, None, None].expand(length, 2, dim)
+    q = torch.full((1, tokens, 8, dim), 4.0, dtype=dtype, device="cuda").transpose(1, 2)
+    clean = attention_cached(q, cache, scale=1.0)
+    assert bool(torch.isfinite(clean).all())
+    for place in places:
+        for what in (math.nan, math.inf):
+            v = cache.v.clone()
+            v[int(page[place]), 1, int(slot[place]), 5] = what
+            got = attention_cached(q, KVCache(cache.k, v, cache.lengths, cache.table), scale=1.0)
+            touched = torch.zeros_like(clean, dtype=torch.bool)
+            touched[:, 4:, :, 5] = True
+            assert not bool(torch.isfinite(got[touched]).any()), place
+            assert torch.equal(got[~touched], clean[~touched])
+    assert _lib.device_status() == 0
