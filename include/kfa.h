@@ -340,7 +340,8 @@ int kfa_cache_weigh(const KfaTensor4* q, const float* stats, const KfaCache* cac
  * weights (fp32 [B, Hkv, >= capacity], strides in floats; of equal ones the lower position; NaN counts as largest). They are
  * written to positions 0, 1, ... of `out` in ascending order (out->lengths is not read; its capacity is at least keep, and the pages that are written are none of those that are read).
  * kept: int32 [B, Hkv, keep], the positions, -1 behind the last; weights_out: fp32 [B, Hkv, keep], their weights, 0 behind the last;
- * lengths_out: int32 [B]. clear: rows of `out` behind the last kept position up to keep are zeroed, else left. */
+ * lengths_out: int32 [B]. clear: rows of `out` behind the last kept position up to keep are zeroed, else left. A kept row whose page the table of
+ * `cache` names wrongly is reported and reads as NaN. */
 int kfa_cache_evict(const KfaCache* cache, const float* weights, const int64_t* weights_stride, int64_t keep, int64_t recent,
                     const KfaCache* out, float* weights_out, int32_t* kept, int32_t* lengths_out, int clear, int* dev_status,
                     void* stream);

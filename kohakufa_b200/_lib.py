@@ -306,7 +306,7 @@ def check_status(device=None) -> None:
     The kernels never hang: a wait that exceeds its (seconds-long) limit makes the CTA fill the output
     rows it owns with NaN, record ``100 + wait id`` in a per-device status word and leave; every later
     launch on that device may still do part or all of its work, but leaves its outputs as NaN as well (what only copies, ``cache_append``
-    and ``cache_evict``, runs on). Nothing on the
+    and ``cache_evict``, runs on: tokens without a place are dropped, rows without a page are kept as NaN). Nothing on the
     launch path reads the word back (that would synchronise), so call this where the program
     synchronises anyway, e.g. after ``loss.item()`` or the optimizer step: NaN gradients plus a nonzero
     status mean "a kernel timed out", not "the model diverged". Reads one int from the device."""
@@ -314,7 +314,8 @@ def check_status(device=None) -> None:
     if code == DEV_BAD_CACHE:
         raise KfaError(
             f"a call on a KVCache met a page outside the pool, a length or position outside the capacity, or an index outside its rows "
-            f"(status {code}); outputs since then are NaN. Call reset_status() to re-enable the kernels"
+            f"(status {code}); outputs since then are NaN, appended tokens may be missing and evicted rows be NaN. "
+            f"Call reset_status() to re-enable the kernels"
         )
     if code != 0:
         raise KfaError(

@@ -244,7 +244,7 @@ __global__ void __launch_bounds__(SELECT_THREADS) kfa_cache_select_kernel(const 
 
 // Moves the rows that stay. A warp takes 32 slots of a (sequence, K / V head): each lane finds where one of them comes from and goes to, then
 // lanes 0 - 15 move the key's 16-byte pieces and lanes 16 - 31 the value's, row after row (short rows several at once), GATHER_ROWS
-// loads in flight. Bound by memory: 2 x 2 D bytes read and written a row.
+// loads in flight. Bound by memory: 2 x 2 D bytes read and written a row. A row whose page is not there reads as NaN.
 constexpr int GATHER_ROWS = 4;
 __global__ void __launch_bounds__(256) kfa_cache_gather_kernel(const EvictParams p) {
   wait_for_previous();
@@ -256,13 +256,16 @@ __global__ void __launch_bounds__(256) kfa_cache_gather_kernel(const EvictParams
   const unsigned b = p.by_head.div(row), g = row - b * p.by_head.d;
   const int i = static_cast<int>(first) + lane;
   int pos = -1, page = 0, slot = 0, page_o = -1, slot_o = 0;
+  bool lost = false;
   if (i < p.keep) {
     pos = p.kept[static_cast<long long>(row) * p.keep + i];
-    if ((pos >= 0 && !cache_place(p.c, b, pos, page, slot)) || ((pos >= 0 || p.clear) && !cache_place(p.out, b, i, page_o, slot_o))) {
-      report(p.status, DEV_BAD_CACHE);
-      page_o = -1;
-    }
+    lost = pos >= 0 && !cache_place(p.c, b, pos, page, slot);
+    const bool nowhere = (pos >= 0 || p.clear) && !cache_place(p.out, b, i, page_o, slot_o);
+    if (nowhere) page_o = -1;
+    if (lost) pos = -1;
+    if (lost || nowhere) report(p.status, DEV_BAD_CACHE);
   }
+  const unsigned all_lost = __ballot_sync(0xffffffffu, lost);
   const unsigned live = __ballot_sync(0xffffffffu, page_o >= 0);
   if (live == 0) return;
   const bool values = lane >= 16;
@@ -280,8 +283,9 @@ __global__ void __launch_bounds__(256) kfa_cache_gather_kernel(const EvictParams
       const int r = (r0 + k * at_once + mine) & 31;
       const int at = __shfl_sync(0xffffffffu, pos, r), pg = __shfl_sync(0xffffffffu, page, r), sl = __shfl_sync(0xffffffffu, slot, r);
       const int pg_o = __shfl_sync(0xffffffffu, page_o, r), sl_o = __shfl_sync(0xffffffffu, slot_o, r);
+      const uint32_t fill = (all_lost >> r) & 1u ? 0x7fff7fffu : 0u;
       dst[k] = nullptr;
-      x[k] = make_uint4(0, 0, 0, 0);
+      x[k] = make_uint4(fill, fill, fill, fill);
       if (pg_o < 0 || piece >= pieces || r0 + k * at_once + mine >= 32) continue;
       if (at >= 0) x[k] = *reinterpret_cast<const uint4*>(from + pg * f_n + sl * f_s);
       dst[k] = to + pg_o * t_n + sl_o * t_s;

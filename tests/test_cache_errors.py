@@ -4,8 +4,9 @@ took part in, every other result as ever or NaN, and nothing outside the positio
 import pytest
 import torch
 
-from kohakufa_b200 import _lib, attention_cached, cache_append, cache_weights
-from tests.test_cache import exact_attention, make_cache, rows
+from kohakufa_b200 import _lib, attention_cached, cache_append, cache_evict, cache_weights
+from kohakufa_b200.cache import cache_evict_op
+from tests.test_cache import exact_attention, logical, make_cache, rows
 
 pytestmark = pytest.mark.gpu
 DTYPE, DIM, HEADS, COLUMNS = torch.bfloat16, 64, 4, 16  # 256 positions
@@ -106,3 +107,35 @@ def test_append_writes_nothing_else(fault, tokens):
                     w[page, :, p % 16] = new[b, :, t]
     reported(lambda: cache_append(c, k, v, index=index.cuda() if fault == "index" else None))
     assert torch.equal(c.k, want[0]) and torch.equal(c.v, want[1])
+
+
+@pytest.mark.parametrize("page", [-1, 10_000, 2**31 - 1])
+@pytest.mark.parametrize("clear", [False, True])
+def test_eviction_leaves_nan_where_a_page_is_not_there(page, clear):
+    """Rows of a page that is not there read as NaN, whatever the memory held before that takes them."""
+    c, keep = cache_with(page=page), 80
+    weights = torch.rand(2, 2, 256, device="cuda")
+    weights[0, :, 50:60] = 2.0  # (these stay)
+    want = reported(lambda: cache_evict(c, weights, keep, recent=8))
+    kept = want[2]
+    assert kept[0, 0, 0] >= 0 and bool((kept[1, :, 60:] == -1).all())
+    lost = (kept >= 48) & (kept < 64)
+    lost[1] = False
+    assert bool(lost[0, 0].sum() >= 10)
+    if clear:  # a new cache, in memory of which is known what it held
+        k_out, v_out = (torch.full((2, keep, 2, DIM), 7.0, dtype=DTYPE, device="cuda").transpose(1, 2) for _ in range(2))
+        lengths, w_out, again = torch.empty_like(c.lengths), torch.empty_like(want[1]), torch.empty_like(kept)
+        reported(lambda: cache_evict_op(*c._tensors(), weights, keep, 8, k_out, v_out, None, lengths, w_out, again, True))
+        behind = torch.zeros(2, 2, keep, DIM, dtype=torch.float64)
+    else:
+        target = make_cache([keep, keep], 2, DIM, DTYPE, 16, seed=3)
+        behind = logical(target, "k")[:, :, :keep]
+        got, w_out, again = reported(lambda: cache_evict(c, weights, keep, recent=8, out=target))
+        k_out, lengths = logical(got, "k")[:, :, :keep].to(DTYPE).cuda(), got.lengths
+    assert torch.equal(again, kept) and torch.equal(w_out, want[1]) and lengths.tolist() == [keep, 60]
+    assert bool(torch.isnan(k_out[lost]).all())
+    here = (kept >= 0) & ~lost
+    source = logical(c, "k").gather(2, kept.cpu().clamp(min=0).long()[..., None].expand(-1, -1, -1, DIM))
+    assert torch.equal(k_out.double().cpu()[here.cpu()], source[here.cpu()])
+    assert torch.equal(k_out.double().cpu()[kept.cpu() < 0], behind[kept.cpu() < 0])
+    assert bool(torch.isnan(want[0].k[lost]).all()) and bool(torch.isnan(want[0].v[lost]).all())
