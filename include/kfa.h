@@ -341,10 +341,15 @@ int kfa_cache_weigh(const KfaTensor4* q, const float* stats, const KfaCache* cac
  * written to positions 0, 1, ... of `out` in ascending order (out->lengths is not read; its capacity is at least keep, and the pages that are written are none of those that are read).
  * kept: int32 [B, Hkv, keep], the positions, -1 behind the last; weights_out: fp32 [B, Hkv, keep], their weights, 0 behind the last;
  * lengths_out: int32 [B]. clear: rows of `out` behind the last kept position up to keep are zeroed, else left. A kept row whose page the table of
- * `cache` names wrongly is reported and reads as NaN. */
+ * `cache` names wrongly is reported and reads as NaN.
+ * kfa_cache_evict_room: the same with weights_out [B, Hkv, room], room >= keep, zeros behind the last kept position; clear zeroes the rows of `out`
+ * up to room, which is at most its capacity then. (kfa_cache_evict: room = keep.) */
 int kfa_cache_evict(const KfaCache* cache, const float* weights, const int64_t* weights_stride, int64_t keep, int64_t recent,
                     const KfaCache* out, float* weights_out, int32_t* kept, int32_t* lengths_out, int clear, int* dev_status,
                     void* stream);
+int kfa_cache_evict_room(const KfaCache* cache, const float* weights, const int64_t* weights_stride, int64_t keep, int64_t recent,
+                         int64_t room, const KfaCache* out, float* weights_out, int32_t* kept, int32_t* lengths_out, int clear,
+                         int* dev_status, void* stream);
 
 /* Diagnostic: the raw scores Q K^T (unscaled, unmasked) as fp32 [B, H, Sq, Skv] (contiguous), produced by
  * the same tensor-core instruction sequence the attention kernels use (one fp32-accumulating MMA per 16

@@ -62,6 +62,7 @@ SYMBOLS = (
     "kfa_cache_weigh_bytes",
     "kfa_cache_weigh",
     "kfa_cache_evict",
+    "kfa_cache_evict_room",
 )
 
 
@@ -195,6 +196,7 @@ def load() -> ctypes.CDLL:
         lib.kfa_cache_weigh_bytes.argtypes = [T, C, R]
         lib.kfa_cache_weigh.argtypes = [T, fp, C, R, fp, I64P, i64, i32, vp, f32, i32, ip, vp]
         lib.kfa_cache_evict.argtypes = [C, fp, I64P, i64, i64, C, fp, ip, ip, i32, ip, vp]
+        lib.kfa_cache_evict_room.argtypes = [C, fp, I64P, i64, i64, i64, C, fp, ip, ip, i32, ip, vp]
         for name in SYMBOLS:
             if name not in ("kfa_abi_version", "kfa_last_error", "kfa_bwd_stats_bytes", "kfa_bwd_dq_acc_bytes", "kfa_bwd_parts_bytes",
                             "kfa_cache_attend_bytes", "kfa_cache_weigh_bytes"):  # fmt: skip
@@ -211,7 +213,7 @@ HOST_SYMBOLS = (
     "kfa_bwd_varlen", "kfa_pack_mask", "kfa_fwd_narrow", "kfa_bwd_narrow",
     "kfa_bwd_parts_bytes", "kfa_bwd_parts_count", "kfa_bwd_parts", "kfa_varlen_zero_rows",
     "kfa_cache_attend_bytes", "kfa_cache_attend", "kfa_cache_append", "kfa_cache_weigh_bytes", "kfa_cache_weigh",
-    "kfa_cache_evict",
+    "kfa_cache_evict_room",
 )  # fmt: skip
 HOST_PATH = Path(__file__).resolve().parent / "_kfa_host.so"
 _host = None

@@ -1,11 +1,14 @@
 """A cache of keys and values, and what a program that generates from a model does with it in every layer:
 
     cache = KVCache(k_pages, v_pages, lengths, table)          # or KVCache.empty(...)
-    out, stats = attention_cached(q, cache, k, v, tree=tree, return_stats=True)   # drafted tokens, or one (T = 1)
-    cache_append(cache, k, v, index=accepted, counts=n)         # the accepted ones go into the cache
-    cache_weights(cache, q, stats, index=accepted, counts=n, weights=w)   # who was looked at, accumulated
-    lengths += n                                                # once per step, for all layers
-    cache, w, kept = cache_evict(cache, w, keep=2048, recent=256)         # back to the budget
+    w = torch.zeros(batch, kv_heads, cache.capacity, device="cuda")
+    while generating:
+        out, stats = attention_cached(q, cache, k, v, tree=tree, return_stats=True)   # drafted tokens, or one (T = 1)
+        cache_append(cache, k, v, index=accepted, counts=n)         # the accepted ones go into the cache
+        cache_weights(cache, q, stats, index=accepted, counts=n, weights=w)   # who was looked at, accumulated
+        cache.lengths += n                                          # once a step where layers share their lengths
+        if full:                                                    # back to the budget, with room for what comes
+            cache, w, kept = cache_evict(cache, w, keep=2048, recent=256, room=4096)
 
 All of it is for inference: there are no gradients, and a call on tensors that autograd would record is refused. The calls go to
 ``libkfa.so`` through the C++ launch path like ``attention``: current stream, no host synchronisation, scratch from the
@@ -228,34 +231,40 @@ def cache_evict_op(
 
 
 def cache_evict(
-    cache: KVCache, weights: Tensor, keep: int, *, recent: int = 0, out: KVCache | None = None
+    cache: KVCache, weights: Tensor, keep: int, *, recent: int = 0, room: int | None = None, out: KVCache | None = None
 ) -> tuple[KVCache, Tensor, Tensor]:
     """Reduces every sequence to at most ``keep`` positions: the ``recent`` newest, and of the others those with the largest accumulated
     ``weights`` (fp32 ``[B, Hkv, W]``, ``W`` at least the capacity). Each K / V head keeps positions of its own; of equal weights the
     lower position stays, NaN counts as the largest. What stays moves to positions ``0, 1, ...`` in ascending order.
 
-    ``out``: the cache that takes it (other pages than those that are read, e.g. of the same pool; room for ``keep`` positions; what
-    lies behind the kept positions is left as it was); without it a new one of one stretch per sequence, zeros behind the kept. ``cache`` itself is not changed.
-    Returns the cache that holds the rest, with its new lengths, their weights, fp32 ``[B, Hkv, keep]`` (0 behind the last), and the positions they
+    ``out``: the cache that takes it (other pages than those that are read, e.g. of the same pool; a capacity of ``keep`` or more; what
+    lies behind the kept positions is left as it was); without it a new one of one stretch per sequence and a capacity of ``room`` positions, zeros behind
+    the kept. ``cache`` itself is not changed. ``room`` (at least ``keep``, which it is by default): how many positions the returned weights are wide. Where
+    generation goes on, ask for the tokens that come before the next eviction as well: a cache without room for them drops what is appended, and
+    ``cache_weights`` wants weights as wide as the cache's capacity (``room=out.capacity``).
+    Returns the cache that holds the rest, with lengths of its own, their weights, fp32 ``[B, Hkv, room]`` (0 behind the last), and the positions they
     had, int32 ``[B, Hkv, keep]`` (-1 behind the last)."""
     pages = cache._tensors()
     keep, recent = int(keep), int(recent)
     if not 0 <= recent <= keep or keep < 1:
         raise ValueError(f"cache_evict: keep {keep}, recent {recent}: 0 <= recent <= keep, keep at least 1")
+    room = keep if room is None else int(room)
+    if room < keep:
+        raise ValueError(f"cache_evict: room {room}: at least keep, {keep}")
     if out is cache:
         raise ValueError("cache_evict: out must have pages of its own")
     k, target = cache.k, (None, None, None, None) if out is None else out._tensors()
     if _lib.plain_eager(*pages, weights, *target):
         word = _lib.status_word(k.device) if k.is_cuda else None
-        k_out, v_out, lengths_out, weights_out, kept = _lib.host().evict(*pages, weights, keep, recent, *target, word)
+        k_out, v_out, lengths_out, weights_out, kept = _lib.host().evict(*pages, weights, keep, recent, room, *target, word)
         return _new_cache(k_out, v_out, lengths_out, target[3]), weights_out, kept
     _refuse_autograd("cache_evict", cache.k, cache.v, weights, *target[:2])
     batch, heads, dim = cache.lengths.numel(), k.shape[1], k.shape[3]
     k_out, v_out, _, table_out = target
     if out is None:
-        k_out, v_out = (k.new_empty(batch, keep, heads, dim).transpose(1, 2) for _ in range(2))
+        k_out, v_out = (k.new_empty(batch, room, heads, dim).transpose(1, 2) for _ in range(2))
     lengths_out = cache.lengths.new_empty(batch)
-    weights_out = k.new_empty(batch, heads, keep, dtype=torch.float32)
+    weights_out = k.new_empty(batch, heads, room, dtype=torch.float32)
     kept = cache.lengths.new_empty(batch, heads, keep)
     cache_evict_op(*pages, weights, keep, recent, k_out, v_out, table_out, lengths_out, weights_out, kept, out is None)
     return _new_cache(k_out, v_out, lengths_out, table_out), weights_out, kept

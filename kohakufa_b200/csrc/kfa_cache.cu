@@ -462,6 +462,12 @@ int kfa_cache_weigh(const KfaTensor4* q, const float* stats, const KfaCache* cac
 int kfa_cache_evict(const KfaCache* cache, const float* weights, const int64_t* weights_stride, int64_t keep, int64_t recent,
                     const KfaCache* out, float* weights_out, int32_t* kept, int32_t* lengths_out, int clear, int* dev_status,
                     void* stream) {
+  return kfa_cache_evict_room(cache, weights, weights_stride, keep, recent, keep, out, weights_out, kept, lengths_out, clear, dev_status, stream);
+}
+
+int kfa_cache_evict_room(const KfaCache* cache, const float* weights, const int64_t* weights_stride, int64_t keep, int64_t recent, int64_t room,
+                         const KfaCache* out, float* weights_out, int32_t* kept, int32_t* lengths_out, int clear, int* dev_status,
+                         void* stream) {
   kfa::EvictParams p;
   std::memset(&p, 0, sizeof(p));
   int rc;
@@ -471,6 +477,8 @@ int kfa_cache_evict(const KfaCache* cache, const float* weights, const int64_t* 
   if (keep < 1 || recent < 0 || recent > keep || keep > p.out.capacity)
     return fail(KFA_ERR_ARG, "keep %lld, recent %lld: 0 <= recent <= keep, 1 <= keep <= %d, the room of out", (long long)keep,
                 (long long)recent, p.out.capacity);
+  if (room < keep || room > 0x7fff0000 || (clear && room > p.out.capacity))
+    return fail(KFA_ERR_ARG, "room %lld: at least keep, up to 2^31 - 65536 (with clear up to %d, the room of out)", (long long)room, p.out.capacity);
   if (!weights || !weights_stride || !weights_out || !kept || !lengths_out || !dev_status)
     return fail(KFA_ERR_ARG, "kfa_cache_evict: null pointer");
   p.w = weights;
@@ -479,10 +487,11 @@ int kfa_cache_evict(const KfaCache* cache, const float* weights, const int64_t* 
   p.keep = static_cast<int>(keep);
   p.recent = static_cast<int>(recent);
   p.clear = clear != 0;
+  p.room = static_cast<int>(room);
   p.w_out = weights_out;
   p.kept = kept;
   p.lengths_out = lengths_out;
-  const long long groups = (keep + 31) / 32, total = static_cast<long long>(p.c.batch) * p.c.heads * groups;
+  const long long groups = ((clear ? room : keep) + 31) / 32, total = static_cast<long long>(p.c.batch) * p.c.heads * groups;
   if (total > 0x7fffffffll) return fail(KFA_ERR_ARG, "kfa_cache_evict: too many rows in one call");
   p.by_slot = kfa::FastDiv::by(static_cast<uint32_t>(groups));
   p.by_head = kfa::FastDiv::by(p.c.heads);

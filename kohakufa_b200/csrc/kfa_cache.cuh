@@ -91,10 +91,11 @@ struct EvictParams {
   const float* w;
   long long w_sb, w_sh;
   int keep, recent, clear;
+  int room;                  // positions of w_out; with clear also of out that get zeros behind the kept ones
   float* w_out;
   int* kept;
   int* lengths_out;
-  FastDiv by_slot, by_head;  // 32 slots of a (sequence, head) at a time; heads
+  FastDiv by_slot, by_head;  // 32 slots of a (sequence, head) at a time (clear: up to room, else up to keep); heads
   unsigned total;            // such groups
   int* status;
 };
@@ -126,13 +127,11 @@ __global__ void __launch_bounds__(SELECT_THREADS) kfa_cache_select_kernel(const 
   const float* w = p.w + b * p.w_sb + g * p.w_sh;
   const long long row = static_cast<long long>(b) * p.c.heads + g;
   int* kept = p.kept + row * p.keep;
-  float* w_out = p.w_out + row * p.keep;
+  float* w_out = p.w_out + row * p.room;
   const int left = min(len, p.keep);
   if (g == 0 && tid == 0) p.lengths_out[b] = left;
-  for (int i = left + tid; i < p.keep; i += SELECT_THREADS) {
-    kept[i] = -1;
-    w_out[i] = 0.f;
-  }
+  for (int i = left + tid; i < p.keep; i += SELECT_THREADS) kept[i] = -1;
+  for (int i = left + tid; i < p.room; i += SELECT_THREADS) w_out[i] = 0.f;
   if (len <= p.keep) {
     for (int i = tid; i < len; i += SELECT_THREADS) {
       kept[i] = i;
@@ -257,8 +256,8 @@ __global__ void __launch_bounds__(256) kfa_cache_gather_kernel(const EvictParams
   const int i = static_cast<int>(first) + lane;
   int pos = -1, page = 0, slot = 0, page_o = -1, slot_o = 0;
   bool lost = false;
-  if (i < p.keep) {
-    pos = p.kept[static_cast<long long>(row) * p.keep + i];
+  if (i < (p.clear ? p.room : p.keep)) {
+    if (i < p.keep) pos = p.kept[static_cast<long long>(row) * p.keep + i];
     lost = pos >= 0 && !cache_place(p.c, b, pos, page, slot);
     const bool nowhere = (pos >= 0 || p.clear) && !cache_place(p.out, b, i, page_o, slot_o);
     if (nowhere) page_o = -1;

@@ -51,7 +51,7 @@ struct Api {
   decltype(&kfa_cache_append) cache_append = nullptr;
   decltype(&kfa_cache_weigh_bytes) cache_weigh_bytes = nullptr;
   decltype(&kfa_cache_weigh) cache_weigh = nullptr;
-  decltype(&kfa_cache_evict) cache_evict = nullptr;
+  decltype(&kfa_cache_evict_room) cache_evict = nullptr;
 } api;
 
 PyObject* g_error = nullptr;  // kohakufa_b200._lib.KfaError
@@ -862,7 +862,7 @@ PyObject* py_cache_weights(Args a, Py_ssize_t n) {
   Py_RETURN_NONE;
 }
 
-// What cache_evict fills: the pages of `out`, or of a new cache of one stretch per sequence, lengths, weights, positions.
+// What cache_evict fills: the pages of `out`, or of a new cache of one stretch per sequence, lengths, weights (as wide as there is to be room), positions.
 struct Evicted {
   Cache out;
   at::Tensor weights, kept;
@@ -871,15 +871,16 @@ struct Evicted {
 void run_evict(const Cache& c, const at::Tensor& w, int64_t keep, int64_t recent, const Evicted& e, bool clear, const at::Tensor& status) {
   const KfaCache dc = cache_desc(c), dn = cache_desc(e.out);
   const int64_t stride[2] = {w.stride(0), w.stride(1)};
-  check(api.cache_evict(&dc, w.data_ptr<float>(), stride, keep, recent, &dn, e.weights.data_ptr<float>(), e.kept.data_ptr<int32_t>(),
+  check(api.cache_evict(&dc, w.data_ptr<float>(), stride, keep, recent, e.weights.size(2), &dn, e.weights.data_ptr<float>(), e.kept.data_ptr<int32_t>(),
                         e.out.lengths.data_ptr<int32_t>(), clear, status.data_ptr<int32_t>(), stream_of(w)));
 }
 
-void check_evict(const Cache& c, const at::Tensor& w, int64_t keep, int64_t recent) {
+void check_evict(const Cache& c, const at::Tensor& w, int64_t keep, int64_t recent, int64_t room) {
   const char* who = "cache_evict";
   check_cache(who, c);
   check_weights(who, c, w);
   TORCH_CHECK_VALUE(recent >= 0 && recent <= keep && keep >= 1 && keep <= 0x7fffffff, who, ": 0 <= recent <= keep, keep at least 1");
+  TORCH_CHECK_VALUE(room >= keep && room <= 0x7fff0000, who, ": room ", std::to_string(room), ": at least keep, up to 2^31 - 65536");
 }
 void check_evict_out(const Cache& c, const Cache& o, int64_t keep) {
   const char* who = "cache_evict";
@@ -894,19 +895,19 @@ void check_evict_out(const Cache& c, const Cache& o, int64_t keep) {
   TORCH_CHECK_VALUE(tables || (c.k.data_ptr() != o.k.data_ptr() && c.v.data_ptr() != o.v.data_ptr()), who, ": out must have pages of its own");
 }
 
-// evict(k_pages, v_pages, lengths, table, weights, keep, recent, k_out or None, v_out, lengths of out, table_out, status) -> k_out, v_out, lengths,
-// weights, kept
+// evict(k_pages, v_pages, lengths, table, weights, keep, recent, room, k_out or None, v_out, lengths of out, table_out, status) -> k_out, v_out,
+// lengths, weights, kept
 PyObject* py_evict(Args a, Py_ssize_t n) {
-  need(n, 12);
+  need(n, 13);
   const char* who = "cache_evict";
   const Cache c = cache_of(a);
-  const at::Tensor w = tensor(a[4]), status = maybe(a[11]);
-  const int64_t keep = integer(a[5]), recent = integer(a[6]);
-  const bool clear = a[7] == Py_None;
+  const at::Tensor w = tensor(a[4]), status = maybe(a[12]);
+  const int64_t keep = integer(a[5]), recent = integer(a[6]), room = integer(a[7]);
+  const bool clear = a[8] == Py_None;
   Evicted e;
-  if (!clear) e.out = cache_of(a + 7);
+  if (!clear) e.out = cache_of(a + 8);
   check_no_grad(who, {&c.k, &c.v, &w, &e.out.k, &e.out.v});
-  check_evict(c, w, keep, recent);
+  check_evict(c, w, keep, recent, room);
   if (!clear) check_evict_out(c, e.out, keep);
   check_where(who, c, {&w, &e.out.k, &e.out.v, &e.out.table, &status});
   const int64_t b = c.lengths.numel(), heads = c.k.size(1);
@@ -914,11 +915,11 @@ PyObject* py_evict(Args a, Py_ssize_t n) {
   released([&] {
     const c10::cuda::CUDAGuard guard(w.device());
     if (clear) {
-      e.out.k = at::empty({b, keep, heads, c.k.size(3)}, c.k.options()).transpose(1, 2);
-      e.out.v = at::empty({b, keep, heads, c.k.size(3)}, c.k.options()).transpose(1, 2);
+      e.out.k = at::empty({b, room, heads, c.k.size(3)}, c.k.options()).transpose(1, 2);
+      e.out.v = at::empty({b, room, heads, c.k.size(3)}, c.k.options()).transpose(1, 2);
     }
     e.out.lengths = at::empty({b}, c.lengths.options());
-    e.weights = floats(w, {b, heads, keep});
+    e.weights = floats(w, {b, heads, room});
     e.kept = at::empty({b, heads, keep}, c.lengths.options());
     run_evict(c, w, keep, recent, e, clear, status);
     return 0;
@@ -934,13 +935,15 @@ PyObject* py_cache_evict(Args a, Py_ssize_t n) {
   const Cache c = cache_of(a);
   const Evicted e{{tensor(a[7]), tensor(a[8]), tensor(a[10]), maybe(a[9])}, tensor(a[11]), tensor(a[12])};
   const at::Tensor w = tensor(a[4]), status = maybe(a[14]);
-  const int64_t keep = integer(a[5]), recent = integer(a[6]), size = c.lengths.numel() * c.k.size(1) * keep;
+  const int64_t keep = integer(a[5]), recent = integer(a[6]), rows = c.lengths.numel() * c.k.size(1);
   const bool clear = PyObject_IsTrue(a[13]);
+  TORCH_CHECK_VALUE(e.weights.dim() == 3, who, ": results of another size");
+  const int64_t room = e.weights.size(2);
   check_no_grad(who, {&c.k, &c.v, &w, &e.out.k, &e.out.v});
-  check_evict(c, w, keep, recent);
-  check_evict_out(c, e.out, keep);
+  check_evict(c, w, keep, recent, room);
+  check_evict_out(c, e.out, clear ? room : keep);
   TORCH_CHECK(e.weights.scalar_type() == at::kFloat && e.kept.scalar_type() == at::kInt && e.weights.is_contiguous() && e.kept.is_contiguous() &&
-                  e.weights.numel() == size && e.kept.numel() == size,
+                  e.weights.numel() == rows * room && e.kept.numel() == rows * keep && e.out.lengths.numel() == c.lengths.numel(),
               who, ": results of another size");
   check_where(who, c, {&w, &e.out.k, &e.out.v, &e.out.lengths, &e.out.table, &e.weights, &e.kept, &status});
   released([&] {
@@ -982,7 +985,7 @@ PyObject* py_bind(Args a, Py_ssize_t n) {
   take("kfa_cache_append", api.cache_append);
   take("kfa_cache_weigh_bytes", api.cache_weigh_bytes);
   take("kfa_cache_weigh", api.cache_weigh);
-  take("kfa_cache_evict", api.cache_evict);
+  take("kfa_cache_evict_room", api.cache_evict);
   Py_INCREF(a[0]);
   Py_XDECREF(g_error);
   g_error = a[0];
