@@ -20,6 +20,7 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 
+#include <algorithm>
 #include <array>
 #include <cmath>
 #include <initializer_list>
@@ -842,8 +843,14 @@ PyObject* py_cache_weights(Args a, Py_ssize_t n) {
                     who, ": stats must be the contiguous [B, H, 2, T] of these queries");
   const KfaRows rows = rows_of(who, c, index, counts, q.size(2));
   check_weights(who, c, w);
-  for (int i = 0; i < 2; ++i)  // (it is written: no two entries may be one)
-    TORCH_CHECK_VALUE(w.size(i) == 1 || w.stride(i) >= w.size(2), who, ": weights must not overlap itself");
+  // (it is written: no two entries may be one. Rows (b, g) and (b', g') lie (b - b') s + (g - g') t apart; per g - g' the two b - b' next to 0)
+  const int64_t s = w.size(0) > 1 ? w.stride(0) : 0, t = w.stride(1), width = w.size(2);
+  bool apart = w.size(0) == 1 || s >= width;
+  for (int64_t j = 1; apart && j < w.size(1); ++j) {
+    const int64_t back = s > 0 ? std::min(j * t / s, w.size(0) - 1) : 0, off = j * t - back * s;
+    apart = off >= width && (back + 1 >= w.size(0) || s - off >= width);
+  }
+  TORCH_CHECK_VALUE(apart, who, ": weights must not overlap itself");
   check_scale(who, scale);
   check_where(who, c, {&q, &stats, &index, &counts, &w, &status});
   will_write({&w});
