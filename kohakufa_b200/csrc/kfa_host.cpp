@@ -899,7 +899,9 @@ void check_evict_out(const Cache& c, const Cache& o, int64_t keep) {
   check_written(who, o);
   // (two tables over one pool may name different pages)
   const bool tables = c.table.defined() && o.table.defined() && c.table.data_ptr() != o.table.data_ptr();
-  TORCH_CHECK_VALUE(tables || (c.k.data_ptr() != o.k.data_ptr() && c.v.data_ptr() != o.v.data_ptr()), who, ": out must have pages of its own");
+  for (const at::Tensor* read : {&c.k, &c.v})
+    for (const at::Tensor* written : {&o.k, &o.v})
+      TORCH_CHECK_VALUE(tables || read->data_ptr() != written->data_ptr(), who, ": out must have pages of its own");
 }
 
 // evict(k_pages, v_pages, lengths, table, weights, keep, recent, room, k_out or None, v_out, lengths of out, table_out, status) -> k_out, v_out,

@@ -6,7 +6,7 @@ import itertools
 import pytest
 import torch
 
-from kohakufa_b200 import cache_weights
+from kohakufa_b200 import KVCache, cache_evict, cache_weights
 from tests.test_cache import cpu_cache
 
 
@@ -22,3 +22,14 @@ def test_weights_that_overlap_themselves(batch, heads):
         meet = any(y - x < 32 for x, y in zip(starts, starts[1:]))
         with pytest.raises(ValueError, match="overlap" if meet else "CUDA tensors only"):
             cache_weights(c, q, stats, weights=w)
+
+
+def test_eviction_into_the_pages_that_it_reads():
+    c, other, w, ints = cpu_cache(), cpu_cache(), torch.zeros(2, 2, 32), torch.zeros(2, dtype=torch.int32)
+    for k, v in ((c.k, other.v), (other.k, c.v), (c.v, other.v), (other.k, c.k), (c.v, c.k)):
+        with pytest.raises(ValueError, match="pages of its own"):
+            cache_evict(c, w, 4, out=KVCache(k, v, ints, c.table))
+        with pytest.raises(ValueError, match="pages of its own"):
+            cache_evict(c, w, 4, out=KVCache(k[:2], v[:2], ints))
+        with pytest.raises(ValueError, match="CUDA tensors only"):  # (two tables over one pool may name different pages)
+            cache_evict(c, w, 4, out=KVCache(k, v, ints, c.table.clone()))
