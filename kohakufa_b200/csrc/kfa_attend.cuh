@@ -453,7 +453,7 @@ __device__ __forceinline__ void att_produce(const AttendParams& p, const Walk& f
       const unsigned cached = __ballot_sync(0xffffffffu, kind == 1), fresh = __ballot_sync(0xffffffffu, kind == 2);
       const int stage = values ? R::v_stage(T) : R::k_stage(T), turn = values ? R::v_turn(T) : R::k_turn(T);
       if (turn > 0) {
-        ok = wait_warp(bar(R::B_KVFREE + stage), (turn - 1) & 1, ctl, 72);
+        ok = wait_warp(bar(R::B_KVFREE + stage), (turn - 1) & 1, ctl, values ? 71 : 72);
         if (!ok) break;
       }
       if (lane == 0) mbar_expect_tx(bar(R::B_KV + stage), R::NC * 128 * (__popc(cached) * p.box + __popc(fresh) * ATT_UNIT));

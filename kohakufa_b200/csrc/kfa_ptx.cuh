@@ -18,8 +18,10 @@ namespace kfa {
 // Status codes written to the device status word (first failure wins).
 enum : int {
   KFA_DEV_OK = 0,
-  // 100 + id of the wait that gave up; every wait in the library has an id of its own:
-  // 1-9 forward, 11-21 dK/dV kernel, 30-50 fused backward, 51-62 dQ kernel, 70-90 attention over a cache, 91-99 self-test and diagnostics
+  // 100 + id of the wait that gave up; every wait has an id of its own:
+  // 1-9 forward, 11-21 dK/dV kernel, 30-50 fused backward, 51-62 dQ kernel, 91-99 self-test and diagnostics.
+  // 70-83 attention over a cache, 84-90 and 76 its weights: an id says what is waited for, in either of the two kernels of the operator
+  // (and in either stream).
   KFA_DEV_TIMEOUT_BASE = 100,
   KFA_DEV_BAD_SMEM_BASE = 99,  // the dynamic shared memory of a kernel that needs it did not start on a 1 KB boundary
 };

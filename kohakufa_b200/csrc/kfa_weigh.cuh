@@ -554,7 +554,7 @@ kfa_cache_weigh_rows_kernel(const __grid_constant__ CUtensorMap tmQ, const __gri
             tma_load_4d(sQ + stage * R::STAGE + ch * R::CHUNK, &tmQ, bar(R::B_Q + stage), ch * 64, w.g * a.group + head, token, w.b);
         }
         q_issued = T + 1;
-        if (T >= R::DS) ok = wait_warp(bar(R::B_STFREE + slot), (T / R::DS - 1) & 1, ctl, 85);
+        if (T >= R::DS) ok = wait_warp(bar(R::B_STFREE + slot), (T / R::DS - 1) & 1, ctl, 76);
         if (!ok) break;
         bool two = false;
 #pragma unroll
