@@ -43,9 +43,9 @@ __device__ __forceinline__ float2 row_stats(const AttendParams& a, const WeighPa
 __device__ __forceinline__ int rows_before(int ahead, int heads) { return max(ahead, 0) * heads; }
 
 // The weights of a key, summed: N scores against N rows, whose -m and -log2 l stand one after the other (two at a time in the packed
-// instructions). slow: some rows are not there (-m = -inf, and their scores may be anything), or do not see the key: those below r_min.
+// instructions). Rows that are not there (-m = -inf; their scores may be anything) and those that do not see the key (below r_min) count nothing.
 template <int N>
-__device__ __forceinline__ float weigh_scores(const float* x, const float* neg_m, const float* neg_l, float c_log2, bool slow, int r_min) {
+__device__ __forceinline__ float weigh_scores(const float* x, const float* neg_m, const float* neg_l, float c_log2, int r_min) {
   const float2 c2 = make_float2(c_log2, c_log2);
   float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
@@ -55,12 +55,10 @@ __device__ __forceinline__ float weigh_scores(const float* x, const float* neg_m
     float2 e1 = __ffma2_rn(__fadd2_rn(make_float2(x[i + 2], x[i + 3]), make_float2(m.z, m.w)), c2, make_float2(l.z, l.w));
     e0 = make_float2(ex2(e0.x), ex2(e0.y));
     e1 = make_float2(ex2(e1.x), ex2(e1.y));
-    if (slow) {
-      if (m.x == -INFINITY || i < r_min) e0.x = 0.f;
-      if (m.y == -INFINITY || i + 1 < r_min) e0.y = 0.f;
-      if (m.z == -INFINITY || i + 2 < r_min) e1.x = 0.f;
-      if (m.w == -INFINITY || i + 3 < r_min) e1.y = 0.f;
-    }
+    if (m.x == -INFINITY || i < r_min) e0.x = 0.f;
+    if (m.y == -INFINITY || i + 1 < r_min) e0.y = 0.f;
+    if (m.z == -INFINITY || i + 2 < r_min) e1.x = 0.f;
+    if (m.w == -INFINITY || i + 3 < r_min) e1.y = 0.f;
     sum[0] = __fadd2_rn(sum[0], e0);
     sum[1] = __fadd2_rn(sum[1], e1);
   }
@@ -287,7 +285,7 @@ kfa_cache_weigh_kernel(const __grid_constant__ CUtensorMap tmK, const AttendPara
         mbar_arrive(bar(R::B_SFREE + 2 * st + (c & 1)));
         // (tokens that are not there have m = +inf; their scores come from what the buffer held before)
         const float* rows = s_rows + (s & 1) * 2 * N;
-        const float sum = weigh_scores<N>(x, rows, rows + N, a.c_log2, true, rows_before(pos - old, a.gt));  // (token i sees positions up to old + i)
+        const float sum = weigh_scores<N>(x, rows, rows + N, a.c_log2, rows_before(pos - old, a.gt));  // (token i sees positions up to old + i)
         if (mine) out[pos] = *ac.bad != 0 ? __int_as_float(0x7fc00000) : before + sum;
         ++c;
       }
@@ -577,6 +575,7 @@ kfa_cache_weigh_rows_kernel(const __grid_constant__ CUtensorMap tmQ, const __gri
       if (ok) more = w.next() || w.next_run(a, p);
     }
   } else if (warp == 9) {
+    // (nothing: one warp issues for both halves of the rows)
   } else if (warp == 8) {
     // =========================== MMA issue ===========================
     const bool lead = elect_one();
@@ -654,7 +653,7 @@ kfa_cache_weigh_rows_kernel(const __grid_constant__ CUtensorMap tmQ, const __gri
             if (one) {
               part += weigh_scores_one<32>(x, rows + i, a.c_log2);
             } else {  // (token t sees positions up to len + t)
-              part += weigh_scores<32>(x, rows + 128 + i, rows + 256 + i, a.c_log2, true, rows_before(pos - w.len - token, p.tile_h) - 64 * half - i);
+              part += weigh_scores<32>(x, rows + 128 + i, rows + 256 + i, a.c_log2, rows_before(pos - w.len - token, p.tile_h) - 64 * half - i);
             }
           }
           mbar_arrive(bar(R::B_STFREE + slot));
