@@ -114,7 +114,8 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
 // warp takes a stretch of the positions, counts those above that key and those equal to it, and lists them in ascending order: all above it
 // stay, of the equal ones the first, until there are enough. Bound by latency; a thread's first 8 positions are read once and held.
 // SELECT_THREADS: 512 for caches of up to 2048 positions, else 1024. (The whole call in us with 256, 512, 1024: 2 x 4 heads over 320
-// positions 10.7, 10.0, 11.1; 16 x 8 over 1500 to 8192 93.7, 76.8, 57.4.)
+// positions 10.7, 10.0, 11.1; 16 x 8 over 1500 to 8192 93.7, 76.8, 57.4.) A long row is one CTA's as well: 8 heads over 8192, 32768, 131072 positions
+// take 21, 45, 193.
 template <int SELECT_THREADS>
 __global__ void __launch_bounds__(SELECT_THREADS) kfa_cache_select_kernel(const EvictParams p) {
   constexpr int WARPS = SELECT_THREADS / 32, BINS = 2048, PER = BINS / SELECT_THREADS;
