@@ -170,7 +170,8 @@ def cache_append(cache: KVCache, k: Tensor, v: Tensor, *, index: Tensor | None =
     """Writes keys and values of new tokens behind the cached ones: position ``lengths[b] + i`` gets token ``index[b, i]`` of ``k`` and
     ``v`` ``[B, Hkv, T, D]`` (``index``: int32 ``[B, A]``, e.g. the accepted path of a draft; without it token ``i``), for ``i <
     counts[b]`` (int32 ``[B]``; without it all). ``lengths`` is left as it is: add the counts to it once all layers have appended. The pages that
-    are written must belong to one sequence each, and ``k`` and ``v`` must not lie in the positions that are written. Positions beyond the capacity are dropped and reported by ``check_status``."""
+    are written must belong to one sequence each, and ``k`` and ``v`` must not lie in the positions that are written. Positions beyond the
+    capacity are dropped and reported by ``check_status``."""
     pages = cache._tensors()
     if _lib.plain_eager(*pages, k, v, index, counts):
         _lib.host().cache_append(*pages, k, v, index, counts, _lib.status_word(k.device) if k.is_cuda else None)

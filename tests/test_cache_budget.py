@@ -1,6 +1,8 @@
 """Generation with a bounded cache as the module's documentation writes it: the loop runs on behind its evictions. Tolerances as in test_cache.py;
 a position's accumulated weight has up to 60 additions of fp32 behind it, each half a step off: 2^-24 * 60 relative, below the 2^-13 of the weights."""
 
+import ctypes
+
 import pytest
 import torch
 
@@ -78,6 +80,45 @@ def test_room(keep, room):
     behind = torch.ones(before.shape[:3], dtype=torch.bool)
     behind[:, :, :keep] = kept.cpu() < 0
     assert torch.equal(logical(got, "k")[behind], before[behind]) and _lib.device_status() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("clear", [0, 1])
+def test_the_c_entries(clear):
+    """kfa_cache_evict is kfa_cache_evict_room with room for what is kept; rooms that do not fit are refused before a launch."""
+    lib, keep = _lib.load(), 24
+    cache = make_cache([300, 5], 2, 64, torch.float16, 16)
+    weights = torch.rand(2, 2, cache.capacity, device="cuda")
+    want = cache_evict(cache, weights, keep, recent=4)
+    word, stream = _lib.status_word(weights.device), _lib.stream_ptr(weights.device)
+    stride = (ctypes.c_int64 * 2)(weights.stride(0), weights.stride(1))
+
+    def describe(c):
+        d = _lib.KfaCache(_lib.tensor4(c.k), _lib.tensor4(c.v), None, 0, 0, c.lengths.data_ptr(), c.lengths.numel())
+        if c.table is not None:
+            d.table, d.table_stride, d.table_cols = c.table.data_ptr(), c.table.stride(0), c.table.shape[1]
+        return ctypes.byref(d)
+
+    for room in (None, keep, 40):
+        out = KVCache(*(torch.full((2, 32, 2, 64), 7.0, dtype=torch.float16, device="cuda").transpose(1, 2) for _ in range(2)), cache.lengths)
+        w, kept = torch.full((2, 2, room or keep), 7.0, device="cuda"), torch.empty(2, 2, keep, dtype=torch.int32, device="cuda")
+        lengths = torch.empty_like(cache.lengths)
+        behind = (describe(out), w.data_ptr(), kept.data_ptr(), lengths.data_ptr(), clear, word.data_ptr(), stream)
+        if room is None:
+            rc = lib.kfa_cache_evict(describe(cache), weights.data_ptr(), stride, keep, 4, *behind)
+        else:
+            rc = lib.kfa_cache_evict_room(describe(cache), weights.data_ptr(), stride, keep, 4, room, *behind)
+        if room == 40 and clear:  # out has room for 32
+            assert rc != 0 and b"room" in lib.kfa_last_error()
+            continue
+        assert rc == 0 and torch.equal(kept, want[2]) and lengths.tolist() == [24, 5]
+        assert torch.equal(w[..., :keep], want[1]) and bool((w[..., keep:] == 0).all())
+        there = want[2] >= 0
+        assert torch.equal(out.k[:, :, :keep][there], want[0].k[there]) and bool((out.v[:, :, :keep][~there] == (0 if clear else 7)).all())
+        assert bool((out.k[:, :, keep:] == 7).all())
+    assert lib.kfa_cache_evict_room(describe(cache), weights.data_ptr(), stride, keep, 4, keep - 1, *behind) != 0
+    torch.cuda.synchronize()
+    assert _lib.device_status() == 0
 
 
 def test_refused_rooms():
