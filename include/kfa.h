@@ -36,6 +36,7 @@ extern "C" {
 
 #define KFA_F16 0
 #define KFA_BF16 1
+#define KFA_F32 2 /* kfa_rotary only */
 
 #define KFA_OK 0
 #define KFA_ERR_ARG (-1)      /* shape / stride / alignment / dtype not supported */
@@ -326,6 +327,40 @@ int kfa_cache_attend(const KfaTensor4* q, const KfaCache* cache, const KfaTensor
  * written and reported. The written pages belong to one sequence each. */
 int kfa_cache_append(const KfaCache* cache, const KfaTensor4* k, const KfaTensor4* v, const KfaRows* rows, int* dev_status,
                      void* stream);
+
+/* ---------------------------------------------------------------------------------------------
+ * Rotary positions. No counterpart in the reference.
+ *
+ * A row at position p has `pairs` pairs of columns turned by p * f_i, i = 0 .. pairs - 1: (y1, y2) = amplitude * (x1 cos - x2 sin,
+ * x2 cos + x1 sin); the columns behind 2 * pairs are copied. interleaved = 0: pair i is columns i and pairs + i; else 2 i and 2 i + 1.
+ * turns: f_i / (2 pi) modulo 1 as a 64-bit fraction (2^64 is a whole turn), so that the angle of any position is exact to 2^-65 turns
+ * times the position. positions: int32 (wide_positions: int64) [B, T] with the two strides in entries (0: broadcast), or NULL: what the call says.
+ * offset: int32 [B], added to every position of a sequence, or NULL. Positions may be negative.
+ * --------------------------------------------------------------------------------------------- */
+typedef struct KfaRotary {
+  const int64_t* turns;
+  int64_t pairs;
+  int interleaved;
+  float amplitude;
+  const void* positions;
+  int64_t position_stride[2];
+  int wide_positions;
+  const int32_t* offset;
+} KfaRotary;
+
+/* q_out = q, k_out = k turned (k and k_out may both be NULL): [B, H, T, D] and [B, Hkv, T, D], D up to 1024, fp16, bf16 or fp32. Rows may
+ * begin anywhere (whole elements; strides 0 or more, those of the outputs apart); those on 16 bytes are fastest. Without
+ * positions token t stands at t. inverse != 0: turned back, which is the gradient (the amplitude stays). Sines, cosines and products are fp32, rounded once. */
+int kfa_rotary(const KfaTensor4* q, const KfaTensor4* k, const KfaTensor4* q_out, const KfaTensor4* k_out, const KfaRotary* rotary,
+               int inverse, int dtype, void* stream);
+
+/* kfa_cache_append with turned keys: position lengths[b] + i of the cache <- the i-th of the given rows of k, turned, and of v. The row stands at
+ * offset[b] + lengths[b] + i, or at offset[b] + positions[b, t] with t its index among the T new tokens. q (may be NULL): the same tokens'
+ * queries [B, H, T, D], turned into q_out; k_out (may be NULL): [B, Hkv, T, D], the turned keys once more. Both only without an index
+ * and with steps = T; their rows that counts leaves out are zeros. */
+int kfa_cache_append_rotary(const KfaCache* cache, const KfaTensor4* q, const KfaTensor4* k, const KfaTensor4* v, const KfaRows* rows,
+                            const KfaRotary* rotary, const KfaTensor4* q_out, const KfaTensor4* k_out, int dtype, int* dev_status,
+                            void* stream);
 
 /* weights[b, g, p] = (add: +=) the attention that the given rows of q gave to cached position p, summed over rows and over the query heads
  * of K / V head g. Row i stands at position lengths[b] + i (appended before this call) and sees positions up to its own; its

@@ -17,9 +17,18 @@ health word, see ``check_status``).
 
 from kohakufa_b200._lib import check_status, reset_status
 from kohakufa_b200.api import attention, attention_varlen, varlen_plan
-from kohakufa_b200.cache import KVCache, attention_cached, cache_append, cache_evict, cache_weights, tree_mask  # noqa: F401
+from kohakufa_b200.cache import (  # noqa: F401
+    KVCache,
+    attention_cached,
+    cache_append,
+    cache_append_rotary,
+    cache_evict,
+    cache_weights,
+    tree_mask,
+)
 from kohakufa_b200.mask import PackedMask, pack_mask
 from kohakufa_b200.op import get_backward, is_deterministic, set_backward, set_deterministic
+from kohakufa_b200.rotary import Rotary, apply_rotary, rotary_frequencies  # noqa: F401
 
 # What `import *` takes is the drop-in's surface; the cache's names are exported by their own module as well.
 __all__ = [

@@ -16,7 +16,7 @@ import torch
 # sources (e.g. one compiled with different tuning macros) without touching the tree.
 LIB_PATH = Path(os.environ.get("KFA_LIBRARY") or Path(__file__).resolve().parent / "libkfa.so")
 
-KFA_F16, KFA_BF16 = 0, 1
+KFA_F16, KFA_BF16, KFA_F32 = 0, 1, 2
 DEV_BAD_CACHE = 90  # KFA_DEV_BAD_CACHE
 ABI_VERSION = 1
 
@@ -63,6 +63,8 @@ SYMBOLS = (
     "kfa_cache_weigh",
     "kfa_cache_evict",
     "kfa_cache_evict_room",
+    "kfa_rotary",
+    "kfa_cache_append_rotary",
 )
 
 
@@ -105,6 +107,19 @@ class KfaRows(ctypes.Structure):
         ("index_stride", ctypes.c_int64),
         ("counts", ctypes.c_void_p),
         ("steps", ctypes.c_int64),
+    ]
+
+
+class KfaRotary(ctypes.Structure):
+    _fields_ = [
+        ("turns", ctypes.c_void_p),
+        ("pairs", ctypes.c_int64),
+        ("interleaved", ctypes.c_int),
+        ("amplitude", ctypes.c_float),
+        ("positions", ctypes.c_void_p),
+        ("position_stride", ctypes.c_int64 * 2),
+        ("wide_positions", ctypes.c_int),
+        ("offset", ctypes.c_void_p),
     ]
 
 
@@ -197,6 +212,9 @@ def load() -> ctypes.CDLL:
         lib.kfa_cache_weigh.argtypes = [T, fp, C, R, fp, I64P, i64, i32, vp, f32, i32, ip, vp]
         lib.kfa_cache_evict.argtypes = [C, fp, I64P, i64, i64, C, fp, ip, ip, i32, ip, vp]
         lib.kfa_cache_evict_room.argtypes = [C, fp, I64P, i64, i64, i64, C, fp, ip, ip, i32, ip, vp]
+        O = ctypes.POINTER(KfaRotary)
+        lib.kfa_rotary.argtypes = [T, T, T, T, O, i32, i32, vp]
+        lib.kfa_cache_append_rotary.argtypes = [C, T, T, T, R, O, T, T, i32, ip, vp]
         for name in SYMBOLS:
             if name not in ("kfa_abi_version", "kfa_last_error", "kfa_bwd_stats_bytes", "kfa_bwd_dq_acc_bytes", "kfa_bwd_parts_bytes",
                             "kfa_cache_attend_bytes", "kfa_cache_weigh_bytes"):  # fmt: skip
@@ -213,7 +231,7 @@ HOST_SYMBOLS = (
     "kfa_bwd_varlen", "kfa_pack_mask", "kfa_fwd_narrow", "kfa_bwd_narrow",
     "kfa_bwd_parts_bytes", "kfa_bwd_parts_count", "kfa_bwd_parts", "kfa_varlen_zero_rows",
     "kfa_cache_attend_bytes", "kfa_cache_attend", "kfa_cache_append", "kfa_cache_weigh_bytes", "kfa_cache_weigh",
-    "kfa_cache_evict_room",
+    "kfa_cache_evict_room", "kfa_rotary", "kfa_cache_append_rotary",
 )  # fmt: skip
 HOST_PATH = Path(__file__).resolve().parent / "_kfa_host.so"
 _host = None

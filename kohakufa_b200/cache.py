@@ -21,8 +21,9 @@ import torch
 from torch import Tensor
 
 from kohakufa_b200 import _lib
+from kohakufa_b200.rotary import Rotary
 
-__all__ = ["KVCache", "attention_cached", "cache_append", "cache_evict", "cache_weights", "tree_mask"]
+__all__ = ["KVCache", "attention_cached", "cache_append", "cache_append_rotary", "cache_evict", "cache_weights", "tree_mask"]
 
 
 class KVCache:
@@ -178,6 +179,52 @@ def cache_append(cache: KVCache, k: Tensor, v: Tensor, *, index: Tensor | None =
         return
     _refuse_autograd("cache_append", cache.k, cache.v, k, v)
     cache_append_op(*pages, k, v, index, counts)
+
+
+@torch.library.custom_op("kohakufa_b200::cache_append_rotary", mutates_args=("k_pages", "v_pages"), device_types="cuda")
+def cache_append_rotary_op(
+    k_pages: Tensor, v_pages: Tensor, lengths: Tensor, table: Tensor | None, q: Tensor | None, k: Tensor, v: Tensor, index: Tensor | None,
+    counts: Tensor | None, turns: Tensor, positions: Tensor | None, offset: Tensor | None, amplitude: float, interleaved: bool, keys: bool,
+) -> tuple[Tensor, Tensor]:  # fmt: skip
+    q_out, k_out = _lib.host().cache_append_rotary(
+        k_pages, v_pages, lengths, table, q, k, v, index, counts, turns, positions, offset, amplitude, interleaved, keys, _lib.status_word(k.device)
+    )
+    return k.new_empty(0) if q_out is None else q_out, k.new_empty(0) if k_out is None else k_out
+
+
+@cache_append_rotary_op.register_fake
+def _(k_pages, v_pages, lengths, table, q, k, v, index, counts, turns, positions, offset, amplitude, interleaved, keys):
+    like = lambda t: t.new_empty(t.shape[0], t.shape[2], t.shape[1], t.shape[3]).transpose(1, 2)  # noqa: E731
+    return k.new_empty(0) if q is None else like(q), like(k) if keys else k.new_empty(0)
+
+
+def cache_append_rotary(
+    cache: KVCache, q: Tensor | None, k: Tensor, v: Tensor, rotary: Rotary, *, index: Tensor | None = None, counts: Tensor | None = None,
+    positions: Tensor | None = None, offset: Tensor | None = None, return_keys: bool = False,
+):  # fmt: skip
+    """``cache_append`` for keys that are not turned yet (``apply_rotary``), with the new tokens' queries in the same pass: position
+    ``lengths[b] + i`` gets token ``i`` of ``k``, turned, and of ``v``.
+
+    Token ``i`` stands at ``offset[b] + lengths[b] + i``: ``offset`` (int32 ``[B]``) is what a sequence has before its cache begins, a prefix that is stored
+    elsewhere or positions that were evicted. Or at ``offset[b] + positions[b, t]`` (int32 or int64, ``[B, T]``, ``[1, T]`` or ``[T]``), whatever the cache holds.
+    ``q`` ``[B, H, T, D]`` or None. Returns the turned queries (None without ``q``), and with ``return_keys`` also the turned keys, for
+    ``attention_cached`` or ``attention_shared`` in the same step, before ``lengths`` grows:
+
+        q, k = cache_append_rotary(cache, q, k, v, rotary, return_keys=True)
+        out = attention_cached(q, cache, k, v)
+
+    Rows that ``counts`` leaves out are zeros there. ``index`` and what else is said of ``cache_append`` holds here too; with an index only the pages are written: ``q`` is
+    None and no keys are returned."""
+    pages = cache._tensors()
+    tensors = (q, k, v, index, counts, rotary.turns, positions, offset)
+    more = (rotary.amplitude, rotary.interleaved, bool(return_keys))
+    if _lib.plain_eager(*pages, *tensors):
+        q_out, k_out = _lib.host().cache_append_rotary(*pages, *tensors, *more, _lib.status_word(k.device) if k.is_cuda else None)
+        return (q_out, k_out) if return_keys else q_out
+    _refuse_autograd("cache_append_rotary", cache.k, cache.v, q, k, v)
+    q_out, k_out = cache_append_rotary_op(*pages, *tensors, *more)
+    q_out = None if q is None else q_out
+    return (q_out, k_out) if return_keys else q_out
 
 
 @torch.library.custom_op("kohakufa_b200::cache_weights", mutates_args=("weights",), device_types="cuda")

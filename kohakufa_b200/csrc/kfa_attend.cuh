@@ -27,7 +27,7 @@
 //   warps 10, 11    TMA producers: keys (and queries), values; a lane per box of up to 32 rows inside a page
 #pragma once
 
-#include "kfa_cache.cuh"
+#include "kfa_cache_view.cuh"
 
 namespace kfa {
 

@@ -53,6 +53,8 @@ struct Api {
   decltype(&kfa_cache_weigh_bytes) cache_weigh_bytes = nullptr;
   decltype(&kfa_cache_weigh) cache_weigh = nullptr;
   decltype(&kfa_cache_evict_room) cache_evict = nullptr;
+  decltype(&kfa_rotary) rotary = nullptr;
+  decltype(&kfa_cache_append_rotary) cache_append_rotary = nullptr;
 } api;
 
 PyObject* g_error = nullptr;  // kohakufa_b200._lib.KfaError
@@ -463,10 +465,10 @@ struct Gil {
   ~Gil() { PyGILState_Release(state); }
 };
 
-// What Python says about a backward that is about to run: the route (see run_backward), or less than 0 where the registered op
-// has to run instead: it is itself recorded, something is interposed, or a tensor is not a plain one.
-int64_t backward_route(const variable_list& saved, const at::Tensor& g) {
-  if (at::GradMode::is_enabled() || !nothing_interposed()) return -1;
+// Whether a backward that is about to run may go straight to its kernels: it is not itself recorded, nothing is interposed, and
+// all tensors are plain ones.
+bool plain_backward(const variable_list& saved, const at::Tensor& g) {
+  if (at::GradMode::is_enabled() || !nothing_interposed()) return false;
   const Gil held;
   auto plain = [](const at::Tensor& t) {
     PyObject* o = THPVariable_Wrap(t);
@@ -475,11 +477,14 @@ int64_t backward_route(const variable_list& saved, const at::Tensor& g) {
     return yes;
   };
   for (const at::Tensor& t : saved)
-    if (!plain(t)) return -1;
-  if (!plain(g)) return -1;
-  const at::Tensor& q = saved[0];
-  PyObject* r = PyObject_CallFunction(g_route, "LL", static_cast<long long>(q.size(-1)),
-                                      static_cast<long long>(q.dim() == 4 ? q.size(0) * q.size(1) : 0));
+    if (!plain(t)) return false;
+  return plain(g);
+}
+// What Python says about it, for a head dim and a number of batch entries times heads: the route (see run_backward), or less than 0 where the
+// registered op has to run instead.
+int64_t python_route(int64_t dim, int64_t heads) {
+  const Gil held;
+  PyObject* r = PyObject_CallFunction(g_route, "LL", static_cast<long long>(dim), static_cast<long long>(heads));
   const long long route = r ? PyLong_AsLongLong(r) : -1;
   Py_XDECREF(r);
   if (PyErr_Occurred()) {
@@ -488,6 +493,11 @@ int64_t backward_route(const variable_list& saved, const at::Tensor& g) {
     throw e;
   }
   return route;
+}
+int64_t backward_route(const variable_list& saved, const at::Tensor& g) {
+  if (!plain_backward(saved, g)) return -1;
+  const at::Tensor& q = saved[0];
+  return python_route(q.size(-1), q.dim() == 4 ? q.size(0) * q.size(1) : 0);
 }
 
 // A libkfa error on a thread of the engine: the exception that Python sees is the same as from a direct call.
@@ -963,6 +973,183 @@ PyObject* py_cache_evict(Args a, Py_ssize_t n) {
   Py_RETURN_NONE;
 }
 
+// ---------------------------------------------------------------------------------------------------------------------
+// Rotary positions (rotary.py, cache.py)
+// ---------------------------------------------------------------------------------------------------------------------
+struct RotaryArgs {
+  at::Tensor turns, positions, offset;
+  double amplitude;
+  bool interleaved, inverse;
+};
+// turns, positions, offset, amplitude, interleaved
+RotaryArgs rotary_of(Args a) { return {tensor(a[0]), maybe(a[1]), maybe(a[2]), number(a[3]), PyObject_IsTrue(a[4]) != 0, false}; }
+
+// batch, tokens: of the rows; packed ones [T, H, D] are one sequence
+void check_rotary(const char* who, const RotaryArgs& r, const at::Tensor& x, int64_t batch, int64_t tokens) {
+  TORCH_CHECK_TYPE(r.turns.scalar_type() == at::kLong, who, ": the rotary's turns must be int64");
+  TORCH_CHECK_VALUE(r.turns.dim() == 1 && r.turns.is_contiguous() && r.turns.numel() > 0 && 2 * r.turns.numel() <= x.size(-1), who,
+                    ": a rotary of ", std::to_string(2 * r.turns.numel()), " columns does not fit head_dim ", std::to_string(x.size(-1)));
+  TORCH_CHECK_VALUE(std::isfinite(r.amplitude), who, ": the rotary's amplitude must be finite");
+  if (r.positions.defined()) {
+    const int64_t d = r.positions.dim();
+    TORCH_CHECK_TYPE(r.positions.scalar_type() == at::kInt || r.positions.scalar_type() == at::kLong, who, ": positions must be int32 or int64");
+    TORCH_CHECK_VALUE((d == 1 || (d == 2 && x.dim() == 4 && (r.positions.size(0) == batch || r.positions.size(0) == 1))) && r.positions.size(d - 1) == tokens,
+                      who, ": positions must be one per token");
+  }
+  if (r.offset.defined()) {
+    TORCH_CHECK_TYPE(r.offset.scalar_type() == at::kInt, who, ": offset must be int32");
+    TORCH_CHECK_VALUE(x.dim() == 4 && r.offset.dim() == 1 && r.offset.is_contiguous() && r.offset.numel() == batch, who,
+                      ": offset must be a contiguous vector, one entry per sequence");
+  }
+  for (const at::Tensor* t : {&r.turns, &r.positions, &r.offset})
+    TORCH_CHECK_VALUE(!t->defined() || t->device() == x.device(), who, ": tensors on different devices");
+}
+
+KfaRotary rotary_desc(const RotaryArgs& r) {
+  KfaRotary d{r.turns.data_ptr<int64_t>(), r.turns.numel(), r.interleaved, static_cast<float>(r.amplitude), nullptr, {0, 0}, 0, nullptr};
+  if (r.positions.defined()) {
+    const int64_t n = r.positions.dim();
+    d.positions = r.positions.data_ptr();
+    d.position_stride[0] = n == 2 && r.positions.size(0) > 1 ? r.positions.stride(0) : 0;
+    d.position_stride[1] = r.positions.stride(n - 1);
+    d.wide_positions = r.positions.scalar_type() == at::kLong;
+  }
+  if (r.offset.defined()) d.offset = r.offset.data_ptr<int32_t>();
+  return d;
+}
+
+void check_rotated(const char* who, const char* name, const at::Tensor& x, const at::Tensor& q) {
+  TORCH_CHECK_TYPE((x.scalar_type() == at::kHalf || x.scalar_type() == at::kBFloat16 || x.scalar_type() == at::kFloat) &&
+                       x.scalar_type() == q.scalar_type(),
+                   who, ": q and k must be fp16, bf16 or fp32 (both the same)");
+  TORCH_CHECK_VALUE((x.dim() == 4 || x.dim() == 3) && x.dim() == q.dim(), who, ": ", name, " must be [B, H, S, D], or [T, H, D] of packed sequences");
+  TORCH_CHECK_VALUE(x.size(0) == q.size(0) && x.size(-1) == q.size(-1) && (x.dim() == 3 || x.size(2) == q.size(2)), who,
+                    ": k must have the batch, tokens and head dim of q");
+  TORCH_CHECK_VALUE(x.size(1) > 0 && x.size(-1) >= 1 && x.size(-1) <= 1024, who, ": head_dim 1 .. 1024 and at least one head");
+}
+
+KfaTensor4 desc_rows(const at::Tensor& t) { return t.dim() == 3 ? desc_packed(t) : desc(t); }
+
+// q and k (may be undefined) turned
+Two run_rotary(const at::Tensor& q, const at::Tensor& k, const RotaryArgs& r) {
+  const char* who = "apply_rotary";
+  check_rotated(who, "q", q, q);
+  if (k.defined()) check_rotated(who, "k", k, q);
+  check_rotary(who, r, q, q.dim() == 4 ? q.size(0) : 1, q.dim() == 4 ? q.size(2) : q.size(0));
+  for (const at::Tensor* t : {&q, &k}) {
+    if (!t->defined()) continue;
+    TORCH_CHECK_VALUE(t->size(-1) == 1 || t->stride(-1) == 1, who, ": q and k need a contiguous last dim");
+    TORCH_CHECK_VALUE(t->is_cuda(), who, ": CUDA tensors only (there is no CPU path)");
+    TORCH_CHECK_VALUE(t->device() == q.device(), who, ": tensors on different devices");
+  }
+  const c10::cuda::CUDAGuard guard(q.device());
+  auto like = [](const at::Tensor& t) { return t.dim() == 4 ? bshd_like(t) : at::empty(t.sizes(), t.options()); };
+  at::Tensor q_out = like(q), k_out = k.defined() ? like(k) : at::Tensor();
+  if (q.numel() == 0) return {std::move(q_out), std::move(k_out)};  // no tokens
+  const KfaTensor4 d[4] = {desc_rows(q), k.defined() ? desc_rows(k) : KfaTensor4{}, desc_rows(q_out), k.defined() ? desc_rows(k_out) : KfaTensor4{}};
+  const KfaRotary dr = rotary_desc(r);
+  const int dtype = q.scalar_type() == at::kFloat ? KFA_F32 : dtype_code(q);
+  check(api.rotary(d, k.defined() ? d + 1 : nullptr, d + 2, k.defined() ? d + 3 : nullptr, &dr, r.inverse, dtype, stream_of(q)));
+  return {std::move(q_out), std::move(k_out)};
+}
+
+// The gradient is the inverse turn of the gradient: nothing is kept but the angles.
+struct RotaryTurn : torch::autograd::Function<RotaryTurn> {
+  static constexpr bool is_traceable = true;
+  static variable_list forward(AutogradContext* ctx, const at::Tensor& q, const std::optional<at::Tensor>& keys, const RotaryArgs& r) {
+    const at::Tensor k = keys ? *keys : at::Tensor();
+    auto [q_out, k_out] = released([&] { return run_rotary(q, k, r); });
+    ctx->save_for_backward({r.turns, r.positions, r.offset});
+    ctx->saved_data["amplitude"] = r.amplitude;
+    ctx->saved_data["interleaved"] = r.interleaved;
+    ctx->set_materialize_grads(false);
+    if (!k.defined()) return {q_out};
+    return {q_out, k_out};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const variable_list s = ctx->get_saved_variables();
+    const RotaryArgs r{s[0], s[1], s[2], ctx->saved_data["amplitude"].toDouble(), ctx->saved_data["interleaved"].toBool(), true};
+    variable_list out(3), rows;
+    for (const at::Tensor& g : grads)
+      if (g.defined()) rows.push_back(g.unsafeGetTensorImpl()->has_symbolic_sizes_strides() || g.stride(-1) == 1 ? g : g.contiguous());
+    if (rows.empty()) return out;
+    variable_list others;
+    for (const at::Tensor& t : s)
+      if (t.defined()) others.push_back(t);
+    if (rows.size() > 1) others.push_back(rows[1]);
+    variable_list turned;
+    if (plain_backward(others, rows[0]) && python_route(16, 0) >= 0) {  // (the attention kernels' choice of route is nothing to this one)
+      auto [a, b] = in_engine([&] { return run_rotary(rows[0], rows.size() > 1 ? rows[1] : at::Tensor(), r); });
+      turned = {a, b};
+    } else {
+      const auto op = c10::Dispatcher::singleton()
+                          .findSchemaOrThrow("kohakufa_b200::rotary", "")
+                          .typed<at::Tensor(const at::Tensor&, const at::Tensor&, const std::optional<at::Tensor>&, const std::optional<at::Tensor>&, double, bool, bool)>();
+      auto given = [](const at::Tensor& t) { return t.defined() ? std::optional<at::Tensor>(t) : std::nullopt; };
+      for (const at::Tensor& g : rows) turned.push_back(op.call(g, r.turns, given(r.positions), given(r.offset), r.amplitude, r.interleaved, true));
+    }
+    size_t next = 0;
+    for (size_t i = 0; i < grads.size(); ++i)
+      if (grads[i].defined()) out[i] = turned[next++];
+    return out;
+  }
+};
+
+// rotary(q, k, turns, positions, offset, amplitude, interleaved, inverse) -> q and k turned, or q alone where k is None; with its
+// gradient where autograd records
+PyObject* py_rotary(Args a, Py_ssize_t n) {
+  need(n, 8);
+  const at::Tensor q = tensor(a[0]), k = maybe(a[1]);
+  RotaryArgs r = rotary_of(a + 2);
+  r.inverse = PyObject_IsTrue(a[7]);
+  if (at::GradMode::is_enabled() && !r.inverse && (q.requires_grad() || (k.defined() && k.requires_grad()))) {
+    variable_list out = RotaryTurn::apply(q, k.defined() ? std::optional<at::Tensor>(k) : std::nullopt, r);
+    if (!k.defined()) return THPVariable_Wrap(std::move(out[0]));
+    return pack(Two{std::move(out[0]), std::move(out[1])});
+  }
+  auto [q_out, k_out] = released([&] { return run_rotary(q, k, r); });
+  if (!k.defined()) return THPVariable_Wrap(std::move(q_out));
+  return pack(Two{std::move(q_out), std::move(k_out)});
+}
+
+// cache_append_rotary(k_pages, v_pages, lengths, table, q, k, v, index, counts, turns, positions, offset, amplitude, interleaved, return_keys,
+// status) -> q and k turned, None for what is not asked for
+PyObject* py_cache_append_rotary(Args a, Py_ssize_t n) {
+  need(n, 16);
+  const char* who = "cache_append_rotary";
+  const Cache c = cache_of(a);
+  const at::Tensor q = maybe(a[4]), k = tensor(a[5]), v = tensor(a[6]), index = maybe(a[7]), counts = maybe(a[8]), status = maybe(a[15]);
+  const RotaryArgs r = rotary_of(a + 9);
+  const bool keys = PyObject_IsTrue(a[14]);
+  check_no_grad(who, {&c.k, &c.v, &q, &k, &v});
+  check_cache(who, c);
+  check_new(who, "k", c, k, c.k.size(1));
+  check_new(who, "v", c, v, c.k.size(1));
+  TORCH_CHECK_VALUE(k.size(2) == v.size(2), who, ": k and v must have as many tokens");
+  if (q.defined()) {
+    check_new(who, "q", c, q, 0);
+    TORCH_CHECK_VALUE(q.size(2) == k.size(2), who, ": q must have as many tokens as k");
+  }
+  TORCH_CHECK_VALUE(!index.defined() || (!q.defined() && !keys), who, ": with an index only the pages are written: no q, no return_keys");
+  const KfaRows rows = rows_of(who, c, index, counts, k.size(2));
+  check_rotary(who, r, k, k.size(0), k.size(2));
+  check_written(who, c);
+  check_where(who, c, {&q, &k, &v, &index, &counts, &status});
+  will_write({&c.k, &c.v});
+  auto [q_out, k_out] = released([&] {
+    const c10::cuda::CUDAGuard guard(k.device());
+    at::Tensor qo = q.defined() ? bshd_like(q) : at::Tensor(), ko = keys ? bshd_like(k) : at::Tensor();
+    const KfaCache dc = cache_desc(c);
+    const KfaTensor4 dk = desc(k), dv = desc(v), dq = q.defined() ? desc(q) : KfaTensor4{}, dqo = q.defined() ? desc(qo) : KfaTensor4{},
+                     dko = keys ? desc(ko) : KfaTensor4{};
+    const KfaRotary dr = rotary_desc(r);
+    check(api.cache_append_rotary(&dc, q.defined() ? &dq : nullptr, &dk, &dv, &rows, &dr, q.defined() ? &dqo : nullptr, keys ? &dko : nullptr,
+                                  dtype_code(k), status.data_ptr<int32_t>(), stream_of(k)));
+    return Two{std::move(qo), std::move(ko)};
+  });
+  return pack(Two{std::move(q_out), std::move(k_out)});
+}
+
 // bind(KfaError, {entry point: address}, route)
 PyObject* py_bind(Args a, Py_ssize_t n) {
   need(n, 3);
@@ -995,6 +1182,8 @@ PyObject* py_bind(Args a, Py_ssize_t n) {
   take("kfa_cache_weigh_bytes", api.cache_weigh_bytes);
   take("kfa_cache_weigh", api.cache_weigh);
   take("kfa_cache_evict_room", api.cache_evict);
+  take("kfa_rotary", api.rotary);
+  take("kfa_cache_append_rotary", api.cache_append_rotary);
   Py_INCREF(a[0]);
   Py_XDECREF(g_error);
   g_error = a[0];
@@ -1041,6 +1230,8 @@ PyMethodDef methods[] = {
     KFA_METHOD(cache_weights),
     KFA_METHOD(evict),
     KFA_METHOD(cache_evict),
+    KFA_METHOD(rotary),
+    KFA_METHOD(cache_append_rotary),
     {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_kfa_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

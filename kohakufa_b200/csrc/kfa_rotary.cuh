@@ -1,0 +1,222 @@
+// Rotary positions: pairs of a row's columns turned by angles that grow with the row's position, as a pass of its own or on the way into a
+// cache of keys and values.
+//
+//   (y1, y2) = a (x1 cos - x2 sin, x2 cos + x1 sin),   angle = position * f_pair      (the gradient: the same with -sin)
+//
+// Bound by memory: every row is read once and written once. What has to be kept out of the way are the angles. They are not read from a
+// table of positions: f is given in turns as a 64-bit fraction, position * f modulo 2^64 is the angle's fraction of a turn without any error but f's
+// own 2^-65, for every position of 32 bits and more, and sine and cosine are taken of a remainder within an eighth of a turn. A CTA takes a stretch of
+// rows, token by token and head by head, so that one token's sines and cosines, in shared memory, serve all its heads (40 of 32 query and 8 key
+// heads), and asks for its rows before it makes them: what a sine costs (some 40 instructions) passes while the rows are on their way.
+//
+// A thread's unit is a cell: two pieces (of up to 16 bytes) of a row that hold each other's partners. Half layout (columns i and i + R / 2 are a
+// pair): pieces R / 2 apart; interleaved (2 i and 2 i + 1): adjacent ones. Both ways cell j has the pairs j * V .. (j + 1) * V - 1, V columns a piece. Cells behind
+// the turned columns are copied as they are.
+#pragma once
+
+#include "kfa_cache_view.cuh"
+
+namespace kfa {
+
+constexpr int ROT_THREADS = 256;
+constexpr int ROT_CELLS = 2;  // of a thread
+
+struct RotaryStream {  // queries, keys, values
+  const uint8_t* in;
+  long long in_b, in_h, in_s;  // bytes
+  uint8_t* out;                // or nullptr (append: only the pages get it)
+  long long out_b, out_h, out_s;
+};
+
+struct RotaryParams {
+  RotaryStream x[3];
+  int q_heads, qk_heads;          // heads before the keys', before the values'
+  FastDiv by_cell, by_head, by_step, by_pair;  // cells of a row, heads of a token, tokens of a sequence, pairs of a row
+  int pairs, pair_cells, columns, tokens;  // pair_cells: cells with turned columns; tokens: rows of x a sequence has
+  unsigned total, all_tokens;     // cells, tokens
+  const uint64_t* turns;
+  float amplitude, sine;          // of cosine; of sine (negative: the gradient)
+  const void* positions;
+  long long pos_b, pos_s;
+  int pos_wide;                   // int64
+  const int* offset;
+  // append
+  CacheView c;
+  RowsView r;
+  int* status;
+};
+
+__device__ __forceinline__ long long rotary_position(const RotaryParams& p, int b, int i, int t, bool append) {
+  long long at;
+  if (p.positions) {
+    const long long where = b * p.pos_b + t * p.pos_s;
+    at = p.pos_wide ? static_cast<const long long*>(p.positions)[where] : static_cast<const int*>(p.positions)[where];
+  } else {
+    at = append ? static_cast<long long>(p.c.lengths[b]) + i : t;
+  }
+  return p.offset ? at + p.offset[b] : at;
+}
+
+// cos and sin of a position's angle: the fraction of a turn is cut into a quarter and what is left, within an eighth on both sides, of which 32 bits
+// are taken (2^-34 turns; fp32 rounds them by 2^-24 of themselves).
+__device__ __forceinline__ float2 rotary_turn(uint64_t turns, long long position, float amplitude, float sine) {
+  const uint64_t angle = turns * static_cast<uint64_t>(position);
+  const uint64_t quarter = (angle + (1ull << 61)) >> 62;
+  const long long left = static_cast<long long>(angle - (quarter << 62));
+  float s, c;
+  sincospif(static_cast<float>(static_cast<int>(left >> 30)) * 0x1p-33f, &s, &c);
+  const float x = quarter & 1 ? -s : c, y = quarter & 1 ? c : s;
+  const float sign = quarter & 2 ? -1.f : 1.f;
+  return make_float2(x * sign * amplitude, y * sign * sine);
+}
+
+template <int BYTES>
+struct RotaryPiece;
+template <>
+struct RotaryPiece<16> { using type = uint4; };
+template <>
+struct RotaryPiece<8> { using type = uint2; };
+template <>
+struct RotaryPiece<4> { using type = uint32_t; };
+template <>
+struct RotaryPiece<2> { using type = uint16_t; };
+
+template <typename T, int BYTES>
+union RotaryHalf {
+  typename RotaryPiece<BYTES>::type piece;
+  T x[BYTES / sizeof(T)];
+  __device__ RotaryHalf() {}
+};
+
+__device__ __forceinline__ float rotary_float(float x) { return x; }
+__device__ __forceinline__ float rotary_float(__half x) { return __half2float(x); }
+__device__ __forceinline__ float rotary_float(__nv_bfloat16 x) { return __bfloat162float(x); }
+__device__ __forceinline__ void rotary_round(float x, float& y) { y = x; }
+__device__ __forceinline__ void rotary_round(float x, __half& y) { y = __float2half_rn(x); }
+__device__ __forceinline__ void rotary_round(float x, __nv_bfloat16& y) { y = __float2bfloat16_rn(x); }
+
+template <typename T, int BYTES, bool INTERLEAVED, bool APPEND>
+__global__ void __launch_bounds__(ROT_THREADS) kfa_rotary_kernel(const RotaryParams p) {
+  constexpr int V = BYTES / sizeof(T), CHUNK = V < 2 ? 1 : 2, CHUNKS = V / CHUNK;  // pairs of a cell; of a 16-byte piece of them in shared memory
+  using Piece = typename RotaryPiece<BYTES>::type;
+  extern __shared__ float4 rotary_smem[];
+  float2* cs = reinterpret_cast<float2*>(rotary_smem);  // [token][chunk][cell][CHUNK]
+  const unsigned first = blockIdx.x * static_cast<unsigned>(ROT_THREADS * ROT_CELLS);
+  const unsigned last = min(first + ROT_THREADS * ROT_CELLS, p.total) - 1;
+  const unsigned token0 = p.by_head.div(p.by_cell.div(first)), tokens = p.by_head.div(p.by_cell.div(last)) - token0 + 1;
+  wait_for_previous();
+  let_next_begin();
+
+  // ---- this thread's cells are asked for ----
+  RotaryHalf<T, BYTES> a[ROT_CELLS], b[ROT_CELLS];
+  unsigned where[ROT_CELLS];  // token, counted from the CTA's first; head; cell
+  uint8_t* to[ROT_CELLS][2];  // output, page
+  bool zero[ROT_CELLS], two[ROT_CELLS];
+  int second[ROT_CELLS];  // bytes from a to b
+#pragma unroll
+  for (int u = 0; u < ROT_CELLS; ++u) {
+    const unsigned at = first + u * ROT_THREADS + threadIdx.x;
+    to[u][0] = to[u][1] = nullptr;
+    zero[u] = two[u] = false;
+    second[u] = 0;
+    where[u] = 0;
+    if (at >= p.total) continue;
+    const unsigned row = p.by_cell.div(at), cell = at - row * p.by_cell.d;
+    const unsigned token = p.by_head.div(row);
+    int head = static_cast<int>(row - token * p.by_head.d);
+    const unsigned seq = p.by_step.div(token);
+    const int i = static_cast<int>(token - seq * p.by_step.d);
+    const int kind = head < p.q_heads ? 0 : (head < p.qk_heads ? 1 : 2);
+    const RotaryStream& x = p.x[kind];
+    head -= kind == 0 ? 0 : (kind == 1 ? p.q_heads : p.qk_heads);
+    // the first column, and how far the second piece is
+    int column = static_cast<int>(cell) * 2 * V, apart = V;
+    const bool turned = kind < 2 && static_cast<int>(cell) < p.pair_cells;
+    if (!INTERLEAVED && kind < 2) {
+      if (turned) column = static_cast<int>(cell) * V, apart = p.pairs;
+      else column = 2 * p.pairs + (static_cast<int>(cell) - p.pair_cells) * 2 * V;
+    }
+    two[u] = column + apart < p.columns;
+    second[u] = apart * static_cast<int>(sizeof(T));
+    where[u] = (token - token0) << 17 | (turned ? 1u << 16 : 0u) | cell;
+    int t = i;
+    bool there = true, placed = false;
+    int page = -1, slot = 0;
+    if constexpr (APPEND) {
+      there = i < p.r.count(static_cast<int>(seq));
+      if (there) {
+        t = p.r.row(static_cast<int>(seq), i);
+        if (t < 0 || t >= p.r.T) {
+          report(p.status, DEV_BAD_CACHE);
+          there = false;
+        }
+      }
+      if (there && kind > 0) {
+        const int length = p.c.lengths[seq];
+        const long long pos = static_cast<long long>(length) + i;
+        placed = length >= 0 && pos < p.c.capacity && cache_place(p.c, static_cast<int>(seq), static_cast<int>(pos), page, slot);
+        if (!placed) report(p.status, DEV_BAD_CACHE);
+      }
+    }
+    const int bytes = column * static_cast<int>(sizeof(T));
+    if (there) {
+      const uint8_t* from = x.in + seq * x.in_b + head * x.in_h + t * x.in_s + bytes;
+      a[u].piece = *reinterpret_cast<const Piece*>(from);
+      if (two[u]) b[u].piece = *reinterpret_cast<const Piece*>(from + second[u]);
+    }
+    zero[u] = !there;
+    if (x.out != nullptr) to[u][0] = x.out + seq * x.out_b + head * x.out_h + i * x.out_s + bytes;
+    if constexpr (APPEND) {
+      if (placed)
+        to[u][1] = kind == 1 ? p.c.k + page * p.c.k_sn + head * p.c.k_sh + slot * p.c.k_ss + bytes
+                             : p.c.v + page * p.c.v_sn + head * p.c.v_sh + slot * p.c.v_ss + bytes;
+    }
+  }
+
+  // ---- the CTA's tokens' angles ----
+  for (unsigned at = threadIdx.x; at < tokens * p.pairs; at += ROT_THREADS) {
+    const unsigned token = p.by_pair.div(at), pair = at - token * p.pairs;
+    const unsigned seq = p.by_step.div(token0 + token);
+    const int i = static_cast<int>(token0 + token - seq * p.by_step.d);
+    int t = i;
+    if constexpr (APPEND) {
+      if (i >= p.r.count(static_cast<int>(seq))) continue;
+      t = p.r.row(static_cast<int>(seq), i);
+      if (t < 0 || t >= p.r.T) continue;
+    }
+    const unsigned cell = pair / V, in = pair % V;
+    cs[((token * CHUNKS + in / CHUNK) * p.pair_cells + cell) * CHUNK + in % CHUNK] =
+        rotary_turn(p.turns[pair], rotary_position(p, static_cast<int>(seq), i, t, APPEND), p.amplitude, p.sine);
+  }
+  __syncthreads();
+
+#pragma unroll
+  for (int u = 0; u < ROT_CELLS; ++u) {
+    if (to[u][0] == nullptr && to[u][1] == nullptr) continue;
+    const unsigned token = where[u] >> 17, cell = where[u] & 0xffffu;
+    if (zero[u]) {
+      a[u].piece = b[u].piece = Piece{};
+    } else if (where[u] & 1u << 16) {
+      const float2* angles = cs + (token * CHUNKS * p.pair_cells + cell) * CHUNK;
+#pragma unroll
+      for (int k = 0; k < V; ++k) {
+        const float2 y = angles[(k / CHUNK) * p.pair_cells * CHUNK + k % CHUNK];
+        // (pair k of the cell; interleaved: the first half of them lies in the first piece)
+        T& lo = INTERLEAVED ? (2 * k < V ? a[u].x[2 * k % V] : b[u].x[2 * k % V]) : a[u].x[k];
+        T& hi = INTERLEAVED ? (2 * k + 1 < V ? a[u].x[(2 * k + 1) % V] : b[u].x[(2 * k + 1) % V]) : b[u].x[k];
+        if (INTERLEAVED && static_cast<int>(cell) * V + k >= p.pairs) continue;
+        const float x1 = rotary_float(lo), x2 = rotary_float(hi);
+        rotary_round(x1 * y.x - x2 * y.y, lo);
+        rotary_round(x2 * y.x + x1 * y.y, hi);
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < (APPEND ? 2 : 1); ++k) {
+      if (to[u][k] == nullptr) continue;
+      *reinterpret_cast<Piece*>(to[u][k]) = a[u].piece;
+      if (two[u]) *reinterpret_cast<Piece*>(to[u][k] + second[u]) = b[u].piece;
+    }
+  }
+}
+
+}  // namespace kfa
