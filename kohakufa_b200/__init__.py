@@ -20,6 +20,7 @@ from kohakufa_b200.api import attention, attention_varlen, varlen_plan
 from kohakufa_b200.cache import (  # noqa: F401
     KVCache,
     attention_cached,
+    attention_shared,
     cache_append,
     cache_append_rotary,
     cache_evict,

@@ -65,6 +65,8 @@ SYMBOLS = (
     "kfa_cache_evict_room",
     "kfa_rotary",
     "kfa_cache_append_rotary",
+    "kfa_cache_attend_shared_bytes",
+    "kfa_cache_attend_shared",
 )
 
 
@@ -215,9 +217,12 @@ def load() -> ctypes.CDLL:
         O = ctypes.POINTER(KfaRotary)
         lib.kfa_rotary.argtypes = [T, T, T, T, O, i32, i32, vp]
         lib.kfa_cache_append_rotary.argtypes = [C, T, T, T, R, O, T, T, i32, ip, vp]
+        lib.kfa_cache_attend_shared_bytes.restype = ctypes.c_int64
+        lib.kfa_cache_attend_shared_bytes.argtypes = [T, C, C, T]
+        lib.kfa_cache_attend_shared.argtypes = [T, C, ip, C, T, T, vp, I64P, ip, T, fp, vp, f32, i32, ip, vp]
         for name in SYMBOLS:
             if name not in ("kfa_abi_version", "kfa_last_error", "kfa_bwd_stats_bytes", "kfa_bwd_dq_acc_bytes", "kfa_bwd_parts_bytes",
-                            "kfa_cache_attend_bytes", "kfa_cache_weigh_bytes"):  # fmt: skip
+                            "kfa_cache_attend_bytes", "kfa_cache_weigh_bytes", "kfa_cache_attend_shared_bytes"):  # fmt: skip
                 getattr(lib, name).restype = ctypes.c_int
         if lib.kfa_abi_version() != ABI_VERSION:
             raise KfaError(f"libkfa ABI {lib.kfa_abi_version()} != expected {ABI_VERSION}: rebuild")
@@ -232,6 +237,7 @@ HOST_SYMBOLS = (
     "kfa_bwd_parts_bytes", "kfa_bwd_parts_count", "kfa_bwd_parts", "kfa_varlen_zero_rows",
     "kfa_cache_attend_bytes", "kfa_cache_attend", "kfa_cache_append", "kfa_cache_weigh_bytes", "kfa_cache_weigh",
     "kfa_cache_evict_room", "kfa_rotary", "kfa_cache_append_rotary",
+    "kfa_cache_attend_shared_bytes", "kfa_cache_attend_shared",
 )  # fmt: skip
 HOST_PATH = Path(__file__).resolve().parent / "_kfa_host.so"
 _host = None

@@ -28,11 +28,13 @@ HOST = PKG / "_kfa_host.so"
 HOST_SOURCES = [CSRC / "kfa_host.cpp", PKG.parent / "include" / "kfa.h"]
 SHARED = [CSRC / "kfa_ptx.cuh", CSRC / "kfa_call.cuh", PKG.parent / "include" / "kfa.h"]
 CACHE = [CSRC / "kfa_cache_view.cuh", CSRC / "kfa_cache_call.cuh"]
+ATTEND = [CSRC / "kfa_attend.cuh", CSRC / "kfa_attend_call.cuh"]
 # Each source and what it includes; compiled side by side, a source whose object is newer than all of these is not compiled again.
 SOURCES = {
     CSRC / "kfa_api.cu": SHARED
     + [CSRC / f"kfa_{part}.cuh" for part in ("fwd", "bwd", "bwd_fused", "selftest", "cp", "mask", "scores")],
-    CSRC / "kfa_cache.cu": SHARED + CACHE + [CSRC / "kfa_cache.cuh", CSRC / "kfa_attend.cuh", CSRC / "kfa_weigh.cuh"],
+    CSRC / "kfa_cache.cu": SHARED + CACHE + ATTEND + [CSRC / "kfa_cache.cuh", CSRC / "kfa_weigh.cuh"],
+    CSRC / "kfa_shared.cu": SHARED + CACHE + ATTEND,
     CSRC / "kfa_rotary.cu": SHARED + CACHE + [CSRC / "kfa_rotary.cuh"],
 }
 OBJECTS = CSRC / "build"

@@ -23,7 +23,7 @@ from torch import Tensor
 from kohakufa_b200 import _lib
 from kohakufa_b200.rotary import Rotary
 
-__all__ = ["KVCache", "attention_cached", "cache_append", "cache_append_rotary", "cache_evict", "cache_weights", "tree_mask"]
+__all__ = ["KVCache", "attention_cached", "attention_shared", "cache_append", "cache_append_rotary", "cache_evict", "cache_weights", "tree_mask"]
 
 
 class KVCache:
@@ -156,6 +156,60 @@ def attention_cached(
         )
     _refuse_autograd("attention_cached", q, cache.k, cache.v, k, v)
     out, stats = cached_attention_op(q, *pages, k, v, tree, counts, softmax_scale)
+    return (out, stats) if return_stats else out
+
+
+@torch.library.custom_op("kohakufa_b200::shared_attention", mutates_args=(), device_types="cuda")
+def shared_attention_op(
+    q: Tensor, k_prefix: Tensor, v_prefix: Tensor, prefix_lengths: Tensor, prefix_table: Tensor | None, k_pages: Tensor, v_pages: Tensor,
+    lengths: Tensor, table: Tensor | None, starts: Tensor | None, k: Tensor | None, v: Tensor | None, tree: Tensor | None,
+    counts: Tensor | None, scale: float,
+) -> tuple[Tensor, Tensor]:  # fmt: skip
+    return _lib.host().shared_attention(
+        q, k_prefix, v_prefix, prefix_lengths, prefix_table, k_pages, v_pages, lengths, table, starts, k, v, tree, counts, scale, True,
+        _lib.status_word(q.device),
+    )  # fmt: skip
+
+
+@shared_attention_op.register_fake
+def _(q, k_prefix, v_prefix, prefix_lengths, prefix_table, k_pages, v_pages, lengths, table, starts, k, v, tree, counts, scale):
+    batch, heads, tokens, dim = q.shape
+    return q.new_empty(batch, tokens, heads, dim).transpose(1, 2), q.new_empty(batch, heads, 2, tokens, dtype=torch.float32)
+
+
+def attention_shared(
+    q: Tensor,
+    prefix: KVCache,
+    cache: KVCache,
+    k: Tensor | None = None,
+    v: Tensor | None = None,
+    *,
+    starts: Tensor | None = None,
+    tree: Tensor | None = None,
+    counts: Tensor | None = None,
+    scale: float | None = None,
+    return_stats: bool = False,
+):
+    """``attention_cached`` for sequences that go on from prefixes which are stored, and read, once: a system prompt, a document with many
+    questions, many samples of one prompt.
+
+    ``prefix`` holds the prefixes, one per entry of its batch (pages of their own or of the same pool), ``cache`` what each sequence has behind its prefix.
+    ``starts``: int32 ``[P + 1]`` on the device, ascending: sequences ``starts[p] .. starts[p + 1] - 1`` go on from prefix ``p``, those before ``starts[0]`` and from ``starts[P]`` on
+    have none; so the batch is in the order of its prefixes. Without it there is one prefix, of all sequences. New token ``t`` of a sequence sees its
+    whole prefix, all of the sequence's cached positions, and of the new tokens what ``attention_cached`` says, whose other arguments and results are these. The
+    statistics are those over all that a row sees, as ``cache_weights`` wants them, for the cache's own positions.
+
+    The rows of a prefix's sequences are put together, up to 256 of a K / V head, and the prefix is read once for them; what they get from it and from their own
+    cache is joined in fp32. Results repeat bit for bit, but a sequence's last bits depend on how many are in the batch. Keys turned by their positions
+    stand behind the prefix: ``cache_append_rotary(..., offset=lengths of the sequences' prefixes)``."""
+    pages, shared = cache._tensors(), prefix._tensors()
+    softmax_scale = float(q.shape[-1] ** -0.5 if scale is None else scale)
+    if _lib.plain_eager(q, *shared, *pages, starts, k, v, tree, counts):
+        return _lib.host().shared_attention(
+            q, *shared, *pages, starts, k, v, tree, counts, softmax_scale, return_stats, _lib.status_word(q.device) if q.is_cuda else None
+        )
+    _refuse_autograd("attention_shared", q, prefix.k, prefix.v, cache.k, cache.v, k, v)
+    out, stats = shared_attention_op(q, *shared, *pages, starts, k, v, tree, counts, softmax_scale)
     return (out, stats) if return_stats else out
 
 

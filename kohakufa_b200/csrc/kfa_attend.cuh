@@ -25,6 +25,12 @@
 //                   (with more than 128 rows both see every tile, each with half of the rows)
 //   warps 8, 9      MMA issue for the two streams
 //   warps 10, 11    TMA producers: keys (and queries), values; a lane per box of up to 32 rows inside a page
+//
+// Sequences that go on from a shared prefix: the same kernels in two more modes. The softmax over (prefix, own keys) is that of two parts whose (O,
+// m, l) are joined. ATT_PREFIX walks the prefixes: a row tile's rows are those of several sequences (one after the other in the batch, tokens, heads), so that a
+// prefix is read once for up to 256 rows and K / V head; what comes out, fp32, is the carry: per row O before it is divided, m, l, the largest score.
+// ATT_OWN is the plain walk over the sequences' own keys, which at an item's end adds the carry as one more part. Its main loop needs nothing of the
+// kernels before it in the stream, so it waits for them only there: it runs while the prefixes' last CTAs and their join end.
 #pragma once
 
 #include "kfa_cache_view.cuh"
@@ -37,6 +43,8 @@ constexpr int ATT_UNIT = 32;  // keys: what work is counted in
 // issuing warps do not need. (A CTA owns what it was launched with: budgets beyond that would wait for ever.)
 constexpr int ATT_REGS = 168, ATT_REGS_STREAM = 208, ATT_REGS_ISSUE = 88;
 static_assert(2 * 128 * ATT_REGS_STREAM + 128 * ATT_REGS_ISSUE <= ATT_THREADS * ATT_REGS, "register budgets exceed the CTA's allocation");
+
+enum { ATT_PLAIN = 0, ATT_PREFIX = 1, ATT_OWN = 2 };
 
 struct AttendParams {
   CacheView c;
@@ -64,15 +72,44 @@ struct AttendParams {
   float* part_ml;  // [slot][3][rows]: m, l, largest score
   int4* part_meta; // [CTA]: parts of the item that begins in it and ends in another (0: none), sequence, item
   int* status;
+  // shared prefixes. ATT_PREFIX: c has the prefixes, its batch is their number; `items` are those of one tile of sequences
+  const int* starts;  // sequences starts[i] .. starts[i + 1] - 1 go on from prefix i; or nullptr: all from the only one
+  int groups, seqs;   // prefixes, sequences
+  int ts;             // sequences of a row tile
+  FastDiv by_ts, by_seq_rows;  // by_seq_rows: rows of a sequence in a tile, gt x tt
+  float* carry_o;     // [(sequence, head, token)][128]
+  float* carry_ml;    // [3][(sequence, head, token)]: m, l, largest score
+  long long carry_rows;
 };
 
+// The sequences that go on from prefix i: first and behind the last, inside the batch whatever `starts` says.
+__device__ __forceinline__ void prefix_group(const AttendParams& p, int i, int& s0, int& s1) {
+  s0 = 0;
+  s1 = p.seqs;
+  if (p.starts) {
+    s0 = min(max(p.starts[i], 0), p.seqs);
+    s1 = min(max(p.starts[i + 1], s0), p.seqs);
+  }
+}
+// Whether sequence b goes on from a prefix (an empty one counts).
+__device__ __forceinline__ bool has_prefix(const AttendParams& p, int b) { return !p.starts || (b >= p.starts[0] && b < p.starts[p.groups]); }
+
 // The stretch of work of a CTA, from (b, item, unit) to (end_b, end_item, end_unit), walked item by item; every role walks for itself.
-struct Walk {
+// (ATT_PREFIX: b is a prefix.)
+template <int MODE>
+struct WalkOf {
   int b, item, unit, end_b, end_item, end_unit;
   int units, uc, ud, len, count;  // of the item; uc, ud: units of cached and of new keys
   int n;                          // units of the current segment, the part of the item that is this CTA's
+  int items;                      // of b
   __device__ __forceinline__ static void size(const AttendParams& p, int b, int& len, int& count, int& uc, int& ud) {
     len = cache_length(p.c, b);
+    if constexpr (MODE == ATT_PREFIX) {
+      count = 0;
+      uc = (len + ATT_UNIT - 1) / ATT_UNIT;
+      ud = 0;
+      return;
+    }
     count = p.counts ? min(max(p.counts[b], 0), p.T) : p.T;
     if (p.appended) len = count ? min(len + count, p.c.capacity) : 0;
     uc = count ? (len + ATT_UNIT - 1) / ATT_UNIT : 0;
@@ -83,10 +120,17 @@ struct Walk {
     size(p, b, len, count, uc, ud);
     return max(uc + ud, 1);
   }
+  __device__ __forceinline__ static int items_of(const AttendParams& p, int b) {
+    if constexpr (MODE != ATT_PREFIX) return p.items;
+    int s0, s1;
+    prefix_group(p, b, s0, s1);
+    return p.items * static_cast<int>(p.by_ts.div(s1 - s0 + p.ts - 1));
+  }
   __device__ __forceinline__ bool last() const { return b == end_b && item == end_item; }
   __device__ __forceinline__ void load(const AttendParams& p) {
     size(p, b, len, count, uc, ud);
     units = max(uc + ud, 1);
+    items = items_of(p, b);
   }
   __device__ __forceinline__ void cut() { n = (last() ? min(units, end_unit) : units) - unit; }
   __device__ __forceinline__ bool start(const AttendParams& p) {  // false: nothing to do
@@ -97,8 +141,12 @@ struct Walk {
   }
   __device__ __forceinline__ bool next(const AttendParams& p) {  // false: that was the last segment, and it stays the current one
     if (last()) return false;
-    const bool other = item + 1 == p.items;
-    const int b2 = b + (other ? 1 : 0), item2 = other ? 0 : item + 1;
+    const bool other = item + 1 == items;
+    int b2 = b + (other ? 1 : 0);
+    const int item2 = other ? 0 : item + 1;
+    if constexpr (MODE == ATT_PREFIX) {  // (prefixes that nobody goes on from have no items)
+      while (other && b2 < end_b && items_of(p, b2) == 0) ++b2;
+    }
     if (b2 == end_b && item2 == end_item && end_unit == 0) return false;
     b = b2;
     item = item2;
@@ -111,6 +159,7 @@ struct Walk {
   __device__ __forceinline__ bool begins() const { return unit == 0; }
   __device__ __forceinline__ bool ends() const { return unit + n == units; }
 };
+using Walk = WalkOf<ATT_PLAIN>;
 
 // Shares out the whole batch's work, counted(b) of it sequence b's (0 or more), equally: at[0] .. at[1] is this CTA's stretch, found(i, b, off,
 // counted(b)) is called by one thread for each of the two ends that lies inside sequence b, off into it. All threads of the CTA; s_i: 32 ints of
@@ -167,9 +216,10 @@ __device__ __forceinline__ int att_share(const AttendParams& p, int* s_i, F coun
 
 // Which work is this CTA's (all its threads; s_i: 32 ints of shared memory). Synchronises the CTA. chunk, end: units per CTA and where this
 // one's stretch ends, both as they are counted.
-__device__ __forceinline__ bool my_work(const AttendParams& p, int* s_i, Walk& w, int& chunk, int& end) {
+template <int MODE>
+__device__ __forceinline__ bool my_work(const AttendParams& p, int* s_i, WalkOf<MODE>& w, int& chunk, int& end) {
   chunk = end = 0;
-  if (p.whole) {
+  if (MODE != ATT_PREFIX && p.whole) {
     const unsigned all = static_cast<unsigned>(p.c.batch) * p.items;
     const unsigned i0 = p.by_grid.div(static_cast<unsigned>(all)) * blockIdx.x + min(blockIdx.x, all - p.by_grid.div(all) * gridDim.x);
     const unsigned i1 = i0 + p.by_grid.div(all) + (blockIdx.x < all - p.by_grid.div(all) * gridDim.x ? 1 : 0);
@@ -182,8 +232,9 @@ __device__ __forceinline__ bool my_work(const AttendParams& p, int* s_i, Walk& w
     return w.start(p);
   }
   int at[2], total;
-  chunk = att_share(p, s_i, [&](int b) { return (Walk::units_of(p, b) + p.extra) * p.items; }, at, total, [&](int i, int b, int off, int own) {
-    const int each = own / p.items, item = off / each;
+  using W = WalkOf<MODE>;
+  chunk = att_share(p, s_i, [&](int b) { return (W::units_of(p, b) + p.extra) * W::items_of(p, b); }, at, total, [&](int i, int b, int off, int own) {
+    const int each = own / W::items_of(p, b), item = off / each;
     s_i[3 * i] = b;
     s_i[3 * i + 1] = item;
     s_i[3 * i + 2] = max(off - item * each - p.extra, 0);
@@ -341,22 +392,67 @@ __device__ __forceinline__ float part_factor(float m, float l, float m_all, floa
   return ex2((m - m_all) * c_log2);
 }
 
-// The heads and tokens of a row tile's rows.
-struct RowMap {
+// The heads and tokens (ATT_PREFIX: and sequences) of a row tile's rows.
+template <int MODE>
+struct RowMapOf {
   int g, h0, heads, t0;  // K / V head; first head, heads that exist, first token
-  __device__ __forceinline__ RowMap(const AttendParams& p, int item) {
-    g = static_cast<int>(p.by_row_tiles.div(item));
-    const int rt = item - g * p.row_tiles;
+  int s0, s1;            // first sequence, behind the last of the group (else the sequence)
+  __device__ __forceinline__ RowMapOf(const AttendParams& p, int b, int item) {
+    int rt;
+    s0 = b;
+    s1 = b + 1;
+    if constexpr (MODE == ATT_PREFIX) {  // items of a K / V head one after the other: CTAs that run together read the same keys
+      prefix_group(p, b, s0, s1);
+      const int tiles = static_cast<int>(p.by_ts.div(s1 - s0 + p.ts - 1)), per = p.row_tiles * tiles;
+      g = item / per;
+      const int rest = item - g * per, tile_s = static_cast<int>(p.by_row_tiles.div(rest));
+      s0 += tile_s * p.ts;
+      rt = rest - tile_s * p.row_tiles;
+    } else {
+      g = static_cast<int>(p.by_row_tiles.div(item));
+      rt = item - g * p.row_tiles;
+    }
     const int tile_t = static_cast<int>(p.by_head_tiles.div(rt)), tile_h = rt - tile_t * p.head_tiles;
     h0 = g * p.group + tile_h * p.gt;
     heads = min(p.gt, p.group - tile_h * p.gt);
     t0 = tile_t * p.tt;
   }
   __device__ __forceinline__ bool row(const AttendParams& p, int r, int& h, int& t) const {
+    int s;
+    return row(p, r, h, t, s);
+  }
+  __device__ __forceinline__ bool row(const AttendParams& p, int r, int& h, int& t, int& s) const {
+    s = s0;
+    bool in = true;
+    if constexpr (MODE == ATT_PREFIX) {
+      const int ds = static_cast<int>(p.by_seq_rows.div(r));
+      s += ds;
+      in = ds < p.ts && s < s1;
+      r -= ds * static_cast<int>(p.by_seq_rows.d);
+    }
     const int dt = static_cast<int>(p.by_gt.div(r)), dh = r - dt * p.gt;
     h = h0 + dh;
     t = t0 + dt;
-    return dt < p.tt && dh < heads && t < p.T;
+    return in && dt < p.tt && dh < heads && t < p.T;
+  }
+};
+// Rows of a tile that may exist.
+template <int MODE>
+__device__ __forceinline__ int tile_rows(const AttendParams& p) {
+  return MODE == ATT_PREFIX ? p.gt * p.tt * p.ts : p.gt * p.tt;
+}
+
+// What the prefixes have left of a row (ATT_OWN), behind the wait for their kernels. m = -inf, l = 0: nothing.
+struct Carry {
+  float m = -INFINITY, l = 0.f, top = -INFINITY;
+  const float* o = nullptr;
+  __device__ __forceinline__ void load(const AttendParams& p, int b, int h, int t) {
+    if (!has_prefix(p, b)) return;
+    const long long at = (static_cast<long long>(b) * p.H + h) * p.T + t;
+    m = p.carry_ml[at];
+    l = p.carry_ml[p.carry_rows + at];
+    top = p.carry_ml[2 * p.carry_rows + at];
+    o = p.carry_o + at * 128;
   }
 };
 
@@ -376,8 +472,8 @@ struct AttCtl {
 };
 
 // Both kernels' beginning: barriers, tensor memory, the CTA's work.
-template <class R>
-__device__ __forceinline__ bool att_setup(const AttendParams& p, uint32_t bar0, const AttCtl& ctl, int tmem_cols, Walk& first, int& chunk,
+template <class R, int MODE>
+__device__ __forceinline__ bool att_setup(const AttendParams& p, uint32_t bar0, const AttCtl& ctl, int tmem_cols, WalkOf<MODE>& first, int& chunk,
                                           int& end) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (warp == 10) {
@@ -397,8 +493,13 @@ __device__ __forceinline__ bool att_setup(const AttendParams& p, uint32_t bar0, 
     tmem_alloc(smem_u32(ctl.tmem), tmem_cols);
     tmem_relinquish();
   }
-  wait_for_previous();
+  // (ATT_OWN: what is before the prefixes' kernel has ended, that one's CTAs have waited for it before they let others begin.)
+  if (MODE != ATT_OWN) wait_for_previous();
   if (warp == 10 && lane == 0) *ctl.bad = load_status(p.status) != 0;
+  if (MODE == ATT_PREFIX && p.starts && blockIdx.x == 0) {
+    for (int i = threadIdx.x; i <= p.groups; i += ATT_THREADS)
+      if (p.starts[i] < 0 || p.starts[i] > p.seqs || (i > 0 && p.starts[i] < p.starts[i - 1])) report(p.status, DEV_BAD_CACHE);
+  }
   tc_fence_before();
   const bool work = my_work(p, ctl.ints, first, chunk, end);
   let_next_begin();
@@ -407,19 +508,19 @@ __device__ __forceinline__ bool att_setup(const AttendParams& p, uint32_t bar0, 
 }
 
 // The producers' role: warp 10 queries and keys, warp 11 values. Leaves how many tiles and segments' queries it has started.
-template <class R>
-__device__ __forceinline__ void att_produce(const AttendParams& p, const Walk& first, bool values, uint32_t sKV, uint32_t sQ, uint32_t bar0,
+template <class R, int MODE>
+__device__ __forceinline__ void att_produce(const AttendParams& p, const WalkOf<MODE>& first, bool values, uint32_t sKV, uint32_t sQ, uint32_t bar0,
                                             const AttCtl& ac, const CUtensorMap* q_map, const CUtensorMap* map, const CUtensorMap* map_new,
                                             int& kv_issued, int& q_issued) {
   const int lane = threadIdx.x & 31;
   const Ctl ctl{ac.abort};
   auto bar = [&](int i) { return bar0 + 8u * i; };
-  Walk w = first;
+  WalkOf<MODE> w = first;
   const int per_unit = ATT_UNIT / p.box, boxes = 4 * per_unit;
   bool ok = true, more = true;
   int T = 0, s = 0;  // tiles and segments so far
   while (more && ok) {
-    const RowMap rows(p, w.item);
+    const RowMapOf<MODE> rows(p, w.b, w.item);
     if (lane == 0 && !length_ok(p.c, w.b)) *ac.bad = 1;
     if (!values) {
       if (s >= R::NQ) {  // both streams are done with the segment that used this buffer
@@ -427,9 +528,9 @@ __device__ __forceinline__ void att_produce(const AttendParams& p, const Walk& f
         if (!ok) break;
       }
       if (lane == 0) {
-        mbar_expect_tx(bar(R::B_Q + s % R::NQ), R::NC * p.gt * p.tt * 128);
+        mbar_expect_tx(bar(R::B_Q + s % R::NQ), R::NC * tile_rows<MODE>(p) * 128);
         for (int ch = 0; ch < R::NC; ++ch)
-          tma_load_4d(sQ + (s % R::NQ) * R::Q_BYTES + ch * R::Q_CHUNK, q_map, bar(R::B_Q + s % R::NQ), ch * 64, rows.h0, rows.t0, w.b);
+          tma_load_4d(sQ + (s % R::NQ) * R::Q_BYTES + ch * R::Q_CHUNK, q_map, bar(R::B_Q + s % R::NQ), ch * 64, rows.h0, rows.t0, rows.s0);
       }
       q_issued = s + 1;
     }
@@ -478,9 +579,9 @@ struct AttTile {
   bool opens;  // the stream's first tile of segment s
   bool closes; // the segment's last tile
 };
-template <bool BOTH>
+template <bool BOTH, class W = Walk>
 struct AttTiles {
-  Walk w;
+  W w;
   int st, at = 0, T = 0, s = 0, uses = 0;
   bool more = true, opens = true;
   __device__ __forceinline__ bool take(const AttendParams& p, AttTile& t) {
@@ -508,10 +609,10 @@ struct AttTiles {
 // values of piece i - 2 have been issued, values of piece j as soon as P and V are there, whichever comes first: neither holds the other up
 // (keys that are late would delay values whose results others wait for). PIECES of a tile: 1, or 2 halves of 64 keys.
 // issue_S(tile, c, piece), issue_PV(tile, c, piece) issue and commit; c counts the stream's tiles.
-template <class R, int PIECES, int NP, typename FS, typename FP>
-__device__ __forceinline__ void att_issue(const AttendParams& p, const Walk& first, int st, uint32_t bar0, const AttCtl& ac, FS issue_S, FP issue_PV) {
+template <class R, int PIECES, int NP, class W, typename FS, typename FP>
+__device__ __forceinline__ void att_issue(const AttendParams& p, const W& first, int st, uint32_t bar0, const AttCtl& ac, FS issue_S, FP issue_PV) {
   auto ready = [&](int i, uint32_t parity) { return __all_sync(0xffffffffu, mbar_test(bar0 + 8u * i, parity)); };
-  AttTiles<R::BOTH> tiles{first, st};
+  AttTiles<R::BOTH, W> tiles{first, st};
   AttTile ahead = {0, 0, 0, false, false}, even = ahead, odd = ahead;  // the next to get scores; those that have, by c (at most two wait for values)
   bool have = tiles.take(p, ahead);
   int i_s = 0, i_p = 0;  // pieces of scores and of values issued
@@ -580,7 +681,8 @@ __device__ __forceinline__ uint32_t tree_bits(const uint8_t* at, long long strid
 }
 
 // Which keys of a unit the row of token t sees, a bit each (the first pass of a masked tile).
-__device__ __forceinline__ uint32_t seen_word(const AttendParams& p, const Walk& w, int unit, int t) {
+template <class W>
+__device__ __forceinline__ uint32_t seen_word(const AttendParams& p, const W& w, int unit, int t) {
   if (unit >= w.unit + w.n) return 0u;
   if (unit < w.uc) {
     const int left = w.len - unit * ATT_UNIT;
@@ -605,8 +707,8 @@ __device__ __forceinline__ bool odd_half(uint32_t x) {  // all exponent bits: in
   constexpr uint32_t E = BF16 ? 0x7f80u : 0x7c00u;
   return (x & E) == E;
 }
-template <bool BF16>
-__device__ __forceinline__ uint32_t odd_values(const AttendParams& p, const Walk& w, int g, int fresh) {
+template <bool BF16, class W>
+__device__ __forceinline__ uint32_t odd_values(const AttendParams& p, const W& w, int g, int fresh) {
   if (fresh < 0) return 0u;
   const uint8_t* row = p.v + w.b * p.v_sb + g * p.v_sh + fresh * p.v_ss;
   uint32_t found = 0;
@@ -619,8 +721,8 @@ __device__ __forceinline__ uint32_t odd_values(const AttendParams& p, const Walk
   }
   return found;
 }
-template <int NC, bool BF16>
-__device__ __forceinline__ void clean_values(const AttendParams& p, const Walk& w, int g, uint32_t stage, int key, bool valid, int fresh, uint32_t odd) {
+template <int NC, bool BF16, class W>
+__device__ __forceinline__ void clean_values(const AttendParams& p, const W& w, int g, uint32_t stage, int key, bool valid, int fresh, uint32_t odd) {
   const uint32_t row = stage + key * 128;
   if (!valid) {
 #pragma unroll
@@ -643,7 +745,8 @@ __device__ __forceinline__ void clean_values(const AttendParams& p, const Walk& 
   }
 }
 // What key `key` of the tile at unit ub is: whether it exists; the new token that it is, < 0: a cached one.
-__device__ __forceinline__ bool which_key(const Walk& w, int ub, int key, int& fresh) {
+template <class W>
+__device__ __forceinline__ bool which_key(const W& w, int ub, int key, int& fresh) {
   const int unit = ub + (key >> 5);
   fresh = -1;
   if (unit >= w.unit + w.n) return false;
@@ -654,14 +757,15 @@ __device__ __forceinline__ bool which_key(const Walk& w, int ub, int key, int& f
   return true;
 }
 // Whether the row of token t sees new token j.
-__device__ __forceinline__ bool sees_new(const AttendParams& p, const Walk& w, int t, int j) {
+template <class W>
+__device__ __forceinline__ bool sees_new(const AttendParams& p, const W& w, int t, int j) {
   return t < w.count && (p.tree ? p.tree[w.b * p.tree_sb + t * p.tree_st + j * p.tree_sj] != 0 : j <= t);
 }
 
 // After a wait that ran out: the copies that the producers have started land, and the rows of what the CTA had whole read as NaN (what
 // was cut, the joining kernel sees to). All threads, behind a barrier.
-template <class R>
-__device__ __forceinline__ void att_give_up(const AttendParams& p, const Walk& first, bool work, uint32_t bar0, const AttCtl& ac, int kv_issued,
+template <class R, int MODE>
+__device__ __forceinline__ void att_give_up(const AttendParams& p, const WalkOf<MODE>& first, bool work, uint32_t bar0, const AttCtl& ac, int kv_issued,
                                             int q_issued) {
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) report_abort(ac.abort, p.status);
@@ -670,11 +774,12 @@ __device__ __forceinline__ void att_give_up(const AttendParams& p, const Walk& f
     for (int T = max(kv_issued - R::RINGS * (warp == 10 ? R::DK : R::DV), 0); T < kv_issued; ++T)
       mbar_drain(bar0 + 8u * (R::B_KV + (warp == 10 ? R::k_stage(T) : R::v_stage(T))), (warp == 10 ? R::k_turn(T) : R::v_turn(T)) & 1);
   }
-  Walk w = first;
+  if (MODE == ATT_PREFIX) return;  // (the carry is not used then: the kernel behind this one sees the status word)
+  WalkOf<MODE> w = first;
   bool more = work;
   while (more) {
     if (w.begins() && w.ends()) {
-      const RowMap rows(p, w.item);
+      const RowMapOf<MODE> rows(p, w.b, w.item);
       const int pieces = p.c.cols / 8;
       for (int i = tid; i < p.gt * p.tt * pieces; i += ATT_THREADS) {
         int h, t;
@@ -692,7 +797,8 @@ __device__ __forceinline__ void att_give_up(const AttendParams& p, const Walk& f
 }
 
 // What begins in this CTA and ends in another, for the joining kernel: only its last item can. w: the walk at its end.
-__device__ __forceinline__ void note_parts(const AttendParams& p, const Walk& w, bool work, int chunk, int end) {
+template <class W>
+__device__ __forceinline__ void note_parts(const AttendParams& p, const W& w, bool work, int chunk, int end) {
   int4 meta = make_int4(0, 0, 0, 0);
   if (work && w.begins() && !w.ends()) meta = make_int4((end - w.n + w.units - 1) / chunk - static_cast<int>(blockIdx.x) + 1, w.b, w.item, 0);
   p.part_meta[blockIdx.x] = meta;
@@ -706,7 +812,7 @@ struct AttCfg : AttRings<NC, N, 2, false, 2 * (N <= 32 ? 2 : 1) * 128 * N * 2 + 
   static constexpr int TMEM = N == 64 ? 512 : (N == 32 ? 256 : 128);  // 6 N columns: S 2 x 2, O 2
 };
 
-template <int NC, int N, bool BF16>
+template <int NC, int N, bool BF16, int MODE = ATT_PLAIN>
 __global__ void __launch_bounds__(ATT_THREADS, 1)
 kfa_cache_attend_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                         const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmKn,
@@ -730,7 +836,7 @@ kfa_cache_attend_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
   if (tid == 32 * 11) {
     for (const CUtensorMap* map : {&tmQ, &tmK, &tmV, &tmKn, &tmVn}) asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
   }
-  Walk first;
+  WalkOf<MODE> first;
   int chunk, end;
   const bool work = att_setup<R>(p, bar0, ac, R::TMEM, first, chunk, end);
   const uint32_t tmem = *ac.tmem;
@@ -739,7 +845,7 @@ kfa_cache_attend_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
   int kv_issued = 0, q_issued = 0;
 
   if (!work) {
-    if (tid == 0 && !p.whole) note_parts(p, first, false, 1, 0);
+    if (tid == 0 && (MODE == ATT_PREFIX || !p.whole)) note_parts(p, first, false, 1, 0);
   } else if (warp >= 10) {
     if constexpr (N == 64) reg_budget<ATT_REGS_ISSUE, ATT_REGS>();
     const bool values = warp == 11;
@@ -782,11 +888,11 @@ kfa_cache_attend_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
     float* shift = s_shift + warp * N;
     const float c_log2 = p.c_log2;
     const float2 c2 = make_float2(c_log2, c_log2);
-    Walk w = first;
+    WalkOf<MODE> w = first;
     bool more = true, ok = true;
     int c = 0, T0 = 0, s = 0;  // the stream's tiles; tiles and segments before
     while (more) {
-      const RowMap rows(p, w.item);
+      const RowMapOf<MODE> rows(p, w.b, w.item);
       float l[N], m_ref[PER], m_top[PER];
 #pragma unroll
       for (int i = 0; i < N; ++i) l[i] = 0.f;
@@ -937,8 +1043,9 @@ kfa_cache_attend_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
       tc_fence_before();
       named_sync<3, 256>();
       tc_fence_after();
-      const bool bad = *ac.bad != 0;
       const bool whole = w.begins() && w.ends();
+      if (MODE == ATT_OWN && whole) wait_for_previous();  // the carry is there
+      const bool bad = *ac.bad != 0 || (MODE == ATT_OWN && whole && load_status(p.status) != 0);
       const long long slot = 2ll * blockIdx.x + (w.begins() ? 1 : 0);
       // new tokens of the segment, where some of their values were left out (a stream may be one segment ahead: >=)
       const bool odd = ac.odd[0] >= s + 1 || ac.odd[1] >= s + 1;
@@ -952,21 +1059,41 @@ kfa_cache_attend_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
       const float m0 = f0[4 * N], m1 = f1[4 * N], m = fmaxf(m0, m1), top = fmaxf(f0[5 * N], f1[5 * N]);
       const float l0 = (f0[0] + f0[N]) + (f0[2 * N] + f0[3 * N]), l1 = (f1[0] + f1[N]) + (f1[2 * N] + f1[3 * N]);
       float a0 = part_factor(m0, l0, m, c_log2), a1 = part_factor(m1, l1, m, c_log2);
-      const float l_all = l0 * a0 + l1 * a1;
-      int h, tk;
-      const bool exists = rows.row(p, c0 + (lane & (W - 1)), h, tk);
-      const long long off = exists ? w.b * p.o_sb + h * p.o_sh + tk * p.o_ss : -1;
+      float l_all = l0 * a0 + l1 * a1, m_all = m, top_all = top, ac_carry = -1.f;
+      int h, tk, sq;
+      const bool exists = rows.row(p, c0 + (lane & (W - 1)), h, tk, sq);
+      // (ATT_PREFIX: of the carry's rows)
+      const long long row_at = exists ? (static_cast<long long>(sq) * p.H + h) * p.T + tk : -1;
+      const long long off = MODE == ATT_PREFIX ? row_at : (exists ? w.b * p.o_sb + h * p.o_sh + tk * p.o_ss : -1);
+      [[maybe_unused]] Carry carry;
+      if (MODE == ATT_OWN && whole && exists) {
+        carry.load(p, w.b, h, tk);
+        m_all = fmaxf(m, carry.m);
+        top_all = fmaxf(top, carry.top);
+        const float own = part_factor(m, l_all, m_all, c_log2);
+        ac_carry = part_factor(carry.m, carry.l, m_all, c_log2);
+        a0 = own < 0.f || a0 < 0.f ? -1.f : a0 * own;
+        a1 = own < 0.f || a1 < 0.f ? -1.f : a1 * own;
+        l_all = l_all * own + carry.l * ac_carry;
+      }
       const bool some = exists && tk < w.count && l_all != 0.f;
       const float nan = __int_as_float(0x7fc00000);
-      if (whole) {
+      if (MODE == ATT_PREFIX && whole) {
+        if (wl == 0 && exists && lane < W) {
+          p.carry_ml[row_at] = m;
+          p.carry_ml[p.carry_rows + row_at] = l_all;
+          p.carry_ml[2 * p.carry_rows + row_at] = top;
+        }
+      } else if (whole) {
         const float inv = some ? 1.f / l_all : 0.f;
         if (p.stats && wl == 0 && exists && lane < W) {
           float* at = p.stats + (static_cast<long long>(w.b) * p.H + h) * 2 * p.T + tk;
-          at[0] = bad ? nan : (some ? top : INFINITY);
-          at[p.T] = bad ? nan : (some ? log2f(l_all) + (m - top) * c_log2 : 0.f);
+          at[0] = bad ? nan : (some ? top_all : INFINITY);
+          at[p.T] = bad ? nan : (some ? log2f(l_all) + (m_all - top_all) * c_log2 : 0.f);
         }
         a0 = some ? a0 * inv : -1.f;
         a1 = some ? a1 * inv : -1.f;
+        if (MODE == ATT_OWN) ac_carry = some ? ac_carry * inv : -1.f;
       } else if (wl == 0 && lane < W) {
         float* at = p.part_ml + slot * 3 * p.rows + c0 + lane;
         at[0] = m;
@@ -991,7 +1118,21 @@ kfa_cache_attend_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
             if (sees_new(p, w, rows.t0 + static_cast<int>(p.by_gt.div(c0 + i)), j)) o0[i] += y;
         }
       }
-      if (whole) {
+      if (MODE == ATT_OWN && whole) {
+#pragma unroll
+        for (int i = 0; i < W; ++i) {
+          const float x = __shfl_sync(0xffffffffu, ac_carry, i);
+          const long long at = __shfl_sync(0xffffffffu, row_at, i);
+          if (!(x < 0.f) && d < p.c.cols) o0[i] += x * p.carry_o[at * 128 + d];
+        }
+      }
+      if (MODE == ATT_PREFIX && whole) {
+#pragma unroll
+        for (int i = 0; i < W; ++i) {
+          const long long at = __shfl_sync(0xffffffffu, off, i);
+          if (at >= 0) p.carry_o[at * 128 + d] = o0[i];
+        }
+      } else if (whole) {
 #pragma unroll
         for (int i = 0; i < W; ++i) {
           const long long at = __shfl_sync(0xffffffffu, off, i);
@@ -1003,7 +1144,7 @@ kfa_cache_attend_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
       } else {
 #pragma unroll
         for (int i = 0; i < W; ++i)
-          if (c0 + i < p.gt * p.tt) p.part_o[(slot * p.rows + c0 + i) * 128 + d] = o0[i];
+          if (c0 + i < tile_rows<MODE>(p)) p.part_o[(slot * p.rows + c0 + i) * 128 + d] = o0[i];
       }
       tc_fence_before();
       if (tiles > 1 || ((T0 - 1) & 1) == 0) mbar_arrive(bar(R::B_OFREE));
@@ -1012,10 +1153,11 @@ kfa_cache_attend_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
       ++s;
       more = w.next(p);
     }
-    if (tid == 0 && !p.whole) note_parts(p, w, true, chunk, end);
+    if (tid == 0 && (MODE == ATT_PREFIX || !p.whole)) note_parts(p, w, true, chunk, end);
   }
 
   // ---- teardown (every thread gets here, also after an abort) ----
+  if (MODE == ATT_OWN) wait_for_previous();  // (so that who waits for this kernel has waited for those before it)
   tc_fence_before();
   __syncthreads();
   if (tid == 0 && *ac.bad) report(p.status, DEV_BAD_CACHE);
@@ -1035,7 +1177,7 @@ struct AttRowsCfg : AttRings<NC, 128 * HALVES, HALVES == 1 ? 2 : 1, HALVES == 2,
 
 // A tile's 128 score columns are made and used as two halves of 64 keys, each with its own barriers: P (16-bit) lies over the first 32
 // of its half's columns, and while one half's values are multiplied and its next scores made, the thread works on the other.
-template <int NC, int HALVES, bool BF16>
+template <int NC, int HALVES, bool BF16, int MODE = ATT_PLAIN>
 __global__ void __launch_bounds__(ATT_THREADS, 1)
 kfa_cache_attend_rows_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                              const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmKn,
@@ -1058,7 +1200,7 @@ kfa_cache_attend_rows_kernel(const __grid_constant__ CUtensorMap tmQ, const __gr
   if (tid == 32 * 11) {
     for (const CUtensorMap* map : {&tmQ, &tmK, &tmV, &tmKn, &tmVn}) asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
   }
-  Walk first;
+  WalkOf<MODE> first;
   int chunk, end;
   const bool work = att_setup<R>(p, bar0, ac, R::TMEM, first, chunk, end);
   const uint32_t tmem = *ac.tmem;
@@ -1066,7 +1208,7 @@ kfa_cache_attend_rows_kernel(const __grid_constant__ CUtensorMap tmQ, const __gr
   int kv_issued = 0, q_issued = 0;
 
   if (!work) {
-    if (tid == 0 && !p.whole) note_parts(p, first, false, 1, 0);
+    if (tid == 0 && (MODE == ATT_PREFIX || !p.whole)) note_parts(p, first, false, 1, 0);
   } else if (warp >= 10) {
     reg_budget<ATT_REGS_ISSUE, ATT_REGS>();
     const bool values = warp == 11;
@@ -1108,13 +1250,13 @@ kfa_cache_attend_rows_kernel(const __grid_constant__ CUtensorMap tmQ, const __gr
     const float c_log2 = p.c_log2;
     const float2 c2 = make_float2(c_log2, c_log2);
     const int r = (BOTH ? 128 * st : 0) + r_in;  // the thread's row of the tile
-    Walk w = first;
+    WalkOf<MODE> w = first;
     bool more = true, ok = true;
     int c = 0, T0 = 0, s = 0;  // the stream's tiles; tiles and segments before
     while (more) {
-      const RowMap rows(p, w.item);
-      int h, tk;
-      const bool exists = rows.row(p, r, h, tk);
+      const RowMapOf<MODE> rows(p, w.b, w.item);
+      int h, tk, sq;
+      const bool exists = rows.row(p, r, h, tk, sq);
       float l = 0.f, m_ref = -INFINITY, m_top = -INFINITY;
       const int tiles = w.tiles();
       // the stream's tiles of the segment, every STEP-th from t_first on, as pieces of 64 keys; those below t_full hold cached keys only
@@ -1251,15 +1393,36 @@ kfa_cache_attend_rows_kernel(const __grid_constant__ CUtensorMap tmQ, const __gr
         l_all = l0 * a0 + l1 * a1;
       }
       tc_fence_after();
-      const bool bad = *ac.bad != 0;
       const bool whole = w.begins() && w.ends();
+      if (MODE == ATT_OWN && whole) wait_for_previous();  // the carry is there
+      const bool bad = *ac.bad != 0 || (MODE == ATT_OWN && whole && load_status(p.status) != 0);
       const long long slot = 2ll * blockIdx.x + (w.begins() ? 1 : 0);
       const bool odd = ac.odd[st] >= s + 1 || (!BOTH && ac.odd[1 - st] >= s + 1);
       const int j0 = max(w.unit - w.uc, 0) * ATT_UNIT, j1 = odd ? min((w.unit + w.n - w.uc) * ATT_UNIT, w.count) : 0;
+      const long long row_at = exists ? (static_cast<long long>(sq) * p.H + h) * p.T + tk : -1;  // of the carry
+      float ac_carry = -1.f;
+      [[maybe_unused]] Carry carry;
+      if (MODE == ATT_OWN && whole && exists) {
+        carry.load(p, w.b, h, tk);
+        const float m_own = m;
+        m = fmaxf(m, carry.m);
+        top = fmaxf(top, carry.top);
+        const float own = part_factor(m_own, l_all, m, c_log2);
+        ac_carry = part_factor(carry.m, carry.l, m, c_log2);
+        a0 = own < 0.f || a0 < 0.f ? -1.f : a0 * own;
+        a1 = own < 0.f || a1 < 0.f ? -1.f : a1 * own;
+        l_all = l_all * own + carry.l * ac_carry;
+      }
       const bool some = exists && tk < w.count && l_all != 0.f;
       const float nan = __int_as_float(0x7fc00000);
       const bool writes = BOTH || st == 0;  // of the row's statistics
-      if (whole) {
+      if (MODE == ATT_PREFIX && whole) {
+        if (exists && writes) {
+          p.carry_ml[row_at] = m;
+          p.carry_ml[p.carry_rows + row_at] = l_all;
+          p.carry_ml[2 * p.carry_rows + row_at] = top;
+        }
+      } else if (whole) {
         const float inv = some ? 1.f / l_all : 0.f;
         if (p.stats && exists && writes) {
           float* at = p.stats + (static_cast<long long>(w.b) * p.H + h) * 2 * p.T + tk;
@@ -1268,7 +1431,8 @@ kfa_cache_attend_rows_kernel(const __grid_constant__ CUtensorMap tmQ, const __gr
         }
         a0 = some ? a0 * inv : -1.f;
         a1 = some ? a1 * inv : -1.f;
-      } else if (writes && r < p.gt * p.tt) {
+        if (MODE == ATT_OWN) ac_carry = some ? ac_carry * inv : -1.f;
+      } else if (writes && r < tile_rows<MODE>(p)) {
         float* at = p.part_ml + slot * 3 * p.rows + r;
         at[0] = m;
         at[p.rows] = l_all;
@@ -1279,7 +1443,7 @@ kfa_cache_attend_rows_kernel(const __grid_constant__ CUtensorMap tmQ, const __gr
       // lies as the threads have it, 4 columns of 32 rows after 4 columns of 32 rows: each store is 512 bytes in one piece.
       const uint32_t turn = (lane >> 1) & 3;
       const uint32_t out_stage = smem_u32(s_fin) + 6144 + warp * 2048;  // 32 rows of 64 bytes
-      const long long off = exists ? w.b * p.o_sb + static_cast<long long>(h) * p.o_sh + tk * p.o_ss : -1;
+      const long long off = MODE == ATT_PREFIX ? row_at : (exists ? w.b * p.o_sb + static_cast<long long>(h) * p.o_sh + tk * p.o_ss : -1);
       const int r_warp = r - lane;
 #pragma unroll 1
       for (int i = BOTH ? 0 : 32 * st; i < D; i += BOTH ? 32 : 64) {
@@ -1305,8 +1469,41 @@ kfa_cache_attend_rows_kernel(const __grid_constant__ CUtensorMap tmQ, const __gr
             if (!(fabsf(y) < INFINITY)) o0[k] += y;
           }
         }
+        if (MODE == ATT_OWN && !(ac_carry < 0.f)) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            if (i + 4 * j >= p.c.cols) break;
+            const float4 y = *reinterpret_cast<const float4*>(carry.o + i + 4 * j);
+            o0[4 * j] += ac_carry * y.x;
+            o0[4 * j + 1] += ac_carry * y.y;
+            o0[4 * j + 2] += ac_carry * y.z;
+            o0[4 * j + 3] += ac_carry * y.w;
+          }
+        }
         __syncwarp();
-        if (whole) {
+        if (MODE == ATT_PREFIX && whole) {
+#pragma unroll
+          for (int q = 0; q < 2; ++q) {  // rows of 16 columns: 4 pieces
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(out_stage + lane * 64 + ((j ^ turn) << 4)), "f"(o0[16 * q + 4 * j]),
+                           "f"(o0[16 * q + 4 * j + 1]), "f"(o0[16 * q + 4 * j + 2]), "f"(o0[16 * q + 4 * j + 3])
+                           : "memory");
+            __syncwarp();
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const int row = 8 * k + (lane >> 2), piece = lane & 3;
+              const long long at = __shfl_sync(0xffffffffu, off, row);
+              float4 y;
+              asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+                           : "=f"(y.x), "=f"(y.y), "=f"(y.z), "=f"(y.w)
+                           : "r"(out_stage + row * 64 + ((piece ^ ((row >> 1) & 3)) << 4))
+                           : "memory");
+              if (at >= 0) *reinterpret_cast<float4*>(p.carry_o + at * 128 + i + 16 * q + 4 * piece) = y;
+            }
+            __syncwarp();
+          }
+        } else if (whole) {
 #pragma unroll
           for (int j = 0; j < 4; ++j)  // rows of 64 bytes: 4 pieces
             asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(out_stage + lane * 64 + ((j ^ turn) << 4)),
@@ -1326,7 +1523,7 @@ kfa_cache_attend_rows_kernel(const __grid_constant__ CUtensorMap tmQ, const __gr
             if (bad) y = make_uint4(0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu);
             if (at >= 0 && i + 8 * piece < p.c.cols) *reinterpret_cast<uint4*>(p.o + at + 2 * i + 16 * piece) = y;
           }
-        } else if (r_warp < p.gt * p.tt) {
+        } else if (r_warp < tile_rows<MODE>(p)) {
           float4* at = reinterpret_cast<float4*>(p.part_o + (slot * p.rows + r_warp) * 128) + 8 * i + lane;
 #pragma unroll
           for (int j = 0; j < 8; ++j) at[32 * j] = make_float4(o0[4 * j], o0[4 * j + 1], o0[4 * j + 2], o0[4 * j + 3]);
@@ -1343,10 +1540,11 @@ kfa_cache_attend_rows_kernel(const __grid_constant__ CUtensorMap tmQ, const __gr
       ++s;
       more = w.next(p);
     }
-    if (tid == 0 && !p.whole) note_parts(p, w, true, chunk, end);
+    if (tid == 0 && (MODE == ATT_PREFIX || !p.whole)) note_parts(p, w, true, chunk, end);
   }
 
   // ---- teardown (every thread gets here, also after an abort) ----
+  if (MODE == ATT_OWN) wait_for_previous();  // (so that who waits for this kernel has waited for those before it)
   tc_fence_before();
   __syncthreads();
   if (tid == 0 && *ac.bad) report(p.status, DEV_BAD_CACHE);
@@ -1360,19 +1558,21 @@ kfa_cache_attend_rows_kernel(const __grid_constant__ CUtensorMap tmQ, const __gr
 // Joins the parts of the items that were cut: CTA x has the item that begins in CTA x of the kernel above, a warp a row, a lane four
 // columns. Starts while that kernel ends and waits for it. 32 parts at a time: a lane has the factor of one, and all add up their columns; the
 // first AHEAD parts' columns are on their way while the factors are found (drafts of 7 tokens 15.2 -> 14.2 us).
-template <bool BF16>
+template <bool BF16, int MODE = ATT_PLAIN>
 __global__ void __launch_bounds__(256) kfa_cache_join_kernel(const AttendParams p) {
   constexpr int AHEAD = 4;
+  if (MODE == ATT_PREFIX) let_next_begin();  // (it waits for this kernel when it needs the carry)
   wait_for_previous();
-  let_next_begin();
+  if (MODE != ATT_PREFIX) let_next_begin();
   const int4 meta = p.part_meta[blockIdx.x];
   if (meta.x == 0) return;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = blockIdx.y * 8 + warp;
-  const RowMap rows(p, meta.z);
-  int h, t;
-  if (!rows.row(p, r, h, t)) return;
+  const RowMapOf<MODE> rows(p, meta.y, meta.z);
+  int h, t, sq;
+  if (!rows.row(p, r, h, t, sq)) return;
   const bool bad = *reinterpret_cast<const volatile int*>(p.status) != 0;
-  const int count = p.counts ? min(max(p.counts[meta.y], 0), p.T) : p.T;
+  const int count = MODE != ATT_PREFIX && p.counts ? min(max(p.counts[meta.y], 0), p.T) : p.T;
+  const long long row_at = (static_cast<long long>(sq) * p.H + h) * p.T + t;  // of the carry
   // part i: the first in slot 1 of its CTA, the others in slot 0 of theirs
   auto slot = [&](int i) { return 2ll * (blockIdx.x + i) + (i == 0 ? 1 : 0); };
   const float* o_row = p.part_o + r * 128 + 4 * lane;
@@ -1417,6 +1617,28 @@ __global__ void __launch_bounds__(256) kfa_cache_join_kernel(const AttendParams 
 #pragma unroll 4
     for (int i = AHEAD; i < n; ++i) add(i, part(i));
   }
+  if constexpr (MODE == ATT_PREFIX) {
+    *reinterpret_cast<float4*>(p.carry_o + row_at * 128 + 4 * lane) = o;
+    if (lane == 0) {
+      p.carry_ml[row_at] = m;
+      p.carry_ml[p.carry_rows + row_at] = l;
+      p.carry_ml[2 * p.carry_rows + row_at] = top;
+    }
+    return;
+  }
+  if constexpr (MODE == ATT_OWN) {
+    Carry carry;
+    carry.load(p, meta.y, h, t);
+    const float m_new = fmaxf(m, carry.m), own = part_factor(m, l, m_new, p.c_log2), a = part_factor(carry.m, carry.l, m_new, p.c_log2);
+    const float a_own = own < 0.f ? 0.f : own;
+    float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (!(a < 0.f) && 4 * lane < p.c.cols) y = *reinterpret_cast<const float4*>(carry.o + 4 * lane);
+    o = make_float4(o.x * a_own, o.y * a_own, o.z * a_own, o.w * a_own);
+    if (!(a < 0.f)) o = make_float4(o.x + a * y.x, o.y + a * y.y, o.z + a * y.z, o.w + a * y.w);
+    l = l * a_own + carry.l * a;
+    m = m_new;
+    top = fmaxf(top, carry.top);
+  }
   const bool some = t < count && l != 0.f;
   const float nan = __int_as_float(0x7fc00000), inv = some ? 1.f / l : 0.f;
   if (bad) o = make_float4(nan, nan, nan, nan);
@@ -1434,18 +1656,20 @@ __global__ void __launch_bounds__(256) kfa_cache_join_kernel(const AttendParams 
 // The same for the kernel for more rows, whose parts lie by columns: a lane a row, a warp 16 columns of 32 rows, nothing exchanged. One pass:
 // what is there is scaled down when a part has a larger maximum. (16 trees of 64 tokens, 256 rows mostly in two parts: 102.9 us with parts by
 // rows and a warp a row, 96.4 with 8 lanes a row, 93.7 so.)
-template <bool BF16>
+template <bool BF16, int MODE = ATT_PLAIN>
 __global__ void __launch_bounds__(256) kfa_cache_join_rows_kernel(const AttendParams p) {
+  if (MODE == ATT_PREFIX) let_next_begin();  // (it waits for this kernel when it needs the carry)
   wait_for_previous();
-  let_next_begin();
+  if (MODE != ATT_PREFIX) let_next_begin();
   const int4 meta = p.part_meta[blockIdx.x];
   if (meta.x == 0) return;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = blockIdx.y * 32 + lane;
-  const RowMap rows(p, meta.z);
-  int h, t;
-  if (16 * warp >= p.c.cols || !rows.row(p, r, h, t)) return;
+  const RowMapOf<MODE> rows(p, meta.y, meta.z);
+  int h, t, sq;
+  if (16 * warp >= p.c.cols || !rows.row(p, r, h, t, sq)) return;
   const bool bad = *reinterpret_cast<const volatile int*>(p.status) != 0;
-  const int count = p.counts ? min(max(p.counts[meta.y], 0), p.T) : p.T;
+  const int count = MODE != ATT_PREFIX && p.counts ? min(max(p.counts[meta.y], 0), p.T) : p.T;
+  const long long row_at = (static_cast<long long>(sq) * p.H + h) * p.T + t;  // of the carry
   const float* ml = p.part_ml + (2ll * blockIdx.x + 1) * 3 * p.rows + r;  // the first part in slot 1 of its CTA, the others in slot 0 of theirs
   const float4* from = reinterpret_cast<const float4*>(p.part_o + ((2ll * blockIdx.x + 1) * p.rows + 32 * blockIdx.y) * 128) + 128 * warp + lane;
   float m = -INFINITY, top = -INFINITY, l = 0.f, o[16];
@@ -1470,6 +1694,38 @@ __global__ void __launch_bounds__(256) kfa_cache_join_rows_kernel(const AttendPa
 #pragma unroll
       for (int q = 0; q < 4; ++q) o[4 * k + q] = o[4 * k + q] * f + (fi < 0.f ? 0.f : y[q] * fi);
     }
+  }
+  if constexpr (MODE == ATT_PREFIX) {
+    float4* to = reinterpret_cast<float4*>(p.carry_o + row_at * 128 + 16 * warp);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) to[k] = make_float4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
+    if (warp == 0) {
+      p.carry_ml[row_at] = m;
+      p.carry_ml[p.carry_rows + row_at] = l;
+      p.carry_ml[2 * p.carry_rows + row_at] = top;
+    }
+    return;
+  }
+  if constexpr (MODE == ATT_OWN) {
+    Carry carry;
+    carry.load(p, meta.y, h, t);
+    const float m_new = fmaxf(m, carry.m), own = part_factor(m, l, m_new, p.c_log2), a = part_factor(carry.m, carry.l, m_new, p.c_log2);
+    const float a_own = own < 0.f ? 0.f : own;
+#pragma unroll
+    for (int k = 0; k < 16; ++k) o[k] *= a_own;
+    if (!(a < 0.f)) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float4 y = *reinterpret_cast<const float4*>(carry.o + 16 * warp + 4 * k);
+        o[4 * k] += a * y.x;
+        o[4 * k + 1] += a * y.y;
+        o[4 * k + 2] += a * y.z;
+        o[4 * k + 3] += a * y.w;
+      }
+    }
+    l = l * a_own + carry.l * a;
+    m = m_new;
+    top = fmaxf(top, carry.top);
   }
   const bool some = t < count && l != 0.f;
   const float nan = __int_as_float(0x7fc00000), inv = some ? 1.f / l : 0.f;

@@ -83,15 +83,15 @@ int check_dtype(int dtype) {
 }
 
 // 4-D tiled map over rows of D 16-bit columns: dims (D, n1, n2, n3) with element strides s1, s2, s3, boxes of 64 columns (128 bytes,
-// swizzled) x b1 x b2; what is out of range reads as zeros.
-int make_box_map(void* ptr, int64_t D, int64_t n1, int64_t s1, int64_t n2, int64_t s2, int64_t n3, int64_t s3, int b1, int b2, int dtype,
+// swizzled) x b1 x b2 x b3; what is out of range reads as zeros.
+int make_box_map(void* ptr, int64_t D, int64_t n1, int64_t s1, int64_t n2, int64_t s2, int64_t n3, int64_t s3, int b1, int b2, int b3, int dtype,
                  CUtensorMap* map, const char* name) {
   EncodeFn enc = encode_fn();
   if (!enc) return fail(KFA_ERR_CUDA, "cuTensorMapEncodeTiled not available from the driver");
   auto st = [&](int64_t n, int64_t s) { return static_cast<cuuint64_t>(n > 1 ? s : D) * 2; };  // (an extent of 1 never advances)
   const cuuint64_t dims[4] = {static_cast<cuuint64_t>(D), static_cast<cuuint64_t>(n1), static_cast<cuuint64_t>(n2), static_cast<cuuint64_t>(n3)};
   const cuuint64_t strides[3] = {st(n1, s1), st(n2, s2), st(n3, s3)};
-  const cuuint32_t box[4] = {64, static_cast<cuuint32_t>(b1), static_cast<cuuint32_t>(b2), 1}, one[4] = {1, 1, 1, 1};
+  const cuuint32_t box[4] = {64, static_cast<cuuint32_t>(b1), static_cast<cuuint32_t>(b2), static_cast<cuuint32_t>(b3)}, one[4] = {1, 1, 1, 1};
   const CUresult r = enc(map, dtype == KFA_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, ptr, dims, strides, box,
                          one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);

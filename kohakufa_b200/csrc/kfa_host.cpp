@@ -55,6 +55,8 @@ struct Api {
   decltype(&kfa_cache_evict_room) cache_evict = nullptr;
   decltype(&kfa_rotary) rotary = nullptr;
   decltype(&kfa_cache_append_rotary) cache_append_rotary = nullptr;
+  decltype(&kfa_cache_attend_shared_bytes) cache_attend_shared_bytes = nullptr;
+  decltype(&kfa_cache_attend_shared) cache_attend_shared = nullptr;
 } api;
 
 PyObject* g_error = nullptr;  // kohakufa_b200._lib.KfaError
@@ -754,20 +756,13 @@ KfaCache cache_desc(const Cache& c) {
   return d;
 }
 
-// cached_attention(q, k_pages, v_pages, lengths, table, k, v, tree, counts, scale, return_stats, status) -> out, or out and stats
-PyObject* py_cached_attention(Args a, Py_ssize_t n) {
-  need(n, 12);
-  const char* who = "attention_cached";
-  const at::Tensor q = tensor(a[0]), k = maybe(a[5]), v = maybe(a[6]), tree = maybe(a[7]), counts = maybe(a[8]), status = maybe(a[11]);
-  const Cache c = cache_of(a + 1);
-  const double scale = number(a[9]);
-  const bool with_stats = PyObject_IsTrue(a[10]);
-  check_no_grad(who, {&q, &c.k, &c.v, &k, &v});
+// New tokens beside a cache: q, and k, v and tree or not. Leaves the tree's strides.
+void check_tokens(const char* who, const Cache& c, const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& tree,
+                  const at::Tensor& counts, double scale, int64_t (&tree_stride)[3]) {
   check_cache(who, c);
   check_new(who, "q", c, q, 0);
   TORCH_CHECK_VALUE(k.defined() == v.defined(), who, ": give k and v, or neither");
   TORCH_CHECK_VALUE(!tree.defined() || k.defined(), who, ": tree shows new tokens to one another: it needs k and v");
-  int64_t tree_stride[3] = {0, 0, 0};
   if (k.defined()) {
     check_new(who, "k", c, k, c.k.size(1));
     check_new(who, "v", c, v, c.k.size(1));
@@ -784,6 +779,19 @@ PyObject* py_cached_attention(Args a, Py_ssize_t n) {
   }
   check_counts(who, c, counts);
   check_scale(who, scale);
+}
+
+// cached_attention(q, k_pages, v_pages, lengths, table, k, v, tree, counts, scale, return_stats, status) -> out, or out and stats
+PyObject* py_cached_attention(Args a, Py_ssize_t n) {
+  need(n, 12);
+  const char* who = "attention_cached";
+  const at::Tensor q = tensor(a[0]), k = maybe(a[5]), v = maybe(a[6]), tree = maybe(a[7]), counts = maybe(a[8]), status = maybe(a[11]);
+  const Cache c = cache_of(a + 1);
+  const double scale = number(a[9]);
+  const bool with_stats = PyObject_IsTrue(a[10]);
+  check_no_grad(who, {&q, &c.k, &c.v, &k, &v});
+  int64_t tree_stride[3] = {0, 0, 0};
+  check_tokens(who, c, q, k, v, tree, counts, scale, tree_stride);
   check_where(who, c, {&q, &k, &v, &tree, &counts, &status});
   auto [out, stats] = released([&] {
     const c10::cuda::CUDAGuard guard(q.device());
@@ -798,6 +806,48 @@ PyObject* py_cached_attention(Args a, Py_ssize_t n) {
                            counts.defined() ? counts.data_ptr<int32_t>() : nullptr, &dout, st.defined() ? st.data_ptr<float>() : nullptr,
                            bytes ? scratch.data_ptr() : nullptr, static_cast<float>(scale), dtype_code(q), status.data_ptr<int32_t>(),
                            stream_of(q)));
+    return Two{std::move(o), std::move(st)};
+  });
+  if (!with_stats) return THPVariable_Wrap(std::move(out));
+  return pack(Two{std::move(out), std::move(stats)});
+}
+
+// shared_attention(q, k_pages, v_pages, lengths, table of the prefixes, the same of the cache, starts, k, v, tree, counts, scale, return_stats,
+// status) -> out, or out and stats
+PyObject* py_shared_attention(Args a, Py_ssize_t n) {
+  need(n, 17);
+  const char* who = "attention_shared";
+  const at::Tensor q = tensor(a[0]), starts = maybe(a[9]), k = maybe(a[10]), v = maybe(a[11]), tree = maybe(a[12]), counts = maybe(a[13]),
+                   status = maybe(a[16]);
+  const Cache p = cache_of(a + 1), c = cache_of(a + 5);
+  const double scale = number(a[14]);
+  const bool with_stats = PyObject_IsTrue(a[15]);
+  check_no_grad(who, {&q, &p.k, &p.v, &c.k, &c.v, &k, &v});
+  int64_t tree_stride[3] = {0, 0, 0};
+  check_tokens(who, c, q, k, v, tree, counts, scale, tree_stride);
+  check_cache(who, p);
+  TORCH_CHECK_TYPE(p.k.scalar_type() == c.k.scalar_type(), who, ": prefix must have the cache's type");
+  TORCH_CHECK_VALUE(p.k.size(1) == c.k.size(1) && p.k.size(3) == c.k.size(3), who, ": prefix must have the cache's heads and head dim");
+  if (starts.defined()) {
+    TORCH_CHECK_TYPE(starts.scalar_type() == at::kInt, who, ": starts must be int32");
+    TORCH_CHECK_VALUE(starts.dim() == 1 && starts.is_contiguous() && starts.numel() == p.lengths.numel() + 1, who,
+                      ": starts must be a contiguous vector, one entry per prefix and one more");
+  } else {
+    TORCH_CHECK_VALUE(p.lengths.numel() == 1, who, ": several prefixes need starts");
+  }
+  check_where(who, c, {&p.k, &p.v, &p.lengths, &p.table, &starts, &q, &k, &v, &tree, &counts, &status});
+  auto [out, stats] = released([&] {
+    const c10::cuda::CUDAGuard guard(q.device());
+    at::Tensor o = bshd_like(q), st;
+    if (with_stats) st = floats(q, {q.size(0), q.size(1), 2, q.size(2)});
+    const KfaTensor4 dq = desc(q), dout = desc(o), dk = k.defined() ? desc(k) : KfaTensor4{}, dv = k.defined() ? desc(v) : KfaTensor4{};
+    const KfaCache dp = cache_desc(p), dc = cache_desc(c);
+    const KfaTensor4* new_k = k.defined() ? &dk : nullptr;
+    const at::Tensor scratch = floats(q, {(api.cache_attend_shared_bytes(&dq, &dp, &dc, new_k) + 3) / 4});
+    check(api.cache_attend_shared(&dq, &dp, starts.defined() ? starts.data_ptr<int32_t>() : nullptr, &dc, new_k, k.defined() ? &dv : nullptr,
+                                  tree.defined() ? static_cast<const uint8_t*>(tree.data_ptr()) : nullptr, tree_stride,
+                                  counts.defined() ? counts.data_ptr<int32_t>() : nullptr, &dout, st.defined() ? st.data_ptr<float>() : nullptr,
+                                  scratch.data_ptr(), static_cast<float>(scale), dtype_code(q), status.data_ptr<int32_t>(), stream_of(q)));
     return Two{std::move(o), std::move(st)};
   });
   if (!with_stats) return THPVariable_Wrap(std::move(out));
@@ -1184,6 +1234,8 @@ PyObject* py_bind(Args a, Py_ssize_t n) {
   take("kfa_cache_evict_room", api.cache_evict);
   take("kfa_rotary", api.rotary);
   take("kfa_cache_append_rotary", api.cache_append_rotary);
+  take("kfa_cache_attend_shared_bytes", api.cache_attend_shared_bytes);
+  take("kfa_cache_attend_shared", api.cache_attend_shared);
   Py_INCREF(a[0]);
   Py_XDECREF(g_error);
   g_error = a[0];
@@ -1232,6 +1284,7 @@ PyMethodDef methods[] = {
     KFA_METHOD(cache_evict),
     KFA_METHOD(rotary),
     KFA_METHOD(cache_append_rotary),
+    KFA_METHOD(shared_attention),
     {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_kfa_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
