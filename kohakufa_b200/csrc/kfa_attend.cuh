@@ -164,7 +164,7 @@ using Walk = WalkOf<ATT_PLAIN>;
 // Shares out the whole batch's work, counted(b) of it sequence b's (0 or more), equally: at[0] .. at[1] is this CTA's stretch, found(i, b, off,
 // counted(b)) is called by one thread for each of the two ends that lies inside sequence b, off into it. All threads of the CTA; s_i: 32 ints of
 // shared memory, of which the first 8 are found's. Returns the length of a stretch.
-template <typename F, typename G>
+template <int THREADS = ATT_THREADS, typename F, typename G>
 __device__ __forceinline__ int att_share(const AttendParams& p, int* s_i, F counted, int (&at)[2], int& total, G found) {
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   auto of = [&](int b) { return b < p.c.batch ? counted(b) : 0; };
@@ -176,30 +176,30 @@ __device__ __forceinline__ int att_share(const AttendParams& p, int* s_i, F coun
     }
     return x;
   };
-  // 384 sequences at a time; then the sequences in which this CTA's stretch begins and ends
+  // a sequence a thread at a time; then the sequences in which this CTA's stretch begins and ends
   total = 0;
   const int own0 = of(tid), scan0 = warp_scan(own0);
-  for (int b0 = 0; b0 < p.c.batch; b0 += ATT_THREADS) {
+  for (int b0 = 0; b0 < p.c.batch; b0 += THREADS) {
     const int s = b0 == 0 ? scan0 : warp_scan(of(b0 + tid));
     if (b0 > 0) __syncthreads();
     if (lane == 31) s_i[8 + warp] = s;
     __syncthreads();
-    for (int i = 0; i < ATT_THREADS / 32; ++i) total += s_i[8 + i];
+    for (int i = 0; i < THREADS / 32; ++i) total += s_i[8 + i];
   }
   const int chunk = max(static_cast<int>(p.by_grid.div(total + gridDim.x - 1)), p.least);
   at[0] = chunk * static_cast<int>(blockIdx.x);
   at[1] = at[0] + chunk;
   int before = 0;
-  for (int b0 = 0; b0 < p.c.batch; b0 += ATT_THREADS) {
+  for (int b0 = 0; b0 < p.c.batch; b0 += THREADS) {
     const int own = b0 == 0 ? own0 : of(b0 + tid);
     int upto = b0 == 0 ? scan0 : warp_scan(own);
-    if (p.c.batch > ATT_THREADS) {
+    if (p.c.batch > THREADS) {
       __syncthreads();
       if (lane == 31) s_i[8 + warp] = upto;
       __syncthreads();
     }
     int all = 0;
-    for (int i = 0; i < ATT_THREADS / 32; ++i) {
+    for (int i = 0; i < THREADS / 32; ++i) {
       const int x = s_i[8 + i];
       if (i < warp) upto += x;
       all += x;
@@ -216,7 +216,7 @@ __device__ __forceinline__ int att_share(const AttendParams& p, int* s_i, F coun
 
 // Which work is this CTA's (all its threads; s_i: 32 ints of shared memory). Synchronises the CTA. chunk, end: units per CTA and where this
 // one's stretch ends, both as they are counted.
-template <int MODE>
+template <int THREADS = ATT_THREADS, int MODE>
 __device__ __forceinline__ bool my_work(const AttendParams& p, int* s_i, WalkOf<MODE>& w, int& chunk, int& end) {
   chunk = end = 0;
   if (MODE != ATT_PREFIX && p.whole) {
@@ -233,7 +233,7 @@ __device__ __forceinline__ bool my_work(const AttendParams& p, int* s_i, WalkOf<
   }
   int at[2], total;
   using W = WalkOf<MODE>;
-  chunk = att_share(p, s_i, [&](int b) { return (W::units_of(p, b) + p.extra) * W::items_of(p, b); }, at, total, [&](int i, int b, int off, int own) {
+  chunk = att_share<THREADS>(p, s_i, [&](int b) { return (W::units_of(p, b) + p.extra) * W::items_of(p, b); }, at, total, [&](int i, int b, int off, int own) {
     const int each = own / W::items_of(p, b), item = off / each;
     s_i[3 * i] = b;
     s_i[3 * i + 1] = item;
@@ -285,29 +285,30 @@ __device__ __forceinline__ bool wait_warp(uint32_t bar, uint32_t parity, const C
 }
 
 // Shared memory and rings that both kernels lay out alike. NC: chunks of 64 columns of the head dim; Q_ROWS: rows of the query buffer;
-// BOTH: both streams see every tile (else they take turns); OTHER: bytes beside keys, values and queries.
-template <int NC_, int Q_ROWS_, int NQ_, bool BOTH_, int OTHER_>
+// BOTH: both streams see every tile (else they take turns); OTHER: bytes beside keys, values and queries; STREAMS: 1: half an SM, the CTA's only stream.
+template <int NC_, int Q_ROWS_, int NQ_, bool BOTH_, int OTHER_, int STREAMS_ = 2>
 struct AttRings {
-  static constexpr int NC = NC_, Q_ROWS = Q_ROWS_, NQ = NQ_;
-  static constexpr bool BOTH = BOTH_;
+  static constexpr int NC = NC_, Q_ROWS = Q_ROWS_, NQ = NQ_, STREAMS = STREAMS_;
+  static constexpr bool BOTH = BOTH_, ALL = BOTH_ || STREAMS_ == 1;  // ALL: a stream sees every tile
+  static constexpr int THREADS = STREAMS == 1 ? 256 : ATT_THREADS, ISSUE_WARP = 4 * STREAMS, LOAD_WARP = STREAMS == 1 ? 5 : 10;
   static constexpr int CHUNK = 128 * 64 * 2;  // 128 keys x 64 columns
   static constexpr int STAGE = NC * CHUNK;
   static constexpr int Q_CHUNK = Q_ROWS * 128, Q_BYTES = NC * Q_CHUNK;
   static constexpr int FIXED = 1024 + NQ * Q_BYTES + OTHER_;
-  static constexpr int FIT = (232448 - FIXED) / STAGE;
+  static constexpr int FIT = ((STREAMS == 1 ? 115712 : 232448) - FIXED) / STAGE;
   // Rings of key tiles and of value tiles, in turn for each stream (BOTH: one of each for both). A stage has one producer and the
   // same consumers every time: who waits for a phase of its barrier has waited for the one before, so that a parity means one phase.
-  static constexpr int RINGS = BOTH ? 1 : 2;
-  static constexpr int DEEP = FIT / RINGS, MOST = BOTH ? 4 : 2;
+  static constexpr int RINGS = ALL ? 1 : 2;
+  static constexpr int DEEP = FIT / RINGS, MOST = ALL ? 4 : 2;
   static constexpr int DV = DEEP / 2 < MOST ? DEEP / 2 : MOST;
   static constexpr int DK = DEEP - DV < MOST ? DEEP - DV : MOST;
   static_assert(DV >= 1 && DK >= 1, "no room for a tile of keys and one of values");
   static constexpr int NS = RINGS * (DK + DV);
   static constexpr int SMEM = FIXED + NS * STAGE;
-  __device__ static __forceinline__ int k_stage(int T) { return BOTH ? T % DK : (T & 1) * DK + (T >> 1) % DK; }
-  __device__ static __forceinline__ int v_stage(int T) { return RINGS * DK + (BOTH ? T % DV : (T & 1) * DV + (T >> 1) % DV); }
-  __device__ static __forceinline__ int k_turn(int T) { return (BOTH ? T : T >> 1) / DK; }
-  __device__ static __forceinline__ int v_turn(int T) { return (BOTH ? T : T >> 1) / DV; }
+  __device__ static __forceinline__ int k_stage(int T) { return ALL ? T % DK : (T & 1) * DK + (T >> 1) % DK; }
+  __device__ static __forceinline__ int v_stage(int T) { return RINGS * DK + (ALL ? T % DV : (T & 1) * DV + (T >> 1) % DV); }
+  __device__ static __forceinline__ int k_turn(int T) { return (ALL ? T : T >> 1) / DK; }
+  __device__ static __forceinline__ int v_turn(int T) { return (ALL ? T : T >> 1) / DV; }
   // barriers: tiles there and free, queries there, scores there, P there, P V done, a segment is finished, a stream's O has been read (in the
   // segments in which the stream had tiles), all done
   static constexpr int B_KV = 0, B_KVFREE = NS, B_Q = 2 * NS, B_S = B_Q + NQ, B_P = B_S + 4, B_PV = B_P + 4, B_QFREE = B_PV + 4,
@@ -476,32 +477,32 @@ template <class R, int MODE>
 __device__ __forceinline__ bool att_setup(const AttendParams& p, uint32_t bar0, const AttCtl& ctl, int tmem_cols, WalkOf<MODE>& first, int& chunk,
                                           int& end) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (warp == 10) {
+  if (warp == R::LOAD_WARP) {
     for (int i = lane; i < R::N_BARS; i += 32) {
       int count = 1;
       if (i >= R::B_KVFREE && i < R::B_Q) count = R::BOTH ? 2 : 1;
       if (i >= R::B_P && i < R::B_PV) count = 128;
-      if (i >= R::B_QFREE && i < R::B_OFREE) count = R::BOTH ? 2 : 256;
-      if (i >= R::B_OFREE && i < R::B_DRAIN) count = R::BOTH ? 128 : 256;
+      if (i >= R::B_QFREE && i < R::B_OFREE) count = R::BOTH ? 2 : 128 * R::STREAMS;
+      if (i >= R::B_OFREE && i < R::B_DRAIN) count = R::BOTH ? 128 : 128 * R::STREAMS;
       mbar_init(bar0 + 8u * i, count);
     }
     if (lane == 0) *ctl.abort = ctl.odd[0] = ctl.odd[1] = 0;
     fence_mbar_init();
     fence_async_smem();
   }
-  if (warp == 8) {
+  if (warp == R::ISSUE_WARP) {
     tmem_alloc(smem_u32(ctl.tmem), tmem_cols);
     tmem_relinquish();
   }
   // (ATT_OWN: what is before the prefixes' kernel has ended, that one's CTAs have waited for it before they let others begin.)
   if (MODE != ATT_OWN) wait_for_previous();
-  if (warp == 10 && lane == 0) *ctl.bad = load_status(p.status) != 0;
+  if (warp == R::LOAD_WARP && lane == 0) *ctl.bad = load_status(p.status) != 0;
   if (MODE == ATT_PREFIX && p.starts && blockIdx.x == 0) {
-    for (int i = threadIdx.x; i <= p.groups; i += ATT_THREADS)
+    for (int i = threadIdx.x; i <= p.groups; i += R::THREADS)
       if (p.starts[i] < 0 || p.starts[i] > p.seqs || (i > 0 && p.starts[i] < p.starts[i - 1])) report(p.status, DEV_BAD_CACHE);
   }
   tc_fence_before();
-  const bool work = my_work(p, ctl.ints, first, chunk, end);
+  const bool work = my_work<R::THREADS>(p, ctl.ints, first, chunk, end);
   let_next_begin();
   tc_fence_after();
   return work;
@@ -579,7 +580,7 @@ struct AttTile {
   bool opens;  // the stream's first tile of segment s
   bool closes; // the segment's last tile
 };
-template <bool BOTH, class W = Walk>
+template <bool ALL, class W = Walk>
 struct AttTiles {
   W w;
   int st, at = 0, T = 0, s = 0, uses = 0;
@@ -589,7 +590,7 @@ struct AttTiles {
       while (at < w.tiles()) {
         ++at;
         const int now = T++;
-        if (BOTH || (now & 1) == st) {
+        if (ALL || (now & 1) == st) {
           t = {now, s, uses, opens, at == w.tiles()};
           opens = false;
           return true;
@@ -612,7 +613,7 @@ struct AttTiles {
 template <class R, int PIECES, int NP, class W, typename FS, typename FP>
 __device__ __forceinline__ void att_issue(const AttendParams& p, const W& first, int st, uint32_t bar0, const AttCtl& ac, FS issue_S, FP issue_PV) {
   auto ready = [&](int i, uint32_t parity) { return __all_sync(0xffffffffu, mbar_test(bar0 + 8u * i, parity)); };
-  AttTiles<R::BOTH, W> tiles{first, st};
+  AttTiles<R::ALL, W> tiles{first, st};
   AttTile ahead = {0, 0, 0, false, false}, even = ahead, odd = ahead;  // the next to get scores; those that have, by c (at most two wait for values)
   bool have = tiles.take(p, ahead);
   int i_s = 0, i_p = 0;  // pieces of scores and of values issued
@@ -769,10 +770,11 @@ __device__ __forceinline__ void att_give_up(const AttendParams& p, const WalkOf<
                                             int q_issued) {
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) report_abort(ac.abort, p.status);
-  if (warp >= 10 && lane == 0) {
+  if ((warp == R::LOAD_WARP || warp == R::LOAD_WARP + 1) && lane == 0) {
+    const bool keys = warp == R::LOAD_WARP;
     for (int s = max(q_issued - R::NQ, 0); s < q_issued; ++s) mbar_drain(bar0 + 8u * (R::B_Q + s % R::NQ), (s / R::NQ) & 1);
-    for (int T = max(kv_issued - R::RINGS * (warp == 10 ? R::DK : R::DV), 0); T < kv_issued; ++T)
-      mbar_drain(bar0 + 8u * (R::B_KV + (warp == 10 ? R::k_stage(T) : R::v_stage(T))), (warp == 10 ? R::k_turn(T) : R::v_turn(T)) & 1);
+    for (int T = max(kv_issued - R::RINGS * (keys ? R::DK : R::DV), 0); T < kv_issued; ++T)
+      mbar_drain(bar0 + 8u * (R::B_KV + (keys ? R::k_stage(T) : R::v_stage(T))), (keys ? R::k_turn(T) : R::v_turn(T)) & 1);
   }
   if (MODE == ATT_PREFIX) return;  // (the carry is not used then: the kernel behind this one sees the status word)
   WalkOf<MODE> w = first;
@@ -781,7 +783,7 @@ __device__ __forceinline__ void att_give_up(const AttendParams& p, const WalkOf<
     if (w.begins() && w.ends()) {
       const RowMapOf<MODE> rows(p, w.b, w.item);
       const int pieces = p.c.cols / 8;
-      for (int i = tid; i < p.gt * p.tt * pieces; i += ATT_THREADS) {
+      for (int i = tid; i < p.gt * p.tt * pieces; i += R::THREADS) {
         int h, t;
         if (!rows.row(p, i / pieces, h, t)) continue;
         *reinterpret_cast<uint4*>(p.o + w.b * p.o_sb + h * p.o_sh + t * p.o_ss + 16 * (i % pieces)) =
@@ -805,26 +807,34 @@ __device__ __forceinline__ void note_parts(const AttendParams& p, const W& w, bo
 }
 
 // ---- up to 64 rows --------------------------------------------------------------------------------------------------------
-template <int NC, int N>
-struct AttCfg : AttRings<NC, N, 2, false, 2 * (N <= 32 ? 2 : 1) * 128 * N * 2 + 1024 + 16 * N * 4 + 8 * N * 4 + 24 * N * 4> {
-  static constexpr int NP = N <= 32 ? 2 : 1;  // buffers for P per stream (each with barriers of its own: a stream may be a buffer ahead)
+// STREAMS = 1: a CTA takes half an SM and has one stream, and an item's end and the next one's beginning, which have little to
+// do, pass while the SM's other CTA works.
+template <int N, int STREAMS>
+constexpr int att_p_buffers() { return STREAMS == 1 ? 1 : (N <= 32 ? 2 : 1); }
+template <int NC, int N, int STREAMS = 2>
+struct AttCfg : AttRings<NC, N, 2, false,
+                         STREAMS * att_p_buffers<N, STREAMS>() * 128 * N * 2 + 1024 + 16 * N * 4 + 8 * N * 4 + 24 * N * 4, STREAMS> {
+  static constexpr int NP = att_p_buffers<N, STREAMS>();  // buffers for P per stream (each with barriers of its own: a stream may be a buffer ahead)
   static constexpr int P_BYTES = 128 * N * 2;
-  static constexpr int TMEM = N == 64 ? 512 : (N == 32 ? 256 : 128);  // 6 N columns: S 2 x 2, O 2
+  static constexpr int TMEM = (N == 64 ? 512 : (N == 32 ? 256 : 128)) * STREAMS / 2;  // 3 N columns a stream: S 2, O
+  static_assert(STREAMS == 2 || N <= 32, "half an SM has registers for 32 columns");
 };
+constexpr int ATT_HALF_REGS = 128, ATT_HALF_REGS_STREAM = 176, ATT_HALF_REGS_ISSUE = 80;  // of a CTA of 256 threads, see ATT_REGS
+static_assert(128 * (ATT_HALF_REGS_STREAM + ATT_HALF_REGS_ISSUE) <= 256 * ATT_HALF_REGS, "register budgets exceed the CTA's allocation");
 
-template <int NC, int N, bool BF16, int MODE = ATT_PLAIN>
-__global__ void __launch_bounds__(ATT_THREADS, 1)
+template <int NC, int N, bool BF16, int MODE = ATT_PLAIN, int STREAMS = 2>
+__global__ void __launch_bounds__(STREAMS == 1 ? 256 : ATT_THREADS, STREAMS == 1 ? 2 : 1)
 kfa_cache_attend_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                         const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmKn,
                         const __grid_constant__ CUtensorMap tmVn, const AttendParams p) {
-  using R = AttCfg<NC, N>;
+  using R = AttCfg<NC, N, STREAMS>;
   constexpr int NP = R::NP;
 
   extern __shared__ uint8_t smem_raw[];
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* smem = smem_raw + (base - smem_u32(smem_raw));
   const uint32_t sKV = base, sQ = sKV + R::NS * R::STAGE, sP = sQ + R::NQ * R::Q_BYTES;
-  uint8_t* small = smem + R::NS * R::STAGE + R::NQ * R::Q_BYTES + 2 * NP * R::P_BYTES;
+  uint8_t* small = smem + R::NS * R::STAGE + R::NQ * R::Q_BYTES + STREAMS * NP * R::P_BYTES;
   uint64_t* bars = reinterpret_cast<uint64_t*>(small);
   float* s_max = reinterpret_cast<float*>(small + 1024);  // [stream][tile & 1][warp][N]
   float* s_shift = s_max + 16 * N;                        // [warp][N]
@@ -833,7 +843,7 @@ kfa_cache_attend_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
   const uint32_t bar0 = smem_u32(bars);
   auto bar = [&](int i) { return bar0 + 8u * i; };
   const int tid = threadIdx.x, warp = warp_index(), lane = tid & 31;
-  if (tid == 32 * 11) {
+  if (tid == 32 * R::LOAD_WARP + 32) {
     for (const CUtensorMap* map : {&tmQ, &tmK, &tmV, &tmKn, &tmVn}) asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
   }
   WalkOf<MODE> first;
@@ -841,18 +851,21 @@ kfa_cache_attend_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
   const bool work = att_setup<R>(p, bar0, ac, R::TMEM, first, chunk, end);
   const uint32_t tmem = *ac.tmem;
   const Ctl ctl{ac.abort};
-  const uint32_t tmS = tmem, tmO = tmem + 4 * N;
+  const uint32_t tmS = tmem, tmO = tmem + 2 * STREAMS * N;
   int kv_issued = 0, q_issued = 0;
 
   if (!work) {
     if (tid == 0 && (MODE == ATT_PREFIX || !p.whole)) note_parts(p, first, false, 1, 0);
-  } else if (warp >= 10) {
-    if constexpr (N == 64) reg_budget<ATT_REGS_ISSUE, ATT_REGS>();
-    const bool values = warp == 11;
-    att_produce<R>(p, first, values, sKV, sQ, bar0, ac, &tmQ, values ? &tmV : &tmK, values ? &tmVn : &tmKn, kv_issued, q_issued);
-  } else if (warp >= 8) {
-    if constexpr (N == 64) reg_budget<ATT_REGS_ISSUE, ATT_REGS>();
-    const int st = warp - 8;
+  } else if (warp >= R::LOAD_WARP) {
+    if constexpr (STREAMS == 1) reg_budget<ATT_HALF_REGS_ISSUE, ATT_HALF_REGS>();
+    else if constexpr (N == 64) reg_budget<ATT_REGS_ISSUE, ATT_REGS>();
+    const bool values = warp == R::LOAD_WARP + 1;
+    if (STREAMS == 2 || warp <= R::LOAD_WARP + 1)
+      att_produce<R>(p, first, values, sKV, sQ, bar0, ac, &tmQ, values ? &tmV : &tmK, values ? &tmVn : &tmKn, kv_issued, q_issued);
+  } else if (warp >= R::ISSUE_WARP) {
+    if constexpr (STREAMS == 1) reg_budget<ATT_HALF_REGS_ISSUE, ATT_HALF_REGS>();
+    else if constexpr (N == 64) reg_budget<ATT_REGS_ISSUE, ATT_REGS>();
+    const int st = warp - R::ISSUE_WARP;
     const bool lead = elect_one();
     constexpr uint32_t IDESC_S = make_idesc(BF16, false, 128, N), IDESC_O = make_idesc(BF16, true, 128, N) | (1u << 15);
     constexpr uint32_t HI_P = sdesc_hi_for(N);
@@ -881,8 +894,9 @@ kfa_cache_attend_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
   } else {
     // =========================== softmax, output ===========================
     // (After a wait that ran out the role goes on without waiting: the warps of a stream meet at barriers.)
-    if constexpr (N == 64) reg_budget<ATT_REGS_STREAM, ATT_REGS>();
-    const int st = warp >> 2, wl = warp & 3, key = tid & 127;
+    if constexpr (STREAMS == 1) reg_budget<ATT_HALF_REGS_STREAM, ATT_HALF_REGS>();
+    else if constexpr (N == 64) reg_budget<ATT_REGS_STREAM, ATT_REGS>();
+    const int st = STREAMS == 1 ? 0 : warp >> 2, wl = warp & 3, key = tid & 127;
     const uint32_t lane_base = static_cast<uint32_t>(wl * 32) << 16;
     constexpr int PER = N / 32 > 0 ? N / 32 : 1;  // columns whose maximum a lane keeps: lane, lane + 32
     float* shift = s_shift + warp * N;
@@ -902,7 +916,7 @@ kfa_cache_attend_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
       const int tiles = w.tiles();
       for (int t = 0; t < tiles; ++t) {
         const int T = T0 + t;
-        if ((T & 1) != st) continue;
+        if (!R::ALL && (T & 1) != st) continue;
         const int ub = w.unit + 4 * t;
         const bool full = 4 * t + 4 <= w.n && (ub + 4) * ATT_UNIT <= w.len && ub + 4 <= w.uc;
         int fresh = -1;
@@ -1041,7 +1055,7 @@ kfa_cache_attend_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
       }
       if (!opens && ok) ok = wait_warp(bar(R::B_PV + 2 * st + (c - 1) % NP), ((c - 1) / NP) & 1, ctl, 83);
       tc_fence_before();
-      named_sync<3, 256>();
+      named_sync<3, 128 * STREAMS>();
       tc_fence_after();
       const bool whole = w.begins() && w.ends();
       if (MODE == ATT_OWN && whole) wait_for_previous();  // the carry is there
@@ -1051,13 +1065,13 @@ kfa_cache_attend_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
       const bool odd = ac.odd[0] >= s + 1 || ac.odd[1] >= s + 1;
       const int j0 = max(w.unit - w.uc, 0) * ATT_UNIT, j1 = odd ? min((w.unit + w.n - w.uc) * ATT_UNIT, w.count) : 0;
       const int d = wl * 32 + lane;
-      constexpr int W = N / 2;  // columns of a thread
+      constexpr int W = N / STREAMS;  // columns of a thread
       const int c0 = st * W;
       // lane i (i < W): column i's factors and statistics
       const float* f0 = s_fin + (s & 1) * 12 * N + c0 + (lane & (W - 1));
       const float* f1 = f0 + 6 * N;
-      const float m0 = f0[4 * N], m1 = f1[4 * N], m = fmaxf(m0, m1), top = fmaxf(f0[5 * N], f1[5 * N]);
-      const float l0 = (f0[0] + f0[N]) + (f0[2 * N] + f0[3 * N]), l1 = (f1[0] + f1[N]) + (f1[2 * N] + f1[3 * N]);
+      const float m0 = f0[4 * N], m1 = STREAMS == 1 ? -INFINITY : f1[4 * N], m = fmaxf(m0, m1), top = STREAMS == 1 ? f0[5 * N] : fmaxf(f0[5 * N], f1[5 * N]);
+      const float l0 = (f0[0] + f0[N]) + (f0[2 * N] + f0[3 * N]), l1 = STREAMS == 1 ? 0.f : (f1[0] + f1[N]) + (f1[2 * N] + f1[3 * N]);
       float a0 = part_factor(m0, l0, m, c_log2), a1 = part_factor(m1, l1, m, c_log2);
       float l_all = l0 * a0 + l1 * a1, m_all = m, top_all = top, ac_carry = -1.f;
       int h, tk, sq;
@@ -1102,12 +1116,13 @@ kfa_cache_attend_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
       }
       float o0[W], o1[W];
       tmem_ld_cols<W>(tmO + lane_base + c0, o0);
-      tmem_ld_cols<W>(tmO + lane_base + N + c0, o1);
+      if constexpr (STREAMS == 2) tmem_ld_cols<W>(tmO + lane_base + N + c0, o1);
       tmem_wait_ld();
 #pragma unroll
       for (int i = 0; i < W; ++i) {
         const float x0 = __shfl_sync(0xffffffffu, a0, i), x1 = __shfl_sync(0xffffffffu, a1, i);
-        o0[i] = (x0 < 0.f ? 0.f : o0[i] * x0) + (x1 < 0.f ? 0.f : o1[i] * x1);  // (a stream without tiles has left nothing there)
+        o0[i] = x0 < 0.f ? 0.f : o0[i] * x0;  // (a stream without tiles has left nothing there)
+        if constexpr (STREAMS == 2) o0[i] += x1 < 0.f ? 0.f : o1[i] * x1;
       }
       if (d < p.c.cols) {
         for (int j = j0; j < j1; ++j) {
@@ -1147,8 +1162,8 @@ kfa_cache_attend_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
           if (c0 + i < tile_rows<MODE>(p)) p.part_o[(slot * p.rows + c0 + i) * 128 + d] = o0[i];
       }
       tc_fence_before();
-      if (tiles > 1 || ((T0 - 1) & 1) == 0) mbar_arrive(bar(R::B_OFREE));
-      if (tiles > 1 || ((T0 - 1) & 1) == 1) mbar_arrive(bar(R::B_OFREE + 1));
+      if (R::ALL || tiles > 1 || ((T0 - 1) & 1) == 0) mbar_arrive(bar(R::B_OFREE));
+      if (!R::ALL && (tiles > 1 || ((T0 - 1) & 1) == 1)) mbar_arrive(bar(R::B_OFREE + 1));
       mbar_arrive(bar(R::B_QFREE + s % R::NQ));
       ++s;
       more = w.next(p);
@@ -1162,7 +1177,7 @@ kfa_cache_attend_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
   __syncthreads();
   if (tid == 0 && *ac.bad) report(p.status, DEV_BAD_CACHE);
   if (*ac.abort) att_give_up<R>(p, first, work, bar0, ac, kv_issued, q_issued);
-  if (warp == 8) {
+  if (warp == R::ISSUE_WARP) {
     tc_fence_after();
     tmem_dealloc(tmem, R::TMEM);
   }

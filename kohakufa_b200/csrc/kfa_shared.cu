@@ -39,7 +39,7 @@ int64_t kfa_cache_attend_shared_bytes(const KfaTensor4* q, const KfaCache* prefi
     return 0;  // (refused by the call)
   int ts;
   const AttendPlan a = plan_prefix(batch, q->shape[1], kv_heads, q->shape[2], prefix->batch, prefix->table ? prefix->table_cols * page : page, &ts);
-  const AttendPlan o = plan_attend(batch, q->shape[1], kv_heads, q->shape[2], cache->table ? cache->table_cols * own : own, k != nullptr);
+  const AttendPlan o = plan_attend(batch, q->shape[1], kv_heads, q->shape[2], cache->table ? cache->table_cols * own : own, k != nullptr, true);
   return padded(a.bytes) + padded(12 * batch * q->shape[1] * q->shape[2]) + 512 * batch * q->shape[1] * q->shape[2] + o.bytes;
 }
 
@@ -61,7 +61,7 @@ int kfa_cache_attend_shared(const KfaTensor4* q, const KfaCache* prefix, const i
   if (plan.most_units > 0x3fffffff || rows > 0x7fffffff) return fail(KFA_ERR_ARG, "too many rows in one call");
   uint8_t* carry = static_cast<uint8_t*>(scratch) + padded(plan.bytes);
   uint8_t* behind = carry + padded(12 * rows) + 512 * rows;
-  if ((rc = prepare_attend(q, cache, k, v, tree, tree_stride, counts, out, stats, behind, scale, dtype, dev_status, o, own, mo))) return rc;
+  if ((rc = prepare_attend(q, cache, k, v, tree, tree_stride, counts, out, stats, behind, scale, dtype, dev_status, o, own, mo, true))) return rc;
   if (o.c.heads != p.c.heads || o.c.cols != p.c.cols) return fail(KFA_ERR_ARG, "prefix: heads or head dim differ from the cache's");
   p.H = o.H;
   p.T = o.T;
