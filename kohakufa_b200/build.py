@@ -34,7 +34,7 @@ SOURCES = {
     CSRC / "kfa_api.cu": SHARED
     + [CSRC / f"kfa_{part}.cuh" for part in ("fwd", "bwd", "bwd_fused", "selftest", "cp", "mask", "scores")],
     CSRC / "kfa_cache.cu": SHARED + CACHE + ATTEND + [CSRC / "kfa_cache.cuh", CSRC / "kfa_weigh.cuh"],
-    CSRC / "kfa_shared.cu": SHARED + CACHE + ATTEND,
+    CSRC / "kfa_shared.cu": SHARED + CACHE + ATTEND + [CSRC / "kfa_shared.cuh"],
     CSRC / "kfa_rotary.cu": SHARED + CACHE + [CSRC / "kfa_rotary.cuh"],
 }
 OBJECTS = CSRC / "build"

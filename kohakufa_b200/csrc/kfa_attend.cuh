@@ -25,12 +25,6 @@
 //                   (with more than 128 rows both see every tile, each with half of the rows)
 //   warps 8, 9      MMA issue for the two streams
 //   warps 10, 11    TMA producers: keys (and queries), values; a lane per box of up to 32 rows inside a page
-//
-// Sequences that go on from a shared prefix: the same kernels in two more modes. The softmax over (prefix, own keys) is that of two parts whose (O,
-// m, l) are joined. ATT_PREFIX walks the prefixes: a row tile's rows are those of several sequences (one after the other in the batch, tokens, heads), so that a
-// prefix is read once for up to 256 rows and K / V head; what comes out, fp32, is the carry: per row O before it is divided, m, l, the largest score.
-// ATT_OWN is the plain walk over the sequences' own keys, which at an item's end adds the carry as one more part. Its main loop needs nothing of the
-// kernels before it in the stream, so it waits for them only there: it runs while the prefixes' last CTAs and their join end.
 #pragma once
 
 #include "kfa_cache_view.cuh"
@@ -44,7 +38,7 @@ constexpr int ATT_UNIT = 32;  // keys: what work is counted in
 constexpr int ATT_REGS = 168, ATT_REGS_STREAM = 208, ATT_REGS_ISSUE = 88;
 static_assert(2 * 128 * ATT_REGS_STREAM + 128 * ATT_REGS_ISSUE <= ATT_THREADS * ATT_REGS, "register budgets exceed the CTA's allocation");
 
-enum { ATT_PLAIN = 0, ATT_PREFIX = 1, ATT_OWN = 2 };
+enum { ATT_PLAIN = 0, ATT_PREFIX = 1, ATT_OWN = 2 };  // (the last two: kfa_shared.cuh)
 
 struct AttendParams {
   CacheView c;
@@ -80,6 +74,7 @@ struct AttendParams {
   float* carry_o;     // [(sequence, head, token)][128]
   float* carry_ml;    // [3][(sequence, head, token)]: m, l, largest score
   long long carry_rows;
+  int2* dir;          // [(K / V head, row tile)][first sequence of the tile]: the half CTA in which the item begins, its parts (0: in the carry)
 };
 
 // The sequences that go on from prefix i: first and behind the last, inside the batch whatever `starts` says.
@@ -91,8 +86,6 @@ __device__ __forceinline__ void prefix_group(const AttendParams& p, int i, int& 
     s1 = min(max(p.starts[i + 1], s0), p.seqs);
   }
 }
-// Whether sequence b goes on from a prefix (an empty one counts).
-__device__ __forceinline__ bool has_prefix(const AttendParams& p, int b) { return !p.starts || (b >= p.starts[0] && b < p.starts[p.groups]); }
 
 // The stretch of work of a CTA, from (b, item, unit) to (end_b, end_item, end_unit), walked item by item; every role walks for itself.
 // (ATT_PREFIX: b is a prefix.)
@@ -155,7 +148,10 @@ struct WalkOf {
     cut();
     return true;
   }
-  __device__ __forceinline__ int tiles() const { return (n + 3) >> 2; }
+  template <int UNITS = 4>
+  __device__ __forceinline__ int tiles() const {
+    return (n + UNITS - 1) / UNITS;
+  }
   __device__ __forceinline__ bool begins() const { return unit == 0; }
   __device__ __forceinline__ bool ends() const { return unit + n == units; }
 };
@@ -164,7 +160,7 @@ using Walk = WalkOf<ATT_PLAIN>;
 // Shares out the whole batch's work, counted(b) of it sequence b's (0 or more), equally: at[0] .. at[1] is this CTA's stretch, found(i, b, off,
 // counted(b)) is called by one thread for each of the two ends that lies inside sequence b, off into it. All threads of the CTA; s_i: 32 ints of
 // shared memory, of which the first 8 are found's. Returns the length of a stretch.
-template <int THREADS = ATT_THREADS, typename F, typename G>
+template <typename F, typename G>
 __device__ __forceinline__ int att_share(const AttendParams& p, int* s_i, F counted, int (&at)[2], int& total, G found) {
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   auto of = [&](int b) { return b < p.c.batch ? counted(b) : 0; };
@@ -176,30 +172,30 @@ __device__ __forceinline__ int att_share(const AttendParams& p, int* s_i, F coun
     }
     return x;
   };
-  // a sequence a thread at a time; then the sequences in which this CTA's stretch begins and ends
+  // 384 sequences at a time; then the sequences in which this CTA's stretch begins and ends
   total = 0;
   const int own0 = of(tid), scan0 = warp_scan(own0);
-  for (int b0 = 0; b0 < p.c.batch; b0 += THREADS) {
+  for (int b0 = 0; b0 < p.c.batch; b0 += ATT_THREADS) {
     const int s = b0 == 0 ? scan0 : warp_scan(of(b0 + tid));
     if (b0 > 0) __syncthreads();
     if (lane == 31) s_i[8 + warp] = s;
     __syncthreads();
-    for (int i = 0; i < THREADS / 32; ++i) total += s_i[8 + i];
+    for (int i = 0; i < ATT_THREADS / 32; ++i) total += s_i[8 + i];
   }
   const int chunk = max(static_cast<int>(p.by_grid.div(total + gridDim.x - 1)), p.least);
   at[0] = chunk * static_cast<int>(blockIdx.x);
   at[1] = at[0] + chunk;
   int before = 0;
-  for (int b0 = 0; b0 < p.c.batch; b0 += THREADS) {
+  for (int b0 = 0; b0 < p.c.batch; b0 += ATT_THREADS) {
     const int own = b0 == 0 ? own0 : of(b0 + tid);
     int upto = b0 == 0 ? scan0 : warp_scan(own);
-    if (p.c.batch > THREADS) {
+    if (p.c.batch > ATT_THREADS) {
       __syncthreads();
       if (lane == 31) s_i[8 + warp] = upto;
       __syncthreads();
     }
     int all = 0;
-    for (int i = 0; i < THREADS / 32; ++i) {
+    for (int i = 0; i < ATT_THREADS / 32; ++i) {
       const int x = s_i[8 + i];
       if (i < warp) upto += x;
       all += x;
@@ -216,10 +212,9 @@ __device__ __forceinline__ int att_share(const AttendParams& p, int* s_i, F coun
 
 // Which work is this CTA's (all its threads; s_i: 32 ints of shared memory). Synchronises the CTA. chunk, end: units per CTA and where this
 // one's stretch ends, both as they are counted.
-template <int THREADS = ATT_THREADS, int MODE>
-__device__ __forceinline__ bool my_work(const AttendParams& p, int* s_i, WalkOf<MODE>& w, int& chunk, int& end) {
+__device__ __forceinline__ bool my_work(const AttendParams& p, int* s_i, Walk& w, int& chunk, int& end) {
   chunk = end = 0;
-  if (MODE != ATT_PREFIX && p.whole) {
+  if (p.whole) {
     const unsigned all = static_cast<unsigned>(p.c.batch) * p.items;
     const unsigned i0 = p.by_grid.div(static_cast<unsigned>(all)) * blockIdx.x + min(blockIdx.x, all - p.by_grid.div(all) * gridDim.x);
     const unsigned i1 = i0 + p.by_grid.div(all) + (blockIdx.x < all - p.by_grid.div(all) * gridDim.x ? 1 : 0);
@@ -232,9 +227,8 @@ __device__ __forceinline__ bool my_work(const AttendParams& p, int* s_i, WalkOf<
     return w.start(p);
   }
   int at[2], total;
-  using W = WalkOf<MODE>;
-  chunk = att_share<THREADS>(p, s_i, [&](int b) { return (W::units_of(p, b) + p.extra) * W::items_of(p, b); }, at, total, [&](int i, int b, int off, int own) {
-    const int each = own / W::items_of(p, b), item = off / each;
+  chunk = att_share(p, s_i, [&](int b) { return (Walk::units_of(p, b) + p.extra) * p.items; }, at, total, [&](int i, int b, int off, int own) {
+    const int each = own / p.items, item = off / each;
     s_i[3 * i] = b;
     s_i[3 * i + 1] = item;
     s_i[3 * i + 2] = max(off - item * each - p.extra, 0);
@@ -267,6 +261,13 @@ __device__ __forceinline__ bool mbar_suspend(uint32_t bar, uint32_t parity) {
     return ok != 0;
   }
 }
+// Suspended until the phase is over, or for about 100 ns.
+__device__ __forceinline__ void mbar_nap(uint32_t bar, uint32_t parity) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%0], %1, %2;\n\t}" ::"r"(bar), "r"(parity), "r"(100u)
+      : "memory");
+}
 __device__ __forceinline__ bool wait_warp(uint32_t bar, uint32_t parity, const Ctl& ctl, int site) {
   bool ok = mbar_suspend(bar, parity);
   if (__builtin_expect(__all_sync(0xffffffffu, ok), 1)) return true;
@@ -285,30 +286,31 @@ __device__ __forceinline__ bool wait_warp(uint32_t bar, uint32_t parity, const C
 }
 
 // Shared memory and rings that both kernels lay out alike. NC: chunks of 64 columns of the head dim; Q_ROWS: rows of the query buffer;
-// BOTH: both streams see every tile (else they take turns); OTHER: bytes beside keys, values and queries; STREAMS: 1: half an SM, the CTA's only stream.
-template <int NC_, int Q_ROWS_, int NQ_, bool BOTH_, int OTHER_, int STREAMS_ = 2>
+// BOTH: both streams see every tile (else they take turns); OTHER: bytes beside keys, values and queries.
+template <int NC_, int Q_ROWS_, int NQ_, bool BOTH_, int OTHER_>
 struct AttRings {
-  static constexpr int NC = NC_, Q_ROWS = Q_ROWS_, NQ = NQ_, STREAMS = STREAMS_;
-  static constexpr bool BOTH = BOTH_, ALL = BOTH_ || STREAMS_ == 1;  // ALL: a stream sees every tile
-  static constexpr int THREADS = STREAMS == 1 ? 256 : ATT_THREADS, ISSUE_WARP = 4 * STREAMS, LOAD_WARP = STREAMS == 1 ? 5 : 10;
+  static constexpr int NC = NC_, Q_ROWS = Q_ROWS_, NQ = NQ_;
+  static constexpr bool BOTH = BOTH_, ALL = BOTH_;  // ALL: a stream sees every tile
+  static constexpr bool SUSPEND = false;            // whether the issuing warps suspend where there is nothing to issue
+  static constexpr int UNITS = 4;                   // of a tile
   static constexpr int CHUNK = 128 * 64 * 2;  // 128 keys x 64 columns
   static constexpr int STAGE = NC * CHUNK;
   static constexpr int Q_CHUNK = Q_ROWS * 128, Q_BYTES = NC * Q_CHUNK;
   static constexpr int FIXED = 1024 + NQ * Q_BYTES + OTHER_;
-  static constexpr int FIT = ((STREAMS == 1 ? 115712 : 232448) - FIXED) / STAGE;
+  static constexpr int FIT = (232448 - FIXED) / STAGE;
   // Rings of key tiles and of value tiles, in turn for each stream (BOTH: one of each for both). A stage has one producer and the
   // same consumers every time: who waits for a phase of its barrier has waited for the one before, so that a parity means one phase.
-  static constexpr int RINGS = ALL ? 1 : 2;
-  static constexpr int DEEP = FIT / RINGS, MOST = ALL ? 4 : 2;
+  static constexpr int RINGS = BOTH ? 1 : 2;
+  static constexpr int DEEP = FIT / RINGS, MOST = BOTH ? 4 : 2;
   static constexpr int DV = DEEP / 2 < MOST ? DEEP / 2 : MOST;
   static constexpr int DK = DEEP - DV < MOST ? DEEP - DV : MOST;
   static_assert(DV >= 1 && DK >= 1, "no room for a tile of keys and one of values");
   static constexpr int NS = RINGS * (DK + DV);
   static constexpr int SMEM = FIXED + NS * STAGE;
-  __device__ static __forceinline__ int k_stage(int T) { return ALL ? T % DK : (T & 1) * DK + (T >> 1) % DK; }
-  __device__ static __forceinline__ int v_stage(int T) { return RINGS * DK + (ALL ? T % DV : (T & 1) * DV + (T >> 1) % DV); }
-  __device__ static __forceinline__ int k_turn(int T) { return (ALL ? T : T >> 1) / DK; }
-  __device__ static __forceinline__ int v_turn(int T) { return (ALL ? T : T >> 1) / DV; }
+  __device__ static __forceinline__ int k_stage(int T) { return BOTH ? T % DK : (T & 1) * DK + (T >> 1) % DK; }
+  __device__ static __forceinline__ int v_stage(int T) { return RINGS * DK + (BOTH ? T % DV : (T & 1) * DV + (T >> 1) % DV); }
+  __device__ static __forceinline__ int k_turn(int T) { return (BOTH ? T : T >> 1) / DK; }
+  __device__ static __forceinline__ int v_turn(int T) { return (BOTH ? T : T >> 1) / DV; }
   // barriers: tiles there and free, queries there, scores there, P there, P V done, a segment is finished, a stream's O has been read (in the
   // segments in which the stream had tiles), all done
   static constexpr int B_KV = 0, B_KVFREE = NS, B_Q = 2 * NS, B_S = B_Q + NQ, B_P = B_S + 4, B_PV = B_P + 4, B_QFREE = B_PV + 4,
@@ -398,8 +400,8 @@ template <int MODE>
 struct RowMapOf {
   int g, h0, heads, t0;  // K / V head; first head, heads that exist, first token
   int s0, s1;            // first sequence, behind the last of the group (else the sequence)
+  int rt;                // row tile of the K / V head
   __device__ __forceinline__ RowMapOf(const AttendParams& p, int b, int item) {
-    int rt;
     s0 = b;
     s1 = b + 1;
     if constexpr (MODE == ATT_PREFIX) {  // items of a K / V head one after the other: CTAs that run together read the same keys
@@ -437,25 +439,12 @@ struct RowMapOf {
     return in && dt < p.tt && dh < heads && t < p.T;
   }
 };
+using RowMap = RowMapOf<ATT_PLAIN>;
 // Rows of a tile that may exist.
 template <int MODE>
 __device__ __forceinline__ int tile_rows(const AttendParams& p) {
   return MODE == ATT_PREFIX ? p.gt * p.tt * p.ts : p.gt * p.tt;
 }
-
-// What the prefixes have left of a row (ATT_OWN), behind the wait for their kernels. m = -inf, l = 0: nothing.
-struct Carry {
-  float m = -INFINITY, l = 0.f, top = -INFINITY;
-  const float* o = nullptr;
-  __device__ __forceinline__ void load(const AttendParams& p, int b, int h, int t) {
-    if (!has_prefix(p, b)) return;
-    const long long at = (static_cast<long long>(b) * p.H + h) * p.T + t;
-    m = p.carry_ml[at];
-    l = p.carry_ml[p.carry_rows + at];
-    top = p.carry_ml[2 * p.carry_rows + at];
-    o = p.carry_o + at * 128;
-  }
-};
 
 // Control block of a CTA behind its barriers.
 struct AttCtl {
@@ -473,36 +462,31 @@ struct AttCtl {
 };
 
 // Both kernels' beginning: barriers, tensor memory, the CTA's work.
-template <class R, int MODE>
-__device__ __forceinline__ bool att_setup(const AttendParams& p, uint32_t bar0, const AttCtl& ctl, int tmem_cols, WalkOf<MODE>& first, int& chunk,
+template <class R>
+__device__ __forceinline__ bool att_setup(const AttendParams& p, uint32_t bar0, const AttCtl& ctl, int tmem_cols, Walk& first, int& chunk,
                                           int& end) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (warp == R::LOAD_WARP) {
+  if (warp == 10) {
     for (int i = lane; i < R::N_BARS; i += 32) {
       int count = 1;
       if (i >= R::B_KVFREE && i < R::B_Q) count = R::BOTH ? 2 : 1;
       if (i >= R::B_P && i < R::B_PV) count = 128;
-      if (i >= R::B_QFREE && i < R::B_OFREE) count = R::BOTH ? 2 : 128 * R::STREAMS;
-      if (i >= R::B_OFREE && i < R::B_DRAIN) count = R::BOTH ? 128 : 128 * R::STREAMS;
+      if (i >= R::B_QFREE && i < R::B_OFREE) count = R::BOTH ? 2 : 256;
+      if (i >= R::B_OFREE && i < R::B_DRAIN) count = R::BOTH ? 128 : 256;
       mbar_init(bar0 + 8u * i, count);
     }
     if (lane == 0) *ctl.abort = ctl.odd[0] = ctl.odd[1] = 0;
     fence_mbar_init();
     fence_async_smem();
   }
-  if (warp == R::ISSUE_WARP) {
+  if (warp == 8) {
     tmem_alloc(smem_u32(ctl.tmem), tmem_cols);
     tmem_relinquish();
   }
-  // (ATT_OWN: what is before the prefixes' kernel has ended, that one's CTAs have waited for it before they let others begin.)
-  if (MODE != ATT_OWN) wait_for_previous();
-  if (warp == R::LOAD_WARP && lane == 0) *ctl.bad = load_status(p.status) != 0;
-  if (MODE == ATT_PREFIX && p.starts && blockIdx.x == 0) {
-    for (int i = threadIdx.x; i <= p.groups; i += R::THREADS)
-      if (p.starts[i] < 0 || p.starts[i] > p.seqs || (i > 0 && p.starts[i] < p.starts[i - 1])) report(p.status, DEV_BAD_CACHE);
-  }
+  wait_for_previous();
+  if (warp == 10 && lane == 0) *ctl.bad = load_status(p.status) != 0;
   tc_fence_before();
-  const bool work = my_work<R::THREADS>(p, ctl.ints, first, chunk, end);
+  const bool work = my_work(p, ctl.ints, first, chunk, end);
   let_next_begin();
   tc_fence_after();
   return work;
@@ -517,7 +501,7 @@ __device__ __forceinline__ void att_produce(const AttendParams& p, const WalkOf<
   const Ctl ctl{ac.abort};
   auto bar = [&](int i) { return bar0 + 8u * i; };
   WalkOf<MODE> w = first;
-  const int per_unit = ATT_UNIT / p.box, boxes = 4 * per_unit;
+  const int per_unit = ATT_UNIT / p.box, boxes = R::UNITS * per_unit;
   bool ok = true, more = true;
   int T = 0, s = 0;  // tiles and segments so far
   while (more && ok) {
@@ -535,10 +519,10 @@ __device__ __forceinline__ void att_produce(const AttendParams& p, const WalkOf<
       }
       q_issued = s + 1;
     }
-    const int tiles = w.tiles();
+    const int tiles = w.template tiles<R::UNITS>();
     for (int t = 0; t < tiles && ok; ++t, ++T) {
       // this lane's box
-      const int in_unit = (lane % per_unit) * p.box, unit = w.unit + 4 * t + lane / per_unit;
+      const int in_unit = (lane % per_unit) * p.box, unit = w.unit + R::UNITS * t + lane / per_unit;
       const bool mine = lane < boxes && unit < w.unit + w.n;
       const int row = (lane / per_unit) * ATT_UNIT + in_unit;
       int c1 = 0, c3 = w.b, kind = 0;  // 1: cached rows, 2: new ones
@@ -580,18 +564,19 @@ struct AttTile {
   bool opens;  // the stream's first tile of segment s
   bool closes; // the segment's last tile
 };
-template <bool ALL, class W = Walk>
+template <bool ALL, int UNITS = 4, class W = Walk>
 struct AttTiles {
   W w;
   int st, at = 0, T = 0, s = 0, uses = 0;
   bool more = true, opens = true;
   __device__ __forceinline__ bool take(const AttendParams& p, AttTile& t) {
     while (more) {
-      while (at < w.tiles()) {
+      const int tiles = w.template tiles<UNITS>();
+      while (at < tiles) {
         ++at;
         const int now = T++;
         if (ALL || (now & 1) == st) {
-          t = {now, s, uses, opens, at == w.tiles()};
+          t = {now, s, uses, opens, at == tiles};
           opens = false;
           return true;
         }
@@ -612,8 +597,13 @@ struct AttTiles {
 // issue_S(tile, c, piece), issue_PV(tile, c, piece) issue and commit; c counts the stream's tiles.
 template <class R, int PIECES, int NP, class W, typename FS, typename FP>
 __device__ __forceinline__ void att_issue(const AttendParams& p, const W& first, int st, uint32_t bar0, const AttCtl& ac, FS issue_S, FP issue_PV) {
-  auto ready = [&](int i, uint32_t parity) { return __all_sync(0xffffffffu, mbar_test(bar0 + 8u * i, parity)); };
-  AttTiles<R::ALL, W> tiles{first, st};
+  uint32_t held = 0, held_parity = 0;  // what the last test failed at
+  auto ready = [&](int i, uint32_t parity) {
+    const bool there = __all_sync(0xffffffffu, mbar_test(bar0 + 8u * i, parity));
+    if (R::SUSPEND && !there) held = bar0 + 8u * i, held_parity = parity;
+    return there;
+  };
+  AttTiles<R::ALL, R::UNITS, W> tiles{first, st};
   AttTile ahead = {0, 0, 0, false, false}, even = ahead, odd = ahead;  // the next to get scores; those that have, by c (at most two wait for values)
   bool have = tiles.take(p, ahead);
   int i_s = 0, i_p = 0;  // pieces of scores and of values issued
@@ -658,6 +648,8 @@ __device__ __forceinline__ void att_issue(const AttendParams& p, const W& first,
     } else if (clock64() - t0 > KFA_WAIT_CYCLES) {
       *ac.abort = KFA_DEV_TIMEOUT_BASE + 73;
       break;
+    } else if (R::SUSPEND) {  // (a warp that polls takes issue slots from those that compute)
+      mbar_nap(held, held_parity);
     }
   }
   // what was issued has retired before tensor memory is freed
@@ -708,8 +700,8 @@ __device__ __forceinline__ bool odd_half(uint32_t x) {  // all exponent bits: in
   constexpr uint32_t E = BF16 ? 0x7f80u : 0x7c00u;
   return (x & E) == E;
 }
-template <bool BF16, class W>
-__device__ __forceinline__ uint32_t odd_values(const AttendParams& p, const W& w, int g, int fresh) {
+template <bool BF16>
+__device__ __forceinline__ uint32_t odd_values(const AttendParams& p, const Walk& w, int g, int fresh) {
   if (fresh < 0) return 0u;
   const uint8_t* row = p.v + w.b * p.v_sb + g * p.v_sh + fresh * p.v_ss;
   uint32_t found = 0;
@@ -722,8 +714,8 @@ __device__ __forceinline__ uint32_t odd_values(const AttendParams& p, const W& w
   }
   return found;
 }
-template <int NC, bool BF16, class W>
-__device__ __forceinline__ void clean_values(const AttendParams& p, const W& w, int g, uint32_t stage, int key, bool valid, int fresh, uint32_t odd) {
+template <int NC, bool BF16>
+__device__ __forceinline__ void clean_values(const AttendParams& p, const Walk& w, int g, uint32_t stage, int key, bool valid, int fresh, uint32_t odd) {
   const uint32_t row = stage + key * 128;
   if (!valid) {
 #pragma unroll
@@ -765,25 +757,23 @@ __device__ __forceinline__ bool sees_new(const AttendParams& p, const W& w, int 
 
 // After a wait that ran out: the copies that the producers have started land, and the rows of what the CTA had whole read as NaN (what
 // was cut, the joining kernel sees to). All threads, behind a barrier.
-template <class R, int MODE>
-__device__ __forceinline__ void att_give_up(const AttendParams& p, const WalkOf<MODE>& first, bool work, uint32_t bar0, const AttCtl& ac, int kv_issued,
+template <class R>
+__device__ __forceinline__ void att_give_up(const AttendParams& p, const Walk& first, bool work, uint32_t bar0, const AttCtl& ac, int kv_issued,
                                             int q_issued) {
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) report_abort(ac.abort, p.status);
-  if ((warp == R::LOAD_WARP || warp == R::LOAD_WARP + 1) && lane == 0) {
-    const bool keys = warp == R::LOAD_WARP;
+  if (warp >= 10 && lane == 0) {
     for (int s = max(q_issued - R::NQ, 0); s < q_issued; ++s) mbar_drain(bar0 + 8u * (R::B_Q + s % R::NQ), (s / R::NQ) & 1);
-    for (int T = max(kv_issued - R::RINGS * (keys ? R::DK : R::DV), 0); T < kv_issued; ++T)
-      mbar_drain(bar0 + 8u * (R::B_KV + (keys ? R::k_stage(T) : R::v_stage(T))), (keys ? R::k_turn(T) : R::v_turn(T)) & 1);
+    for (int T = max(kv_issued - R::RINGS * (warp == 10 ? R::DK : R::DV), 0); T < kv_issued; ++T)
+      mbar_drain(bar0 + 8u * (R::B_KV + (warp == 10 ? R::k_stage(T) : R::v_stage(T))), (warp == 10 ? R::k_turn(T) : R::v_turn(T)) & 1);
   }
-  if (MODE == ATT_PREFIX) return;  // (the carry is not used then: the kernel behind this one sees the status word)
-  WalkOf<MODE> w = first;
+  Walk w = first;
   bool more = work;
   while (more) {
     if (w.begins() && w.ends()) {
-      const RowMapOf<MODE> rows(p, w.b, w.item);
+      const RowMap rows(p, w.b, w.item);
       const int pieces = p.c.cols / 8;
-      for (int i = tid; i < p.gt * p.tt * pieces; i += R::THREADS) {
+      for (int i = tid; i < p.gt * p.tt * pieces; i += ATT_THREADS) {
         int h, t;
         if (!rows.row(p, i / pieces, h, t)) continue;
         *reinterpret_cast<uint4*>(p.o + w.b * p.o_sb + h * p.o_sh + t * p.o_ss + 16 * (i % pieces)) =
@@ -799,42 +789,33 @@ __device__ __forceinline__ void att_give_up(const AttendParams& p, const WalkOf<
 }
 
 // What begins in this CTA and ends in another, for the joining kernel: only its last item can. w: the walk at its end.
-template <class W>
-__device__ __forceinline__ void note_parts(const AttendParams& p, const W& w, bool work, int chunk, int end) {
+__device__ __forceinline__ void note_parts(const AttendParams& p, const Walk& w, bool work, int chunk, int end) {
   int4 meta = make_int4(0, 0, 0, 0);
   if (work && w.begins() && !w.ends()) meta = make_int4((end - w.n + w.units - 1) / chunk - static_cast<int>(blockIdx.x) + 1, w.b, w.item, 0);
   p.part_meta[blockIdx.x] = meta;
 }
 
 // ---- up to 64 rows --------------------------------------------------------------------------------------------------------
-// STREAMS = 1: a CTA takes half an SM and has one stream, and an item's end and the next one's beginning, which have little to
-// do, pass while the SM's other CTA works.
-template <int N, int STREAMS>
-constexpr int att_p_buffers() { return STREAMS == 1 ? 1 : (N <= 32 ? 2 : 1); }
-template <int NC, int N, int STREAMS = 2>
-struct AttCfg : AttRings<NC, N, 2, false,
-                         STREAMS * att_p_buffers<N, STREAMS>() * 128 * N * 2 + 1024 + 16 * N * 4 + 8 * N * 4 + 24 * N * 4, STREAMS> {
-  static constexpr int NP = att_p_buffers<N, STREAMS>();  // buffers for P per stream (each with barriers of its own: a stream may be a buffer ahead)
+template <int NC, int N>
+struct AttCfg : AttRings<NC, N, 2, false, 2 * (N <= 32 ? 2 : 1) * 128 * N * 2 + 1024 + 16 * N * 4 + 8 * N * 4 + 24 * N * 4> {
+  static constexpr int NP = N <= 32 ? 2 : 1;  // buffers for P per stream (each with barriers of its own: a stream may be a buffer ahead)
   static constexpr int P_BYTES = 128 * N * 2;
-  static constexpr int TMEM = (N == 64 ? 512 : (N == 32 ? 256 : 128)) * STREAMS / 2;  // 3 N columns a stream: S 2, O
-  static_assert(STREAMS == 2 || N <= 32, "half an SM has registers for 32 columns");
+  static constexpr int TMEM = N == 64 ? 512 : (N == 32 ? 256 : 128);  // 6 N columns: S 2 x 2, O 2
 };
-constexpr int ATT_HALF_REGS = 128, ATT_HALF_REGS_STREAM = 176, ATT_HALF_REGS_ISSUE = 80;  // of a CTA of 256 threads, see ATT_REGS
-static_assert(128 * (ATT_HALF_REGS_STREAM + ATT_HALF_REGS_ISSUE) <= 256 * ATT_HALF_REGS, "register budgets exceed the CTA's allocation");
 
-template <int NC, int N, bool BF16, int MODE = ATT_PLAIN, int STREAMS = 2>
-__global__ void __launch_bounds__(STREAMS == 1 ? 256 : ATT_THREADS, STREAMS == 1 ? 2 : 1)
+template <int NC, int N, bool BF16>
+__global__ void __launch_bounds__(ATT_THREADS, 1)
 kfa_cache_attend_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                         const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmKn,
                         const __grid_constant__ CUtensorMap tmVn, const AttendParams p) {
-  using R = AttCfg<NC, N, STREAMS>;
+  using R = AttCfg<NC, N>;
   constexpr int NP = R::NP;
 
   extern __shared__ uint8_t smem_raw[];
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* smem = smem_raw + (base - smem_u32(smem_raw));
   const uint32_t sKV = base, sQ = sKV + R::NS * R::STAGE, sP = sQ + R::NQ * R::Q_BYTES;
-  uint8_t* small = smem + R::NS * R::STAGE + R::NQ * R::Q_BYTES + STREAMS * NP * R::P_BYTES;
+  uint8_t* small = smem + R::NS * R::STAGE + R::NQ * R::Q_BYTES + 2 * NP * R::P_BYTES;
   uint64_t* bars = reinterpret_cast<uint64_t*>(small);
   float* s_max = reinterpret_cast<float*>(small + 1024);  // [stream][tile & 1][warp][N]
   float* s_shift = s_max + 16 * N;                        // [warp][N]
@@ -843,29 +824,26 @@ kfa_cache_attend_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
   const uint32_t bar0 = smem_u32(bars);
   auto bar = [&](int i) { return bar0 + 8u * i; };
   const int tid = threadIdx.x, warp = warp_index(), lane = tid & 31;
-  if (tid == 32 * R::LOAD_WARP + 32) {
+  if (tid == 32 * 11) {
     for (const CUtensorMap* map : {&tmQ, &tmK, &tmV, &tmKn, &tmVn}) asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
   }
-  WalkOf<MODE> first;
+  Walk first;
   int chunk, end;
   const bool work = att_setup<R>(p, bar0, ac, R::TMEM, first, chunk, end);
   const uint32_t tmem = *ac.tmem;
   const Ctl ctl{ac.abort};
-  const uint32_t tmS = tmem, tmO = tmem + 2 * STREAMS * N;
+  const uint32_t tmS = tmem, tmO = tmem + 4 * N;
   int kv_issued = 0, q_issued = 0;
 
   if (!work) {
-    if (tid == 0 && (MODE == ATT_PREFIX || !p.whole)) note_parts(p, first, false, 1, 0);
-  } else if (warp >= R::LOAD_WARP) {
-    if constexpr (STREAMS == 1) reg_budget<ATT_HALF_REGS_ISSUE, ATT_HALF_REGS>();
-    else if constexpr (N == 64) reg_budget<ATT_REGS_ISSUE, ATT_REGS>();
-    const bool values = warp == R::LOAD_WARP + 1;
-    if (STREAMS == 2 || warp <= R::LOAD_WARP + 1)
-      att_produce<R>(p, first, values, sKV, sQ, bar0, ac, &tmQ, values ? &tmV : &tmK, values ? &tmVn : &tmKn, kv_issued, q_issued);
-  } else if (warp >= R::ISSUE_WARP) {
-    if constexpr (STREAMS == 1) reg_budget<ATT_HALF_REGS_ISSUE, ATT_HALF_REGS>();
-    else if constexpr (N == 64) reg_budget<ATT_REGS_ISSUE, ATT_REGS>();
-    const int st = warp - R::ISSUE_WARP;
+    if (tid == 0 && !p.whole) note_parts(p, first, false, 1, 0);
+  } else if (warp >= 10) {
+    if constexpr (N == 64) reg_budget<ATT_REGS_ISSUE, ATT_REGS>();
+    const bool values = warp == 11;
+    att_produce<R>(p, first, values, sKV, sQ, bar0, ac, &tmQ, values ? &tmV : &tmK, values ? &tmVn : &tmKn, kv_issued, q_issued);
+  } else if (warp >= 8) {
+    if constexpr (N == 64) reg_budget<ATT_REGS_ISSUE, ATT_REGS>();
+    const int st = warp - 8;
     const bool lead = elect_one();
     constexpr uint32_t IDESC_S = make_idesc(BF16, false, 128, N), IDESC_O = make_idesc(BF16, true, 128, N) | (1u << 15);
     constexpr uint32_t HI_P = sdesc_hi_for(N);
@@ -894,19 +872,18 @@ kfa_cache_attend_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
   } else {
     // =========================== softmax, output ===========================
     // (After a wait that ran out the role goes on without waiting: the warps of a stream meet at barriers.)
-    if constexpr (STREAMS == 1) reg_budget<ATT_HALF_REGS_STREAM, ATT_HALF_REGS>();
-    else if constexpr (N == 64) reg_budget<ATT_REGS_STREAM, ATT_REGS>();
-    const int st = STREAMS == 1 ? 0 : warp >> 2, wl = warp & 3, key = tid & 127;
+    if constexpr (N == 64) reg_budget<ATT_REGS_STREAM, ATT_REGS>();
+    const int st = warp >> 2, wl = warp & 3, key = tid & 127;
     const uint32_t lane_base = static_cast<uint32_t>(wl * 32) << 16;
     constexpr int PER = N / 32 > 0 ? N / 32 : 1;  // columns whose maximum a lane keeps: lane, lane + 32
     float* shift = s_shift + warp * N;
     const float c_log2 = p.c_log2;
     const float2 c2 = make_float2(c_log2, c_log2);
-    WalkOf<MODE> w = first;
+    Walk w = first;
     bool more = true, ok = true;
     int c = 0, T0 = 0, s = 0;  // the stream's tiles; tiles and segments before
     while (more) {
-      const RowMapOf<MODE> rows(p, w.b, w.item);
+      const RowMap rows(p, w.b, w.item);
       float l[N], m_ref[PER], m_top[PER];
 #pragma unroll
       for (int i = 0; i < N; ++i) l[i] = 0.f;
@@ -916,7 +893,7 @@ kfa_cache_attend_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
       const int tiles = w.tiles();
       for (int t = 0; t < tiles; ++t) {
         const int T = T0 + t;
-        if (!R::ALL && (T & 1) != st) continue;
+        if ((T & 1) != st) continue;
         const int ub = w.unit + 4 * t;
         const bool full = 4 * t + 4 <= w.n && (ub + 4) * ATT_UNIT <= w.len && ub + 4 <= w.uc;
         int fresh = -1;
@@ -1055,59 +1032,38 @@ kfa_cache_attend_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
       }
       if (!opens && ok) ok = wait_warp(bar(R::B_PV + 2 * st + (c - 1) % NP), ((c - 1) / NP) & 1, ctl, 83);
       tc_fence_before();
-      named_sync<3, 128 * STREAMS>();
+      named_sync<3, 256>();
       tc_fence_after();
+      const bool bad = *ac.bad != 0;
       const bool whole = w.begins() && w.ends();
-      if (MODE == ATT_OWN && whole) wait_for_previous();  // the carry is there
-      const bool bad = *ac.bad != 0 || (MODE == ATT_OWN && whole && load_status(p.status) != 0);
       const long long slot = 2ll * blockIdx.x + (w.begins() ? 1 : 0);
       // new tokens of the segment, where some of their values were left out (a stream may be one segment ahead: >=)
       const bool odd = ac.odd[0] >= s + 1 || ac.odd[1] >= s + 1;
       const int j0 = max(w.unit - w.uc, 0) * ATT_UNIT, j1 = odd ? min((w.unit + w.n - w.uc) * ATT_UNIT, w.count) : 0;
       const int d = wl * 32 + lane;
-      constexpr int W = N / STREAMS;  // columns of a thread
+      constexpr int W = N / 2;  // columns of a thread
       const int c0 = st * W;
       // lane i (i < W): column i's factors and statistics
       const float* f0 = s_fin + (s & 1) * 12 * N + c0 + (lane & (W - 1));
       const float* f1 = f0 + 6 * N;
-      const float m0 = f0[4 * N], m1 = STREAMS == 1 ? -INFINITY : f1[4 * N], m = fmaxf(m0, m1), top = STREAMS == 1 ? f0[5 * N] : fmaxf(f0[5 * N], f1[5 * N]);
-      const float l0 = (f0[0] + f0[N]) + (f0[2 * N] + f0[3 * N]), l1 = STREAMS == 1 ? 0.f : (f1[0] + f1[N]) + (f1[2 * N] + f1[3 * N]);
+      const float m0 = f0[4 * N], m1 = f1[4 * N], m = fmaxf(m0, m1), top = fmaxf(f0[5 * N], f1[5 * N]);
+      const float l0 = (f0[0] + f0[N]) + (f0[2 * N] + f0[3 * N]), l1 = (f1[0] + f1[N]) + (f1[2 * N] + f1[3 * N]);
       float a0 = part_factor(m0, l0, m, c_log2), a1 = part_factor(m1, l1, m, c_log2);
-      float l_all = l0 * a0 + l1 * a1, m_all = m, top_all = top, ac_carry = -1.f;
-      int h, tk, sq;
-      const bool exists = rows.row(p, c0 + (lane & (W - 1)), h, tk, sq);
-      // (ATT_PREFIX: of the carry's rows)
-      const long long row_at = exists ? (static_cast<long long>(sq) * p.H + h) * p.T + tk : -1;
-      const long long off = MODE == ATT_PREFIX ? row_at : (exists ? w.b * p.o_sb + h * p.o_sh + tk * p.o_ss : -1);
-      [[maybe_unused]] Carry carry;
-      if (MODE == ATT_OWN && whole && exists) {
-        carry.load(p, w.b, h, tk);
-        m_all = fmaxf(m, carry.m);
-        top_all = fmaxf(top, carry.top);
-        const float own = part_factor(m, l_all, m_all, c_log2);
-        ac_carry = part_factor(carry.m, carry.l, m_all, c_log2);
-        a0 = own < 0.f || a0 < 0.f ? -1.f : a0 * own;
-        a1 = own < 0.f || a1 < 0.f ? -1.f : a1 * own;
-        l_all = l_all * own + carry.l * ac_carry;
-      }
+      const float l_all = l0 * a0 + l1 * a1;
+      int h, tk;
+      const bool exists = rows.row(p, c0 + (lane & (W - 1)), h, tk);
+      const long long off = exists ? w.b * p.o_sb + h * p.o_sh + tk * p.o_ss : -1;
       const bool some = exists && tk < w.count && l_all != 0.f;
       const float nan = __int_as_float(0x7fc00000);
-      if (MODE == ATT_PREFIX && whole) {
-        if (wl == 0 && exists && lane < W) {
-          p.carry_ml[row_at] = m;
-          p.carry_ml[p.carry_rows + row_at] = l_all;
-          p.carry_ml[2 * p.carry_rows + row_at] = top;
-        }
-      } else if (whole) {
+      if (whole) {
         const float inv = some ? 1.f / l_all : 0.f;
         if (p.stats && wl == 0 && exists && lane < W) {
           float* at = p.stats + (static_cast<long long>(w.b) * p.H + h) * 2 * p.T + tk;
-          at[0] = bad ? nan : (some ? top_all : INFINITY);
-          at[p.T] = bad ? nan : (some ? log2f(l_all) + (m_all - top_all) * c_log2 : 0.f);
+          at[0] = bad ? nan : (some ? top : INFINITY);
+          at[p.T] = bad ? nan : (some ? log2f(l_all) + (m - top) * c_log2 : 0.f);
         }
         a0 = some ? a0 * inv : -1.f;
         a1 = some ? a1 * inv : -1.f;
-        if (MODE == ATT_OWN) ac_carry = some ? ac_carry * inv : -1.f;
       } else if (wl == 0 && lane < W) {
         float* at = p.part_ml + slot * 3 * p.rows + c0 + lane;
         at[0] = m;
@@ -1116,13 +1072,12 @@ kfa_cache_attend_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
       }
       float o0[W], o1[W];
       tmem_ld_cols<W>(tmO + lane_base + c0, o0);
-      if constexpr (STREAMS == 2) tmem_ld_cols<W>(tmO + lane_base + N + c0, o1);
+      tmem_ld_cols<W>(tmO + lane_base + N + c0, o1);
       tmem_wait_ld();
 #pragma unroll
       for (int i = 0; i < W; ++i) {
         const float x0 = __shfl_sync(0xffffffffu, a0, i), x1 = __shfl_sync(0xffffffffu, a1, i);
-        o0[i] = x0 < 0.f ? 0.f : o0[i] * x0;  // (a stream without tiles has left nothing there)
-        if constexpr (STREAMS == 2) o0[i] += x1 < 0.f ? 0.f : o1[i] * x1;
+        o0[i] = (x0 < 0.f ? 0.f : o0[i] * x0) + (x1 < 0.f ? 0.f : o1[i] * x1);  // (a stream without tiles has left nothing there)
       }
       if (d < p.c.cols) {
         for (int j = j0; j < j1; ++j) {
@@ -1133,21 +1088,7 @@ kfa_cache_attend_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
             if (sees_new(p, w, rows.t0 + static_cast<int>(p.by_gt.div(c0 + i)), j)) o0[i] += y;
         }
       }
-      if (MODE == ATT_OWN && whole) {
-#pragma unroll
-        for (int i = 0; i < W; ++i) {
-          const float x = __shfl_sync(0xffffffffu, ac_carry, i);
-          const long long at = __shfl_sync(0xffffffffu, row_at, i);
-          if (!(x < 0.f) && d < p.c.cols) o0[i] += x * p.carry_o[at * 128 + d];
-        }
-      }
-      if (MODE == ATT_PREFIX && whole) {
-#pragma unroll
-        for (int i = 0; i < W; ++i) {
-          const long long at = __shfl_sync(0xffffffffu, off, i);
-          if (at >= 0) p.carry_o[at * 128 + d] = o0[i];
-        }
-      } else if (whole) {
+      if (whole) {
 #pragma unroll
         for (int i = 0; i < W; ++i) {
           const long long at = __shfl_sync(0xffffffffu, off, i);
@@ -1159,25 +1100,24 @@ kfa_cache_attend_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
       } else {
 #pragma unroll
         for (int i = 0; i < W; ++i)
-          if (c0 + i < tile_rows<MODE>(p)) p.part_o[(slot * p.rows + c0 + i) * 128 + d] = o0[i];
+          if (c0 + i < p.gt * p.tt) p.part_o[(slot * p.rows + c0 + i) * 128 + d] = o0[i];
       }
       tc_fence_before();
-      if (R::ALL || tiles > 1 || ((T0 - 1) & 1) == 0) mbar_arrive(bar(R::B_OFREE));
-      if (!R::ALL && (tiles > 1 || ((T0 - 1) & 1) == 1)) mbar_arrive(bar(R::B_OFREE + 1));
+      if (tiles > 1 || ((T0 - 1) & 1) == 0) mbar_arrive(bar(R::B_OFREE));
+      if (tiles > 1 || ((T0 - 1) & 1) == 1) mbar_arrive(bar(R::B_OFREE + 1));
       mbar_arrive(bar(R::B_QFREE + s % R::NQ));
       ++s;
       more = w.next(p);
     }
-    if (tid == 0 && (MODE == ATT_PREFIX || !p.whole)) note_parts(p, w, true, chunk, end);
+    if (tid == 0 && !p.whole) note_parts(p, w, true, chunk, end);
   }
 
   // ---- teardown (every thread gets here, also after an abort) ----
-  if (MODE == ATT_OWN) wait_for_previous();  // (so that who waits for this kernel has waited for those before it)
   tc_fence_before();
   __syncthreads();
   if (tid == 0 && *ac.bad) report(p.status, DEV_BAD_CACHE);
   if (*ac.abort) att_give_up<R>(p, first, work, bar0, ac, kv_issued, q_issued);
-  if (warp == R::ISSUE_WARP) {
+  if (warp == 8) {
     tc_fence_after();
     tmem_dealloc(tmem, R::TMEM);
   }
@@ -1192,7 +1132,7 @@ struct AttRowsCfg : AttRings<NC, 128 * HALVES, HALVES == 1 ? 2 : 1, HALVES == 2,
 
 // A tile's 128 score columns are made and used as two halves of 64 keys, each with its own barriers: P (16-bit) lies over the first 32
 // of its half's columns, and while one half's values are multiplied and its next scores made, the thread works on the other.
-template <int NC, int HALVES, bool BF16, int MODE = ATT_PLAIN>
+template <int NC, int HALVES, bool BF16>
 __global__ void __launch_bounds__(ATT_THREADS, 1)
 kfa_cache_attend_rows_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                              const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmKn,
@@ -1215,7 +1155,7 @@ kfa_cache_attend_rows_kernel(const __grid_constant__ CUtensorMap tmQ, const __gr
   if (tid == 32 * 11) {
     for (const CUtensorMap* map : {&tmQ, &tmK, &tmV, &tmKn, &tmVn}) asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
   }
-  WalkOf<MODE> first;
+  Walk first;
   int chunk, end;
   const bool work = att_setup<R>(p, bar0, ac, R::TMEM, first, chunk, end);
   const uint32_t tmem = *ac.tmem;
@@ -1223,7 +1163,7 @@ kfa_cache_attend_rows_kernel(const __grid_constant__ CUtensorMap tmQ, const __gr
   int kv_issued = 0, q_issued = 0;
 
   if (!work) {
-    if (tid == 0 && (MODE == ATT_PREFIX || !p.whole)) note_parts(p, first, false, 1, 0);
+    if (tid == 0 && !p.whole) note_parts(p, first, false, 1, 0);
   } else if (warp >= 10) {
     reg_budget<ATT_REGS_ISSUE, ATT_REGS>();
     const bool values = warp == 11;
@@ -1265,13 +1205,13 @@ kfa_cache_attend_rows_kernel(const __grid_constant__ CUtensorMap tmQ, const __gr
     const float c_log2 = p.c_log2;
     const float2 c2 = make_float2(c_log2, c_log2);
     const int r = (BOTH ? 128 * st : 0) + r_in;  // the thread's row of the tile
-    WalkOf<MODE> w = first;
+    Walk w = first;
     bool more = true, ok = true;
     int c = 0, T0 = 0, s = 0;  // the stream's tiles; tiles and segments before
     while (more) {
-      const RowMapOf<MODE> rows(p, w.b, w.item);
-      int h, tk, sq;
-      const bool exists = rows.row(p, r, h, tk, sq);
+      const RowMap rows(p, w.b, w.item);
+      int h, tk;
+      const bool exists = rows.row(p, r, h, tk);
       float l = 0.f, m_ref = -INFINITY, m_top = -INFINITY;
       const int tiles = w.tiles();
       // the stream's tiles of the segment, every STEP-th from t_first on, as pieces of 64 keys; those below t_full hold cached keys only
@@ -1408,36 +1348,15 @@ kfa_cache_attend_rows_kernel(const __grid_constant__ CUtensorMap tmQ, const __gr
         l_all = l0 * a0 + l1 * a1;
       }
       tc_fence_after();
+      const bool bad = *ac.bad != 0;
       const bool whole = w.begins() && w.ends();
-      if (MODE == ATT_OWN && whole) wait_for_previous();  // the carry is there
-      const bool bad = *ac.bad != 0 || (MODE == ATT_OWN && whole && load_status(p.status) != 0);
       const long long slot = 2ll * blockIdx.x + (w.begins() ? 1 : 0);
       const bool odd = ac.odd[st] >= s + 1 || (!BOTH && ac.odd[1 - st] >= s + 1);
       const int j0 = max(w.unit - w.uc, 0) * ATT_UNIT, j1 = odd ? min((w.unit + w.n - w.uc) * ATT_UNIT, w.count) : 0;
-      const long long row_at = exists ? (static_cast<long long>(sq) * p.H + h) * p.T + tk : -1;  // of the carry
-      float ac_carry = -1.f;
-      [[maybe_unused]] Carry carry;
-      if (MODE == ATT_OWN && whole && exists) {
-        carry.load(p, w.b, h, tk);
-        const float m_own = m;
-        m = fmaxf(m, carry.m);
-        top = fmaxf(top, carry.top);
-        const float own = part_factor(m_own, l_all, m, c_log2);
-        ac_carry = part_factor(carry.m, carry.l, m, c_log2);
-        a0 = own < 0.f || a0 < 0.f ? -1.f : a0 * own;
-        a1 = own < 0.f || a1 < 0.f ? -1.f : a1 * own;
-        l_all = l_all * own + carry.l * ac_carry;
-      }
       const bool some = exists && tk < w.count && l_all != 0.f;
       const float nan = __int_as_float(0x7fc00000);
       const bool writes = BOTH || st == 0;  // of the row's statistics
-      if (MODE == ATT_PREFIX && whole) {
-        if (exists && writes) {
-          p.carry_ml[row_at] = m;
-          p.carry_ml[p.carry_rows + row_at] = l_all;
-          p.carry_ml[2 * p.carry_rows + row_at] = top;
-        }
-      } else if (whole) {
+      if (whole) {
         const float inv = some ? 1.f / l_all : 0.f;
         if (p.stats && exists && writes) {
           float* at = p.stats + (static_cast<long long>(w.b) * p.H + h) * 2 * p.T + tk;
@@ -1446,8 +1365,7 @@ kfa_cache_attend_rows_kernel(const __grid_constant__ CUtensorMap tmQ, const __gr
         }
         a0 = some ? a0 * inv : -1.f;
         a1 = some ? a1 * inv : -1.f;
-        if (MODE == ATT_OWN) ac_carry = some ? ac_carry * inv : -1.f;
-      } else if (writes && r < tile_rows<MODE>(p)) {
+      } else if (writes && r < p.gt * p.tt) {
         float* at = p.part_ml + slot * 3 * p.rows + r;
         at[0] = m;
         at[p.rows] = l_all;
@@ -1458,7 +1376,7 @@ kfa_cache_attend_rows_kernel(const __grid_constant__ CUtensorMap tmQ, const __gr
       // lies as the threads have it, 4 columns of 32 rows after 4 columns of 32 rows: each store is 512 bytes in one piece.
       const uint32_t turn = (lane >> 1) & 3;
       const uint32_t out_stage = smem_u32(s_fin) + 6144 + warp * 2048;  // 32 rows of 64 bytes
-      const long long off = MODE == ATT_PREFIX ? row_at : (exists ? w.b * p.o_sb + static_cast<long long>(h) * p.o_sh + tk * p.o_ss : -1);
+      const long long off = exists ? w.b * p.o_sb + static_cast<long long>(h) * p.o_sh + tk * p.o_ss : -1;
       const int r_warp = r - lane;
 #pragma unroll 1
       for (int i = BOTH ? 0 : 32 * st; i < D; i += BOTH ? 32 : 64) {
@@ -1484,41 +1402,8 @@ kfa_cache_attend_rows_kernel(const __grid_constant__ CUtensorMap tmQ, const __gr
             if (!(fabsf(y) < INFINITY)) o0[k] += y;
           }
         }
-        if (MODE == ATT_OWN && !(ac_carry < 0.f)) {
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            if (i + 4 * j >= p.c.cols) break;
-            const float4 y = *reinterpret_cast<const float4*>(carry.o + i + 4 * j);
-            o0[4 * j] += ac_carry * y.x;
-            o0[4 * j + 1] += ac_carry * y.y;
-            o0[4 * j + 2] += ac_carry * y.z;
-            o0[4 * j + 3] += ac_carry * y.w;
-          }
-        }
         __syncwarp();
-        if (MODE == ATT_PREFIX && whole) {
-#pragma unroll
-          for (int q = 0; q < 2; ++q) {  // rows of 16 columns: 4 pieces
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-              asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(out_stage + lane * 64 + ((j ^ turn) << 4)), "f"(o0[16 * q + 4 * j]),
-                           "f"(o0[16 * q + 4 * j + 1]), "f"(o0[16 * q + 4 * j + 2]), "f"(o0[16 * q + 4 * j + 3])
-                           : "memory");
-            __syncwarp();
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const int row = 8 * k + (lane >> 2), piece = lane & 3;
-              const long long at = __shfl_sync(0xffffffffu, off, row);
-              float4 y;
-              asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
-                           : "=f"(y.x), "=f"(y.y), "=f"(y.z), "=f"(y.w)
-                           : "r"(out_stage + row * 64 + ((piece ^ ((row >> 1) & 3)) << 4))
-                           : "memory");
-              if (at >= 0) *reinterpret_cast<float4*>(p.carry_o + at * 128 + i + 16 * q + 4 * piece) = y;
-            }
-            __syncwarp();
-          }
-        } else if (whole) {
+        if (whole) {
 #pragma unroll
           for (int j = 0; j < 4; ++j)  // rows of 64 bytes: 4 pieces
             asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(out_stage + lane * 64 + ((j ^ turn) << 4)),
@@ -1538,7 +1423,7 @@ kfa_cache_attend_rows_kernel(const __grid_constant__ CUtensorMap tmQ, const __gr
             if (bad) y = make_uint4(0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu);
             if (at >= 0 && i + 8 * piece < p.c.cols) *reinterpret_cast<uint4*>(p.o + at + 2 * i + 16 * piece) = y;
           }
-        } else if (r_warp < tile_rows<MODE>(p)) {
+        } else if (r_warp < p.gt * p.tt) {
           float4* at = reinterpret_cast<float4*>(p.part_o + (slot * p.rows + r_warp) * 128) + 8 * i + lane;
 #pragma unroll
           for (int j = 0; j < 8; ++j) at[32 * j] = make_float4(o0[4 * j], o0[4 * j + 1], o0[4 * j + 2], o0[4 * j + 3]);
@@ -1555,11 +1440,10 @@ kfa_cache_attend_rows_kernel(const __grid_constant__ CUtensorMap tmQ, const __gr
       ++s;
       more = w.next(p);
     }
-    if (tid == 0 && (MODE == ATT_PREFIX || !p.whole)) note_parts(p, w, true, chunk, end);
+    if (tid == 0 && !p.whole) note_parts(p, w, true, chunk, end);
   }
 
   // ---- teardown (every thread gets here, also after an abort) ----
-  if (MODE == ATT_OWN) wait_for_previous();  // (so that who waits for this kernel has waited for those before it)
   tc_fence_before();
   __syncthreads();
   if (tid == 0 && *ac.bad) report(p.status, DEV_BAD_CACHE);
@@ -1573,21 +1457,19 @@ kfa_cache_attend_rows_kernel(const __grid_constant__ CUtensorMap tmQ, const __gr
 // Joins the parts of the items that were cut: CTA x has the item that begins in CTA x of the kernel above, a warp a row, a lane four
 // columns. Starts while that kernel ends and waits for it. 32 parts at a time: a lane has the factor of one, and all add up their columns; the
 // first AHEAD parts' columns are on their way while the factors are found (drafts of 7 tokens 15.2 -> 14.2 us).
-template <bool BF16, int MODE = ATT_PLAIN>
+template <bool BF16>
 __global__ void __launch_bounds__(256) kfa_cache_join_kernel(const AttendParams p) {
   constexpr int AHEAD = 4;
-  if (MODE == ATT_PREFIX) let_next_begin();  // (it waits for this kernel when it needs the carry)
   wait_for_previous();
-  if (MODE != ATT_PREFIX) let_next_begin();
+  let_next_begin();
   const int4 meta = p.part_meta[blockIdx.x];
   if (meta.x == 0) return;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = blockIdx.y * 8 + warp;
-  const RowMapOf<MODE> rows(p, meta.y, meta.z);
-  int h, t, sq;
-  if (!rows.row(p, r, h, t, sq)) return;
+  const RowMap rows(p, meta.y, meta.z);
+  int h, t;
+  if (!rows.row(p, r, h, t)) return;
   const bool bad = *reinterpret_cast<const volatile int*>(p.status) != 0;
-  const int count = MODE != ATT_PREFIX && p.counts ? min(max(p.counts[meta.y], 0), p.T) : p.T;
-  const long long row_at = (static_cast<long long>(sq) * p.H + h) * p.T + t;  // of the carry
+  const int count = p.counts ? min(max(p.counts[meta.y], 0), p.T) : p.T;
   // part i: the first in slot 1 of its CTA, the others in slot 0 of theirs
   auto slot = [&](int i) { return 2ll * (blockIdx.x + i) + (i == 0 ? 1 : 0); };
   const float* o_row = p.part_o + r * 128 + 4 * lane;
@@ -1632,28 +1514,6 @@ __global__ void __launch_bounds__(256) kfa_cache_join_kernel(const AttendParams 
 #pragma unroll 4
     for (int i = AHEAD; i < n; ++i) add(i, part(i));
   }
-  if constexpr (MODE == ATT_PREFIX) {
-    *reinterpret_cast<float4*>(p.carry_o + row_at * 128 + 4 * lane) = o;
-    if (lane == 0) {
-      p.carry_ml[row_at] = m;
-      p.carry_ml[p.carry_rows + row_at] = l;
-      p.carry_ml[2 * p.carry_rows + row_at] = top;
-    }
-    return;
-  }
-  if constexpr (MODE == ATT_OWN) {
-    Carry carry;
-    carry.load(p, meta.y, h, t);
-    const float m_new = fmaxf(m, carry.m), own = part_factor(m, l, m_new, p.c_log2), a = part_factor(carry.m, carry.l, m_new, p.c_log2);
-    const float a_own = own < 0.f ? 0.f : own;
-    float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (!(a < 0.f) && 4 * lane < p.c.cols) y = *reinterpret_cast<const float4*>(carry.o + 4 * lane);
-    o = make_float4(o.x * a_own, o.y * a_own, o.z * a_own, o.w * a_own);
-    if (!(a < 0.f)) o = make_float4(o.x + a * y.x, o.y + a * y.y, o.z + a * y.z, o.w + a * y.w);
-    l = l * a_own + carry.l * a;
-    m = m_new;
-    top = fmaxf(top, carry.top);
-  }
   const bool some = t < count && l != 0.f;
   const float nan = __int_as_float(0x7fc00000), inv = some ? 1.f / l : 0.f;
   if (bad) o = make_float4(nan, nan, nan, nan);
@@ -1671,20 +1531,18 @@ __global__ void __launch_bounds__(256) kfa_cache_join_kernel(const AttendParams 
 // The same for the kernel for more rows, whose parts lie by columns: a lane a row, a warp 16 columns of 32 rows, nothing exchanged. One pass:
 // what is there is scaled down when a part has a larger maximum. (16 trees of 64 tokens, 256 rows mostly in two parts: 102.9 us with parts by
 // rows and a warp a row, 96.4 with 8 lanes a row, 93.7 so.)
-template <bool BF16, int MODE = ATT_PLAIN>
+template <bool BF16>
 __global__ void __launch_bounds__(256) kfa_cache_join_rows_kernel(const AttendParams p) {
-  if (MODE == ATT_PREFIX) let_next_begin();  // (it waits for this kernel when it needs the carry)
   wait_for_previous();
-  if (MODE != ATT_PREFIX) let_next_begin();
+  let_next_begin();
   const int4 meta = p.part_meta[blockIdx.x];
   if (meta.x == 0) return;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = blockIdx.y * 32 + lane;
-  const RowMapOf<MODE> rows(p, meta.y, meta.z);
-  int h, t, sq;
-  if (16 * warp >= p.c.cols || !rows.row(p, r, h, t, sq)) return;
+  const RowMap rows(p, meta.y, meta.z);
+  int h, t;
+  if (16 * warp >= p.c.cols || !rows.row(p, r, h, t)) return;
   const bool bad = *reinterpret_cast<const volatile int*>(p.status) != 0;
-  const int count = MODE != ATT_PREFIX && p.counts ? min(max(p.counts[meta.y], 0), p.T) : p.T;
-  const long long row_at = (static_cast<long long>(sq) * p.H + h) * p.T + t;  // of the carry
+  const int count = p.counts ? min(max(p.counts[meta.y], 0), p.T) : p.T;
   const float* ml = p.part_ml + (2ll * blockIdx.x + 1) * 3 * p.rows + r;  // the first part in slot 1 of its CTA, the others in slot 0 of theirs
   const float4* from = reinterpret_cast<const float4*>(p.part_o + ((2ll * blockIdx.x + 1) * p.rows + 32 * blockIdx.y) * 128) + 128 * warp + lane;
   float m = -INFINITY, top = -INFINITY, l = 0.f, o[16];
@@ -1709,38 +1567,6 @@ __global__ void __launch_bounds__(256) kfa_cache_join_rows_kernel(const AttendPa
 #pragma unroll
       for (int q = 0; q < 4; ++q) o[4 * k + q] = o[4 * k + q] * f + (fi < 0.f ? 0.f : y[q] * fi);
     }
-  }
-  if constexpr (MODE == ATT_PREFIX) {
-    float4* to = reinterpret_cast<float4*>(p.carry_o + row_at * 128 + 16 * warp);
-#pragma unroll
-    for (int k = 0; k < 4; ++k) to[k] = make_float4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
-    if (warp == 0) {
-      p.carry_ml[row_at] = m;
-      p.carry_ml[p.carry_rows + row_at] = l;
-      p.carry_ml[2 * p.carry_rows + row_at] = top;
-    }
-    return;
-  }
-  if constexpr (MODE == ATT_OWN) {
-    Carry carry;
-    carry.load(p, meta.y, h, t);
-    const float m_new = fmaxf(m, carry.m), own = part_factor(m, l, m_new, p.c_log2), a = part_factor(carry.m, carry.l, m_new, p.c_log2);
-    const float a_own = own < 0.f ? 0.f : own;
-#pragma unroll
-    for (int k = 0; k < 16; ++k) o[k] *= a_own;
-    if (!(a < 0.f)) {
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const float4 y = *reinterpret_cast<const float4*>(carry.o + 16 * warp + 4 * k);
-        o[4 * k] += a * y.x;
-        o[4 * k + 1] += a * y.y;
-        o[4 * k + 2] += a * y.z;
-        o[4 * k + 3] += a * y.w;
-      }
-    }
-    l = l * a_own + carry.l * a;
-    m = m_new;
-    top = fmaxf(top, carry.top);
   }
   const bool some = t < count && l != 0.f;
   const float nan = __int_as_float(0x7fc00000), inv = some ? 1.f / l : 0.f;

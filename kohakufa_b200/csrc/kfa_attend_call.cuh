@@ -14,8 +14,7 @@ struct AttendPlan {
   int64_t most_units, meta_bytes, ml_bytes, bytes;
 };
 
-// halves: the kernels of half an SM, where there are any.
-AttendPlan plan_attend(int64_t batch, int64_t heads, int64_t kv_heads, int64_t T, int64_t capacity, bool fresh, bool halves = false) {
+AttendPlan plan_attend(int64_t batch, int64_t heads, int64_t kv_heads, int64_t T, int64_t capacity, bool fresh) {
   AttendPlan a;
   const int64_t group = heads / kv_heads;
   // Rows that share a K / V head, up to 256 of them in a tile: whole groups of heads, the tokens in equal parts.
@@ -37,7 +36,7 @@ AttendPlan plan_attend(int64_t batch, int64_t heads, int64_t kv_heads, int64_t T
   a.extra = a.rows > 64 ? 16 : 12;
   a.least = 4;
   a.most_units = items * (units + a.extra);
-  a.grid = static_cast<int>(std::min<int64_t>(halves && a.rows <= 32 ? 2 * SMS : SMS, a.whole ? items : (items * units + 3) / 4));
+  a.grid = static_cast<int>(std::min<int64_t>(SMS, a.whole ? items : (items * units + 3) / 4));
   a.meta_bytes = a.ml_bytes = a.bytes = 0;
   if (!a.whole) {
     a.meta_bytes = (16 * a.grid + 255) / 256 * 256;
@@ -47,37 +46,30 @@ AttendPlan plan_attend(int64_t batch, int64_t heads, int64_t kv_heads, int64_t T
   return a;
 }
 
-template <int MODE, bool BF16, class R, typename K>
+template <bool BF16, class R, typename K>
 int launch_attend(K kern, const CUtensorMap (&m)[5], const kfa::AttendParams& p, const AttendPlan& plan, cudaStream_t s) {
   static std::atomic<uint64_t> allowed{0};
   int rc = allow_smem(allowed, reinterpret_cast<const void*>(kern), R::SMEM);
   if (rc) return rc;
-  if ((rc = launch(kern, dim3(plan.grid), R::THREADS, R::SMEM, s, m[0], m[1], m[2], m[3], m[4], p)) || plan.whole) return rc;
-  if (plan.rows > 64) return launch(kfa::kfa_cache_join_rows_kernel<BF16, MODE>, dim3(plan.grid, (plan.tile_rows + 31) / 32), 256, 0, s, p);
-  return launch(kfa::kfa_cache_join_kernel<BF16, MODE>, dim3(plan.grid, (plan.tile_rows + 7) / 8), 256, 0, s, p);
+  if ((rc = launch(kern, dim3(plan.grid), kfa::ATT_THREADS, R::SMEM, s, m[0], m[1], m[2], m[3], m[4], p)) || plan.whole) return rc;
+  if (plan.rows > 64) return launch(kfa::kfa_cache_join_rows_kernel<BF16>, dim3(plan.grid, (plan.tile_rows + 31) / 32), 256, 0, s, p);
+  return launch(kfa::kfa_cache_join_kernel<BF16>, dim3(plan.grid, (plan.tile_rows + 7) / 8), 256, 0, s, p);
 }
 
-template <int MODE, int NC, bool BF16>
+template <int NC, bool BF16>
 int launch_attend_rows(const CUtensorMap (&m)[5], const kfa::AttendParams& p, const AttendPlan& plan, cudaStream_t s) {
-  if constexpr (MODE == kfa::ATT_OWN) {  // (caches behind a prefix are short, and their items' ends many)
-    if (plan.rows == 16)
-      return launch_attend<MODE, BF16, kfa::AttCfg<NC, 16, 1>>(kfa::kfa_cache_attend_kernel<NC, 16, BF16, MODE, 1>, m, p, plan, s);
-    if (plan.rows == 32)
-      return launch_attend<MODE, BF16, kfa::AttCfg<NC, 32, 1>>(kfa::kfa_cache_attend_kernel<NC, 32, BF16, MODE, 1>, m, p, plan, s);
-  }
   switch (plan.rows) {
-    case 16: return launch_attend<MODE, BF16, kfa::AttCfg<NC, 16>>(kfa::kfa_cache_attend_kernel<NC, 16, BF16, MODE>, m, p, plan, s);
-    case 32: return launch_attend<MODE, BF16, kfa::AttCfg<NC, 32>>(kfa::kfa_cache_attend_kernel<NC, 32, BF16, MODE>, m, p, plan, s);
-    case 64: return launch_attend<MODE, BF16, kfa::AttCfg<NC, 64>>(kfa::kfa_cache_attend_kernel<NC, 64, BF16, MODE>, m, p, plan, s);
-    case 128: return launch_attend<MODE, BF16, kfa::AttRowsCfg<NC, 1>>(kfa::kfa_cache_attend_rows_kernel<NC, 1, BF16, MODE>, m, p, plan, s);
-    default: return launch_attend<MODE, BF16, kfa::AttRowsCfg<NC, 2>>(kfa::kfa_cache_attend_rows_kernel<NC, 2, BF16, MODE>, m, p, plan, s);
+    case 16: return launch_attend<BF16, kfa::AttCfg<NC, 16>>(kfa::kfa_cache_attend_kernel<NC, 16, BF16>, m, p, plan, s);
+    case 32: return launch_attend<BF16, kfa::AttCfg<NC, 32>>(kfa::kfa_cache_attend_kernel<NC, 32, BF16>, m, p, plan, s);
+    case 64: return launch_attend<BF16, kfa::AttCfg<NC, 64>>(kfa::kfa_cache_attend_kernel<NC, 64, BF16>, m, p, plan, s);
+    case 128: return launch_attend<BF16, kfa::AttRowsCfg<NC, 1>>(kfa::kfa_cache_attend_rows_kernel<NC, 1, BF16>, m, p, plan, s);
+    default: return launch_attend<BF16, kfa::AttRowsCfg<NC, 2>>(kfa::kfa_cache_attend_rows_kernel<NC, 2, BF16>, m, p, plan, s);
   }
 }
 
-template <int MODE>
 int launch_attend_call(const CUtensorMap (&m)[5], const kfa::AttendParams& p, const AttendPlan& plan, int dtype, cudaStream_t s) {
-  if (dtype == KFA_BF16) return p.c.cols > 64 ? launch_attend_rows<MODE, 2, true>(m, p, plan, s) : launch_attend_rows<MODE, 1, true>(m, p, plan, s);
-  return p.c.cols > 64 ? launch_attend_rows<MODE, 2, false>(m, p, plan, s) : launch_attend_rows<MODE, 1, false>(m, p, plan, s);
+  if (dtype == KFA_BF16) return p.c.cols > 64 ? launch_attend_rows<2, true>(m, p, plan, s) : launch_attend_rows<1, true>(m, p, plan, s);
+  return p.c.cols > 64 ? launch_attend_rows<2, false>(m, p, plan, s) : launch_attend_rows<1, false>(m, p, plan, s);
 }
 
 // What a plan's rows, items and scratch are, in the kernels' parameters.
@@ -109,10 +101,15 @@ int pages_map(const KfaTensor4* t, const kfa::AttendParams& p, int dtype, CUtens
   return make_box_map(t->ptr, p.c.cols, t->shape[2], t->stride[2], t->shape[1], t->stride[1], t->shape[0], t->stride[0], p.box, 1, 1, dtype, map, name);
 }
 
-// The checks of an attention call to a cache, its plan, parameters and tensor maps.
-int prepare_attend(const KfaTensor4* q, const KfaCache* cache, const KfaTensor4* k, const KfaTensor4* v, const uint8_t* tree,
-                   const int64_t* tree_stride, const int32_t* counts, const KfaTensor4* out, float* stats, void* scratch, float scale, int dtype,
-                   int* dev_status, kfa::AttendParams& p, AttendPlan& plan, CUtensorMap (&m)[5], bool halves = false) {
+// Rows of new tokens' keys or values, in boxes of a unit.
+int new_map(const KfaTensor4* t, const kfa::AttendParams& p, int dtype, CUtensorMap* map, const char* name) {
+  return make_box_map(t->ptr, p.c.cols, p.T, t->stride[2], p.c.heads, t->stride[1], p.c.batch, t->stride[0], kfa::ATT_UNIT, 1, 1, dtype, map, name);
+}
+
+// The checks of an attention call to a cache, and the parameters that do not depend on how it is cut up.
+int check_attend(const KfaTensor4* q, const KfaCache* cache, const KfaTensor4* k, const KfaTensor4* v, const uint8_t* tree,
+                 const int64_t* tree_stride, const int32_t* counts, const KfaTensor4* out, float* stats, float scale, int dtype,
+                 int* dev_status, kfa::AttendParams& p) {
   std::memset(&p, 0, sizeof(p));
   int rc;
   if ((rc = check_cache(cache, &p.c)) || (rc = check_new(q, p.c, 0, "q")) || (rc = check_new(out, p.c, 0, "out")) ||
@@ -143,7 +140,16 @@ int prepare_attend(const KfaTensor4* q, const KfaCache* cache, const KfaTensor4*
   p.c_log2 = std::max(scale * LOG2E, 1e-30f);
   p.slack = 8.f / p.c_log2;
   p.status = dev_status;
-  plan = plan_attend(p.c.batch, p.H, p.c.heads, p.T, p.c.capacity, k != nullptr, halves);
+  return KFA_OK;
+}
+
+// The same with its plan and tensor maps.
+int prepare_attend(const KfaTensor4* q, const KfaCache* cache, const KfaTensor4* k, const KfaTensor4* v, const uint8_t* tree,
+                   const int64_t* tree_stride, const int32_t* counts, const KfaTensor4* out, float* stats, void* scratch, float scale, int dtype,
+                   int* dev_status, kfa::AttendParams& p, AttendPlan& plan, CUtensorMap (&m)[5]) {
+  int rc = check_attend(q, cache, k, v, tree, tree_stride, counts, out, stats, scale, dtype, dev_status, p);
+  if (rc) return rc;
+  plan = plan_attend(p.c.batch, p.H, p.c.heads, p.T, p.c.capacity, k != nullptr);
   if (plan.most_units > 0x3fffffff) return fail(KFA_ERR_ARG, "too many rows in one call");
   if (plan.bytes && (!scratch || reinterpret_cast<uintptr_t>(scratch) % 16)) return fail(KFA_ERR_ARG, "scratch: null or not 16-byte aligned");
   fill_plan(p, plan, scratch);
@@ -153,10 +159,7 @@ int prepare_attend(const KfaTensor4* q, const KfaCache* cache, const KfaTensor4*
     return rc;
   m[3] = m[1];
   m[4] = m[2];
-  auto fresh = [&](const KfaTensor4* t, CUtensorMap* map, const char* name) {
-    return make_box_map(t->ptr, D, p.T, t->stride[2], p.c.heads, t->stride[1], p.c.batch, t->stride[0], kfa::ATT_UNIT, 1, 1, dtype, map, name);
-  };
-  if (k && ((rc = fresh(k, &m[3], "k")) || (rc = fresh(v, &m[4], "v")))) return rc;
+  if (k && ((rc = new_map(k, p, dtype, &m[3], "k")) || (rc = new_map(v, p, dtype, &m[4], "v")))) return rc;
   return KFA_OK;
 }
 

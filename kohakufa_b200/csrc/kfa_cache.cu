@@ -87,7 +87,7 @@ int kfa_cache_attend(const KfaTensor4* q, const KfaCache* cache, const KfaTensor
   CUtensorMap m[5];
   int rc = prepare_attend(q, cache, k, v, tree, tree_stride, counts, out, stats, scratch, scale, dtype, dev_status, p, plan, m);
   if (rc) return rc;
-  return launch_attend_call<kfa::ATT_PLAIN>(m, p, plan, dtype, static_cast<cudaStream_t>(stream));
+  return launch_attend_call(m, p, plan, dtype, static_cast<cudaStream_t>(stream));
 }
 
 int kfa_cache_append(const KfaCache* cache, const KfaTensor4* k, const KfaTensor4* v, const KfaRows* rows, int* dev_status,

@@ -1,32 +1,114 @@
 // C ABI of attention behind shared prefixes (declared in include/kfa.h): argument checks and launches.
-#include "kfa_attend.cuh"
 #include "kfa_attend_call.cuh"
+#include "kfa_shared.cuh"
 
 namespace {
 
-// How the prefixes' part is cut up: row tiles of up to 256 rows out of the sequences that go on from a prefix, otherwise as plan_attend does it. What each
-// prefix has of them only the device knows; the tile is made for twice their mean number (for all where there is one prefix, in equal parts).
-AttendPlan plan_prefix(int64_t batch, int64_t heads, int64_t kv_heads, int64_t T, int64_t prefixes, int64_t capacity, int* ts) {
-  AttendPlan a = plan_attend(1, heads, kv_heads, T, capacity, false);
-  const int64_t per_seq = static_cast<int64_t>(a.gt) * a.tt, mean = (batch + prefixes - 1) / prefixes;
-  int64_t n = 1;
-  if (a.tt == T) n = std::min(std::max<int64_t>(256 / per_seq, 1), prefixes == 1 ? batch : std::min(batch, 2 * mean));
-  if (prefixes == 1) n = (batch + (batch + n - 1) / n - 1) / ((batch + n - 1) / n);
-  *ts = static_cast<int>(n);
-  a.tile_rows = static_cast<int>(per_seq * n);
-  a.rows = a.tile_rows <= 16 ? 16 : (a.tile_rows <= 32 ? 32 : (a.tile_rows <= 64 ? 64 : (a.tile_rows <= 128 ? 128 : 256)));
-  a.whole = false;
-  a.extra = a.rows > 64 ? 16 : 12;
-  const int64_t items = kv_heads * a.row_tiles * ((batch + n - 1) / n + prefixes - 1), units = std::max<int64_t>((capacity + 31) / 32, 1);
-  a.most_units = items * (units + a.extra);
-  a.grid = static_cast<int>(std::min<int64_t>(SMS, (items * units + 3) / 4));
-  a.meta_bytes = (16 * a.grid + 255) / 256 * 256;
-  a.ml_bytes = 2ll * a.grid * 3 * a.rows * 4;
-  a.bytes = a.meta_bytes + a.ml_bytes + 2ll * a.grid * a.rows * 128 * 4;
+int64_t padded(int64_t bytes) { return (bytes + 255) / 256 * 256; }
+int matrix_rows(int64_t rows) { return rows <= 16 ? 16 : (rows <= 32 ? 32 : 128); }
+
+// How a call is cut up: a function of the shapes alone, so that the scratch it needs is known beforehand.
+struct SharedPlan {
+  int gt, tt, head_tiles, row_tiles, ts;  // a row tile: gt heads x tt tokens, of a prefix x ts sequences
+  int n_pre, n_own;                       // the kernel's rows
+  int grid, extra_pre, extra_own;
+  int64_t most_pre, most_own;             // counted units
+  int64_t part_ml, part_o, carry_ml, carry_o, dir_pre, dir_own, bytes;  // where each begins in the scratch: [4 grid][3][rows]; [4 grid][rows][128]; ...
+  int64_t carry_bytes;                    // of one of the two
+};
+
+SharedPlan plan_shared(int64_t batch, int64_t heads, int64_t kv_heads, int64_t T, int64_t prefixes, int64_t prefix_room, int64_t room, bool fresh) {
+  SharedPlan a;
+  const int64_t group = heads / kv_heads, gt = std::min<int64_t>(group, 128), most = 128 / gt;
+  const int64_t token_tiles = (T + most - 1) / most, tt = (T + token_tiles - 1) / token_tiles, per = gt * tt;
+  a.gt = static_cast<int>(gt);
+  a.tt = static_cast<int>(tt);
+  a.head_tiles = static_cast<int>((group + gt - 1) / gt);
+  a.row_tiles = static_cast<int>(a.head_tiles * token_tiles);
+  // Sequences of a prefix' row tile: what 128 rows hold, of one prefix in equal parts. How many each prefix has only the device knows: where they are
+  // many the tile is made for twice their mean number.
+  int64_t ts = token_tiles == 1 ? std::max<int64_t>(128 / per, 1) : 1;
+  const int64_t mean = (batch + prefixes - 1) / prefixes;
+  ts = std::min(ts, prefixes == 1 ? batch : std::min(batch, 2 * mean));
+  if (prefixes == 1) ts = (batch + (batch + ts - 1) / ts - 1) / ((batch + ts - 1) / ts);
+  a.ts = static_cast<int>(ts);
+  a.n_own = matrix_rows(per);
+  a.n_pre = std::max(matrix_rows(per * ts), a.n_own);
+  a.extra_pre = a.n_pre == 128 ? 8 : 6;
+  a.extra_own = a.n_own == 128 ? 8 : 6;
+  const int64_t pre_items = kv_heads * a.row_tiles * ((batch + ts - 1) / ts + prefixes - 1), own_items = batch * kv_heads * a.row_tiles;
+  const int64_t pre_units = std::max<int64_t>((prefix_room + 31) / 32, 1);
+  const int64_t own_units = std::max<int64_t>((room + 31) / 32 + (fresh ? (T + 31) / 32 : 0), 1);
+  a.most_pre = pre_items * (pre_units + a.extra_pre);
+  a.most_own = own_items * (own_units + a.extra_own);
+  // (each kind of work has CTAs of its own, of two halves that have at least 4 units each)
+  const auto ctas = [](int64_t items, int64_t units) { return (std::min<int64_t>(items, 2 * SMS) * ((units + 3) / 4) + 1) / 2; };
+  a.grid = static_cast<int>(std::min<int64_t>(SMS, ctas(pre_items, pre_units) + ctas(own_items, own_units)));
+  const int64_t rows = batch * heads * T;
+  const int r = std::max(a.n_pre, a.n_own);
+  int64_t at = 0;
+  auto take = [&](int64_t bytes) {
+    const int64_t here = at;
+    at += padded(bytes);
+    return here;
+  };
+  a.part_ml = take(4ll * a.grid * 3 * r * 4);
+  a.part_o = take(4ll * a.grid * r * 512);
+  a.carry_bytes = padded(12 * rows) + padded(512 * rows);
+  a.carry_ml = take(2 * a.carry_bytes);
+  a.carry_o = a.carry_ml + padded(12 * rows);
+  a.dir_pre = take(8 * kv_heads * a.row_tiles * batch);
+  a.dir_own = take(8 * kv_heads * a.row_tiles * batch);
+  a.bytes = at;
   return a;
 }
 
-int64_t padded(int64_t bytes) { return (bytes + 255) / 256 * 256; }
+void fill_part(kfa::AttendParams& p, const SharedPlan& plan, bool pre, int64_t batch, void* scratch) {
+  p.gt = plan.gt;
+  p.tt = plan.tt;
+  p.head_tiles = plan.head_tiles;
+  p.row_tiles = plan.row_tiles;
+  p.items = p.c.heads * plan.row_tiles;
+  p.by_gt = kfa::FastDiv::by(p.gt);
+  p.by_items = kfa::FastDiv::by(p.items);
+  p.by_row_tiles = kfa::FastDiv::by(p.row_tiles);
+  p.by_head_tiles = kfa::FastDiv::by(p.head_tiles);
+  p.least = 4;
+  p.extra = pre ? plan.extra_pre : plan.extra_own;
+  p.rows = std::max(plan.n_pre, plan.n_own);
+  p.box = page_box(p.c);
+  p.seqs = static_cast<int>(batch);
+  p.ts = plan.ts;
+  p.by_ts = kfa::FastDiv::by(plan.ts);
+  p.by_seq_rows = kfa::FastDiv::by(plan.gt * plan.tt);
+  uint8_t* at = static_cast<uint8_t*>(scratch);
+  p.part_ml = reinterpret_cast<float*>(at + plan.part_ml);
+  p.part_o = reinterpret_cast<float*>(at + plan.part_o);
+  p.carry_ml = reinterpret_cast<float*>(at + plan.carry_ml + (pre ? 0 : plan.carry_bytes));
+  p.carry_o = reinterpret_cast<float*>(at + plan.carry_o + (pre ? 0 : plan.carry_bytes));
+  p.dir = reinterpret_cast<int2*>(at + (pre ? plan.dir_pre : plan.dir_own));
+}
+
+template <int NC, int N_PRE, int N_OWN, bool BF16>
+int launch_shared(const CUtensorMap (&m)[8], const kfa::SharedParams& p, const SharedPlan& plan, cudaStream_t s) {
+  auto kern = kfa::kfa_shared_kernel<NC, N_PRE, N_OWN, BF16>;
+  constexpr int SMEM = 2 * kfa::SH_SMEM + 1024;
+  static_assert(std::max(kfa::ShCfg<NC, N_PRE>::SMEM, kfa::ShCfg<NC, N_OWN>::SMEM) <= kfa::SH_SMEM && SMEM <= 232448, "shared memory");
+  static std::atomic<uint64_t> allowed{0};
+  int rc = allow_smem(allowed, reinterpret_cast<const void*>(kern), SMEM);
+  if (rc) return rc;
+  if ((rc = launch(kern, dim3(plan.grid), 2 * kfa::SH_THREADS, SMEM, s, m[0], m[1], m[2], m[3], m[4], m[5], m[6], m[7], p))) return rc;
+  return launch(kfa::kfa_shared_join_kernel<BF16>, dim3(static_cast<unsigned>((p.own.carry_rows + 7) / 8)), 256, 0, s, p, kfa::FastDiv::by(p.own.H),
+                kfa::FastDiv::by(p.own.T));
+}
+
+template <int NC, bool BF16>
+int launch_shared_rows(const CUtensorMap (&m)[8], const kfa::SharedParams& p, const SharedPlan& plan, cudaStream_t s) {
+  if (plan.n_own == 128) return launch_shared<NC, 128, 128, BF16>(m, p, plan, s);
+  if (plan.n_own == 32) return plan.n_pre == 128 ? launch_shared<NC, 128, 32, BF16>(m, p, plan, s) : launch_shared<NC, 32, 32, BF16>(m, p, plan, s);
+  if (plan.n_pre == 128) return launch_shared<NC, 128, 16, BF16>(m, p, plan, s);
+  return plan.n_pre == 32 ? launch_shared<NC, 32, 16, BF16>(m, p, plan, s) : launch_shared<NC, 16, 16, BF16>(m, p, plan, s);
+}
 
 }  // namespace
 
@@ -37,56 +119,54 @@ int64_t kfa_cache_attend_shared_bytes(const KfaTensor4* q, const KfaCache* prefi
   const int64_t page = prefix->k.shape[2], kv_heads = prefix->k.shape[1], own = cache->k.shape[2], batch = q->shape[0];
   if (batch < 1 || q->shape[1] < 1 || q->shape[2] < 1 || kv_heads < 1 || q->shape[1] < kv_heads || page < 1 || own < 1 || prefix->batch < 1)
     return 0;  // (refused by the call)
-  int ts;
-  const AttendPlan a = plan_prefix(batch, q->shape[1], kv_heads, q->shape[2], prefix->batch, prefix->table ? prefix->table_cols * page : page, &ts);
-  const AttendPlan o = plan_attend(batch, q->shape[1], kv_heads, q->shape[2], cache->table ? cache->table_cols * own : own, k != nullptr, true);
-  return padded(a.bytes) + padded(12 * batch * q->shape[1] * q->shape[2]) + 512 * batch * q->shape[1] * q->shape[2] + o.bytes;
+  return plan_shared(batch, q->shape[1], kv_heads, q->shape[2], prefix->batch, prefix->table ? prefix->table_cols * page : page,
+                     cache->table ? cache->table_cols * own : own, k != nullptr)
+      .bytes;
 }
 
 int kfa_cache_attend_shared(const KfaTensor4* q, const KfaCache* prefix, const int32_t* starts, const KfaCache* cache, const KfaTensor4* k,
                             const KfaTensor4* v, const uint8_t* tree, const int64_t* tree_stride, const int32_t* counts,
                             const KfaTensor4* out, float* stats, void* scratch, float scale, int dtype, int* dev_status, void* stream) {
-  kfa::AttendParams p, o;
-  AttendPlan plan, own;
-  CUtensorMap m[5], mo[5];
+  kfa::SharedParams p;
   std::memset(&p, 0, sizeof(p));
   int rc;
-  if (!scratch || reinterpret_cast<uintptr_t>(scratch) % 16) return fail(KFA_ERR_ARG, "scratch: null or not 16-byte aligned");
-  if ((rc = check_cache(prefix, &p.c, "prefix")) || (rc = check_tensor(q, "q"))) return rc;
-  if (!starts && p.c.batch != 1) return fail(KFA_ERR_ARG, "starts: needed for %d prefixes", p.c.batch);
-  if (q->shape[1] % p.c.heads || q->shape[3] != p.c.cols) return fail(KFA_ERR_ARG, "q: does not fit the prefixes' heads and head dim");
-  int ts;
-  plan = plan_prefix(q->shape[0], q->shape[1], p.c.heads, q->shape[2], p.c.batch, p.c.capacity, &ts);
-  const int64_t rows = q->shape[0] * q->shape[1] * q->shape[2];
-  if (plan.most_units > 0x3fffffff || rows > 0x7fffffff) return fail(KFA_ERR_ARG, "too many rows in one call");
-  uint8_t* carry = static_cast<uint8_t*>(scratch) + padded(plan.bytes);
-  uint8_t* behind = carry + padded(12 * rows) + 512 * rows;
-  if ((rc = prepare_attend(q, cache, k, v, tree, tree_stride, counts, out, stats, behind, scale, dtype, dev_status, o, own, mo, true))) return rc;
-  if (o.c.heads != p.c.heads || o.c.cols != p.c.cols) return fail(KFA_ERR_ARG, "prefix: heads or head dim differ from the cache's");
-  p.H = o.H;
-  p.T = o.T;
-  p.group = o.group;
-  p.c_log2 = o.c_log2;
-  p.slack = o.slack;
-  p.status = dev_status;
-  fill_plan(p, plan, scratch);
-  p.seqs = static_cast<int>(q->shape[0]);
-  p.ts = ts;
-  p.by_ts = kfa::FastDiv::by(ts);
-  p.by_seq_rows = kfa::FastDiv::by(p.gt * p.tt);
-  p.starts = o.starts = starts;
-  p.groups = o.groups = p.c.batch;
-  p.carry_rows = o.carry_rows = rows;
-  p.carry_ml = o.carry_ml = reinterpret_cast<float*>(carry);
-  p.carry_o = o.carry_o = reinterpret_cast<float*>(carry + padded(12 * rows));
-  if ((rc = make_box_map(q->ptr, p.c.cols, p.H, q->stride[1], p.T, q->stride[2], p.seqs, q->stride[0], p.gt, p.tt, ts, dtype, &m[0], "q")) ||
-      (rc = pages_map(&prefix->k, p, dtype, &m[1], "prefix keys")) || (rc = pages_map(&prefix->v, p, dtype, &m[2], "prefix values")))
+  if ((rc = check_attend(q, cache, k, v, tree, tree_stride, counts, out, stats, scale, dtype, dev_status, p.own)) ||
+      (rc = check_cache(prefix, &p.pre.c, "prefix")))
     return rc;
-  m[3] = m[1];
-  m[4] = m[2];
+  kfa::AttendParams &own = p.own, &pre = p.pre;
+  if (own.c.heads != pre.c.heads || own.c.cols != pre.c.cols) return fail(KFA_ERR_ARG, "prefix: heads or head dim differ from the cache's");
+  if (!starts && pre.c.batch != 1) return fail(KFA_ERR_ARG, "starts: needed for %d prefixes", pre.c.batch);
+  if (!scratch || reinterpret_cast<uintptr_t>(scratch) % 16) return fail(KFA_ERR_ARG, "scratch: null or not 16-byte aligned");
+  const int64_t batch = own.c.batch, rows = batch * own.H * own.T, D = own.c.cols;
+  const SharedPlan plan = plan_shared(batch, own.H, own.c.heads, own.T, pre.c.batch, pre.c.capacity, own.c.capacity, k != nullptr);
+  if (plan.most_pre > 0x3fffffff || plan.most_own > 0x3fffffff || rows > 0x7fffff00) return fail(KFA_ERR_ARG, "too many rows in one call");
+  pre.H = own.H;
+  pre.T = own.T;
+  pre.group = own.group;
+  pre.c_log2 = own.c_log2;
+  pre.slack = own.slack;
+  pre.status = dev_status;
+  pre.starts = own.starts = starts;
+  pre.groups = own.groups = pre.c.batch;
+  pre.carry_rows = own.carry_rows = rows;
+  fill_part(pre, plan, true, batch, scratch);
+  fill_part(own, plan, false, batch, scratch);
+  p.rows = pre.rows;
+  p.weight = 1.f;
+  CUtensorMap m[8];
+  auto queries = [&](int ts, CUtensorMap* map) {
+    return make_box_map(q->ptr, D, own.H, q->stride[1], own.T, q->stride[2], batch, q->stride[0], plan.gt, plan.tt, ts, dtype, map, "q");
+  };
+  if ((rc = queries(plan.ts, &m[0])) || (rc = pages_map(&prefix->k, pre, dtype, &m[1], "prefix keys")) ||
+      (rc = pages_map(&prefix->v, pre, dtype, &m[2], "prefix values")) || (rc = queries(1, &m[3])) ||
+      (rc = pages_map(&cache->k, own, dtype, &m[4], "cache keys")) || (rc = pages_map(&cache->v, own, dtype, &m[5], "cache values")))
+    return rc;
+  m[6] = m[4];
+  m[7] = m[5];
+  if (k && ((rc = new_map(k, own, dtype, &m[6], "k")) || (rc = new_map(v, own, dtype, &m[7], "v")))) return rc;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if ((rc = launch_attend_call<kfa::ATT_PREFIX>(m, p, plan, dtype, s))) return rc;
-  return launch_attend_call<kfa::ATT_OWN>(mo, o, own, dtype, s);
+  if (dtype == KFA_BF16) return D > 64 ? launch_shared_rows<2, true>(m, p, plan, s) : launch_shared_rows<1, true>(m, p, plan, s);
+  return D > 64 ? launch_shared_rows<2, false>(m, p, plan, s) : launch_shared_rows<1, false>(m, p, plan, s);
 }
 
 }  // extern "C"
