@@ -23,6 +23,8 @@
 //   warps 5, 6                   TMA producers: keys and queries, values
 #pragma once
 
+#include <type_traits>
+
 #include "kfa_attend.cuh"
 
 namespace kfa {
@@ -226,6 +228,7 @@ __device__ __forceinline__ void sh_columns(const AttendParams& p, const WalkOf<M
         p, first, 0, x.bar0, ac,
         [&](const AttTile& t, int c, int) {
           const uint32_t k_lo = sdesc_lo(x.sKV + R::k_stage(t.T) * R::STAGE, 16), q_lo = sdesc_lo(x.sQ + (t.s % R::NQ) * R::Q_BYTES, 16);
+#pragma unroll 2
           for (int kk = 0; kk < k_steps; ++kk)
             umma_ss_lead2(lead, tmS + (c & 1) * N, k_lo + (((kk >> 2) * R::CHUNK + (kk & 3) * 32) >> 4), SDESC_HI,
                           q_lo + (((kk >> 2) * R::Q_CHUNK + (kk & 3) * 32) >> 4), SDESC_HI, IDESC_S, kk > 0 ? 1u : 0u);
@@ -236,7 +239,7 @@ __device__ __forceinline__ void sh_columns(const AttendParams& p, const WalkOf<M
         [&](const AttTile& t, int, int) {
           // (64 columns or fewer: the matrix' rows 64 .. 127 repeat the first ones, and nobody reads them)
           const uint32_t v_lo = sdesc_lo(x.sKV + R::v_stage(t.T) * R::STAGE, NC == 2 ? R::CHUNK : 0), p_lo = sdesc_lo(x.sP, 16);
-#pragma unroll
+#pragma unroll 2
           for (int kk = 0; kk < 8; ++kk)
             umma_ss_lead2(lead, tmO, v_lo + ((kk * 16 * 128) >> 4), SDESC_HI, p_lo + ((kk * 16 * 2 * N) >> 4), HI_P, IDESC_O,
                           (!t.opens || kk > 0) ? 1u : 0u);
@@ -273,18 +276,19 @@ __device__ __forceinline__ void sh_columns(const AttendParams& p, const WalkOf<M
         }
       }
       const int tiles = w.template tiles<R::UNITS>(), c0 = c;
-      for (int t = 0; t < tiles; ++t, ++c) {
-        const int ub = w.unit + R::UNITS * t;
-        const bool full = R::UNITS * t + R::UNITS <= w.n && (ub + R::UNITS) * ATT_UNIT <= w.len && ub + R::UNITS <= w.uc;
+      const int t_full = max(min(w.n, min(w.len / ATT_UNIT, w.uc) - w.unit), 0) / R::UNITS;  // tiles below hold cached keys only
+      // (The masked tiles, an item's last ones, have code of their own: it does not share the instruction cache with the loop over the others.)
+      auto tile = [&](auto masked, int t) {
+        constexpr bool full = !decltype(masked)::value;
         int fresh = -1;
-        const bool valid = full || which_key(w, ub, tid & 127, fresh);
+        const bool valid = full || which_key(w, w.unit + R::UNITS * t, tid & 127, fresh);
         const uint32_t see = !valid ? 0u : (fresh >= 0 ? see_new : 0xffffffffu);
         if (ok) ok = wait_warp(bar(R::B_S + (c & 1)), (c >> 1) & 1, ctl, 78);
         tc_fence_after();
         float e[N];
         tmem_ld_cols<N>(tmS + lane_base + (c & 1) * N, e);
         tmem_wait_ld();
-        if (!full) {
+        if constexpr (!full) {
 #pragma unroll
           for (int i = 0; i < N; ++i) {
             const int dt = fresh >= 0 ? static_cast<int>(p.by_gt.div(i)) : 0;
@@ -313,7 +317,7 @@ __device__ __forceinline__ void sh_columns(const AttendParams& p, const WalkOf<M
         const bool grew = __any_sync(0xffffffffu, move);  // the same in all warps
         __syncwarp();
         if (c > 0 && ok) ok = wait_warp(bar(R::B_PV), (c - 1) & 1, ctl, 80);  // P and O are free
-        if (grew && c > c0) {
+        if (__builtin_expect(grew && c > c0, 0)) {
           // sums and O of the earlier tiles, to the new maxima
           tc_fence_after();
 #pragma unroll
@@ -349,14 +353,18 @@ __device__ __forceinline__ void sh_columns(const AttendParams& p, const WalkOf<M
                        "r"(pack16<BF16>(e[i + 2], e[i + 3])), "r"(pack16<BF16>(e[i + 4], e[i + 5])), "r"(pack16<BF16>(e[i + 6], e[i + 7]))
                        : "memory");
         }
-        if (!full) {
+        if constexpr (!full) {
           if (ok) ok = wait_warp(bar(R::B_KV + R::v_stage(c)), R::v_turn(c) & 1, ctl, 82);
           if (sh_clean<R, BF16>(x.sKV + R::v_stage(c) * R::STAGE, tid & 127, valid, fresh >= 0)) ac.odd[0] = s + 1;
         }
         fence_async_smem();
         tc_fence_before();
         mbar_arrive(bar(R::B_P));
-      }
+      };
+#pragma unroll 1
+      for (int t = 0; t < min(t_full, tiles); ++t, ++c) tile(std::false_type{}, t);
+#pragma unroll 1
+      for (int t = t_full; t < tiles; ++t, ++c) tile(std::true_type{}, t);
       // ---- the segment's end ----
       const ShOut to(p, w, x.half);
       columns_over_lanes<N>(l, lane);
@@ -444,6 +452,7 @@ __device__ __forceinline__ void sh_rows(const AttendParams& p, const WalkOf<MODE
         p, first, 0, x.bar0, ac,
         [&](const AttTile& t, int c, int) {
           const uint32_t q_lo = sdesc_lo(x.sQ + (t.s % R::NQ) * R::Q_BYTES, 16), k_lo = sdesc_lo(x.sKV + R::k_stage(t.T) * R::STAGE, 16);
+#pragma unroll 2
           for (int kk = 0; kk < k_steps; ++kk)
             umma_ss_lead(lead, tS + 64 * (c & 1), q_lo + (((kk >> 2) * R::Q_CHUNK + (kk & 3) * 32) >> 4),
                          k_lo + (((kk >> 2) * R::CHUNK + (kk & 3) * 32) >> 4), IDESC_S, kk > 0 ? 1u : 0u);
@@ -479,11 +488,11 @@ __device__ __forceinline__ void sh_rows(const AttendParams& p, const WalkOf<MODE
       const int t_full = max(min(w.n, min(w.len / ATT_UNIT, w.uc) - w.unit), 0) / R::UNITS;  // tiles below hold cached keys only
       float2 e[32];
       bool loaded = false;
-#pragma unroll 1
-      for (int t = 0; t < tiles; ++t, ++c) {
-        const bool full = t < t_full;
+      // (The masked tiles, an item's last ones, have code of their own: it does not share the instruction cache with the loop over the others.)
+      auto tile = [&](auto masked, int t) {
+        constexpr bool full = !decltype(masked)::value;
         uint32_t seen[2] = {0xffffffffu, 0xffffffffu};
-        if (!full) {
+        if constexpr (!full) {
           const int ub = w.unit + R::UNITS * t;
           seen[0] = exists ? seen_word(p, w, ub, tk) : 0u;
           seen[1] = exists ? seen_word(p, w, ub + 1, tk) : 0u;
@@ -494,7 +503,7 @@ __device__ __forceinline__ void sh_rows(const AttendParams& p, const WalkOf<MODE
           tmem_ld_cols<64>(tS + 64 * (c & 1), reinterpret_cast<float*>(e));
           tmem_wait_ld();
         }
-        if (!full) {
+        if constexpr (!full) {
 #pragma unroll
           for (int j = 0; j < 32; ++j) {
             if (!((seen[j / 16] >> (2 * j & 31)) & 1u)) e[j].x = -INFINITY;
@@ -507,19 +516,19 @@ __device__ __forceinline__ void sh_rows(const AttendParams& p, const WalkOf<MODE
         const float top = fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3]));
         m_top = fmaxf(m_top, top);
         const bool move = m_ref == -INFINITY ? top > -INFINITY : top > m_ref + p.slack;
-        if (__any_sync(0xffffffffu, move)) {
+        if (__builtin_expect(__any_sync(0xffffffffu, move), 0)) {
           const float alpha = !move ? 1.f : (m_ref == -INFINITY ? 0.f : ex2((m_ref - top) * c_log2));
           if (t > 0) {  // every product issued so far has to have retired
             if (ok) ok = wait_warp(bar(R::B_PV + ((c - 1) & 1)), ((c - 1) >> 1) & 1, ctl, 79);
             tc_fence_after();
-#pragma unroll
-            for (int k = 0; k < D; k += 32) {
-              float o[32];
-              tmem_ld32(tO + k, reinterpret_cast<uint32_t*>(o));
+#pragma unroll 1
+            for (int k = 0; k < D; k += 16) {
+              float o[16];
+              tmem_ld16(tO + k, reinterpret_cast<uint32_t*>(o));
               tmem_wait_ld();
 #pragma unroll
-              for (int j = 0; j < 32; ++j) o[j] *= alpha;
-              tmem_st32(tO + k, reinterpret_cast<const uint32_t*>(o));
+              for (int j = 0; j < 16; ++j) o[j] *= alpha;
+              tmem_st16(tO + k, reinterpret_cast<const uint32_t*>(o));
             }
             tmem_wait_st();
             l *= alpha;
@@ -544,7 +553,7 @@ __device__ __forceinline__ void sh_rows(const AttendParams& p, const WalkOf<MODE
         }
         const bool early = mbar_test(bar(R::B_S + ((c + 1) & 1)), ((c + 1) >> 1) & 1);  // the next tile's scores are there already
         l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
-        if (!full) {
+        if constexpr (!full) {
           // (The tile before has to be done with: until then the barrier of this one's stage may be a turn behind.)
           if (c > 0 && ok) ok = wait_warp(bar(R::B_PV + ((c - 1) & 1)), ((c - 1) >> 1) & 1, ctl, 81);
           if (ok) ok = wait_warp(bar(R::B_KV + R::v_stage(c)), R::v_turn(c) & 1, ctl, 82);
@@ -571,7 +580,11 @@ __device__ __forceinline__ void sh_rows(const AttendParams& p, const WalkOf<MODE
         } else {
           announce();
         }
-      }
+      };
+#pragma unroll 1
+      for (int t = 0; t < min(t_full, tiles); ++t, ++c) tile(std::false_type{}, t);
+#pragma unroll 1
+      for (int t = t_full; t < tiles; ++t, ++c) tile(std::true_type{}, t);
       // ---- the segment's end ----
       const ShOut to(p, w, x.half);
       const long long at = exists ? to.row(p, r, sq, h, tk) : -1;
