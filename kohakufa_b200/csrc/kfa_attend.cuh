@@ -261,13 +261,6 @@ __device__ __forceinline__ bool mbar_suspend(uint32_t bar, uint32_t parity) {
     return ok != 0;
   }
 }
-// Suspended until the phase is over, or for about 100 ns.
-__device__ __forceinline__ void mbar_nap(uint32_t bar, uint32_t parity) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.try_wait.parity.shared::cta.b64 p, [%0], %1, %2;\n\t}" ::"r"(bar), "r"(parity), "r"(100u)
-      : "memory");
-}
 __device__ __forceinline__ bool wait_warp(uint32_t bar, uint32_t parity, const Ctl& ctl, int site) {
   bool ok = mbar_suspend(bar, parity);
   if (__builtin_expect(__all_sync(0xffffffffu, ok), 1)) return true;
@@ -290,9 +283,8 @@ __device__ __forceinline__ bool wait_warp(uint32_t bar, uint32_t parity, const C
 template <int NC_, int Q_ROWS_, int NQ_, bool BOTH_, int OTHER_>
 struct AttRings {
   static constexpr int NC = NC_, Q_ROWS = Q_ROWS_, NQ = NQ_;
-  static constexpr bool BOTH = BOTH_, ALL = BOTH_;  // ALL: a stream sees every tile
-  static constexpr bool SUSPEND = false;            // whether the issuing warps suspend where there is nothing to issue
-  static constexpr int UNITS = 4;                   // of a tile
+  static constexpr bool BOTH = BOTH_, KEYS_FIRST = false;  // KEYS_FIRST: whether the first values wait for the first keys
+  static constexpr int UNITS = 4;                          // of a tile
   static constexpr int CHUNK = 128 * 64 * 2;  // 128 keys x 64 columns
   static constexpr int STAGE = NC * CHUNK;
   static constexpr int Q_CHUNK = Q_ROWS * 128, Q_BYTES = NC * Q_CHUNK;
@@ -504,6 +496,8 @@ __device__ __forceinline__ void att_produce(const AttendParams& p, const WalkOf<
   const int per_unit = ATT_UNIT / p.box, boxes = R::UNITS * per_unit;
   bool ok = true, more = true;
   int T = 0, s = 0;  // tiles and segments so far
+  // (At the start all CTAs ask for all that their rings hold: the first keys, which everything waits for, go ahead of the values.)
+  if (R::KEYS_FIRST && values) ok = wait_warp(bar(R::B_KV + R::k_stage(0)), 0, ctl, 77);
   while (more && ok) {
     const RowMapOf<MODE> rows(p, w.b, w.item);
     if (lane == 0 && !length_ok(p.c, w.b)) *ac.bad = 1;
@@ -595,15 +589,10 @@ struct AttTiles {
 // values of piece i - 2 have been issued, values of piece j as soon as P and V are there, whichever comes first: neither holds the other up
 // (keys that are late would delay values whose results others wait for). PIECES of a tile: 1, or 2 halves of 64 keys.
 // issue_S(tile, c, piece), issue_PV(tile, c, piece) issue and commit; c counts the stream's tiles.
-template <class R, int PIECES, int NP, class W, typename FS, typename FP>
-__device__ __forceinline__ void att_issue(const AttendParams& p, const W& first, int st, uint32_t bar0, const AttCtl& ac, FS issue_S, FP issue_PV) {
-  uint32_t held = 0, held_parity = 0;  // what the last test failed at
-  auto ready = [&](int i, uint32_t parity) {
-    const bool there = __all_sync(0xffffffffu, mbar_test(bar0 + 8u * i, parity));
-    if (R::SUSPEND && !there) held = bar0 + 8u * i, held_parity = parity;
-    return there;
-  };
-  AttTiles<R::ALL, R::UNITS, W> tiles{first, st};
+template <class R, int PIECES, int NP, typename FS, typename FP>
+__device__ __forceinline__ void att_issue(const AttendParams& p, const Walk& first, int st, uint32_t bar0, const AttCtl& ac, FS issue_S, FP issue_PV) {
+  auto ready = [&](int i, uint32_t parity) { return __all_sync(0xffffffffu, mbar_test(bar0 + 8u * i, parity)); };
+  AttTiles<R::BOTH> tiles{first, st};
   AttTile ahead = {0, 0, 0, false, false}, even = ahead, odd = ahead;  // the next to get scores; those that have, by c (at most two wait for values)
   bool have = tiles.take(p, ahead);
   int i_s = 0, i_p = 0;  // pieces of scores and of values issued
@@ -648,8 +637,6 @@ __device__ __forceinline__ void att_issue(const AttendParams& p, const W& first,
     } else if (clock64() - t0 > KFA_WAIT_CYCLES) {
       *ac.abort = KFA_DEV_TIMEOUT_BASE + 73;
       break;
-    } else if (R::SUSPEND) {  // (a warp that polls takes issue slots from those that compute)
-      mbar_nap(held, held_parity);
     }
   }
   // what was issued has retired before tensor memory is freed

@@ -5,7 +5,7 @@
 namespace {
 
 int64_t padded(int64_t bytes) { return (bytes + 255) / 256 * 256; }
-int matrix_rows(int64_t rows) { return rows <= 16 ? 16 : (rows <= 32 ? 32 : 128); }
+int matrix_rows(int64_t rows) { return rows <= 16 ? 16 : (rows <= 32 ? 32 : (rows <= 128 ? 128 : 256)); }
 
 // How a call is cut up: a function of the shapes alone, so that the scratch it needs is known beforehand.
 struct SharedPlan {
@@ -25,16 +25,19 @@ SharedPlan plan_shared(int64_t batch, int64_t heads, int64_t kv_heads, int64_t T
   a.tt = static_cast<int>(tt);
   a.head_tiles = static_cast<int>((group + gt - 1) / gt);
   a.row_tiles = static_cast<int>(a.head_tiles * token_tiles);
-  // Sequences of a prefix' row tile: what 128 rows hold, of one prefix in equal parts. How many each prefix has only the device knows: where they are
+  // Sequences of a prefix' row tile: what 256 rows hold (128, where all fit), of one prefix in equal parts. How many each prefix has only the device knows: where they are
   // many the tile is made for twice their mean number.
-  int64_t ts = token_tiles == 1 ? std::max<int64_t>(128 / per, 1) : 1;
-  const int64_t mean = (batch + prefixes - 1) / prefixes;
-  ts = std::min(ts, prefixes == 1 ? batch : std::min(batch, 2 * mean));
+  const int64_t mean = (batch + prefixes - 1) / prefixes, wanted = prefixes == 1 ? batch : std::min(batch, 2 * mean);
+  int64_t ts = 1;
+  if (token_tiles == 1) {  // (tiles of 256 rows where they are no more CTAs than those of 128, two in one)
+    const int64_t half = std::max<int64_t>(128 / per, 1), whole = std::max<int64_t>(256 / per, 1), n = prefixes == 1 ? batch : mean;
+    ts = std::min((n + half - 1) / half < 2 * ((n + whole - 1) / whole) ? half : whole, wanted);
+  }
   if (prefixes == 1) ts = (batch + (batch + ts - 1) / ts - 1) / ((batch + ts - 1) / ts);
   a.ts = static_cast<int>(ts);
   a.n_own = matrix_rows(per);
   a.n_pre = std::max(matrix_rows(per * ts), a.n_own);
-  a.extra_pre = a.n_pre == 128 ? 8 : 6;
+  a.extra_pre = a.n_pre >= 128 ? 8 : 6;
   a.extra_own = a.n_own == 128 ? 8 : 6;
   const int64_t pre_items = kv_heads * a.row_tiles * ((batch + ts - 1) / ts + prefixes - 1), own_items = batch * kv_heads * a.row_tiles;
   const int64_t pre_units = std::max<int64_t>((prefix_room + 31) / 32, 1);
@@ -45,7 +48,7 @@ SharedPlan plan_shared(int64_t batch, int64_t heads, int64_t kv_heads, int64_t T
   const auto ctas = [](int64_t items, int64_t units) { return (std::min<int64_t>(items, 2 * SMS) * ((units + 3) / 4) + 1) / 2; };
   a.grid = static_cast<int>(std::min<int64_t>(SMS, ctas(pre_items, pre_units) + ctas(own_items, own_units)));
   const int64_t rows = batch * heads * T;
-  const int r = std::max(a.n_pre, a.n_own);
+  const int r = std::min(std::max(a.n_pre, a.n_own), 128);
   int64_t at = 0;
   auto take = [&](int64_t bytes) {
     const int64_t here = at;
@@ -75,7 +78,7 @@ void fill_part(kfa::AttendParams& p, const SharedPlan& plan, bool pre, int64_t b
   p.by_head_tiles = kfa::FastDiv::by(p.head_tiles);
   p.least = 4;
   p.extra = pre ? plan.extra_pre : plan.extra_own;
-  p.rows = std::max(plan.n_pre, plan.n_own);
+  p.rows = std::min(std::max(plan.n_pre, plan.n_own), 128);
   p.box = page_box(p.c);
   p.seqs = static_cast<int>(batch);
   p.ts = plan.ts;
@@ -93,7 +96,8 @@ template <int NC, int N_PRE, int N_OWN, bool BF16>
 int launch_shared(const CUtensorMap (&m)[8], const kfa::SharedParams& p, const SharedPlan& plan, cudaStream_t s) {
   auto kern = kfa::kfa_shared_kernel<NC, N_PRE, N_OWN, BF16>;
   constexpr int SMEM = 2 * kfa::SH_SMEM + 1024;
-  static_assert(std::max(kfa::ShCfg<NC, N_PRE>::SMEM, kfa::ShCfg<NC, N_OWN>::SMEM) <= kfa::SH_SMEM && SMEM <= 232448, "shared memory");
+  static_assert(kfa::ShCfg<NC, N_PRE>::SMEM <= (N_PRE == 256 ? 2 : 1) * kfa::SH_SMEM && kfa::ShCfg<NC, N_OWN>::SMEM <= kfa::SH_SMEM && SMEM <= 232448,
+                "shared memory");
   static std::atomic<uint64_t> allowed{0};
   int rc = allow_smem(allowed, reinterpret_cast<const void*>(kern), SMEM);
   if (rc) return rc;
@@ -104,8 +108,12 @@ int launch_shared(const CUtensorMap (&m)[8], const kfa::SharedParams& p, const S
 
 template <int NC, bool BF16>
 int launch_shared_rows(const CUtensorMap (&m)[8], const kfa::SharedParams& p, const SharedPlan& plan, cudaStream_t s) {
-  if (plan.n_own == 128) return launch_shared<NC, 128, 128, BF16>(m, p, plan, s);
-  if (plan.n_own == 32) return plan.n_pre == 128 ? launch_shared<NC, 128, 32, BF16>(m, p, plan, s) : launch_shared<NC, 32, 32, BF16>(m, p, plan, s);
+  if (plan.n_own == 128) return plan.n_pre == 256 ? launch_shared<NC, 256, 128, BF16>(m, p, plan, s) : launch_shared<NC, 128, 128, BF16>(m, p, plan, s);
+  if (plan.n_own == 32) {
+    if (plan.n_pre == 256) return launch_shared<NC, 256, 32, BF16>(m, p, plan, s);
+    return plan.n_pre == 128 ? launch_shared<NC, 128, 32, BF16>(m, p, plan, s) : launch_shared<NC, 32, 32, BF16>(m, p, plan, s);
+  }
+  if (plan.n_pre == 256) return launch_shared<NC, 256, 16, BF16>(m, p, plan, s);
   if (plan.n_pre == 128) return launch_shared<NC, 128, 16, BF16>(m, p, plan, s);
   return plan.n_pre == 32 ? launch_shared<NC, 32, 16, BF16>(m, p, plan, s) : launch_shared<NC, 16, 16, BF16>(m, p, plan, s);
 }
@@ -151,8 +159,9 @@ int kfa_cache_attend_shared(const KfaTensor4* q, const KfaCache* prefix, const i
   pre.carry_rows = own.carry_rows = rows;
   fill_part(pre, plan, true, batch, scratch);
   fill_part(own, plan, false, batch, scratch);
-  p.rows = pre.rows;
-  p.weight = 1.f;
+  p.pre_pair = plan.n_pre == 256;
+  p.pre_items = pre.c.batch == 1 && !starts ? static_cast<int>(own.c.heads * plan.row_tiles * ((batch + plan.ts - 1) / plan.ts)) : 0;
+  p.weight = p.pre_pair ? 1.f : 0.5f;
   CUtensorMap m[8];
   auto queries = [&](int ts, CUtensorMap* map) {
     return make_box_map(q->ptr, D, own.H, q->stride[1], own.T, q->stride[2], batch, q->stride[0], plan.gt, plan.tt, ts, dtype, map, "q");

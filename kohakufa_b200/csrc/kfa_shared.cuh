@@ -11,6 +11,10 @@
 // brings; a prefix is read once for each of them, out of L2 but the first time.
 // (64 sequences behind 8192 positions, 1 to 1024 of their own, 32 / 8 heads, one token: the prefix first, its join, then the own part took 76 us.)
 //
+// More than 128 rows of a prefix: a tile has up to 256, half of them in each half of the CTA, which share its keys and values. (They are
+// copied once a CTA then: two halves with tiles of their own ask L2 for 30 bytes a clock and SM.) Where there is one prefix, the row tiles of a K / V head are cut at the same
+// keys, and CTAs that run together read the same.
+//
 // What a part leaves is fp32: O before the division, m, l and the largest score per row. Items that one CTA has whole go to the carry, rows (sequence,
 // head, token); parts of cut ones to the CTA's slots; the item's entry in a directory says which. A second kernel gives every row a warp, which
 // takes its prefix' parts and its own in the order of the keys: results repeat bit for bit.
@@ -37,24 +41,26 @@ constexpr int SH_TMEM = 256;  // columns of a half
 
 struct SharedParams {
   AttendParams pre, own;
-  float weight;  // what a unit of the prefixes counts beside one of the sequences' own
-  int rows;      // of scratch per part
+  float weight;   // what a unit of the prefixes, of a CTA, counts beside one of the sequences' own, of a half
+  int pre_items;  // where there is one prefix: its items; else 0
+  int pre_pair;   // whether a prefix' row tile takes both halves of a CTA
 };
 
-// Shared memory and barriers of a half, whichever work it has: 1 KB of barriers and control, then its rings.
+// Shared memory and barriers of a half, whichever work it has: 1 KB of barriers and control, then its rings. N = 256: of the whole CTA, whose first half
+// has the rings and their barriers.
 template <int NC_, int N>
 struct ShCfg {
   static constexpr int NC = NC_;
-  static constexpr bool ROWS = N == 128, ALL = true, SUSPEND = true;
+  static constexpr bool ROWS = N >= 128, PAIR = N == 256, KEYS_FIRST = true;
   static constexpr int KEYS = ROWS ? 64 : 128, UNITS = KEYS / ATT_UNIT;
   static constexpr int CHUNK = KEYS * 128, STAGE = NC * CHUNK;  // KEYS keys x 64 columns
   static constexpr int Q_CHUNK = N * 128, Q_BYTES = NC * Q_CHUNK, NQ = ROWS ? 1 : 2;
   static constexpr int NP = ROWS ? 2 : 1;                  // buffers for P
   static constexpr int P_BYTES = ROWS ? 0 : 128 * N * 2;   // in shared memory
   // column maxima of two tiles, shifts, sums and maxima of two segments; rows on their way out
-  static constexpr int OTHER = ROWS ? 4 * 2048 : (2 * 4 * N + 4 * N + 2 * 6 * N) * 4;
-  static constexpr int FIXED = 2048 + NQ * Q_BYTES + P_BYTES + OTHER;
-  static constexpr int FIT = (SH_SMEM - FIXED) / STAGE;
+  static constexpr int OTHER = ROWS ? (PAIR ? 8 : 4) * 2048 : (2 * 4 * N + 4 * N + 2 * 6 * N) * 4;
+  static constexpr int FIXED = (PAIR ? 3072 : 2048) + NQ * Q_BYTES + P_BYTES + OTHER;
+  static constexpr int FIT = ((PAIR ? 2 * SH_SMEM : SH_SMEM) - FIXED) / STAGE;
   static constexpr int DV = FIT / 2 < 4 ? FIT / 2 : 4;
   static constexpr int DK = FIT - DV < 4 ? FIT - DV : 4;
   static_assert(DV >= 1 && DK >= 1, "no room for a tile of keys and one of values");
@@ -87,13 +93,28 @@ __device__ __forceinline__ int sh_counted(const AttendParams& p, int b) {
   return b < p.c.batch ? (W::units_of(p, b) + p.extra) * W::items_of(p, b) : 0;
 }
 
-// The stretch of half `index` of `count` that share this work, `total` as it is counted. s_i: 32 ints of shared memory. Synchronises the CTA, whose halves
-// both come here.
+// The stretch of half (or CTA) `index` of `count` that share this work, `total` as it is counted. s_i: 32 ints of shared memory. Synchronises the CTA,
+// whose halves both come here. split: of one prefix: every item is cut into so many stretches; 0: all stretches have the same length.
 template <int MODE>
-__device__ __forceinline__ bool sh_work(const AttendParams& p, int* s_i, int index, int count, int total, WalkOf<MODE>& w, int& chunk, int& end) {
+__device__ __forceinline__ bool sh_work(const AttendParams& p, int* s_i, int index, int count, int total, int split, WalkOf<MODE>& w, int& chunk,
+                                        int& end) {
   using W = WalkOf<MODE>;
   const int tid = threadIdx.x & (SH_THREADS - 1), warp = tid >> 5, lane = tid & 31;
   chunk = max((total + count - 1) / count, p.least);
+  if (split > 0) {
+    const int items = W::items_of(p, 0), each = total / items, k = index % split;
+    auto unit = [&](int i) { return max(static_cast<int>(static_cast<long long>(each) * i / split) - p.extra, 0); };
+    w.b = 0;
+    w.item = index / split;
+    w.unit = unit(k);
+    w.end_b = 0;
+    w.end_item = k + 1 < split ? w.item : w.item + 1;
+    w.end_unit = k + 1 < split ? unit(k + 1) : 0;
+    if (w.end_item == items) w.end_b = p.c.batch, w.end_item = 0;
+    end = 0;
+    __syncthreads();
+    return w.item < items && w.start(p);
+  }
   const int at[2] = {chunk * index, chunk * index + chunk};
   end = at[1];
   int before = 0;
@@ -137,6 +158,35 @@ __device__ __forceinline__ bool sh_work(const AttendParams& p, int* s_i, int ind
   return w.b < p.c.batch && w.start(p);
 }
 
+// How many CTAs the prefixes' work gets, and into how many stretches each of its items is cut (0: wherever stretches end).
+template <bool PAIR>
+__device__ __forceinline__ void sh_share(const SharedParams& p, int total_pre, int total_own, int grid, int& pre_ctas, int& split) {
+  split = 0;
+  const float pre = total_pre * p.weight, own = 0.5f * total_own;  // a CTA's time for all of it (own: two halves work at once)
+  const float most = static_cast<float>(grid - 1);                 // (the own work is never nothing)
+  pre_ctas = total_pre == 0 ? 0 : static_cast<int>(fminf(fmaxf(grid * pre / (pre + own) + 0.5f, 1.f), most));
+  if (total_pre == 0 || p.pre_items == 0) return;
+  // one prefix: so many stretches an item that what ends last ends first
+  const float per = PAIR ? 1.f : 0.5f;  // CTAs of a stretch
+  const float ideal = pre_ctas / (per * p.pre_items);
+  float best = 0.f;
+  const int each = total_pre / p.pre_items;  // (a stretch has a unit at least)
+  for (int s = max(static_cast<int>(ideal), 1); s <= min(static_cast<int>(ideal) + 1, max(each / p.pre.least, 1)); ++s) {
+    const float ctas = ceilf(s * per * p.pre_items);
+    if (ctas > most) break;
+    const float time = fmaxf(pre / (s * per * p.pre_items), own / (grid - ctas));
+    if (split == 0 || time < best) {
+      best = time;
+      split = s;
+      pre_ctas = static_cast<int>(ctas);
+    }
+  }
+  if (split > 0 && ideal < 0.8f) {  // fewer CTAs than items: cut where stretches end
+    split = 0;
+    pre_ctas = static_cast<int>(fminf(fmaxf(grid * pre / (pre + own) + 0.5f, 1.f), most));
+  }
+}
+
 // Where a segment's rows go: the carry, or one of the half's two slots of parts.
 struct ShOut {
   float* o;       // rows of 128
@@ -158,9 +208,10 @@ struct ShOut {
 
 struct ShHalf {
   uint32_t sKV, sQ, sP, bar0, tmem;
+  uint32_t ring0;       // the barriers of keys, values and queries (of a pair: the first half's)
   uint8_t* other;       // OTHER bytes
-  int half, index;      // among all halves, among those that have this kind of work
-  int chunk, end;       // see sh_work
+  int half, index;      // among all halves; among those (of a pair: the CTAs) that have this kind of work
+  int chunk, end, split;  // see sh_work
   int *kv_issued, *q_issued;
   __device__ __forceinline__ void meet() const { asm volatile("bar.sync %0, 128;" ::"r"(1 + (half & 1)) : "memory"); }  // of the softmax warps
 };
@@ -170,7 +221,7 @@ template <int MODE, class W>
 __device__ __forceinline__ void sh_note(const AttendParams& p, const W& w, const RowMapOf<MODE>& rows, const ShHalf& x) {
   if (!w.begins()) return;
   int parts = 0;
-  if (!w.ends()) parts = (x.end - w.n + w.units - 1) / x.chunk - x.index + 1;
+  if (!w.ends()) parts = x.split > 0 ? x.split - x.index % x.split : (x.end - w.n + w.units - 1) / x.chunk - x.index + 1;
   p.dir[(static_cast<long long>(rows.g) * p.row_tiles + rows.rt) * p.seqs + rows.s0] = make_int2(x.half, parts);
 }
 
@@ -203,6 +254,70 @@ __device__ __forceinline__ bool sh_clean(uint32_t stage, int key, bool valid, bo
   return odd;
 }
 
+// Suspended until the phase is over, or for about 100 ns.
+__device__ __forceinline__ void mbar_nap(uint32_t bar, uint32_t parity) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%0], %1, %2;\n\t}" ::"r"(bar), "r"(parity), "r"(100u)
+      : "memory");
+}
+// The issuing warps' loop: see att_issue. Scores of tile i as soon as their keys (and queries) are there and the values of tile i - 2 have been issued, values
+// of tile j as soon as P and V are there, whichever comes first. Where nothing can go the warp is suspended: one that polls takes issue slots from those that
+// compute.
+template <class R, class W, typename FS, typename FP>
+__device__ __forceinline__ void sh_issue(const AttendParams& p, const W& first, const ShHalf& x, const AttCtl& ac, FS issue_S, FP issue_PV) {
+  uint32_t held = 0, held_parity = 0;  // what the last test failed at
+  auto ready = [&](uint32_t bar, uint32_t parity) {
+    const bool there = __all_sync(0xffffffffu, mbar_test(bar, parity));
+    if (!there) held = bar, held_parity = parity;
+    return there;
+  };
+  auto ring = [&](int i) { return x.ring0 + 8u * i; };
+  auto bar = [&](int i) { return x.bar0 + 8u * i; };
+  AttTiles<true, R::UNITS, W> tiles{first, 0};
+  AttTile ahead = {0, 0, 0, false, false}, even = ahead, odd = ahead;  // the next to get scores; those that have, by tile (at most two wait for values)
+  bool have = tiles.take(p, ahead);
+  int i_s = 0, i_p = 0;  // tiles whose scores and whose values are issued
+  long long t0 = clock64();
+  while (have || i_p < i_s) {
+    bool went = false;
+    if (have && i_s <= i_p + 1 && ready(ring(R::B_KV + R::k_stage(ahead.T)), R::k_turn(ahead.T) & 1) &&
+        (!ahead.opens || ready(ring(R::B_Q + ahead.s % R::NQ), (ahead.s / R::NQ) & 1))) {
+      tc_fence_after();
+      issue_S(ahead, i_s);
+      if (i_s & 1) odd = ahead;
+      else even = ahead;
+      ++i_s;
+      went = true;
+      have = tiles.take(p, ahead);
+    }
+    if (i_p < i_s) {
+      const AttTile now = (i_p & 1) ? odd : even;
+      if (ready(bar(R::B_P + i_p % R::NP), (i_p / R::NP) & 1) && ready(ring(R::B_KV + R::v_stage(now.T)), R::v_turn(now.T) & 1) &&
+          (!now.opens || now.uses == 0 || ready(bar(R::B_OFREE), (now.uses - 1) & 1))) {
+        tc_fence_after();
+        issue_PV(now, i_p);
+        ++i_p;
+        went = true;
+      }
+    }
+    if (went) {
+      t0 = clock64();
+    } else if (*ac.abort != 0) {
+      break;
+    } else if (clock64() - t0 > KFA_WAIT_CYCLES) {
+      *ac.abort = KFA_DEV_TIMEOUT_BASE + 73;
+      break;
+    } else {
+      mbar_nap(held, held_parity);
+    }
+  }
+  // what was issued has retired before tensor memory is freed
+  const bool lead = elect_one();
+  umma_commit_lead(lead, bar(R::B_DRAIN));
+  mbar_drain(bar(R::B_DRAIN), 0);
+}
+
 // ---- up to 32 rows: keys as matrix rows ---------------------------------------------------------------------------------------
 template <int NC, int N, bool BF16, int MODE>
 __device__ __forceinline__ void sh_columns(const AttendParams& p, const WalkOf<MODE>& first, const ShHalf& x, const AttCtl& ac, const CUtensorMap* tmQ,
@@ -224,9 +339,9 @@ __device__ __forceinline__ void sh_columns(const AttendParams& p, const WalkOf<M
     constexpr uint32_t IDESC_S = make_idesc(BF16, false, 128, N), IDESC_O = make_idesc(BF16, true, 128, N) | (1u << 15);
     constexpr uint32_t HI_P = sdesc_hi_for(N);
     const int k_steps = (p.c.cols + 15) / 16;
-    att_issue<R, 1, R::NP>(
-        p, first, 0, x.bar0, ac,
-        [&](const AttTile& t, int c, int) {
+    sh_issue<R>(
+        p, first, x, ac,
+        [&](const AttTile& t, int c) {
           const uint32_t k_lo = sdesc_lo(x.sKV + R::k_stage(t.T) * R::STAGE, 16), q_lo = sdesc_lo(x.sQ + (t.s % R::NQ) * R::Q_BYTES, 16);
 #pragma unroll 2
           for (int kk = 0; kk < k_steps; ++kk)
@@ -236,7 +351,7 @@ __device__ __forceinline__ void sh_columns(const AttendParams& p, const WalkOf<M
           umma_commit_lead(lead, bar(R::B_KVFREE + R::k_stage(t.T)));
           if (t.closes) umma_commit_lead(lead, bar(R::B_QFREE + t.s % R::NQ));
         },
-        [&](const AttTile& t, int, int) {
+        [&](const AttTile& t, int) {
           // (64 columns or fewer: the matrix' rows 64 .. 127 repeat the first ones, and nobody reads them)
           const uint32_t v_lo = sdesc_lo(x.sKV + R::v_stage(t.T) * R::STAGE, NC == 2 ? R::CHUNK : 0), p_lo = sdesc_lo(x.sP, 16);
 #pragma unroll 2
@@ -428,17 +543,19 @@ __device__ __forceinline__ void sh_columns(const AttendParams& p, const WalkOf<M
 // ---- more rows: rows as matrix rows -------------------------------------------------------------------------------------------
 // Tiles of 64 keys, scores and P in two buffers of 64 columns in turn: P (16-bit) lies over the first 32 columns of its scores, and while one tile's values are
 // multiplied and its next scores made, the threads work on the other's.
-template <int NC, bool BF16, int MODE>
+template <int NC, int N, bool BF16, int MODE>
 __device__ __forceinline__ void sh_rows(const AttendParams& p, const WalkOf<MODE>& first, const ShHalf& x, const AttCtl& ac, const CUtensorMap* tmQ,
                                         const CUtensorMap* tmK, const CUtensorMap* tmV, const CUtensorMap* tmKn, const CUtensorMap* tmVn) {
-  using R = ShCfg<NC, 128>;
+  using R = ShCfg<NC, N>;
+  const int side = R::PAIR ? x.half & 1 : 0;
   constexpr int D = 64 * NC;  // columns of O (those that the head dim does not have are zeros)
   const int tid = threadIdx.x & (SH_THREADS - 1), warp = warp_index() & 7, lane = tid & 31;
   auto bar = [&](int i) { return x.bar0 + 8u * i; };
+  auto ring = [&](int i) { return x.ring0 + 8u * i; };
   const Ctl ctl{ac.abort};
   if (warp > 4) {
     reg_budget<SH_REGS_ISSUE, SH_REGS>();
-    if (warp < 7) {
+    if (warp < 7 && side == 0) {
       const bool values = warp == 6;
       att_produce<R>(p, first, values, x.sKV, x.sQ, x.bar0, ac, tmQ, values ? tmV : tmK, values ? tmVn : tmKn, *x.kv_issued, *x.q_issued);
     }
@@ -448,30 +565,30 @@ __device__ __forceinline__ void sh_rows(const AttendParams& p, const WalkOf<MODE
     constexpr uint32_t IDESC_S = make_idesc(BF16, false, 128, 64), IDESC_O = make_idesc(BF16, true, 128, D);
     const uint32_t tS = x.tmem, tO = x.tmem + 128;
     const int k_steps = (p.c.cols + 15) / 16;
-    att_issue<R, 1, R::NP>(
-        p, first, 0, x.bar0, ac,
-        [&](const AttTile& t, int c, int) {
-          const uint32_t q_lo = sdesc_lo(x.sQ + (t.s % R::NQ) * R::Q_BYTES, 16), k_lo = sdesc_lo(x.sKV + R::k_stage(t.T) * R::STAGE, 16);
+    sh_issue<R>(
+        p, first, x, ac,
+        [&](const AttTile& t, int c) {
+          const uint32_t q_lo = sdesc_lo(x.sQ + (t.s % R::NQ) * R::Q_BYTES + side * 128 * 128, 16), k_lo = sdesc_lo(x.sKV + R::k_stage(t.T) * R::STAGE, 16);
 #pragma unroll 2
           for (int kk = 0; kk < k_steps; ++kk)
             umma_ss_lead(lead, tS + 64 * (c & 1), q_lo + (((kk >> 2) * R::Q_CHUNK + (kk & 3) * 32) >> 4),
                          k_lo + (((kk >> 2) * R::CHUNK + (kk & 3) * 32) >> 4), IDESC_S, kk > 0 ? 1u : 0u);
           umma_commit_lead(lead, bar(R::B_S + (c & 1)));
-          umma_commit_lead(lead, bar(R::B_KVFREE + R::k_stage(t.T)));
-          if (t.closes) umma_commit_lead(lead, bar(R::B_QFREE + t.s % R::NQ));
+          umma_commit_lead(lead, ring(R::B_KVFREE + R::k_stage(t.T)));
+          if (t.closes) umma_commit_lead(lead, ring(R::B_QFREE + t.s % R::NQ));
         },
-        [&](const AttTile& t, int c, int) {
+        [&](const AttTile& t, int c) {
           const uint32_t v_lo = sdesc_lo(x.sKV + R::v_stage(t.T) * R::STAGE, R::CHUNK);
 #pragma unroll
           for (int kk = 0; kk < 4; ++kk)
             umma_ts_lead(lead, tO, tS + 64 * (c & 1) + kk * 8, v_lo + ((kk * 16 * 128) >> 4), IDESC_O, (!t.opens || kk > 0) ? 1u : 0u);
           umma_commit_lead(lead, bar(R::B_PV + (c & 1)));
-          umma_commit_lead(lead, bar(R::B_KVFREE + R::v_stage(t.T)));
+          umma_commit_lead(lead, ring(R::B_KVFREE + R::v_stage(t.T)));
         });
   } else {
     // (After a wait that ran out the role goes on without waiting.)
     reg_budget<SH_REGS_STREAM, SH_REGS>();
-    const int r = tid & 127;  // the thread's row of the tile
+    const int r = tid & 127, tile_row = side * 128 + r;  // the thread's row of the half, of the tile
     const uint32_t lane_base = static_cast<uint32_t>(warp * 32) << 16;
     const uint32_t tS = x.tmem + lane_base, tO = x.tmem + 128 + lane_base;
     const float c_log2 = p.c_log2;
@@ -482,9 +599,9 @@ __device__ __forceinline__ void sh_rows(const AttendParams& p, const WalkOf<MODE
     while (more) {
       const RowMapOf<MODE> rows(p, w.b, w.item);
       int h, tk, sq;
-      const bool exists = rows.row(p, r, h, tk, sq);
+      const bool exists = rows.row(p, tile_row, h, tk, sq);
       float l = 0.f, m_ref = -INFINITY, m_top = -INFINITY;
-      const int tiles = w.template tiles<R::UNITS>(), c0 = c;
+      const int tiles = w.template tiles<R::UNITS>();
       const int t_full = max(min(w.n, min(w.len / ATT_UNIT, w.uc) - w.unit), 0) / R::UNITS;  // tiles below hold cached keys only
       float2 e[32];
       bool loaded = false;
@@ -556,7 +673,7 @@ __device__ __forceinline__ void sh_rows(const AttendParams& p, const WalkOf<MODE
         if constexpr (!full) {
           // (The tile before has to be done with: until then the barrier of this one's stage may be a turn behind.)
           if (c > 0 && ok) ok = wait_warp(bar(R::B_PV + ((c - 1) & 1)), ((c - 1) >> 1) & 1, ctl, 81);
-          if (ok) ok = wait_warp(bar(R::B_KV + R::v_stage(c)), R::v_turn(c) & 1, ctl, 82);
+          if (ok) ok = wait_warp(ring(R::B_KV + R::v_stage(c)), R::v_turn(c) & 1, ctl, 82);
           if (r < R::KEYS) {
             int fresh = -1;
             const bool valid = which_key(w, w.unit + R::UNITS * t, r, fresh);
@@ -588,7 +705,7 @@ __device__ __forceinline__ void sh_rows(const AttendParams& p, const WalkOf<MODE
       // ---- the segment's end ----
       const ShOut to(p, w, x.half);
       const long long at = exists ? to.row(p, r, sq, h, tk) : -1;
-      if (tid == 0) sh_note<MODE>(p, w, rows, x);
+      if (tid == 0 && side == 0) sh_note<MODE>(p, w, rows, x);
       if (exists) {
         to.ml[at] = m_ref;
         to.ml[to.plane + at] = l;
@@ -661,9 +778,9 @@ kfa_shared_kernel(const __grid_constant__ CUtensorMap tmQp, const __grid_constan
   using RO = ShCfg<NC, N_OWN>;
   extern __shared__ uint8_t smem_raw[];
   const int tid = threadIdx.x & (SH_THREADS - 1), warp = warp_index() & 7, lane = tid & 31, side = warp_index() >> 3;
-  const uint32_t base0 = (smem_u32(smem_raw) + 1023u) & ~1023u, base = base0 + side * SH_SMEM;
-  uint8_t *smem0 = smem_raw + (base0 - smem_u32(smem_raw)), *smem = smem0 + side * SH_SMEM;
-  const AttCtl ac(reinterpret_cast<uint64_t*>(smem) + RP::N_BARS);
+  const uint32_t base0 = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  uint8_t* smem0 = smem_raw + (base0 - smem_u32(smem_raw));  // the halves' barriers and control, 1 KB each; what they have of their own, or what both have
+  const AttCtl ac(reinterpret_cast<uint64_t*>(smem0 + 1024 * side) + RP::N_BARS);
   long long* s_sum = reinterpret_cast<long long*>(smem0 + 512);
   uint32_t* s_tmem = reinterpret_cast<uint32_t*>(smem0 + 768);
   if (threadIdx.x == 32 * 7) {
@@ -671,11 +788,11 @@ kfa_shared_kernel(const __grid_constant__ CUtensorMap tmQp, const __grid_constan
   }
   ShHalf x;
   x.half = 2 * static_cast<int>(blockIdx.x) + side;
-  x.bar0 = base;
+  x.bar0 = base0 + 1024 * side;
   if (warp == 5) {
     for (int i = lane; i < RP::N_BARS; i += 32) {
-      const bool streams = (i >= RP::B_P && i < RP::B_PV) || i == RP::B_OFREE;
-      mbar_init(x.bar0 + 8u * i, streams ? 128 : 1);
+      const bool streams = (i >= RP::B_P && i < RP::B_PV) || i == RP::B_OFREE, frees = i >= RP::B_KVFREE || (i >= RP::B_QFREE && i < RP::B_OFREE);
+      if (!frees) mbar_init(x.bar0 + 8u * i, streams ? 128 : 1);
     }
     if (lane == 0) *ac.abort = ac.odd[0] = ac.odd[1] = 0;
     fence_mbar_init();
@@ -700,33 +817,45 @@ kfa_shared_kernel(const __grid_constant__ CUtensorMap tmQp, const __grid_constan
   total_pre = static_cast<int>(both >> 32);
   total_own = static_cast<int>(both & 0xffffffffll);
   const int grid = static_cast<int>(gridDim.x);
-  const float share = total_pre * p.weight / (total_pre * p.weight + total_own);
-  const int pre_ctas = total_pre == 0 ? 0 : min(max(static_cast<int>(grid * share + 0.5f), 1), grid - 1);  // (the own work is never nothing)
+  int pre_ctas, split;
+  sh_share<RP::PAIR>(p, total_pre, total_own, grid, pre_ctas, split);
   const bool pre = static_cast<int>(blockIdx.x) < pre_ctas;
-  x.index = x.half - (pre ? 0 : 2 * pre_ctas);
+  x.index = pre ? (RP::PAIR ? static_cast<int>(blockIdx.x) : x.half) : x.half - 2 * pre_ctas;
+  x.split = pre ? split : 0;
+  if (warp == 5) {  // (Rings that both halves read are freed by both. The others see these barriers behind those of sh_work.)
+    for (int i = lane; i < RP::N_BARS; i += 32)
+      if (i >= RP::B_KVFREE || (i >= RP::B_QFREE && i < RP::B_OFREE)) mbar_init(x.bar0 + 8u * i, RP::PAIR && pre ? 2 : 1);
+    fence_mbar_init();
+    fence_async_smem();
+  }
   WalkOf<ATT_PREFIX> wp;
   WalkOf<ATT_OWN> wo;
   bool work;
-  if (pre) work = sh_work<ATT_PREFIX>(p.pre, ac.ints, x.index, 2 * pre_ctas, total_pre, wp, x.chunk, x.end);
-  else work = sh_work<ATT_OWN>(p.own, ac.ints, x.index, 2 * (grid - pre_ctas), total_own, wo, x.chunk, x.end);
+  if (pre) work = sh_work<ATT_PREFIX>(p.pre, ac.ints, x.index, RP::PAIR ? pre_ctas : 2 * pre_ctas, total_pre, split, wp, x.chunk, x.end);
+  else work = sh_work<ATT_OWN>(p.own, ac.ints, x.index, 2 * (grid - pre_ctas), total_own, 0, wo, x.chunk, x.end);
   let_next_begin();
   tc_fence_after();
   x.tmem = *s_tmem + side * SH_TMEM;
-  x.sKV = base + 1024;
+  x.sKV = base0 + 2048 + side * (SH_SMEM - 1024);
+  x.ring0 = x.bar0;
   int kv_issued = 0, q_issued = 0;
   x.kv_issued = &kv_issued;
   x.q_issued = &q_issued;
   if (work && pre) {
+    if (RP::PAIR) {
+      x.ring0 = base0;
+      x.sKV = base0 + 2048;
+    }
     x.sQ = x.sKV + RP::NS * RP::STAGE;
     x.sP = x.sQ + RP::NQ * RP::Q_BYTES;
-    x.other = smem + (x.sP - base) + RP::P_BYTES;
-    if constexpr (RP::ROWS) sh_rows<NC, BF16, ATT_PREFIX>(p.pre, wp, x, ac, &tmQp, &tmKp, &tmVp, &tmKp, &tmVp);
+    x.other = smem0 + (x.sP - base0) + RP::P_BYTES + (RP::PAIR ? side * 4 * 2048 : 0);
+    if constexpr (RP::ROWS) sh_rows<NC, N_PRE, BF16, ATT_PREFIX>(p.pre, wp, x, ac, &tmQp, &tmKp, &tmVp, &tmKp, &tmVp);
     else sh_columns<NC, N_PRE, BF16, ATT_PREFIX>(p.pre, wp, x, ac, &tmQp, &tmKp, &tmVp, &tmKp, &tmVp);
   } else if (work) {
     x.sQ = x.sKV + RO::NS * RO::STAGE;
     x.sP = x.sQ + RO::NQ * RO::Q_BYTES;
-    x.other = smem + (x.sP - base) + RO::P_BYTES;
-    if constexpr (RO::ROWS) sh_rows<NC, BF16, ATT_OWN>(p.own, wo, x, ac, &tmQ, &tmK, &tmV, &tmKn, &tmVn);
+    x.other = smem0 + (x.sP - base0) + RO::P_BYTES;
+    if constexpr (RO::ROWS) sh_rows<NC, N_OWN, BF16, ATT_OWN>(p.own, wo, x, ac, &tmQ, &tmK, &tmV, &tmKn, &tmVn);
     else sh_columns<NC, N_OWN, BF16, ATT_OWN>(p.own, wo, x, ac, &tmQ, &tmK, &tmV, &tmKn, &tmVn);
   }
 
@@ -772,7 +901,7 @@ __global__ void __launch_bounds__(256) kfa_shared_join_kernel(const __grid_const
   const long long at = (static_cast<long long>(b) * own.H + h) * own.T + t;
   // the row's tile of its own
   int2 mine, before = make_int2(0, -1);  // -1: no prefix
-  int r_own, r_pre = 0;
+  int r_own, r_pre = 0, pair = 0;
   {
     const int th = dh / own.gt, tt = t / own.tt;
     mine = own.dir[(static_cast<long long>(g) * own.row_tiles + tt * own.head_tiles + th) * own.seqs + b];
@@ -798,6 +927,9 @@ __global__ void __launch_bounds__(256) kfa_shared_join_kernel(const __grid_const
     const int ds = static_cast<int>(pre.by_ts.div(max(static_cast<int>(b) - s0, 0))), th = dh / pre.gt, tt = t / pre.tt, first = s0 + ds * pre.ts;
     if (!bad) before = pre.dir[(static_cast<long long>(g) * pre.row_tiles + tt * pre.head_tiles + th) * pre.seqs + first];
     r_pre = ((static_cast<int>(b) - first) * pre.tt + t - tt * pre.tt) * pre.gt + dh - th * pre.gt;
+    pair = p.pre_pair;  // rows 128 .. 255 are the second half's, and a part's CTA has both
+    if (before.y > 0) before.x += r_pre >> 7;
+    r_pre &= 127;
   }
   if (bad) mine = make_int2(0, 0), before = make_int2(0, -1);  // (the directory may not have been written)
   const int n_pre = before.y < 0 ? 0 : max(before.y, 1), n = n_pre + max(mine.y, 1);
@@ -811,7 +943,7 @@ __global__ void __launch_bounds__(256) kfa_shared_join_kernel(const __grid_const
       ml = q.carry_ml + at;
       plane = q.carry_rows;
     } else {
-      const long long slot = 2ll * (d.x + j) + (j == 0 ? 1 : 0);
+      const long long slot = 2ll * (d.x + (i < n_pre && pair ? 2 * j : j)) + (j == 0 ? 1 : 0);
       o = q.part_o + (slot * q.rows + r) * 128;
       ml = q.part_ml + slot * 3 * q.rows + r;
       plane = q.rows;
