@@ -140,8 +140,7 @@ __global__ void __launch_bounds__(ROT_THREADS) kfa_rotary_kernel(const RotaryPar
     second[u] = apart * static_cast<int>(sizeof(T));
     where[u] = (token - token0) << 17 | (turned ? 1u << 16 : 0u) | cell;
     int t = i;
-    bool there = true, placed = false;
-    int page = -1, slot = 0;
+    bool there = true;
     if constexpr (APPEND) {
       there = i < p.r.count(static_cast<int>(seq));
       if (there) {
@@ -150,12 +149,6 @@ __global__ void __launch_bounds__(ROT_THREADS) kfa_rotary_kernel(const RotaryPar
           report(p.status, DEV_BAD_CACHE);
           there = false;
         }
-      }
-      if (there && kind > 0) {
-        const int length = p.c.lengths[seq];
-        const long long pos = static_cast<long long>(length) + i;
-        placed = length >= 0 && pos < p.c.capacity && cache_place(p.c, static_cast<int>(seq), static_cast<int>(pos), page, slot);
-        if (!placed) report(p.status, DEV_BAD_CACHE);
       }
     }
     const int bytes = column * static_cast<int>(sizeof(T));
@@ -166,10 +159,18 @@ __global__ void __launch_bounds__(ROT_THREADS) kfa_rotary_kernel(const RotaryPar
     }
     zero[u] = !there;
     if (x.out != nullptr) to[u][0] = x.out + seq * x.out_b + head * x.out_h + i * x.out_s + bytes;
-    if constexpr (APPEND) {
-      if (placed)
+    if constexpr (APPEND) {  // (looked up behind the rows' loads)
+      if (there && kind > 0) {
+        const int length = p.c.lengths[seq];
+        const long long pos = static_cast<long long>(length) + i;
+        int page = -1, slot = 0;
+        if (length < 0 || pos >= p.c.capacity || !cache_place(p.c, static_cast<int>(seq), static_cast<int>(pos), page, slot)) {
+          report(p.status, DEV_BAD_CACHE);
+          continue;
+        }
         to[u][1] = kind == 1 ? p.c.k + page * p.c.k_sn + head * p.c.k_sh + slot * p.c.k_ss + bytes
                              : p.c.v + page * p.c.v_sn + head * p.c.v_sh + slot * p.c.v_ss + bytes;
+      }
     }
   }
 

@@ -37,8 +37,11 @@ SharedPlan plan_shared(int64_t batch, int64_t heads, int64_t kv_heads, int64_t T
   a.ts = static_cast<int>(ts);
   a.n_own = matrix_rows(per);
   a.n_pre = std::max(matrix_rows(per * ts), a.n_own);
-  a.extra_pre = a.n_pre >= 128 ? 8 : 6;
-  a.extra_own = a.n_own == 128 ? 8 : 6;
+  // What an item's beginning and end count, in units of 32 keys, and in the call below what a unit of the prefixes counts beside one of a sequence's own.
+  // Graph time in us of 7 prefixes of 96 sequences, drafts of 8 tokens, 64 sequences and 256: own items count 6 units more 32.6, 72.1, 50.2, 282; 10 30.2,
+  // 71.0, 50.3, 284; 14 32.8, 70.8, 51.7, 283. With 10, a unit counts 1.0 33.8, 71.0, 50.7, 284; 1.2 30.2, 71.0, 50.3, 284; 1.7 32.6, 70.6, 51.6, 283.
+  a.extra_pre = 8;
+  a.extra_own = 10;
   const int64_t pre_items = kv_heads * a.row_tiles * ((batch + ts - 1) / ts + prefixes - 1), own_items = batch * kv_heads * a.row_tiles;
   const int64_t pre_units = std::max<int64_t>((prefix_room + 31) / 32, 1);
   const int64_t own_units = std::max<int64_t>((room + 31) / 32 + (fresh ? (T + 31) / 32 : 0), 1);
@@ -161,7 +164,7 @@ int kfa_cache_attend_shared(const KfaTensor4* q, const KfaCache* prefix, const i
   fill_part(own, plan, false, batch, scratch);
   p.pre_pair = plan.n_pre == 256;
   p.pre_items = pre.c.batch == 1 && !starts ? static_cast<int>(own.c.heads * plan.row_tiles * ((batch + plan.ts - 1) / plan.ts)) : 0;
-  p.weight = p.pre_pair ? 1.f : 0.5f;
+  p.weight = p.pre_pair ? 1.2f : 0.6f;  // (of a CTA's time: without a pair its halves do two at once)
   CUtensorMap m[8];
   auto queries = [&](int ts, CUtensorMap* map) {
     return make_box_map(q->ptr, D, own.H, q->stride[1], own.T, q->stride[2], batch, q->stride[0], plan.gt, plan.tt, ts, dtype, map, "q");

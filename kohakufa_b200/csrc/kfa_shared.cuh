@@ -61,7 +61,7 @@ struct ShCfg {
   static constexpr int OTHER = ROWS ? (PAIR ? 8 : 4) * 2048 : (2 * 4 * N + 4 * N + 2 * 6 * N) * 4;
   static constexpr int FIXED = (PAIR ? 3072 : 2048) + NQ * Q_BYTES + P_BYTES + OTHER;
   static constexpr int FIT = ((PAIR ? 2 * SH_SMEM : SH_SMEM) - FIXED) / STAGE;
-  static constexpr int DV = FIT / 2 < 4 ? FIT / 2 : 4;
+  static constexpr int DV = (FIT + 1) / 2 < 4 ? (FIT + 1) / 2 : 4;  // (of three stages two: values stay until a tile is done with, keys only until its scores are made)
   static constexpr int DK = FIT - DV < 4 ? FIT - DV : 4;
   static_assert(DV >= 1 && DK >= 1, "no room for a tile of keys and one of values");
   static constexpr int RINGS = 1, NS = DK + DV;
