@@ -64,42 +64,64 @@ void fill_angles(kfa::RotaryParams& p, const KfaRotary* r, bool inverse) {
   p.offset = r->offset;
 }
 
-template <typename T, int BYTES, bool INTERLEAVED, bool APPEND>
+// APPEND: 0: the pass of its own; else into a cache, so many heads a thread.
+template <typename T, int BYTES, bool INTERLEAVED, int APPEND>
 int launch_pieces(kfa::RotaryParams& p, int64_t batch, int64_t heads, int64_t steps, cudaStream_t s) {
   constexpr int V = BYTES / static_cast<int>(sizeof(T));
   const int cells = (p.columns + 2 * V - 1) / (2 * V);  // of a row (half layout: the turned ones and the others are whole cells up to a last single piece)
   p.pair_cells = (p.pairs + V - 1) / V;
-  const int64_t all_tokens = batch * steps, total = all_tokens * heads * cells;
+  constexpr int HEADS = APPEND ? APPEND : 1;
+  constexpr int64_t PER = kfa::ROT_THREADS * (APPEND ? 1 : kfa::ROT_CELLS);  // cells of a CTA
+  const int64_t groups = (heads + HEADS - 1) / HEADS, all_tokens = batch * steps, total = all_tokens * groups * cells;
   if (total > 0xfffff000ll) return fail(KFA_ERR_ARG, "rotary: too many rows in one call");
+  p.heads = static_cast<int>(heads);
   p.by_cell = kfa::FastDiv::by(cells);
-  p.by_head = kfa::FastDiv::by(static_cast<uint32_t>(heads));
+  p.by_group = kfa::FastDiv::by(static_cast<uint32_t>(groups));
   p.by_step = kfa::FastDiv::by(static_cast<uint32_t>(steps));
   p.total = static_cast<unsigned>(total);
-  constexpr int PER = kfa::ROT_THREADS * kfa::ROT_CELLS;
   // tokens that a CTA's stretch of cells can touch
-  const int64_t touched = std::min<int64_t>((PER + heads * cells - 2) / (heads * cells) + 1, all_tokens);
+  const int64_t touched = std::min<int64_t>((PER + groups * cells - 2) / (groups * cells) + 1, all_tokens);
   const int smem = static_cast<int>(touched) * p.pair_cells * V * 8;
-  return launch(kfa::kfa_rotary_kernel<T, BYTES, INTERLEAVED, APPEND>, dim3(static_cast<unsigned>((total + PER - 1) / PER)), kfa::ROT_THREADS, smem, s, p);
+  const dim3 grid(static_cast<unsigned>((total + PER - 1) / PER));
+  if constexpr (APPEND) return launch(kfa::kfa_rotary_append_kernel<T, BYTES, INTERLEAVED, APPEND>, grid, kfa::ROT_THREADS, smem, s, p);
+  else return launch(kfa::kfa_rotary_kernel<T, BYTES, INTERLEAVED>, grid, kfa::ROT_THREADS, smem, s, p);
 }
 
-template <typename T, bool APPEND>
+template <typename T>
 int launch_rotary(kfa::RotaryParams& p, bool interleaved, int piece, int64_t batch, int64_t heads, int64_t steps, cudaStream_t s) {
   if (interleaved) {
-    if constexpr (APPEND) return launch_pieces<T, 16, true, true>(p, batch, heads, steps, s);  // (pages: rows of whole 16 bytes)
-    else
-      switch (piece) {
-        case 16: return launch_pieces<T, 16, true, false>(p, batch, heads, steps, s);
-        case 8: return launch_pieces<T, 8, true, false>(p, batch, heads, steps, s);
-        case 4: return launch_pieces<T, 4, true, false>(p, batch, heads, steps, s);
-        default: return launch_pieces<T, sizeof(T), true, false>(p, batch, heads, steps, s);
-      }
+    switch (piece) {
+      case 16: return launch_pieces<T, 16, true, 0>(p, batch, heads, steps, s);
+      case 8: return launch_pieces<T, 8, true, 0>(p, batch, heads, steps, s);
+      case 4: return launch_pieces<T, 4, true, 0>(p, batch, heads, steps, s);
+      default: return launch_pieces<T, sizeof(T), true, 0>(p, batch, heads, steps, s);
+    }
   }
   switch (piece) {
-    case 16: return launch_pieces<T, 16, false, APPEND>(p, batch, heads, steps, s);
-    case 8: return launch_pieces<T, 8, false, APPEND>(p, batch, heads, steps, s);
-    case 4: return launch_pieces<T, 4, false, APPEND>(p, batch, heads, steps, s);
-    default: return launch_pieces<T, sizeof(T), false, APPEND>(p, batch, heads, steps, s);
+    case 16: return launch_pieces<T, 16, false, 0>(p, batch, heads, steps, s);
+    case 8: return launch_pieces<T, 8, false, 0>(p, batch, heads, steps, s);
+    case 4: return launch_pieces<T, 4, false, 0>(p, batch, heads, steps, s);
+    default: return launch_pieces<T, sizeof(T), false, 0>(p, batch, heads, steps, s);
   }
+}
+
+template <typename T, int HEADS>
+int launch_append(kfa::RotaryParams& p, bool interleaved, int64_t batch, int64_t heads, int64_t steps, cudaStream_t s) {
+  if (interleaved) return launch_pieces<T, 16, true, HEADS>(p, batch, heads, steps, s);  // (tensors and pages: rows of whole 16 bytes)
+  int piece = 16;
+  while (p.pairs * 2 % piece) piece >>= 1;
+  switch (piece) {
+    case 16: return launch_pieces<T, 16, false, HEADS>(p, batch, heads, steps, s);
+    case 8: return launch_pieces<T, 8, false, HEADS>(p, batch, heads, steps, s);
+    case 4: return launch_pieces<T, 4, false, HEADS>(p, batch, heads, steps, s);
+    default: return launch_pieces<T, 2, false, HEADS>(p, batch, heads, steps, s);
+  }
+}
+template <typename T>
+int launch_append(kfa::RotaryParams& p, bool interleaved, int64_t batch, int64_t heads, int64_t steps, cudaStream_t s) {
+  // (one head a thread where that leaves room on the GPU: four CTAs an SM of 32-byte cells)
+  const bool few = batch * steps * heads * ((p.columns + 15) / 16) <= 4ll * SMS * kfa::ROT_THREADS;
+  return few ? launch_append<T, 1>(p, interleaved, batch, heads, steps, s) : launch_append<T, 3>(p, interleaved, batch, heads, steps, s);
 }
 
 }  // namespace
@@ -135,9 +157,9 @@ int kfa_rotary(const KfaTensor4* q, const KfaTensor4* k, const KfaTensor4* q_out
   while (!rotary->interleaved && piece > size && rotary->pairs * size % piece) piece >>= 1;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const bool inter = rotary->interleaved != 0;
-  if (dtype == KFA_F32) return launch_rotary<float, false>(p, inter, piece, q->shape[0], heads, q->shape[2], s);
-  if (dtype == KFA_BF16) return launch_rotary<__nv_bfloat16, false>(p, inter, piece, q->shape[0], heads, q->shape[2], s);
-  return launch_rotary<__half, false>(p, inter, piece, q->shape[0], heads, q->shape[2], s);
+  if (dtype == KFA_F32) return launch_rotary<float>(p, inter, piece, q->shape[0], heads, q->shape[2], s);
+  if (dtype == KFA_BF16) return launch_rotary<__nv_bfloat16>(p, inter, piece, q->shape[0], heads, q->shape[2], s);
+  return launch_rotary<__half>(p, inter, piece, q->shape[0], heads, q->shape[2], s);
 }
 
 int kfa_cache_append_rotary(const KfaCache* cache, const KfaTensor4* q, const KfaTensor4* k, const KfaTensor4* v, const KfaRows* rows,
@@ -175,11 +197,9 @@ int kfa_cache_append_rotary(const KfaCache* cache, const KfaTensor4* q, const Kf
   p.status = dev_status;
   const int64_t heads = p.qk_heads + static_cast<int64_t>(p.c.heads);
   if (static_cast<int64_t>(p.c.batch) * p.r.steps > 0x7fffffff) return fail(KFA_ERR_ARG, "rotary: too many rows in one call");
-  int piece = 16;  // (what the tensors and pages are whole numbers of)
-  while (!rotary->interleaved && rotary->pairs * 2 % piece) piece >>= 1;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (dtype == KFA_BF16) return launch_rotary<__nv_bfloat16, true>(p, rotary->interleaved != 0, piece, p.c.batch, heads, p.r.steps, s);
-  return launch_rotary<__half, true>(p, rotary->interleaved != 0, piece, p.c.batch, heads, p.r.steps, s);
+  if (dtype == KFA_BF16) return launch_append<__nv_bfloat16>(p, rotary->interleaved != 0, p.c.batch, heads, p.r.steps, s);
+  return launch_append<__half>(p, rotary->interleaved != 0, p.c.batch, heads, p.r.steps, s);
 }
 
 }  // extern "C"
