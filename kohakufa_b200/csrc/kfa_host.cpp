@@ -1152,6 +1152,14 @@ PyObject* py_rotary(Args a, Py_ssize_t n) {
   const at::Tensor q = tensor(a[0]), k = maybe(a[1]);
   RotaryArgs r = rotary_of(a + 2);
   r.inverse = PyObject_IsTrue(a[7]);
+  if (at::GradMode::is_enabled() && !r.inverse && k.defined() && q.requires_grad() != k.requires_grad()) {
+    // (the one that needs no gradient stays outside the graph)
+    check_rotated("apply_rotary", "k", k, q);
+    const bool first = q.requires_grad();
+    variable_list out = RotaryTurn::apply(first ? q : k, std::optional<at::Tensor>(), r);
+    at::Tensor other = std::get<0>(released([&] { return run_rotary(first ? k : q, at::Tensor(), r); }));
+    return first ? pack(Two{std::move(out[0]), std::move(other)}) : pack(Two{std::move(other), std::move(out[0])});
+  }
   if (at::GradMode::is_enabled() && !r.inverse && (q.requires_grad() || (k.defined() && k.requires_grad()))) {
     variable_list out = RotaryTurn::apply(q, k.defined() ? std::optional<at::Tensor>(k) : std::nullopt, r);
     if (!k.defined()) return THPVariable_Wrap(std::move(out[0]));

@@ -279,7 +279,9 @@ def test_gradient(dtype, interleaved, dim, turned):
     assert torch.equal(torch.autograd.grad(out, q, g[0])[0], got[0])
     out = apply_rotary(q.detach(), k, r)
     out[1].backward(g[1])
-    assert q.grad is None and torch.equal(k.grad, got[1])
+    assert q.grad is None and torch.equal(k.grad, got[1]) and not out[0].requires_grad
+    out = apply_rotary(q, k.detach(), r)
+    assert out[0].requires_grad and not out[1].requires_grad and torch.equal(out[1], apply_rotary(q, k, r)[1])
 
 
 @gpu
@@ -530,6 +532,38 @@ def test_append_reports_what_has_no_place():
         else:  # the other sequence's is
             assert torch.equal(bad.k[int(table[0, 0]), :, 14], keys[0][:, 0]) and torch.equal(bad.v[int(table[0, 0]), :, 15], v[0, :, 1])
         assert out is None or bool(torch.isfinite(out).all())
+
+
+@gpu
+def test_append_compiled():
+    """Through the registered op, which a compiler sees."""
+    r, cache = Rotary.of(64), make_cache([3, 20], 2, 64, torch.bfloat16, 16, 4)
+    q, k, v = rows(2, 4, 4, 64), rows(2, 2, 4, 64, seed=1), rows(2, 2, 4, 64, seed=2)
+    want = clone(cache)
+    a, b = cache_append_rotary(want, q, k, v, r, return_keys=True)
+
+    def step(kp, vp, q, k, v):
+        x, y = cache_append_rotary(KVCache(kp, vp, cache.lengths, cache.table), q * 1.0, k, v, r, return_keys=True)
+        return x + 0.0, y + 0.0
+
+    with torch.no_grad():
+        x, y = torch.compile(step, backend="aot_eager")(cache.k, cache.v, q, k, v)
+    assert torch.equal(x, a) and torch.equal(y, b) and torch.equal(cache.k, want.k) and torch.equal(cache.v, want.v)
+
+
+@gpu
+def test_append_many_heads_and_long_prompts():
+    """More tokens than one head a thread takes, with heads that are no multiple of three, against the pass of its own."""
+    dtype, r = torch.bfloat16, Rotary.of(64, interleaved=True)
+    for heads, kv_heads, tokens in ((7, 1, 3000), (4, 4, 2000), (40, 8, 500)):
+        cache = make_cache([5, 100], kv_heads, 96, dtype, 32, tokens)
+        q, k, v = (rows(2, h, tokens, 96, dtype=dtype, seed=s) for h, s in ((heads, 1), (kv_heads, 2), (kv_heads, 3)))
+        want = clone(cache)
+        got_q, got_k = cache_append_rotary(cache, q, k, v, r, return_keys=True)
+        q2, k2 = apply_rotary(q, k, r, offset=cache.lengths)
+        cache_append(want, k2, v)
+        assert torch.equal(got_q, q2) and torch.equal(got_k, k2) and torch.equal(cache.k, want.k) and torch.equal(cache.v, want.v)
+    assert _lib.device_status() == 0
 
 
 @gpu

@@ -138,6 +138,67 @@ def test_rows_of_every_kernel(batch, tokens, dim):
 
 
 @gpu
+@pytest.mark.parametrize("batch,tokens,heads", [(5, 16, 4), (40, 12, 4), (200, 1, 4), (33, 5, 8), (2, 300, 2)])
+def test_several_prefixes_with_many_rows(batch, tokens, heads):
+    """Row tiles that take both halves of a CTA, of groups that do not fill them, beside own rows of each kind; prompts behind a prefix."""
+    gen = torch.Generator().manual_seed(batch)
+    lengths = torch.randint(0, 300, (batch,), generator=gen).tolist()
+    starts = [0, batch // 3, batch // 3, batch - 1, batch]
+    for before in ([700, 50, 2500, 33], [64, 9000, 1, 0]):
+        prefix, cache = make_cache(before, 1, 64, torch.bfloat16, 16, seed=1), make_cache(lengths, 1, 64, torch.bfloat16, 16)
+        check_shared(prefix, cache, starts, heads, tokens, torch.bfloat16, "tree" if tokens < 100 else "causal")
+
+
+@gpu
+@pytest.mark.parametrize("dim", range(8, 129, 24))
+@pytest.mark.parametrize("batch,tokens", [(3, 1), (3, 7), (50, 4)])
+def test_head_dims(dim, batch, tokens):
+    lengths = [40 * i % 333 for i in range(batch)]
+    check_shared(make_cache([777], 2, dim, torch.float16, 16, seed=1), make_cache(lengths, 2, dim, torch.float16, 16), None, 8, tokens, torch.float16, "tree", seed=dim)
+
+
+@gpu
+def test_pages_far_into_a_pool():
+    """Pages whose bytes lie beyond 2^32, of the prefix and of the caches."""
+    dtype, page = torch.bfloat16, 64
+    k = torch.zeros(140000, page, 2, 128, dtype=dtype, device="cuda").transpose(1, 2)
+    v = torch.zeros_like(k)
+    at = torch.tensor([139999 - 7 * i for i in range(60)], dtype=torch.int32)
+    gen = torch.Generator().manual_seed(0)
+    for t in (k, v):
+        t[at.long().cuda()] = torch.randn(60, page, 2, 128, generator=gen).to(dtype).cuda().transpose(1, 2)
+    far = [KVCache(k, v, torch.tensor(n, dtype=torch.int32).cuda(), table.cuda()) for n, table in (([3000], at[:47].view(1, 47)), ([100, 200, 3], at[47:59].view(3, 4)))]
+    near = [KVCache(c.k[c.table.flatten().long()], c.v[c.table.flatten().long()], c.lengths, torch.arange(c.table.numel(), dtype=torch.int32, device="cuda").view(c.table.shape)) for c in far]
+    q, kn, vn = (rows(3, h, 2, 128, dtype, s) for h, s in ((8, 1), (2, 2), (2, 3)))
+    assert torch.equal(attention_shared(q, *far, kn, vn), check_shared(*near, None, 8, 2, dtype, "causal", q=q, k=kn, v=vn))
+    assert _lib.device_status() == 0
+
+
+@gpu
+def test_nobody_has_tokens():
+    dtype = torch.bfloat16
+    prefix, cache = make_cache([300], 2, 64, dtype, 16, seed=1), make_cache([5, 0, 90], 2, 64, dtype, 16)
+    got = check_shared(prefix, cache, None, 8, 3, dtype, "causal", counts=[0, 0, 0])
+    assert bool((got == 0).all())
+
+
+@gpu
+def test_compiled():
+    dtype = torch.bfloat16
+    prefix, cache = make_cache([300], 2, 64, dtype, 16, seed=1), make_cache([5, 0, 90], 2, 64, dtype, 16)
+    q, k, v = (rows(3, h, 2, 64, dtype, s) for h, s in ((8, 1), (2, 2), (2, 3)))
+
+    def step(q, k, v):
+        out, stats = attention_shared(q * 1.0, prefix, cache, k, v, return_stats=True)
+        return out + 0.0, stats + 0.0
+
+    with torch.no_grad():
+        a, b = torch.compile(step, backend="aot_eager")(q, k, v)
+        x, y = step(q, k, v)
+    assert torch.equal(a, x) and torch.equal(b, y)
+
+
+@gpu
 def test_many_prefixes():
     """More prefixes than the GPU has SMs and a CTA has threads, most with few sequences or none; whole items and cut ones in one call."""
     dtype = torch.float16
