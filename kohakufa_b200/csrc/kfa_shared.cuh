@@ -1,7 +1,10 @@
 // Attention behind shared prefixes: sequences of a batch that go on from a few prefixes, which are stored, and read, once.
 //
 //   a row's softmax over (its prefix, its sequence's cache, the new tokens) is that of two parts:
-//   m = max(m1, m2),  l = l1 2^((m1 - m) c) + l2 2^((m2 - m) c),  O = (O1 2^((m1 - m) c) + O2 2^((m2 - m) c)) / l
+//   m = max(m1, m2),  l = l1 2^(m1 - m) + l2 2^(m2 - m),  O = (O1 2^(m1 - m) + O2 2^(m2 - m)) / l
+//
+// with P = 2^(S c - m). The reference m is the largest score when it was taken times c = scale * log2 e, rounded: P, l and O of a part belong to it as it is
+// stored, so that its rounding cancels, and an exponent is one multiply-add.
 //
 // What bounds it: the keys and values, each read once; and where many rows share a long prefix the two products and the exponentials. One kernel does both
 // parts side by side: its CTAs have two halves, each a stream of its own, and a CTA takes either two stretches of the prefixes' work or two of the
@@ -100,12 +103,13 @@ __device__ __forceinline__ bool sh_work(const AttendParams& p, int* s_i, int ind
                                         int& end) {
   using W = WalkOf<MODE>;
   const int tid = threadIdx.x & (SH_THREADS - 1), warp = tid >> 5, lane = tid & 31;
-  chunk = max((total + count - 1) / count, p.least);
+  chunk = 0;
   if (split > 0) {
-    const int items = W::items_of(p, 0), each = total / items, k = index % split;
-    auto unit = [&](int i) { return max(static_cast<int>(static_cast<long long>(each) * i / split) - p.extra, 0); };
+    const int items = W::items_of(p, 0), each = total / items, long_ones = each % split, length = each / split;
+    auto unit = [&](int i) { return max(length * i + min(i, long_ones) - p.extra, 0); };
     w.b = 0;
     w.item = index / split;
+    const int k = index - w.item * split;
     w.unit = unit(k);
     w.end_b = 0;
     w.end_item = k + 1 < split ? w.item : w.item + 1;
@@ -115,6 +119,7 @@ __device__ __forceinline__ bool sh_work(const AttendParams& p, int* s_i, int ind
     __syncthreads();
     return w.item < items && w.start(p);
   }
+  chunk = max((total + count - 1) / count, p.least);
   const int at[2] = {chunk * index, chunk * index + chunk};
   end = at[1];
   int before = 0;
@@ -158,23 +163,31 @@ __device__ __forceinline__ bool sh_work(const AttendParams& p, int* s_i, int ind
   return w.b < p.c.batch && w.start(p);
 }
 
+// See part_factor, for references that are scaled.
+__device__ __forceinline__ float sh_factor(float m, float l, float m_all) {
+  if (m == -INFINITY) return l == 0.f ? -1.f : 1.f;
+  return ex2(m - m_all);
+}
+constexpr float SH_SLACK = 8.f;  // how far a maximum may grow before O is rescaled: a factor of 2^8
+
 // How many CTAs the prefixes' work gets, and into how many stretches each of its items is cut (0: wherever stretches end).
 template <bool PAIR>
 __device__ __forceinline__ void sh_share(const SharedParams& p, int total_pre, int total_own, int grid, int& pre_ctas, int& split) {
   split = 0;
   const float pre = total_pre * p.weight, own = 0.5f * total_own;  // a CTA's time for all of it (own: two halves work at once)
   const float most = static_cast<float>(grid - 1);                 // (the own work is never nothing)
-  pre_ctas = total_pre == 0 ? 0 : static_cast<int>(fminf(fmaxf(grid * pre / (pre + own) + 0.5f, 1.f), most));
+  pre_ctas = total_pre == 0 ? 0 : static_cast<int>(fminf(fmaxf(grid * __fdividef(pre, pre + own) + 0.5f, 1.f), most));
   if (total_pre == 0 || p.pre_items == 0) return;
   // one prefix: so many stretches an item that what ends last ends first
   const float per = PAIR ? 1.f : 0.5f;  // CTAs of a stretch
-  const float ideal = pre_ctas / (per * p.pre_items);
+  const float stretch = per * p.pre_items, ideal = __fdividef(static_cast<float>(pre_ctas), stretch);
   float best = 0.f;
+  const float continuous = pre_ctas;
   const int each = total_pre / p.pre_items;  // (a stretch has a unit at least)
   for (int s = max(static_cast<int>(ideal), 1); s <= min(static_cast<int>(ideal) + 1, max(each / p.pre.least, 1)); ++s) {
-    const float ctas = ceilf(s * per * p.pre_items);
+    const float ctas = ceilf(s * stretch);
     if (ctas > most) break;
-    const float time = fmaxf(pre / (s * per * p.pre_items), own / (grid - ctas));
+    const float time = fmaxf(__fdividef(pre, s * stretch), __fdividef(own, grid - ctas));
     if (split == 0 || time < best) {
       best = time;
       split = s;
@@ -183,7 +196,7 @@ __device__ __forceinline__ void sh_share(const SharedParams& p, int total_pre, i
   }
   if (split > 0 && ideal < 0.8f) {  // fewer CTAs than items: cut where stretches end
     split = 0;
-    pre_ctas = static_cast<int>(fminf(fmaxf(grid * pre / (pre + own) + 0.5f, 1.f), most));
+    pre_ctas = static_cast<int>(continuous);
   }
 }
 
@@ -420,12 +433,12 @@ __device__ __forceinline__ void sh_columns(const AttendParams& p, const WalkOf<M
         float* mx = s_max + (c & 1) * 4 * N;
         if (lane < N) mx[warp * N + lane] = top;
         x.meet();
-        const float y = fmaxf(fmaxf(mx[col], mx[N + col]), fmaxf(mx[2 * N + col], mx[3 * N + col]));
-        m_top = fmaxf(m_top, y);
-        const bool move = m_ref == -INFINITY ? y > -INFINITY : y > m_ref + p.slack;
+        const float raw = fmaxf(fmaxf(mx[col], mx[N + col]), fmaxf(mx[2 * N + col], mx[3 * N + col])), y = raw * c_log2;
+        m_top = fmaxf(m_top, raw);
+        const bool move = m_ref == -INFINITY ? y > -INFINITY : y > m_ref + SH_SLACK;
         float alpha = 1.f;
         if (move) {
-          alpha = m_ref == -INFINITY ? 0.f : ex2((m_ref - y) * c_log2);
+          alpha = m_ref == -INFINITY ? 0.f : ex2(m_ref - y);
           m_ref = y;
         }
         if (lane < N) shift[col] = m_ref == -INFINITY ? 0.f : -m_ref;
@@ -457,7 +470,7 @@ __device__ __forceinline__ void sh_columns(const AttendParams& p, const WalkOf<M
           const float2 mm[4] = {make_float2(a.x, a.y), make_float2(a.z, a.w), make_float2(b.x, b.y), make_float2(b.z, b.w)};
 #pragma unroll
           for (int j = 0; j < 8; j += 2) {
-            const float2 z = __fmul2_rn(__fadd2_rn(make_float2(e[i + j], e[i + j + 1]), mm[j / 2]), c2);
+            const float2 z = __ffma2_rn(make_float2(e[i + j], e[i + j + 1]), c2, mm[j / 2]);
             e[i + j] = ex2(z.x);
             e[i + j + 1] = ex2(z.y);
             const float2 sum = __fadd2_rn(make_float2(l[i + j], l[i + j + 1]), make_float2(e[i + j], e[i + j + 1]));
@@ -509,7 +522,7 @@ __device__ __forceinline__ void sh_columns(const AttendParams& p, const WalkOf<M
         to.ml[to.plane + at] = l_all;
         to.ml[2 * to.plane + at] = fin[5 * N + col];
       }
-      const bool none = part_factor(m, l_all, m, c_log2) < 0.f;  // nothing was seen: O is not defined
+      const bool none = sh_factor(m, l_all, m) < 0.f;  // nothing was seen: O is not defined
       tmem_wait_ld();
       tc_fence_before();
       mbar_arrive(bar(R::B_OFREE));
@@ -632,9 +645,10 @@ __device__ __forceinline__ void sh_rows(const AttendParams& p, const WalkOf<MODE
         for (int j = 0; j < 32; ++j) y[j & 3] = fmaxf(y[j & 3], fmaxf(e[j].x, e[j].y));
         const float top = fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3]));
         m_top = fmaxf(m_top, top);
-        const bool move = m_ref == -INFINITY ? top > -INFINITY : top > m_ref + p.slack;
+        const float y_top = top * c_log2;
+        const bool move = m_ref == -INFINITY ? y_top > -INFINITY : y_top > m_ref + SH_SLACK;
         if (__builtin_expect(__any_sync(0xffffffffu, move), 0)) {
-          const float alpha = !move ? 1.f : (m_ref == -INFINITY ? 0.f : ex2((m_ref - top) * c_log2));
+          const float alpha = !move ? 1.f : (m_ref == -INFINITY ? 0.f : ex2(m_ref - y_top));
           if (t > 0) {  // every product issued so far has to have retired
             if (ok) ok = wait_warp(bar(R::B_PV + ((c - 1) & 1)), ((c - 1) >> 1) & 1, ctl, 79);
             tc_fence_after();
@@ -650,7 +664,7 @@ __device__ __forceinline__ void sh_rows(const AttendParams& p, const WalkOf<MODE
             tmem_wait_st();
             l *= alpha;
           }
-          if (move) m_ref = top;
+          if (move) m_ref = y_top;
         }
         const float sh = m_ref == -INFINITY ? 0.f : -m_ref;
         const float2 s2 = make_float2(sh, sh);
@@ -660,7 +674,7 @@ __device__ __forceinline__ void sh_rows(const AttendParams& p, const WalkOf<MODE
           uint32_t pk[16];
 #pragma unroll
           for (int j = 0; j < 16; ++j) {
-            float2 z = __fmul2_rn(__fadd2_rn(e[k + j], s2), c2);
+            float2 z = __ffma2_rn(e[k + j], c2, s2);
             z.x = ex2(z.x);
             z.y = ex2(z.y);
             sum[j & 1] = __fadd2_rn(sum[j & 1], z);
@@ -711,7 +725,7 @@ __device__ __forceinline__ void sh_rows(const AttendParams& p, const WalkOf<MODE
         to.ml[to.plane + at] = l;
         to.ml[2 * to.plane + at] = m_top;
       }
-      const bool none = part_factor(m_ref, l, m_ref, c_log2) < 0.f;  // nothing was seen: O is not defined
+      const bool none = sh_factor(m_ref, l, m_ref) < 0.f;  // nothing was seen: O is not defined
       if (ok) ok = wait_warp(bar(R::B_PV + ((c - 1) & 1)), ((c - 1) >> 1) & 1, ctl, 83);
       tc_fence_before();
       x.meet();  // (what the threads have met of values that are not finite)
@@ -972,12 +986,12 @@ __global__ void __launch_bounds__(256) kfa_shared_join_kernel(const __grid_const
     const float m_new = fmaxf(m, warp_max(mi));
     top = fmaxf(top, warp_max(ti));
     if (i0) {
-      const float old = part_factor(m, l, m_new, own.c_log2), a = old < 0.f ? 0.f : old;
+      const float old = sh_factor(m, l, m_new), a = old < 0.f ? 0.f : old;
       l *= a;
       o = make_float4(o.x * a, o.y * a, o.z * a, o.w * a);
     }
     m = m_new;
-    const float a = lane < k ? part_factor(mi, li, m, own.c_log2) : -1.f;
+    const float a = lane < k ? sh_factor(mi, li, m) : -1.f;
     li *= a;
     auto add = [&](int i, const float4& z) {
       const float ai = __shfl_sync(0xffffffffu, a, i);
@@ -1010,7 +1024,7 @@ __global__ void __launch_bounds__(256) kfa_shared_join_kernel(const __grid_const
   if (own.stats && lane == 0) {
     float* to = own.stats + (static_cast<long long>(b) * own.H + h) * 2 * own.T + t;
     to[0] = bad ? nan : (some ? top : INFINITY);
-    to[own.T] = bad ? nan : (some ? log2f(l) + (m - top) * own.c_log2 : 0.f);
+    to[own.T] = bad ? nan : (some ? log2f(l) + __fmaf_rn(-top, own.c_log2, m) : 0.f);
   }
 }
 
