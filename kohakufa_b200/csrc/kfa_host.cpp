@@ -150,7 +150,7 @@ int dtype_code(const at::Tensor& t) {
 at::Tensor bshd_like(const at::Tensor& t) {
   return at::empty({t.size(0), t.size(2), t.size(1), t.size(3)}, t.options()).transpose(1, 2);
 }
-// the same layout for a gradient, which need not be a view
+// the same layout where it need not be a view, e.g. for a gradient
 at::Tensor grad_like(const at::Tensor& t) {
   const int64_t h = t.size(1), s = t.size(2), d = t.size(3);
   return at::empty_strided(t.sizes(), {h * s * d, d, h * d, 1}, t.options());
@@ -1093,7 +1093,7 @@ Two run_rotary(const at::Tensor& q, const at::Tensor& k, const RotaryArgs& r) {
     TORCH_CHECK_VALUE(t->device() == q.device(), who, ": tensors on different devices");
   }
   const c10::cuda::CUDAGuard guard(q.device());
-  auto like = [](const at::Tensor& t) { return t.dim() == 4 ? bshd_like(t) : at::empty(t.sizes(), t.options()); };
+  auto like = [](const at::Tensor& t) { return t.dim() == 4 ? grad_like(t) : at::empty(t.sizes(), t.options()); };
   at::Tensor q_out = like(q), k_out = k.defined() ? like(k) : at::Tensor();
   if (q.numel() == 0) return {std::move(q_out), std::move(k_out)};  // no tokens
   const KfaTensor4 d[4] = {desc_rows(q), k.defined() ? desc_rows(k) : KfaTensor4{}, desc_rows(q_out), k.defined() ? desc_rows(k_out) : KfaTensor4{}};
@@ -1196,7 +1196,7 @@ PyObject* py_cache_append_rotary(Args a, Py_ssize_t n) {
   will_write({&c.k, &c.v});
   auto [q_out, k_out] = released([&] {
     const c10::cuda::CUDAGuard guard(k.device());
-    at::Tensor qo = q.defined() ? bshd_like(q) : at::Tensor(), ko = keys ? bshd_like(k) : at::Tensor();
+    at::Tensor qo = q.defined() ? grad_like(q) : at::Tensor(), ko = keys ? grad_like(k) : at::Tensor();
     const KfaCache dc = cache_desc(c);
     const KfaTensor4 dk = desc(k), dv = desc(v), dq = q.defined() ? desc(q) : KfaTensor4{}, dqo = q.defined() ? desc(qo) : KfaTensor4{},
                      dko = keys ? desc(ko) : KfaTensor4{};
