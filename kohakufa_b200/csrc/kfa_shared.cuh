@@ -909,7 +909,7 @@ __global__ void __launch_bounds__(256) kfa_shared_join_kernel(const __grid_const
   let_next_begin();
   const AttendParams &own = p.own, &pre = p.pre;
   if (row >= own.carry_rows) return;
-  const bool bad = load_status(own.status) != 0;
+  bool bad = false;
   const int count = own.counts ? min(max(own.counts[b], 0), own.T) : own.T;
   const int g = h / own.group, dh = h - g * own.group;
   const long long at = (static_cast<long long>(b) * own.H + h) * own.T + t;
@@ -939,13 +939,17 @@ __global__ void __launch_bounds__(256) kfa_shared_join_kernel(const __grid_const
     int s0, s1;
     prefix_group(pre, group, s0, s1);
     const int ds = static_cast<int>(pre.by_ts.div(max(static_cast<int>(b) - s0, 0))), th = dh / pre.gt, tt = t / pre.tt, first = s0 + ds * pre.ts;
-    if (!bad) before = pre.dir[(static_cast<long long>(g) * pre.row_tiles + tt * pre.head_tiles + th) * pre.seqs + first];
+    before = pre.dir[(static_cast<long long>(g) * pre.row_tiles + tt * pre.head_tiles + th) * pre.seqs + first];
     r_pre = ((static_cast<int>(b) - first) * pre.tt + t - tt * pre.tt) * pre.gt + dh - th * pre.gt;
     pair = p.pre_pair;  // rows 128 .. 255 are the second half's, and a part's CTA has both
     if (before.y > 0) before.x += r_pre >> 7;
     r_pre &= 127;
   }
-  if (bad) mine = make_int2(0, 0), before = make_int2(0, -1);  // (the directory may not have been written)
+  if (load_status(own.status) != 0) {  // (the directory may not have been written)
+    bad = true;
+    mine = make_int2(0, 0);
+    before = make_int2(0, -1);
+  }
   const int n_pre = before.y < 0 ? 0 : max(before.y, 1), n = n_pre + max(mine.y, 1);
   // source i: the prefix' parts, then the row's own. Parts: the first in slot 1 of its half, the others in slot 0 of theirs.
   auto find = [&](int i, const float*& o, const float*& ml, long long& plane) {
