@@ -8,9 +8,11 @@
     out = attention(q, k, v, mask=pack_mask(mask, B, H, Sq, Skv))  # boolean mask, packed once
 
     out = attention_cached(q, KVCache(k_pages, v_pages, lengths, table), k, v)  # generation: new tokens over a cache
+    q, k = apply_rotary(q, k, Rotary.of(128))  # rotary positions
 
 Same exports as the reference (``src/kohakufa/__init__.py:12``), plus a few of this package's own: a cache
-of keys and values for generation (``kohakufa_b200.cache``: ``KVCache``, ``attention_cached``, ``cache_append``, ``cache_weights``, ``cache_evict``, ``tree_mask``),
+of keys and values for generation (``kohakufa_b200.cache``: ``KVCache``, ``attention_cached``, ``attention_shared``, ``cache_append``, ``cache_append_rotary``,
+``cache_weights``, ``cache_evict``, ``tree_mask``), rotary positions (``kohakufa_b200.rotary``: ``Rotary``, ``apply_rotary``, ``rotary_frequencies``),
 ``set_backward`` / ``set_deterministic`` (which backward kernels run; bit-reproducible gradients), ``check_status`` / ``reset_status`` (the device-side
 health word, see ``check_status``).
 """

@@ -10,6 +10,9 @@
         if full:                                                    # back to the budget, with room for what comes
             cache, w, kept = cache_evict(cache, w, keep=2048, recent=256, room=4096)
 
+Keys that are turned by their positions (``kohakufa_b200.rotary``) go in through ``cache_append_rotary``; sequences that go on from prefixes which are stored
+once attend through ``attention_shared``.
+
 All of it is for inference: there are no gradients, and a call on tensors that autograd would record is refused. The calls go to
 ``libkfa.so`` through the C++ launch path like ``attention``: current stream, no host synchronisation, scratch from the
 caching allocator, CUDA-graph capture after one eager call on the device. ``lengths`` and ``table`` are read on the device,

@@ -12,7 +12,9 @@
 // SM's instruction cache together. A prefix' tile took 4000 clk beside an own one and that 3800, two of a kind take 1900 and 2800.) Both kinds are cut
 // by keys as in kfa_attend.cuh. A prefix's row tile has the rows of several sequences (sequences, tokens, heads of a K / V head, up to 128), whose queries one TMA box
 // brings; a prefix is read once for each of them, out of L2 but the first time.
-// (64 sequences behind 8192 positions, 1 to 1024 of their own, 32 / 8 heads, one token: the prefix first, its join, then the own part took 76 us.)
+// Graph time with 32 / 8 heads, D = 128: 64 sequences behind 8192 positions, 1 to 1024 of their own, one token 50 us (floor 28, memory; the prefix first, its join, then
+// the own part 76); 32 behind 8192, trees of 8 tokens 70 (floor 17); 256 behind 32768, 200 to 2048 of their own 283 (floor 208). A tile of 256 rows x 64 keys takes
+// 2030 clk, an own one of 128 keys 2800 to 3300 (0.9 of the copy rate), what lies between two own items 7000.
 //
 // More than 128 rows of a prefix: a tile has up to 256, half of them in each half of the CTA, which share its keys and values. (They are
 // copied once a CTA then: two halves with tiles of their own ask L2 for 30 bytes a clock and SM.) Where there is one prefix, the row tiles of a K / V head are cut at the same
