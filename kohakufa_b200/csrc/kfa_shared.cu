@@ -163,6 +163,7 @@ int kfa_cache_attend_shared(const KfaTensor4* q, const KfaCache* prefix, const i
   fill_part(pre, plan, true, batch, scratch);
   fill_part(own, plan, false, batch, scratch);
   p.pre_pair = plan.n_pre == 256;
+  p.halves = 2 * plan.grid;
   p.pre_items = pre.c.batch == 1 && !starts ? static_cast<int>(own.c.heads * plan.row_tiles * ((batch + plan.ts - 1) / plan.ts)) : 0;
   p.weight = p.pre_pair ? 1.2f : 0.6f;  // (of a CTA's time: without a pair its halves do two at once)
   CUtensorMap m[8];

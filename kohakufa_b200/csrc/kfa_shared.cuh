@@ -49,6 +49,7 @@ struct SharedParams {
   float weight;   // what a unit of the prefixes, of a CTA, counts beside one of the sequences' own, of a half
   int pre_items;  // where there is one prefix: its items; else 0
   int pre_pair;   // whether a prefix' row tile takes both halves of a CTA
+  int halves;     // of all CTAs
 };
 
 // Shared memory and barriers of a half, whichever work it has: 1 KB of barriers and control, then its rings. N = 256: of the whole CTA, whose first half
@@ -947,6 +948,9 @@ __global__ void __launch_bounds__(256) kfa_shared_join_kernel(const __grid_const
     if (before.y > 0) before.x += r_pre >> 7;
     r_pre &= 127;
   }
+  // (Lengths that another stream changes while the kernel before this one runs may leave anything there; it stays inside the scratch.)
+  mine.y = min(max(mine.y, 0), p.halves);
+  before.y = min(before.y, p.halves);
   if (load_status(own.status) != 0) {  // (the directory may not have been written)
     bad = true;
     mine = make_int2(0, 0);
@@ -963,7 +967,8 @@ __global__ void __launch_bounds__(256) kfa_shared_join_kernel(const __grid_const
       ml = q.carry_ml + at;
       plane = q.carry_rows;
     } else {
-      const long long slot = 2ll * (d.x + (i < n_pre && pair ? 2 * j : j)) + (j == 0 ? 1 : 0);
+      const int half = min(max(d.x, 0) + (i < n_pre && pair ? 2 * j : j), p.halves - 1);
+      const long long slot = 2ll * half + (j == 0 ? 1 : 0);
       o = q.part_o + (slot * q.rows + r) * 128;
       ml = q.part_ml + slot * 3 * q.rows + r;
       plane = q.rows;
