@@ -326,7 +326,7 @@ int kfa_cache_attend(const KfaTensor4* q, const KfaCache* cache, const KfaTensor
 /* The same for sequences that go on from prefixes which are stored once: `prefix` holds starts[n] .. starts[n + 1] - 1's (sequences, int32
  * [prefix->batch + 1], ascending, inside the batch; NULL: one prefix, of all sequences) first positions, `cache` what each has behind them; sequences outside starts
  * have no prefix. A row sees its whole prefix and what kfa_cache_attend shows it. starts that do not ascend are reported like a bad table.
- * scratch: kfa_cache_attend_shared_bytes bytes. */
+ * scratch: kfa_cache_attend_shared_bytes bytes (1 KB a row of q, and what cut rows take: up to 78 MB). */
 int64_t kfa_cache_attend_shared_bytes(const KfaTensor4* q, const KfaCache* prefix, const KfaCache* cache, const KfaTensor4* k);
 int kfa_cache_attend_shared(const KfaTensor4* q, const KfaCache* prefix, const int32_t* starts, const KfaCache* cache, const KfaTensor4* k,
                             const KfaTensor4* v, const uint8_t* tree, const int64_t* tree_stride, const int32_t* counts,
