@@ -65,7 +65,7 @@ struct ShCfg {
   static constexpr int P_BYTES = ROWS ? 0 : 128 * N * 2;   // in shared memory
   // column maxima of two tiles, shifts, sums and maxima of two segments; rows on their way out
   static constexpr int OTHER = ROWS ? (PAIR ? 8 : 4) * 2048 : (2 * 4 * N + 4 * N + 2 * 6 * N) * 4;
-  static constexpr int FIXED = (PAIR ? 3072 : 2048) + NQ * Q_BYTES + P_BYTES + OTHER;
+  static constexpr int FIXED = 1024 * (PAIR ? 3 : 2) + NQ * Q_BYTES + P_BYTES + OTHER;
   static constexpr int FIT = ((PAIR ? 2 * SH_SMEM : SH_SMEM) - FIXED) / STAGE;
   static constexpr int DV = (FIT + 1) / 2 < 4 ? (FIT + 1) / 2 : 4;  // (of three stages two: values stay until a tile is done with, keys only until its scores are made)
   static constexpr int DK = FIT - DV < 4 ? FIT - DV : 4;
