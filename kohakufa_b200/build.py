@@ -24,6 +24,10 @@ LIB = PKG / "libkfa.so"
 # give-up path (status word, NaN outputs, clean teardown) run on a device without hanging anything.
 LIB_SHORT_WAIT = PKG / "libkfa_shortwait.so"
 SHORT_WAIT_FLAGS = ["-DKFA_WAIT_CYCLES=300ll"]
+# Attention behind shared prefixes with producers of values that begin 200,000 clk behind everything else: what tests/test_shared_late.py
+# loads to see that results do not depend on which of a kernel's warps is held up.
+LIB_LATE = PKG / "libkfa_late.so"
+LATE_FLAGS = ["-DKFA_LATE_VALUES=200000ll"]
 HOST = PKG / "_kfa_host.so"
 HOST_SOURCES = [CSRC / "kfa_host.cpp", PKG.parent / "include" / "kfa.h"]
 SHARED = [CSRC / "kfa_ptx.cuh", CSRC / "kfa_call.cuh", PKG.parent / "include" / "kfa.h"]
@@ -37,6 +41,8 @@ SOURCES = {
     CSRC / "kfa_shared.cu": SHARED + CACHE + ATTEND + [CSRC / "kfa_shared.cuh"],
     CSRC / "kfa_rotary.cu": SHARED + CACHE + [CSRC / "kfa_rotary.cuh"],
 }
+# What each library is compiled with, and of which sources.
+LIBS = {LIB: ([], list(SOURCES)), LIB_SHORT_WAIT: (SHORT_WAIT_FLAGS, list(SOURCES)), LIB_LATE: (LATE_FLAGS, [CSRC / "kfa_shared.cu"])}
 OBJECTS = CSRC / "build"
 NVCC_FLAGS = [
     "-gencode",
@@ -74,7 +80,7 @@ def stale(lib: Path = LIB) -> bool:
     if not lib.exists() or (lib == HOST and not host_fits(lib)):
         return True
     built = lib.stat().st_mtime
-    return any(p.stat().st_mtime > built for p in (HOST_SOURCES if lib == HOST else [f for s in SOURCES for f in (s, *SOURCES[s])]))
+    return any(p.stat().st_mtime > built for p in (HOST_SOURCES if lib == HOST else [f for s in LIBS[lib][1] for f in (s, *SOURCES[s])]))
 
 
 def _run(cmd, log: str, verbose: bool) -> None:
@@ -98,7 +104,7 @@ def _compile(lib: Path, source: Path, extra, force: bool, verbose: bool) -> None
 
 
 def _link(lib: Path) -> None:
-    cmd = [nvcc_path(), *NVCC_FLAGS[:2], "-shared", "-o", str(lib), *(str(_object(lib, s)) for s in SOURCES)]
+    cmd = [nvcc_path(), *NVCC_FLAGS[:2], "-shared", "-o", str(lib), *(str(_object(lib, s)) for s in LIBS[lib][1])]
     _run(cmd, f"csrc/build/{lib.stem}_link.log", False)
 
 
@@ -117,18 +123,17 @@ def _compile_host() -> None:
 
 
 def build(force: bool = False, verbose: bool = False, short_wait: bool = True) -> Path:
-    """Compile the library, the host extension (and, with ``short_wait``, the library's short-wait test twin) if
+    """Compile the library, the host extension (and, with ``short_wait``, the library's test twins) if
     missing or older than the sources; returns the library's path."""
-    libs = [(LIB, [])] + ([(LIB_SHORT_WAIT, SHORT_WAIT_FLAGS)] if short_wait else [])
-    libs = [(lib, extra) for lib, extra in libs if force or stale(lib)]
+    libs = [lib for lib in (LIBS if short_wait else [LIB]) if force or stale(lib)]
     OBJECTS.mkdir(exist_ok=True)
     with ThreadPoolExecutor() as pool:
-        jobs = [pool.submit(_compile, lib, src, extra, force, verbose and lib is LIB) for lib, extra in libs for src in SOURCES]
+        jobs = [pool.submit(_compile, lib, src, LIBS[lib][0], force, verbose and lib is LIB) for lib in libs for src in LIBS[lib][1]]
         if force or stale(HOST):
             jobs.append(pool.submit(_compile_host))
         for job in jobs:
             job.result()
-    for lib, _ in libs:
+    for lib in libs:
         _link(lib)
     return LIB
 

@@ -283,7 +283,7 @@ __device__ __forceinline__ bool wait_warp(uint32_t bar, uint32_t parity, const C
 template <int NC_, int Q_ROWS_, int NQ_, bool BOTH_, int OTHER_>
 struct AttRings {
   static constexpr int NC = NC_, Q_ROWS = Q_ROWS_, NQ = NQ_;
-  static constexpr bool BOTH = BOTH_, KEYS_FIRST = false;  // KEYS_FIRST: whether the first values wait for the first keys
+  static constexpr bool BOTH = BOTH_, KEYS_FIRST = false;  // KEYS_FIRST: whether the first values wait for the first keys' scores
   static constexpr int UNITS = 4;                          // of a tile
   static constexpr int CHUNK = 128 * 64 * 2;  // 128 keys x 64 columns
   static constexpr int STAGE = NC * CHUNK;
@@ -496,8 +496,15 @@ __device__ __forceinline__ void att_produce(const AttendParams& p, const WalkOf<
   const int per_unit = ATT_UNIT / p.box, boxes = R::UNITS * per_unit;
   bool ok = true, more = true;
   int T = 0, s = 0;  // tiles and segments so far
-  // (At the start all CTAs ask for all that their rings hold: the first keys, which everything waits for, go ahead of the values.)
-  if (R::KEYS_FIRST && values) ok = wait_warp(bar(R::B_KV + R::k_stage(0)), 0, ctl, 77);
+  if constexpr (KFA_LATE_VALUES > 0) {
+    const long long t0 = clock64();
+    while (values && clock64() - t0 < KFA_LATE_VALUES) {}
+  }
+  // (At the start all CTAs ask for all that their rings hold: the first keys, which everything waits for, go ahead of the values. What is waited for are the first
+  // scores, not the keys' own barrier: a key stage is filled again as soon as its scores are made, so that a warp which is held up could come to that barrier a
+  // phase or two late, and wait for what only its own values bring about. The phase behind that of the first scores belongs to the third tile's, which are made
+  // when the first values have been multiplied: it cannot be over before this wait.)
+  if (R::KEYS_FIRST && values) ok = wait_warp(bar(R::B_S), 0, ctl, 77);
   while (more && ok) {
     const RowMapOf<MODE> rows(p, w.b, w.item);
     if (lane == 0 && !length_ok(p.c, w.b)) *ac.bad = 1;

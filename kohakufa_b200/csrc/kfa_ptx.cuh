@@ -32,6 +32,10 @@ enum : int {
 #ifndef KFA_WAIT_CYCLES
 #define KFA_WAIT_CYCLES 4000000000ll
 #endif
+// How many clocks the producers of values begin behind the other roles: 0 but in a library for tests, where it must not matter.
+#ifndef KFA_LATE_VALUES
+#define KFA_LATE_VALUES 0ll
+#endif
 // The limit of the waits of the teardown itself (a CTA that gives up still lets the MMAs it has issued
 // retire and the copies it has started land before it frees its tensor memory and shared memory):
 // never shortened, also not in the test build that sets a tiny KFA_WAIT_CYCLES.
