@@ -821,14 +821,19 @@ kfa_shared_kernel(const __grid_constant__ CUtensorMap tmQp, const __grid_constan
   }
   wait_for_previous();
   if (warp == 5 && lane == 0) *ac.bad = load_status(p.pre.status) != 0;
-  if (p.pre.starts && blockIdx.x == 0) {
+  // starts that do not ascend inside the batch: prefixes would have sequences in common, and more work than the host's limit on its units allows for. There is
+  // none of it then, in any CTA, and the joining kernel sees the status word.
+  bool wrong = false;
+  if (p.pre.starts) {
     for (int i = threadIdx.x; i <= p.pre.groups; i += 2 * SH_THREADS)
-      if (p.pre.starts[i] < 0 || p.pre.starts[i] > p.pre.seqs || (i > 0 && p.pre.starts[i] < p.pre.starts[i - 1])) report(p.pre.status, DEV_BAD_CACHE);
+      wrong |= p.pre.starts[i] < 0 || p.pre.starts[i] > p.pre.seqs || (i > 0 && p.pre.starts[i] < p.pre.starts[i - 1]);
   }
+  wrong = __syncthreads_or(wrong) != 0;
+  if (wrong && blockIdx.x == 0 && threadIdx.x == 0) report(p.pre.status, DEV_BAD_CACHE);
   tc_fence_before();
   // ---- how much there is of both kinds of work, and which is this CTA's ----
   int total_pre = 0, total_own = 0;
-  for (int b = threadIdx.x; b < p.pre.c.batch; b += 2 * SH_THREADS) total_pre += sh_counted<ATT_PREFIX>(p.pre, b);
+  for (int b = threadIdx.x; b < (wrong ? 0 : p.pre.c.batch); b += 2 * SH_THREADS) total_pre += sh_counted<ATT_PREFIX>(p.pre, b);
   for (int b = threadIdx.x; b < p.own.c.batch; b += 2 * SH_THREADS) total_own += sh_counted<ATT_OWN>(p.own, b);
   const long long both = sh_sum((static_cast<long long>(total_pre) << 32) + total_own, s_sum);
   total_pre = static_cast<int>(both >> 32);
