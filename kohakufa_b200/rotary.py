@@ -34,7 +34,7 @@ def rotary_frequencies(
         ``factor``;
       * ``"ramp"``: a pair that turns more than ``high`` times over ``length`` keeps its frequency, one that turns less than ``low`` times
         gets ``f_i / factor``, in between in proportion to the turns;
-      * ``"yarn"``: the same with an amplitude of ``0.1 ln(factor) + 1``."""
+      * ``"yarn"``: the same with an amplitude of ``0.1 ln(factor) + 1`` (1 for a factor below 1)."""
     if isinstance(dim, bool) or int(dim) != dim or dim < 2 or dim % 2:
         raise ValueError(f"rotary_frequencies: dim {dim}: an even number of columns")
     if method not in METHODS:
@@ -55,7 +55,7 @@ def rotary_frequencies(
             raise ValueError(f"rotary_frequencies: low {low}, high {high}: 0 <= low < high")
         keep = ((length * f / (2 * math.pi) - low) / (high - low)).clamp(0.0, 1.0)
         f = keep * f + (1.0 - keep) * f / factor
-    return f, (0.1 * math.log(factor) + 1.0 if method == "yarn" else 1.0)
+    return f, (0.1 * math.log(max(factor, 1.0)) + 1.0 if method == "yarn" else 1.0)
 
 
 class Rotary:
