@@ -1,6 +1,6 @@
 """Rotary positions: queries and keys turned by angles that grow with a token's position.
 
-    rotary = Rotary.of(128, base=500000.0)                       # once, e.g. Rotary.of(128, method="yarn", factor=16, length=4096)
+    rotary = Rotary.of(128, base=500000.0)                       # once, e.g. Rotary.of(128, method="yarn_pairs", factor=16, length=4096)
     q, k = apply_rotary(q, k, rotary)                            # training, prompts: tokens 0 .. S - 1
     out = attention(q, k, v, causal=True)
 
@@ -19,7 +19,7 @@ from kohakufa_b200 import _lib
 
 __all__ = ["Rotary", "apply_rotary", "rotary_frequencies"]
 
-METHODS = ("none", "linear", "base", "ramp", "yarn")
+METHODS = ("none", "linear", "base", "ramp", "yarn", "yarn_pairs")
 
 
 def rotary_frequencies(
@@ -34,7 +34,10 @@ def rotary_frequencies(
         ``factor``;
       * ``"ramp"``: a pair that turns more than ``high`` times over ``length`` keeps its frequency, one that turns less than ``low`` times
         gets ``f_i / factor``, in between in proportion to the turns;
-      * ``"yarn"``: the same with an amplitude of ``0.1 ln(factor) + 1`` (1 for a factor below 1)."""
+      * ``"yarn"``: the same with an amplitude of ``0.1 ln(factor) + 1`` (1 for a factor below 1);
+      * ``"yarn_pairs"``: ``"yarn"`` with a ramp in proportion to the pair's index: the last pair that turns at least ``high`` times and those before it keep their
+        frequency, the first that turns at most ``low`` times and those behind it get ``f_i / factor``. Published models of the name were trained and are run
+        with this one. The two ramps meet at their ends only: with 128 columns, ``length`` 4096 and ``factor`` 16 a pair between them differs by up to 3 times."""
     if isinstance(dim, bool) or int(dim) != dim or dim < 2 or dim % 2:
         raise ValueError(f"rotary_frequencies: dim {dim}: an even number of columns")
     if method not in METHODS:
@@ -48,14 +51,32 @@ def rotary_frequencies(
     f = torch.tensor([base ** (-2.0 * i / dim) for i in range(dim // 2)], dtype=torch.float64)
     if method == "linear":
         f = f / factor
-    if method in ("ramp", "yarn"):
+    if method in ("ramp", "yarn", "yarn_pairs"):
         if length is None or length < 1:
             raise ValueError(f"rotary_frequencies: method {method!r} needs the trained length")
         if not 0 <= low < high:
             raise ValueError(f"rotary_frequencies: low {low}, high {high}: 0 <= low < high")
-        keep = ((length * f / (2 * math.pi) - low) / (high - low)).clamp(0.0, 1.0)
+        if method == "yarn_pairs":
+            first, last = _turning_pairs(dim, base, length, low, high)
+            keep = 1.0 - ((torch.arange(dim // 2, dtype=torch.float64) - first) / (last - first)).clamp(0.0, 1.0)
+        else:
+            keep = ((length * f / (2 * math.pi) - low) / (high - low)).clamp(0.0, 1.0)
         f = keep * f + (1.0 - keep) * f / factor
-    return f, (0.1 * math.log(max(factor, 1.0)) + 1.0 if method == "yarn" else 1.0)
+    return f, (0.1 * math.log(max(factor, 1.0)) + 1.0 if method.startswith("yarn") else 1.0)
+
+
+def _turning_pairs(dim: int, base: float, length: float, low: float, high: float) -> tuple[float, float]:
+    """The index of the last pair that turns at least ``high`` times over ``length`` positions, and of the first that turns at most ``low`` times, whole
+    numbers inside ``0 .. dim - 1`` (the bounds that published models were trained with: of columns, not of pairs); apart by something."""
+    if base <= 1:
+        raise ValueError(f"rotary_frequencies: base {base}: method 'yarn_pairs' needs one above 1")
+
+    def pair(turns: float) -> float:  # length * base ** (-2 pair / dim) = 2 pi turns
+        return math.inf if turns == 0 else dim * math.log(length / (2 * math.pi * turns)) / (2 * math.log(base))
+
+    first = max(math.floor(pair(high)), 0)
+    last = min(math.ceil(min(pair(low), dim)), dim - 1)
+    return first, last if last > first else first + 0.001
 
 
 class Rotary:
