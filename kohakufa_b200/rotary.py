@@ -171,6 +171,8 @@ def apply_rotary(
     args = (rotary.turns, positions, offset, rotary.amplitude, rotary.interleaved, False)
     if _lib.plain_eager(q, k, *args[:3]):
         return _lib.host().rotary(q, k, *args)
+    if any(t is not None and t.shape[-1] > 1 and t.stride(-1) != 1 for t in (q, k)):  # (the op itself takes any gradient)
+        raise ValueError("apply_rotary: q and k need a contiguous last dim")
     if k is None:
         return rotary_op(q, *args)
     if q.dtype != k.dtype:
