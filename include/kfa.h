@@ -326,7 +326,7 @@ int kfa_cache_attend(const KfaTensor4* q, const KfaCache* cache, const KfaTensor
 /* The same for sequences that go on from prefixes which are stored once: `prefix` holds starts[n] .. starts[n + 1] - 1's (sequences, int32
  * [prefix->batch + 1], ascending, inside the batch; NULL: one prefix, of all sequences) first positions, `cache` what each has behind them; sequences outside starts
  * have no prefix. A row sees its whole prefix and what kfa_cache_attend shows it. starts that do not ascend are reported like a bad table.
- * scratch: kfa_cache_attend_shared_bytes bytes (1 KB a row of q, and what cut rows take: up to 78 MB). */
+ * scratch: kfa_cache_attend_shared_bytes bytes (1 KB a row of q, 16 bytes a sequence, K / V head and tile of its rows, and what cut rows take: up to 40 MB). */
 int64_t kfa_cache_attend_shared_bytes(const KfaTensor4* q, const KfaCache* prefix, const KfaCache* cache, const KfaTensor4* k);
 int kfa_cache_attend_shared(const KfaTensor4* q, const KfaCache* prefix, const int32_t* starts, const KfaCache* cache, const KfaTensor4* k,
                             const KfaTensor4* v, const uint8_t* tree, const int64_t* tree_stride, const int32_t* counts,
@@ -342,8 +342,8 @@ int kfa_cache_append(const KfaCache* cache, const KfaTensor4* k, const KfaTensor
  *
  * A row at position p has `pairs` pairs of columns turned by p * f_i, i = 0 .. pairs - 1: (y1, y2) = amplitude * (x1 cos - x2 sin,
  * x2 cos + x1 sin); the columns behind 2 * pairs are copied. interleaved = 0: pair i is columns i and pairs + i; else 2 i and 2 i + 1.
- * turns: f_i / (2 pi) modulo 1 as a 64-bit fraction (2^64 is a whole turn), so that the angle of any position is exact to 2^-65 turns
- * times the position. positions: int32 (wide_positions: int64) [B, T] with the two strides in entries (0: broadcast), or NULL: what the call says.
+ * turns: f_i / (2 pi) modulo 1 as a 64-bit fraction (2^64 is a whole turn): the angle of any position is off by the position times the
+ * fraction's error (2^-65 turns where it is the nearest one) and no more. positions: int32 (wide_positions: int64) [B, T] with the two strides in entries (0: broadcast), or NULL: what the call says.
  * offset: int32 [B], added to every position of a sequence, or NULL. Positions may be negative.
  * --------------------------------------------------------------------------------------------- */
 typedef struct KfaRotary {

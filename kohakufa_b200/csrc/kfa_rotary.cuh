@@ -4,8 +4,8 @@
 //   (y1, y2) = a (x1 cos - x2 sin, x2 cos + x1 sin),   angle = position * f_pair      (the gradient: the same with -sin)
 //
 // Bound by memory: every row is read once and written once. What has to be kept out of the way are the angles. They are not read from a
-// table of positions: f is given in turns as a 64-bit fraction, position * f modulo 2^64 is the angle's fraction of a turn without any error but f's
-// own 2^-65, for every position of 32 bits and more, and sine and cosine are taken of a remainder within an eighth of a turn. A CTA takes a stretch of
+// table of positions: f is given in turns as a 64-bit fraction, position * f modulo 2^64 is the angle's fraction of a turn without any error but the position
+// times that of the fraction (2^-65 turns at best; made of a frequency in radians in 64-bit floats 2^-52 of it), for positions of any size, and sine and cosine are taken of a remainder within an eighth of a turn. A CTA takes a stretch of
 // rows, token by token and head by head, so that one token's sines and cosines, in shared memory, serve all its heads (40 of 32 query and 8 key
 // heads), and asks for its rows before it makes them: what a sine costs (some 40 instructions) passes while the rows are on their way.
 //

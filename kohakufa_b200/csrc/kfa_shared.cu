@@ -37,9 +37,11 @@ SharedPlan plan_shared(int64_t batch, int64_t heads, int64_t kv_heads, int64_t T
   a.ts = static_cast<int>(ts);
   a.n_own = matrix_rows(per);
   a.n_pre = std::max(matrix_rows(per * ts), a.n_own);
-  // What an item's beginning and end count, in units of 32 keys, and in the call below what a unit of the prefixes counts beside one of a sequence's own.
-  // Graph time in us of 7 prefixes of 96 sequences, drafts of 8 tokens, 64 sequences and 256: own items count 6 units more 32.6, 72.1, 50.2, 282; 10 30.2,
-  // 71.0, 50.3, 284; 14 32.8, 70.8, 51.7, 283. With 10, a unit counts 1.0 33.8, 71.0, 50.7, 284; 1.2 30.2, 71.0, 50.3, 284; 1.7 32.6, 70.6, 51.6, 283.
+  // What an item's beginning and end count, in units of 32 keys, and in the call below what a unit of the prefixes counts beside one of a sequence's own. No
+  // close fit: the 7000 clk between two own items are what 9 units take, and times hardly follow. Graph time in us of 7 prefixes of 96 sequences, drafts of 8 tokens,
+  // 64 sequences and 256: own items count 6 units more 32.6, 72.1, 50.2, 282; 10 30.2, 71.0, 50.3, 284; 14 32.8, 70.8, 51.7, 283. With 10, a unit counts 1.0 33.8,
+  // 71.0, 50.7, 284; 1.2 30.2, 71.0, 50.3, 284; 1.7 32.6, 70.6, 51.6, 283. (The first is the only one that moves by more than 3 %, both ways: with where its
+  // stretches happen to end.)
   a.extra_pre = 8;
   a.extra_own = 10;
   const int64_t pre_items = kv_heads * a.row_tiles * ((batch + ts - 1) / ts + prefixes - 1), own_items = batch * kv_heads * a.row_tiles;

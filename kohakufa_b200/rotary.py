@@ -7,7 +7,8 @@
     q, k = apply_rotary(q, k, rotary, positions=positions)       # packed [T, H, D] for attention_varlen, drafted trees, ...
 
 On the way into a cache: ``cache_append_rotary``. There is no table of cosines: angles come from the position itself in fixed point,
-off by no more than the position times the frequency's own rounding in 64 bits whatever the position, so that nothing has to be made for a longest length. The reference has no counterpart.
+off by no more than the position times 2^-52 of the frequency (its division by 2 pi in 64-bit floats) and 2^-65 turns whatever the position, so that nothing has to be
+made for a longest length. The reference has no counterpart.
 """
 
 import math
@@ -94,7 +95,7 @@ class Rotary:
             raise ValueError("Rotary: frequencies is a vector of finite numbers, one per pair of columns")
         if not math.isfinite(amplitude) or not math.isfinite(float(torch.tensor(float(amplitude), dtype=torch.float32))):
             raise ValueError(f"Rotary: amplitude {amplitude}")
-        # turns as 64-bit fractions: position * fraction modulo 2^64 is the angle
+        # turns as 64-bit fractions: position * fraction modulo 2^64 is the angle (2 pi is off by 2^-54.5 of itself and the quotient rounded by 2^-53)
         whole = [round(math.fmod(x / (2 * math.pi), 1.0) * 2**64) % 2**64 for x in f.tolist()]
         self.turns = torch.tensor([w - 2**64 if w >= 2**63 else w for w in whole], dtype=torch.int64, device=device)
         self.interleaved, self.amplitude = bool(interleaved), float(amplitude)

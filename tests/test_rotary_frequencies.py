@@ -62,3 +62,32 @@ def test_yarn_by_pairs_at_its_bounds(dim, length, low):
 def test_yarn_by_pairs_refuses(more):
     with pytest.raises(ValueError):
         rotary_frequencies(16, method="yarn_pairs", factor=2.0, **{"length": 4096, **more})
+
+
+def inverse_of_two_pi(bits):
+    """floor(2^bits / (2 pi)) in whole numbers, by Machin's formula: pi / 4 = 4 arctan(1 / 5) - arctan(1 / 239)."""
+    room = 1 << (bits + 64)
+
+    def arctan(n):
+        power, total, k = room // n, 0, 0
+        while power:
+            total += (power // (2 * k + 1)) * (-1) ** k
+            power //= n * n
+            k += 1
+        return total
+
+    return (room << bits) // (8 * (4 * arctan(5) - arctan(239)))
+
+
+@pytest.mark.parametrize("dim,base,more", [(128, 1e4, {}), (64, 5e5, {"method": "yarn", "factor": 16.0, "length": 4096}), (1024, 1e6, {"method": "linear", "factor": 3.0})])
+def test_turns_within_their_bound(dim, base, more):
+    """2^-52 of the frequency and half a unit: 2 pi in 64 bits is off by 2^-54.5 of itself, the quotient by 2^-53."""
+    f, _ = rotary_frequencies(dim, base, **more)
+    turns = Rotary(f, device="cpu").turns.tolist()
+    assert inverse_of_two_pi(64) == 2935890503282001226  # 0.15915494309189533577 * 2^64
+    one = inverse_of_two_pi(256)
+    for x, got in zip(f.tolist(), turns):
+        num, den = x.as_integer_ratio()
+        off = got * 2**192 - num * one // den  # in units of 2^-256 turns
+        off = (off + 2**255) % 2**256 - 2**255
+        assert abs(off) <= num * one // den // 2**52 + 2**191, (x, off / 2**192)
