@@ -157,7 +157,6 @@ int kfa_cache_attend_shared(const KfaTensor4* q, const KfaCache* prefix, const i
   pre.T = own.T;
   pre.group = own.group;
   pre.c_log2 = own.c_log2;
-  pre.slack = own.slack;
   pre.status = dev_status;
   pre.starts = own.starts = starts;
   pre.groups = own.groups = pre.c.batch;
